@@ -48,7 +48,7 @@
 extern "C" {
 #endif
 
-#define MSS_ABI_VERSION 18
+#define MSS_ABI_VERSION 19
 /* dstate limits (MSS_ERR_UNSUPPORTED beyond, MSS_ERR_INVALID_ARGUMENT beyond 256):
  * MSS_MAX_DSTATE_WIDE for the float32 real-A scans — mss_fwd / mss_bwd / mss_bwd_noalloc with
  * io and bc dtype MSS_F32, and the reference-signature mss_scan_* entry points (whose C
@@ -602,6 +602,103 @@ int mss_scan_bwd_ws(void* stream, int32_t batch, int32_t length, int32_t dim, in
                     const float* u, const float* initial_x, const float* chunk_states,
                     const float* dout, const float* dfinal_x, float* dA, float* ddeltas, float* dB,
                     float* dC, float* du, float* dinitial_x, void* workspace, size_t workspace_bytes);
+
+/* --- 8-bit serving operators (no counterpart symbols in the reference, whose layers are float32
+ * XLA ops: mamba/mamba1.py:52-67, 107-124, 272-276, 300-337). ------------------------------
+ * The 8-bit form of a matrix is e4m3 bytes (1 sign, 4 exponent, 3 fraction bits, no infinity,
+ * largest finite 448) in rows along the features, 16-byte aligned with a row stride ld (bytes)
+ * that is a multiple of 16 and at least the row's length, and float32 scales: one for each
+ * MSS_FP8_BLOCK features and token ([ceil(features / 128)][tokens]) for activations, one for
+ * each MSS_FP8_BLOCK x MSS_FP8_BLOCK block ([ceil(M / 128)][ceil(K / 128)]) for weights. A
+ * value stands for byte * scale; a scale is max(largest magnitude of its block / 448, 2^-126),
+ * the bytes are rounded to nearest even. A NaN or infinity makes its block's scale NaN or
+ * infinite. Bytes between a row's length and its stride are neither written nor relied on.
+ *
+ * mss_quant_fp8: x (features, tokens) float32 or bf16 with element strides stride_f, stride_t
+ * (not negative) -> q [tokens][ldq], scales.
+ * mss_norm_fp8: mss_norm_fwd with the normalised output in this form: hn = h + delta (hn may be
+ * NULL without delta, and is not written then; hn may be h), y = hn rstd weight; h, delta, hn
+ * [features][tokens], delta of delta_dtype.
+ * mss_quant_fp8_weight: w (M, K) float32 or bf16, rows of stride ldw elements -> q, scales.
+ * mss_fp8_mm: C = W X^T with W (M, K) in weight form and X (T, K) in activation form, C float32
+ * or bf16 (out_dtype): [M][ldc], or [T][ldc] with token_major != 0 (ldc in elements). Each
+ * block of 128 features is summed and scaled in float32. T at most MSS_FP8_MM_MAX_TOKENS
+ * (MSS_ERR_UNSUPPORTED beyond). Outputs overlap no operand. */
+#define MSS_FP8_BLOCK 128
+#define MSS_FP8_MM_MAX_TOKENS 524288
+typedef struct mss_quant_fp8_args {
+  int32_t features, tokens, io_dtype;
+  int64_t stride_f, stride_t, ldq;
+  const void* x;
+  void* q;
+  float* scales;
+} mss_quant_fp8_args;
+
+int mss_quant_fp8(const mss_quant_fp8_args* args, void* stream);
+
+typedef struct mss_norm_fp8_args {
+  int32_t features, tokens, delta_dtype;
+  float eps;
+  int64_t ldq;
+  const float* h;
+  const void* delta; /* or NULL */
+  const float* weight;
+  float* hn;
+  void* q;
+  float* scales;
+} mss_norm_fp8_args;
+
+int mss_norm_fp8(const mss_norm_fp8_args* args, void* stream);
+
+typedef struct mss_quant_fp8_weight_args {
+  int32_t M, K, io_dtype;
+  int64_t ldw, ldq;
+  const void* w;
+  void* q;
+  float* scales;
+} mss_quant_fp8_weight_args;
+
+int mss_quant_fp8_weight(const mss_quant_fp8_weight_args* args, void* stream);
+
+typedef struct mss_fp8_mm_args {
+  int32_t M, K, T, out_dtype, token_major;
+  int64_t ldw, ldx, ldc;
+  const void* W;
+  const float* w_scales;
+  const void* X;
+  const float* x_scales;
+  void* C;
+} mss_fp8_mm_args;
+
+int mss_fp8_mm(const mss_fp8_mm_args* args, void* stream);
+
+/* --- Token draw (no counterpart symbol in the reference, which stops at logits:
+ * experiments/mamba_inductionheads.py:143-160 takes their argmax). --------------------------
+ * mss_sample: one token (int64) for each row of logits (rows, vocab), float32 or bf16 with
+ * element strides stride_row, stride_word (not negative), from a uniform float32 in [0, 1) each.
+ * A word whose logit is -inf is absent. In the order "larger logit first, then lower index",
+ * with w = exp((logit - largest) / temperature): top_k > 0 keeps the first top_k words; top_p < 1
+ * keeps of those the ones before which less than top_p of their weight lies; min_p > 0 keeps of
+ * those the ones with w >= min_p; the first word always stays. The token is the lowest index at
+ * which the running weight of the words kept, in index order, exceeds uniform times their
+ * weight. A temperature that is not above 0 gives the first word; a row without a word or with a
+ * NaN gives -1. Settings are one value for all rows, or one a row where the pointer is set.
+ * vocab at most MSS_SAMPLE_MAX_VOCAB (MSS_ERR_UNSUPPORTED beyond). */
+#define MSS_SAMPLE_MAX_VOCAB 1048576
+typedef struct mss_sample_args {
+  int32_t rows, vocab, io_dtype, top_k;
+  float temperature, top_p, min_p;
+  int64_t stride_row, stride_word;
+  const void* logits;
+  const float* uniform;
+  const float* temperatures; /* [rows] or NULL, and so the next three */
+  const int32_t* top_ks;
+  const float* top_ps;
+  const float* min_ps;
+  int64_t* tokens;
+} mss_sample_args;
+
+int mss_sample(const mss_sample_args* args, void* stream);
 
 /* Human-readable text for a status code. */
 const char* mss_strerror(int status);

@@ -19,6 +19,7 @@
 
 #include "../../include/mamba_selective_scan.h"
 #include "mss_common.h"
+#include "mss_serve.h"
 
 namespace mss {
 hipError_t launch_fwd(const FwdParams& p, int zoh, int io_bf16, int bc_bf16, hipStream_t stream);
@@ -55,6 +56,11 @@ hipError_t launch_transpose(const TransposeParams& p, hipStream_t stream);
 hipError_t launch_adamw(const AdamWParams& p, hipStream_t stream);
 hipError_t launch_embed_cm(const EmbedParams& p, hipStream_t stream);
 hipError_t launch_embed_cm_backward(const EmbedParams& p, hipStream_t stream);
+hipError_t launch_quant_fp8(const QuantParams& p, bool io_bf16, hipStream_t stream);
+hipError_t launch_quant_fp8_weight(const QuantWeightParams& p, bool io_bf16, hipStream_t stream);
+hipError_t launch_norm_fp8(const QuantParams& p, bool delta_bf16, hipStream_t stream);
+hipError_t launch_fp8mm(const Fp8MmParams& p, hipStream_t stream);
+hipError_t launch_sample(const SampleParams& p, bool io_bf16, hipStream_t stream);
 }  // namespace mss
 
 namespace {
@@ -840,6 +846,173 @@ bool spans_overlap(const void* a, long long rows_a, long long ld_a, long long co
 }
 
 }  // namespace
+
+// ------------------------------------------------------------------ 8-bit serving, token draw
+namespace {
+bool valid_dtype(int dt) { return dt == MSS_F32 || dt == MSS_BF16; }
+
+// Whether the byte ranges [a, a + na) and [b, b + nb) meet.
+bool bytes_overlap(const void* a, long long na, const void* b, long long nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return b != nullptr && x < y + static_cast<uintptr_t>(nb) && y < x + static_cast<uintptr_t>(na);
+}
+
+// Rows of 8-bit values: 16-byte aligned, the stride a multiple of 16 that holds a row.
+bool valid_rows8(const void* q, long long ld, long long cols) {
+  return q != nullptr && aligned16(q) && ld % 16 == 0 && ld >= cols;
+}
+
+// Bytes of `rows` rows with stride ld, the last one `cols` long.
+long long span8(long long rows, long long ld, long long cols) { return (rows - 1) * ld + cols; }
+
+constexpr long long kMaxSpan = 1LL << 46;  // no product of sizes and strides below passes 63 bits
+bool too_far(long long n, long long ld) { return ld >= kMaxSpan || (ld > 0 && n > kMaxSpan / ld); }
+
+long long blocks8(long long n) { return (n + MSS_FP8_BLOCK - 1) / MSS_FP8_BLOCK; }
+
+static_assert(MSS_FP8_BLOCK == mss::kFp8Block, "header and kernels disagree");
+}  // namespace
+
+int mss_quant_fp8(const mss_quant_fp8_args* a, void* stream) {
+  if (a == nullptr || a->features <= 0 || a->tokens <= 0 || !a->x || !a->scales || !valid_dtype(a->io_dtype) ||
+      a->stride_f < 0 || a->stride_t < 0 || !valid_rows8(a->q, a->ldq, a->features))
+    return MSS_ERR_INVALID_ARGUMENT;
+  if (too_far(a->features, a->stride_f) || too_far(a->tokens, a->stride_t) || too_far(a->tokens, a->ldq) ||
+      blocks8(a->features) > 65535)
+    return MSS_ERR_UNSUPPORTED;
+  const long long nq = span8(a->tokens, a->ldq, a->features), ns = 4 * blocks8(a->features) * a->tokens;
+  const long long nx = ((a->features - 1) * a->stride_f + (a->tokens - 1) * a->stride_t + 1) *
+                       static_cast<long long>(dtype_size(a->io_dtype));
+  if (bytes_overlap(a->q, nq, a->x, nx) || bytes_overlap(a->scales, ns, a->x, nx) || bytes_overlap(a->q, nq, a->scales, ns))
+    return MSS_ERR_INVALID_ARGUMENT;
+  mss::QuantParams p{};
+  p.features = a->features;
+  p.tokens = a->tokens;
+  p.sf = a->stride_f;
+  p.st = a->stride_t;
+  p.ldq = a->ldq;
+  p.x = a->x;
+  p.q = static_cast<unsigned char*>(a->q);
+  p.scales = a->scales;
+  const hipError_t e = mss::launch_quant_fp8(p, a->io_dtype == MSS_BF16, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? MSS_OK : hip_fail(e, "launching fp8 quantisation");
+}
+
+int mss_norm_fp8(const mss_norm_fp8_args* a, void* stream) {
+  if (a == nullptr || a->features <= 0 || a->tokens <= 0 || !(a->eps >= 0.f) || !a->h || !a->weight || !a->scales ||
+      !valid_dtype(a->delta_dtype) || (a->delta && !a->hn) || !valid_rows8(a->q, a->ldq, a->features))
+    return MSS_ERR_INVALID_ARGUMENT;
+  if (too_far(a->tokens, a->ldq) || blocks8(a->features) > 65535) return MSS_ERR_UNSUPPORTED;
+  const long long n = static_cast<long long>(a->features) * a->tokens;
+  const long long nq = span8(a->tokens, a->ldq, a->features), ns = 4 * blocks8(a->features) * a->tokens;
+  const long long nd = n * static_cast<long long>(dtype_size(a->delta_dtype));
+  if (bytes_overlap(a->q, nq, a->h, 4 * n) || bytes_overlap(a->q, nq, a->delta, nd) ||
+      bytes_overlap(a->q, nq, a->weight, 4LL * a->features) || bytes_overlap(a->q, nq, a->scales, ns) ||
+      bytes_overlap(a->scales, ns, a->h, 4 * n) || bytes_overlap(a->scales, ns, a->delta, nd) ||
+      bytes_overlap(a->scales, ns, a->weight, 4LL * a->features))
+    return MSS_ERR_INVALID_ARGUMENT;
+  if (a->delta && (bytes_overlap(a->hn, 4 * n, a->q, nq) || bytes_overlap(a->hn, 4 * n, a->scales, ns) ||
+                   bytes_overlap(a->hn, 4 * n, a->delta, nd) || bytes_overlap(a->hn, 4 * n, a->weight, 4LL * a->features) ||
+                   (a->hn != a->h && bytes_overlap(a->hn, 4 * n, a->h, 4 * n))))
+    return MSS_ERR_INVALID_ARGUMENT;
+  mss::QuantParams p{};
+  p.features = a->features;
+  p.tokens = a->tokens;
+  p.sf = a->tokens;
+  p.st = 1;
+  p.ldq = a->ldq;
+  p.x = a->h;
+  p.q = static_cast<unsigned char*>(a->q);
+  p.scales = a->scales;
+  p.eps = a->eps;
+  p.delta = a->delta;
+  p.w = a->weight;
+  p.hn = a->hn;
+  const hipError_t e = mss::launch_norm_fp8(p, a->delta_dtype == MSS_BF16, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? MSS_OK : hip_fail(e, "launching rmsnorm with fp8 output");
+}
+
+int mss_quant_fp8_weight(const mss_quant_fp8_weight_args* a, void* stream) {
+  if (a == nullptr || a->M <= 0 || a->K <= 0 || !a->w || !a->scales || !valid_dtype(a->io_dtype) || a->ldw < a->K ||
+      !valid_rows8(a->q, a->ldq, a->K))
+    return MSS_ERR_INVALID_ARGUMENT;
+  if (too_far(a->M, a->ldw) || too_far(a->M, a->ldq) || blocks8(a->M) > 65535) return MSS_ERR_UNSUPPORTED;
+  const long long nq = span8(a->M, a->ldq, a->K), ns = 4 * blocks8(a->M) * blocks8(a->K);
+  const long long nw = span8(a->M, a->ldw, a->K) * static_cast<long long>(dtype_size(a->io_dtype));
+  if (bytes_overlap(a->q, nq, a->w, nw) || bytes_overlap(a->scales, ns, a->w, nw) || bytes_overlap(a->q, nq, a->scales, ns))
+    return MSS_ERR_INVALID_ARGUMENT;
+  mss::QuantWeightParams p{};
+  p.M = a->M;
+  p.K = a->K;
+  p.ldw = a->ldw;
+  p.ldq = a->ldq;
+  p.w = a->w;
+  p.q = static_cast<unsigned char*>(a->q);
+  p.scales = a->scales;
+  const hipError_t e = mss::launch_quant_fp8_weight(p, a->io_dtype == MSS_BF16, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? MSS_OK : hip_fail(e, "launching fp8 weight quantisation");
+}
+
+int mss_fp8_mm(const mss_fp8_mm_args* a, void* stream) {
+  if (a == nullptr || a->M <= 0 || a->K <= 0 || a->T <= 0 || !a->w_scales || !a->x_scales || !a->C ||
+      !valid_dtype(a->out_dtype) || !valid_rows8(a->W, a->ldw, a->K) || !valid_rows8(a->X, a->ldx, a->K))
+    return MSS_ERR_INVALID_ARGUMENT;
+  const long long rows = a->token_major ? a->T : a->M, cols = a->token_major ? a->M : a->T;
+  if (a->ldc < cols) return MSS_ERR_INVALID_ARGUMENT;
+  if (a->T > MSS_FP8_MM_MAX_TOKENS || too_far(a->M, a->ldw) || too_far(a->T, a->ldx) || too_far(rows, a->ldc))
+    return MSS_ERR_UNSUPPORTED;
+  const long long nc = span8(rows, a->ldc, cols) * static_cast<long long>(dtype_size(a->out_dtype));
+  if (bytes_overlap(a->C, nc, a->W, span8(a->M, a->ldw, a->K)) || bytes_overlap(a->C, nc, a->X, span8(a->T, a->ldx, a->K)) ||
+      bytes_overlap(a->C, nc, a->w_scales, 4 * blocks8(a->M) * blocks8(a->K)) ||
+      bytes_overlap(a->C, nc, a->x_scales, 4 * blocks8(a->K) * a->T))
+    return MSS_ERR_INVALID_ARGUMENT;
+  mss::Fp8MmParams p{};
+  p.M = a->M;
+  p.K = a->K;
+  p.T = a->T;
+  p.token_major = a->token_major != 0;
+  p.out_bf16 = a->out_dtype == MSS_BF16;
+  p.ldw = a->ldw;
+  p.ldx = a->ldx;
+  p.ldc = a->ldc;
+  p.w = static_cast<const unsigned char*>(a->W);
+  p.ws = a->w_scales;
+  p.x = static_cast<const unsigned char*>(a->X);
+  p.xs = a->x_scales;
+  p.c = a->C;
+  const hipError_t e = mss::launch_fp8mm(p, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? MSS_OK : hip_fail(e, "launching fp8 matrix product");
+}
+
+int mss_sample(const mss_sample_args* a, void* stream) {
+  if (a == nullptr || a->rows <= 0 || a->vocab <= 0 || !valid_dtype(a->io_dtype) || a->stride_row < 0 ||
+      a->stride_word < 0 || !a->logits || !a->uniform || !a->tokens)
+    return MSS_ERR_INVALID_ARGUMENT;
+  if (a->vocab > MSS_SAMPLE_MAX_VOCAB || too_far(a->rows, a->stride_row) || too_far(a->vocab, a->stride_word))
+    return MSS_ERR_UNSUPPORTED;
+  const long long nx = ((a->rows - 1) * a->stride_row + (a->vocab - 1) * a->stride_word + 1) *
+                       static_cast<long long>(dtype_size(a->io_dtype));
+  if (bytes_overlap(a->tokens, 8LL * a->rows, a->logits, nx) || bytes_overlap(a->tokens, 8LL * a->rows, a->uniform, 4LL * a->rows))
+    return MSS_ERR_INVALID_ARGUMENT;
+  mss::SampleParams p{};
+  p.rows = a->rows;
+  p.vocab = a->vocab;
+  p.sr = a->stride_row;
+  p.sv = a->stride_word;
+  p.logits = a->logits;
+  p.uniform = a->uniform;
+  p.temperature = a->temperature;
+  p.top_k = a->top_k;
+  p.top_p = a->top_p;
+  p.min_p = a->min_p;
+  p.temperatures = a->temperatures;
+  p.top_ks = a->top_ks;
+  p.top_ps = a->top_ps;
+  p.min_ps = a->min_ps;
+  p.tokens = reinterpret_cast<long long*>(a->tokens);
+  const hipError_t e = mss::launch_sample(p, a->io_dtype == MSS_BF16, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? MSS_OK : hip_fail(e, "launching token draw");
+}
 
 int mss_proj(const mss_proj_args* a, void* stream) {
   if (a == nullptr || a->M <= 0 || a->K <= 0 || a->T <= 0 || !a->W || !a->X || !a->C)

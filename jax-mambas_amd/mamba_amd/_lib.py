@@ -13,7 +13,7 @@ from pathlib import Path
 
 LIBRARY_NAME = "libmamba_selective_scan_hip.so"
 
-MSS_ABI_VERSION = 18
+MSS_ABI_VERSION = 19
 MSS_OK = 0
 MSS_ERR_INVALID_ARGUMENT = 1
 MSS_ERR_UNSUPPORTED = 2
@@ -31,6 +31,9 @@ MSS_SEG_STEPS = 8
 MSS_REF_CHUNK = 2048
 MSS_NORM_GEMV_MAX_FEATURES = 1024
 MSS_XENT_FUSED_MAX_VOCAB = 65536
+MSS_FP8_BLOCK = 128
+MSS_FP8_MM_MAX_TOKENS = 1 << 19
+MSS_SAMPLE_MAX_VOCAB = 1 << 20
 
 # Every symbol include/mamba_selective_scan.h declares.
 EXPORTED_SYMBOLS = (
@@ -79,6 +82,11 @@ EXPORTED_SYMBOLS = (
     "mss_adamw",
     "mss_embed_cm",
     "mss_embed_cm_backward",
+    "mss_quant_fp8",
+    "mss_norm_fp8",
+    "mss_quant_fp8_weight",
+    "mss_fp8_mm",
+    "mss_sample",
     "mss_strerror",
     "mss_last_hip_error",
     "mss_abi_version",
@@ -200,6 +208,35 @@ class ConvStepArgs(ctypes.Structure):
     ]
 
 
+class QuantFp8Args(ctypes.Structure):
+    _fields_ = [("features", _i32), ("tokens", _i32), ("io_dtype", _i32), ("stride_f", ctypes.c_int64),
+                ("stride_t", ctypes.c_int64), ("ldq", ctypes.c_int64), ("x", _p), ("q", _p), ("scales", _p)]
+
+
+class NormFp8Args(ctypes.Structure):
+    _fields_ = [("features", _i32), ("tokens", _i32), ("delta_dtype", _i32), ("eps", ctypes.c_float),
+                ("ldq", ctypes.c_int64), ("h", _p), ("delta", _p), ("weight", _p), ("hn", _p), ("q", _p),
+                ("scales", _p)]
+
+
+class QuantFp8WeightArgs(ctypes.Structure):
+    _fields_ = [("M", _i32), ("K", _i32), ("io_dtype", _i32), ("ldw", ctypes.c_int64), ("ldq", ctypes.c_int64),
+                ("w", _p), ("q", _p), ("scales", _p)]
+
+
+class Fp8MmArgs(ctypes.Structure):
+    _fields_ = [("M", _i32), ("K", _i32), ("T", _i32), ("out_dtype", _i32), ("token_major", _i32),
+                ("ldw", ctypes.c_int64), ("ldx", ctypes.c_int64), ("ldc", ctypes.c_int64), ("W", _p),
+                ("w_scales", _p), ("X", _p), ("x_scales", _p), ("C", _p)]
+
+
+class SampleArgs(ctypes.Structure):
+    _fields_ = [("rows", _i32), ("vocab", _i32), ("io_dtype", _i32), ("top_k", _i32), ("temperature", ctypes.c_float),
+                ("top_p", ctypes.c_float), ("min_p", ctypes.c_float), ("stride_row", ctypes.c_int64),
+                ("stride_word", ctypes.c_int64), ("logits", _p), ("uniform", _p), ("temperatures", _p), ("top_ks", _p),
+                ("top_ps", _p), ("min_ps", _p), ("tokens", _p)]
+
+
 _LIBRARY = None
 _LIBRARY_PATH = None
 
@@ -307,6 +344,11 @@ def register_hip_kernel(library_path=None):
     lib.mss_embed_cm_backward.argtypes = [_p, ctypes.c_int64, _p, _p, ctypes.c_int64, _i32, _i32, _p, _p, ctypes.c_int64,
                                           _p]
     lib.mss_embed_cm_backward.restype = ctypes.c_int
+    for name, args in (("mss_quant_fp8", QuantFp8Args), ("mss_norm_fp8", NormFp8Args),
+                       ("mss_quant_fp8_weight", QuantFp8WeightArgs), ("mss_fp8_mm", Fp8MmArgs),
+                       ("mss_sample", SampleArgs)):
+        getattr(lib, name).argtypes = [ctypes.POINTER(args), _p]
+        getattr(lib, name).restype = ctypes.c_int
     lib.mss_strerror.argtypes = [ctypes.c_int]
     lib.mss_strerror.restype = ctypes.c_char_p
     lib.mss_last_hip_error.argtypes = []

@@ -1,0 +1,392 @@
+"""8-bit serving operators: block-scaled e4m3 activations and weights, the residual add + RMSNorm
+that writes them (mamba/mamba1.py:300-337), and the product of the two.
+
+CPU: refusals. GPU: against the definitions in float64 on the same inputs.
+
+Tolerances, all per element. An e4m3 rounding moves a value y by at most half a step,
+2^(max(floor(log2 |y|), -6) - 4). float32 roundings count 2^-24 each: two between a value and its
+quotient by the scale; the norm's sum of F squares at most F of them (halved by the root) and six
+more up to the output. For a float32 product the sum of 128 products and the sum over blocks
+count one whole step, 2^-23, for each addition, relative to the sum of the magnitudes. For a bf16
+product the 8-bit matrix instructions may add the products 8 at a time, of which each loses less
+than 2^-13 of the largest: 7 of them, so 2^-10 of the sum of the magnitudes covers the rest too.
+"""
+import numpy as np
+import pytest
+import torch
+
+from mamba_amd import _lib
+from mamba_amd.fp8 import add_rmsnorm_fp8, fp8_matmul, quantize_fp8, quantize_fp8_weight
+
+BLOCK = 128
+FP8 = torch.float8_e4m3fn
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return _lib.register_hip_kernel()
+
+
+# ------------------------------------------------------------------------------- refusals
+QUANT = dict(features=300, tokens=10, io_dtype=0, stride_f=10, stride_t=1, ldq=304, x=1 << 32, q=1 << 36,
+             scales=1 << 37)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(features=0), 1), (dict(tokens=-1), 1), (dict(io_dtype=2), 1), (dict(x=None), 1), (dict(q=None), 1),
+    (dict(scales=None), 1), (dict(stride_f=-1), 1), (dict(stride_t=-10), 1), (dict(ldq=288), 1), (dict(ldq=305), 1),
+    (dict(q=(1 << 36) + 8), 1), (dict(q=1 << 32), 1), (dict(scales=(1 << 32) + 64), 1), (dict(scales=(1 << 36) + 16), 1),
+    (dict(stride_f=1 << 50), 2), (dict(features=65536 * 128, ldq=65536 * 128), 2),
+])
+def test_quant_validation(lib, kw, status):
+    assert lib.mss_quant_fp8(_lib.QuantFp8Args(**{**QUANT, **kw}), None) == status
+    assert lib.mss_quant_fp8(None, None) == 1
+
+
+NORM = dict(features=300, tokens=10, delta_dtype=1, eps=1e-5, ldq=304, h=1 << 32, delta=1 << 33, weight=1 << 34,
+            hn=1 << 35, q=1 << 36, scales=1 << 37)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(features=0), 1), (dict(tokens=0), 1), (dict(eps=-1.0), 1), (dict(eps=float("nan")), 1), (dict(h=None), 1),
+    (dict(weight=None), 1), (dict(hn=None), 1), (dict(q=None), 1), (dict(scales=None), 1), (dict(delta_dtype=3), 1),
+    (dict(ldq=302), 1), (dict(q=1 << 32), 1), (dict(hn=(1 << 32) + 16), 1), (dict(hn=1 << 33), 1),
+    (dict(scales=(1 << 35) + 64), 1), (dict(q=1 << 34), 1), (dict(features=65536 * 128, ldq=65536 * 128), 2),
+])
+def test_norm_validation(lib, kw, status):
+    assert lib.mss_norm_fp8(_lib.NormFp8Args(**{**NORM, **kw}), None) == status
+    assert lib.mss_norm_fp8(None, None) == 1
+
+
+WEIGHT = dict(M=200, K=300, io_dtype=0, ldw=300, ldq=304, w=1 << 32, q=1 << 36, scales=1 << 37)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(M=0), 1), (dict(K=0), 1), (dict(io_dtype=-1), 1), (dict(ldw=299), 1), (dict(ldq=300), 1), (dict(w=None), 1),
+    (dict(q=(1 << 36) + 4), 1), (dict(q=1 << 32), 1), (dict(scales=None), 1), (dict(ldw=1 << 50), 2),
+    (dict(M=65536 * 128), 2),
+])
+def test_weight_validation(lib, kw, status):
+    assert lib.mss_quant_fp8_weight(_lib.QuantFp8WeightArgs(**{**WEIGHT, **kw}), None) == status
+    assert lib.mss_quant_fp8_weight(None, None) == 1
+
+
+MM = dict(M=200, K=300, T=10, out_dtype=1, token_major=0, ldw=304, ldx=304, ldc=10, W=1 << 32, w_scales=1 << 33,
+          X=1 << 34, x_scales=1 << 35, C=1 << 36)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(M=0), 1), (dict(K=0), 1), (dict(T=0), 1), (dict(out_dtype=7), 1), (dict(ldw=296), 1), (dict(ldx=312), 1),
+    (dict(ldc=9), 1), (dict(token_major=1, ldc=199), 1), (dict(W=None), 1), (dict(X=None), 1), (dict(w_scales=None), 1),
+    (dict(x_scales=None), 1), (dict(C=None), 1), (dict(W=(1 << 32) + 8), 1), (dict(X=(1 << 34) + 1), 1),
+    (dict(C=(1 << 32) + 1024), 1), (dict(C=1 << 34), 1), (dict(C=1 << 35), 1), (dict(C=1 << 33), 1),
+    (dict(T=(1 << 19) + 1, ldc=1 << 20), 2), (dict(ldw=1 << 50), 2), (dict(ldc=1 << 50), 2),
+])
+def test_mm_validation(lib, kw, status):
+    assert lib.mss_fp8_mm(_lib.Fp8MmArgs(**{**MM, **kw}), None) == status
+    assert lib.mss_fp8_mm(None, None) == 1
+
+
+def test_python_errors():
+    x = torch.randn(8, 4)
+    q8 = lambda *s: torch.zeros(*s).to(FP8)  # noqa: E731
+    with pytest.raises(TypeError):
+        quantize_fp8(x.double())
+    with pytest.raises(ValueError):
+        quantize_fp8(x[0])
+    with pytest.raises(RuntimeError):
+        quantize_fp8(x)  # no CPU path
+    with pytest.raises(RuntimeError):
+        quantize_fp8(x.requires_grad_(True))
+    x = torch.randn(8, 4)
+    with pytest.raises(TypeError):
+        add_rmsnorm_fp8(x.bfloat16(), None, torch.ones(8))
+    with pytest.raises(ValueError):
+        add_rmsnorm_fp8(x, None, torch.ones(4))
+    with pytest.raises(ValueError):
+        add_rmsnorm_fp8(x, torch.randn(8, 5), torch.ones(8))
+    with pytest.raises(TypeError):
+        add_rmsnorm_fp8(x, x.half(), torch.ones(8))
+    with pytest.raises(RuntimeError):
+        add_rmsnorm_fp8(x, None, torch.ones(8))
+    with pytest.raises(ValueError):
+        quantize_fp8_weight(torch.randn(8, 4).t())
+    with pytest.raises(RuntimeError):
+        quantize_fp8_weight(x)
+    one, s = torch.ones(1, 1), torch.ones(1, 4)
+    with pytest.raises(TypeError):
+        fp8_matmul(x, one, q8(4, 16), s)
+    with pytest.raises(ValueError):
+        fp8_matmul(q8(8, 16), one, q8(4, 32), s)
+    with pytest.raises(ValueError):
+        fp8_matmul(q8(8, 17), one, q8(4, 17), s)  # rows that do not start on 16 bytes
+    with pytest.raises(ValueError):
+        fp8_matmul(q8(8, 16), torch.ones(1, 2), q8(4, 16), s)
+    with pytest.raises(ValueError):
+        fp8_matmul(q8(8, 16), one, q8(4, 16), torch.ones(4, 1))
+    with pytest.raises(ValueError):
+        fp8_matmul(q8(8, 16), one, q8(4, 16), s, out=torch.zeros(4, 8, dtype=torch.bfloat16))
+    with pytest.raises(TypeError):
+        fp8_matmul(q8(8, 16), one, q8(4, 16), s, out_dtype=torch.float16)
+    with pytest.raises(RuntimeError):
+        fp8_matmul(q8(8, 16), one, q8(4, 16), s)
+
+
+# ------------------------------------------------------------------------------------ GPU
+def half_step(y):
+    """Half an e4m3 step at float64 y."""
+    return 2.0 ** (np.maximum(np.floor(np.log2(np.maximum(np.abs(y), 1e-300))), -6) - 4)
+
+
+def spread_blocks(scales, n):
+    """Scales (blocks, tokens) as one for each of n features: (n, tokens)."""
+    return np.repeat(scales, BLOCK, axis=0)[:n]
+
+
+def check_quantised(y, q, scales, rel):
+    """q (tokens, features), scales (blocks, tokens) against y (features, tokens) in float64,
+    itself known up to `rel`."""
+    f, t = y.shape
+    pad = np.zeros((-(-f // BLOCK) * BLOCK, t))
+    pad[:f] = np.abs(y)
+    want = np.maximum(pad.reshape(-1, BLOCK, t).max(1) / 448.0, 2.0 ** -126)
+    s = scales.double().cpu().numpy()
+    assert s.shape == want.shape
+    assert np.all(np.abs(s - want) <= want * (rel + 2.0 ** -24) * 1.001)
+    got = q.float().double().cpu().numpy().T
+    assert got.shape == y.shape
+    per = spread_blocks(s, f)
+    assert np.all(np.abs(got - y / per) <= half_step(y / per) + np.abs(y / per) * (2 * rel + 2.0 ** -22) + 1e-30)
+
+
+def rand(*shape, seed=0, dtype=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(*shape, generator=g) * torch.exp(2 * torch.randn(shape[0], 1, generator=g))
+    return x.to(dtype).to("cuda")
+
+
+LAYOUTS = ["channel", "token", "rows_apart", "strided"]
+
+
+def laid_out(x, layout):
+    if layout == "token":
+        return x.t().contiguous().t()
+    if layout == "rows_apart":
+        big = torch.full((x.shape[0], x.shape[1] + 5), float("nan"), dtype=x.dtype, device=x.device)
+        big[:, 3:3 + x.shape[1]] = x
+        return big[:, 3:3 + x.shape[1]]
+    if layout == "strided":
+        big = torch.full((2 * x.shape[0], 3 * x.shape[1]), float("nan"), dtype=x.dtype, device=x.device)
+        big[::2, ::3] = x
+        return big[::2, ::3]
+    return x.contiguous()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("f,t", [(1, 1), (5, 3), (128, 64), (129, 65), (1000, 7), (2560, 8), (300, 257), (768, 1031),
+                                 (2560, 1)])
+def test_quantise(f, t, layout, dtype):
+    x = laid_out(rand(f, t, dtype=dtype), layout)
+    q, scales = quantize_fp8(x)
+    assert q.shape == (t, f) and q.dtype == FP8
+    check_quantised(x.double().cpu().numpy(), q, scales, 0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [4, 200])
+def test_quantise_edges(t):
+    """Zeros, subnormals, the largest floats, and values that are not finite, each in a block of
+    its own; what they do stays there."""
+    x = rand(6 * BLOCK, t)
+    x[:BLOCK] = 0
+    x[BLOCK:2 * BLOCK] = 1e-42
+    x[2 * BLOCK:3 * BLOCK] = 3.4e38
+    x[3 * BLOCK + 5, 1] = float("nan")
+    x[4 * BLOCK + 9, 2] = float("-inf")
+    q, scales = quantize_fp8(x)
+    s, v = scales.cpu(), q.float().cpu() * scales.cpu().repeat_interleave(BLOCK, 0).t()
+    assert torch.all(s[0] == 2.0 ** -126) and torch.all(v[:, :BLOCK] == 0)
+    assert torch.all(s[1] == 2.0 ** -126) and torch.all(v[:, BLOCK:2 * BLOCK].abs() <= 2.0 ** -126 * 2.0 ** -9)
+    assert torch.allclose(v[:, 2 * BLOCK:3 * BLOCK], torch.tensor(3.4e38), rtol=2.0 ** -22, atol=0)
+    assert torch.isnan(s[3, 1]) and torch.isnan(v[1, 3 * BLOCK:4 * BLOCK]).all()
+    assert torch.isinf(s[4, 2]) and torch.isnan(v[2, 4 * BLOCK:5 * BLOCK]).all()
+    ok = torch.ones_like(v, dtype=torch.bool)
+    ok[1, 3 * BLOCK:4 * BLOCK] = ok[2, 4 * BLOCK:5 * BLOCK] = False
+    assert torch.isfinite(v[ok]).all()
+    sub = x[5 * BLOCK:].double().cpu().numpy()
+    check_quantised(sub, q[:, 5 * BLOCK:], scales[5:], 0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,k,ld", [(1, 1, 1), (128, 128, 128), (130, 127, 140), (257, 1001, 1001), (1280, 2560, 2560)])
+def test_quantise_weight(m, k, ld, dtype):
+    w = rand(m, ld, dtype=dtype)[:, :k]
+    q, scales = quantize_fp8_weight(w)
+    assert q.shape == (m, k) and scales.shape == (-(-m // BLOCK), -(-k // BLOCK))
+    y = w.double().cpu().numpy()
+    s = scales.double().cpu().numpy()
+    pad = np.zeros((s.shape[0] * BLOCK, s.shape[1] * BLOCK))
+    pad[:m, :k] = np.abs(y)
+    want = pad.reshape(s.shape[0], BLOCK, s.shape[1], BLOCK).max((1, 3)) / 448.0
+    assert np.all(np.abs(s - want) <= want * 2.0 ** -24 * 1.001)
+    per = np.repeat(np.repeat(s, BLOCK, 0), BLOCK, 1)[:m, :k]
+    got = q.float().double().cpu().numpy()
+    assert np.all(np.abs(got - y / per) <= half_step(y / per) + np.abs(y / per) * 2.0 ** -22)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("delta", [None, torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("f,t", [(1, 1), (5, 3), (128, 8), (768, 1), (1000, 70), (1280, 300), (129, 1031), (2048, 513),
+                                 (2049, 40), (5120, 9), (4100, 515), (640, 4111)])
+def test_norm(f, t, delta):
+    h = rand(f, t, seed=1)
+    d = None if delta is None else rand(f, t, seed=2, dtype=delta)
+    w = 1 + 0.3 * torch.randn(f, generator=torch.Generator().manual_seed(3)).to("cuda")
+    before = h.clone()
+    hn, q, scales = add_rmsnorm_fp8(h, d, w, 1e-5)
+    assert torch.equal(h, before)
+    if d is None:
+        assert hn is h
+    else:
+        assert torch.equal(hn, h + d.float())
+    x = h.double().cpu().numpy()
+    if d is not None:
+        x = x + d.double().cpu().numpy()
+    y = x / np.sqrt((x * x).mean(0) + 1e-5) * w.double().cpu().numpy()[:, None]
+    rel = (f / 2 + 6) * 2.0 ** -24
+    if d is not None:  # the sum's own rounding, relative to the sum: 2^-24 more
+        rel += 2.0 ** -24
+    check_quantised(y, q, scales, rel)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [3, 700])
+def test_norm_not_finite(t):
+    h = rand(300, t, seed=4)
+    h[7, 1] = float("nan")
+    h[:, 2] = 0
+    _, q, scales = add_rmsnorm_fp8(h, None, torch.ones(300, device="cuda"))
+    v = q.float() * scales.repeat_interleave(BLOCK, 0)[:300].t()
+    assert torch.isnan(v[1]).all() and torch.all(v[2] == 0)
+    keep = torch.arange(t, device="cuda") != 1
+    assert torch.isfinite(v[keep]).all()
+
+
+def operands(m, k, t, seed=0):
+    w = rand(m, k, seed=seed)
+    x = rand(k, t, seed=seed + 1)
+    return *quantize_fp8_weight(w), *quantize_fp8(x)
+
+
+def check_mm(got, wq, ws, xq, xs, token_major, out_dtype, only=slice(None)):
+    m, k = wq.shape
+    w = wq.float().double().cpu() * ws.double().cpu().repeat_interleave(BLOCK, 0)[:m].repeat_interleave(BLOCK, 1)[:, :k]
+    x = (xq.float().double().cpu().t() * xs.double().cpu().repeat_interleave(BLOCK, 0)[:k])[:, only]
+    want, size = w @ x, w.abs() @ x.abs()
+    got = (got.double().cpu().t() if token_major else got.double().cpu())[:, only]
+    bound = size * (min(k, BLOCK) + 3 * xs.shape[0] + 4) * 2.0 ** -23
+    if out_dtype == torch.bfloat16:
+        bound = size * 2.0 ** -10
+    bound += want.abs() * (torch.finfo(out_dtype).eps / 2) * 1.01
+    assert got.shape == want.shape
+    assert torch.all((got - want).abs() <= bound), float(((got - want).abs() - bound).max())
+
+
+SHAPES = [(1, 1, 1), (16, 128, 16), (17, 129, 3), (130, 256, 1), (100, 1000, 77), (1280, 2560, 8), (257, 1250, 300),
+          (300, 384, 513), (5120, 1280, 1), (1000, 640, 33), (128, 4096, 64), (64, 15, 129), (1280, 2560, 333),
+          (515, 143, 1025), (768, 768, 2048)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("token_major", [False, True])
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,k,t", SHAPES)
+def test_matmul(m, k, t, out_dtype, token_major):
+    a = operands(m, k, t)
+    got = fp8_matmul(*a, out_dtype=out_dtype, token_major=token_major)
+    assert got.dtype == out_dtype and got.is_contiguous()
+    check_mm(got, *a, token_major, out_dtype)
+    assert torch.equal(got, fp8_matmul(*a, out_dtype=out_dtype, token_major=token_major))  # the same every time
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,t", [(100, 1000, 5), (300, 200, 140), (520, 384, 600)])
+def test_matmul_layouts(m, k, t):
+    """Rows apart, an output with rows apart, and what lies between the rows not relied on (NaN
+    bytes) nor written."""
+    wq, ws, xq, xs = operands(m, k, t)
+    wide = lambda q: torch.full((q.shape[0], -(-k // 16) * 16 + 48), 0x7F, dtype=torch.uint8, device="cuda").view(FP8)  # noqa: E731
+    w2, x2 = wide(wq), wide(xq)
+    w2[:, :k], x2[:, :k] = wq, xq
+    for token_major in (False, True):
+        rows, cols = (t, m) if token_major else (m, t)
+        for dtype in (torch.bfloat16, torch.float32):
+            big = torch.full((rows, cols + 3), 7.0, dtype=dtype, device="cuda")
+            out = big[:, 1:1 + cols]
+            got = fp8_matmul(w2[:, :k], ws, x2[:, :k], xs, out_dtype=dtype, token_major=token_major, out=out)
+            assert got is out
+            check_mm(got, wq, ws, xq, xs, token_major, dtype)
+            assert torch.all(big[:, 0] == 7) and torch.all(big[:, 1 + cols:] == 7)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [4, 40, 300])
+def test_matmul_not_finite(t):
+    """A token with a NaN, and one with an infinity, give NaN; the other tokens are untouched."""
+    m, k = 200, 600
+    w, x = rand(m, k), rand(k, t, seed=1)
+    clean = operands(m, k, t)
+    x[130, 1], x[599, 2] = float("nan"), float("inf")
+    q, s = quantize_fp8(x)
+    got = fp8_matmul(clean[0], clean[1], q, s)
+    keep = [i for i in range(t) if i not in (1, 2)]
+    assert torch.isnan(got[:, 1:3]).all()
+    assert torch.equal(got[:, keep], fp8_matmul(*clean)[:, keep])
+
+
+@pytest.mark.gpu
+def test_empty():
+    z = lambda *s: torch.zeros(*s, device="cuda")  # noqa: E731
+    q, s = quantize_fp8(z(300, 0))
+    assert q.shape == (0, 300) and s.shape == (3, 0)
+    hn, q, s = add_rmsnorm_fp8(z(300, 0), None, z(300))
+    assert hn.shape == (300, 0) and q.shape == (0, 300) and s.shape == (3, 0)
+    wq, ws = quantize_fp8_weight(torch.randn(8, 300, device="cuda"))
+    assert fp8_matmul(wq, ws, q, s).shape == (8, 0)
+    wq, ws = quantize_fp8_weight(z(0, 300))
+    q, s = quantize_fp8(z(300, 4))
+    assert fp8_matmul(wq, ws, q, s, token_major=True).shape == (4, 0)
+    wq, ws = quantize_fp8_weight(z(8, 0))
+    q, s = quantize_fp8(z(0, 4))
+    assert torch.equal(fp8_matmul(wq, ws, q, s), z(8, 4).bfloat16())
+
+
+@pytest.mark.gpu
+def test_side_stream_and_graph():
+    """On a stream of its own, and replayed from a graph with new inputs."""
+    h, d = rand(640, 9, seed=5), rand(640, 9, seed=6, dtype=torch.bfloat16)
+    w, nw = rand(256, 640, seed=7), torch.ones(640, device="cuda")
+    wq, ws = quantize_fp8_weight(w)
+
+    def step():
+        hn, q, s = add_rmsnorm_fp8(h, d, nw)
+        return hn, fp8_matmul(wq, ws, q, s)
+
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (8, 9, 10):
+        h.copy_(rand(640, 9, seed=seed))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, step()))
