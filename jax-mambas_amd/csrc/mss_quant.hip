@@ -5,18 +5,130 @@
 //              eps), y = hn r_t w[f]   (reference mamba/mamba1.py:300-337: nnx.RMSNorm before
 //              the in-projections, the block's output added back)
 //   s[b][t]  = max(max_{f in block b} |y[f][t]| / 448, 2^-126)
-//   q[t][f]  = e4m3(y[f][t] * (1 / s[b][t])), rounded to nearest even
+//   q[t][f]  = e4m3(y[f][t] / s[b][t]), rounded to nearest even
 //
 // The stream is channel-major (features, tokens) and a matrix-core product wants 8-bit operands
 // with the features contiguous, so these kernels also transpose: a workgroup owns a tile of
-// tokens, one token a lane, and each thread 4 consecutive features of a block, which it packs
-// into one dword of the token's row in LDS; the rows leave as whole dwords. y and the norm's
-// sums are float32; q is the only rounding to fewer bits.
+// tokens, a thread 4 to 8 neighbouring tokens of 4 features, whose bytes it packs into a dword of
+// each token's row in LDS; the rows leave as 16-byte stores. y and the norm's sums are float32;
+// q is the only rounding to fewer bits.
 #include <hip/hip_runtime.h>
 
 #include "mss_serve.h"
 
 namespace mss {
+
+// y / s for the reciprocal inv of s, rounded as the division is (one Newton step on the
+// quotient; q * s is never near overflow, |y| <= 448 s). bf16 values over a scale of 7 significant
+// bits meet e4m3's borders exactly, so a quotient off by one float32 step rounds the wrong way.
+__device__ __forceinline__ float divide_by(float y, float s, float inv) {
+  const float q = y * inv;
+  return __builtin_fmaf(__builtin_fmaf(-q, s, y), inv, q);
+}
+
+// kN neighbouring values, of any alignment.
+template <int kN, typename io_t>
+__device__ __forceinline__ void load_run(const io_t* __restrict__ p, float (&v)[kN]) {
+  io_t e[kN];
+  __builtin_memcpy(e, p, sizeof(e));
+#pragma unroll
+  for (int i = 0; i < kN; ++i) v[i] = to_f32(e[i]);
+}
+
+// The larger of v and the value kLanes away (kLanes a power of two below 64), for all lanes.
+template <int kLanes>
+__device__ __forceinline__ uint32_t max_across(uint32_t v) {
+  if constexpr (kLanes == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max(static_cast<uint32_t>(r[0]), static_cast<uint32_t>(r[1]));
+  } else if constexpr (kLanes == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return max(static_cast<uint32_t>(r[0]), static_cast<uint32_t>(r[1]));
+  } else if constexpr (kLanes == 8) {  // row_ror:8 within 16 lanes
+    return max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x128, 0xF, 0xF, true)));
+  } else {
+    return max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), kLanes)));
+  }
+}
+// The same over every lane whose index differs above kFrom - 1.
+template <int kFrom>
+__device__ __forceinline__ uint32_t max_above(uint32_t v) {
+  if constexpr (kFrom < 64) return max_above<2 * kFrom>(max_across<kFrom>(v));
+  return v;
+}
+template <int kFrom>
+__device__ __forceinline__ float sum_above(float v) {
+#pragma unroll
+  for (int s = kFrom; s < 64; s *= 2) v += __shfl_xor(v, s);
+  return v;
+}
+
+// 16 bytes of a token's row from LDS (8-byte aligned there) to the features f .. f + 16 of q.
+__device__ __forceinline__ void store_row16(unsigned char* __restrict__ q, const uint32_t* __restrict__ src, int f, int F) {
+  if (f >= F) return;
+  const uint2 a = reinterpret_cast<const uint2*>(src)[0], b = reinterpret_cast<const uint2*>(src)[1];
+  if (f + 16 <= F) {
+    *reinterpret_cast<u32x4*>(q) = u32x4{a.x, a.y, b.x, b.y};
+  } else {
+    const uint32_t w[4] = {a.x, a.y, b.x, b.y};
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (f + i < F) q[i] = static_cast<unsigned char>(w[i / 4] >> (8 * (i & 3)));
+  }
+}
+
+// --------------------------------------------------------------- quantisation, token-contiguous
+// A workgroup: one block of features, 64 tokens. A thread holds 16 bytes (kTV tokens) of 4
+// features; a feature's 64 tokens are one 128- or 256-byte read.
+template <typename io_t>
+__global__ __launch_bounds__(128 * sizeof(io_t)) void quant_tile_kernel(QuantParams p) {
+  constexpr int kTV = 16 / sizeof(io_t), kLanes = 64 / kTV, kWaves = 2 * sizeof(io_t);
+  constexpr int kPitch = kFp8Block / 4 + 2;  // dwords of a row in LDS: 8-byte aligned, and rows shift banks
+  __shared__ uint32_t s_m[kWaves][64];
+  __shared__ alignas(8) uint32_t s_q[64 * kPitch];
+  const int l = threadIdx.x % kLanes, g = threadIdx.x / kLanes, wave = threadIdx.x / 64;
+  const long long t0 = blockIdx.x * 64ll;
+  const int b = blockIdx.y, f0 = b * kFp8Block + 4 * g;
+  const long long t = t0 + l * kTV;
+  const io_t* __restrict__ x = static_cast<const io_t*>(p.x) + t;
+  float v[4][kTV];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (f0 + i < p.features && t + kTV <= p.tokens) {
+      load_run(x + (f0 + i) * p.sf, v[i]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kTV; ++j) v[i][j] = f0 + i < p.features && t + j < p.tokens ? to_f32(x[(f0 + i) * p.sf + j]) : 0.f;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kTV; ++j) {
+    uint32_t m = max(max(magnitude_bits(v[0][j]), magnitude_bits(v[1][j])),
+                     max(magnitude_bits(v[2][j]), magnitude_bits(v[3][j])));
+    m = max_above<kLanes>(m);
+    if ((threadIdx.x & 63) < kLanes) s_m[wave][l * kTV + j] = m;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kTV; ++j) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) m = max(m, s_m[i][l * kTV + j]);
+    const float s = fp8_scale(__uint_as_float(m));
+    const float inv = 1.f / s;
+    if (g == 0 && t + j < p.tokens) p.scales[static_cast<long long>(b) * p.tokens + t + j] = s;
+    s_q[(l * kTV + j) * kPitch + g] = pack_fp8x4(divide_by(v[0][j], s, inv), divide_by(v[1][j], s, inv),
+                                                 divide_by(v[2][j], s, inv), divide_by(v[3][j], s, inv));
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = threadIdx.x; i < 64 * (kFp8Block / 16); i += 64 * kWaves) {
+    const int row = i / (kFp8Block / 16), c = i % (kFp8Block / 16);
+    if (t0 + row < p.tokens)
+      store_row16(p.q + (t0 + row) * p.ldq + b * kFp8Block + 16 * c, s_q + row * kPitch + 4 * c, b * kFp8Block + 16 * c,
+                  p.features);
+  }
+}
 
 // ------------------------------------------------------------------ any strides, or few tokens
 // 16 lanes hold one token's block, 8 features each; a wave covers 4 tokens.
@@ -55,8 +167,10 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(QuantParams p) {
   // A row of q is 16-byte aligned and holds at least ceil16(features) bytes up to the next row;
   // the last row's end is the tensor's, so the bytes past the features are not touched.
   unsigned char* q = p.q + t * p.ldq + f0;
-  const uint32_t lo = pack_fp8x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-  const uint32_t hi = pack_fp8x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+  const uint32_t lo = pack_fp8x4(divide_by(v[0], scale, inv), divide_by(v[1], scale, inv), divide_by(v[2], scale, inv),
+                                 divide_by(v[3], scale, inv));
+  const uint32_t hi = pack_fp8x4(divide_by(v[4], scale, inv), divide_by(v[5], scale, inv), divide_by(v[6], scale, inv),
+                                 divide_by(v[7], scale, inv));
   if (f0 + 8 <= p.features) {
     *reinterpret_cast<uint2*>(q) = make_uint2(lo, hi);
   } else {
@@ -98,7 +212,7 @@ __global__ __launch_bounds__(256) void quant_weight_kernel(QuantWeightParams p) 
   for (int i = 0; i < 32; ++i) {
     const int r = row0 + 4 * i;
     if (r >= p.M || k >= p.K) continue;
-    const uint32_t two = pack_fp8x4(v[i][0] * inv, v[i][1] * inv, 0.f, 0.f);
+    const uint32_t two = pack_fp8x4(divide_by(v[i][0], scale, inv), divide_by(v[i][1], scale, inv), 0.f, 0.f);
     unsigned char* q = p.q + r * p.ldq + k;  // k even, rows 16-byte aligned
     if (k + 1 < p.K) *reinterpret_cast<uint16_t*>(q) = static_cast<uint16_t>(two);
     else *q = static_cast<unsigned char>(two);
@@ -106,7 +220,162 @@ __global__ __launch_bounds__(256) void quant_weight_kernel(QuantWeightParams p) 
 }
 
 // ------------------------------------------------------------------ residual add + norm
-// One token a workgroup: two passes over its column.
+// The norm's factor r_t is the same for a token's whole block, so it drops out of q = y / s:
+// with y' = hn w and m' = max |y'| over the block, q = e4m3(448 y' / m') and s = r m' / 448. So
+// q needs no second pass over the features: each block leaves as it is read, and the scales,
+// kept in LDS until the sum of squares is whole, are the only thing that waits for r. That is
+// also one rounding less than hn r w. Where it does not hold (m' far below 1 or not finite, or
+// a scale at its lower bound) the block is done again from the formula.
+__device__ __forceinline__ bool scale_is_plain(float m, float r) {
+  return m == 0.f || (m > 7.9e-31f && m < __builtin_inff() && !(m * r < kFp8Max * 1.1754943508222875e-38f));
+}
+
+// One block of one token from the formula, by one thread: its scale.
+__device__ __noinline__ float norm_block_again(const float* __restrict__ hn, const float* __restrict__ w, long long T,
+                                               float r, int n, unsigned char* __restrict__ q) {
+  uint32_t m = 0;
+  for (int i = 0; i < n; ++i) m = max(m, magnitude_bits(hn[i * T] * r * w[i]));
+  const float s = fp8_scale(__uint_as_float(m));
+  const float inv = 1.f / s;
+  for (int i = 0; i < n; ++i)
+    q[i] = static_cast<unsigned char>(pack_fp8x4(divide_by(hn[i * T] * r * w[i], s, inv), 0.f, 0.f, 0.f));
+  return s;
+}
+
+// A workgroup owns 4 kL tokens and walks the features, kRound of them at a time: kL lanes hold a
+// row of 4 tokens each, a thread 4 consecutive features. The next round's rows are on their way
+// while a round is worked on (bare barriers: __syncthreads would wait for them).
+constexpr int kNormMaxBlocks = 64;  // of a token, whose maxima wait in LDS
+
+__device__ __forceinline__ void meet() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Workgroups go to the 8 XCDs in turn, and each has an L2 of its own: neighbouring tiles, which
+// share cache lines, are given to one XCD.
+__device__ __forceinline__ unsigned tile_of_xcd(unsigned id, unsigned n) {
+  const unsigned per = n / 8, rem = n % 8, x = id % 8;
+  return x * per + min(x, rem) + id / 8;
+}
+
+template <typename delta_t, bool kDelta, int kL, int kWaves>
+__global__ __launch_bounds__(64 * kWaves) void norm_fp8_tile_kernel(QuantParams p) {
+  constexpr int kTok = 4 * kL, kGroups = 64 * kWaves / kL, kRound = 4 * kGroups;
+  constexpr int kBlockWaves = kL / 2;  // waves that hold one block: 32 groups of kL lanes
+  constexpr int kPitch = kRound / 4 + 2;
+  static_assert(kRound % kFp8Block == 0 && kBlockWaves >= 1, "whole blocks and waves");
+  __shared__ uint32_t s_m[kWaves][kTok];
+  __shared__ alignas(8) uint32_t s_q[kTok * kPitch];
+  __shared__ float s_block[kNormMaxBlocks][kTok];
+  __shared__ float s_ss[kWaves][kTok];
+  const int l = threadIdx.x % kL, g = threadIdx.x / kL;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const long long T = p.tokens, t0 = static_cast<long long>(tile_of_xcd(blockIdx.x, gridDim.x)) * kTok, t = t0 + 4 * l;
+  const int F = p.features;
+  const bool whole = t + 4 <= T;
+  const float* __restrict__ h = static_cast<const float*>(p.x) + t;
+  const delta_t* __restrict__ delta = static_cast<const delta_t*>(p.delta) + t;
+
+  float hv[4][4], dv[4][4], wv[4];
+  const auto fetch = [&](int f0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int f = f0 + i < F ? f0 + i : F - 1;
+      wv[i] = p.w[f];
+      if (whole) {
+        load_run(h + f * T, hv[i]);
+        if constexpr (kDelta) load_run(delta + f * T, dv[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          hv[i][j] = t + j < T ? h[f * T + j] : 0.f;
+          if constexpr (kDelta) dv[i][j] = t + j < T ? to_f32(delta[f * T + j]) : 0.f;
+        }
+      }
+    }
+  };
+  float ss[4] = {0.f, 0.f, 0.f, 0.f};
+  fetch(4 * g);
+  for (int f0 = 4 * g; f0 - 4 * g < F; f0 += kRound) {
+    float y[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool in = f0 + i < F;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float x = kDelta ? hv[i][j] + dv[i][j] : hv[i][j];
+        y[i][j] = in ? x : 0.f;
+        ss[j] = __builtin_fmaf(y[i][j], y[i][j], ss[j]);
+      }
+      if constexpr (kDelta) {
+        if (in) {
+          float* o = p.hn + (f0 + i) * T + t;
+          if (whole) {
+            __builtin_memcpy(o, y[i], 16);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (t + j < T) o[j] = y[i][j];
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[i][j] *= wv[i];
+    }
+    if (f0 - 4 * g + kRound < F) fetch(f0 + kRound);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t m = max(max(magnitude_bits(y[0][j]), magnitude_bits(y[1][j])),
+                       max(magnitude_bits(y[2][j]), magnitude_bits(y[3][j])));
+      m = max_above<kL>(m);
+      if ((threadIdx.x & 63) < kL) s_m[wave][4 * l + j] = m;
+    }
+    meet();
+    const int b = f0 / kFp8Block;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < kBlockWaves; ++i) m = max(m, s_m[wave / kBlockWaves * kBlockWaves + i][4 * l + j]);
+      const float mf = __uint_as_float(m);
+      if (g % 32 == 0 && b < kNormMaxBlocks) s_block[b][4 * l + j] = mf;
+      const float inv = m ? kFp8Max / mf : 0.f;
+      s_q[(4 * l + j) * kPitch + g] = pack_fp8x4(y[0][j] * inv, y[1][j] * inv, y[2][j] * inv, y[3][j] * inv);
+    }
+    meet();
+    // 16 bytes of the tile each
+    const int row = threadIdx.x / (kRound / 16), c = threadIdx.x % (kRound / 16), f = f0 - 4 * g + 16 * c;
+    if (t0 + row < T) store_row16(p.q + (t0 + row) * p.ldq + f, s_q + row * kPitch + 4 * c, f, F);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float s = sum_above<kL>(ss[j]);
+    if ((threadIdx.x & 63) < kL) s_ss[wave][4 * l + j] = s;
+  }
+  __syncthreads();  // hn and q of this tile are written too, for the blocks done again
+  const int nb = (F + kFp8Block - 1) / kFp8Block;
+  for (int i = threadIdx.x; i < nb * kTok; i += 64 * kWaves) {
+    const int b = i / kTok, j = i % kTok;
+    if (t0 + j >= T) continue;
+    float tot = 0.f;
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) tot += s_ss[k][j];
+    const float r = 1.f / __builtin_sqrtf(tot / F + p.eps);
+    const float m = s_block[b][j];
+    float s = fp8_scale(m * r);
+    if (!scale_is_plain(m, r)) {
+      const int f = b * kFp8Block;
+      s = norm_block_again((kDelta ? p.hn : static_cast<const float*>(p.x)) + f * T + t0 + j, p.w + f, T, r,
+                           min(kFp8Block, F - f), p.q + (t0 + j) * p.ldq + f);
+    }
+    p.scales[b * T + t0 + j] = s;
+  }
+}
+
+// Few tokens, or more features than the tiles take: one token a workgroup, two passes over its
+// column.
 template <typename delta_t, bool kDelta>
 __global__ __launch_bounds__(512) void norm_fp8_rows_kernel(QuantParams p) {
   __shared__ float s_part[8];
@@ -150,7 +419,8 @@ __global__ __launch_bounds__(512) void norm_fp8_rows_kernel(QuantParams p) {
     const float scale = fp8_scale(__uint_as_float(m));
     const float inv = 1.f / scale;
     if ((threadIdx.x & 31) == 0) p.scales[(f0 / kFp8Block) * T + t] = scale;
-    const uint32_t q4 = pack_fp8x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+    const uint32_t q4 = pack_fp8x4(divide_by(v[0], scale, inv), divide_by(v[1], scale, inv), divide_by(v[2], scale, inv),
+                                   divide_by(v[3], scale, inv));
     unsigned char* q = p.q + t * p.ldq + f0;
     if (f0 + 4 <= p.features) {
       *reinterpret_cast<uint32_t*>(q) = q4;
@@ -163,9 +433,25 @@ __global__ __launch_bounds__(512) void norm_fp8_rows_kernel(QuantParams p) {
 }
 
 // --------------------------------------------------------------------------------- launches
+// Where each kernel starts to win (MI355X, us for features x tokens).
+// quant: rows/tile 2560 x 32 5.0/4.3, x 8 3.1/3.9; 2560 x 16384 bf16 81/26.4, 4.8 TB/s of the 5.2 that
+// a copy reaches.
+constexpr int kQuantTileTokens = 32;
+// norm, bf16 delta: a token a workgroup 1280 x 64 6.9, x 256 11.5; tiles of 8 tokens 9.1 and 9.5,
+// 1280 x 2048 14.2, x 4096 21.8; of 16 tokens 14.8 and 16.6, x 8192 25.1, x 16384 65; of 32 tokens
+// 19.7, 20.8, 25.7, and 50 at 16384: 4.6 TB/s.
+constexpr int kNormTileTokens = 128;
+constexpr int kNormNarrowTokens = 2560;
+constexpr int kNormMiddleTokens = 8192;
+
 template <typename io_t>
-static void launch_quant_rows(const QuantParams& p, hipStream_t stream) {
-  const dim3 grid((p.tokens + 15) / 16, (p.features + kFp8Block - 1) / kFp8Block);
+static void launch_quant(const QuantParams& p, hipStream_t stream) {
+  const unsigned blocks = (p.features + kFp8Block - 1) / kFp8Block;
+  if (p.st == 1 && p.tokens >= kQuantTileTokens) {
+    hipLaunchKernelGGL((quant_tile_kernel<io_t>), dim3((p.tokens + 63) / 64, blocks), dim3(128 * sizeof(io_t)), 0, stream, p);
+    return;
+  }
+  const dim3 grid((p.tokens + 15) / 16, blocks);
   // 16-byte loads where a token's features are contiguous and its row starts on 16 bytes.
   const bool vec = p.sf == 1 && (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 &&
                    (p.st * static_cast<long long>(sizeof(io_t))) % 16 == 0;
@@ -174,8 +460,8 @@ static void launch_quant_rows(const QuantParams& p, hipStream_t stream) {
 }
 
 hipError_t launch_quant_fp8(const QuantParams& p, bool io_bf16, hipStream_t stream) {
-  if (io_bf16) launch_quant_rows<bf16_t>(p, stream);
-  else launch_quant_rows<float>(p, stream);
+  if (io_bf16) launch_quant<bf16_t>(p, stream);
+  else launch_quant<float>(p, stream);
   return hipGetLastError();
 }
 
@@ -186,11 +472,23 @@ hipError_t launch_quant_fp8_weight(const QuantWeightParams& p, bool io_bf16, hip
   return hipGetLastError();
 }
 
+template <typename delta_t, bool kDelta>
+static void launch_norm(const QuantParams& p, hipStream_t stream) {
+  const auto tiles = [&](int n) { return dim3((p.tokens + n - 1) / n); };
+  if (p.tokens < kNormTileTokens || p.features > kNormMaxBlocks * kFp8Block)
+    hipLaunchKernelGGL((norm_fp8_rows_kernel<delta_t, kDelta>), tiles(1), dim3(512), 0, stream, p);
+  else if (p.tokens <= kNormNarrowTokens)
+    hipLaunchKernelGGL((norm_fp8_tile_kernel<delta_t, kDelta, 2, 8>), tiles(8), dim3(512), 0, stream, p);
+  else if (p.tokens <= kNormMiddleTokens)
+    hipLaunchKernelGGL((norm_fp8_tile_kernel<delta_t, kDelta, 4, 8>), tiles(16), dim3(512), 0, stream, p);
+  else
+    hipLaunchKernelGGL((norm_fp8_tile_kernel<delta_t, kDelta, 8, 8>), tiles(32), dim3(512), 0, stream, p);
+}
+
 hipError_t launch_norm_fp8(const QuantParams& p, bool delta_bf16, hipStream_t stream) {
-  const dim3 grid(p.tokens), block(512);
-  if (!p.delta) hipLaunchKernelGGL((norm_fp8_rows_kernel<float, false>), grid, block, 0, stream, p);
-  else if (delta_bf16) hipLaunchKernelGGL((norm_fp8_rows_kernel<bf16_t, true>), grid, block, 0, stream, p);
-  else hipLaunchKernelGGL((norm_fp8_rows_kernel<float, true>), grid, block, 0, stream, p);
+  if (!p.delta) launch_norm<float, false>(p, stream);
+  else if (delta_bf16) launch_norm<bf16_t, true>(p, stream);
+  else launch_norm<float, true>(p, stream);
   return hipGetLastError();
 }
 
