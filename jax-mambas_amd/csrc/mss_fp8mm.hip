@@ -24,11 +24,6 @@ namespace mss {
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-// The sum over one block: rows of `a` (16) by rows of `b` (16). Lane l holds a's row l % 16 (the
-// result's rows) and b's row l % 16 (its columns), features 16 (l / 16) .. + 16 of the block's
-// first half and the same of the second; the result's lane l has column l % 16, rows
-// 4 (l / 16) .. + 4. The order of the features inside a block is the same in both operands, and
-// that is all their sum needs.
 // 8 e4m3 values as bf16.
 __device__ __forceinline__ bf16x8 to_bf16x8(int lo, int hi) {
   const bf16x2_t v0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false);
@@ -38,77 +33,444 @@ __device__ __forceinline__ bf16x8 to_bf16x8(int lo, int hi) {
   return bf16x8{v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
 }
 
-__device__ __forceinline__ f32x4 mfma_block_bf16(const i32x8& a, const i32x8& b) {
-  f32x4 d = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < 8; i += 2)
-    d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(to_bf16x8(a[i], a[i + 1]), to_bf16x8(b[i], b[i + 1]), d, 0, 0, 0);
-  return d;
-}
-
 __device__ __forceinline__ i32x8 join(const u32x4& lo, const u32x4& hi) {
   return i32x8{static_cast<int>(lo[0]), static_cast<int>(lo[1]), static_cast<int>(lo[2]), static_cast<int>(lo[3]),
                static_cast<int>(hi[0]), static_cast<int>(hi[1]), static_cast<int>(hi[2]), static_cast<int>(hi[3])};
 }
 
-template <typename out_t>
-__device__ __forceinline__ void store_out(const Fp8MmParams& p, int m, int t, float v) {
-  out_t* c = static_cast<out_t*>(p.c);
-  store_as(c + (p.token_major ? t * p.ldc + m : m * p.ldc + t), v);
+// A lane's 32 values of an operand's block, ready for the matrix instructions.
+template <bool kF8>
+struct MmFrag;
+template <>
+struct MmFrag<true> {
+  i32x8 v;
+  __device__ __forceinline__ void set(const u32x4& lo, const u32x4& hi) { v = join(lo, hi); }
+};
+template <>
+struct MmFrag<false> {
+  bf16x8 v[4];
+  __device__ __forceinline__ void set(const u32x4& lo, const u32x4& hi) {
+    v[0] = to_bf16x8(lo[0], lo[1]);
+    v[1] = to_bf16x8(lo[2], lo[3]);
+    v[2] = to_bf16x8(hi[0], hi[1]);
+    v[3] = to_bf16x8(hi[2], hi[3]);
+  }
+};
+// The sum over one block: rows of `a` (16) by rows of `b` (16). Lane l holds a's row l % 16 (the
+// result's rows) and b's row l % 16 (its columns), features 16 (l / 16) .. + 16 of the block's
+// first half and the same of the second; the result's lane l has column l % 16, rows
+// 4 (l / 16) .. + 4. The order of the features inside a block is the same in both operands, and
+// that is all their sum needs.
+__device__ __forceinline__ f32x4 mfma_block(const MmFrag<true>& a, const MmFrag<true>& b) {
+  const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.v, b.v, z, 0, 0, 0, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma_block(const MmFrag<false>& a, const MmFrag<false>& b) {
+  f32x4 d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[i], b.v[i], d, 0, 0, 0);
+  return d;
 }
 
-// A lane's 32 bytes of a row's block: 16 at k and 16 at k + 64. Rows start on 16 bytes; a
-// 16-byte piece is read where it begins before the row's end, but for the part of the last one
-// that is past the tensor's end, which is read byte by byte.
-__device__ __forceinline__ i32x8 load_row(const unsigned char* __restrict__ base, long long ld, int row, int rows,
-                                          int k, int K) {
-  u32x4 v[2] = {};
-  if (row < rows) {
-    const unsigned char* r = base + row * ld;
+// The 16 bytes of a row from k on, zero past K (k a multiple of 16, below the row's stride). The
+// bytes between K and the stride may hold anything, and the last row may end at K.
+__device__ __forceinline__ u32x4 load_chunk(const unsigned char* __restrict__ base, long long ld, int row, int rows, int k,
+                                         int K) {
+  const unsigned char* r = base + row * ld + k;
+  const int n = K - k;
+  u32x4 v = {};
+  if (n >= 16 || (n > 0 && row < rows - 1)) {
+    v = *reinterpret_cast<const u32x4*>(r);
+  } else {
+#pragma unroll 1
+    for (int i = n - 1; i >= 0; --i)
+      v = u32x4{(v[0] << 8) | r[i], (v[1] << 8) | (v[0] >> 24), (v[2] << 8) | (v[1] >> 24), (v[3] << 8) | (v[2] >> 24)};
+  }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int kk = k + 64 * h;
-      if (kk + 16 <= K) {
-        v[h] = *reinterpret_cast<const u32x4*>(r + kk);
-      } else if (kk < K) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (kk + i < K) v[h][i / 4] |= static_cast<uint32_t>(r[kk + i]) << (8 * (i % 4));
+  for (int d = 0; d < 4; ++d) {
+    const int left = n - 4 * d;
+    v[d] &= left <= 0 ? 0u : left >= 4 ? 0xffffffffu : (1u << (8 * left)) - 1;
+  }
+  return v;
+}
+
+// ------------------------------------------------------------------------- few tokens, few tiles
+// No LDS on the way in: a wave reads its operands' rows straight from memory and the caches, a
+// block ahead of the products. The kKS waves of a workgroup share one tile of 16 kMT x 16 kNT,
+// every kKS-th block each, and their sums meet in LDS in a fixed order.
+struct RowBlock {
+  u32x4 v[2];  // 16 bytes at 16 g and 16 at 16 g + 64 of the block
+  __device__ __forceinline__ void load(const unsigned char* __restrict__ base, long long ld, int row, int rows, int k,
+                                       int K) {
+    v[0] = v[1] = u32x4{0, 0, 0, 0};
+    if (row < rows) {
+      const unsigned char* r = base + row * ld + k;
+      if (k + 80 <= K) {
+        v[0] = *reinterpret_cast<const u32x4*>(r);
+        v[1] = *reinterpret_cast<const u32x4*>(r + 64);
+      } else {
+        v[0] = load_chunk(base, ld, row, rows, k, K);
+        v[1] = load_chunk(base, ld, row, rows, k + 64, K);
       }
     }
   }
-  return join(v[0], v[1]);
-}
+};
 
-// One wave, one 16 x 16 tile of C.
-template <typename out_t>
-__global__ __launch_bounds__(64) void fp8mm_kernel(Fp8MmParams p) {
-  const int lane = threadIdx.x, col = lane & 15, grp = lane >> 4;
-  const int m0 = blockIdx.x * 16, t0 = blockIdx.y * 16;
+template <int kMT, int kNT, int kKS, typename out_t>
+__global__ __launch_bounds__(64 * kKS) void fp8mm_rows_kernel(Fp8MmParams p) {
+  constexpr int kTiles = kMT * kNT;
+  __shared__ f32x4 s_part[kKS - 1][kTiles * 64];
+  const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int m0 = blockIdx.x * 16 * kMT, t0 = blockIdx.y * 16 * kNT;
   const int nkb = (p.K + kFp8Block - 1) / kFp8Block;
-  const float* __restrict__ ws = p.ws + static_cast<long long>(m0 / kFp8Block) * nkb;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int b = 0; b < nkb; ++b) {
-    const int k = b * kFp8Block + grp * 16;
-    const i32x8 w = load_row(p.w, p.ldw, m0 + col, p.M, k, p.K);
-    const i32x8 x = load_row(p.x, p.ldx, t0 + col, p.T, k, p.K);
-    const float s = t0 + col < p.T ? p.xs[static_cast<long long>(b) * p.T + t0 + col] * ws[b] : 0.f;
-    const f32x4 d = mfma_block_bf16(w, x);
+  const float* __restrict__ ws = p.ws + static_cast<long long>(m0 / kFp8Block) * nkb;  // 16 kMT divides 128
+  f32x4 acc[kMT][kNT];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(d[i], s, acc[i]);
+  for (int a = 0; a < kMT; ++a)
+#pragma unroll
+    for (int c = 0; c < kNT; ++c) acc[a][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  RowBlock w[kMT], x[kNT];
+  float s[kNT];
+  const auto fetch = [&](int b) {
+    const int k = b * kFp8Block + 16 * g;
+#pragma unroll
+    for (int a = 0; a < kMT; ++a) w[a].load(p.w, p.ldw, m0 + 16 * a + j, p.M, k, p.K);
+    const float sw = ws[b];
+#pragma unroll
+    for (int c = 0; c < kNT; ++c) {
+      const int t = t0 + 16 * c + j;
+      x[c].load(p.x, p.ldx, t, p.T, k, p.K);
+      s[c] = t < p.T ? p.xs[static_cast<long long>(b) * p.T + t] * sw : 0.f;
+    }
+  };
+  int b = wave;
+  if (b < nkb) fetch(b);
+  for (; b < nkb; b += kKS) {
+    MmFrag<false> wf[kMT], xf[kNT];
+    float sc[kNT];
+#pragma unroll
+    for (int a = 0; a < kMT; ++a) wf[a].set(w[a].v[0], w[a].v[1]);
+#pragma unroll
+    for (int c = 0; c < kNT; ++c) {
+      xf[c].set(x[c].v[0], x[c].v[1]);
+      sc[c] = s[c];
+    }
+    if (b + kKS < nkb) fetch(b + kKS);
+#pragma unroll
+    for (int c = 0; c < kNT; ++c)
+#pragma unroll
+      for (int a = 0; a < kMT; ++a) {
+        const f32x4 d = mfma_block(wf[a], xf[c]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[a][c][e] = __builtin_fmaf(d[e], sc[c], acc[a][c][e]);
+      }
   }
-  if (t0 + col >= p.T) return;
+  if (wave > 0) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int m = m0 + grp * 4 + i;
-    if (m < p.M) store_out<out_t>(p, m, t0 + col, acc[i]);
+    for (int i = 0; i < kTiles; ++i) s_part[wave - 1][i * 64 + lane] = acc[i / kNT][i % kNT];
+  }
+  __syncthreads();
+  if (wave > 0) return;
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+    for (int q = 0; q < kKS - 1; ++q) acc[i / kNT][i % kNT] += s_part[q][i * 64 + lane];
+  // Lane: column t of the tile, 4 rows of W.
+  out_t* __restrict__ C = static_cast<out_t*>(p.c);
+#pragma unroll
+  for (int c = 0; c < kNT; ++c) {
+    const int t = t0 + 16 * c + j;
+    if (t >= p.T) continue;
+#pragma unroll
+    for (int a = 0; a < kMT; ++a) {
+      const int m = m0 + 16 * a + 4 * g;
+      out_t v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) store_as(&v[e], acc[a][c][e]);
+      if (p.token_major && m + 4 <= p.M) {
+        __builtin_memcpy(C + t * p.ldc + m, v, sizeof(v));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (m + e < p.M) C[p.token_major ? t * p.ldc + m + e : (m + e) * p.ldc + t] = v[e];
+      }
+    }
   }
 }
 
+template <int kMT, int kNT, int kKS>
+static void launch_rows(const Fp8MmParams& p, hipStream_t stream) {
+  const dim3 grid((p.M + 16 * kMT - 1) / (16 * kMT), (p.T + 16 * kNT - 1) / (16 * kNT));
+  if (p.out_bf16) hipLaunchKernelGGL((fp8mm_rows_kernel<kMT, kNT, kKS, bf16_t>), grid, dim3(64 * kKS), 0, stream, p);
+  else hipLaunchKernelGGL((fp8mm_rows_kernel<kMT, kNT, kKS, float>), grid, dim3(64 * kKS), 0, stream, p);
+}
+
+// ------------------------------------------------------------------------------ large products
+// Both operands are "rows of K bytes", so the kernel is written for a row operand R, whose index
+// runs along C's rows in memory, and a column operand Q: C[q * ldc + r]. R is X for a
+// features-major C and W for a token-major one.
+//
+// A workgroup computes a kBR x kBQ tile. The operands' blocks of 128 features travel global ->
+// LDS in two stages by direct copies (16 bytes a lane), one in flight while the other is
+// multiplied. A row's 8 chunks of 16 bytes are stored at chunk ^ key(row), with keys that let the
+// 16 rows of an operand read cover all banks. The wave's tiles of 16 R rows take every fourth
+// group of 4 out of 64 rows, so that a lane ends up with 16 consecutive rows of a column and C
+// leaves in 16-byte stores, whole 128-byte lines for a bf16 wave; they are not kept in the L2, which
+// the operands need (130 us against 149 for 5120 x 1280 x 16384).
+//
+// What bounds that size: its parts alone take 80 us (the copies), 97 (LDS reads, products and sums
+// of one block's data over and over) and about 35 (the stores, 168 MB), and the two workgroups of a
+// CU overlap them in part.
+__device__ __forceinline__ int r_key(int row) { return ((row >> 3) & 6) | ((row >> 1) & 1); }
+__device__ __forceinline__ int q_key(int row) { return (row >> 1) & 7; }
+
+template <int kBR_, int kBQ_, int kWR_, int kWQ_>
+struct MmShape {
+  static constexpr int kBR = kBR_, kBQ = kBQ_, kWR = kWR_, kWQ = kWQ_, kWaves = kWR * kWQ, kThreads = 64 * kWaves;
+  static constexpr int kRT = kBR / kWR / 16, kQT = kBQ / kWQ / 16;  // 16 x 16 tiles of a wave
+  static constexpr int kRCopies = kBR * 8 / kThreads, kQCopies = kBQ * 8 / kThreads;
+  static_assert(kRT % 4 == 0 && kBR / 64 <= kWaves && kBQ / 64 <= kWaves && kBR * 8 % kThreads == 0 &&
+                kBQ * 8 % kThreads == 0, "");
+};
+
+typedef const __attribute__((address_space(4))) float* const_f32_t;
+
+struct MmOperand {
+  const unsigned char* base;
+  long long ld;
+  int rows;
+};
+
+template <typename S, bool kF8, typename out_t, bool kTokenRows>
+__global__ __launch_bounds__(S::kThreads, 2) void fp8mm_tile_kernel(Fp8MmParams p, int tiles_r, int tiles_q) {
+#if defined(__HIP_DEVICE_COMPILE__)  // the host's pass knows no buffer resources
+  constexpr int kToks = kTokenRows ? S::kBR : S::kBQ;
+  __shared__ u32x4 sR0[S::kBR * 8], sQ0[S::kBQ * 8], sR1[S::kBR * 8], sQ1[S::kBQ * 8];
+  __shared__ alignas(16) float sS0[kToks], sS1[kToks];
+  const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wr = wave % S::kWR, wq = wave / S::kWR;
+  const MmOperand R = kTokenRows ? MmOperand{p.x, p.ldx, p.T} : MmOperand{p.w, p.ldw, p.M};
+  const MmOperand Q = kTokenRows ? MmOperand{p.w, p.ldw, p.M} : MmOperand{p.x, p.ldx, p.T};
+  const int nkb = (p.K + kFp8Block - 1) / kFp8Block;
+
+  // Neighbouring tiles on one XCD: 8 of R by 4 of Q share their operands in its L2.
+  int tr, tq;
+  {
+    const unsigned n = gridDim.x, per = n / 8, rem = n % 8, x = blockIdx.x % 8;
+    const unsigned id = x * per + min(x, rem) + blockIdx.x / 8;
+    const unsigned group = id / (8 * tiles_q), first = group * 8, wide = min(8u, tiles_r - first);
+    const unsigned in = id - group * 8 * tiles_q;
+    tr = first + in % wide;
+    tq = in / wide;
+  }
+  const int r0 = tr * S::kBR, q0 = tq * S::kBQ;
+
+  // Copy i of a stage: slots 64 i + lane, row slot / 8, stored chunk slot % 8. Rows past the
+  // operand's end read its last row; their products are not stored.
+  uint32_t off_r[S::kRCopies], off_q[S::kQCopies];
+#pragma unroll
+  for (int t = 0; t < S::kRCopies; ++t) {
+    const int row = 8 * (wave + S::kWaves * t) + (lane >> 3);
+    off_r[t] = static_cast<uint32_t>(min(row, R.rows - 1 - r0)) * static_cast<uint32_t>(R.ld) + 16 * ((lane & 7) ^ r_key(row));
+  }
+#pragma unroll
+  for (int t = 0; t < S::kQCopies; ++t) {
+    const int row = 8 * (wave + S::kWaves * t) + (lane >> 3);
+    off_q[t] = static_cast<uint32_t>(min(row, Q.rows - 1 - q0)) * static_cast<uint32_t>(Q.ld) + 16 * ((lane & 7) ^ q_key(row));
+  }
+  const auto rsrc = [](const MmOperand& o, int first, int K) {
+    const long long n = (o.rows - 1 - first) * o.ld + K;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(o.base + first * o.ld), 0,
+                                             static_cast<uint32_t>(n < 0xffffffffll ? n : 0xffffffffll), 0x00027000);
+  };
+  const auto bufR = rsrc(R, r0, p.K), bufQ = rsrc(Q, q0, p.K);
+  const int t0 = kTokenRows ? r0 : q0;
+  const auto issue_scales = [&](int b, float* dS) {
+    if (wave < kToks / 64)
+      __builtin_amdgcn_global_load_lds((gbl_void_t)(p.xs + static_cast<long long>(b) * p.T + min(t0 + 64 * wave + lane, p.T - 1)),
+                                       (lds_void_t)(dS + 64 * wave), 4, 0, 0);
+  };
+  const auto issue = [&](int b, u32x4* dR, u32x4* dQ, float* dS) {
+    issue_scales(b, dS);
+#pragma unroll
+    for (int t = 0; t < S::kRCopies; ++t)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(bufR, (lds_void_t)(dR + 64 * (wave + S::kWaves * t)), 16, off_r[t],
+                                               b * kFp8Block, 0, 0);
+#pragma unroll
+    for (int t = 0; t < S::kQCopies; ++t)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(bufQ, (lds_void_t)(dQ + 64 * (wave + S::kWaves * t)), 16, off_q[t],
+                                               b * kFp8Block, 0, 0);
+  };
+
+  // The wave's rows of W lie in one block.
+  const int wrow = (kTokenRows ? q0 + wq * (16 * S::kQT) : r0 + wr * (16 * S::kRT)) / kFp8Block;
+  static_assert(kFp8Block % (16 * (kTokenRows ? S::kQT : S::kRT)) == 0, "a wave's part of W lies in one block");
+  // (constant address space: a scalar load, where a vector load would be waited for together with
+  // the copies issued before it)
+  const auto ws = reinterpret_cast<const_f32_t>(
+      reinterpret_cast<uintptr_t>(p.ws + static_cast<long long>(min(wrow, (p.M - 1) / kFp8Block)) * nkb));
+
+  f32x4 acc[S::kRT][S::kQT];
+#pragma unroll
+  for (int a = 0; a < S::kRT; ++a)
+#pragma unroll
+    for (int b = 0; b < S::kQT; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  // This lane's rows in the stages: of R, tile a at + 4 (a % 4) + 64 (a / 4) rows; of Q, tile c at
+  // + 16 c rows. The keys are the same for all tiles.
+  const int row_r = wr * (16 * S::kRT) + 16 * (j >> 2) + (j & 3), key_r = r_key(16 * (j >> 2) + (j & 3));
+  const int row_q = wq * (16 * S::kQT) + j, key_q = q_key(j);
+  const int r_lo = row_r * 8 + (g ^ key_r), r_hi = row_r * 8 + ((g + 4) ^ key_r);
+  const int q_lo = row_q * 8 + (g ^ key_q), q_hi = row_q * 8 + ((g + 4) ^ key_q);
+  const auto compute = [&](const u32x4* bR, const u32x4* bQ, const float* bS, float w) {
+    MmFrag<kF8> r[S::kRT];
+    f32x4 sr[kTokenRows ? S::kRT : 1];
+#pragma unroll
+    for (int a = 0; a < S::kRT; ++a) {
+      const int at = 4 * (a & 3) + 64 * (a / 4);
+      r[a].set(bR[r_lo + 8 * at], bR[r_hi + 8 * at]);
+      if constexpr (kTokenRows) sr[a] = *reinterpret_cast<const f32x4*>(bS + wr * (16 * S::kRT) + 16 * g + at) * w;
+    }
+    // Products two by two; each pair is scaled and added while the next one is under way. The
+    // empty asm statements and scheduler barriers keep it so: left alone, the sums move behind all
+    // of the block's products, whose results then spill.
+    constexpr int kPairs = S::kRT / 2;
+    f32x4 d[2][2];
+    float sq[2];
+    MmFrag<kF8> q[2];
+    const auto load_q = [&](int c) {
+      q[c & 1].set(bQ[q_lo + 128 * c], bQ[q_hi + 128 * c]);
+      if constexpr (!kTokenRows) sq[c & 1] = bS[row_q + 16 * c] * w;
+    };
+    const auto add = [&](int i) {
+      const int c = i / kPairs;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int a = 2 * (i % kPairs) + h;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          acc[a][c][e] = __builtin_fmaf(d[i & 1][h][e], kTokenRows ? sr[a][e] : sq[c & 1], acc[a][c][e]);
+        asm volatile("" : "+v"(acc[a][c]));
+      }
+    };
+    load_q(0);
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int i = 0; i < kPairs * S::kQT; ++i) {
+      const int c = i / kPairs;
+      if (i % kPairs == 1 && c + 1 < S::kQT) load_q(c + 1);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) d[i & 1][h] = mfma_block(r[2 * (i % kPairs) + h], q[c & 1]);
+      __builtin_amdgcn_sched_barrier(0);
+      if (i > 0) add(i - 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    add(kPairs * S::kQT - 1);
+    __builtin_amdgcn_s_setprio(0);
+  };
+
+  const auto meet = [] {  // this wave's copies have landed and its reads are done; so have all waves'
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0), the builtin so that the compiler knows too
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  const int full = p.K / kFp8Block;
+  if (full > 0) issue(0, sR0, sQ0, sS0);
+  for (int b = 0; b + 1 < full; b += 2) {
+    meet();
+    issue(b + 1, sR1, sQ1, sS1);
+    compute(sR0, sQ0, sS0, ws[b]);
+    meet();
+    if (b + 2 < full) issue(b + 2, sR0, sQ0, sS0);
+    compute(sR1, sQ1, sS1, ws[b + 1]);
+  }
+  if (full & 1) {
+    meet();
+    compute(sR0, sQ0, sS0, ws[full - 1]);
+  }
+  if (full < nkb) {  // the features past K are zeros, whatever lies in the rows' padding
+    const int k0 = full * kFp8Block;
+    meet();
+    issue_scales(full, sS0);
+#pragma unroll 1
+    for (int t = 0; t < S::kRCopies; ++t) {
+      const int i = wave + S::kWaves * t, row = 8 * i + (lane >> 3);
+      sR0[64 * i + lane] = load_chunk(R.base, R.ld, min(r0 + row, R.rows - 1), R.rows, k0 + 16 * ((lane & 7) ^ r_key(row)), p.K);
+    }
+#pragma unroll 1
+    for (int t = 0; t < S::kQCopies; ++t) {
+      const int i = wave + S::kWaves * t, row = 8 * i + (lane >> 3);
+      sQ0[64 * i + lane] = load_chunk(Q.base, Q.ld, min(q0 + row, Q.rows - 1), Q.rows, k0 + 16 * ((lane & 7) ^ q_key(row)), p.K);
+    }
+    meet();
+    compute(sR0, sQ0, sS0, ws[full]);
+  }
+
+  // A lane's 16 rows of a column.
+  out_t* __restrict__ C = static_cast<out_t*>(p.c);
+#pragma unroll
+  for (int c = 0; c < S::kQT; ++c) {
+    const int q = q0 + wq * (16 * S::kQT) + 16 * c + j;
+    if (q >= Q.rows) continue;
+#pragma unroll
+    for (int h = 0; h < S::kRT / 4; ++h) {
+      const int r = r0 + wr * (16 * S::kRT) + 64 * h + 16 * g;
+      out_t* __restrict__ dst = C + q * p.ldc + r;
+      alignas(16) out_t v[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) store_as(&v[e], acc[4 * h + e / 4][c][e % 4]);
+      if (r + 16 <= R.rows) {
+#pragma unroll
+        for (int e = 0; e < static_cast<int>(sizeof(v) / 16); ++e)
+          __builtin_nontemporal_store(reinterpret_cast<const u32x4*>(v)[e], reinterpret_cast<u32x4_any*>(dst) + e);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (r + e < R.rows) dst[e] = v[e];
+      }
+    }
+  }
+#endif
+}
+
+template <typename S, bool kF8, typename out_t>
+static void launch_tiles(const Fp8MmParams& p, hipStream_t stream) {
+  const int nr = p.token_major ? p.M : p.T, nq = p.token_major ? p.T : p.M;
+  const int tr = (nr + S::kBR - 1) / S::kBR, tq = (nq + S::kBQ - 1) / S::kBQ;
+  if (p.token_major)
+    hipLaunchKernelGGL((fp8mm_tile_kernel<S, kF8, out_t, false>), dim3(tr * tq), dim3(S::kThreads), 0, stream, p, tr, tq);
+  else
+    hipLaunchKernelGGL((fp8mm_tile_kernel<S, kF8, out_t, true>), dim3(tr * tq), dim3(S::kThreads), 0, stream, p, tr, tq);
+}
+
+// 128 x 128 tiles, four waves of 64 x 64, two workgroups a CU, whose copies, products and stores
+// fall at different times. (256 x 256 tiles of eight waves, one workgroup a CU: 139 us against 130
+// for 5120 x 1280 x 16384, 139 against 115 for 5120 x 5120 x 4096.)
+typedef MmShape<128, 128, 2, 2> MmTiles;
+
+// Which kernel. The time of the rows kernels goes with the row blocks that their workgroups read
+// (0.27 ns each over about 3 us), that of the tiles with the blocks of K, 0.75 us each while every
+// tile has a CU to itself and 1.3 us (float32 output: 1.15 and 2.1) for each 512 tiles beyond.
+// Measured (us, M x K x T): 1 x 1 tiles of eight waves, 2 x 1 and 2 x 2 of four, 128 x 128:
+// 5120 x 1280 x 1 3.8 / 4.8 / - / 10.4; 5120 x 1280 x 64 8.4 / 7.8 / 8.7 / 10.4; 50280 x 768 x 8
+// 12.8 / 10.5 / - / -; 1280 x 2560 x 333 18.0 / 16.8 / 13.8 / 17.2; 1280 x 2560 x 600 29.5 / 23.4 /
+// 18.4 / 17.6; 5120 x 1280 x 16384 - / - / - / 130: 1.65 PFLOP/s, where the library's product with
+// one scale an operand reaches 3.0 at 8192^3.
 hipError_t launch_fp8mm(const Fp8MmParams& p, hipStream_t stream) {
-  const dim3 grid((p.M + 15) / 16, (p.T + 15) / 16);
-  if (p.out_bf16) hipLaunchKernelGGL(fp8mm_kernel<bf16_t>, grid, dim3(64), 0, stream, p);
-  else hipLaunchKernelGGL(fp8mm_kernel<float>, grid, dim3(64), 0, stream, p);
+  const long long nkb = (p.K + kFp8Block - 1) / kFp8Block;
+  const auto tiles = [&](int m, int t) { return ((p.M + m - 1ll) / m) * ((p.T + t - 1ll) / t); };
+  const double rows22 = 3 + 0.00027 * static_cast<double>(4 * tiles(32, 32) * nkb);
+  const double block = p.out_bf16 ? 1.0 : 1.6, big = static_cast<double>((tiles(128, 128) + 511) / 512);
+  const double whole = 3 + block * static_cast<double>(nkb) * (tiles(128, 128) <= 256 ? 0.75 : 1.3 * big);
+  const bool far = p.ldw >= 1 << 24 || p.ldx >= 1 << 24;  // the tiles' offsets have 32 bits
+  if (2 * tiles(16, 16) * nkb <= 16000) launch_rows<1, 1, 8>(p, stream);
+  else if (p.T <= 16 || 3 * tiles(32, 16) * nkb <= 24000) launch_rows<2, 1, 4>(p, stream);
+  else if (far || rows22 < whole) launch_rows<2, 2, 4>(p, stream);
+  else if (p.out_bf16) launch_tiles<MmTiles, true, bf16_t>(p, stream);
+  else launch_tiles<MmTiles, false, float>(p, stream);
   return hipGetLastError();
 }
 
