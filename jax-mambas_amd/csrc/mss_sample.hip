@@ -12,9 +12,19 @@
 // A temperature that is not above zero takes the first word of the order. A row without a
 // word, or with a NaN, gives -1.
 //
-// The filters keep a prefix of the order, so they come down to one cut (a logit, and the last
-// index kept among the words with that logit), found by radix selection on the logits' order
-// in integers, counting words for top-k and adding weights for top-p; nothing is sorted.
+// One workgroup a row. The filters keep a prefix of the order, so they come down to one cut: a
+// logit, and the last index kept among the words with that logit. Nothing is sorted:
+//
+//   1. the largest logit, and the largest of 3072 groups of the row. The k-th largest of those is a
+//      bound that k words reach and few others do; min-p is a bound by itself.
+//   2. the words that reach the bound go into a list in LDS, and the cuts and the draw are found in
+//      the list: its weights added into 2048 bins (by logit, or by index for the draw), the bin
+//      in which the sum reaches its target, and the few words of that bin one by one.
+//   3. without such a bound, or when more words reach it than the list holds, the bins are filled
+//      from the whole row, and the draw adds the words left by segments of 512.
+//   4. where one bin holds too many words (ties), a radix selection on the logits' order in
+//      integers takes any row, three passes of 11 bits.
+//
 // Weights are added as integers of 2^-43, which makes every sum exact and independent of its
 // order: at most 2^20 words a row keep it below 2^63.
 #include <hip/hip_runtime.h>
@@ -31,6 +41,11 @@ constexpr int kSampleChunk = kSampleThreads * 8;  // words a pass of the workgro
 constexpr int kSampleMaxVocab = 1 << 20;
 constexpr int kSampleMaxSeg = kSampleMaxVocab / kSampleChunk * kSampleWaves;
 constexpr int kSampleBins = 2048;  // 11 bits of the key at a time
+constexpr int kSampleRegVocab = 8 * kSampleChunk;  // rows that stay in registers, 64 words a thread
+constexpr int kSampleList = 12288;
+constexpr int kSampleSmall = 256;                  // words of one bin that are looked at one by one
+constexpr int kSampleFew = 128;                    // a list as short as this needs no bins
+constexpr int kSampleGroups = 3 * kSampleThreads;  // a thread's chunks c, c + 3, ... have one largest logit
 constexpr float kFixed = 8796093022208.f;  // 2^43
 
 // Integers in the order of the floats; -0 and 0 are the same.
@@ -43,9 +58,30 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 }
 constexpr uint32_t kAbsent = 0x007fffffu;  // order_key(-inf)
 
-// w = 2^((v - m) c), c = log2(e) / temperature in two float32 parts. The difference and the
-// product carry their rounding errors along (they would be the largest of the whole draw:
-// 2^-24 of an exponent of 20 is 1e-6 of the weight), the exponential is v_exp_f32's.
+// w = 2^((v - m) c), c = log2(e) / temperature in two float32 parts. The product carries its
+// rounding error along (c's own would shift all weights the same way), the exponential is
+// v_exp_f32's. The difference is rounded: 2^-24 of an exponent y is 2^-24 y of a weight 2^y, and
+// words far below the largest are either a small part of the sum or many, whose errors cancel.
+// For 2^-100 < c < 2^100 and finite m only. A word that is absent or below 2^-64 counts as 2^-64,
+// which is no unit of the sums.
+struct FastWeight {
+  float m, c, c_lo, least;
+  __device__ __forceinline__ float operator()(float v) const {
+    const float d = fmaxf(v - m, least);
+    const float y = d * c;
+    const float lo = __builtin_fmaf(d, c_lo, __builtin_fmaf(d, c, -y));
+    const float e = __builtin_amdgcn_exp2f(y);
+    return __builtin_fmaf(e, lo * kLn2, e);
+  }
+};
+// w (at most 1) as an integer of 2^-43, in the low bits of a double of 512 and more.
+constexpr u64 kFixedBias = 0x4080000000000000ull;  // 512.0
+__device__ __forceinline__ u64 biased_fixed(float w) {
+  return __builtin_bit_cast(u64, static_cast<double>(w) + 512.0);
+}
+
+// The same for any row (an infinite largest logit, any temperature above zero), the difference's
+// rounding error carried along too.
 struct Weight {
   float m, c, c_lo;
   __device__ __forceinline__ void set(float max, float temperature) {
@@ -72,6 +108,13 @@ __device__ __forceinline__ u64 shfl_up64(u64 v, int d) {
   const uint32_t lo = __shfl_up(static_cast<int>(v), d), hi = __shfl_up(static_cast<int>(v >> 32), d);
   return (static_cast<u64>(hi) << 32) | lo;
 }
+__device__ __forceinline__ u64 shfl64(u64 v, int lane) {
+  const uint32_t lo = __shfl(static_cast<int>(v), lane), hi = __shfl(static_cast<int>(v >> 32), lane);
+  return (static_cast<u64>(hi) << 32) | lo;
+}
+__device__ __forceinline__ int words_segments(int vocab) {  // segments that a pass over the row writes
+  return (vocab + kSampleChunk - 1) / kSampleChunk * kSampleWaves;
+}
 __device__ __forceinline__ u64 wave_incl(u64 v) {
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
@@ -90,6 +133,15 @@ struct SampleShared {
   uint32_t found_bin, found_count;
   uint32_t key;
   int index;
+  // the list: logits and their words
+  float list_v[kSampleList];
+  int list_i[kSampleList];
+  int list_n, small_n, picked;
+  struct alignas(16) Entry {
+    u64 w;
+    float v;
+    int i;
+  } small[kSampleSmall];
 };
 
 // Exclusive sum over the workgroup in thread order; `total` gets the whole sum.
@@ -116,17 +168,61 @@ struct Row {
   // Words i .. i + 8; past the row's end they are absent.
   __device__ __forceinline__ void load8(int i, float (&v)[8]) const {
     if (kVec && i + 8 <= vocab) {
-      union {
-        u32x4 w[sizeof(io_t) / 2];
-        io_t e[8];
-      } u;
+      io_t e[8];
+      __builtin_memcpy(e, x + i, sizeof(e));
 #pragma unroll
-      for (int k = 0; k < static_cast<int>(sizeof(io_t) / 2); ++k) u.w[k] = reinterpret_cast<const u32x4*>(x + i)[k];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = to_f32(u.e[k]);
+      for (int k = 0; k < 8; ++k) v[k] = to_f32(e[k]);
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] = i + k < vocab ? to_f32(x[(i + k) * sv]) : -__builtin_inff();
+    }
+  }
+};
+
+// A row's words, 8 at a time to a thread: f(words, index of the first, chunk, chunk % 3 as a type).
+// Short rows are read once and stay in registers.
+template <int kV>
+struct Third {
+  static constexpr int value = kV;
+};
+template <typename io_t, bool kVec, bool kReg>
+struct Words {
+  Row<io_t, kVec> row;
+  float held[kReg ? 8 : 1][8];
+  __device__ __forceinline__ void start() {
+    if constexpr (kReg) {
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (c * kSampleChunk < row.vocab) row.load8(c * kSampleChunk + threadIdx.x * 8, held[c]);
+    }
+  }
+  template <typename F>
+  __device__ __forceinline__ void each(const F& f) const {
+    const int i = threadIdx.x * 8;
+    if constexpr (kReg) {
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        if (c * kSampleChunk < row.vocab) {
+          if (c % 3 == 0) f(held[c], c * kSampleChunk + i, c, Third<0>());
+          else if (c % 3 == 1) f(held[c], c * kSampleChunk + i, c, Third<1>());
+          else f(held[c], c * kSampleChunk + i, c, Third<2>());
+        }
+      }
+    } else {  // two chunks ahead
+      float v[3][8];
+      const int n = (row.vocab + kSampleChunk - 1) / kSampleChunk;
+      row.load8(i, v[0]);
+      row.load8(kSampleChunk + i, v[1]);
+      for (int c = 0; c < n; c += 3) {
+        row.load8((c + 2) * kSampleChunk + i, v[2]);
+        f(v[0], c * kSampleChunk + i, c, Third<0>());
+        if (c + 1 >= n) break;
+        row.load8((c + 3) * kSampleChunk + i, v[0]);
+        f(v[1], (c + 1) * kSampleChunk + i, c + 1, Third<1>());
+        if (c + 2 >= n) break;
+        row.load8((c + 4) * kSampleChunk + i, v[1]);
+        f(v[2], (c + 2) * kSampleChunk + i, c + 2, Third<2>());
+      }
     }
   }
 };
@@ -222,50 +318,10 @@ __device__ void select(SampleShared& s, const row_t& row, const Weight& weight, 
   __syncthreads();
 }
 
-template <typename io_t, bool kVec>
-__global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleParams p) {
-  __shared__ SampleShared s;
-  const long long r = blockIdx.x;
-  const Row<io_t, kVec> row{static_cast<const io_t*>(p.logits) + r * p.sr, p.sv, p.vocab};
-  const float temperature = p.temperatures ? p.temperatures[r] : p.temperature;
-  const int top_k = p.top_ks ? p.top_ks[r] : p.top_k;
-  const float top_p = p.top_ps ? p.top_ps[r] : p.top_p;
-  const float min_p = p.min_ps ? p.min_ps[r] : p.min_p;
-  const double u = static_cast<double>(p.uniform[r]);
-
-  // The largest logit's key; a NaN counts as the largest of all.
-  uint32_t top = 0;
-  for (int i = threadIdx.x * 8; i < row.vocab; i += kSampleChunk) {
-    float v[8];
-    row.load8(i, v);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) top = max(top, v[k] != v[k] ? 0xffffffffu : order_key(v[k]));
-  }
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d)));
-  if ((threadIdx.x & 63) == 0) s.wave[threadIdx.x >> 6] = top;
-  if (threadIdx.x == 0) s.index = 0x7fffffff;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kSampleWaves; ++i) top = max(top, static_cast<uint32_t>(s.wave[i]));
-  if (top == 0xffffffffu || top <= kAbsent) {
-    if (threadIdx.x == 0) p.tokens[r] = -1;
-    return;
-  }
-  if (!(temperature > 0.f) || top_k == 1 || min_p > 1.f) {  // the first word of the order
-    for (int i = threadIdx.x * 8; i < row.vocab; i += kSampleChunk) {
-      float v[8];
-      row.load8(i, v);
-      int first = 0x7fffffff;
-#pragma unroll
-      for (int k = 7; k >= 0; --k)
-        if (order_key(v[k]) == top) first = i + k;
-      if (first != 0x7fffffff) atomicMin(&s.index, first);
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) p.tokens[r] = s.index;
-    return;
-  }
+// The draw of any row, whole passes over it each time.
+template <typename row_t>
+__device__ __forceinline__ void draw_by_radix(SampleShared& s, const row_t row, uint32_t top, float temperature, int top_k,
+                                           float top_p, float min_p, double u, long long* token) {
   Weight weight;
   weight.set(key_value(top), temperature);
 
@@ -273,7 +329,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleParams p) 
   uint32_t cut_key = kAbsent;
   int cut_index = -1;
   u64 total;
-  const bool by_k = top_k > 0 && top_k < p.vocab, by_p = top_p < 1.f;
+  const bool by_k = top_k > 0 && top_k < row.vocab, by_p = top_p < 1.f;
   if (by_k) {
     u64 words = 0;
     for (int i = threadIdx.x * 8; i < row.vocab; i += kSampleChunk) {
@@ -338,18 +394,493 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleParams p) 
   u64 run = before + wave_incl(sum) - sum;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    if (run <= at && at < run + w[k]) p.tokens[r] = i + k;
+    if (run <= at && at < run + w[k]) *token = i + k;
     run += w[k];
   }
 }
 
+// ------------------------------------------------------------------------- bins and the list
+// Zeroes the bins; ends with a barrier.
+__device__ __forceinline__ void clear_bins(SampleShared& s) {
+  for (int i = threadIdx.x; i < kSampleBins; i += kSampleThreads) s.mass[i] = 0;
+  if (threadIdx.x == 0) {
+    s.small_n = 0;
+    s.found_bin = kSampleBins;
+  }
+  __syncthreads();
+}
+
+// The first bin at which the running sum reaches `target` (at least 1): its number and the sum
+// before it; kSampleBins where the whole sum does not. Ends with a barrier.
+__device__ __forceinline__ void reach_bin(SampleShared& s, u64 target, uint32_t& bin, u64& before) {
+  __syncthreads();
+  const int at = 2 * threadIdx.x;
+  const u64 a = s.mass[at], b = s.mass[at + 1];
+  u64 total;
+  const u64 excl = block_excl(s, a + b, total);
+  if (excl < target && target <= excl + a + b) {
+    const bool first = target <= excl + a;
+    s.found_bin = first ? at : at + 1;
+    s.found_above = first ? excl : excl + a;
+  }
+  __syncthreads();
+  bin = s.found_bin;
+  before = s.found_above;
+}
+
+// Bins by logit: monotone in it, the largest in bin 0.
+struct ByLogit {
+  float m, scale;
+  __device__ __forceinline__ ByLogit(float max, float least) : m(max), scale(0.f) {
+    const float range = max - least;  // the least logit's bin is the last
+    if (range > 0.f) scale = (kSampleBins - 1) / range;
+    if (!(scale < 1e37f)) scale = 0.f;  // (a range too small to divide by: one bin)
+  }
+  __device__ __forceinline__ uint32_t bin(float v, int) const {
+    return static_cast<uint32_t>(fminf((m - v) * scale, static_cast<float>(kSampleBins - 1)));
+  }
+  static __device__ __forceinline__ bool before(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
+};
+struct ByIndex {
+  int shift;
+  __device__ __forceinline__ explicit ByIndex(int vocab) : shift(max(0, 21 - __clz(vocab))) {}  // vocab >> shift < 2048
+  __device__ __forceinline__ uint32_t bin(float, int i) const { return static_cast<uint32_t>(i) >> shift; }
+  static __device__ __forceinline__ bool before(float, int i, float, int j) { return i < j; }
+};
+
+// Of the list's words, the one at which the running weight in `order` reaches `target`; false where
+// its bin holds too many. Every thread gets it.
+template <typename order_t, typename weight_t>
+__device__ __forceinline__ bool pick(SampleShared& s, int n, const order_t& order, const weight_t& weight, u64 target,
+                                     float& v, int& i) {
+  clear_bins(s);
+  for (int e = threadIdx.x; e < n; e += kSampleThreads) {
+    const u64 w = weight(e);
+    if (w) atomicAdd(&s.mass[order.bin(s.list_v[e], s.list_i[e])], w);
+  }
+  uint32_t bin;
+  u64 before;
+  reach_bin(s, target, bin, before);
+  for (int e = threadIdx.x; e < n; e += kSampleThreads) {
+    if (order.bin(s.list_v[e], s.list_i[e]) != bin) continue;
+    const u64 w = weight(e);
+    if (w) {
+      const int at = atomicAdd(&s.small_n, 1);
+      if (at < kSampleSmall) s.small[at] = SampleShared::Entry{w, s.list_v[e], s.list_i[e]};
+    }
+  }
+  __syncthreads();
+  const int few = s.small_n;
+  if (few > kSampleSmall) return false;
+  if (static_cast<int>(threadIdx.x) < few) {
+    const SampleShared::Entry mine = s.small[threadIdx.x];
+    u64 sum = before;
+#pragma unroll 4
+    for (int k = 0; k < few; ++k) {
+      const SampleShared::Entry o = s.small[k];
+      sum += order.before(o.v, o.i, mine.v, mine.i) ? o.w : 0;
+    }
+    if (sum < target && target <= sum + mine.w) s.picked = threadIdx.x;
+  }
+  __syncthreads();
+  v = s.small[s.picked].v;
+  i = s.small[s.picked].i;
+  __syncthreads();
+  return true;
+}
+
+// Puts those of a thread's 8 words into the list that `takes` says, a wave's at once: one atomic for
+// its places. By whole waves.
+template <typename takes_t>
+__device__ __forceinline__ void append(SampleShared& s, const float (&v)[8], int i, const takes_t& takes) {
+  u64 mask[8], any = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) any |= mask[k] = __ballot(takes(v[k], i + k));
+  if (any == 0) return;
+  int n = 0, at = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) n += __popcll(mask[k]);
+  if ((threadIdx.x & 63) == 0) at = atomicAdd(&s.list_n, n);
+  at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    if (mask[k]) {
+      const int mine = at + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask[k] >> 32),
+                                                      __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask[k]), 0));
+      if ((mask[k] >> (threadIdx.x & 63) & 1) && mine < kSampleList) {
+        s.list_v[mine] = v[k];
+        s.list_i[mine] = i + k;
+      }
+      at += __popcll(mask[k]);
+    }
+  }
+}
+
+// The prefix of the order that a filter leaves: words above v, and those with it up to index i.
+struct Cut {
+  float v;
+  int i;
+  __device__ __forceinline__ bool keeps(float x, int at) const { return x > v || (x == v && at <= i); }
+};
+
+__device__ __forceinline__ u64 wave_total(u64 v) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const uint32_t lo = __shfl_xor(static_cast<int>(v), d), hi = __shfl_xor(static_cast<int>(v >> 32), d);
+    v += (static_cast<u64>(hi) << 32) | lo;
+  }
+  return v;
+}
+__device__ __forceinline__ u64 block_total(SampleShared& s, u64 v) {
+  v = wave_total(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) s.wave[threadIdx.x >> 6] = v;
+  __syncthreads();
+  u64 t = 0;
+#pragma unroll
+  for (int i = 0; i < kSampleWaves; ++i) t += s.wave[i];
+  return t;
+}
+
+__device__ __forceinline__ u64 reach_of(float top_p, u64 total) {  // the sum at which top-p's prefix ends
+  const double want = __builtin_ceil((top_p > 0.f ? static_cast<double>(top_p) : 0.0) * static_cast<double>(total));
+  const u64 t = want < 1.0 ? 1 : static_cast<u64>(want);
+  return t > total ? total : t;
+}
+// u of `total` as an integer below it; a number outside [0, 1) takes the nearest end.
+__device__ __forceinline__ u64 draw_of(double u, u64 total) {
+  const u64 at = u >= 1.0 ? total - 1 : u > 0.0 ? static_cast<u64>(u * static_cast<double>(total)) : 0;
+  return at >= total ? total - 1 : at;
+}
+
+// The token, or -1 where a bin holds too many words to look at one by one.
+template <typename words_t>
+__device__ __forceinline__ int draw_by_bins(SampleShared& s, const words_t& words, const float (&most)[3], float m, float temperature,
+                                            float c, int top_k, float top_p, float min_p, double u) {
+  const int vocab = words.row.vocab;
+  FastWeight weight;
+  weight.m = m;
+  weight.c = c;
+  weight.c_lo = static_cast<float>(1.4426950408889634 / static_cast<double>(temperature) - static_cast<double>(c));
+  weight.least = -64.f / c;
+  const auto fixed = [&](float v) { return biased_fixed(weight(v)) - kFixedBias; };
+  const bool by_k = top_k > 0 && top_k < vocab, by_p = top_p < 1.f, by_m = min_p > 0.f;
+  // Words below `least` weigh nothing. (At a high temperature that is far below them all.)
+  float least = m - 46.f / c;
+  if (c < 0.25f) {
+    float mine = m;
+    words.each([&](const float (&v)[8], int, int, auto) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) mine = fminf(mine, v[k] > -__builtin_inff() ? v[k] : mine);
+    });
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) mine = fminf(mine, __shfl_xor(mine, d));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s.wave[threadIdx.x >> 6] = __float_as_uint(mine);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kSampleWaves; ++i) mine = fminf(mine, __uint_as_float(static_cast<uint32_t>(s.wave[i])));
+    least = fmaxf(least, mine);
+  }
+  const float m_bound = by_m ? fmaxf(least, m + (__builtin_amdgcn_logf(min_p) - 0.01f) / c) : least;  // just below min-p's
+
+  // The list of the words that matter, where there is a bound for them: the bin that the k-th
+  // largest of the groups' largest logits lies in. (Top-p counts all of top-k's words, also those
+  // below min-p.) Where top-p counts the whole row, its sum is taken in the same pass, and the
+  // bound is a guess at its prefix: one that a share of the words reaches which grows with top_p.
+  const ByLogit order(m, least);
+  const int groups = min(kSampleGroups, (vocab + 7) / 8);
+  const bool listed = by_k ? top_k <= kSampleGroups * 15 / 16 : by_m || by_p, whole = listed && by_p && !by_k;
+  int n = kSampleList + 1;
+  float low = m_bound;
+  u64 all = 0;
+  Cut cut{-__builtin_inff(), 0x7fffffff};
+  if (listed) {
+    if (threadIdx.x == 0) s.list_n = 0;
+    if (by_k || by_p) {
+      clear_bins(s);
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+        if (most[q] >= least) atomicAdd(reinterpret_cast<uint32_t*>(&s.mass[order.bin(most[q], 0)]), 1u);
+      const float share = top_p <= 0.6f ? 0.005f : top_p <= 0.85f ? 0.02f : top_p <= 0.92f ? 0.05f : 0.1f;
+      const float guess = fminf(share * vocab, kSampleList * 0.85f) / groups;  // words a group
+      const int k = by_k ? top_k : max(1, static_cast<int>(groups * (1.f - __builtin_amdgcn_exp2f(-guess / kLn2))));
+      uint32_t bin;
+      u64 before;
+      reach_bin(s, k, bin, before);
+      low = bin < kSampleBins && order.scale > 0.f ? m - (bin + 1.01f) / order.scale : least;
+      low = fmaxf(low, by_k && by_p ? least : m_bound);
+    }
+    __syncthreads();
+    words.each([&](const float (&v)[8], int i, int, auto) {
+      append(s, v, i, [&](float x, int) { return x >= low; });
+      if (whole) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) all += biased_fixed(weight(v[k]));
+        all -= 8 * kFixedBias;
+      }
+    });
+    __syncthreads();
+    n = s.list_n;
+    if (whole) all = block_total(s, all);
+  }
+  if (n <= kSampleFew) {  // all in one: a word a thread, its place and the weight before it by looking at every other
+    const int t = threadIdx.x;
+    SampleShared::Entry mine{0, 0.f, 0};
+    if (t < n) s.small[t] = mine = SampleShared::Entry{fixed(s.list_v[t]), s.list_v[t], s.list_i[t]};
+    __syncthreads();
+    int rank = 0;
+    u64 before = 0;
+    if (t < n) {
+#pragma unroll 4
+      for (int k = 0; k < n; ++k) {
+        const SampleShared::Entry o = s.small[k];
+        const bool first = ByLogit::before(o.v, o.i, mine.v, mine.i);
+        rank += first ? 1 : 0;
+        before += first ? o.w : 0;
+      }
+    }
+    bool keep = t < n && (!by_k || rank < top_k), found = true;
+    if (by_p) {
+      const u64 here = block_total(s, keep ? mine.w : 0), target = reach_of(top_p, whole ? all : here);
+      keep = keep && before < target;
+      found = target <= here || (by_m && low == m_bound);
+    }
+    if (found) {
+      keep = keep && !(weight(mine.v) < min_p);
+      const u64 at = draw_of(u, block_total(s, keep ? mine.w : 0));
+      if (t < n) s.small[t].w = keep ? mine.w : 0;
+      __syncthreads();
+      if (keep) {
+        u64 run = 0;
+#pragma unroll 4
+        for (int k = 0; k < n; ++k) {
+          const SampleShared::Entry o = s.small[k];
+          run += o.i < mine.i ? o.w : 0;
+        }
+        if (run <= at && at < run + mine.w) s.picked = mine.i;
+      }
+      __syncthreads();
+      return s.picked;
+    }
+    __syncthreads();
+  }
+  if (n > kSampleFew && n <= kSampleList) {
+    const ByLogit order(m, low);
+    const auto kept = [&](int e) { return cut.keeps(s.list_v[e], s.list_i[e]) ? fixed(s.list_v[e]) : 0; };
+    const auto sum = [&](const auto& weight_of) {
+      u64 mine = 0;
+      for (int e = threadIdx.x; e < n; e += kSampleThreads) mine += weight_of(e);
+      return block_total(s, mine);
+    };
+    if (by_k && n > top_k) {
+      if (!pick(s, n, order, [](int) -> u64 { return 1; }, top_k, cut.v, cut.i)) return -1;
+    }
+    bool found = true;
+    if (by_p) {
+      const u64 here = sum(kept), target = reach_of(top_p, whole ? all : here);
+      if (target <= here) {
+        Cut to{0.f, 0};
+        if (!pick(s, n, order, kept, target, to.v, to.i)) return -1;
+        cut = to;
+      } else {
+        found = by_m && low == m_bound;  // all of min-p's words are here, and top-p leaves more
+      }
+    }
+    if (found) {
+      const auto drawn = [&](int e) -> u64 {
+        const float w = weight(s.list_v[e]);
+        return cut.keeps(s.list_v[e], s.list_i[e]) && !(w < min_p) ? biased_fixed(w) - kFixedBias : 0;
+      };
+      float v;
+      int i;
+      return pick(s, n, ByIndex(vocab), drawn, draw_of(u, sum(drawn)) + 1, v, i) ? i : -1;
+    }
+  }
+
+  // No list: the cuts from bins of the whole row.
+  const auto gather = [&](uint32_t bin) {  // the words of a bin that the cut keeps
+    if (threadIdx.x == 0) s.list_n = 0;
+    __syncthreads();
+    words.each([&](const float (&v)[8], int i, int, auto) {
+      append(s, v, i, [&](float x, int at) { return x >= least && order.bin(x, 0) == bin && cut.keeps(x, at); });
+    });
+    __syncthreads();
+    return s.list_n;
+  };
+  if (by_k) {
+    clear_bins(s);
+    words.each([&](const float (&v)[8], int, int, auto) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (v[k] >= least) atomicAdd(reinterpret_cast<uint32_t*>(&s.mass[order.bin(v[k], 0)]), 1u);
+    });
+    uint32_t bin;
+    u64 before;
+    reach_bin(s, top_k, bin, before);
+    if (bin < kSampleBins) {  // else top-k's words include all that weigh anything
+      const int g = gather(bin);
+      if (g > kSampleList) return -1;
+      if (!pick(s, g, order, [](int) -> u64 { return 1; }, top_k - before, cut.v, cut.i)) return -1;
+    }
+  }
+  if (by_p) {
+    if (!whole) {
+      words.each([&](const float (&v)[8], int i, int, auto) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (cut.keeps(v[k], i + k)) all += fixed(v[k]);
+      });
+      all = block_total(s, all);
+    }
+    const u64 target = reach_of(top_p, all);
+    // Words that weigh less than the mass past the target shared among all cannot be the last of
+    // the prefix: they need no bin.
+    const float least_w = static_cast<float>(static_cast<double>(all - target) / kFixed / vocab) * 0.999f;
+    const float floor_v = fmaxf(least, m + (__builtin_amdgcn_logf(least_w) - 0.01f) / c);
+    clear_bins(s);
+    words.each([&](const float (&v)[8], int i, int, auto) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (v[k] >= floor_v && cut.keeps(v[k], i + k)) {
+          const u64 w = fixed(v[k]);
+          if (w) atomicAdd(&s.mass[order.bin(v[k], 0)], w);
+        }
+    });
+    uint32_t bin;
+    u64 before;
+    reach_bin(s, target, bin, before);
+    if (bin >= kSampleBins) return -1;
+    const int g = gather(bin);
+    if (g > kSampleList) return -1;
+    if (!pick(s, g, order, [&](int e) { return fixed(s.list_v[e]); }, target - before, cut.v, cut.i)) return -1;
+  }
+
+  // The draw: the words left by segments of 512 in index order, and one of them.
+  const auto left = [&](float v, int i) -> u64 {
+    const float w = weight(v);
+    return cut.keeps(v, i) && !(w < min_p) ? biased_fixed(w) - kFixedBias : 0;
+  };
+  const bool filtered = by_k || by_p || by_m;
+  u64 mine = 0;
+  words.each([&](const float (&v)[8], int i, int c, auto) {
+    u64 w = 0;
+    if (filtered) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w += left(v[k], i + k);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w += biased_fixed(weight(v[k]));
+      w -= 8 * kFixedBias;
+    }
+    mine += w;
+    w = wave_total(w);
+    if ((threadIdx.x & 63) == 0) s.seg[c * kSampleWaves + (threadIdx.x >> 6)] = w;
+  });
+  const u64 at = draw_of(u, block_total(s, mine));
+  if (threadIdx.x < 64) {
+    // the segment, 64 at a time, then its word
+    u64 before = 0;
+    int g = 0;
+    while (g < words_segments(vocab)) {
+      const u64 in = wave_incl(g + static_cast<int>(threadIdx.x) < words_segments(vocab) ? s.seg[g + threadIdx.x] : 0);
+      const u64 hit = __ballot(before + in > at);
+      if (hit) {
+        const int lane = __ffsll(static_cast<long long>(hit)) - 1;
+        g += lane;
+        before += lane ? shfl64(in, lane - 1) : 0;
+        break;
+      }
+      before += shfl64(in, 63);
+      g += 64;
+    }
+    const int i = g * 512 + threadIdx.x * 8;
+    float v[8];
+    words.row.load8(i, v);
+    u64 w[8], sum = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum += w[k] = left(v[k], i + k);
+    u64 run = before + wave_incl(sum) - sum;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (run <= at && at < run + w[k]) s.index = i + k;
+      run += w[k];
+    }
+  }
+  __syncthreads();
+  return s.index;
+}
+
+template <typename io_t, bool kVec, bool kReg>
+__global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleParams p) {
+  __shared__ SampleShared s;
+  const long long r = blockIdx.x;
+  Words<io_t, kVec, kReg> words;
+  words.row = Row<io_t, kVec>{static_cast<const io_t*>(p.logits) + r * p.sr, p.sv, p.vocab};
+  words.start();
+  const float temperature = p.temperatures ? p.temperatures[r] : p.temperature;
+  const int top_k = p.top_ks ? p.top_ks[r] : p.top_k;
+  const float top_p = p.top_ps ? p.top_ps[r] : p.top_p;
+  const float min_p = p.min_ps ? p.min_ps[r] : p.min_p;
+  const double u = static_cast<double>(p.uniform[r]);
+
+  // The largest logit of each group, and whether any is NaN.
+  float most[3] = {-__builtin_inff(), -__builtin_inff(), -__builtin_inff()};
+  bool nan = false;
+  words.each([&](const float (&v)[8], int, int, auto third) {
+    float& mine = most[decltype(third)::value];
+#pragma unroll
+    for (int k = 0; k < 8; k += 2) {
+      mine = fmaxf(fmaxf(mine, v[k]), v[k + 1]);
+      nan |= __builtin_isunordered(v[k], v[k + 1]);
+    }
+  });
+  const uint32_t my_top = nan ? 0xffffffffu : order_key(fmaxf(fmaxf(most[0], most[1]), most[2]));
+  uint32_t top = my_top;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d)));
+  if ((threadIdx.x & 63) == 0) s.wave[threadIdx.x >> 6] = top;
+  if (threadIdx.x == 0) s.index = 0x7fffffff;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kSampleWaves; ++i) top = max(top, static_cast<uint32_t>(s.wave[i]));
+  if (top == 0xffffffffu || top <= kAbsent) {
+    if (threadIdx.x == 0) p.tokens[r] = -1;
+    return;
+  }
+  if (!(temperature > 0.f) || top_k == 1 || min_p > 1.f) {  // the first word of the order
+    if (my_top == top) {
+      words.each([&](const float (&v)[8], int i, int, auto) {
+        int first = 0x7fffffff;
+#pragma unroll
+        for (int k = 7; k >= 0; --k)
+          if (order_key(v[k]) == top) first = i + k;
+        if (first != 0x7fffffff) atomicMin(&s.index, first);
+      });
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) p.tokens[r] = s.index;
+    return;
+  }
+  const float m = key_value(top), c = 1.442695041f / temperature;
+  if (m < __builtin_inff() && c > 0x1p-100f && c < 0x1p100f && m - 46.f / c > -__builtin_inff()) {
+    const int token = draw_by_bins(s, words, most, m, temperature, c, top_k, top_p, min_p, u);
+    if (token >= 0) {
+      if (threadIdx.x == 0) p.tokens[r] = token;
+      return;
+    }
+    __syncthreads();
+  }
+  draw_by_radix(s, words.row, top, temperature, top_k, top_p, min_p, u, p.tokens + r);
+}
+
 template <typename io_t>
 static void launch_sample_as(const SampleParams& p, hipStream_t stream) {
-  // 16-byte loads where a row's words are contiguous and it starts on 16 bytes.
-  const bool vec = p.sv == 1 && (reinterpret_cast<uintptr_t>(p.logits) & 15) == 0 &&
-                   (p.sr * static_cast<long long>(sizeof(io_t))) % 16 == 0;
-  if (vec) hipLaunchKernelGGL((sample_kernel<io_t, true>), dim3(p.rows), dim3(kSampleThreads), 0, stream, p);
-  else hipLaunchKernelGGL((sample_kernel<io_t, false>), dim3(p.rows), dim3(kSampleThreads), 0, stream, p);
+  const dim3 grid(p.rows), block(kSampleThreads);
+  if (p.sv == 1 && p.vocab <= kSampleRegVocab) hipLaunchKernelGGL((sample_kernel<io_t, true, true>), grid, block, 0, stream, p);
+  else if (p.sv == 1) hipLaunchKernelGGL((sample_kernel<io_t, true, false>), grid, block, 0, stream, p);
+  else if (p.vocab <= kSampleRegVocab) hipLaunchKernelGGL((sample_kernel<io_t, false, true>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((sample_kernel<io_t, false, false>), grid, block, 0, stream, p);
 }
 
 hipError_t launch_sample(const SampleParams& p, bool io_bf16, hipStream_t stream) {
