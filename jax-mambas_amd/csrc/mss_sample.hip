@@ -104,24 +104,43 @@ struct Weight {
 };
 __device__ __forceinline__ u64 fixed(float w) { return static_cast<u64>(__builtin_fmaf(w, kFixed, 0.5f)); }
 
-__device__ __forceinline__ u64 shfl_up64(u64 v, int d) {
-  const uint32_t lo = __shfl_up(static_cast<int>(v), d), hi = __shfl_up(static_cast<int>(v >> 32), d);
+// Cross-lane sums by DPP moves: a few clocks each, where a shuffle through LDS takes over a hundred.
+template <int kCtrl, int kRowMask>
+__device__ __forceinline__ u64 dpp64(u64 v) {  // lanes without a source get 0
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), kCtrl, kRowMask, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), kCtrl, kRowMask, 0xF, false);
   return (static_cast<u64>(hi) << 32) | lo;
 }
-__device__ __forceinline__ u64 shfl64(u64 v, int lane) {
-  const uint32_t lo = __shfl(static_cast<int>(v), lane), hi = __shfl(static_cast<int>(v >> 32), lane);
+__device__ __forceinline__ u64 readlane64(u64 v, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), lane);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane);
   return (static_cast<u64>(hi) << 32) | lo;
+}
+__device__ __forceinline__ u64 wave_incl(u64 v) {
+  v += dpp64<kRowShr1, 0xF>(v);
+  v += dpp64<kRowShr2, 0xF>(v);
+  v += dpp64<kRowShr4, 0xF>(v);
+  v += dpp64<kRowShr8, 0xF>(v);
+  v += dpp64<kRowBcast15, 0xA>(v);
+  v += dpp64<kRowBcast31, 0xC>(v);
+  return v;
+}
+__device__ __forceinline__ u64 wave_total(u64 v) { return readlane64(wave_incl(v), 63); }
+template <int kCtrl, int kRowMask>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+  return max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), kCtrl, kRowMask, 0xF, false)));
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+  v = dpp_max<kRowShr1, 0xF>(v);
+  v = dpp_max<kRowShr2, 0xF>(v);
+  v = dpp_max<kRowShr4, 0xF>(v);
+  v = dpp_max<kRowShr8, 0xF>(v);
+  v = dpp_max<kRowBcast15, 0xA>(v);
+  v = dpp_max<kRowBcast31, 0xC>(v);
+  return __builtin_amdgcn_readlane(static_cast<int>(v), 63);
 }
 __device__ __forceinline__ int words_segments(int vocab) {  // segments that a pass over the row writes
   return (vocab + kSampleChunk - 1) / kSampleChunk * kSampleWaves;
-}
-__device__ __forceinline__ u64 wave_incl(u64 v) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const u64 o = shfl_up64(v, d);
-    if ((threadIdx.x & 63) >= static_cast<unsigned>(d)) v += o;
-  }
-  return v;
 }
 
 struct SampleShared {
@@ -194,6 +213,19 @@ struct Words {
 #pragma unroll
       for (int c = 0; c < 8; ++c)
         if (c * kSampleChunk < row.vocab) row.load8(c * kSampleChunk + threadIdx.x * 8, held[c]);
+    }
+  }
+  template <typename F>
+  __device__ __forceinline__ void chunk(int at, const F& f) const {  // one chunk (the same for a wave)
+    const int i = threadIdx.x * 8;
+    if constexpr (kReg) {
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (c == at) f(held[c], c * kSampleChunk + i);
+    } else {
+      float v[8];
+      row.load8(at * kSampleChunk + i, v);
+      f(v, at * kSampleChunk + i);
     }
   }
   template <typename F>
@@ -523,14 +555,6 @@ struct Cut {
   __device__ __forceinline__ bool keeps(float x, int at) const { return x > v || (x == v && at <= i); }
 };
 
-__device__ __forceinline__ u64 wave_total(u64 v) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const uint32_t lo = __shfl_xor(static_cast<int>(v), d), hi = __shfl_xor(static_cast<int>(v >> 32), d);
-    v += (static_cast<u64>(hi) << 32) | lo;
-  }
-  return v;
-}
 __device__ __forceinline__ u64 block_total(SampleShared& s, u64 v) {
   v = wave_total(v);
   __syncthreads();
@@ -561,7 +585,8 @@ __device__ __forceinline__ int draw_by_bins(SampleShared& s, const words_t& word
   FastWeight weight;
   weight.m = m;
   weight.c = c;
-  weight.c_lo = static_cast<float>(1.4426950408889634 / static_cast<double>(temperature) - static_cast<double>(c));
+  // what c = log2(e) / temperature lacks (log2(e) = 1.442695022 + 1.92596e-8)
+  weight.c_lo = (__builtin_fmaf(-c, temperature, 1.442695022f) + 1.92596301e-8f) / temperature;
   weight.least = -64.f / c;
   const auto fixed = [&](float v) { return biased_fixed(weight(v)) - kFixedBias; };
   const bool by_k = top_k > 0 && top_k < vocab, by_p = top_p < 1.f, by_m = min_p > 0.f;
@@ -573,14 +598,13 @@ __device__ __forceinline__ int draw_by_bins(SampleShared& s, const words_t& word
 #pragma unroll
       for (int k = 0; k < 8; ++k) mine = fminf(mine, v[k] > -__builtin_inff() ? v[k] : mine);
     });
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) mine = fminf(mine, __shfl_xor(mine, d));
+    uint32_t last = wave_max(~order_key(mine));
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) s.wave[threadIdx.x >> 6] = __float_as_uint(mine);
+    if ((threadIdx.x & 63) == 0) s.wave[threadIdx.x >> 6] = last;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kSampleWaves; ++i) mine = fminf(mine, __uint_as_float(static_cast<uint32_t>(s.wave[i])));
-    least = fmaxf(least, mine);
+    for (int i = 0; i < kSampleWaves; ++i) last = max(last, static_cast<uint32_t>(s.wave[i]));
+    least = fmaxf(least, key_value(~last));
   }
   const float m_bound = by_m ? fmaxf(least, m + (__builtin_amdgcn_logf(min_p) - 0.01f) / c) : least;  // just below min-p's
 
@@ -778,34 +802,34 @@ __device__ __forceinline__ int draw_by_bins(SampleShared& s, const words_t& word
     if ((threadIdx.x & 63) == 0) s.seg[c * kSampleWaves + (threadIdx.x >> 6)] = w;
   });
   const u64 at = draw_of(u, block_total(s, mine));
-  if (threadIdx.x < 64) {
-    // the segment, 64 at a time, then its word
-    u64 before = 0;
-    int g = 0;
-    while (g < words_segments(vocab)) {
-      const u64 in = wave_incl(g + static_cast<int>(threadIdx.x) < words_segments(vocab) ? s.seg[g + threadIdx.x] : 0);
-      const u64 hit = __ballot(before + in > at);
-      if (hit) {
-        const int lane = __ffsll(static_cast<long long>(hit)) - 1;
-        g += lane;
-        before += lane ? shfl64(in, lane - 1) : 0;
-        break;
+  // Every wave finds the segment, 64 at a time, and the one that holds it the word.
+  u64 before = 0;
+  int g = 0;
+  while (g < words_segments(vocab)) {
+    const int lane = threadIdx.x & 63;
+    const u64 in = wave_incl(g + lane < words_segments(vocab) ? s.seg[g + lane] : 0);
+    const u64 hit = __ballot(before + in > at);
+    if (hit) {
+      const int first = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<long long>(hit)) - 1);
+      g += first;
+      if (first) before += readlane64(in, first - 1);
+      break;
+    }
+    before += readlane64(in, 63);
+    g += 64;
+  }
+  if (g % kSampleWaves == __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6))) {
+    words.chunk(g / kSampleWaves, [&](const float (&v)[8], int i) {
+      u64 w[8], sum = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum += w[k] = left(v[k], i + k);
+      u64 run = before + wave_incl(sum) - sum;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (run <= at && at < run + w[k]) s.index = i + k;
+        run += w[k];
       }
-      before += shfl64(in, 63);
-      g += 64;
-    }
-    const int i = g * 512 + threadIdx.x * 8;
-    float v[8];
-    words.row.load8(i, v);
-    u64 w[8], sum = 0;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) sum += w[k] = left(v[k], i + k);
-    u64 run = before + wave_incl(sum) - sum;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if (run <= at && at < run + w[k]) s.index = i + k;
-      run += w[k];
-    }
+    });
   }
   __syncthreads();
   return s.index;
@@ -837,8 +861,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleParams p) 
   });
   const uint32_t my_top = nan ? 0xffffffffu : order_key(fmaxf(fmaxf(most[0], most[1]), most[2]));
   uint32_t top = my_top;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d)));
+  top = wave_max(top);
   if ((threadIdx.x & 63) == 0) s.wave[threadIdx.x >> 6] = top;
   if (threadIdx.x == 0) s.index = 0x7fffffff;
   __syncthreads();
@@ -862,7 +885,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleParams p) 
     if (threadIdx.x == 0) p.tokens[r] = s.index;
     return;
   }
-  const float m = key_value(top), c = 1.442695041f / temperature;
+  const float m = key_value(top), c = 1.442695022f / temperature;
   if (m < __builtin_inff() && c > 0x1p-100f && c < 0x1p100f && m - 46.f / c > -__builtin_inff()) {
     const int token = draw_by_bins(s, words, most, m, temperature, c, top_k, top_p, min_p, u);
     if (token >= 0) {
