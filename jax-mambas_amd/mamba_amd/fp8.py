@@ -36,6 +36,8 @@ __all__ = ["quantize_fp8", "add_rmsnorm_fp8", "quantize_fp8_weight", "fp8_matmul
 
 _BLOCK = _lib.MSS_FP8_BLOCK
 FP8 = torch.float8_e4m3fn
+_F32 = torch.float32
+_TAGS = {torch.float32: _lib.MSS_F32, torch.bfloat16: _lib.MSS_BF16}
 
 
 def _blocks(n):
@@ -45,116 +47,135 @@ def _blocks(n):
 def _empty_rows(rows, cols, device):
     """An uninitialised (rows, cols) 8-bit matrix whose rows start on 16 bytes."""
     if cols % 16 == 0:
-        return torch.empty((rows, cols), dtype=FP8, device=device)
-    return torch.empty((rows, -(-cols // 16) * 16), dtype=FP8, device=device)[:, :cols]
+        return torch.empty(rows, cols, dtype=FP8, device=device)
+    return torch.empty(rows, -(-cols // 16) * 16, dtype=FP8, device=device)[:, :cols]
 
 
-def _row_stride(q, cols):
+def _row_stride(q, rows, cols):
     """The row stride of an 8-bit matrix (one that a single row may have, where it has one row)."""
-    return q.stride(0) if q.shape[0] > 1 else -(-cols // 16) * 16
+    return q.stride(0) if rows > 1 else -(-cols // 16) * 16
 
 
-def _no_grad_needed(*tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+def _no_grad_needed(a, b=None, c=None):
+    if torch.is_grad_enabled() and (a.requires_grad or (b is not None and b.requires_grad)
+                                    or (c is not None and c.requires_grad)):
         raise RuntimeError("the 8-bit operators are for inference: call them under torch.no_grad()")
 
 
 def quantize_fp8(x):
-    if x.ndim != 2:
+    if x.dim() != 2:
         raise ValueError("x must be a (features, tokens) matrix")
-    io = _io_tag(x.dtype, "x")
+    io = _TAGS.get(x.dtype)
+    if io is None:
+        io = _io_tag(x.dtype, "x")  # raises
     _no_grad_needed(x)
     _require_gpu(x)
     f, t = x.shape
-    q = _empty_rows(t, f, x.device)
-    scales = torch.empty((_blocks(f), t), dtype=torch.float32, device=x.device)
+    dev = x.device
+    q = _empty_rows(t, f, dev)
+    scales = torch.empty(_blocks(f), t, dtype=_F32, device=dev)
     if f == 0 or t == 0:
         return q, scales
     sf, st = x.stride()
-    a = _lib.QuantFp8Args(features=f, tokens=t, io_dtype=io, stride_f=sf, stride_t=st, ldq=_row_stride(q, f),
-                          x=x.data_ptr(), q=q.data_ptr(), scales=scales.data_ptr())
-    lib = _lib.register_hip_kernel()
-    _lib.check(lib.mss_quant_fp8(a, _stream(x)), "mss_quant_fp8")
+    a = _lib.QuantFp8Args(f, t, io, sf, st, _row_stride(q, t, f), x.data_ptr(), q.data_ptr(), scales.data_ptr())
+    _lib.check(_lib.register_hip_kernel().mss_quant_fp8(a, _stream(x)), "mss_quant_fp8")
     return q, scales
 
 
 def add_rmsnorm_fp8(h, delta, weight, eps=1e-5):
-    if h.dtype != torch.float32 or h.ndim != 2:
+    if h.dtype != _F32 or h.dim() != 2:
         raise TypeError("h must be a float32 (features, tokens) matrix")
     f, t = h.shape
-    if weight.dtype != torch.float32 or tuple(weight.shape) != (f,):
+    if weight.dtype != _F32 or weight.dim() != 1 or weight.shape[0] != f:
         raise ValueError(f"weight must be float32 with shape ({f},)")
-    if delta is not None and delta.shape != h.shape:
-        raise ValueError("delta must have h's shape")
-    tag = _lib.MSS_F32 if delta is None else _io_tag(delta.dtype, "delta")
+    tag = _lib.MSS_F32
+    if delta is not None:
+        if delta.shape != h.shape:
+            raise ValueError("delta must have h's shape")
+        tag = _TAGS.get(delta.dtype)
+        if tag is None:
+            tag = _io_tag(delta.dtype, "delta")  # raises
     if f == 0:
         raise ValueError("h has no features")
     _no_grad_needed(h, delta, weight)
     _require_gpu(h, delta, weight)
     h, weight = h.contiguous(), weight.contiguous()
-    delta = None if delta is None else delta.contiguous()
-    q = _empty_rows(t, f, h.device)
-    scales = torch.empty((_blocks(f), t), dtype=torch.float32, device=h.device)
-    hn = h if delta is None else torch.empty_like(h)
+    dev = h.device
+    q = _empty_rows(t, f, dev)
+    scales = torch.empty(_blocks(f), t, dtype=_F32, device=dev)
+    hn = h
+    if delta is not None:
+        delta = delta.contiguous()
+        hn = torch.empty(f, t, dtype=_F32, device=dev)
     if t == 0:
         return hn, q, scales
-    a = _lib.NormFp8Args(features=f, tokens=t, delta_dtype=tag, eps=float(eps), ldq=_row_stride(q, f),
-                         h=h.data_ptr(), delta=_ptr(delta), weight=weight.data_ptr(), hn=hn.data_ptr(),
-                         q=q.data_ptr(), scales=scales.data_ptr())
-    lib = _lib.register_hip_kernel()
-    _lib.check(lib.mss_norm_fp8(a, _stream(h)), "mss_norm_fp8")
+    a = _lib.NormFp8Args(f, t, tag, eps, _row_stride(q, t, f), h.data_ptr(), _ptr(delta), weight.data_ptr(),
+                         hn.data_ptr(), q.data_ptr(), scales.data_ptr())
+    _lib.check(_lib.register_hip_kernel().mss_norm_fp8(a, _stream(h)), "mss_norm_fp8")
     return hn, q, scales
 
 
 def quantize_fp8_weight(w):
-    if w.ndim != 2 or (w.shape[1] > 1 and w.stride(1) != 1):
+    if w.dim() != 2 or (w.shape[1] > 1 and w.stride(1) != 1):
         raise ValueError("w must be a (M, K) matrix with contiguous rows")
     io = _io_tag(w.dtype, "w")
     _no_grad_needed(w)
     _require_gpu(w)
     m, k = w.shape
     q = _empty_rows(m, k, w.device)
-    scales = torch.empty((_blocks(m), _blocks(k)), dtype=torch.float32, device=w.device)
+    scales = torch.empty(_blocks(m), _blocks(k), dtype=_F32, device=w.device)
     if m == 0 or k == 0:
         return q, scales
-    a = _lib.QuantFp8WeightArgs(M=m, K=k, io_dtype=io, ldw=w.stride(0) if m > 1 else k, ldq=_row_stride(q, k),
-                                w=w.data_ptr(), q=q.data_ptr(), scales=scales.data_ptr())
-    lib = _lib.register_hip_kernel()
-    _lib.check(lib.mss_quant_fp8_weight(a, _stream(w)), "mss_quant_fp8_weight")
+    a = _lib.QuantFp8WeightArgs(m, k, io, w.stride(0) if m > 1 else k, _row_stride(q, m, k), w.data_ptr(),
+                                q.data_ptr(), scales.data_ptr())
+    _lib.check(_lib.register_hip_kernel().mss_quant_fp8_weight(a, _stream(w)), "mss_quant_fp8_weight")
     return q, scales
 
 
-def _check_rows(name, q, k=None):
-    if q.dtype != FP8 or q.ndim != 2:
+def _check_rows(name, q, k):
+    """Refuses what is not an 8-bit matrix of k columns in the layout the kernels read; its rows and
+    their stride."""
+    if q.dtype != FP8 or q.dim() != 2:
         raise TypeError(f"{name} must be a float8_e4m3fn matrix")
-    if k is not None and q.shape[1] != k:
-        raise ValueError(f"{name} must have {k} columns, got {q.shape[1]}")
     rows, cols = q.shape
-    if rows and cols and (cols > 1 and q.stride(1) != 1 or rows > 1 and q.stride(0) % 16 != 0 or q.data_ptr() % 16 != 0):
+    if cols != k:
+        raise ValueError(f"{name} must have {k} columns, got {cols}")
+    ld, step = q.stride()
+    if rows and cols and (cols > 1 and step != 1 or rows > 1 and ld % 16 != 0 or q.data_ptr() % 16 != 0):
         raise ValueError(f"{name} must have contiguous rows that start on 16 bytes")
+    return rows, ld if rows > 1 else -(-cols // 16) * 16
+
+
+def _check_scales(name, s, rows, cols):
+    if s.dtype != _F32 or s.shape != (rows, cols) or not s.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous float32 tensor of shape {(rows, cols)}")
 
 
 def fp8_matmul(wq, w_scales, xq, x_scales, out_dtype=torch.bfloat16, token_major=False, out=None):
-    _check_rows("wq", wq)
-    (m, k), t = wq.shape, xq.shape[0]
-    _check_rows("xq", xq, k)
-    for name, s, shape in (("w_scales", w_scales, (_blocks(m), _blocks(k))), ("x_scales", x_scales, (_blocks(k), t))):
-        if s.dtype != torch.float32 or tuple(s.shape) != shape or not s.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous float32 tensor of shape {shape}")
-    shape = (t, m) if token_major else (m, t)
-    if out is None:
-        out = torch.empty(shape, dtype=out_dtype, device=wq.device)
-    elif tuple(out.shape) != shape or out.dtype != out_dtype or (shape[1] > 1 and out.stride(1) != 1):
-        raise ValueError(f"out must be {out_dtype} of shape {shape} with contiguous rows")
-    tag = _io_tag(out_dtype, "out_dtype")
+    k = wq.shape[-1] if wq.dim() else 0
+    m, ldw = _check_rows("wq", wq, k)
+    t, ldx = _check_rows("xq", xq, k)
+    kb = -(-k // _BLOCK)
+    _check_scales("w_scales", w_scales, -(-m // _BLOCK), kb)
+    _check_scales("x_scales", x_scales, kb, t)
+    tag = _TAGS.get(out_dtype)
+    if tag is None:
+        tag = _io_tag(out_dtype, "out_dtype")  # raises
+    rows, cols = (t, m) if token_major else (m, t)
+    ldc = cols
+    if out is not None:
+        if out.shape != (rows, cols) or out.dtype != out_dtype or (cols > 1 and out.stride(1) != 1):
+            raise ValueError(f"out must be {out_dtype} of shape {(rows, cols)} with contiguous rows")
+        if rows > 1:
+            ldc = out.stride(0)
     _require_gpu(wq, w_scales, xq, x_scales, out)
+    if out is None:
+        out = torch.empty(rows, cols, dtype=out_dtype, device=wq.device)
     if m == 0 or t == 0:
         return out
     if k == 0:
         return out.zero_()
-    a = _lib.Fp8MmArgs(M=m, K=k, T=t, out_dtype=tag, token_major=int(bool(token_major)), ldw=_row_stride(wq, k),
-                       ldx=_row_stride(xq, k), ldc=out.stride(0) if shape[0] > 1 else shape[1], W=wq.data_ptr(),
-                       w_scales=w_scales.data_ptr(), X=xq.data_ptr(), x_scales=x_scales.data_ptr(), C=out.data_ptr())
-    lib = _lib.register_hip_kernel()
-    _lib.check(lib.mss_fp8_mm(a, _stream(wq)), "mss_fp8_mm")
+    a = _lib.Fp8MmArgs(m, k, t, tag, 1 if token_major else 0, ldw, ldx, ldc, wq.data_ptr(), w_scales.data_ptr(),
+                       xq.data_ptr(), x_scales.data_ptr(), out.data_ptr())
+    _lib.check(_lib.register_hip_kernel().mss_fp8_mm(a, _stream(wq)), "mss_fp8_mm")
     return out

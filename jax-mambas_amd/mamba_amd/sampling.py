@@ -28,10 +28,13 @@ from .selective_scan_hip import _io_tag, _ptr, _require_gpu, _stream
 __all__ = ["sample_tokens"]
 
 
+_F32, _I32, _I64 = torch.float32, torch.int32, torch.int64
+
+
 def _setting(name, v, rows, dtype, low, high):
     """(number, None) or (0, checked per-row tensor)."""
     if isinstance(v, torch.Tensor):
-        if v.dtype != dtype or tuple(v.shape) != (rows,):
+        if v.dtype != dtype or v.shape != (rows,):
             raise ValueError(f"{name} must be a number or a {dtype} tensor of shape ({rows},)")
         return 0, v.contiguous()
     if not low <= v <= high:  # a NaN too
@@ -40,28 +43,26 @@ def _setting(name, v, rows, dtype, low, high):
 
 
 def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
-    if logits.ndim != 2:
+    if logits.dim() != 2:
         raise ValueError("logits must be a (rows, vocab) matrix")
     io = _io_tag(logits.dtype, "logits")
     rows, vocab = logits.shape
     if vocab == 0:
         raise ValueError("logits have no words")
-    if uniform.dtype != torch.float32 or tuple(uniform.shape) != (rows,):
+    if uniform.dtype != _F32 or uniform.shape != (rows,):
         raise ValueError(f"uniform must be float32 with shape ({rows},)")
-    temperature, temperatures = _setting("temperature", temperature, rows, torch.float32, 0.0, math.inf)
-    top_k, top_ks = _setting("top_k", top_k, rows, torch.int32, 0, 2**31 - 1)
-    top_p, top_ps = _setting("top_p", top_p, rows, torch.float32, 0.0, 1.0)
-    min_p, min_ps = _setting("min_p", min_p, rows, torch.float32, 0.0, 1.0)
+    temperature, temperatures = _setting("temperature", temperature, rows, _F32, 0.0, math.inf)
+    top_k, top_ks = _setting("top_k", top_k, rows, _I32, 0, 2**31 - 1)
+    top_p, top_ps = _setting("top_p", top_p, rows, _F32, 0.0, 1.0)
+    min_p, min_ps = _setting("min_p", min_p, rows, _F32, 0.0, 1.0)
     _require_gpu(logits, uniform, temperatures, top_ks, top_ps, min_ps)
-    tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    tokens = torch.empty(rows, dtype=_I64, device=logits.device)
     if rows == 0:
         return tokens
     uniform = uniform.contiguous()
     sr, sv = logits.stride()
-    a = _lib.SampleArgs(rows=rows, vocab=vocab, io_dtype=io, top_k=top_k, temperature=temperature, top_p=top_p,
-                        min_p=min_p, stride_row=sr if rows > 1 else 0, stride_word=sv if vocab > 1 else 1,
-                        logits=logits.data_ptr(), uniform=uniform.data_ptr(), temperatures=_ptr(temperatures),
-                        top_ks=_ptr(top_ks), top_ps=_ptr(top_ps), min_ps=_ptr(min_ps), tokens=tokens.data_ptr())
-    lib = _lib.register_hip_kernel()
-    _lib.check(lib.mss_sample(a, _stream(logits)), "mss_sample")
+    a = _lib.SampleArgs(rows, vocab, io, top_k, temperature, top_p, min_p, sr if rows > 1 else 0,
+                        sv if vocab > 1 else 1, logits.data_ptr(), uniform.data_ptr(), _ptr(temperatures),
+                        _ptr(top_ks), _ptr(top_ps), _ptr(min_ps), tokens.data_ptr())
+    _lib.check(_lib.register_hip_kernel().mss_sample(a, _stream(logits)), "mss_sample")
     return tokens

@@ -61,7 +61,14 @@ def _strides(u, io_layout, B, bc_layout):
     return _lib.Strides(io_batch=io_b, io_dim=io_r, bc_batch=bc_b, bc_state=bc_r)
 
 
+# The current stream's handle without a Stream object around it (0.1 us against 2; a private name of
+# torch's, so only where this torch has it).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(t):
+    if _raw_stream is not None:
+        return _raw_stream(t.get_device())
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
