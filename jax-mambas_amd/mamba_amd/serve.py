@@ -1,0 +1,121 @@
+"""Serving a MambaLM with 8-bit projections: prompt, single tokens, and the draw of the next one.
+
+``Fp8LM(model)`` takes a ``mamba1.MambaLM`` (its blocks: mamba/mamba1.py:216-363) and holds its in-, gate- and
+out-projections and the tied head in the 8-bit form of ``mamba_amd.fp8``, written once from the
+float32 masters; the small S6 projections stay in bf16. Every norm writes the 8-bit operand of
+the product behind it (``add_rmsnorm_fp8``), the scan's output is quantised for the
+out-projection (``quantize_fp8``), and logits are float32.
+
+``prefill(tokens) -> (logits, caches)`` — tokens (B, L) int64, right-aligned; logits (B, vocab) of
+the last position, and each block's decode state.
+
+``step(token, caches) -> logits`` — token (B,) int64; caches update in place.
+
+``generate(tokens, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, graph=True) -> drawn`` —
+draws uniforms.shape[0] tokens a row after the prompt with ``sample_tokens``: uniforms (n, B)
+float32 in [0, 1), settings numbers or one a row; drawn (n, B) int64. With ``graph`` the decode
+step and its draw are captured once in a HIP graph and replayed.
+
+Weights that change afterwards are not seen until ``refresh()``. Inference only; there is no CPU path.
+"""
+from __future__ import annotations
+
+import torch
+import torch.nn.functional as F
+
+from .conv1d_hip import causal_conv1d_fn
+from .decode import causal_conv1d_update
+from .fp8 import add_rmsnorm_fp8, fp8_matmul, quantize_fp8, quantize_fp8_weight
+from .mamba1 import MambaLM, ShadowWeights
+from .sampling import sample_tokens
+from .selective_scan_hip import _require_gpu
+
+__all__ = ["Fp8LM"]
+
+
+class Fp8LM:
+    def __init__(self, model):
+        if not isinstance(model, MambaLM):
+            raise TypeError("model must be a MambaLM")
+        _require_gpu(model.embedding)
+        self.model = model
+        self._small = ShadowWeights([w for b in model.blocks for w in (b.s6.x_proj, b.s6.dt_proj)])
+        self.refresh()
+
+    @torch.no_grad()
+    def refresh(self):
+        """Writes the 8-bit and bf16 weights from the model's float32 ones."""
+        m = self.model
+        self.head = quantize_fp8_weight(m.embedding)
+        self.in_z = [quantize_fp8_weight(torch.cat([b.in_proj, b.z_proj])) for b in m.blocks]
+        self.out = [quantize_fp8_weight(b.out_proj) for b in m.blocks]
+        self.A = [a.contiguous() for a in m.a_matrices()]
+        self._small.refresh(torch.bfloat16)
+
+    def _logits(self, h, delta):
+        norm = self.model.final_norm
+        _, q, s = add_rmsnorm_fp8(h, delta, norm.weight, norm.eps)
+        return fp8_matmul(*self.head, q, s, out_dtype=torch.float32, token_major=True)
+
+    @torch.no_grad()
+    def prefill(self, tokens):
+        batch, length = tokens.shape
+        if length == 0:
+            raise ValueError("the prompt has no tokens")
+        h = self.model.embedding[tokens.reshape(-1)].t().contiguous()  # (d_model, B L)
+        delta, caches = None, []
+        for blk, in_z, out, A in zip(self.model.blocks, self.in_z, self.out, self.A):
+            h, q, s = add_rmsnorm_fp8(h, delta, blk.norm.weight, blk.norm.eps)
+            xz = fp8_matmul(*in_z, q, s)
+            di, k = blk.conv_weight.shape
+            rows = xz.view(2 * di, batch, length).permute(1, 0, 2)
+            xin, z = rows[:, :di], xz[di:]
+            u = causal_conv1d_fn(xin, blk.conv_weight, blk.conv_bias)
+            y = blk.s6(u.permute(1, 0, 2).reshape(di, batch * length), batch, z=z, weights=self._small)
+            tail = xin[:, :, max(0, length - (k - 1)):]
+            conv = F.pad(tail, (k - 1 - tail.shape[2], 0)).contiguous()
+            caches.append({"conv": conv, "ssm": blk.s6.last_state, "A": A})
+            blk.s6.last_state = None
+            delta = fp8_matmul(*out, *quantize_fp8(y))
+        last = slice(length - 1, None, length)
+        return self._logits(h[:, last].contiguous(), delta[:, last].contiguous()), caches
+
+    @torch.no_grad()
+    def step(self, token, caches):
+        h = self.model.embedding[token].t().contiguous()  # (d_model, B)
+        delta = None
+        for blk, in_z, out, cache in zip(self.model.blocks, self.in_z, self.out, caches):
+            h, q, s = add_rmsnorm_fp8(h, delta, blk.norm.weight, blk.norm.eps)
+            xz = fp8_matmul(*in_z, q, s)
+            di = blk.conv_weight.shape[0]
+            u = causal_conv1d_update(cache["conv"], xz[:di].t(), blk.conv_weight, blk.conv_bias).t()
+            y = blk.s6.step(u, xz[di:], cache["ssm"], self._small, cache["A"])
+            delta = fp8_matmul(*out, *quantize_fp8(y))
+        return self._logits(h, delta)
+
+    @torch.no_grad()
+    def generate(self, tokens, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, graph=True):
+        if uniforms.dim() != 2 or uniforms.shape[1] != tokens.shape[0]:
+            raise ValueError(f"uniforms must be (steps, {tokens.shape[0]})")
+        n = uniforms.shape[0]
+        drawn = torch.empty(n, tokens.shape[0], dtype=torch.int64, device=tokens.device)
+        if n == 0:
+            return drawn
+        settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        logits, caches = self.prefill(tokens)
+        drawn[0] = sample_tokens(logits, uniforms[0], **settings)
+        if n <= 2 or not graph:
+            for i in range(1, n):
+                drawn[i] = sample_tokens(self.step(drawn[i - 1], caches), uniforms[i], **settings)
+            return drawn
+        # The first step runs eagerly (its launches are what a capture needs warm), the rest as a graph.
+        drawn[1] = sample_tokens(self.step(drawn[0], caches), uniforms[1], **settings)
+        token, uniform = drawn[1].clone(), uniforms[2].clone()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            token.copy_(sample_tokens(self.step(token, caches), uniform, **settings))
+        for i in range(2, n):
+            uniform.copy_(uniforms[i])
+            g.replay()
+            drawn[i] = token
+        return drawn

@@ -1,0 +1,140 @@
+"""Serving a MambaLM with 8-bit projections (serve.Fp8LM): prompt, steps and draws together
+(mamba/mamba1.py:300-363 with 8-bit products).
+
+CPU: refusals. GPU: the pieces against the same calls made by hand (bit for bit), a step against
+a longer prompt, and the whole against the model in float32. An 8-bit operand differs from its
+value by at most 2^-4 of it, so a product of two, whose errors have random signs, by at most
+sqrt(2) 2^-4 of its size; the stream takes one such error from each of a block's two products
+and the logits one more: for two blocks 5 x 0.089 = 0.44 of the logits' size.
+"""
+import pytest
+import torch
+
+from mamba_amd.fp8 import add_rmsnorm_fp8, fp8_matmul, quantize_fp8, quantize_fp8_weight
+from mamba_amd.mamba1 import MambaLM
+from mamba_amd.sampling import sample_tokens
+from mamba_amd.serve import Fp8LM
+
+VOCAB, DIM, LAYERS = 1000, 192, 2
+
+
+def lm(seed=0, **kw):
+    torch.manual_seed(seed)
+    return MambaLM(VOCAB, DIM, LAYERS, device="cuda", **kw)
+
+
+def prompt(batch, length, seed=1):
+    return torch.randint(0, VOCAB, (batch, length), generator=torch.Generator().manual_seed(seed)).cuda()
+
+
+def test_refusals():
+    with pytest.raises(TypeError):
+        Fp8LM(torch.nn.Linear(2, 2))
+    with pytest.raises(RuntimeError):  # no CPU path
+        Fp8LM(MambaLM(10, 16, 1))
+
+
+@pytest.mark.gpu
+def test_gpu_refusals():
+    m = Fp8LM(lm())
+    with pytest.raises(ValueError):
+        m.prefill(prompt(2, 0))
+    with pytest.raises(ValueError):
+        m.generate(prompt(2, 4), torch.rand(5, 3, device="cuda"))
+    with pytest.raises(ValueError):
+        m.generate(prompt(2, 4), torch.rand(5, 2, device="cuda"), top_p=2.0)
+    assert m.generate(prompt(2, 4), torch.rand(0, 2, device="cuda")).shape == (0, 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,length", [(1, 1), (2, 2), (3, 37), (1, 300)])
+def test_prefill_is_close_to_float32(batch, length):
+    model = lm()
+    tokens = prompt(batch, length)
+    logits, caches = Fp8LM(model).prefill(tokens)
+    with torch.no_grad():
+        want = model(tokens, act_dtype=torch.float32).view(batch, length, -1)[:, -1]
+    assert logits.dtype == torch.float32 and logits.shape == (batch, VOCAB) and logits.is_contiguous()
+    assert len(caches) == LAYERS and caches[0]["ssm"].shape == (batch, 2 * DIM, 16)
+    err = float((logits - want).norm() / want.norm())
+    print("relative error", err, flush=True)
+    assert err < 0.44
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch", [1, 3, 8])
+def test_step_is_the_pieces_together(batch):
+    """One block's step by hand, and the logits, bit for bit."""
+    model = lm(2)
+    m = Fp8LM(model)
+    _, caches = m.prefill(prompt(batch, 9))
+    mine = [{k: v.clone() for k, v in c.items()} for c in caches]
+    token = prompt(batch, 1, seed=3)[:, 0]
+    got = m.step(token, caches)
+    from mamba_amd.decode import causal_conv1d_update
+
+    with torch.no_grad():
+        h, delta = model.embedding[token].t().contiguous(), None
+        for blk, c in zip(model.blocks, mine):
+            h, q, s = add_rmsnorm_fp8(h, delta, blk.norm.weight, blk.norm.eps)
+            xz = fp8_matmul(*quantize_fp8_weight(torch.cat([blk.in_proj, blk.z_proj])), q, s)
+            u = causal_conv1d_update(c["conv"], xz[:2 * DIM].t(), blk.conv_weight, blk.conv_bias).t()
+            y = blk.s6.step(u, xz[2 * DIM:], c["ssm"], m._small, c["A"])
+            delta = fp8_matmul(*quantize_fp8_weight(blk.out_proj), *quantize_fp8(y))
+        _, q, s = add_rmsnorm_fp8(h, delta, model.final_norm.weight, model.final_norm.eps)
+        want = fp8_matmul(*quantize_fp8_weight(model.embedding), q, s, out_dtype=torch.float32, token_major=True)
+    assert torch.equal(got, want)
+    for a, b in zip(caches, mine):
+        assert torch.equal(a["conv"], b["conv"]) and torch.equal(a["ssm"], b["ssm"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,length", [(2, 1), (2, 2), (3, 40)])
+def test_steps_follow_a_prompt(batch, length):
+    """Prompt then three steps against the whole as a prompt: the same function, up to roundings
+    to 8 bits that fall differently (as far apart as either may be from float32)."""
+    m = Fp8LM(lm(4))
+    tokens = prompt(batch, length + 3)
+    _, caches = m.prefill(tokens[:, :length])
+    for i in range(3):
+        logits = m.step(tokens[:, length + i], caches)
+    want, _ = m.prefill(tokens)
+    err = float((logits - want).norm() / want.norm())
+    print("relative error", err, flush=True)
+    assert err < 0.44
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(), dict(temperature=0.7, top_k=40, top_p=0.95), dict(temperature=0.0),
+                                dict(min_p=0.05, by_row=True)], ids=str)
+def test_generate(kw):
+    """Graph and eager runs give the same tokens, which are the draws made by hand."""
+    kw = dict(kw)
+    if kw.pop("by_row", False):
+        kw["temperature"] = torch.tensor([0.0, 0.8, 1.2], device="cuda")
+        kw["top_k"] = torch.tensor([0, 5, 900], dtype=torch.int32, device="cuda")
+    m = Fp8LM(lm(5))
+    tokens = prompt(3, 11)
+    uniforms = torch.rand(7, 3, generator=torch.Generator().manual_seed(6)).cuda()
+    eager = m.generate(tokens, uniforms, graph=False, **kw)
+    for _ in range(2):
+        assert torch.equal(m.generate(tokens, uniforms, **kw), eager)
+    logits, caches = m.prefill(tokens)
+    for i in range(7):
+        token = sample_tokens(logits, uniforms[i], **kw)
+        assert torch.equal(token, eager[i])
+        logits = m.step(token, caches)
+
+
+@pytest.mark.gpu
+def test_refresh_and_complex_states():
+    model = lm(7, complex_ssm=True)
+    m = Fp8LM(model)
+    tokens = prompt(2, 5)
+    before, caches = m.prefill(tokens)
+    assert torch.isfinite(m.step(tokens[:, 0], caches)).all()
+    with torch.no_grad():
+        model.blocks[0].out_proj.mul_(3.0)
+    assert torch.equal(m.prefill(tokens)[0], before)
+    m.refresh()
+    assert not torch.equal(m.prefill(tokens)[0], before)
