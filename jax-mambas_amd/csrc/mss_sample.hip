@@ -208,6 +208,7 @@ struct Third {
 };
 template <typename io_t, bool kVec, bool kReg>
 struct Words {
+  static constexpr bool kHeld = kReg;
   Row<io_t, kVec> row;
   float held[kReg ? 8 : 1][8];
   __device__ __forceinline__ void start() {
@@ -437,21 +438,22 @@ __device__ __forceinline__ void draw_by_radix(SampleShared& s, const row_t row, 
 // Zeroes the bins; ends with a barrier.
 __device__ __forceinline__ void clear_bins(SampleShared& s) {
   for (int i = threadIdx.x; i < kSampleBins; i += kSampleThreads) s.mass[i] = 0;
-  if (threadIdx.x == 0) {
-    s.small_n = 0;
-    s.found_bin = kSampleBins;
-  }
+  if (threadIdx.x == 0) s.found_bin = kSampleBins;
   __syncthreads();
 }
 
-// The first bin at which the running sum reaches `target` (at least 1): its number and the sum
-// before it; kSampleBins where the whole sum does not. Ends with a barrier.
-__device__ __forceinline__ void reach_bin(SampleShared& s, u64 target, uint32_t& bin, u64& before) {
+// The first bin at which the running sum reaches the target, which may depend on the whole sum
+// (at least 1): its number, the sum before it and the target; kSampleBins where the whole sum does
+// not reach it. Begins and ends with a barrier.
+template <typename target_t>
+__device__ __forceinline__ void reach_bin(SampleShared& s, const target_t& target_of, uint32_t& bin, u64& before,
+                                          u64& target) {
   __syncthreads();
   const int at = 2 * threadIdx.x;
   const u64 a = s.mass[at], b = s.mass[at + 1];
   u64 total;
   const u64 excl = block_excl(s, a + b, total);
+  target = target_of(total);
   if (excl < target && target <= excl + a + b) {
     const bool first = target <= excl + a;
     s.found_bin = first ? at : at + 1;
@@ -471,7 +473,7 @@ struct ByLogit {
     if (!(scale < 1e37f)) scale = 0.f;  // (a range too small to divide by: one bin)
   }
   __device__ __forceinline__ uint32_t bin(float v, int) const {
-    return static_cast<uint32_t>(fminf((m - v) * scale, static_cast<float>(kSampleBins - 1)));
+    return static_cast<uint32_t>(fminf((v - m) * -scale, static_cast<float>(kSampleBins - 1)));
   }
   static __device__ __forceinline__ bool before(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
 };
@@ -496,6 +498,7 @@ __device__ __forceinline__ void places(SampleShared& s, int n, const order_t& or
     const SampleShared::Entry mine = s.small[t];
     u64 sum = 0;
     uint32_t rank = 0;
+#pragma unroll 4
     for (int k = threadIdx.x >> 6; k < n; k += kSampleWaves) {
       const SampleShared::Entry o = s.small[k];
       const bool first = order.before(o.v, o.i, mine.v, mine.i);
@@ -510,19 +513,14 @@ __device__ __forceinline__ void places(SampleShared& s, int n, const order_t& or
   __syncthreads();
 }
 
-// Of the list's words, the one at which the running weight in `order` reaches `target`; false where
-// its bin holds too many. Every thread gets it.
+// Of the list's words in bin `bin` of `order`, the one at which the running weight reaches
+// `target`, `before` being the weight of the bins before; false where they are too many. Every
+// thread gets it.
 template <typename order_t, typename weight_t>
-__device__ __forceinline__ bool pick(SampleShared& s, int n, const order_t& order, const weight_t& weight, u64 target,
-                                     float& v, int& i) {
-  clear_bins(s);
-  for (int e = threadIdx.x; e < n; e += kSampleThreads) {
-    const u64 w = weight(e);
-    if (w) atomicAdd(&s.mass[order.bin(s.list_v[e], s.list_i[e])], w);
-  }
-  uint32_t bin;
-  u64 before;
-  reach_bin(s, target, bin, before);
+__device__ __forceinline__ bool settle(SampleShared& s, int n, const order_t& order, const weight_t& weight, uint32_t bin,
+                                       u64 before, u64 target, float& v, int& i) {
+  if (threadIdx.x == 0) s.small_n = 0;
+  __syncthreads();
   for (int e = threadIdx.x; e < n; e += kSampleThreads) {
     if (order.bin(s.list_v[e], s.list_i[e]) != bin) continue;
     const u64 w = weight(e);
@@ -544,6 +542,20 @@ __device__ __forceinline__ bool pick(SampleShared& s, int n, const order_t& orde
   i = s.small[s.picked].i;
   __syncthreads();
   return true;
+}
+// The same with bins filled from the list.
+template <typename order_t, typename weight_t, typename target_t>
+__device__ __forceinline__ bool pick(SampleShared& s, int n, const order_t& order, const weight_t& weight,
+                                     const target_t& target_of, float& v, int& i) {
+  clear_bins(s);
+  for (int e = threadIdx.x; e < n; e += kSampleThreads) {
+    const u64 w = weight(e);
+    if (w) atomicAdd(&s.mass[order.bin(s.list_v[e], s.list_i[e])], w);
+  }
+  uint32_t bin;
+  u64 before, target;
+  reach_bin(s, target_of, bin, before, target);
+  return settle(s, n, order, weight, bin, before, target, v, i);
 }
 
 // Puts those of a thread's 8 words into the list that `takes` says, a wave's at once: one atomic for
@@ -635,18 +647,23 @@ __device__ __forceinline__ int draw_by_bins(SampleShared& s, const words_t& word
 
   // The list of the words that matter, where there is a bound for them: the bin that the k-th
   // largest of the groups' largest logits lies in. (Top-p counts all of top-k's words, also those
-  // below min-p.) Where top-p counts the whole row, its sum is taken in the same pass, and the
-  // bound is a guess at its prefix: one that a share of the words reaches which grows with top_p.
+  // below min-p.) Where top-p counts the whole row, its sum is taken in the same pass, and
+  // without min-p the bound is a guess at its prefix: one that a share of the words reaches which
+  // grows with top_p. (Rows in registers need no guess: their bins are filled from the whole row.)
   const ByLogit order(m, least);
+  const auto low_of = [&](uint32_t bin) {  // a logit that all words of the bins up to it reach
+    return bin < kSampleBins && order.scale > 0.f ? fmaxf(least, m - (bin + 1.01f) / order.scale) : least;
+  };
   const int groups = min(kSampleGroups, (vocab + 7) / 8);
-  const bool listed = by_k ? top_k <= kSampleGroups * 15 / 16 : by_m || by_p, whole = listed && by_p && !by_k;
+  const bool listed = by_k ? top_k <= kSampleGroups * 15 / 16 : by_m || (by_p && !words_t::kHeld);
+  const bool whole = listed && by_p && !by_k;
   int n = kSampleList + 1;
   float low = m_bound;
   u64 all = 0;
   Cut cut{-__builtin_inff(), 0x7fffffff};
   if (listed) {
     if (threadIdx.x == 0) s.list_n = 0;
-    if (by_k || by_p) {
+    if (by_k || !by_m) {
       clear_bins(s);
 #pragma unroll
       for (int q = 0; q < 3; ++q)
@@ -655,10 +672,9 @@ __device__ __forceinline__ int draw_by_bins(SampleShared& s, const words_t& word
       const float guess = fminf(share * vocab, kSampleList * 0.85f) / groups;  // words a group
       const int k = by_k ? top_k : max(1, static_cast<int>(groups * (1.f - __builtin_amdgcn_exp2f(-guess / kLn2))));
       uint32_t bin;
-      u64 before;
-      reach_bin(s, k, bin, before);
-      low = bin < kSampleBins && order.scale > 0.f ? m - (bin + 1.01f) / order.scale : least;
-      low = fmaxf(low, by_k && by_p ? least : m_bound);
+      u64 before, target;
+      reach_bin(s, [&](u64) -> u64 { return k; }, bin, before, target);
+      low = fmaxf(low_of(bin), by_k && by_p ? least : m_bound);
     }
     __syncthreads();
     words.each([&](const float (&v)[8], int i, int, auto) {
@@ -697,49 +713,48 @@ __device__ __forceinline__ int draw_by_bins(SampleShared& s, const words_t& word
     }
     __syncthreads();
   }
+  const auto draw_listed = [&](int n) {  // among the list's words that the cut and min-p leave
+    const auto drawn = [&](int e) -> u64 {
+      const float w = weight(s.list_v[e]);
+      return cut.keeps(s.list_v[e], s.list_i[e]) && !(w < min_p) ? biased_fixed(w) - kFixedBias : 0;
+    };
+    float v;
+    int i;
+    return pick(s, n, ByIndex(vocab), drawn, [&](u64 total) { return draw_of(u, total) + 1; }, v, i) ? i : -1;
+  };
   if (n > kSampleFew && n <= kSampleList) {
     const ByLogit order(m, low);
     const auto kept = [&](int e) { return cut.keeps(s.list_v[e], s.list_i[e]) ? fixed(s.list_v[e]) : 0; };
-    const auto sum = [&](const auto& weight_of) {
-      u64 mine = 0;
-      for (int e = threadIdx.x; e < n; e += kSampleThreads) mine += weight_of(e);
-      return block_total(s, mine);
-    };
     if (by_k && n > top_k) {
-      if (!pick(s, n, order, [](int) -> u64 { return 1; }, top_k, cut.v, cut.i)) return -1;
+      if (!pick(s, n, order, [](int) -> u64 { return 1; }, [&](u64) -> u64 { return top_k; }, cut.v, cut.i)) return -1;
     }
     bool found = true;
     if (by_p) {
-      const u64 here = sum(kept), target = reach_of(top_p, whole ? all : here);
+      u64 mine = 0;
+      for (int e = threadIdx.x; e < n; e += kSampleThreads) mine += kept(e);
+      const u64 here = block_total(s, mine), target = reach_of(top_p, whole ? all : here);
       if (target <= here) {
         Cut to{0.f, 0};
-        if (!pick(s, n, order, kept, target, to.v, to.i)) return -1;
+        if (!pick(s, n, order, kept, [&](u64) { return target; }, to.v, to.i)) return -1;
         cut = to;
       } else {
         found = by_m && low == m_bound;  // all of min-p's words are here, and top-p leaves more
       }
     }
-    if (found) {
-      const auto drawn = [&](int e) -> u64 {
-        const float w = weight(s.list_v[e]);
-        return cut.keeps(s.list_v[e], s.list_i[e]) && !(w < min_p) ? biased_fixed(w) - kFixedBias : 0;
-      };
-      float v;
-      int i;
-      return pick(s, n, ByIndex(vocab), drawn, draw_of(u, sum(drawn)) + 1, v, i) ? i : -1;
-    }
+    if (found) return draw_listed(n);
   }
 
   // No list: the cuts from bins of the whole row.
-  const auto gather = [&](uint32_t bin) {  // the words of a bin that the cut keeps
+  const auto gather = [&](const auto& takes) {
     if (threadIdx.x == 0) s.list_n = 0;
     __syncthreads();
-    words.each([&](const float (&v)[8], int i, int, auto) {
-      append(s, v, i, [&](float x, int at) { return x >= least && order.bin(x, 0) == bin && cut.keeps(x, at); });
-    });
+    words.each([&](const float (&v)[8], int i, int, auto) { append(s, v, i, takes); });
     __syncthreads();
     return s.list_n;
   };
+  uint32_t bin;
+  u64 before, target;
+  const auto in_bin = [&](float x, int at) { return x >= least && order.bin(x, 0) == bin && cut.keeps(x, at); };
   if (by_k) {
     clear_bins(s);
     words.each([&](const float (&v)[8], int, int, auto) {
@@ -747,45 +762,35 @@ __device__ __forceinline__ int draw_by_bins(SampleShared& s, const words_t& word
       for (int k = 0; k < 8; ++k)
         if (v[k] >= least) atomicAdd(reinterpret_cast<uint32_t*>(&s.mass[order.bin(v[k], 0)]), 1u);
     });
-    uint32_t bin;
-    u64 before;
-    reach_bin(s, top_k, bin, before);
+    reach_bin(s, [&](u64) -> u64 { return top_k; }, bin, before, target);
     if (bin < kSampleBins) {  // else top-k's words include all that weigh anything
-      const int g = gather(bin);
-      if (g > kSampleList) return -1;
-      if (!pick(s, g, order, [](int) -> u64 { return 1; }, top_k - before, cut.v, cut.i)) return -1;
+      const int g = gather(in_bin);
+      if (g > kSampleList || !settle(s, g, order, [](int) -> u64 { return 1; }, bin, before, target, cut.v, cut.i)) return -1;
     }
   }
   if (by_p) {
-    if (!whole) {
-      words.each([&](const float (&v)[8], int i, int, auto) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (cut.keeps(v[k], i + k)) all += fixed(v[k]);
-      });
-      all = block_total(s, all);
-    }
-    const u64 target = reach_of(top_p, all);
-    // Words that weigh less than the mass past the target shared among all cannot be the last of
-    // the prefix: they need no bin.
-    const float least_w = static_cast<float>(static_cast<double>(all - target) / kFixed / vocab) * 0.999f;
-    const float floor_v = fmaxf(least, m + (__builtin_amdgcn_logf(least_w) - 0.01f) / c);
     clear_bins(s);
     words.each([&](const float (&v)[8], int i, int, auto) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (v[k] >= floor_v && cut.keeps(v[k], i + k)) {
-          const u64 w = fixed(v[k]);
-          if (w) atomicAdd(&s.mass[order.bin(v[k], 0)], w);
-        }
+      for (int k = 0; k < 8; ++k) {
+        const u64 w = !by_k || cut.keeps(v[k], i + k) ? fixed(v[k]) : 0;
+        if (w) atomicAdd(&s.mass[order.bin(v[k], 0)], w);
+      }
     });
-    uint32_t bin;
-    u64 before;
-    reach_bin(s, target, bin, before);
+    reach_bin(s, [&](u64 total) { return reach_of(top_p, total); }, bin, before, target);
     if (bin >= kSampleBins) return -1;
-    const int g = gather(bin);
-    if (g > kSampleList) return -1;
-    if (!pick(s, g, order, [&](int e) { return fixed(s.list_v[e]); }, target - before, cut.v, cut.i)) return -1;
+    const auto weigh = [&](int e) { return cut.keeps(s.list_v[e], s.list_i[e]) ? fixed(s.list_v[e]) : 0; };
+    const float reach = low_of(bin);
+    const int g = gather([&](float x, int) { return x >= reach; });
+    Cut to{0.f, 0};
+    if (g <= kSampleList) {  // the whole prefix fits the list: the draw is made there
+      if (!settle(s, g, order, weigh, bin, before, target, to.v, to.i)) return -1;
+      cut = to;
+      return draw_listed(g);
+    }
+    const int h = gather(in_bin);
+    if (h > kSampleList || !settle(s, h, order, weigh, bin, before, target, to.v, to.i)) return -1;
+    cut = to;
   }
 
   // The draw: the words left by segments of 512 in index order, and one of them.
@@ -811,7 +816,7 @@ __device__ __forceinline__ int draw_by_bins(SampleShared& s, const words_t& word
   });
   const u64 at = draw_of(u, block_total(s, mine));
   // Every wave finds the segment, 64 at a time, and the one that holds it the word.
-  u64 before = 0;
+  before = 0;
   int g = 0;
   while (g < words_segments(vocab)) {
     const int lane = threadIdx.x & 63;
