@@ -17,6 +17,8 @@
 // instructions, at half the rate; a bf16 output does so where that rate is not what bounds it.
 #include <hip/hip_runtime.h>
 
+#include <cmath>
+
 #include "mss_serve.h"
 
 namespace mss {
@@ -230,7 +232,7 @@ struct MmShape {
   static constexpr int kBR = kBR_, kBQ = kBQ_, kWR = kWR_, kWQ = kWQ_, kWaves = kWR * kWQ, kThreads = 64 * kWaves;
   static constexpr int kRT = kBR / kWR / 16, kQT = kBQ / kWQ / 16;  // 16 x 16 tiles of a wave
   static constexpr int kRCopies = kBR * 8 / kThreads, kQCopies = kBQ * 8 / kThreads;
-  static_assert(kRT % 4 == 0 && kBR / 64 <= kWaves && kBQ / 64 <= kWaves && kBR * 8 % kThreads == 0 &&
+  static_assert(kRT % 4 == 0 &&  kBR * 8 % kThreads == 0 &&
                 kBQ * 8 % kThreads == 0, "");
 };
 
@@ -246,8 +248,9 @@ template <typename S, bool kF8, typename out_t, bool kTokenRows>
 __global__ __launch_bounds__(S::kThreads, 2) void fp8mm_tile_kernel(Fp8MmParams p, int tiles_r, int tiles_q) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host's pass knows no buffer resources
   constexpr int kToks = kTokenRows ? S::kBR : S::kBQ;
-  __shared__ u32x4 sR0[S::kBR * 8], sQ0[S::kBQ * 8], sR1[S::kBR * 8], sQ1[S::kBQ * 8];
-  __shared__ alignas(16) float sS0[kToks], sS1[kToks];
+  // A stage: R's rows, Q's rows, the tokens' scales.
+  constexpr int kSlots = 8 * (S::kBR + S::kBQ) + kToks / 4;
+  __shared__ u32x4 s0[kSlots], s1[kSlots];
   const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wr = wave % S::kWR, wq = wave / S::kWR;
@@ -287,21 +290,21 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp8mm_tile_kernel(Fp8MmParams 
   };
   const auto bufR = rsrc(R, r0, p.K), bufQ = rsrc(Q, q0, p.K);
   const int t0 = kTokenRows ? r0 : q0;
-  const auto issue_scales = [&](int b, float* dS) {
-    if (wave < kToks / 64)
-      __builtin_amdgcn_global_load_lds((gbl_void_t)(p.xs + static_cast<long long>(b) * p.T + min(t0 + 64 * wave + lane, p.T - 1)),
-                                       (lds_void_t)(dS + 64 * wave), 4, 0, 0);
+  const auto issue_scales = [&](int b, u32x4* d) {  // by every wave, some of them the same ones
+    const int i = wave % ((kToks + 63) / 64);
+    __builtin_amdgcn_global_load_lds((gbl_void_t)(p.xs + static_cast<long long>(b) * p.T + min(t0 + 64 * i + lane, p.T - 1)),
+                                     (lds_void_t)(d + 8 * (S::kBR + S::kBQ) + 16 * i), 4, 0, 0);
   };
-  const auto issue = [&](int b, u32x4* dR, u32x4* dQ, float* dS) {
-    issue_scales(b, dS);
+  const auto issue = [&](int b, u32x4* d) {
+    issue_scales(b, d);
 #pragma unroll
     for (int t = 0; t < S::kRCopies; ++t)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(bufR, (lds_void_t)(dR + 64 * (wave + S::kWaves * t)), 16, off_r[t],
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(bufR, (lds_void_t)(d + 64 * (wave + S::kWaves * t)), 16, off_r[t],
                                                b * kFp8Block, 0, 0);
 #pragma unroll
     for (int t = 0; t < S::kQCopies; ++t)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(bufQ, (lds_void_t)(dQ + 64 * (wave + S::kWaves * t)), 16, off_q[t],
-                                               b * kFp8Block, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(bufQ, (lds_void_t)(d + 8 * S::kBR + 64 * (wave + S::kWaves * t)), 16,
+                                               off_q[t], b * kFp8Block, 0, 0);
   };
 
   // The wave's rows of W lie in one block.
@@ -324,7 +327,9 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp8mm_tile_kernel(Fp8MmParams 
   const int row_q = wq * (16 * S::kQT) + j, key_q = q_key(j);
   const int r_lo = row_r * 8 + (g ^ key_r), r_hi = row_r * 8 + ((g + 4) ^ key_r);
   const int q_lo = row_q * 8 + (g ^ key_q), q_hi = row_q * 8 + ((g + 4) ^ key_q);
-  const auto compute = [&](const u32x4* bR, const u32x4* bQ, const float* bS, float w) {
+  const auto compute = [&](const u32x4* bR, float w) {
+    const u32x4* bQ = bR + 8 * S::kBR;
+    const float* bS = reinterpret_cast<const float*>(bQ + 8 * S::kBQ);
     MmFrag<kF8> r[S::kRT];
     f32x4 sr[kTokenRows ? S::kRT : 1];
 #pragma unroll
@@ -371,42 +376,43 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp8mm_tile_kernel(Fp8MmParams 
     __builtin_amdgcn_s_setprio(0);
   };
 
-  const auto meet = [] {  // this wave's copies have landed and its reads are done; so have all waves'
+  const auto meet = [] {  // all waves' copies have landed and their reads are done
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0), the builtin so that the compiler knows too
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
   const int full = p.K / kFp8Block;
-  if (full > 0) issue(0, sR0, sQ0, sS0);
+  if (full > 0) issue(0, s0);
   for (int b = 0; b + 1 < full; b += 2) {
     meet();
-    issue(b + 1, sR1, sQ1, sS1);
-    compute(sR0, sQ0, sS0, ws[b]);
+    issue(b + 1, s1);
+    compute(s0, ws[b]);
     meet();
-    if (b + 2 < full) issue(b + 2, sR0, sQ0, sS0);
-    compute(sR1, sQ1, sS1, ws[b + 1]);
+    if (b + 2 < full) issue(b + 2, s0);
+    compute(s1, ws[b + 1]);
   }
   if (full & 1) {
     meet();
-    compute(sR0, sQ0, sS0, ws[full - 1]);
+    compute(s0, ws[full - 1]);
   }
   if (full < nkb) {  // the features past K are zeros, whatever lies in the rows' padding
     const int k0 = full * kFp8Block;
     meet();
-    issue_scales(full, sS0);
+    issue_scales(full, s0);
 #pragma unroll 1
     for (int t = 0; t < S::kRCopies; ++t) {
       const int i = wave + S::kWaves * t, row = 8 * i + (lane >> 3);
-      sR0[64 * i + lane] = load_chunk(R.base, R.ld, min(r0 + row, R.rows - 1), R.rows, k0 + 16 * ((lane & 7) ^ r_key(row)), p.K);
+      s0[64 * i + lane] = load_chunk(R.base, R.ld, min(r0 + row, R.rows - 1), R.rows, k0 + 16 * ((lane & 7) ^ r_key(row)), p.K);
     }
 #pragma unroll 1
     for (int t = 0; t < S::kQCopies; ++t) {
       const int i = wave + S::kWaves * t, row = 8 * i + (lane >> 3);
-      sQ0[64 * i + lane] = load_chunk(Q.base, Q.ld, min(q0 + row, Q.rows - 1), Q.rows, k0 + 16 * ((lane & 7) ^ q_key(row)), p.K);
+      s0[8 * S::kBR + 64 * i + lane] =
+          load_chunk(Q.base, Q.ld, min(q0 + row, Q.rows - 1), Q.rows, k0 + 16 * ((lane & 7) ^ q_key(row)), p.K);
     }
     meet();
-    compute(sR0, sQ0, sS0, ws[full]);
+    compute(s0, ws[full]);
   }
 
   // A lane's 16 rows of a column.
@@ -448,29 +454,42 @@ static void launch_tiles(const Fp8MmParams& p, hipStream_t stream) {
 
 // 128 x 128 tiles, four waves of 64 x 64, two workgroups a CU, whose copies, products and stores
 // fall at different times. (256 x 256 tiles of eight waves, one workgroup a CU: 139 us against 130
-// for 5120 x 1280 x 16384, 139 against 115 for 5120 x 5120 x 4096.)
-typedef MmShape<128, 128, 2, 2> MmTiles;
+// for 5120 x 1280 x 16384, 139 against 115 for 5120 x 5120 x 4096.) 64 x 64 tiles, four waves of
+// 64 x 16, four workgroups a CU, where there are fewer than 256 of the large ones, and for all float32
+// outputs. (A ring of four stages instead of two: 11.2 us against 9.8 for 1280 x 2560 x 333.)
+typedef MmShape<128, 128, 2, 2> MmLarge;
+typedef MmShape<64, 64, 1, 4> MmSmall;
 
-// Which kernel. The time of the rows kernels goes with the row blocks that their workgroups read
-// (0.27 ns each over about 3 us), that of the tiles with the blocks of K, 0.75 us each while every
-// tile has a CU to itself and 1.3 us (float32 output: 1.15 and 2.1) for each 512 tiles beyond.
-// Measured (us, M x K x T): 1 x 1 tiles of eight waves, 2 x 1 and 2 x 2 of four, 128 x 128:
-// 5120 x 1280 x 1 3.8 / 4.8 / - / 10.4; 5120 x 1280 x 64 8.4 / 7.8 / 8.7 / 10.4; 50280 x 768 x 8
-// 12.8 / 10.5 / - / -; 1280 x 2560 x 333 18.0 / 16.8 / 13.8 / 17.2; 1280 x 2560 x 600 29.5 / 23.4 /
-// 18.4 / 17.6; 5120 x 1280 x 16384 - / - / - / 130: 1.65 PFLOP/s, where the library's product with
-// one scale an operand reaches 3.0 at 8192^3.
+// Which kernel: the one whose time, by the sums below, is the least. Rows: what the workgroups read,
+// or their number where they have little to read, and a wave's blocks one after the other. Tiles:
+// the blocks of K one after the other, a block's time by how many tiles share a CU; a block that is
+// not whole comes last and unstaged. Measured (us, M x K x T: rows 1 x 1 of eight waves, rows 2 x 1 of
+// four, tiles of 64, tiles of 128):
+//   5120 x 1280 x 1        3.8   4.8    -     -      1280 x 2560 x 333   19.0  16.6   9.8  17.5
+//   5120 x 1280 x 8        4.1   5.0   5.6    -      5120 x 1280 x 1024   108  71.5  15.1  12.4
+//   50280 x 768 x 8 (f32) 12.8  10.3  10.8    -      1280 x 2560 x 2048  94.3  70.1  14.2  17.5
+//   1280 x 2560 x 64       6.9   7.7   9.1  17.0     5120 x 1280 x 16384    -     -   182   130
+//   64 x 64 x 16384       13.4   7.6   4.1    -      the same (f32)         -     -   307   356
+// 130 us are 1.65 PFLOP/s; the library's product with one scale an operand reaches 3.0 at 8192^3.
 hipError_t launch_fp8mm(const Fp8MmParams& p, hipStream_t stream) {
-  const long long nkb = (p.K + kFp8Block - 1) / kFp8Block;
-  const auto tiles = [&](int m, int t) { return ((p.M + m - 1ll) / m) * ((p.T + t - 1ll) / t); };
-  const double rows22 = 3 + 0.00027 * static_cast<double>(4 * tiles(32, 32) * nkb);
-  const double block = p.out_bf16 ? 1.0 : 1.6, big = static_cast<double>((tiles(128, 128) + 511) / 512);
-  const double whole = 3 + block * static_cast<double>(nkb) * (tiles(128, 128) <= 256 ? 0.75 : 1.3 * big);
+  const double nkb = (p.K + kFp8Block - 1) / kFp8Block;
+  const auto tiles = [&](double m, double t) { return __builtin_ceil(p.M / m) * __builtin_ceil(p.T / t); };
+  const double n11 = tiles(16, 16), n21 = tiles(32, 16), n64 = tiles(64, 64);
+  const double rows11 = 2.5 + fmax(0.00044 * n11 * nkb, 0.0026 * n11) + 0.09 * nkb;
+  const double rows21 = 2.5 + fmax(0.00072 * n21 * nkb, 0.0025 * n21) + 0.18 * nkb;
+  const double tiles64 = 2 + (p.out_bf16 ? fmax(0.38, 0.0009 * n64) : fmax(0.55, 0.0015 * n64)) * nkb +
+                         (p.K % kFp8Block ? 3 : 0);
   const bool far = p.ldw >= 1 << 24 || p.ldx >= 1 << 24;  // the tiles' offsets have 32 bits
-  if (2 * tiles(16, 16) * nkb <= 16000) launch_rows<1, 1, 8>(p, stream);
-  else if (p.T <= 16 || 3 * tiles(32, 16) * nkb <= 24000) launch_rows<2, 1, 4>(p, stream);
-  else if (far || rows22 < whole) launch_rows<2, 2, 4>(p, stream);
-  else if (p.out_bf16) launch_tiles<MmTiles, true, bf16_t>(p, stream);
-  else launch_tiles<MmTiles, false, float>(p, stream);
+  if (far || tiles64 > fmin(rows11, rows21)) {
+    if (rows11 <= rows21) launch_rows<1, 1, 8>(p, stream);
+    else launch_rows<2, 1, 4>(p, stream);
+  } else if (!p.out_bf16) {
+    launch_tiles<MmSmall, false, float>(p, stream);
+  } else if (tiles(128, 128) < 256) {
+    launch_tiles<MmSmall, true, bf16_t>(p, stream);
+  } else {
+    launch_tiles<MmLarge, true, bf16_t>(p, stream);
+  }
   return hipGetLastError();
 }
 
