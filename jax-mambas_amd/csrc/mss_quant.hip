@@ -5,7 +5,8 @@
 //              eps), y = hn r_t w[f]   (reference mamba/mamba1.py:300-337: nnx.RMSNorm before
 //              the in-projections, the block's output added back)
 //   s[b][t]  = max(max_{f in block b} |y[f][t]| / 448, 2^-126)
-//   q[t][f]  = e4m3(y[f][t] / s[b][t]), rounded to nearest even
+//   q[t][f]  = e4m3(448 y[f][t] / max_{f in block b} |y[f][t]|), or of y 2^126 at the least scale, rounded
+//              to nearest even
 //
 // The stream is channel-major (features, tokens) and a matrix-core product wants 8-bit operands
 // with the features contiguous, so these kernels also transpose: a workgroup owns a tile of
@@ -18,13 +19,24 @@
 
 namespace mss {
 
-// y / s for the reciprocal inv of s, rounded as the division is (one Newton step on the
-// quotient; q * s is never near overflow, |y| <= 448 s). bf16 values over a scale of 7 significant
-// bits meet e4m3's borders exactly, so a quotient off by one float32 step rounds the wrong way.
-__device__ __forceinline__ float divide_by(float y, float s, float inv) {
-  const float q = y * inv;
-  return __builtin_fmaf(__builtin_fmaf(-q, s, y), inv, q);
-}
+// Values over a block's scale. The scale itself is rounded; q is not taken from it but from the
+// block's largest magnitude, y * (448 / m) with the factor in two parts: bf16 values meet e4m3's borders
+// exactly (y / m = 3 / 64, for one, is 21, between 20 and 22), and a quotient that is off by one
+// float32 step there rounds the wrong way.
+struct ToFp8 {
+  float scale, hi, lo;
+  __device__ __forceinline__ explicit ToFp8(uint32_t m) {
+    const float amax = __uint_as_float(m);
+    scale = fp8_scale(amax);
+    hi = kFp8Max / amax;
+    lo = __builtin_fmaf(-hi, amax, kFp8Max) / amax;
+    if (amax < kFp8Max * 1.1754943508222875e-38f) {  // the least scale, 2^-126
+      hi = 8.507059173023462e37f;
+      lo = 0.f;
+    }
+  }
+  __device__ __forceinline__ float operator()(float y) const { return __builtin_fmaf(y, hi, y * lo); }
+};
 
 // kN neighbouring values, of any alignment.
 template <int kN, typename io_t>
@@ -114,11 +126,9 @@ __global__ __launch_bounds__(128 * sizeof(io_t)) void quant_tile_kernel(QuantPar
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) m = max(m, s_m[i][l * kTV + j]);
-    const float s = fp8_scale(__uint_as_float(m));
-    const float inv = 1.f / s;
-    if (g == 0 && t + j < p.tokens) p.scales[static_cast<long long>(b) * p.tokens + t + j] = s;
-    s_q[(l * kTV + j) * kPitch + g] = pack_fp8x4(divide_by(v[0][j], s, inv), divide_by(v[1][j], s, inv),
-                                                 divide_by(v[2][j], s, inv), divide_by(v[3][j], s, inv));
+    const ToFp8 to(m);
+    if (g == 0 && t + j < p.tokens) p.scales[static_cast<long long>(b) * p.tokens + t + j] = to.scale;
+    s_q[(l * kTV + j) * kPitch + g] = pack_fp8x4(to(v[0][j]), to(v[1][j]), to(v[2][j]), to(v[3][j]));
   }
   __syncthreads();
 #pragma unroll
@@ -160,17 +170,14 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(QuantParams p) {
   for (int i = 0; i < 8; ++i) m = max(m, magnitude_bits(v[i]));
 #pragma unroll
   for (int s = 1; s < 16; s *= 2) m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), s)));
-  const float scale = fp8_scale(__uint_as_float(m));
-  const float inv = 1.f / scale;
+  const ToFp8 to(m);
   if (!ok) return;
-  if (lane == 0) p.scales[static_cast<long long>(b) * p.tokens + t] = scale;
+  if (lane == 0) p.scales[static_cast<long long>(b) * p.tokens + t] = to.scale;
   // A row of q is 16-byte aligned and holds at least ceil16(features) bytes up to the next row;
   // the last row's end is the tensor's, so the bytes past the features are not touched.
   unsigned char* q = p.q + t * p.ldq + f0;
-  const uint32_t lo = pack_fp8x4(divide_by(v[0], scale, inv), divide_by(v[1], scale, inv), divide_by(v[2], scale, inv),
-                                 divide_by(v[3], scale, inv));
-  const uint32_t hi = pack_fp8x4(divide_by(v[4], scale, inv), divide_by(v[5], scale, inv), divide_by(v[6], scale, inv),
-                                 divide_by(v[7], scale, inv));
+  const uint32_t lo = pack_fp8x4(to(v[0]), to(v[1]), to(v[2]), to(v[3]));
+  const uint32_t hi = pack_fp8x4(to(v[4]), to(v[5]), to(v[6]), to(v[7]));
   if (f0 + 8 <= p.features) {
     *reinterpret_cast<uint2*>(q) = make_uint2(lo, hi);
   } else {
@@ -205,14 +212,13 @@ __global__ __launch_bounds__(256) void quant_weight_kernel(QuantWeightParams p) 
   if ((threadIdx.x & 63) == 0) s_m[threadIdx.x >> 6] = m;
   __syncthreads();
   m = max(max(s_m[0], s_m[1]), max(s_m[2], s_m[3]));
-  const float scale = fp8_scale(__uint_as_float(m));
-  const float inv = 1.f / scale;
-  if (threadIdx.x == 0) p.scales[static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x] = scale;
+  const ToFp8 to(m);
+  if (threadIdx.x == 0) p.scales[static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x] = to.scale;
 #pragma unroll
   for (int i = 0; i < 32; ++i) {
     const int r = row0 + 4 * i;
     if (r >= p.M || k >= p.K) continue;
-    const uint32_t two = pack_fp8x4(divide_by(v[i][0], scale, inv), divide_by(v[i][1], scale, inv), 0.f, 0.f);
+    const uint32_t two = pack_fp8x4(to(v[i][0]), to(v[i][1]), 0.f, 0.f);
     unsigned char* q = p.q + r * p.ldq + k;  // k even, rows 16-byte aligned
     if (k + 1 < p.K) *reinterpret_cast<uint16_t*>(q) = static_cast<uint16_t>(two);
     else *q = static_cast<unsigned char>(two);
@@ -235,11 +241,9 @@ __device__ __noinline__ float norm_block_again(const float* __restrict__ hn, con
                                                float r, int n, unsigned char* __restrict__ q) {
   uint32_t m = 0;
   for (int i = 0; i < n; ++i) m = max(m, magnitude_bits(hn[i * T] * r * w[i]));
-  const float s = fp8_scale(__uint_as_float(m));
-  const float inv = 1.f / s;
-  for (int i = 0; i < n; ++i)
-    q[i] = static_cast<unsigned char>(pack_fp8x4(divide_by(hn[i * T] * r * w[i], s, inv), 0.f, 0.f, 0.f));
-  return s;
+  const ToFp8 to(m);
+  for (int i = 0; i < n; ++i) q[i] = static_cast<unsigned char>(pack_fp8x4(to(hn[i * T] * r * w[i]), 0.f, 0.f, 0.f));
+  return to.scale;
 }
 
 // A workgroup owns 4 kL tokens and walks the features, kRound of them at a time: kL lanes hold a
@@ -416,11 +420,9 @@ __global__ __launch_bounds__(512) void norm_fp8_rows_kernel(QuantParams p) {
     }
 #pragma unroll
     for (int s = 1; s < 32; s *= 2) m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), s)));
-    const float scale = fp8_scale(__uint_as_float(m));
-    const float inv = 1.f / scale;
-    if ((threadIdx.x & 31) == 0) p.scales[(f0 / kFp8Block) * T + t] = scale;
-    const uint32_t q4 = pack_fp8x4(divide_by(v[0], scale, inv), divide_by(v[1], scale, inv), divide_by(v[2], scale, inv),
-                                   divide_by(v[3], scale, inv));
+    const ToFp8 to(m);
+    if ((threadIdx.x & 31) == 0) p.scales[(f0 / kFp8Block) * T + t] = to.scale;
+    const uint32_t q4 = pack_fp8x4(to(v[0]), to(v[1]), to(v[2]), to(v[3]));
     unsigned char* q = p.q + t * p.ldq + f0;
     if (f0 + 4 <= p.features) {
       *reinterpret_cast<uint32_t*>(q) = q4;
