@@ -38,41 +38,36 @@ struct ToFp8 {
   __device__ __forceinline__ float operator()(float y) const { return __builtin_fmaf(y, hi, y * lo); }
 };
 
-// kN neighbouring values, of any alignment.
-template <int kN, typename io_t>
-__device__ __forceinline__ void load_run(const io_t* __restrict__ p, float (&v)[kN]) {
-  io_t e[kN];
-  __builtin_memcpy(e, p, sizeof(e));
-#pragma unroll
-  for (int i = 0; i < kN; ++i) v[i] = to_f32(e[i]);
-}
-
-// The larger of v and the value kLanes away (kLanes a power of two below 64), for all lanes.
-template <int kLanes>
-__device__ __forceinline__ uint32_t max_across(uint32_t v) {
+// v and the values kLanes away (32, 16, 2, 1: the lane whose index differs there; 8, 4: the lane that
+// far round in a row of 16, so that after both a value has met its three fellows), for all lanes, by
+// `op`: register moves, where a shuffle goes through LDS.
+template <int kLanes, typename op_t>
+__device__ __forceinline__ uint32_t across(uint32_t v, const op_t& op) {
   if constexpr (kLanes == 32) {
     const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return max(static_cast<uint32_t>(r[0]), static_cast<uint32_t>(r[1]));
+    return op(static_cast<uint32_t>(r[0]), static_cast<uint32_t>(r[1]));
   } else if constexpr (kLanes == 16) {
     const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    return max(static_cast<uint32_t>(r[0]), static_cast<uint32_t>(r[1]));
-  } else if constexpr (kLanes == 8) {  // row_ror:8 within 16 lanes
-    return max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x128, 0xF, 0xF, true)));
+    return op(static_cast<uint32_t>(r[0]), static_cast<uint32_t>(r[1]));
   } else {
-    return max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), kLanes)));
+    constexpr int kCtrl = kLanes == 8 ? 0x128 : kLanes == 4 ? 0x124 : kLanes == 2 ? 0x4E : 0xB1;  // row_ror, quad_perm
+    return op(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), kCtrl, 0xF, 0xF, true)));
   }
 }
-// The same over every lane whose index differs above kFrom - 1.
-template <int kFrom>
-__device__ __forceinline__ uint32_t max_above(uint32_t v) {
-  if constexpr (kFrom < 64) return max_above<2 * kFrom>(max_across<kFrom>(v));
+// The same over every lane whose index differs above kFrom - 1 and below kTo (all of 4 and 8, or neither).
+template <int kFrom, int kTo = 64, typename op_t>
+__device__ __forceinline__ uint32_t across_all(uint32_t v, const op_t& op) {
+  if constexpr (kFrom < kTo) return across_all<2 * kFrom, kTo>(across<kFrom>(v, op), op);
   return v;
+}
+template <int kFrom, int kTo = 64>
+__device__ __forceinline__ uint32_t max_above(uint32_t v) {
+  return across_all<kFrom, kTo>(v, [](uint32_t a, uint32_t b) { return max(a, b); });
 }
 template <int kFrom>
 __device__ __forceinline__ float sum_above(float v) {
-#pragma unroll
-  for (int s = kFrom; s < 64; s *= 2) v += __shfl_xor(v, s);
-  return v;
+  return __uint_as_float(across_all<kFrom>(
+      __float_as_uint(v), [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
 }
 
 // 16 bytes of a token's row from LDS (8-byte aligned there) to the features f .. f + 16 of q.
@@ -104,14 +99,19 @@ __global__ __launch_bounds__(128 * sizeof(io_t)) void quant_tile_kernel(QuantPar
   const long long t = t0 + l * kTV;
   const io_t* __restrict__ x = static_cast<const io_t*>(p.x) + t;
   float v[4][kTV];
+  if (t0 + 64 <= p.tokens) {
+    io_t raw[4][kTV];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (f0 + i < p.features && t + kTV <= p.tokens) {
-      load_run(x + (f0 + i) * p.sf, v[i]);
-    } else {
+    for (int i = 0; i < 4; ++i) __builtin_memcpy(raw[i], x + min(f0 + i, p.features - 1) * p.sf, sizeof(raw[i]));
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < kTV; ++j) v[i][j] = f0 + i < p.features ? to_f32(raw[i][j]) : 0.f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < kTV; ++j) v[i][j] = f0 + i < p.features && t + j < p.tokens ? to_f32(x[(f0 + i) * p.sf + j]) : 0.f;
-    }
   }
 #pragma unroll
   for (int j = 0; j < kTV; ++j) {
@@ -246,6 +246,32 @@ __device__ __noinline__ float norm_block_again(const float* __restrict__ hn, con
   return to.scale;
 }
 
+// Four neighbouring values as they lie in memory, of any alignment.
+template <typename T>
+struct Run4;
+template <>
+struct Run4<float> {
+  f32x4 v;
+  __device__ __forceinline__ void load(const float* p) { v = *reinterpret_cast<const f32x4_any*>(p); }
+  __device__ __forceinline__ void set(int j, float x) { v[j] = x; }
+  __device__ __forceinline__ float get(int j) const { return v[j]; }
+};
+template <>
+struct Run4<bf16_t> {
+  uint32_t v[2];
+  __device__ __forceinline__ void load(const bf16_t* p) {
+    const u32x2_any x = *reinterpret_cast<const u32x2_any*>(p);
+    v[0] = x[0];
+    v[1] = x[1];
+  }
+  __device__ __forceinline__ void set(int j, bf16_t x) {
+    v[j / 2] = j % 2 ? (v[j / 2] & 0xffffu) | static_cast<uint32_t>(x.bits) << 16 : x.bits;
+  }
+  __device__ __forceinline__ float get(int j) const {
+    return __uint_as_float(j % 2 ? v[j / 2] & 0xffff0000u : v[j / 2] << 16);
+  }
+};
+
 // A workgroup owns 4 kL tokens and walks the features, kRound of them at a time: kL lanes hold a
 // row of 4 tokens each, a thread 4 consecutive features. The next round's rows are on their way
 // while a round is worked on (bare barriers: __syncthreads would wait for them).
@@ -274,6 +300,7 @@ __global__ __launch_bounds__(64 * kWaves) void norm_fp8_tile_kernel(QuantParams 
   __shared__ alignas(8) uint32_t s_q[kTok * kPitch];
   __shared__ float s_block[kNormMaxBlocks][kTok];
   __shared__ float s_ss[kWaves][kTok];
+  __shared__ int s_again;
   const int l = threadIdx.x % kL, g = threadIdx.x / kL;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const long long T = p.tokens, t0 = static_cast<long long>(tile_of_xcd(blockIdx.x, gridDim.x)) * kTok, t = t0 + 4 * l;
@@ -282,20 +309,32 @@ __global__ __launch_bounds__(64 * kWaves) void norm_fp8_tile_kernel(QuantParams 
   const float* __restrict__ h = static_cast<const float*>(p.x) + t;
   const delta_t* __restrict__ delta = static_cast<const delta_t*>(p.delta) + t;
 
-  float hv[4][4], dv[4][4], wv[4];
+  // (raw vectors, the deltas converted where they are used, and one branch around all loads: they
+  // are in flight together)
+  f32x4 hv[4];
+  float wv[4];
+  Run4<delta_t> dv[4];
+  const bool whole_tile = t0 + kTok <= T;
   const auto fetch = [&](int f0) {
+    if (whole_tile) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int f = f0 + i < F ? f0 + i : F - 1;
-      wv[i] = p.w[f];
-      if (whole) {
-        load_run(h + f * T, hv[i]);
-        if constexpr (kDelta) load_run(delta + f * T, dv[i]);
-      } else {
+      for (int i = 0; i < 4; ++i) {
+        const int f = min(f0 + i, F - 1);
+        wv[i] = p.w[f];
+        hv[i] = *reinterpret_cast<const f32x4_any*>(h + f * T);
+        if constexpr (kDelta) dv[i].load(delta + f * T);
+      }
+    } else {
+      asm volatile("");  // else the compiler takes the single loads for both
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          hv[i][j] = t + j < T ? h[f * T + j] : 0.f;
-          if constexpr (kDelta) dv[i][j] = t + j < T ? to_f32(delta[f * T + j]) : 0.f;
+      for (int i = 0; i < 4; ++i) {
+        const int f = min(f0 + i, F - 1);
+        wv[i] = p.w[f];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {  // (tokens past the end: the last one again, its results unused)
+          const long long o = f * T + min(static_cast<long long>(j), T - 1 - t);
+          hv[i][j] = h[o];
+          if constexpr (kDelta) dv[i].set(j, delta[o]);
         }
       }
     }
@@ -309,7 +348,7 @@ __global__ __launch_bounds__(64 * kWaves) void norm_fp8_tile_kernel(QuantParams 
       const bool in = f0 + i < F;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float x = kDelta ? hv[i][j] + dv[i][j] : hv[i][j];
+        const float x = kDelta ? hv[i][j] + dv[i].get(j) : hv[i][j];
         y[i][j] = in ? x : 0.f;
         ss[j] = __builtin_fmaf(y[i][j], y[i][j], ss[j]);
       }
@@ -358,7 +397,8 @@ __global__ __launch_bounds__(64 * kWaves) void norm_fp8_tile_kernel(QuantParams 
     const float s = sum_above<kL>(ss[j]);
     if ((threadIdx.x & 63) < kL) s_ss[wave][4 * l + j] = s;
   }
-  __syncthreads();  // hn and q of this tile are written too, for the blocks done again
+  if (threadIdx.x == 0) s_again = 0;
+  meet();
   const int nb = (F + kFp8Block - 1) / kFp8Block;
   for (int i = threadIdx.x; i < nb * kTok; i += 64 * kWaves) {
     const int b = i / kTok, j = i % kTok;
@@ -368,20 +408,96 @@ __global__ __launch_bounds__(64 * kWaves) void norm_fp8_tile_kernel(QuantParams 
     for (int k = 0; k < kWaves; ++k) tot += s_ss[k][j];
     const float r = 1.f / __builtin_sqrtf(tot / F + p.eps);
     const float m = s_block[b][j];
-    float s = fp8_scale(m * r);
-    if (!scale_is_plain(m, r)) {
-      const int f = b * kFp8Block;
-      s = norm_block_again((kDelta ? p.hn : static_cast<const float*>(p.x)) + f * T + t0 + j, p.w + f, T, r,
+    if (scale_is_plain(m, r)) p.scales[b * T + t0 + j] = fp8_scale(m * r);
+    else s_again = 1;
+  }
+  meet();
+  if (s_again == 0) return;
+  __syncthreads();  // hn and q of this tile are written
+  for (int i = threadIdx.x; i < nb * kTok; i += 64 * kWaves) {
+    const int b = i / kTok, j = i % kTok, f = b * kFp8Block;
+    if (t0 + j >= T) continue;
+    float tot = 0.f;
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) tot += s_ss[k][j];
+    const float r = 1.f / __builtin_sqrtf(tot / F + p.eps);
+    if (!scale_is_plain(s_block[b][j], r))
+      p.scales[b * T + t0 + j] =
+          norm_block_again((kDelta ? p.hn : static_cast<const float*>(p.x)) + f * T + t0 + j, p.w + f, T, r,
                            min(kFp8Block, F - f), p.q + (t0 + j) * p.ldq + f);
-    }
-    p.scales[b * T + t0 + j] = s;
   }
 }
 
-// Few tokens, or more features than the tiles take: one token a workgroup, two passes over its
-// column.
-template <typename delta_t, bool kDelta>
+// Few tokens: one a workgroup, a feature a lane (neighbouring features of a few tokens share cache
+// lines), kRounds x 512 of them in registers; q by the blocks' maxima before the norm, as above.
+// (1280 x 8: 5.7 us with the features read twice, 4.6 with four neighbours a lane.)
+template <typename delta_t, bool kDelta, int kRounds>
 __global__ __launch_bounds__(512) void norm_fp8_rows_kernel(QuantParams p) {
+  __shared__ float s_ss[8];
+  __shared__ uint32_t s_m[kRounds][8];
+  const long long T = p.tokens, t = blockIdx.x;
+  const int F = p.features, wave = threadIdx.x >> 6;
+  const float* __restrict__ h = static_cast<const float*>(p.x) + t;
+  const delta_t* __restrict__ delta = static_cast<const delta_t*>(p.delta) + t;
+  float x[kRounds], d[kRounds], w[kRounds];
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) {
+    const int f = min(512 * k + static_cast<int>(threadIdx.x), F - 1);
+    x[k] = h[f * T];
+    if constexpr (kDelta) d[k] = to_f32(delta[f * T]);
+    w[k] = p.w[f];
+  }
+  float ss = 0.f;
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) {
+    const bool in = 512 * k + static_cast<int>(threadIdx.x) < F;
+    if constexpr (kDelta) x[k] += d[k];
+    ss = __builtin_fmaf(x[k], in ? x[k] : 0.f, ss);
+    w[k] *= x[k];  // y' = hn w
+    const uint32_t m = max_above<1>(in ? magnitude_bits(w[k]) : 0u);
+    if ((threadIdx.x & 63) == 0) s_m[k][wave] = m;
+  }
+  ss = wave_sum(ss);
+  if ((threadIdx.x & 63) == 0) s_ss[wave] = ss;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) {
+    const int f = 512 * k + threadIdx.x;
+    if (f < F) {
+      const uint32_t m = max(s_m[k][wave], s_m[k][wave ^ 1]);
+      const float inv = m ? kFp8Max / __uint_as_float(m) : 0.f;
+      p.q[t * p.ldq + f] = static_cast<unsigned char>(pack_fp8x4(w[k] * inv, 0.f, 0.f, 0.f));
+      if constexpr (kDelta) p.hn[f * T + t] = x[k];
+    }
+  }
+  const int nb = (F + kFp8Block - 1) / kFp8Block;
+  float tot = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) tot += s_ss[i];
+  const float r = 1.f / __builtin_sqrtf(tot / F + p.eps);
+  float m = 0.f;
+  bool plain = true;
+  if (static_cast<int>(threadIdx.x) < nb) {  // a block a lane
+    const int b = threadIdx.x;
+    m = __uint_as_float(max(s_m[b / 4][2 * (b % 4)], s_m[b / 4][2 * (b % 4) + 1]));
+    plain = scale_is_plain(m, r);
+    if (plain) p.scales[b * T + t] = fp8_scale(m * r);
+  }
+  if (__syncthreads_or(plain ? 0 : 1)) {
+    __syncthreads();  // hn and q of this token are written
+    if (!plain) {
+      const int b = threadIdx.x, f = b * kFp8Block;
+      p.scales[b * T + t] =
+          norm_block_again((kDelta ? p.hn : static_cast<const float*>(p.x)) + f * T + t, p.w + f, T, r,
+                           min(kFp8Block, F - f), p.q + t * p.ldq + f);
+    }
+  }
+}
+
+// More features than registers hold or the tiles take: two passes over a token's column, 32 lanes to
+// a block, 4 consecutive features each.
+template <typename delta_t, bool kDelta>
+__global__ __launch_bounds__(512) void norm_fp8_wide_kernel(QuantParams p) {
   __shared__ float s_part[8];
   const long long T = p.tokens, t = blockIdx.x;
   const float* __restrict__ h = static_cast<const float*>(p.x) + t;
@@ -400,7 +516,6 @@ __global__ __launch_bounds__(512) void norm_fp8_rows_kernel(QuantParams p) {
   for (int i = 0; i < 8; ++i) tot += s_part[i];
   const float r = 1.f / __builtin_sqrtf(tot / p.features + p.eps);
   const int padded = (p.features + kFp8Block - 1) / kFp8Block * kFp8Block;
-  // 32 lanes hold a block, 4 consecutive features each.
   for (int f0 = threadIdx.x * 4; f0 < padded; f0 += 2048) {
     float v[4];
     uint32_t m = 0;
@@ -418,8 +533,7 @@ __global__ __launch_bounds__(512) void norm_fp8_rows_kernel(QuantParams p) {
       }
       m = max(m, magnitude_bits(v[i]));
     }
-#pragma unroll
-    for (int s = 1; s < 32; s *= 2) m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), s)));
+    m = max_above<1, 32>(m);
     const ToFp8 to(m);
     if ((threadIdx.x & 31) == 0) p.scales[(f0 / kFp8Block) * T + t] = to.scale;
     const uint32_t q4 = pack_fp8x4(to(v[0]), to(v[1]), to(v[2]), to(v[3]));
@@ -439,10 +553,10 @@ __global__ __launch_bounds__(512) void norm_fp8_rows_kernel(QuantParams p) {
 // quant: rows/tile 2560 x 32 5.0/4.3, x 8 3.1/3.9; 2560 x 16384 bf16 81/26.4, 4.8 TB/s of the 5.2 that
 // a copy reaches.
 constexpr int kQuantTileTokens = 32;
-// norm, bf16 delta: a token a workgroup 1280 x 64 6.9, x 256 11.5; tiles of 8 tokens 9.1 and 9.5,
-// 1280 x 2048 14.2, x 4096 21.8; of 16 tokens 14.8 and 16.6, x 8192 25.1, x 16384 65; of 32 tokens
-// 19.7, 20.8, 25.7, and 50 at 16384: 4.6 TB/s.
-constexpr int kNormTileTokens = 128;
+// norm, bf16 delta: a token a workgroup 1280 x 128 6.0, x 256 9.0, x 512 14.0; tiles of 8 tokens 9.2,
+// 9.4 and 10.1, 1280 x 2048 14.2, x 4096 21.8; of 16 tokens 14.8 and 16.6, x 8192 25.1, x 16384 65; of
+// 32 tokens 19.7, 20.8, 25.7, and 50 at 16384: 4.6 TB/s.
+constexpr int kNormTileTokens = 256;
 constexpr int kNormNarrowTokens = 2560;
 constexpr int kNormMiddleTokens = 8192;
 
@@ -475,10 +589,19 @@ hipError_t launch_quant_fp8_weight(const QuantWeightParams& p, bool io_bf16, hip
 }
 
 template <typename delta_t, bool kDelta>
+static void launch_norm_rows(const QuantParams& p, hipStream_t stream) {
+  const dim3 grid(p.tokens), block(512);
+  if (p.features <= 1024) hipLaunchKernelGGL((norm_fp8_rows_kernel<delta_t, kDelta, 2>), grid, block, 0, stream, p);
+  else if (p.features <= 2048) hipLaunchKernelGGL((norm_fp8_rows_kernel<delta_t, kDelta, 4>), grid, block, 0, stream, p);
+  else if (p.features <= 8192) hipLaunchKernelGGL((norm_fp8_rows_kernel<delta_t, kDelta, 16>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((norm_fp8_wide_kernel<delta_t, kDelta>), grid, block, 0, stream, p);
+}
+
+template <typename delta_t, bool kDelta>
 static void launch_norm(const QuantParams& p, hipStream_t stream) {
   const auto tiles = [&](int n) { return dim3((p.tokens + n - 1) / n); };
   if (p.tokens < kNormTileTokens || p.features > kNormMaxBlocks * kFp8Block)
-    hipLaunchKernelGGL((norm_fp8_rows_kernel<delta_t, kDelta>), tiles(1), dim3(512), 0, stream, p);
+    launch_norm_rows<delta_t, kDelta>(p, stream);
   else if (p.tokens <= kNormNarrowTokens)
     hipLaunchKernelGGL((norm_fp8_tile_kernel<delta_t, kDelta, 2, 8>), tiles(8), dim3(512), 0, stream, p);
   else if (p.tokens <= kNormMiddleTokens)
