@@ -94,7 +94,8 @@ __global__ __launch_bounds__(128 * sizeof(io_t)) void quant_tile_kernel(QuantPar
   __shared__ uint32_t s_m[kWaves][64];
   __shared__ alignas(8) uint32_t s_q[64 * kPitch];
   const int l = threadIdx.x % kLanes, g = threadIdx.x / kLanes, wave = threadIdx.x / 64;
-  const long long t0 = blockIdx.x * 64ll;
+  long long t0 = blockIdx.x * 64ll;
+  if (t0 + 64 > p.tokens && p.tokens >= 64) t0 = p.tokens - 64;  // the last tile, whole: some tokens come out twice
   const int b = blockIdx.y, f0 = b * kFp8Block + 4 * g;
   const long long t = t0 + l * kTV;
   const io_t* __restrict__ x = static_cast<const io_t*>(p.x) + t;
@@ -303,7 +304,12 @@ __global__ __launch_bounds__(64 * kWaves) void norm_fp8_tile_kernel(QuantParams 
   __shared__ int s_again;
   const int l = threadIdx.x % kL, g = threadIdx.x / kL;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  const long long T = p.tokens, t0 = static_cast<long long>(tile_of_xcd(blockIdx.x, gridDim.x)) * kTok, t = t0 + 4 * l;
+  const long long T = p.tokens;
+  // The last tile begins earlier rather than be cut: its first tokens come out the same twice. (Not
+  // in place, where they would be added to twice.)
+  long long t0 = static_cast<long long>(tile_of_xcd(blockIdx.x, gridDim.x)) * kTok;
+  if (t0 + kTok > T && T >= kTok && (!kDelta || p.hn != p.x)) t0 = T - kTok;
+  const long long t = t0 + 4 * l;
   const int F = p.features;
   const bool whole = t + 4 <= T;
   const float* __restrict__ h = static_cast<const float*>(p.x) + t;
@@ -553,12 +559,12 @@ __global__ __launch_bounds__(512) void norm_fp8_wide_kernel(QuantParams p) {
 // quant: rows/tile 2560 x 32 5.0/4.3, x 8 3.1/3.9; 2560 x 16384 bf16 81/26.4, 4.8 TB/s of the 5.2 that
 // a copy reaches.
 constexpr int kQuantTileTokens = 32;
-// norm, bf16 delta: a token a workgroup 1280 x 128 6.0, x 256 9.0, x 512 14.0; tiles of 8 tokens 9.2,
-// 9.4 and 10.1, 1280 x 2048 14.2, x 4096 21.8; of 16 tokens 14.8 and 16.6, x 8192 25.1, x 16384 65; of
-// 32 tokens 19.7, 20.8, 25.7, and 50 at 16384: 4.6 TB/s.
+// norm, bf16 delta: a token a workgroup 1280 x 128 6.0, x 256 9.0, x 512 13.8; tiles of 8 tokens x 256
+// 8.7, x 512 9.2, x 2048 12.4, x 4096 20; of 16 tokens x 2048 13.3, x 4096 14.7, x 8192 23.5, x 16384 58;
+// of 32 tokens x 4096 17, x 8192 21.6, x 16384 45: 5.1 TB/s.
 constexpr int kNormTileTokens = 256;
-constexpr int kNormNarrowTokens = 2560;
-constexpr int kNormMiddleTokens = 8192;
+constexpr int kNormNarrowTokens = 2048;
+constexpr int kNormMiddleTokens = 6144;
 
 template <typename io_t>
 static void launch_quant(const QuantParams& p, hipStream_t stream) {
