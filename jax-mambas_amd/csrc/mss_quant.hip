@@ -231,10 +231,10 @@ __global__ __launch_bounds__(256) void quant_weight_kernel(QuantWeightParams p) 
 // with y' = hn w and m' = max |y'| over the block, q = e4m3(448 y' / m') and s = r m' / 448. So
 // q needs no second pass over the features: each block leaves as it is read, and the scales,
 // kept in LDS until the sum of squares is whole, are the only thing that waits for r. That is
-// also one rounding less than hn r w. Where it does not hold (m' far below 1 or not finite, or
-// a scale at its lower bound) the block is done again from the formula.
+// also one rounding less than hn r w. Where it does not hold (m' far below 1, m' or m' r not finite,
+// or a scale at its lower bound) the block is done again from the formula.
 __device__ __forceinline__ bool scale_is_plain(float m, float r) {
-  return m == 0.f || (m > 7.9e-31f && m < __builtin_inff() && !(m * r < kFp8Max * 1.1754943508222875e-38f));
+  return m == 0.f || (m > 7.9e-31f && m * r < __builtin_inff() && !(m * r < kFp8Max * 1.1754943508222875e-38f));
 }
 
 // One block of one token from the formula, by one thread: its scale.

@@ -390,3 +390,93 @@ def test_side_stream_and_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, step()))
+
+
+# The kernels' other sizes: each side of the numbers at which another kernel takes over.
+@pytest.mark.gpu
+@pytest.mark.parametrize("delta", [None, torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("f,t", [(300, 255), (300, 256), (1000, 2048), (130, 2049), (260, 6144), (129, 6145), (1025, 31),
+                                 (2049, 255), (8192, 3), (8193, 5), (8192, 300), (8200, 270)])
+def test_norm_sizes(f, t, delta):
+    test_norm(f, t, delta)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f,t", [(300, 31), (300, 32), (129, 63), (1000, 65), (257, 16001)])
+def test_quantise_sizes(f, t):
+    for dtype in (torch.float32, torch.bfloat16):
+        for layout in ("channel", "rows_apart"):
+            test_quantise(f, t, layout, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("token_major", [False, True])
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,k,t", [(2100, 200, 2200), (2048, 384, 2048), (3000, 128, 1500), (64, 64, 4000), (5000, 100, 5),
+                                   (1000, 2600, 200)])
+def test_matmul_sizes(m, k, t, out_dtype, token_major):
+    test_matmul(m, k, t, out_dtype, token_major)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [5, 300, 2500, 6200])
+def test_norm_blocks_done_from_the_formula(t):
+    """Blocks whose maximum before the norm is far from 1, or whose scale is at its lower bound: tiny
+    and huge features, weights of zero and far from 1, no epsilon, one infinite feature."""
+    f = 700
+    h = rand(f, t, seed=11)
+    w = torch.ones(f, device="cuda")
+    h[:BLOCK] *= 1e-36
+    w[BLOCK:2 * BLOCK] = 0
+    w[2 * BLOCK:3 * BLOCK] = 1e-33
+    w[3 * BLOCK:4 * BLOCK] = 1e-38
+    h[:, 1] = 0
+    h[:, 2] *= 1e-30  # its squares vanish
+    h[:, 3] *= 1e25  # and here overflow: 1 / infinity
+    h[130, 4] = float("inf")
+    for delta in (None, torch.zeros(f, t, dtype=torch.bfloat16, device="cuda")):
+        for eps in (1e-5, 0.0):
+            _, q, s = add_rmsnorm_fp8(h, delta, w, eps)
+            got = q.double() * s.double().repeat_interleave(BLOCK, 0)[:f].t()
+            r = 1 / torch.sqrt(h.square().mean(0) + eps)
+            want = (h * r).mul(w[:, None]).double().t()
+            per = s.double().repeat_interleave(BLOCK, 0)[:f].t()
+            ok = torch.isfinite(want).view(t, f)
+            for b in range(s.shape[0]):  # a block with a value that is none stands for none
+                part = slice(b * BLOCK, min(f, (b + 1) * BLOCK))
+                ok[:, part] &= ok[:, part].all(1, keepdim=True)
+            assert torch.equal(torch.isnan(got), ~ok)
+            # half a step of the value over its scale, and float32 roundings of value and sum: F / 2 + 8
+            ratio = (want / per).abs().clamp_min(2.0 ** -40)
+            step = torch.exp2(torch.floor(torch.log2(ratio)).clamp_min(-6) - 4) * per
+            bound = step + want.abs() * (f / 2 + 8) * 2.0 ** -23 + 2.0 ** -126 * 2.0 ** -10
+            assert ((got - want).abs() <= bound)[ok].all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f,t", [(1, 1), (300, 9), (700, 301), (640, 2777), (300, 7001), (9000, 40)])
+def test_norm_in_place(lib, f, t):
+    """The C entry point with hn = h gives what it gives elsewhere, bit for bit."""
+    h, d, w = rand(f, t, seed=12), rand(f, t, seed=13, dtype=torch.bfloat16), torch.rand(f, device="cuda") + 0.5
+    hn, q, s = add_rmsnorm_fp8(h, d, w)
+    q2, s2 = torch.empty_like(q), torch.empty_like(s)
+    ld = -(-f // 16) * 16
+    q2 = torch.zeros(t, ld, dtype=torch.uint8, device="cuda").view(FP8)[:, :f]
+    a = _lib.NormFp8Args(features=f, tokens=t, delta_dtype=1, eps=1e-5, ldq=ld, h=h.data_ptr(), delta=d.data_ptr(),
+                         weight=w.data_ptr(), hn=h.data_ptr(), q=q2.data_ptr(), scales=s2.data_ptr())
+    assert lib.mss_norm_fp8(a, torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(h, hn) and torch.equal(q2.float(), q.float()) and torch.equal(s2, s)
+
+
+@pytest.mark.gpu
+def test_quantise_borders():
+    """Quotients that meet e4m3's borders exactly round to the even neighbour, whatever the scale's
+    own rounding: 21 of 448 lies between 20 and 22, 84 between 80 and 88."""
+    largest = torch.tensor([2.59375, 2.03125, 2.8125, 7.0, 1.5], device="cuda")
+    x = torch.zeros(BLOCK, 5, device="cuda")
+    x[0] = largest
+    x[1], x[2], x[3] = largest * 3 / 64, -largest * 3 / 16, largest * 9 / 448
+    for wide in (1, 20):  # both kernels
+        q, _ = quantize_fp8(x.repeat(1, wide).to(torch.bfloat16) if wide == 1 else x.repeat(1, wide))
+        v = q.float()[:5]
+        assert torch.all(v[:, 0] == 448) and torch.all(v[:, 1] == 20) and torch.all(v[:, 2] == -80) and torch.all(v[:, 3] == 9)
