@@ -98,8 +98,8 @@ __device__ __forceinline__ u32x4 load_chunk(const unsigned char* __restrict__ ba
 
 // ------------------------------------------------------------------------- few tokens, few tiles
 // No LDS on the way in: a wave reads its operands' rows straight from memory and the caches, a
-// block ahead of the products. The kKS waves of a workgroup share one tile of 16 kMT x 16 kNT,
-// every kKS-th block each, and their sums meet in LDS in a fixed order.
+// block ahead of the products. The 8 waves of a workgroup share one tile of 16 x 16, every eighth
+// block each, and their sums meet in LDS in a fixed order.
 struct RowBlock {
   u32x4 v[2];  // 16 bytes at 16 g and 16 at 16 g + 64 of the block
   __device__ __forceinline__ void load(const unsigned char* __restrict__ base, long long ld, int row, int rows, int k,
@@ -118,94 +118,60 @@ struct RowBlock {
   }
 };
 
-template <int kMT, int kNT, int kKS, typename out_t>
-__global__ __launch_bounds__(64 * kKS) void fp8mm_rows_kernel(Fp8MmParams p) {
-  constexpr int kTiles = kMT * kNT;
-  __shared__ f32x4 s_part[kKS - 1][kTiles * 64];
+constexpr int kRowsWaves = 8;
+template <typename out_t>
+__global__ __launch_bounds__(64 * kRowsWaves) void fp8mm_rows_kernel(Fp8MmParams p) {
+  __shared__ f32x4 s_part[kRowsWaves - 1][64];
   const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int m0 = blockIdx.x * 16 * kMT, t0 = blockIdx.y * 16 * kNT;
+  const int m0 = blockIdx.x * 16, t = blockIdx.y * 16 + j;
   const int nkb = (p.K + kFp8Block - 1) / kFp8Block;
-  const float* __restrict__ ws = p.ws + static_cast<long long>(m0 / kFp8Block) * nkb;  // 16 kMT divides 128
-  f32x4 acc[kMT][kNT];
-#pragma unroll
-  for (int a = 0; a < kMT; ++a)
-#pragma unroll
-    for (int c = 0; c < kNT; ++c) acc[a][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-  RowBlock w[kMT], x[kNT];
-  float s[kNT];
+  const float* __restrict__ ws = p.ws + static_cast<long long>(m0 / kFp8Block) * nkb;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  RowBlock w, x;
+  float s;
   const auto fetch = [&](int b) {
     const int k = b * kFp8Block + 16 * g;
-#pragma unroll
-    for (int a = 0; a < kMT; ++a) w[a].load(p.w, p.ldw, m0 + 16 * a + j, p.M, k, p.K);
-    const float sw = ws[b];
-#pragma unroll
-    for (int c = 0; c < kNT; ++c) {
-      const int t = t0 + 16 * c + j;
-      x[c].load(p.x, p.ldx, t, p.T, k, p.K);
-      s[c] = t < p.T ? p.xs[static_cast<long long>(b) * p.T + t] * sw : 0.f;
-    }
+    w.load(p.w, p.ldw, m0 + j, p.M, k, p.K);
+    x.load(p.x, p.ldx, t, p.T, k, p.K);
+    s = t < p.T ? p.xs[static_cast<long long>(b) * p.T + t] * ws[b] : 0.f;
   };
   int b = wave;
   if (b < nkb) fetch(b);
-  for (; b < nkb; b += kKS) {
-    MmFrag<false> wf[kMT], xf[kNT];
-    float sc[kNT];
+  for (; b < nkb; b += kRowsWaves) {
+    MmFrag<false> wf, xf;
+    wf.set(w.v[0], w.v[1]);
+    xf.set(x.v[0], x.v[1]);
+    const float sc = s;
+    if (b + kRowsWaves < nkb) fetch(b + kRowsWaves);
+    const f32x4 d = mfma_block(wf, xf);
 #pragma unroll
-    for (int a = 0; a < kMT; ++a) wf[a].set(w[a].v[0], w[a].v[1]);
-#pragma unroll
-    for (int c = 0; c < kNT; ++c) {
-      xf[c].set(x[c].v[0], x[c].v[1]);
-      sc[c] = s[c];
-    }
-    if (b + kKS < nkb) fetch(b + kKS);
-#pragma unroll
-    for (int c = 0; c < kNT; ++c)
-#pragma unroll
-      for (int a = 0; a < kMT; ++a) {
-        const f32x4 d = mfma_block(wf[a], xf[c]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[a][c][e] = __builtin_fmaf(d[e], sc[c], acc[a][c][e]);
-      }
+    for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(d[e], sc, acc[e]);
   }
-  if (wave > 0) {
-#pragma unroll
-    for (int i = 0; i < kTiles; ++i) s_part[wave - 1][i * 64 + lane] = acc[i / kNT][i % kNT];
-  }
+  if (wave > 0) s_part[wave - 1][lane] = acc;
   __syncthreads();
-  if (wave > 0) return;
+  if (wave > 0 || t >= p.T) return;
 #pragma unroll
-  for (int i = 0; i < kTiles; ++i)
-#pragma unroll
-    for (int q = 0; q < kKS - 1; ++q) acc[i / kNT][i % kNT] += s_part[q][i * 64 + lane];
+  for (int q = 0; q < kRowsWaves - 1; ++q) acc += s_part[q][lane];
   // Lane: column t of the tile, 4 rows of W.
   out_t* __restrict__ C = static_cast<out_t*>(p.c);
+  const int m = m0 + 4 * g;
+  out_t v[4];
 #pragma unroll
-  for (int c = 0; c < kNT; ++c) {
-    const int t = t0 + 16 * c + j;
-    if (t >= p.T) continue;
+  for (int e = 0; e < 4; ++e) store_as(&v[e], acc[e]);
+  if (p.token_major && m + 4 <= p.M) {
+    __builtin_memcpy(C + t * p.ldc + m, v, sizeof(v));
+  } else {
 #pragma unroll
-    for (int a = 0; a < kMT; ++a) {
-      const int m = m0 + 16 * a + 4 * g;
-      out_t v[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) store_as(&v[e], acc[a][c][e]);
-      if (p.token_major && m + 4 <= p.M) {
-        __builtin_memcpy(C + t * p.ldc + m, v, sizeof(v));
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (m + e < p.M) C[p.token_major ? t * p.ldc + m + e : (m + e) * p.ldc + t] = v[e];
-      }
-    }
+    for (int e = 0; e < 4; ++e)
+      if (m + e < p.M) C[p.token_major ? t * p.ldc + m + e : (m + e) * p.ldc + t] = v[e];
   }
 }
 
-template <int kMT, int kNT, int kKS>
 static void launch_rows(const Fp8MmParams& p, hipStream_t stream) {
-  const dim3 grid((p.M + 16 * kMT - 1) / (16 * kMT), (p.T + 16 * kNT - 1) / (16 * kNT));
-  if (p.out_bf16) hipLaunchKernelGGL((fp8mm_rows_kernel<kMT, kNT, kKS, bf16_t>), grid, dim3(64 * kKS), 0, stream, p);
-  else hipLaunchKernelGGL((fp8mm_rows_kernel<kMT, kNT, kKS, float>), grid, dim3(64 * kKS), 0, stream, p);
+  const dim3 grid((p.M + 15) / 16, (p.T + 15) / 16), block(64 * kRowsWaves);
+  if (p.out_bf16) hipLaunchKernelGGL(fp8mm_rows_kernel<bf16_t>, grid, block, 0, stream, p);
+  else hipLaunchKernelGGL(fp8mm_rows_kernel<float>, grid, block, 0, stream, p);
 }
 
 // ------------------------------------------------------------------------------ large products
@@ -460,36 +426,28 @@ static void launch_tiles(const Fp8MmParams& p, hipStream_t stream) {
 typedef MmShape<128, 128, 2, 2> MmLarge;
 typedef MmShape<64, 64, 1, 4> MmSmall;
 
-// Which kernel: the one whose time, by the sums below, is the least. Rows: what the workgroups read,
-// or their number where they have little to read, and a wave's blocks one after the other. Tiles:
-// the blocks of K one after the other, a block's time by how many tiles share a CU; a block that is
-// not whole comes last and unstaged. Measured (us, M x K x T: rows 1 x 1 of eight waves, rows 2 x 1 of
-// four, tiles of 64, tiles of 128):
-//   5120 x 1280 x 1        3.8   4.8    -     -      1280 x 2560 x 333   19.0  16.6   9.8  17.5
-//   5120 x 1280 x 8        4.1   5.0   5.6    -      5120 x 1280 x 1024   108  71.5  15.1  12.4
-//   50280 x 768 x 8 (f32) 12.8  10.3  10.8    -      1280 x 2560 x 2048  94.3  70.1  14.2  17.5
-//   1280 x 2560 x 64       6.9   7.7   9.1  17.0     5120 x 1280 x 16384    -     -   182   130
-//   64 x 64 x 16384       13.4   7.6   4.1    -      the same (f32)         -     -   307   356
+// Which kernel: the one whose time, by the sums below, is less. Rows: what the workgroups read, or
+// their number where they have little to read, and a wave's blocks one after the other. Tiles: the
+// blocks of K one after the other, a block's time by how many tiles share a CU; a block that is
+// not whole comes last and unstaged. Measured (us, M x K x T: rows, tiles of 64, tiles of 128):
+//   5120 x 1280 x 1         3.8     -     -      1280 x 2560 x 333    19.0   9.8  17.5
+//   5120 x 1280 x 8         4.1   5.6     -      5120 x 1280 x 1024    108  15.1  12.4
+//   50280 x 768 x 8 (f32)  12.8  10.8     -      1280 x 2560 x 2048   94.3  14.2  17.5
+//   1280 x 2560 x 64        6.9   9.1  17.0      5120 x 1280 x 16384     -   182   130
+//   64 x 64 x 16384        13.4   4.1     -      the same (f32)          -   307   356
 // 130 us are 1.65 PFLOP/s; the library's product with one scale an operand reaches 3.0 at 8192^3.
 hipError_t launch_fp8mm(const Fp8MmParams& p, hipStream_t stream) {
   const double nkb = (p.K + kFp8Block - 1) / kFp8Block;
-  const auto tiles = [&](double m, double t) { return __builtin_ceil(p.M / m) * __builtin_ceil(p.T / t); };
-  const double n11 = tiles(16, 16), n21 = tiles(32, 16), n64 = tiles(64, 64);
-  const double rows11 = 2.5 + fmax(0.00044 * n11 * nkb, 0.0026 * n11) + 0.09 * nkb;
-  const double rows21 = 2.5 + fmax(0.00072 * n21 * nkb, 0.0025 * n21) + 0.18 * nkb;
-  const double tiles64 = 2 + (p.out_bf16 ? fmax(0.38, 0.0009 * n64) : fmax(0.55, 0.0015 * n64)) * nkb +
-                         (p.K % kFp8Block ? 3 : 0);
-  const bool far = p.ldw >= 1 << 24 || p.ldx >= 1 << 24;  // the tiles' offsets have 32 bits
-  if (far || tiles64 > fmin(rows11, rows21)) {
-    if (rows11 <= rows21) launch_rows<1, 1, 8>(p, stream);
-    else launch_rows<2, 1, 4>(p, stream);
-  } else if (!p.out_bf16) {
-    launch_tiles<MmSmall, false, float>(p, stream);
-  } else if (tiles(128, 128) < 256) {
-    launch_tiles<MmSmall, true, bf16_t>(p, stream);
-  } else {
-    launch_tiles<MmLarge, true, bf16_t>(p, stream);
-  }
+  const auto tiles = [&](double n) { return __builtin_ceil(p.M / n) * __builtin_ceil(p.T / n); };
+  const double rows = 2.5 + fmax(0.00044 * tiles(16) * nkb, 0.0026 * tiles(16)) + 0.09 * nkb;
+  const double small = 2 + (p.out_bf16 ? fmax(0.38, 0.0009 * tiles(64)) : fmax(0.55, 0.0015 * tiles(64))) * nkb +
+                       (p.K % kFp8Block ? 3 : 0);
+  // the tiles' offsets and their number have 32 bits
+  const bool far = p.ldw >= 1 << 24 || p.ldx >= 1 << 24 || tiles(64) > 2e9;
+  if (far || rows < small) launch_rows(p, stream);
+  else if (!p.out_bf16) launch_tiles<MmSmall, false, float>(p, stream);
+  else if (tiles(128) < 256) launch_tiles<MmSmall, true, bf16_t>(p, stream);
+  else launch_tiles<MmLarge, true, bf16_t>(p, stream);
   return hipGetLastError();
 }
 
