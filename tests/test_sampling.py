@@ -231,3 +231,36 @@ def test_empty_and_repeated():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, sample_tokens(x, u, **kw))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [60000, 70001])
+@pytest.mark.parametrize("kw", [dict(top_p=0.95, temperature=3.0), dict(top_k=3000, top_p=0.9), dict(top_k=12000),
+                                dict(top_k=40000, top_p=0.5, temperature=2.0), dict(min_p=1e-6, top_p=0.97, temperature=2.0),
+                                dict(top_p=0.999), dict(top_k=2870, min_p=0.001), dict(min_p=1e-7),
+                                dict(top_p=0.6, temperature=50.0), dict(top_k=300, temperature=20.0)], ids=str)
+def test_long_prefixes(vocab, kw, dtype):
+    """Prefixes longer than the list holds, and those near its length, in rows that stay in registers
+    and rows that do not."""
+    x, u = logits_of(3, vocab, dtype, seed=vocab)
+    check(x, u, sample_tokens(x, u, **kw), **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [50000, 100000])
+def test_sorted_and_equal_words(vocab):
+    """Words in order of their logits (all of the largest in one place), whole stretches alike."""
+    x = torch.empty(6, vocab, device="cuda")
+    x[0] = torch.linspace(5, -5, vocab)
+    x[1] = torch.linspace(-5, 5, vocab)
+    x[2] = 1.0
+    x[3] = torch.arange(vocab, device="cuda").div(7, rounding_mode="floor").remainder(11).float()
+    x[4] = -3.0
+    x[4, 17:400] = 2.0
+    x[5] = -math.inf
+    x[5, ::2] = 0.25
+    u = torch.tensor([0.1, 0.9, 0.5, 0.3, 0.7, 0.999], device="cuda")
+    for kw in (dict(), dict(top_k=50), dict(top_k=1000, top_p=0.5), dict(top_p=0.8), dict(min_p=0.1), dict(top_k=200),
+               dict(top_p=0.3, min_p=0.5, temperature=0.5)):
+        check(x, u, sample_tokens(x, u, **kw), **kw)
