@@ -15,7 +15,7 @@
 // One workgroup a row. The filters keep a prefix of the order, so they come down to one cut: a
 // logit, and the last index kept among the words with that logit. Nothing is sorted:
 //
-//   1. the largest logit, and the largest of 3072 groups of the row. The k-th largest of those is a
+//   1. the largest logit, and the largest of each of three groups a thread. The k-th largest of those is a
 //      bound that k words reach and few others do; min-p is a bound by itself.
 //   2. the words that reach the bound go into a list in LDS, and the cuts and the draw are found in
 //      the list: its weights added into 2048 bins (by logit, or by index for the draw), the bin
