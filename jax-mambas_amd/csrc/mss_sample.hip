@@ -15,18 +15,21 @@
 // One workgroup a row. The filters keep a prefix of the order, so they come down to one cut: a
 // logit, and the last index kept among the words with that logit. Nothing is sorted:
 //
-//   1. the largest logit, and the largest of each of three groups a thread. The k-th largest of those is a
-//      bound that k words reach and few others do; min-p is a bound by itself.
+//   1. the largest logit, and the largest of each of three groups a thread. The k-th largest of
+//      those is a bound that k words reach and few others do; min-p is a bound by itself.
 //   2. the words that reach the bound go into a list in LDS, and the cuts and the draw are found in
 //      the list: its weights added into 2048 bins (by logit, or by index for the draw), the bin
 //      in which the sum reaches its target, and the few words of that bin one by one.
+//      (A row of more words than registers hold is read once for both, its bound taken from its
+//      first 16384 words.)
 //   3. without such a bound, or when more words reach it than the list holds, the bins are filled
 //      from the whole row, and the draw adds the words left by segments of 512.
 //   4. where one bin holds too many words (ties), a radix selection on the logits' order in
 //      integers takes any row, three passes of 11 bits.
 //
 // Weights are added as integers of 2^-43, which makes every sum exact and independent of its
-// order: at most 2^20 words a row keep it below 2^63.
+// order: at most 2^20 words a row keep it below 2^63. (The one pass adds a thread's weights in
+// float64, in the row's order, and makes that an integer.)
 #include <hip/hip_runtime.h>
 
 #include "mss_serve.h"
@@ -66,6 +69,11 @@ constexpr uint32_t kAbsent = 0x007fffffu;  // order_key(-inf)
 // which is no unit of the sums.
 struct FastWeight {
   float m, c, c_lo, least;
+  __device__ __forceinline__ FastWeight(float max, float temperature, float c_) : m(max), c(c_) {
+    // what c = log2(e) / temperature lacks (log2(e) = 1.442695022 + 1.92596e-8)
+    c_lo = (__builtin_fmaf(-c, temperature, 1.442695022f) + 1.92596301e-8f) / temperature;
+    least = -64.f / c;
+  }
   __device__ __forceinline__ float operator()(float v) const {
     const float d = fmaxf(v - m, least);
     const float y = d * c;
@@ -614,17 +622,101 @@ __device__ __forceinline__ u64 draw_of(double u, u64 total) {
   return at >= total ? total - 1 : at;
 }
 
+// A logit that all words of the bins up to `bin` reach.
+__device__ __forceinline__ float low_of_bin(const ByLogit& order, uint32_t bin, float m, float least) {
+  return bin < kSampleBins && order.scale > 0.f ? fmaxf(least, m - (bin + 1.01f) / order.scale) : least;
+}
+// The share of a row's words whose list top-p's prefix is guessed to lie in.
+__device__ __forceinline__ float share_of(float top_p, int vocab) {
+  return fminf(top_p <= 0.6f ? 0.005f : top_p <= 0.85f ? 0.02f : top_p <= 0.92f ? 0.05f : 0.1f,
+               kSampleList * 0.85f / vocab);
+}
+
+// The list made in one pass, of a row that is not held: the bound comes from the first two chunks
+// (top-p's prefix is guessed at also where min-p would bound the list: some rows' first chunks have
+// no large logit), the weights of the row's sum are relative to their largest logit and are put right
+// when the row's is known. 256 x 131072 float32: top-k 50 45 us with a pass for the largest logit and
+// one for the list, 36 with one; top-p 0.9 64 and 48, with min-p 0.001 58 and 50.
+struct OnePass {
+  bool done;       // else the list does not hold the words, or the row is none to do this with
+  bool nan;
+  float m, low;    // the row's largest logit, and the bound
+  u64 all;
+};
+template <typename words_t>
+__device__ __forceinline__ OnePass list_in_one_pass(SampleShared& s, const words_t& words, float temperature, float c,
+                                                    int top_k, float top_p, float min_p) {
+  const int vocab = words.row.vocab;
+  const bool by_k = top_k > 0 && top_k < vocab, by_p = top_p < 1.f, by_m = min_p > 0.f;
+  OnePass out{false, false, 0.f, 0.f, 0};
+  float most[2] = {-__builtin_inff(), -__builtin_inff()};
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    float v[8];
+    words.row.load8(q * kSampleChunk + threadIdx.x * 8, v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) most[q] = fmaxf(most[q], v[k]);
+  }
+  const auto top_of = [&](float v) {
+    uint32_t top = wave_max(order_key(v));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s.wave[threadIdx.x >> 6] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kSampleWaves; ++i) top = max(top, static_cast<uint32_t>(s.wave[i]));
+    return key_value(top);
+  };
+  const float m = top_of(fmaxf(most[0], most[1])), least = m - 46.f / c;
+  if (!(least > -__builtin_inff() && m < __builtin_inff())) return out;
+  out.low = by_m ? fmaxf(least, m + (__builtin_amdgcn_logf(min_p) - 0.01f) / c) : least;
+  {
+    const ByLogit order(m, least);
+    clear_bins(s);
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      if (most[q] >= least) atomicAdd(reinterpret_cast<uint32_t*>(&s.mass[order.bin(most[q], 0)]), 1u);
+    const float guess = share_of(by_p ? top_p : 1.f, vocab) * 8;  // words a group
+    const int k = by_k ? top_k : max(1, static_cast<int>(2 * kSampleThreads * (1.f - __builtin_amdgcn_exp2f(-guess / kLn2))));
+    uint32_t bin;
+    u64 before, target;
+    reach_bin(s, [&](u64) -> u64 { return k; }, bin, before, target);
+    const float reach = low_of_bin(order, bin, m, least);
+    if (!by_k && !by_p && reach > out.low) return out;  // min-p alone needs all of its words
+    out.low = fmaxf(reach, by_k && by_p ? least : out.low);
+  }
+  if (threadIdx.x == 0) s.list_n = 0;
+  __syncthreads();
+  const FastWeight weight(m, temperature, c);
+  const bool whole = by_p && !by_k;
+  double all = 0;
+  float mine = m;
+  bool nan = false;
+  words.each([&](const float (&v)[8], int i, int, auto) {
+    append(s, v, i, [&](float x, int) { return x >= out.low; });
+#pragma unroll
+    for (int k = 0; k < 8; k += 2) {
+      mine = fmaxf(fmaxf(mine, v[k]), v[k + 1]);
+      nan |= __builtin_isunordered(v[k], v[k + 1]);
+    }
+    if (whole) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) all += static_cast<double>(weight(v[k]));
+    }
+  });
+  out.m = top_of(mine);
+  out.nan = __syncthreads_or(nan);
+  const FastWeight shift(out.m, temperature, c);
+  if (whole) out.all = block_total(s, static_cast<u64>(all * (static_cast<double>(shift(m)) * kFixed)));
+  out.done = s.list_n <= kSampleList && (out.m - m) * c < 60.f;
+  return out;
+}
+
 // The token, or -1 where a bin holds too many words to look at one by one.
 template <typename words_t>
-__device__ __forceinline__ int draw_by_bins(SampleShared& s, const words_t& words, const float (&most)[3], float m, float temperature,
-                                            float c, int top_k, float top_p, float min_p, double u) {
+__device__ __forceinline__ int draw_by_bins(SampleShared& s, const words_t& words, const float (&most)[3], const OnePass& made,
+                                            float m, float temperature, float c, int top_k, float top_p, float min_p, double u) {
   const int vocab = words.row.vocab;
-  FastWeight weight;
-  weight.m = m;
-  weight.c = c;
-  // what c = log2(e) / temperature lacks (log2(e) = 1.442695022 + 1.92596e-8)
-  weight.c_lo = (__builtin_fmaf(-c, temperature, 1.442695022f) + 1.92596301e-8f) / temperature;
-  weight.least = -64.f / c;
+  const FastWeight weight(m, temperature, c);
   const auto fixed = [&](float v) { return biased_fixed(weight(v)) - kFixedBias; };
   const bool by_k = top_k > 0 && top_k < vocab, by_p = top_p < 1.f, by_m = min_p > 0.f;
   // Words below `least` weigh nothing. (At a high temperature that is far below them all.)
@@ -651,9 +743,7 @@ __device__ __forceinline__ int draw_by_bins(SampleShared& s, const words_t& word
   // without min-p the bound is a guess at its prefix: one that a share of the words reaches which
   // grows with top_p. (Rows in registers need no guess: their bins are filled from the whole row.)
   const ByLogit order(m, least);
-  const auto low_of = [&](uint32_t bin) {  // a logit that all words of the bins up to it reach
-    return bin < kSampleBins && order.scale > 0.f ? fmaxf(least, m - (bin + 1.01f) / order.scale) : least;
-  };
+  const auto low_of = [&](uint32_t bin) { return low_of_bin(order, bin, m, least); };
   const int groups = min(kSampleGroups, (vocab + 7) / 8);
   const bool listed = by_k ? top_k <= kSampleGroups * 15 / 16 : by_m || (by_p && !words_t::kHeld);
   const bool whole = listed && by_p && !by_k;
@@ -661,15 +751,18 @@ __device__ __forceinline__ int draw_by_bins(SampleShared& s, const words_t& word
   float low = m_bound;
   u64 all = 0;
   Cut cut{-__builtin_inff(), 0x7fffffff};
-  if (listed) {
+  if (made.done) {
+    n = s.list_n;
+    low = made.low;
+    all = made.all;
+  } else if (listed) {
     if (threadIdx.x == 0) s.list_n = 0;
     if (by_k || !by_m) {
       clear_bins(s);
 #pragma unroll
       for (int q = 0; q < 3; ++q)
         if (most[q] >= least) atomicAdd(reinterpret_cast<uint32_t*>(&s.mass[order.bin(most[q], 0)]), 1u);
-      const float share = top_p <= 0.6f ? 0.005f : top_p <= 0.85f ? 0.02f : top_p <= 0.92f ? 0.05f : 0.1f;
-      const float guess = fminf(share * vocab, kSampleList * 0.85f) / groups;  // words a group
+      const float guess = share_of(top_p, vocab) * vocab / groups;  // words a group
       const int k = by_k ? top_k : max(1, static_cast<int>(groups * (1.f - __builtin_amdgcn_exp2f(-guess / kLn2))));
       uint32_t bin;
       u64 before, target;
@@ -700,7 +793,7 @@ __device__ __forceinline__ int draw_by_bins(SampleShared& s, const words_t& word
     if (by_p) {
       const u64 here = block_total(s, keep ? mine.w : 0), target = reach_of(top_p, whole ? all : here);
       keep = keep && before < target;
-      found = target <= here || (by_m && low == m_bound);
+      found = target <= here || (by_m && low <= m_bound);
     }
     if (found) {
       keep = keep && !(weight(mine.v) < min_p);
@@ -738,7 +831,7 @@ __device__ __forceinline__ int draw_by_bins(SampleShared& s, const words_t& word
         if (!pick(s, n, order, kept, [&](u64) { return target; }, to.v, to.i)) return -1;
         cut = to;
       } else {
-        found = by_m && low == m_bound;  // all of min-p's words are here, and top-p leaves more
+        found = by_m && low <= m_bound;  // all of min-p's words are here, and top-p leaves more
       }
     }
     if (found) return draw_listed(n);
@@ -861,6 +954,27 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleParams p) 
   const float min_p = p.min_ps ? p.min_ps[r] : p.min_p;
   const double u = static_cast<double>(p.uniform[r]);
 
+  const float c = 1.442695022f / temperature;
+  OnePass made{false, false, 0.f, 0.f, 0};
+  if constexpr (!kReg) {
+    // (top-k's words: eight times as many and more reach the bound that the first chunks give them)
+    const bool by_k = top_k > 0 && top_k < p.vocab;
+    const bool fits = by_k ? static_cast<long long>(top_k) * p.vocab <= kSampleList * 3ll / 4 * kSampleChunk && top_k <= kSampleThreads
+                           : top_p < 1.f || min_p > 0.f;
+    if (fits && temperature > 0.f && top_k != 1 && !(min_p > 1.f) && c >= 0.25f && c < 0x1p100f)
+      made = list_in_one_pass(s, words, temperature, c, top_k, top_p, min_p);
+    __syncthreads();  // s.wave has been read
+  }
+  if (made.done) {
+    const float none[3] = {};
+    const int token = made.nan ? -1 : draw_by_bins(s, words, none, made, made.m, temperature, c, top_k, top_p, min_p, u);
+    if (token >= 0 || made.nan) {
+      if (threadIdx.x == 0) p.tokens[r] = token;
+      return;
+    }
+    __syncthreads();
+  }
+
   // The largest logit of each group, and whether any is NaN.
   float most[3] = {-__builtin_inff(), -__builtin_inff(), -__builtin_inff()};
   bool nan = false;
@@ -898,9 +1012,9 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleParams p) 
     if (threadIdx.x == 0) p.tokens[r] = s.index;
     return;
   }
-  const float m = key_value(top), c = 1.442695022f / temperature;
+  const float m = key_value(top);
   if (m < __builtin_inff() && c > 0x1p-100f && c < 0x1p100f && m - 46.f / c > -__builtin_inff()) {
-    const int token = draw_by_bins(s, words, most, m, temperature, c, top_k, top_p, min_p, u);
+    const int token = draw_by_bins(s, words, most, OnePass{}, m, temperature, c, top_k, top_p, min_p, u);
     if (token >= 0) {
       if (threadIdx.x == 0) p.tokens[r] = token;
       return;

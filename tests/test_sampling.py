@@ -264,3 +264,25 @@ def test_sorted_and_equal_words(vocab):
     for kw in (dict(), dict(top_k=50), dict(top_k=1000, top_p=0.5), dict(top_p=0.8), dict(min_p=0.1), dict(top_k=200),
                dict(top_p=0.3, min_p=0.5, temperature=0.5)):
         check(x, u, sample_tokens(x, u, **kw), **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [65537, 70001, 131072, 262147])
+def test_long_rows_whose_beginning_differs(vocab, dtype):
+    """Rows too long for registers whose first words say little of the rest: none there, all small or
+    large there, the largest at the end, an infinity or a NaN late."""
+    x, _ = logits_of(10, vocab, dtype, seed=vocab)
+    x[1, :20000] = -math.inf
+    x[2, :20000] -= 30
+    x[3, :20000] += 12
+    x[4, vocab - 1] = x[4].max() + 1
+    x[5, vocab - 1] = 90.0
+    x[6, :16384] = x[6, :16384].clamp(max=-1.0)
+    x[7, 40000:] = -math.inf
+    x[8, vocab - 2] = math.inf
+    x[9, vocab - 3] = math.nan
+    u = torch.linspace(0.02, 0.97, 10, device="cuda")
+    for kw in (dict(top_p=0.9, min_p=0.001), dict(top_p=0.9), dict(top_k=50), dict(top_k=700, top_p=0.8), dict(min_p=0.02),
+               dict(min_p=1e-6), dict(top_p=0.5, temperature=0.3), dict(top_k=1000, min_p=0.01, temperature=0.05)):
+        check(x, u, sample_tokens(x, u, **kw), **kw)
