@@ -193,9 +193,11 @@ static void launch_rows(const Fp8MmParams& p, hipStream_t stream) {
 __device__ __forceinline__ int r_key(int row) { return ((row >> 3) & 6) | ((row >> 1) & 1); }
 __device__ __forceinline__ int q_key(int row) { return (row >> 1) & 7; }
 
-template <int kBR_, int kBQ_, int kWR_, int kWQ_>
+template <int kBR_, int kBQ_, int kWR_, int kWQ_, int kParts_ = 1>
 struct MmShape {
+  // kParts: teams of kWaves waves that share a tile, each taking every kParts-th block of K.
   static constexpr int kBR = kBR_, kBQ = kBQ_, kWR = kWR_, kWQ = kWQ_, kWaves = kWR * kWQ, kThreads = 64 * kWaves;
+  static constexpr int kParts = kParts_;
   static constexpr int kRT = kBR / kWR / 16, kQT = kBQ / kWQ / 16;  // 16 x 16 tiles of a wave
   static constexpr int kRCopies = kBR * 8 / kThreads, kQCopies = kBQ * 8 / kThreads;
   static_assert(kRT % 4 == 0 &&  kBR * 8 % kThreads == 0 &&
@@ -211,14 +213,16 @@ struct MmOperand {
 };
 
 template <typename S, bool kF8, typename out_t, bool kTokenRows>
-__global__ __launch_bounds__(S::kThreads, 2) void fp8mm_tile_kernel(Fp8MmParams p, int tiles_r, int tiles_q) {
+__global__ __launch_bounds__(S::kThreads * S::kParts, 2) void fp8mm_tile_kernel(Fp8MmParams p, int tiles_r, int tiles_q) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host's pass knows no buffer resources
   constexpr int kToks = kTokenRows ? S::kBR : S::kBQ;
   // A stage: R's rows, Q's rows, the tokens' scales.
   constexpr int kSlots = 8 * (S::kBR + S::kBQ) + kToks / 4;
-  __shared__ u32x4 s0[kSlots], s1[kSlots];
+  __shared__ u32x4 s_even[S::kParts * kSlots], s_odd[S::kParts * kSlots];
   const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int part = S::kParts > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / S::kThreads) : 0;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) - part * S::kWaves;
+  u32x4 *const s0 = s_even + part * kSlots, *const s1 = s_odd + part * kSlots;
   const int wr = wave % S::kWR, wq = wave / S::kWR;
   const MmOperand R = kTokenRows ? MmOperand{p.x, p.ldx, p.T} : MmOperand{p.w, p.ldw, p.M};
   const MmOperand Q = kTokenRows ? MmOperand{p.w, p.ldw, p.M} : MmOperand{p.x, p.ldx, p.T};
@@ -349,36 +353,54 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp8mm_tile_kernel(Fp8MmParams 
     asm volatile("" ::: "memory");
   };
   const int full = p.K / kFp8Block;
-  if (full > 0) issue(0, s0);
-  for (int b = 0; b + 1 < full; b += 2) {
+  if (part < full) issue(part, s0);
+  for (int first = 0; first < full; first += 2 * S::kParts) {  // (the teams meet equally often)
+    const int b = first + part;
     meet();
-    issue(b + 1, s1);
-    compute(s0, ws[b]);
+    if (b + S::kParts < full) issue(b + S::kParts, s1);
+    if (b < full) compute(s0, ws[b]);
+    if (first + S::kParts >= full) break;
     meet();
-    if (b + 2 < full) issue(b + 2, s0);
-    compute(s1, ws[b + 1]);
-  }
-  if (full & 1) {
-    meet();
-    compute(s0, ws[full - 1]);
+    if (b + 2 * S::kParts < full) issue(b + 2 * S::kParts, s0);
+    if (b + S::kParts < full) compute(s1, ws[b + S::kParts]);
   }
   if (full < nkb) {  // the features past K are zeros, whatever lies in the rows' padding
     const int k0 = full * kFp8Block;
     meet();
-    issue_scales(full, s0);
+    if (part == 0) {
+      issue_scales(full, s0);
 #pragma unroll 1
-    for (int t = 0; t < S::kRCopies; ++t) {
-      const int i = wave + S::kWaves * t, row = 8 * i + (lane >> 3);
-      s0[64 * i + lane] = load_chunk(R.base, R.ld, min(r0 + row, R.rows - 1), R.rows, k0 + 16 * ((lane & 7) ^ r_key(row)), p.K);
-    }
+      for (int t = 0; t < S::kRCopies; ++t) {
+        const int i = wave + S::kWaves * t, row = 8 * i + (lane >> 3);
+        s0[64 * i + lane] = load_chunk(R.base, R.ld, min(r0 + row, R.rows - 1), R.rows, k0 + 16 * ((lane & 7) ^ r_key(row)), p.K);
+      }
 #pragma unroll 1
-    for (int t = 0; t < S::kQCopies; ++t) {
-      const int i = wave + S::kWaves * t, row = 8 * i + (lane >> 3);
-      s0[8 * S::kBR + 64 * i + lane] =
-          load_chunk(Q.base, Q.ld, min(q0 + row, Q.rows - 1), Q.rows, k0 + 16 * ((lane & 7) ^ q_key(row)), p.K);
+      for (int t = 0; t < S::kQCopies; ++t) {
+        const int i = wave + S::kWaves * t, row = 8 * i + (lane >> 3);
+        s0[8 * S::kBR + 64 * i + lane] =
+            load_chunk(Q.base, Q.ld, min(q0 + row, Q.rows - 1), Q.rows, k0 + 16 * ((lane & 7) ^ q_key(row)), p.K);
+      }
     }
     meet();
-    compute(s0, ws[full]);
+    if (part == 0) compute(s0, ws[full]);
+  }
+  if constexpr (S::kParts > 1) {  // the teams' sums, in a fixed order
+    constexpr int kSums = S::kRT * S::kQT * S::kThreads;
+    static_assert(sizeof(s_even) >= (S::kParts - 1) * kSums * sizeof(f32x4), "");
+    f32x4* const sums = reinterpret_cast<f32x4*>(s_even);
+    meet();
+    if (part > 0) {
+#pragma unroll
+      for (int i = 0; i < S::kRT * S::kQT; ++i)
+        sums[(part - 1) * kSums + i * S::kThreads + 64 * wave + lane] = acc[i / S::kQT][i % S::kQT];
+    }
+    meet();
+    if (part > 0) return;
+#pragma unroll
+    for (int q = 0; q + 1 < S::kParts; ++q)
+#pragma unroll
+      for (int i = 0; i < S::kRT * S::kQT; ++i)
+        acc[i / S::kQT][i % S::kQT] += sums[q * kSums + i * S::kThreads + 64 * wave + lane];
   }
 
   // A lane's 16 rows of a column.
@@ -413,38 +435,45 @@ static void launch_tiles(const Fp8MmParams& p, hipStream_t stream) {
   const int nr = p.token_major ? p.M : p.T, nq = p.token_major ? p.T : p.M;
   const int tr = (nr + S::kBR - 1) / S::kBR, tq = (nq + S::kBQ - 1) / S::kBQ;
   if (p.token_major)
-    hipLaunchKernelGGL((fp8mm_tile_kernel<S, kF8, out_t, false>), dim3(tr * tq), dim3(S::kThreads), 0, stream, p, tr, tq);
+    hipLaunchKernelGGL((fp8mm_tile_kernel<S, kF8, out_t, false>), dim3(tr * tq), dim3(S::kThreads * S::kParts), 0, stream, p, tr, tq);
   else
-    hipLaunchKernelGGL((fp8mm_tile_kernel<S, kF8, out_t, true>), dim3(tr * tq), dim3(S::kThreads), 0, stream, p, tr, tq);
+    hipLaunchKernelGGL((fp8mm_tile_kernel<S, kF8, out_t, true>), dim3(tr * tq), dim3(S::kThreads * S::kParts), 0, stream, p, tr, tq);
 }
 
 // 128 x 128 tiles, four waves of 64 x 64, two workgroups a CU, whose copies, products and stores
 // fall at different times. (256 x 256 tiles of eight waves, one workgroup a CU: 139 us against 130
 // for 5120 x 1280 x 16384, 139 against 115 for 5120 x 5120 x 4096.) 64 x 64 tiles, four waves of
 // 64 x 16, four workgroups a CU, where there are fewer than 256 of the large ones, and for all float32
-// outputs. (A ring of four stages instead of two: 11.2 us against 9.8 for 1280 x 2560 x 333.)
+// outputs. With at most one of those a CU and eight blocks or more, two teams of four waves take every
+// other block: twice the copies in flight. (us, one team, two, four: 1280 x 2560 x 333 10.5, 8.8, 8.6,
+// x 128 9.7, 8.0, 7.5; 2560 x 1280 x 256 6.3, 5.8, 6.1, x 512, two tiles on some CUs, 7.2, 7.5, 10.6;
+// 768 x 128 x 1000 3.7, 4.2, 5.0. A ring of four stages instead: 11.2 for the first.)
 typedef MmShape<128, 128, 2, 2> MmLarge;
 typedef MmShape<64, 64, 1, 4> MmSmall;
+typedef MmShape<64, 64, 1, 4, 2> MmFew;
 
 // Which kernel: the one whose time, by the sums below, is less. Rows: what the workgroups read, or
 // their number where they have little to read, and a wave's blocks one after the other. Tiles: the
 // blocks of K one after the other, a block's time by how many tiles share a CU; a block that is
 // not whole comes last and unstaged. Measured (us, M x K x T: rows, tiles of 64, tiles of 128):
-//   5120 x 1280 x 1         3.8     -     -      1280 x 2560 x 333    19.0   9.8  17.5
+//   5120 x 1280 x 1         3.8     -     -      1280 x 2560 x 333    19.0   8.8  17.5
 //   5120 x 1280 x 8         4.1   5.6     -      5120 x 1280 x 1024    108  15.1  12.4
 //   50280 x 768 x 8 (f32)  12.8  10.8     -      1280 x 2560 x 2048   94.3  14.2  17.5
-//   1280 x 2560 x 64        6.9   9.1  17.0      5120 x 1280 x 16384     -   182   130
+//   1280 x 2560 x 64        6.9   7.9  17.0      5120 x 1280 x 16384     -   182   130
 //   64 x 64 x 16384        13.4   4.1     -      the same (f32)          -   307   356
 // 130 us are 1.65 PFLOP/s; the library's product with one scale an operand reaches 3.0 at 8192^3.
 hipError_t launch_fp8mm(const Fp8MmParams& p, hipStream_t stream) {
   const double nkb = (p.K + kFp8Block - 1) / kFp8Block;
   const auto tiles = [&](double n) { return __builtin_ceil(p.M / n) * __builtin_ceil(p.T / n); };
   const double rows = 2.5 + fmax(0.00044 * tiles(16) * nkb, 0.0026 * tiles(16)) + 0.09 * nkb;
-  const double small = 2 + (p.out_bf16 ? fmax(0.38, 0.0009 * tiles(64)) : fmax(0.55, 0.0015 * tiles(64))) * nkb +
+  const bool few = tiles(64) <= 256 && nkb >= 8;
+  const double small = 2 + (p.out_bf16 ? fmax(few ? 0.33 : 0.38, 0.0009 * tiles(64)) : fmax(0.55, 0.0015 * tiles(64))) * nkb +
                        (p.K % kFp8Block ? 3 : 0);
   // the tiles' offsets and their number have 32 bits
   const bool far = p.ldw >= 1 << 24 || p.ldx >= 1 << 24 || tiles(64) > 2e9;
   if (far || rows < small) launch_rows(p, stream);
+  else if (few && p.out_bf16) launch_tiles<MmFew, true, bf16_t>(p, stream);
+  else if (few) launch_tiles<MmFew, false, float>(p, stream);
   else if (!p.out_bf16) launch_tiles<MmSmall, false, float>(p, stream);
   else if (tiles(128) < 256) launch_tiles<MmSmall, true, bf16_t>(p, stream);
   else launch_tiles<MmLarge, true, bf16_t>(p, stream);

@@ -480,3 +480,12 @@ def test_quantise_borders():
         q, _ = quantize_fp8(x.repeat(1, wide).to(torch.bfloat16) if wide == 1 else x.repeat(1, wide))
         v = q.float()[:5]
         assert torch.all(v[:, 0] == 448) and torch.all(v[:, 1] == 20) and torch.all(v[:, 2] == -80) and torch.all(v[:, 3] == 9)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("token_major", [False, True])
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,k,t", [(1000, 1024, 200), (500, 1025, 150), (260, 1151, 900), (130, 2688, 700), (1024, 1920, 1024)])
+def test_matmul_few_tiles_many_blocks(m, k, t, out_dtype, token_major):
+    """Few tiles of C with 8 to 21 blocks of K, even and odd in number, whole and not."""
+    test_matmul(m, k, t, out_dtype, token_major)
