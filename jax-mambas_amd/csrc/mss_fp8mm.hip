@@ -216,8 +216,8 @@ template <typename S, bool kF8, typename out_t, bool kTokenRows>
 __global__ __launch_bounds__(S::kThreads * S::kParts, 2) void fp8mm_tile_kernel(Fp8MmParams p, int tiles_r, int tiles_q) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host's pass knows no buffer resources
   constexpr int kToks = kTokenRows ? S::kBR : S::kBQ;
-  // A stage: R's rows, Q's rows, the tokens' scales.
-  constexpr int kSlots = 8 * (S::kBR + S::kBQ) + kToks / 4;
+  // A stage: R's rows, Q's rows, the tokens' scales (copied 64 at a time).
+  constexpr int kSlots = 8 * (S::kBR + S::kBQ) + (kToks < 64 ? 64 : kToks) / 4;
   __shared__ u32x4 s_even[S::kParts * kSlots], s_odd[S::kParts * kSlots];
   const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
   const int part = S::kParts > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / S::kThreads) : 0;
@@ -367,19 +367,17 @@ __global__ __launch_bounds__(S::kThreads * S::kParts, 2) void fp8mm_tile_kernel(
   if (full < nkb) {  // the features past K are zeros, whatever lies in the rows' padding
     const int k0 = full * kFp8Block;
     meet();
-    if (part == 0) {
-      issue_scales(full, s0);
+    if (part == 0) issue_scales(full, s0);
 #pragma unroll 1
-      for (int t = 0; t < S::kRCopies; ++t) {
-        const int i = wave + S::kWaves * t, row = 8 * i + (lane >> 3);
-        s0[64 * i + lane] = load_chunk(R.base, R.ld, min(r0 + row, R.rows - 1), R.rows, k0 + 16 * ((lane & 7) ^ r_key(row)), p.K);
-      }
+    for (int i = wave + S::kWaves * part; i < S::kBR / 8; i += S::kWaves * S::kParts) {  // all teams for the first one
+      const int row = 8 * i + (lane >> 3);
+      s_even[64 * i + lane] = load_chunk(R.base, R.ld, min(r0 + row, R.rows - 1), R.rows, k0 + 16 * ((lane & 7) ^ r_key(row)), p.K);
+    }
 #pragma unroll 1
-      for (int t = 0; t < S::kQCopies; ++t) {
-        const int i = wave + S::kWaves * t, row = 8 * i + (lane >> 3);
-        s0[8 * S::kBR + 64 * i + lane] =
-            load_chunk(Q.base, Q.ld, min(q0 + row, Q.rows - 1), Q.rows, k0 + 16 * ((lane & 7) ^ q_key(row)), p.K);
-      }
+    for (int i = wave + S::kWaves * part; i < S::kBQ / 8; i += S::kWaves * S::kParts) {
+      const int row = 8 * i + (lane >> 3);
+      s_even[8 * S::kBR + 64 * i + lane] =
+          load_chunk(Q.base, Q.ld, min(q0 + row, Q.rows - 1), Q.rows, k0 + 16 * ((lane & 7) ^ q_key(row)), p.K);
     }
     meet();
     if (part == 0) compute(s0, ws[full]);
@@ -444,36 +442,49 @@ static void launch_tiles(const Fp8MmParams& p, hipStream_t stream) {
 // fall at different times. (256 x 256 tiles of eight waves, one workgroup a CU: 139 us against 130
 // for 5120 x 1280 x 16384, 139 against 115 for 5120 x 5120 x 4096.) 64 x 64 tiles, four waves of
 // 64 x 16, four workgroups a CU, where there are fewer than 256 of the large ones, and for all float32
-// outputs. With at most one of those a CU and eight blocks or more, two teams of four waves take every
-// other block: twice the copies in flight. (us, one team, two, four: 1280 x 2560 x 333 10.5, 8.8, 8.6,
-// x 128 9.7, 8.0, 7.5; 2560 x 1280 x 256 6.3, 5.8, 6.1, x 512, two tiles on some CUs, 7.2, 7.5, 10.6;
-// 768 x 128 x 1000 3.7, 4.2, 5.0. A ring of four stages instead: 11.2 for the first.)
+// outputs. Where they are few: four teams of two waves, each with a quarter of the blocks of K and its
+// own copies in flight, on tiles of 64 x 32 if that makes no more than one a CU, else on 64 x 64.
+// (us, one team of four waves, two, four of two, the same on 64 x 32: 1280 x 2560 x 333 10.4, 8.9, 8.2,
+// 6.7; x 128 9.6, 8.1, 7.1, 5.9; 768 x 1536 x 512 6.9, 6.2, 5.8, 5.0; 2560 x 1280 x 256 6.3, 5.8, 5.6,
+// and 7.9 with 320 tiles; x 512, 320 tiles of 64, 7.2, 7.5, 9.4. One team with a ring of three or four
+// stages: 11.8, 11.2 for the first.)
 typedef MmShape<128, 128, 2, 2> MmLarge;
 typedef MmShape<64, 64, 1, 4> MmSmall;
-typedef MmShape<64, 64, 1, 4, 2> MmFew;
+typedef MmShape<64, 64, 1, 2, 4> MmTeams;
+typedef MmShape<64, 32, 1, 2, 4> MmFew;
 
 // Which kernel: the one whose time, by the sums below, is less. Rows: what the workgroups read, or
 // their number where they have little to read, and a wave's blocks one after the other. Tiles: the
 // blocks of K one after the other, a block's time by how many tiles share a CU; a block that is
-// not whole comes last and unstaged. Measured (us, M x K x T: rows, tiles of 64, tiles of 128):
-//   5120 x 1280 x 1         3.8     -     -      1280 x 2560 x 333    19.0   8.8  17.5
-//   5120 x 1280 x 8         4.1   5.6     -      5120 x 1280 x 1024    108  15.1  12.4
+// not whole comes last and unstaged. (Teams split a block's time.) Measured (us, M x K x T: rows, tiles of 64, tiles of 128):
+//   5120 x 1280 x 1         3.8     -     -      1280 x 2560 x 333    19.0   6.7  17.5
+//   5120 x 1280 x 8         4.1   4.8     -      5120 x 1280 x 1024    108  15.1  12.4
 //   50280 x 768 x 8 (f32)  12.8  10.8     -      1280 x 2560 x 2048   94.3  14.2  17.5
-//   1280 x 2560 x 64        6.9   7.9  17.0      5120 x 1280 x 16384     -   182   130
+//   1280 x 2560 x 64        7.0   5.9  17.0      5120 x 1280 x 16384     -   182   130
 //   64 x 64 x 16384        13.4   4.1     -      the same (f32)          -   307   356
 // 130 us are 1.65 PFLOP/s; the library's product with one scale an operand reaches 3.0 at 8192^3.
 hipError_t launch_fp8mm(const Fp8MmParams& p, hipStream_t stream) {
   const double nkb = (p.K + kFp8Block - 1) / kFp8Block;
   const auto tiles = [&](double n) { return __builtin_ceil(p.M / n) * __builtin_ceil(p.T / n); };
   const double rows = 2.5 + fmax(0.00044 * tiles(16) * nkb, 0.0026 * tiles(16)) + 0.09 * nkb;
-  const bool few = tiles(64) <= 256 && nkb >= 8;
-  const double small = 2 + (p.out_bf16 ? fmax(few ? 0.33 : 0.38, 0.0009 * tiles(64)) : fmax(0.55, 0.0015 * tiles(64))) * nkb +
-                       (p.K % kFp8Block ? 3 : 0);
+  const double few_tiles = p.token_major ? __builtin_ceil(p.M / 64.) * __builtin_ceil(p.T / 32.)
+                                         : __builtin_ceil(p.T / 64.) * __builtin_ceil(p.M / 32.);
+  const bool few = few_tiles <= 256, teams = !few && tiles(64) <= 256 && nkb >= 8;
+  double block, start = 2;  // of the tiles
+  if (few) {
+    start = 3.5;
+    block = p.out_bf16 ? 0.12 + 0.0002 * few_tiles : 0.16 + 0.0004 * few_tiles;
+  } else {
+    block = p.out_bf16 ? fmax(0.38, 0.0009 * tiles(64)) : fmax(0.55, 0.0015 * tiles(64));
+  }
+  const double staged = start + block * nkb + (p.K % kFp8Block ? (few ? 1.2 : 3) : 0);
   // the tiles' offsets and their number have 32 bits
   const bool far = p.ldw >= 1 << 24 || p.ldx >= 1 << 24 || tiles(64) > 2e9;
-  if (far || rows < small) launch_rows(p, stream);
+  if (far || rows < staged) launch_rows(p, stream);
   else if (few && p.out_bf16) launch_tiles<MmFew, true, bf16_t>(p, stream);
   else if (few) launch_tiles<MmFew, false, float>(p, stream);
+  else if (teams && p.out_bf16) launch_tiles<MmTeams, true, bf16_t>(p, stream);
+  else if (teams) launch_tiles<MmTeams, false, float>(p, stream);
   else if (!p.out_bf16) launch_tiles<MmSmall, false, float>(p, stream);
   else if (tiles(128) < 256) launch_tiles<MmSmall, true, bf16_t>(p, stream);
   else launch_tiles<MmLarge, true, bf16_t>(p, stream);
