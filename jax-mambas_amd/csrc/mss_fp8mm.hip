@@ -428,14 +428,18 @@ __global__ __launch_bounds__(S::kThreads * S::kParts, 2) void fp8mm_tile_kernel(
 #endif
 }
 
-template <typename S, bool kF8, typename out_t>
+template <typename S, bool kF8, typename out_t, bool kBothLayouts = true>
 static void launch_tiles(const Fp8MmParams& p, hipStream_t stream) {
   const int nr = p.token_major ? p.M : p.T, nq = p.token_major ? p.T : p.M;
   const int tr = (nr + S::kBR - 1) / S::kBR, tq = (nq + S::kBQ - 1) / S::kBQ;
-  if (p.token_major)
-    hipLaunchKernelGGL((fp8mm_tile_kernel<S, kF8, out_t, false>), dim3(tr * tq), dim3(S::kThreads * S::kParts), 0, stream, p, tr, tq);
-  else
-    hipLaunchKernelGGL((fp8mm_tile_kernel<S, kF8, out_t, true>), dim3(tr * tq), dim3(S::kThreads * S::kParts), 0, stream, p, tr, tq);
+  const dim3 grid(tr * tq), threads(S::kThreads * S::kParts);
+  if constexpr (kBothLayouts) {
+    if (!p.token_major) {
+      hipLaunchKernelGGL((fp8mm_tile_kernel<S, kF8, out_t, true>), grid, threads, 0, stream, p, tr, tq);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((fp8mm_tile_kernel<S, kF8, out_t, false>), grid, threads, 0, stream, p, tr, tq);
 }
 
 // 128 x 128 tiles, four waves of 64 x 64, two workgroups a CU, whose copies, products and stores
@@ -447,11 +451,14 @@ static void launch_tiles(const Fp8MmParams& p, hipStream_t stream) {
 // (us, one team of four waves, two, four of two, the same on 64 x 32: 1280 x 2560 x 333 10.4, 8.9, 8.2,
 // 6.7; x 128 9.6, 8.1, 7.1, 5.9; 768 x 1536 x 512 6.9, 6.2, 5.8, 5.0; 2560 x 1280 x 256 6.3, 5.8, 5.6,
 // and 7.9 with 320 tiles; x 512, 320 tiles of 64, 7.2, 7.5, 9.4. One team with a ring of three or four
-// stages: 11.8, 11.2 for the first.)
+// stages: 11.8, 11.2 for the first.) Up to 32 tokens in rows of their own: one team of two waves on
+// 64 x 32, where fewer rows of tokens that are not there are copied (50280 x 768 x 8 in float32 11.1 us on 64 x 64,
+// 9.0; x 32 12.6, 12.0; 32000 x 2048 x 8 13.7, 12.3).
 typedef MmShape<128, 128, 2, 2> MmLarge;
 typedef MmShape<64, 64, 1, 4> MmSmall;
 typedef MmShape<64, 64, 1, 2, 4> MmTeams;
 typedef MmShape<64, 32, 1, 2, 4> MmFew;
+typedef MmShape<64, 32, 1, 2> MmThin;
 
 // Which kernel: the one whose time, by the sums below, is less. Rows: what the workgroups read, or
 // their number where they have little to read, and a wave's blocks one after the other. Tiles: the
@@ -459,7 +466,7 @@ typedef MmShape<64, 32, 1, 2, 4> MmFew;
 // not whole comes last and unstaged. (Teams split a block's time.) Measured (us, M x K x T: rows, tiles of 64, tiles of 128):
 //   5120 x 1280 x 1         3.8     -     -      1280 x 2560 x 333    19.0   6.7  17.5
 //   5120 x 1280 x 8         4.1   4.8     -      5120 x 1280 x 1024    108  15.1  12.4
-//   50280 x 768 x 8 (f32)  12.8  10.8     -      1280 x 2560 x 2048   94.3  14.2  17.5
+//   50280 x 768 x 8 (f32)  12.8   9.0     -      1280 x 2560 x 2048   94.3  14.2  17.5
 //   1280 x 2560 x 64        7.0   5.9  17.0      5120 x 1280 x 16384     -   182   130
 //   64 x 64 x 16384        13.4   4.1     -      the same (f32)          -   307   356
 // 130 us are 1.65 PFLOP/s; the library's product with one scale an operand reaches 3.0 at 8192^3.
@@ -469,7 +476,8 @@ hipError_t launch_fp8mm(const Fp8MmParams& p, hipStream_t stream) {
   const double rows = 2.5 + fmax(0.00044 * tiles(16) * nkb, 0.0026 * tiles(16)) + 0.09 * nkb;
   const double few_tiles = p.token_major ? __builtin_ceil(p.M / 64.) * __builtin_ceil(p.T / 32.)
                                          : __builtin_ceil(p.T / 64.) * __builtin_ceil(p.M / 32.);
-  const bool few = few_tiles <= 256, teams = !few && tiles(64) <= 256 && nkb >= 8;
+  const bool few = few_tiles <= 256, thin = p.token_major && p.T <= 32;
+  const bool teams = tiles(64) <= 256 && nkb >= 8;
   double block, start = 2;  // of the tiles
   if (few) {
     start = 3.5;
@@ -483,6 +491,8 @@ hipError_t launch_fp8mm(const Fp8MmParams& p, hipStream_t stream) {
   if (far || rows < staged) launch_rows(p, stream);
   else if (few && p.out_bf16) launch_tiles<MmFew, true, bf16_t>(p, stream);
   else if (few) launch_tiles<MmFew, false, float>(p, stream);
+  else if (thin && p.out_bf16) launch_tiles<MmThin, true, bf16_t, false>(p, stream);
+  else if (thin) launch_tiles<MmThin, false, float, false>(p, stream);
   else if (teams && p.out_bf16) launch_tiles<MmTeams, true, bf16_t>(p, stream);
   else if (teams) launch_tiles<MmTeams, false, float>(p, stream);
   else if (!p.out_bf16) launch_tiles<MmSmall, false, float>(p, stream);

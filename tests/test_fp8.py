@@ -489,3 +489,11 @@ def test_quantise_borders():
 def test_matmul_few_tiles_many_blocks(m, k, t, out_dtype, token_major):
     """Few tiles of C with 8 to 21 blocks of K, even and odd in number, whole and not."""
     test_matmul(m, k, t, out_dtype, token_major)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,k,t", [(20000, 300, 7), (17001, 384, 32), (16500, 128, 1), (33000, 640, 33), (40000, 256, 17)])
+def test_matmul_many_rows_few_tokens(m, k, t, out_dtype):
+    """A head's products: many rows of W, up to 33 tokens, whose logits lie in rows."""
+    test_matmul(m, k, t, out_dtype, True)
