@@ -47,7 +47,8 @@ constexpr int kSampleBins = 2048;  // 11 bits of the key at a time
 constexpr int kSampleRegVocab = 8 * kSampleChunk;  // rows that stay in registers, 64 words a thread
 constexpr int kSampleList = 12288;
 constexpr int kSampleSmall = 256;                  // words of one bin that are looked at one by one
-constexpr int kSampleFew = 256;                    // a list as short as this needs no bins
+// A list as short as this needs no bins (50280 words, top-k 100: 14.9 us, by bins 15.8; 200: 22.3, 16.6).
+constexpr int kSampleFew = 128;
 constexpr int kSampleGroups = 3 * kSampleThreads;  // a thread's chunks c, c + 3, ... have one largest logit
 constexpr float kFixed = 8796093022208.f;  // 2^43
 

@@ -286,3 +286,13 @@ def test_long_rows_whose_beginning_differs(vocab, dtype):
     for kw in (dict(top_p=0.9, min_p=0.001), dict(top_p=0.9), dict(top_k=50), dict(top_k=700, top_p=0.8), dict(min_p=0.02),
                dict(min_p=1e-6), dict(top_p=0.5, temperature=0.3), dict(top_k=1000, min_p=0.01, temperature=0.05)):
         check(x, u, sample_tokens(x, u, **kw), **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("top_k", [127, 128, 129, 130, 200, 255, 256, 257])
+def test_lists_around_the_short_ones(top_k):
+    """Lists about as long as those that are looked at without bins, in both kinds of rows."""
+    for vocab in (700, 50000, 90000):
+        x, u = logits_of(5, vocab, torch.float32, seed=top_k)
+        for kw in (dict(), dict(top_p=0.9), dict(top_p=0.7, min_p=0.01, temperature=1.4)):
+            check(x, u, sample_tokens(x, u, top_k=top_k, **kw), top_k=top_k, **kw)
