@@ -444,7 +444,7 @@ __device__ __forceinline__ void draw_by_radix(SampleShared& s, const row_t row, 
 }
 
 // ------------------------------------------------------------------------- bins and the list
-// Zeroes the bins; ends with a barrier.
+// Zeroes the bins; ends with a barrier. Between a reach_bin and the next call lies a barrier.
 __device__ __forceinline__ void clear_bins(SampleShared& s) {
   for (int i = threadIdx.x; i < kSampleBins; i += kSampleThreads) s.mass[i] = 0;
   if (threadIdx.x == 0) s.found_bin = kSampleBins;
@@ -524,7 +524,8 @@ __device__ __forceinline__ void places(SampleShared& s, int n, const order_t& or
 
 // Of the list's words in bin `bin` of `order`, the one at which the running weight reaches
 // `target`, `before` being the weight of the bins before; false where they are too many. Every
-// thread gets it.
+// thread gets it. (Where false is returned, s.small_n has been read behind the last barrier: the caller
+// meets again before anything else is done with the list.)
 template <typename order_t, typename weight_t>
 __device__ __forceinline__ bool settle(SampleShared& s, int n, const order_t& order, const weight_t& weight, uint32_t bin,
                                        u64 before, u64 target, float& v, int& i) {
@@ -838,8 +839,10 @@ __device__ __forceinline__ int draw_by_bins(SampleShared& s, const words_t& word
     if (found) return draw_listed(n);
   }
 
-  // No list: the cuts from bins of the whole row.
+  // No list: the cuts from bins of the whole row. (gather begins and ends with a barrier: every thread
+  // has read the length of the list before, which is returned behind the last one, when it is cleared.)
   const auto gather = [&](const auto& takes) {
+    __syncthreads();
     if (threadIdx.x == 0) s.list_n = 0;
     __syncthreads();
     words.each([&](const float (&v)[8], int i, int, auto) { append(s, v, i, takes); });
@@ -861,6 +864,7 @@ __device__ __forceinline__ int draw_by_bins(SampleShared& s, const words_t& word
       const int g = gather(in_bin);
       if (g > kSampleList || !settle(s, g, order, [](int) -> u64 { return 1; }, bin, before, target, cut.v, cut.i)) return -1;
     }
+    __syncthreads();  // found_bin has been read
   }
   if (by_p) {
     clear_bins(s);

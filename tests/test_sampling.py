@@ -296,3 +296,20 @@ def test_lists_around_the_short_ones(top_k):
         x, u = logits_of(5, vocab, torch.float32, seed=top_k)
         for kw in (dict(), dict(top_p=0.9), dict(top_p=0.7, min_p=0.01, temperature=1.4)):
             check(x, u, sample_tokens(x, u, top_k=top_k, **kw), top_k=top_k, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [16000, 50280, 70001])
+def test_many_rows_of_long_prefixes(vocab):
+    """Every row's prefix outgrows the list, in more rows than there are compute units: what the waves of
+    a workgroup share has to be read by all of them before it is cleared."""
+    g = torch.Generator().manual_seed(vocab)
+    x = torch.randn(300, vocab, generator=g)
+    x[::2] *= 0.02  # a bin that outgrows the list too
+    x = x.to("cuda")
+    u = torch.rand(300, generator=g).to("cuda")
+    for kw in (dict(top_p=0.97), dict(top_p=0.95, top_k=vocab - 10, temperature=3.0)):
+        got = sample_tokens(x, u, **kw)
+        for _ in range(4):
+            assert torch.equal(got, sample_tokens(x, u, **kw))
+        check(x[::7], u[::7], got[::7], **kw)
