@@ -458,7 +458,8 @@ __global__ __launch_bounds__(512) void norm_fp8_rows_kernel(QuantParams p) {
   for (int k = 0; k < kRounds; ++k) {
     const bool in = 512 * k + static_cast<int>(threadIdx.x) < F;
     if constexpr (kDelta) x[k] += d[k];
-    ss = __builtin_fmaf(x[k], in ? x[k] : 0.f, ss);
+    const float sq = in ? x[k] : 0.f;  // (both factors: the last feature again may be infinite)
+    ss = __builtin_fmaf(sq, sq, ss);
     w[k] *= x[k];  // y' = hn w
     const uint32_t m = max_above<1>(in ? magnitude_bits(w[k]) : 0u);
     if ((threadIdx.x & 63) == 0) s_m[k][wave] = m;

@@ -497,3 +497,28 @@ def test_matmul_few_tiles_many_blocks(m, k, t, out_dtype, token_major):
 def test_matmul_many_rows_few_tokens(m, k, t, out_dtype):
     """A head's products: many rows of W, up to 33 tokens, whose logits lie in rows."""
     test_matmul(m, k, t, out_dtype, True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("delta", [None, torch.bfloat16])
+@pytest.mark.parametrize("t", [3, 255, 300])
+@pytest.mark.parametrize("f", [1, 130, 700, 1024, 1500, 5000, 9000])
+def test_norm_infinite_last_feature(f, t, delta):
+    """An infinity in any place, the last feature among them, makes 1 / rms zero: its own block stands for
+    NaN, the token's other blocks for zero, and the other tokens are what they are without it."""
+    h = rand(f, t, seed=21)
+    d = None if delta is None else torch.zeros(f, t, dtype=delta, device="cuda")
+    w = torch.ones(f, device="cuda")
+    _, q0, s0 = add_rmsnorm_fp8(h, d, w)
+    for token, at in enumerate(dict.fromkeys([f - 1, 0, f // 2])):
+        x = h.clone()
+        x[at, token] = float("-inf")
+        _, q, s = add_rmsnorm_fp8(x, d, w)
+        v = q.float() * s.repeat_interleave(BLOCK, 0)[:f].t()
+        b = at // BLOCK
+        own = slice(b * BLOCK, min(f, (b + 1) * BLOCK))
+        assert torch.isnan(v[token, own]).all()
+        v[token, own] = 0
+        assert torch.all(v[token] == 0)
+        keep = torch.arange(t, device="cuda") != token
+        assert torch.equal(q[keep].float(), q0[keep].float()) and torch.equal(s[:, keep], s0[:, keep])
