@@ -23,19 +23,24 @@ namespace mss {
 // block's largest magnitude, y * (448 / m) with the factor in two parts: bf16 values meet e4m3's borders
 // exactly (y / m = 3 / 64, for one, is 21, between 20 and 22), and a quotient that is off by one
 // float32 step there rounds the wrong way.
-struct ToFp8 {
-  float scale, hi, lo;
-  __device__ __forceinline__ explicit ToFp8(uint32_t m) {
-    const float amax = __uint_as_float(m);
-    scale = fp8_scale(amax);
+struct Ratio448 {  // y -> 448 y / amax
+  float hi, lo;
+  __device__ __forceinline__ explicit Ratio448(float amax) {
     hi = kFp8Max / amax;
-    lo = __builtin_fmaf(-hi, amax, kFp8Max) / amax;
-    if (amax < kFp8Max * 1.1754943508222875e-38f) {  // the least scale, 2^-126
-      hi = 8.507059173023462e37f;
-      lo = 0.f;
-    }
+    lo = __builtin_fmaf(-hi, amax, kFp8Max) * (hi * (1.f / kFp8Max));
   }
   __device__ __forceinline__ float operator()(float y) const { return __builtin_fmaf(y, hi, y * lo); }
+};
+struct ToFp8 {
+  float scale;
+  Ratio448 by;
+  __device__ __forceinline__ explicit ToFp8(uint32_t m) : scale(fp8_scale(__uint_as_float(m))), by(__uint_as_float(m)) {
+    if (__uint_as_float(m) < kFp8Max * 1.1754943508222875e-38f) {  // the least scale, 2^-126
+      by.hi = 8.507059173023462e37f;
+      by.lo = 0.f;
+    }
+  }
+  __device__ __forceinline__ float operator()(float y) const { return by(y); }
 };
 
 // v and the values kLanes away (32, 16, 2, 1: the lane whose index differs there; 8, 4: the lane that
@@ -390,8 +395,8 @@ __global__ __launch_bounds__(64 * kWaves) void norm_fp8_tile_kernel(QuantParams 
       for (int i = 0; i < kBlockWaves; ++i) m = max(m, s_m[wave / kBlockWaves * kBlockWaves + i][4 * l + j]);
       const float mf = __uint_as_float(m);
       if (g % 32 == 0 && b < kNormMaxBlocks) s_block[b][4 * l + j] = mf;
-      const float inv = m ? kFp8Max / mf : 0.f;
-      s_q[(4 * l + j) * kPitch + g] = pack_fp8x4(y[0][j] * inv, y[1][j] * inv, y[2][j] * inv, y[3][j] * inv);
+      const Ratio448 to(m ? mf : 1.f);
+      s_q[(4 * l + j) * kPitch + g] = pack_fp8x4(to(y[0][j]), to(y[1][j]), to(y[2][j]), to(y[3][j]));
     }
     meet();
     // 16 bytes of the tile each
@@ -472,8 +477,8 @@ __global__ __launch_bounds__(512) void norm_fp8_rows_kernel(QuantParams p) {
     const int f = 512 * k + threadIdx.x;
     if (f < F) {
       const uint32_t m = max(s_m[k][wave], s_m[k][wave ^ 1]);
-      const float inv = m ? kFp8Max / __uint_as_float(m) : 0.f;
-      p.q[t * p.ldq + f] = static_cast<unsigned char>(pack_fp8x4(w[k] * inv, 0.f, 0.f, 0.f));
+      const Ratio448 to(m ? __uint_as_float(m) : 1.f);
+      p.q[t * p.ldq + f] = static_cast<unsigned char>(pack_fp8x4(to(w[k]), 0.f, 0.f, 0.f));
       if constexpr (kDelta) p.hn[f * T + t] = x[k];
     }
   }
@@ -524,26 +529,33 @@ __global__ __launch_bounds__(512) void norm_fp8_wide_kernel(QuantParams p) {
   const float r = 1.f / __builtin_sqrtf(tot / p.features + p.eps);
   const int padded = (p.features + kFp8Block - 1) / kFp8Block * kFp8Block;
   for (int f0 = threadIdx.x * 4; f0 < padded; f0 += 2048) {
-    float v[4];
-    uint32_t m = 0;
+    float v[4], y[4];  // y' = hn w, and hn r w
+    uint32_t m = 0, my = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int f = f0 + i;
-      v[i] = 0.f;
+      v[i] = y[i] = 0.f;
       if (f < p.features) {
         float x = h[f * T];
         if constexpr (kDelta) {
           x += to_f32(delta[f * T]);
           p.hn[f * T + t] = x;
         }
-        v[i] = x * r * p.w[f];
+        v[i] = x * p.w[f];
+        y[i] = x * r * p.w[f];
       }
       m = max(m, magnitude_bits(v[i]));
+      my = max(my, magnitude_bits(y[i]));
     }
     m = max_above<1, 32>(m);
-    const ToFp8 to(m);
-    if ((threadIdx.x & 31) == 0) p.scales[(f0 / kFp8Block) * T + t] = to.scale;
-    const uint32_t q4 = pack_fp8x4(to(v[0]), to(v[1]), to(v[2]), to(v[3]));
+    my = max_above<1, 32>(my);
+    const float mf = __uint_as_float(m);
+    const bool plain = scale_is_plain(mf, r);
+    const ToFp8 to(my);
+    const Ratio448 by(m ? mf : 1.f);
+    if ((threadIdx.x & 31) == 0) p.scales[(f0 / kFp8Block) * T + t] = plain ? fp8_scale(mf * r) : to.scale;
+    const uint32_t q4 = plain ? pack_fp8x4(by(v[0]), by(v[1]), by(v[2]), by(v[3]))
+                              : pack_fp8x4(to(y[0]), to(y[1]), to(y[2]), to(y[3]));
     unsigned char* q = p.q + t * p.ldq + f0;
     if (f0 + 4 <= p.features) {
       *reinterpret_cast<uint32_t*>(q) = q4;

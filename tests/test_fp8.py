@@ -522,3 +522,30 @@ def test_norm_infinite_last_feature(f, t, delta):
         assert torch.all(v[token] == 0)
         keep = torch.arange(t, device="cuda") != token
         assert torch.equal(q[keep].float(), q0[keep].float()) and torch.equal(s[:, keep], s0[:, keep])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wide", [0, 8000])
+@pytest.mark.parametrize("t", [4, 300])
+def test_norm_borders(t, wide):
+    """The norm's bytes are 448 y / max |y| of their block, in which 1 / rms cancels, rounded to the even
+    neighbour where that lies on a border: the quantisation's rule."""
+    g = torch.Generator().manual_seed(31)
+    largest = 1 + torch.randint(0, 128, (300,), generator=g) / 128  # bf16 values
+    ratio = torch.tensor([448.0, 21, -84, 9, 5.5, 300, 13, -1.75 / 2, 42, 10.5, 26, -168])
+    h = torch.zeros(2 * BLOCK + wide, t)
+    for b in range(2):
+        m = largest[torch.arange(t) % 150 + 150 * b]
+        h[b * BLOCK:b * BLOCK + 12] = (ratio[:, None].double() * m.double() / 448).float()
+    h = h.to("cuda")
+    exact = h.double()
+    for b in range(2):
+        part = exact[b * BLOCK:(b + 1) * BLOCK]
+        top = part.abs().max(0, keepdim=True).values
+        part.mul_(448).div_(top)
+    # (products with 448 and quotients on a border are exact in float64 where h is)
+    step = torch.exp2(torch.floor(torch.log2(exact.abs().clamp_min(2.0 ** -6))) - 3)
+    want = torch.round(exact / step) * step
+    for delta in (None, torch.zeros(2 * BLOCK + wide, t, dtype=torch.bfloat16, device="cuda")):
+        _, q, _ = add_rmsnorm_fp8(h, delta, torch.ones(2 * BLOCK + wide, device="cuda"))
+        assert torch.equal(q.double().t(), want)
