@@ -30,7 +30,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .selective_scan_hip import _io_tag, _ptr, _require_gpu, _stream
+from .selective_scan_hip import _io_tag, _ptr, _require_gpu, _resolved, _stream
 
 __all__ = ["quantize_fp8", "add_rmsnorm_fp8", "quantize_fp8_weight", "fp8_matmul"]
 
@@ -70,6 +70,8 @@ def quantize_fp8(x):
         io = _io_tag(x.dtype, "x")  # raises
     _no_grad_needed(x)
     _require_gpu(x)
+    if x.is_neg():
+        x = _resolved(x)
     f, t = x.shape
     dev = x.device
     q = _empty_rows(t, f, dev)
@@ -99,6 +101,8 @@ def add_rmsnorm_fp8(h, delta, weight, eps=1e-5):
         raise ValueError("h has no features")
     _no_grad_needed(h, delta, weight)
     _require_gpu(h, delta, weight)
+    if h.is_neg() or weight.is_neg() or (delta is not None and delta.is_neg()):
+        h, delta, weight = _resolved(h), _resolved(delta), _resolved(weight)
     h, weight = h.contiguous(), weight.contiguous()
     dev = h.device
     q = _empty_rows(t, f, dev)
@@ -121,6 +125,7 @@ def quantize_fp8_weight(w):
     io = _io_tag(w.dtype, "w")
     _no_grad_needed(w)
     _require_gpu(w)
+    w = _resolved(w)
     m, k = w.shape
     q = _empty_rows(m, k, w.device)
     scales = torch.empty(_blocks(m), _blocks(k), dtype=_F32, device=w.device)
@@ -166,9 +171,13 @@ def fp8_matmul(wq, w_scales, xq, x_scales, out_dtype=torch.bfloat16, token_major
     if out is not None:
         if out.shape != (rows, cols) or out.dtype != out_dtype or (cols > 1 and out.stride(1) != 1):
             raise ValueError(f"out must be {out_dtype} of shape {(rows, cols)} with contiguous rows")
+        if out.is_neg():
+            raise ValueError("out must not be lazily negated")
         if rows > 1:
             ldc = out.stride(0)
     _require_gpu(wq, w_scales, xq, x_scales, out)
+    if w_scales.is_neg() or x_scales.is_neg():
+        w_scales, x_scales = _resolved(w_scales), _resolved(x_scales)
     if out is None:
         out = torch.empty(rows, cols, dtype=out_dtype, device=wq.device)
     if m == 0 or t == 0:

@@ -23,7 +23,7 @@ import math
 import torch
 
 from . import _lib
-from .selective_scan_hip import _io_tag, _ptr, _require_gpu, _stream
+from .selective_scan_hip import _io_tag, _ptr, _require_gpu, _resolved, _stream
 
 __all__ = ["sample_tokens"]
 
@@ -36,7 +36,7 @@ def _setting(name, v, rows, dtype, low, high):
     if isinstance(v, torch.Tensor):
         if v.dtype != dtype or v.shape != (rows,):
             raise ValueError(f"{name} must be a number or a {dtype} tensor of shape ({rows},)")
-        return 0, v.contiguous()
+        return 0, _resolved(v).contiguous()
     if not low <= v <= high:  # a NaN too
         raise ValueError(f"{name} must be between {low} and {high}, got {v}")
     return v, None
@@ -59,6 +59,8 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     tokens = torch.empty(rows, dtype=_I64, device=logits.device)
     if rows == 0:
         return tokens
+    if logits.is_neg() or uniform.is_neg():
+        logits, uniform = _resolved(logits), _resolved(uniform)
     uniform = uniform.contiguous()
     sr, sv = logits.stride()
     a = _lib.SampleArgs(rows, vocab, io, top_k, temperature, top_p, min_p, sr if rows > 1 else 0,

@@ -41,6 +41,12 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _resolved(t):
+    """t, or a copy that holds its values where it is lazily negated (as z.conj().imag is): a kernel
+    reads what lies behind data_ptr()."""
+    return t.resolve_neg() if t is not None and t.is_neg() else t
+
+
 def _io_tag(dtype, what):
     if dtype == torch.float32:
         return _lib.MSS_F32

@@ -549,3 +549,34 @@ def test_norm_borders(t, wide):
     for delta in (None, torch.zeros(2 * BLOCK + wide, t, dtype=torch.bfloat16, device="cuda")):
         _, q, _ = add_rmsnorm_fp8(h, delta, torch.ones(2 * BLOCK + wide, device="cuda"))
         assert torch.equal(q.double().t(), want)
+
+
+def lazily_negated(x, strided=False):
+    """x's values as a view that torch has yet to negate: contiguous, or the imaginary part of a conjugate."""
+    y = torch.complex(x.float(), -x.float()).conj().imag if strided else torch._neg_view(-x)
+    assert y.is_neg() and torch.equal(y, x)
+    return y
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [5, 300])
+def test_lazily_negated(t):
+    """Operands that torch holds lazily negated give what their values give."""
+    f = 300
+    h, d, x = rand(f, t, seed=41), rand(f, t, seed=42, dtype=torch.bfloat16), rand(f, t, seed=43)
+    w, weight = rand(200, f, seed=44), torch.rand(f, device="cuda") - 0.5
+    same = lambda a, b: all(torch.equal(i.float(), j.float()) for i, j in zip(a, b))  # noqa: E731
+    want = quantize_fp8(x)
+    assert same(quantize_fp8(lazily_negated(x)), want) and same(quantize_fp8(lazily_negated(x, True)), want)
+    want = add_rmsnorm_fp8(h, d, weight)
+    for strided in (False, True):
+        neg = lambda v: lazily_negated(v, strided)  # noqa: E731
+        assert same(add_rmsnorm_fp8(neg(h), lazily_negated(d), neg(weight)), want)
+    assert same(add_rmsnorm_fp8(lazily_negated(h), None, weight), add_rmsnorm_fp8(h, None, weight))
+    wq, ws = quantize_fp8_weight(w)
+    assert same(quantize_fp8_weight(lazily_negated(w)), (wq, ws))
+    _, xq, xs = want
+    got = fp8_matmul(wq, lazily_negated(ws), xq, lazily_negated(xs))
+    assert torch.equal(got, fp8_matmul(wq, ws, xq, xs))
+    with pytest.raises(ValueError):
+        fp8_matmul(wq, ws, xq, xs, out=lazily_negated(got))

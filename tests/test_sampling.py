@@ -313,3 +313,17 @@ def test_many_rows_of_long_prefixes(vocab):
         for _ in range(4):
             assert torch.equal(got, sample_tokens(x, u, **kw))
         check(x[::7], u[::7], got[::7], **kw)
+
+
+@pytest.mark.gpu
+def test_lazily_negated():
+    """Logits, uniform numbers and settings that torch holds lazily negated give what their values give."""
+    x, u = logits_of(6, 1003)
+    settings = dict(temperature=torch.linspace(0.5, 1.5, 6, device="cuda"), top_p=torch.linspace(0.5, 1, 6, device="cuda"),
+                    min_p=torch.linspace(0, 0.2, 6, device="cuda"))
+    want = sample_tokens(x, u, **settings)
+    neg = {k: torch._neg_view(-v) for k, v in settings.items()}
+    assert all(v.is_neg() for v in neg.values())
+    for y in (torch._neg_view(-x), torch.complex(x, -x).conj().imag):
+        assert y.is_neg() and torch.equal(y, x)
+        assert torch.equal(sample_tokens(y, torch._neg_view(-u), **neg), want)
