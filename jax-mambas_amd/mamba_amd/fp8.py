@@ -56,10 +56,11 @@ def _row_stride(q, rows, cols):
     return q.stride(0) if rows > 1 else -(-cols // 16) * 16
 
 
-def _no_grad_needed(a, b=None, c=None):
-    if torch.is_grad_enabled() and (a.requires_grad or (b is not None and b.requires_grad)
-                                    or (c is not None and c.requires_grad)):
-        raise RuntimeError("the 8-bit operators are for inference: call them under torch.no_grad()")
+def _no_grad_needed(*tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("the 8-bit operators are for inference: call them under torch.no_grad()")
 
 
 def quantize_fp8(x):
@@ -175,6 +176,7 @@ def fp8_matmul(wq, w_scales, xq, x_scales, out_dtype=torch.bfloat16, token_major
             raise ValueError("out must not be lazily negated")
         if rows > 1:
             ldc = out.stride(0)
+    _no_grad_needed(wq, w_scales, xq, x_scales, out)
     _require_gpu(wq, w_scales, xq, x_scales, out)
     if w_scales.is_neg() or x_scales.is_neg():
         w_scales, x_scales = _resolved(w_scales), _resolved(x_scales)

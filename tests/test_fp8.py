@@ -580,3 +580,15 @@ def test_lazily_negated(t):
     assert torch.equal(got, fp8_matmul(wq, ws, xq, xs))
     with pytest.raises(ValueError):
         fp8_matmul(wq, ws, xq, xs, out=lazily_negated(got))
+
+
+@pytest.mark.parametrize("which", range(5))
+def test_matmul_refuses_gradients(which):
+    """As the other operators do: a product of operands that ask for a gradient would lose it silently."""
+    a = [torch.zeros(8, 16).to(FP8), torch.ones(1, 1), torch.zeros(4, 16).to(FP8), torch.ones(1, 4),
+         torch.zeros(8, 4, dtype=torch.bfloat16)]
+    a[which].requires_grad_(True)
+    with pytest.raises(RuntimeError, match="inference"):
+        fp8_matmul(*a[:4], out=a[4])
+    with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):
+        fp8_matmul(*a[:4], out=a[4])
