@@ -2,7 +2,8 @@
 
 ``Fp8LM(model)`` takes a ``mamba1.MambaLM`` (its blocks: mamba/mamba1.py:216-363) and holds its in-, gate- and
 out-projections and the tied head in the 8-bit form of ``mamba_amd.fp8``, written once from the
-float32 masters; the small S6 projections stay in bf16. Every norm writes the 8-bit operand of
+float32 masters; the small S6 projections in bf16; copies of what else it reads (the embedding,
+norms, conv and S6 vectors). Every norm writes the 8-bit operand of
 the product behind it (``add_rmsnorm_fp8``), the scan's output is quantised for the
 out-projection (``quantize_fp8``), and logits are float32.
 
@@ -16,11 +17,16 @@ draws uniforms.shape[0] tokens a row after the prompt with ``sample_tokens``: un
 float32 in [0, 1), settings numbers or one a row; drawn (n, B) int64. With ``graph`` the decode
 step and its draw are captured once in a HIP graph and replayed.
 
-Weights that change afterwards are not seen until ``refresh()``. Inference only; there is no CPU path.
+Weights of the model that change afterwards are not seen, none of them, until ``refresh()``, which writes
+the held ones where they lie (a graph captured from ``step`` goes on with the new ones). Inference
+only; there is no CPU path.
 """
 from __future__ import annotations
 
+import copy
+
 import torch
+import torch.nn as nn
 import torch.nn.functional as F
 
 from .conv1d_hip import causal_conv1d_fn
@@ -33,40 +39,68 @@ from .selective_scan_hip import _require_gpu
 __all__ = ["Fp8LM"]
 
 
+_SHADOWED = ("x_proj", "dt_proj")  # of an S6: held in bf16
+
+
+class _Block:
+    """A block's weights as they are served, but for those _SHADOWED."""
+
+    def __init__(self, blk, A):
+        self.norm, self.eps = blk.norm.weight.clone(), blk.norm.eps
+        self.in_z = quantize_fp8_weight(torch.cat([blk.in_proj, blk.z_proj]))
+        self.out = quantize_fp8_weight(blk.out_proj)
+        self.conv_weight, self.conv_bias, self.A = blk.conv_weight.clone(), blk.conv_bias.clone(), A.clone()
+        # An S6 with parameters of its own; the projections stay the model's, by which their copies are found.
+        self.s6 = copy.copy(blk.s6)
+        self.s6._parameters = {k: p if p is None or k in _SHADOWED else nn.Parameter(p.detach().clone(), requires_grad=False)
+                               for k, p in blk.s6._parameters.items()}
+
+    def tensors(self):
+        return [self.norm, *self.in_z, *self.out, self.conv_weight, self.conv_bias, self.A,
+                *(p for k, p in self.s6.named_parameters() if k not in _SHADOWED)]
+
+
 class Fp8LM:
     def __init__(self, model):
         if not isinstance(model, MambaLM):
             raise TypeError("model must be a MambaLM")
         _require_gpu(model.embedding)
         self.model = model
-        self._small = ShadowWeights([w for b in model.blocks for w in (b.s6.x_proj, b.s6.dt_proj)])
+        self._small = ShadowWeights([getattr(b.s6, w) for b in model.blocks for w in _SHADOWED])
+        self._blocks = None
         self.refresh()
 
     @torch.no_grad()
     def refresh(self):
-        """Writes the 8-bit and bf16 weights from the model's float32 ones."""
+        """Writes every weight that is held from the model's."""
         m = self.model
-        self.head = quantize_fp8_weight(m.embedding)
-        self.in_z = [quantize_fp8_weight(torch.cat([b.in_proj, b.z_proj])) for b in m.blocks]
-        self.out = [quantize_fp8_weight(b.out_proj) for b in m.blocks]
-        self.A = [a.contiguous() for a in m.a_matrices()]
+        new = [m.embedding.clone(), *quantize_fp8_weight(m.embedding), m.final_norm.weight.clone()]
+        matrices = m.a_matrices()
+        if self._blocks is None:
+            self._ends = new
+            self._blocks = [_Block(b, A) for b, A in zip(m.blocks, matrices)]
+        else:
+            torch._foreach_copy_(self._ends, new)
+            for mine, b, A in zip(self._blocks, m.blocks, matrices):
+                torch._foreach_copy_(mine.tensors(), _Block(b, A).tensors())
+        self._small._current = None  # (a master may have been changed behind autograd's version counter)
         self._small.refresh(torch.bfloat16)
 
     def _logits(self, h, delta):
-        norm = self.model.final_norm
-        _, q, s = add_rmsnorm_fp8(h, delta, norm.weight, norm.eps)
-        return fp8_matmul(*self.head, q, s, out_dtype=torch.float32, token_major=True)
+        _, *head, norm = self._ends
+        _, q, s = add_rmsnorm_fp8(h, delta, norm, self.model.final_norm.eps)
+        return fp8_matmul(*head, q, s, out_dtype=torch.float32, token_major=True)
 
     @torch.no_grad()
     def prefill(self, tokens):
         batch, length = tokens.shape
         if length == 0:
             raise ValueError("the prompt has no tokens")
-        h = self.model.embedding[tokens.reshape(-1)].t().contiguous()  # (d_model, B L)
+        h = self._ends[0][tokens.reshape(-1)].t().contiguous()  # (d_model, B L)
         delta, caches = None, []
-        for blk, in_z, out, A in zip(self.model.blocks, self.in_z, self.out, self.A):
-            h, q, s = add_rmsnorm_fp8(h, delta, blk.norm.weight, blk.norm.eps)
-            xz = fp8_matmul(*in_z, q, s)
+        for blk in self._blocks:
+            h, q, s = add_rmsnorm_fp8(h, delta, blk.norm, blk.eps)
+            xz = fp8_matmul(*blk.in_z, q, s)
             di, k = blk.conv_weight.shape
             rows = xz.view(2 * di, batch, length).permute(1, 0, 2)
             xin, z = rows[:, :di], xz[di:]
@@ -74,23 +108,23 @@ class Fp8LM:
             y = blk.s6(u.permute(1, 0, 2).reshape(di, batch * length), batch, z=z, weights=self._small)
             tail = xin[:, :, max(0, length - (k - 1)):]
             conv = F.pad(tail, (k - 1 - tail.shape[2], 0)).contiguous()
-            caches.append({"conv": conv, "ssm": blk.s6.last_state, "A": A})
+            caches.append({"conv": conv, "ssm": blk.s6.last_state, "A": blk.A})
             blk.s6.last_state = None
-            delta = fp8_matmul(*out, *quantize_fp8(y))
+            delta = fp8_matmul(*blk.out, *quantize_fp8(y))
         last = slice(length - 1, None, length)
         return self._logits(h[:, last].contiguous(), delta[:, last].contiguous()), caches
 
     @torch.no_grad()
     def step(self, token, caches):
-        h = self.model.embedding[token].t().contiguous()  # (d_model, B)
+        h = self._ends[0][token].t().contiguous()  # (d_model, B)
         delta = None
-        for blk, in_z, out, cache in zip(self.model.blocks, self.in_z, self.out, caches):
-            h, q, s = add_rmsnorm_fp8(h, delta, blk.norm.weight, blk.norm.eps)
-            xz = fp8_matmul(*in_z, q, s)
+        for blk, cache in zip(self._blocks, caches):
+            h, q, s = add_rmsnorm_fp8(h, delta, blk.norm, blk.eps)
+            xz = fp8_matmul(*blk.in_z, q, s)
             di = blk.conv_weight.shape[0]
             u = causal_conv1d_update(cache["conv"], xz[:di].t(), blk.conv_weight, blk.conv_bias).t()
             y = blk.s6.step(u, xz[di:], cache["ssm"], self._small, cache["A"])
-            delta = fp8_matmul(*out, *quantize_fp8(y))
+            delta = fp8_matmul(*blk.out, *quantize_fp8(y))
         return self._logits(h, delta)
 
     @torch.no_grad()

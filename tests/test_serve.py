@@ -138,3 +138,65 @@ def test_refresh_and_complex_states():
     assert torch.equal(m.prefill(tokens)[0], before)
     m.refresh()
     assert not torch.equal(m.prefill(tokens)[0], before)
+
+
+def changed_in_turn(model):
+    """(name, tensor) of every weight of the model, a kind each."""
+    blk = model.blocks[1]
+    return [("embedding", model.embedding), ("final_norm", model.final_norm.weight), *blk.named_parameters()]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(), dict(complex_ssm=True)], ids=str)
+def test_refresh_is_what_changes_weights(kw):
+    """Whatever weight of the model changes, in place or behind autograd's version counter, prompt and
+    step give the same until refresh(), and after it what a new Fp8LM of the model gives."""
+    model = lm(8, **kw)
+    m = Fp8LM(model)
+    tokens = prompt(2, 6)
+
+    def out(m):
+        logits, caches = m.prefill(tokens)
+        return logits, m.step(tokens[:, 3], caches), caches[1]["ssm"]
+
+    same = lambda a, b: all(torch.equal(x, y) for x, y in zip(a, b))  # noqa: E731
+    held = out(m)
+    names = changed_in_turn(model)
+    assert len(names) == 13 + len(kw)
+    for i, (name, w) in enumerate(names):
+        with torch.no_grad():
+            (w.data if i % 2 else w).mul_(0.75).add_(0.01)
+        assert same(out(m), held), name
+        m.refresh()
+        now = out(m)
+        assert same(now, out(Fp8LM(model))) and not same(now, held), name
+        held = now
+
+
+@pytest.mark.gpu
+def test_refresh_reaches_a_captured_step():
+    """refresh() writes the weights where they lie: a graph of a step goes on with the new ones."""
+    model = lm(9)
+    m = Fp8LM(model)
+    tokens = prompt(2, 6)
+    _, caches = m.prefill(tokens)
+    token = tokens[:, 0].clone()
+    copies = lambda: [{k: v.clone() for k, v in c.items()} for c in caches]  # noqa: E731
+    m.step(token, copies())
+    mine = copies()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        logits = m.step(token, mine)
+    for scale in (0.5, 1.5, 1.1):
+        with torch.no_grad():
+            for p in model.parameters():
+                p.mul_(scale)
+        m.refresh()
+        for c, old in zip(mine, caches):
+            c["conv"].copy_(old["conv"]), c["ssm"].copy_(old["ssm"])
+        # (each cache brings the matrix A of its prompt; a step takes that one)
+        eager = copies()
+        want = m.step(token, [dict(c, A=g["A"]) for c, g in zip(eager, mine)])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(logits, want)
