@@ -10,12 +10,14 @@ out-projection (``quantize_fp8``), and logits are float32.
 ``prefill(tokens) -> (logits, caches)`` — tokens (B, L) int64, right-aligned; logits (B, vocab) of
 the last position, and each block's decode state.
 
-``step(token, caches) -> logits`` — token (B,) int64; caches update in place.
+``step(token, caches) -> logits`` — token (B,) int64; caches update in place. A token of -1 (what
+``sample_tokens`` gives for a row without a word or with a NaN) makes its row's logits NaN, in this step and
+those that follow, so that the row's draws stay -1.
 
 ``generate(tokens, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, graph=True) -> drawn`` —
 draws uniforms.shape[0] tokens a row after the prompt with ``sample_tokens``: uniforms (n, B)
 float32 in [0, 1), settings numbers or one a row; drawn (n, B) int64. With ``graph`` the decode
-step and its draw are captured once in a HIP graph and replayed.
+step and its draw are captured once in a HIP graph and replayed. A row whose draw is -1 stays at -1.
 
 Weights of the model that change afterwards are not seen, none of them, until ``refresh()``, which writes
 the held ones where they lie (a graph captured from ``step`` goes on with the new ones). Inference
@@ -74,7 +76,9 @@ class Fp8LM:
     def refresh(self):
         """Writes every weight that is held from the model's."""
         m = self.model
-        new = [m.embedding.clone(), *quantize_fp8_weight(m.embedding), m.final_norm.weight.clone()]
+        # (the embedding has one row more, of NaN, for the token -1)
+        none = torch.full_like(m.embedding[:1], float("nan"))
+        new = [torch.cat([m.embedding, none]), *quantize_fp8_weight(m.embedding), m.final_norm.weight.clone()]
         matrices = m.a_matrices()
         if self._blocks is None:
             self._ends = new

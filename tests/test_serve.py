@@ -200,3 +200,34 @@ def test_refresh_reaches_a_captured_step():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(logits, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("batch", [3, 20])
+def test_a_row_without_a_word_stays_without(batch, graph):
+    """A row whose draw is -1 draws -1 from then on, greedy or not; the others draw what they draw beside a
+    row that is well. So does a loop of steps."""
+    m = Fp8LM(lm(10))
+    tokens = prompt(batch, 5)
+    uniforms = torch.rand(6, batch, generator=torch.Generator().manual_seed(11)).cuda()
+    kw = dict(temperature=torch.linspace(0, 1.2, batch, device="cuda"), top_k=30)
+    want = m.generate(tokens, uniforms, graph=graph, **kw)
+    well = m.prefill
+
+    def prefill(tokens):
+        logits, caches = well(tokens)
+        logits[1] = float("nan")
+        return logits, caches
+
+    m.prefill = prefill
+    got = m.generate(tokens, uniforms, graph=graph, **kw)
+    assert torch.all(got[:, 1] == -1)
+    keep = torch.arange(batch, device="cuda") != 1
+    assert torch.equal(got[:, keep], want[:, keep])
+    logits, caches = m.prefill(tokens)
+    for i in range(3):
+        token = sample_tokens(logits, uniforms[i], **kw)
+        assert torch.equal(token, got[i])
+        logits = m.step(token, caches)
+        assert torch.isnan(logits[1]).all() and torch.isfinite(logits[keep]).all()
