@@ -1038,10 +1038,26 @@ static void launch_sample_as(const SampleParams& p, hipStream_t stream) {
   else hipLaunchKernelGGL((sample_kernel<io_t, false, false>), grid, block, 0, stream, p);
 }
 
+// A launch has fewer than 2^32 threads along x: rows beyond kSampleLaunchRows take another one.
+constexpr int kSampleLaunchRows = 1 << 21;
+
 hipError_t launch_sample(const SampleParams& p, bool io_bf16, hipStream_t stream) {
-  if (io_bf16) launch_sample_as<bf16_t>(p, stream);
-  else launch_sample_as<float>(p, stream);
-  return hipGetLastError();
+  SampleParams part = p;
+  for (long long r = 0; r < p.rows; r += kSampleLaunchRows) {
+    part.rows = static_cast<int>(p.rows - r < kSampleLaunchRows ? p.rows - r : kSampleLaunchRows);
+    part.logits = static_cast<const char*>(p.logits) + r * p.sr * (io_bf16 ? 2 : 4);
+    part.uniform = p.uniform + r;
+    part.temperatures = p.temperatures ? p.temperatures + r : nullptr;
+    part.top_ks = p.top_ks ? p.top_ks + r : nullptr;
+    part.top_ps = p.top_ps ? p.top_ps + r : nullptr;
+    part.min_ps = p.min_ps ? p.min_ps + r : nullptr;
+    part.tokens = p.tokens + r;
+    if (io_bf16) launch_sample_as<bf16_t>(part, stream);
+    else launch_sample_as<float>(part, stream);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace mss

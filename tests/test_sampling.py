@@ -327,3 +327,24 @@ def test_lazily_negated():
     for y in (torch._neg_view(-x), torch.complex(x, -x).conj().imag):
         assert y.is_neg() and torch.equal(y, x)
         assert torch.equal(sample_tokens(y, torch._neg_view(-u), **neg), want)
+
+
+@pytest.mark.gpu
+def test_more_rows_than_one_launch_takes():
+    """2^22 rows and some, each with settings of its own: the first word where the temperature is 0, and
+    elsewhere the word that holds the uniform number's share of the weight (2^-20 from a border)."""
+    rows, vocab = (1 << 22) + 77, 3
+    g = torch.Generator(device="cuda").manual_seed(9)
+    x = torch.randn(rows, vocab, generator=g, device="cuda")
+    u = torch.rand(rows, generator=g, device="cuda")
+    t = torch.rand(rows, generator=g, device="cuda").clamp_min(0.3)
+    t[::3] = 0
+    k = torch.full((rows,), 2, dtype=torch.int32, device="cuda")
+    got = sample_tokens(x, u, temperature=t, top_k=k)
+    w = torch.exp((x - x.amax(1, keepdim=True)).double() / t.double().clamp_min(0.3)[:, None])
+    w[torch.arange(rows, device="cuda"), x.argmin(1)] = 0
+    ends = w.cumsum(1)
+    at = u.double() * ends[:, 2]
+    inside = (ends - w < at[:, None] + 2.0 ** -20) & (at[:, None] - 2.0 ** -20 < ends) & (w > 0)
+    ok = torch.where(t > 0, inside.gather(1, got.clamp(0, 2)[:, None])[:, 0], got == x.argmax(1))
+    assert got.min() >= 0 and got.max() <= 2 and torch.all(ok)
