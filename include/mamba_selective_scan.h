@@ -613,6 +613,8 @@ int mss_scan_bwd_ws(void* stream, int32_t batch, int32_t length, int32_t dim, in
  * value stands for byte * scale; a scale is max(largest magnitude of its block / 448, 2^-126),
  * the bytes are rounded to nearest even. A NaN or infinity makes its block's scale NaN or
  * infinite. Bytes between a row's length and its stride are neither written nor relied on.
+ * Activations have at most MSS_FP8_MAX_TOKENS tokens and 65535 blocks of features, weights 65535 blocks
+ * of rows and MSS_FP8_MAX_FEATURES features (MSS_ERR_UNSUPPORTED beyond).
  *
  * mss_quant_fp8: x (features, tokens) float32 or bf16 with element strides stride_f, stride_t
  * (not negative) -> q [tokens][ldq], scales.
@@ -626,6 +628,8 @@ int mss_scan_bwd_ws(void* stream, int32_t batch, int32_t length, int32_t dim, in
  * (MSS_ERR_UNSUPPORTED beyond). Outputs overlap no operand. */
 #define MSS_FP8_BLOCK 128
 #define MSS_FP8_MM_MAX_TOKENS 524288
+#define MSS_FP8_MAX_TOKENS 134217728
+#define MSS_FP8_MAX_FEATURES 1073741824
 typedef struct mss_quant_fp8_args {
   int32_t features, tokens, io_dtype;
   int64_t stride_f, stride_t, ldq;

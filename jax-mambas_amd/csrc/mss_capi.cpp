@@ -878,7 +878,7 @@ int mss_quant_fp8(const mss_quant_fp8_args* a, void* stream) {
       a->stride_f < 0 || a->stride_t < 0 || !valid_rows8(a->q, a->ldq, a->features))
     return MSS_ERR_INVALID_ARGUMENT;
   if (too_far(a->features, a->stride_f) || too_far(a->tokens, a->stride_t) || too_far(a->tokens, a->ldq) ||
-      blocks8(a->features) > 65535)
+      blocks8(a->features) > 65535 || a->tokens > MSS_FP8_MAX_TOKENS)
     return MSS_ERR_UNSUPPORTED;
   const long long nq = span8(a->tokens, a->ldq, a->features), ns = 4 * blocks8(a->features) * a->tokens;
   const long long nx = ((a->features - 1) * a->stride_f + (a->tokens - 1) * a->stride_t + 1) *
@@ -902,7 +902,8 @@ int mss_norm_fp8(const mss_norm_fp8_args* a, void* stream) {
   if (a == nullptr || a->features <= 0 || a->tokens <= 0 || !(a->eps >= 0.f) || !a->h || !a->weight || !a->scales ||
       !valid_dtype(a->delta_dtype) || (a->delta && !a->hn) || !valid_rows8(a->q, a->ldq, a->features))
     return MSS_ERR_INVALID_ARGUMENT;
-  if (too_far(a->tokens, a->ldq) || blocks8(a->features) > 65535) return MSS_ERR_UNSUPPORTED;
+  if (too_far(a->tokens, a->ldq) || blocks8(a->features) > 65535 || a->tokens > MSS_FP8_MAX_TOKENS)
+    return MSS_ERR_UNSUPPORTED;
   const long long n = static_cast<long long>(a->features) * a->tokens;
   const long long nq = span8(a->tokens, a->ldq, a->features), ns = 4 * blocks8(a->features) * a->tokens;
   const long long nd = n * static_cast<long long>(dtype_size(a->delta_dtype));
@@ -936,7 +937,8 @@ int mss_quant_fp8_weight(const mss_quant_fp8_weight_args* a, void* stream) {
   if (a == nullptr || a->M <= 0 || a->K <= 0 || !a->w || !a->scales || !valid_dtype(a->io_dtype) || a->ldw < a->K ||
       !valid_rows8(a->q, a->ldq, a->K))
     return MSS_ERR_INVALID_ARGUMENT;
-  if (too_far(a->M, a->ldw) || too_far(a->M, a->ldq) || blocks8(a->M) > 65535) return MSS_ERR_UNSUPPORTED;
+  if (too_far(a->M, a->ldw) || too_far(a->M, a->ldq) || blocks8(a->M) > 65535 || a->K > MSS_FP8_MAX_FEATURES)
+    return MSS_ERR_UNSUPPORTED;
   const long long nq = span8(a->M, a->ldq, a->K), ns = 4 * blocks8(a->M) * blocks8(a->K);
   const long long nw = span8(a->M, a->ldw, a->K) * static_cast<long long>(dtype_size(a->io_dtype));
   if (bytes_overlap(a->q, nq, a->w, nw) || bytes_overlap(a->scales, ns, a->w, nw) || bytes_overlap(a->q, nq, a->scales, ns))
@@ -959,7 +961,7 @@ int mss_fp8_mm(const mss_fp8_mm_args* a, void* stream) {
     return MSS_ERR_INVALID_ARGUMENT;
   const long long rows = a->token_major ? a->T : a->M, cols = a->token_major ? a->M : a->T;
   if (a->ldc < cols) return MSS_ERR_INVALID_ARGUMENT;
-  if (a->T > MSS_FP8_MM_MAX_TOKENS || too_far(a->M, a->ldw) || too_far(a->T, a->ldx) || too_far(rows, a->ldc))
+  if (a->T > MSS_FP8_MM_MAX_TOKENS || a->K > MSS_FP8_MAX_FEATURES || too_far(a->M, a->ldw) || too_far(a->T, a->ldx) || too_far(rows, a->ldc))
     return MSS_ERR_UNSUPPORTED;
   const long long nc = span8(rows, a->ldc, cols) * static_cast<long long>(dtype_size(a->out_dtype));
   if (bytes_overlap(a->C, nc, a->W, span8(a->M, a->ldw, a->K)) || bytes_overlap(a->C, nc, a->X, span8(a->T, a->ldx, a->K)) ||

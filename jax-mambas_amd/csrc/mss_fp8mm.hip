@@ -470,7 +470,23 @@ typedef MmShape<64, 32, 1, 2> MmThin;
 //   1280 x 2560 x 64        7.0   5.9  17.0      5120 x 1280 x 16384     -   182   130
 //   64 x 64 x 16384        13.4   4.1     -      the same (f32)          -   307   356
 // 130 us are 1.65 PFLOP/s; the library's product with one scale an operand reaches 3.0 at 8192^3.
+// (A launch has fewer than 2^32 threads along x: M beyond 2^26 takes another one, a whole number of W's
+// blocks further on.)
+constexpr int kMmLaunchRows = 1 << 26;
+
 hipError_t launch_fp8mm(const Fp8MmParams& p, hipStream_t stream) {
+  if (p.M > kMmLaunchRows) {
+    Fp8MmParams part = p;
+    for (long long m = 0; m < p.M; m += kMmLaunchRows) {
+      part.M = static_cast<int>(p.M - m < kMmLaunchRows ? p.M - m : kMmLaunchRows);
+      part.w = p.w + m * p.ldw;
+      part.ws = p.ws + m / kFp8Block * ((p.K + kFp8Block - 1) / kFp8Block);
+      part.c = static_cast<char*>(p.c) + (p.token_major ? m : m * p.ldc) * (p.out_bf16 ? 2 : 4);
+      const hipError_t e = launch_fp8mm(part, stream);
+      if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+  }
   const double nkb = (p.K + kFp8Block - 1) / kFp8Block;
   const auto tiles = [&](double n) { return __builtin_ceil(p.M / n) * __builtin_ceil(p.T / n); };
   const double rows = 2.5 + fmax(0.00044 * tiles(16) * nkb, 0.0026 * tiles(16)) + 0.09 * nkb;

@@ -33,6 +33,8 @@ MSS_NORM_GEMV_MAX_FEATURES = 1024
 MSS_XENT_FUSED_MAX_VOCAB = 65536
 MSS_FP8_BLOCK = 128
 MSS_FP8_MM_MAX_TOKENS = 1 << 19
+MSS_FP8_MAX_TOKENS = 1 << 27
+MSS_FP8_MAX_FEATURES = 1 << 30
 MSS_SAMPLE_MAX_VOCAB = 1 << 20
 
 # Every symbol include/mamba_selective_scan.h declares.

@@ -592,3 +592,37 @@ def test_matmul_refuses_gradients(which):
         fp8_matmul(*a[:4], out=a[4])
     with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):
         fp8_matmul(*a[:4], out=a[4])
+
+
+@pytest.mark.parametrize("call,base,kw", [
+    ("mss_quant_fp8", "QUANT", dict(tokens=(1 << 27) + 1, scales=1 << 40)),
+    ("mss_norm_fp8", "NORM", dict(tokens=(1 << 27) + 1, h=1 << 46, delta=1 << 47, hn=1 << 48, scales=1 << 49)),
+    ("mss_quant_fp8_weight", "WEIGHT", dict(K=(1 << 30) + 1, ldw=1 << 31, ldq=1 << 31, w=1 << 46, q=1 << 47, scales=1 << 48)),
+    ("mss_fp8_mm", "MM", dict(K=(1 << 30) + 1, ldw=1 << 31, ldx=1 << 31, W=1 << 46, X=1 << 47, C=1 << 48)),
+])
+def test_sizes_past_a_launch(lib, call, base, kw):
+    """What a launch's 2^32 threads would not hold is refused."""
+    args = {"QUANT": (_lib.QuantFp8Args, QUANT), "NORM": (_lib.NormFp8Args, NORM),
+            "WEIGHT": (_lib.QuantFp8WeightArgs, WEIGHT), "MM": (_lib.Fp8MmArgs, MM)}[base]
+    assert getattr(lib, call)(args[0](**{**args[1], **kw}), None) == 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("token_major,out_dtype", [(False, torch.float32), (True, torch.bfloat16)])
+def test_matmul_more_rows_than_one_launch_takes(token_major, out_dtype):
+    """2^30 rows of W and some, 16 features, one token: each output against its float32 sum."""
+    m = (1 << 30) + 200
+    g = torch.Generator(device="cuda").manual_seed(51)
+    wq = torch.randint(0, 127, (m, 16), generator=g, device="cuda", dtype=torch.uint8).view(FP8)
+    ws = torch.rand(-(-m // BLOCK), 1, generator=g, device="cuda") + 0.5
+    xq, xs = quantize_fp8(rand(16, 1, seed=52))
+    got = fp8_matmul(wq, ws, xq, xs, out_dtype=out_dtype, token_major=token_major).view(m)
+    x = xq.float()[0] * xs[0, 0]
+    step = 1 << 25
+    for r in range(0, m, step):
+        w = wq[r:r + step].float()
+        s = ws[r // BLOCK:(r + step) // BLOCK, 0].repeat_interleave(BLOCK)[:w.shape[0]]
+        want, size = (w * x).sum(1) * s, (w * x.abs()).sum(1) * s
+        bound = size * (2.0 ** -10 if out_dtype == torch.bfloat16 else 23 * 2.0 ** -23)
+        bound += want.abs() * (torch.finfo(out_dtype).eps / 2) * 1.01
+        assert torch.all((got[r:r + step].float() - want).abs() <= bound)
