@@ -687,7 +687,7 @@ int mss_fp8_mm(const mss_fp8_mm_args* args, void* stream);
  * which the running weight of the words kept, in index order, exceeds uniform times their
  * weight. A temperature that is not above 0 gives the first word; a row without a word or with a
  * NaN gives -1. Settings are one value for all rows, or one a row where the pointer is set.
- * vocab at most MSS_SAMPLE_MAX_VOCAB (MSS_ERR_UNSUPPORTED beyond). */
+ * vocab at most MSS_SAMPLE_MAX_VOCAB (MSS_ERR_UNSUPPORTED beyond). tokens overlap no input. */
 #define MSS_SAMPLE_MAX_VOCAB 1048576
 typedef struct mss_sample_args {
   int32_t rows, vocab, io_dtype, top_k;

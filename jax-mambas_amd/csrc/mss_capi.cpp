@@ -994,8 +994,11 @@ int mss_sample(const mss_sample_args* a, void* stream) {
     return MSS_ERR_UNSUPPORTED;
   const long long nx = ((a->rows - 1) * a->stride_row + (a->vocab - 1) * a->stride_word + 1) *
                        static_cast<long long>(dtype_size(a->io_dtype));
-  if (bytes_overlap(a->tokens, 8LL * a->rows, a->logits, nx) || bytes_overlap(a->tokens, 8LL * a->rows, a->uniform, 4LL * a->rows))
-    return MSS_ERR_INVALID_ARGUMENT;
+  if (bytes_overlap(a->tokens, 8LL * a->rows, a->logits, nx)) return MSS_ERR_INVALID_ARGUMENT;
+  for (const void* v : {static_cast<const void*>(a->uniform), static_cast<const void*>(a->temperatures),
+                        static_cast<const void*>(a->top_ks), static_cast<const void*>(a->top_ps),
+                        static_cast<const void*>(a->min_ps)})  // rows are done in any order
+    if (bytes_overlap(a->tokens, 8LL * a->rows, v, 4LL * a->rows)) return MSS_ERR_INVALID_ARGUMENT;
   mss::SampleParams p{};
   p.rows = a->rows;
   p.vocab = a->vocab;

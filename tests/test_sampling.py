@@ -348,3 +348,9 @@ def test_more_rows_than_one_launch_takes():
     inside = (ends - w < at[:, None] + 2.0 ** -20) & (at[:, None] - 2.0 ** -20 < ends) & (w > 0)
     ok = torch.where(t > 0, inside.gather(1, got.clamp(0, 2)[:, None])[:, 0], got == x.argmax(1))
     assert got.min() >= 0 and got.max() <= 2 and torch.all(ok)
+
+
+@pytest.mark.parametrize("name", ["temperatures", "top_ks", "top_ps", "min_ps"])
+def test_tokens_over_settings(lib, name):
+    """Tokens written over settings that other rows have yet to read are refused."""
+    assert lib.mss_sample(_lib.SampleArgs(**{**BASE, name: (1 << 34) + 8}), None) == 1
