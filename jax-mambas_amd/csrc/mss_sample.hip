@@ -29,7 +29,7 @@
 //
 // Weights are added as integers of 2^-43, which makes every sum exact and independent of its
 // order: at most 2^20 words a row keep it below 2^63. (The one pass adds a thread's weights in
-// float64, in the row's order, and makes that an integer.)
+// float64, in the row's order, and makes that an integer: the same from run to run too.)
 #include <hip/hip_runtime.h>
 
 #include "mss_serve.h"
@@ -64,16 +64,17 @@ constexpr uint32_t kAbsent = 0x007fffffu;  // order_key(-inf)
 
 // w = 2^((v - m) c), c = log2(e) / temperature in two float32 parts. The product carries its
 // rounding error along (c's own would shift all weights the same way), the exponential is
-// v_exp_f32's. The difference is rounded: 2^-24 of an exponent y is 2^-24 y of a weight 2^y, and
-// words far below the largest are either a small part of the sum or many, whose errors cancel.
-// For 2^-100 < c < 2^100 and finite m only. A word that is absent or below 2^-64 counts as 2^-64,
-// which is no unit of the sums.
+// v_exp_f32's. The difference is rounded, which costs a weight 2^-y at most y ln 2 of 2^-24: words far
+// below the largest are a small part of the sum, unless they are many; at worst, a million equal ones at
+// y = 20 that outweigh the rest, a sum is off by 2^-20, and a running sum's share of it by half that.
+// For 2^-100 < c < 2^100 and finite m only. A word that is absent or below 2^-64 (2^-depth) counts as
+// that, which is no unit of the sums.
 struct FastWeight {
   float m, c, c_lo, least;
-  __device__ __forceinline__ FastWeight(float max, float temperature, float c_) : m(max), c(c_) {
+  __device__ __forceinline__ FastWeight(float max, float temperature, float c_, float depth = 64.f) : m(max), c(c_) {
     // what c = log2(e) / temperature lacks (log2(e) = 1.442695022 + 1.92596e-8)
     c_lo = (__builtin_fmaf(-c, temperature, 1.442695022f) + 1.92596301e-8f) / temperature;
-    least = -64.f / c;
+    least = -depth / c;
   }
   __device__ __forceinline__ float operator()(float v) const {
     const float d = fmaxf(v - m, least);
@@ -636,8 +637,8 @@ __device__ __forceinline__ float share_of(float top_p, int vocab) {
 
 // The list made in one pass, of a row that is not held: the bound comes from the first two chunks
 // (top-p's prefix is guessed at also where min-p would bound the list: some rows' first chunks have
-// no large logit), the weights of the row's sum are relative to their largest logit and are put right
-// when the row's is known. 256 x 131072 float32: top-k 50 45 us with a pass for the largest logit and
+// no large logit), the weights of the row's sum are added before the row's largest logit is known and
+// put right afterwards. 256 x 131072 float32: top-k 50 45 us with a pass for the largest logit and
 // one for the list, 36 with one; top-p 0.9 64 and 48, with min-p 0.001 58 and 50.
 struct OnePass {
   bool done;       // else the list does not hold the words, or the row is none to do this with
@@ -688,7 +689,13 @@ __device__ __forceinline__ OnePass list_in_one_pass(SampleShared& s, const words
   }
   if (threadIdx.x == 0) s.list_n = 0;
   __syncthreads();
-  const FastWeight weight(m, temperature, c);
+  // The weights are relative to 2^0 where the logits allow it, else to that largest one: no difference
+  // that is rounded lies between a word that counts and the row's own largest logit. (From 0 there is none;
+  // from m, at m c beyond 40, it is exact for logits between m and twice, or half, of it, and words below
+  // do not count. Rows whose largest is further off are left to the exact sum.)
+  const bool plain = m * c >= -40.f && m * c <= 60.f;
+  const float from = plain ? 0.f : m;
+  const FastWeight weight(from, temperature, c, plain ? 120.f : 64.f);
   const bool whole = by_p && !by_k;
   double all = 0;
   float mine = m;
@@ -707,9 +714,10 @@ __device__ __forceinline__ OnePass list_in_one_pass(SampleShared& s, const words
   });
   out.m = top_of(mine);
   out.nan = __syncthreads_or(nan);
-  const FastWeight shift(out.m, temperature, c);
-  if (whole) out.all = block_total(s, static_cast<u64>(all * (static_cast<double>(shift(m)) * kFixed)));
-  out.done = s.list_n <= kSampleList && (out.m - m) * c < 60.f;
+  const bool exact = plain || out.m == m || out.m <= (m > 0.f ? 2.f * m : 0.5f * m);
+  out.done = s.list_n <= kSampleList && (out.m - m) * c < 60.f && (exact || !whole);
+  const FastWeight shift(out.m, temperature, c, 126.f);
+  if (whole) out.all = block_total(s, out.done ? static_cast<u64>(all * (static_cast<double>(shift(from)) * kFixed)) : 0);
   return out;
 }
 

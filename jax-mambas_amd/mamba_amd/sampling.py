@@ -14,7 +14,8 @@ the lowest index at which the running weight of the words kept, in index order, 
 word, or with a NaN, gives -1. Each setting is a number, or a tensor with one value a row
 (float32; top_k int32).
 
-Sums are exact (integer) and the same from run to run. There is no CPU path.
+Weights are float32 and added as integers, or, for top-p over rows of more than 65536 words, in float64
+in a fixed order: tokens are the same from run to run. There is no CPU path.
 """
 from __future__ import annotations
 

@@ -354,3 +354,29 @@ def test_more_rows_than_one_launch_takes():
 def test_tokens_over_settings(lib, name):
     """Tokens written over settings that other rows have yet to read are refused."""
     assert lib.mss_sample(_lib.SampleArgs(**{**BASE, name: (1 << 34) + 8}), None) == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("temperature", [1.0, 0.5])
+@pytest.mark.parametrize("base", [0.1, -3.2, -17.3, 50.7, 700.3])
+def test_top_p_of_long_rows_whose_beginning_is_far_below(base, temperature):
+    """Rows read once whose first words lie about 32 T below the rest, on both sides of a power of two, where
+    rounded differences differ most: the whole sum is as exact as the list's. Six thousand words of forty
+    logits share the weight, and top_p ends 10^-6 of the sum before and behind a border between two; the
+    last word kept is drawn."""
+    vocab, rows, grid = 70001, 64, 2.0 ** -5
+    rng = np.random.default_rng(int(abs(base) * 10))
+    x = np.full((rows, vocab), -np.inf, np.float32)
+    first = (base + rng.uniform(-0.1, 0.1, rows)).astype(np.float32)
+    top = np.ceil((first.astype(np.float64) + 32 * temperature) / grid) * grid
+    words = top[:, None] - grid * np.arange(1, 41)  # exact in float32
+    x[:, 5], x[:, 20000], x[:, 30000:36000] = first, top, np.repeat(words, 150, 1)
+    w = np.exp((x[:, 20000:36000].astype(np.float64) - top[:, None]) / temperature)
+    mass = np.cumsum(w, 1)
+    at = 10000 + rng.integers(1000, 5900, rows)
+    border = mass[np.arange(rows), at]  # the weight up to a word: the one behind it begins there
+    top_p = border / mass[:, -1] + np.where(np.arange(rows) % 2, 1e-6, -1e-6)
+    u = torch.full((rows,), 1 - 2.0 ** -24, device="cuda")
+    kw = dict(temperature=temperature, top_p=torch.from_numpy(top_p.astype(np.float32)).to("cuda"))
+    x = torch.from_numpy(x).to("cuda")
+    check(x, u, sample_tokens(x, u, **kw), **kw)
