@@ -624,7 +624,11 @@ int mss_scan_bwd_ws(void* stream, int32_t batch, int32_t length, int32_t dim, in
  * mss_quant_fp8_weight: w (M, K) float32 or bf16, rows of stride ldw elements -> q, scales.
  * mss_fp8_mm: C = W X^T with W (M, K) in weight form and X (T, K) in activation form, C float32
  * or bf16 (out_dtype): [M][ldc], or [T][ldc] with token_major != 0 (ldc in elements). Each
- * block of 128 features is summed and scaled in float32. T at most MSS_FP8_MM_MAX_TOKENS
+ * block of 128 features is summed, and scaled and added in float32 (by the float32 product of its two
+ * scales). MSS_F32: a block's products are exact and its sum float32. MSS_BF16: the same, or the 8-bit
+ * matrix instructions' sum, in which each 8 neighbouring products lose what lies below 2^-13 of the
+ * largest of them: less than the output's rounding, but for sums whose largest products cancel each
+ * other (MSS_F32 keeps those). T at most MSS_FP8_MM_MAX_TOKENS
  * (MSS_ERR_UNSUPPORTED beyond). Outputs overlap no operand. */
 #define MSS_FP8_BLOCK 128
 #define MSS_FP8_MM_MAX_TOKENS 524288

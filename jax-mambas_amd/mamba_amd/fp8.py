@@ -19,8 +19,10 @@ q (M, K), scales (ceil(M / 128), ceil(K / 128)), one for each 128 x 128 block.
 
 ``fp8_matmul(wq, w_scales, xq, x_scales, out_dtype=torch.bfloat16, token_major=False, out=None)``
 — W @ X for a weight and activations in 8-bit form: (M, T), or (T, M) with token_major; each
-block of 128 features summed on the matrix cores and scaled in float32, rounded to out_dtype
-(bfloat16 or float32) once.
+block of 128 features summed on the matrix cores, scaled and added in float32, rounded to out_dtype
+(bfloat16 or float32) once. With out_dtype float32 a block's sum is float32 too. With bfloat16 it may
+come from the 8-bit matrix instructions, which drop of each 8 neighbouring products what lies below
+2^-13 of the largest: less than the output's rounding, except where large products cancel each other.
 
 A NaN or infinity makes what its block stands for NaN. Inference only (no autograd); there is no
 CPU path.

@@ -626,3 +626,28 @@ def test_matmul_more_rows_than_one_launch_takes(token_major, out_dtype):
         bound = size * (2.0 ** -10 if out_dtype == torch.bfloat16 else 23 * 2.0 ** -23)
         bound += want.abs() * (torch.finfo(out_dtype).eps / 2) * 1.01
         assert torch.all((got[r:r + step].float() - want).abs() <= bound)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("token_major", [False, True])
+@pytest.mark.parametrize("m,k,t", [(16, 128, 16), (40, 256, 5), (130, 1100, 70), (1280, 2560, 333), (20000, 300, 7),
+                                   (2100, 200, 2200), (300, 1024, 140)])
+def test_matmul_float32_keeps_what_outliers_hide(m, k, t, token_major):
+    """Small whole numbers next to large products that cancel within 8 features: every sum is a whole
+    number below 2^24 on the way, so a float32 output is exact. A bf16 output is off by its rounding and
+    at most 7 of the 8 products' 2^-13 of the largest, in every 8."""
+    g = torch.Generator(device="cuda").manual_seed(61)
+    w = torch.randint(-4, 5, (m, k), generator=g, device="cuda").float()
+    x = torch.randint(-4, 5, (t, k), generator=g, device="cuda").float()
+    at = torch.arange(3, k - 1, 128, device="cuda")
+    w[:, at], w[:, at + 1], x[:, at], x[:, at + 1] = 448, -448, 448, 448
+    want = (w.double().cpu() @ x.double().cpu().t()).cuda()
+    rows = lambda v: torch.nn.functional.pad(v, (0, -k % 16)).to(FP8)[:, :k]  # noqa: E731
+    one = lambda *s: torch.ones(*s, device="cuda")  # noqa: E731
+    kb = -(-k // BLOCK)
+    a = rows(w), one(-(-m // BLOCK), kb), rows(x), one(kb, t)
+    got = fp8_matmul(*a, out_dtype=torch.float32, token_major=token_major)
+    assert torch.equal((got.t() if token_major else got).double(), want)
+    got = fp8_matmul(*a, token_major=token_major).double()
+    bound = 7 * 2.0 ** -13 * (448 * 448 * len(at) + 16 * (k // 8 + 1))
+    assert torch.all(((got.t() if token_major else got) - want).abs() <= bound + (want.abs() + bound) * 2.0 ** -8)
