@@ -90,7 +90,7 @@ __device__ __forceinline__ void store_row16(unsigned char* __restrict__ q, const
 }
 
 // --------------------------------------------------------------- quantisation, token-contiguous
-// A workgroup: one block of features, 64 tokens. A thread holds 16 bytes (kTV tokens) of 4
+// A workgroup: one block of features, 64 tokens (of 64 or more). A thread holds 16 bytes (kTV tokens) of 4
 // features; a feature's 64 tokens are one 128- or 256-byte read.
 template <typename io_t>
 __global__ __launch_bounds__(128 * sizeof(io_t)) void quant_tile_kernel(QuantParams p) {
@@ -100,12 +100,12 @@ __global__ __launch_bounds__(128 * sizeof(io_t)) void quant_tile_kernel(QuantPar
   __shared__ alignas(8) uint32_t s_q[64 * kPitch];
   const int l = threadIdx.x % kLanes, g = threadIdx.x / kLanes, wave = threadIdx.x / 64;
   long long t0 = blockIdx.x * 64ll;
-  if (t0 + 64 > p.tokens && p.tokens >= 64) t0 = p.tokens - 64;  // the last tile, whole: some tokens come out twice
+  if (t0 + 64 > p.tokens) t0 = p.tokens - 64;  // the last tile, whole: some tokens come out twice
   const int b = blockIdx.y, f0 = b * kFp8Block + 4 * g;
   const long long t = t0 + l * kTV;
   const io_t* __restrict__ x = static_cast<const io_t*>(p.x) + t;
   float v[4][kTV];
-  if (t0 + 64 <= p.tokens) {
+  {
     io_t raw[4][kTV];
 #pragma unroll
     for (int i = 0; i < 4; ++i) __builtin_memcpy(raw[i], x + min(f0 + i, p.features - 1) * p.sf, sizeof(raw[i]));
@@ -113,11 +113,6 @@ __global__ __launch_bounds__(128 * sizeof(io_t)) void quant_tile_kernel(QuantPar
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < kTV; ++j) v[i][j] = f0 + i < p.features ? to_f32(raw[i][j]) : 0.f;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < kTV; ++j) v[i][j] = f0 + i < p.features && t + j < p.tokens ? to_f32(x[(f0 + i) * p.sf + j]) : 0.f;
   }
 #pragma unroll
   for (int j = 0; j < kTV; ++j) {
@@ -133,16 +128,15 @@ __global__ __launch_bounds__(128 * sizeof(io_t)) void quant_tile_kernel(QuantPar
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) m = max(m, s_m[i][l * kTV + j]);
     const ToFp8 to(m);
-    if (g == 0 && t + j < p.tokens) p.scales[static_cast<long long>(b) * p.tokens + t + j] = to.scale;
+    if (g == 0) p.scales[static_cast<long long>(b) * p.tokens + t + j] = to.scale;
     s_q[(l * kTV + j) * kPitch + g] = pack_fp8x4(to(v[0][j]), to(v[1][j]), to(v[2][j]), to(v[3][j]));
   }
   __syncthreads();
 #pragma unroll
   for (int i = threadIdx.x; i < 64 * (kFp8Block / 16); i += 64 * kWaves) {
     const int row = i / (kFp8Block / 16), c = i % (kFp8Block / 16);
-    if (t0 + row < p.tokens)
-      store_row16(p.q + (t0 + row) * p.ldq + b * kFp8Block + 16 * c, s_q + row * kPitch + 4 * c, b * kFp8Block + 16 * c,
-                  p.features);
+    store_row16(p.q + (t0 + row) * p.ldq + b * kFp8Block + 16 * c, s_q + row * kPitch + 4 * c, b * kFp8Block + 16 * c,
+                p.features);
   }
 }
 
@@ -569,12 +563,14 @@ __global__ __launch_bounds__(512) void norm_fp8_wide_kernel(QuantParams p) {
 
 // --------------------------------------------------------------------------------- launches
 // Where each kernel starts to win (MI355X, us for features x tokens).
-// quant: rows/tile 2560 x 32 5.0/4.3, x 8 3.1/3.9; 2560 x 16384 bf16 81/26.4, 4.8 TB/s of the 5.2 that
-// a copy reaches.
-constexpr int kQuantTileTokens = 32;
+// quant: rows while a workgroup of them for each CU (float32) or two (bf16) hold all tokens, and for fewer
+// than 64; rows/tile, bf16: 768 x 400 3.5/4.3, 2560 x 64 3.4/4.3, x 400 4.3/4.5, 5120 x 128 4.0/4.3, x 200
+// 5.0/4.4, x 400 6.4/5.3; float32: 768 x 400 3.2/3.5, 2560 x 128 3.2/3.4, x 200 4.0/3.5, 5120 x 128 4.0/3.5.
+// 2560 x 16384 bf16: rows 81, tiles 24.2, at the rate of a copy (5.2 TB/s).
+constexpr int kQuantTileTokens = 64;
 // norm, bf16 delta: a token a workgroup 1280 x 128 6.0, x 256 9.0, x 512 13.8; tiles of 8 tokens x 256
-// 8.7, x 512 9.2, x 2048 12.4, x 4096 20; of 16 tokens x 2048 13.3, x 4096 14.7, x 8192 23.5, x 16384 58;
-// of 32 tokens x 4096 17, x 8192 21.6, x 16384 45: 5.1 TB/s.
+// 8.9, x 512 9.5, x 2048 12.6, x 4096 20; of 16 tokens x 2048 13.3, x 4096 15.4, x 8192 23.5, x 16384 58;
+// of 32 tokens x 4096 17, x 8192 22, x 16384 45: 5.1 TB/s.
 constexpr int kNormTileTokens = 256;
 constexpr int kNormNarrowTokens = 2048;
 constexpr int kNormMiddleTokens = 6144;
@@ -582,7 +578,8 @@ constexpr int kNormMiddleTokens = 6144;
 template <typename io_t>
 static void launch_quant(const QuantParams& p, hipStream_t stream) {
   const unsigned blocks = (p.features + kFp8Block - 1) / kFp8Block;
-  if (p.st == 1 && p.tokens >= kQuantTileTokens) {
+  const long long rows = (p.tokens + 15ll) / 16 * blocks;  // workgroups
+  if (p.st == 1 && p.tokens >= kQuantTileTokens && rows > (sizeof(io_t) == 2 ? 512 : 256)) {
     hipLaunchKernelGGL((quant_tile_kernel<io_t>), dim3((p.tokens + 63) / 64, blocks), dim3(128 * sizeof(io_t)), 0, stream, p);
     return;
   }

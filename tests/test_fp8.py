@@ -651,3 +651,13 @@ def test_matmul_float32_keeps_what_outliers_hide(m, k, t, token_major):
     got = fp8_matmul(*a, token_major=token_major).double()
     bound = 7 * 2.0 ** -13 * (448 * 448 * len(at) + 16 * (k // 8 + 1))
     assert torch.all(((got.t() if token_major else got) - want).abs() <= bound + (want.abs() + bound) * 2.0 ** -8)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("f,t", [(2560, 200), (2560, 208), (2560, 400), (2560, 417), (5120, 129), (5120, 205), (129, 4099),
+                                 (64, 8200), (20000, 63), (20000, 64), (9000, 127)])
+def test_quantise_both_sides_of_the_tiles(f, t, dtype):
+    """Token-contiguous activations about the size from which tiles of 64 tokens take them, whole and not."""
+    for layout in ("channel", "rows_apart"):
+        test_quantise(f, t, layout, dtype)
