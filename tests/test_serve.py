@@ -231,3 +231,71 @@ def test_a_row_without_a_word_stays_without(batch, graph):
         assert torch.equal(token, got[i])
         logits = m.step(token, caches)
         assert torch.isnan(logits[1]).all() and torch.isfinite(logits[keep]).all()
+
+
+def e4m3(v):
+    """float64 values of magnitude at most 448, rounded to e4m3 (nearest, ties to even)."""
+    step = torch.exp2(torch.floor(torch.log2(v.abs().clamp_min(2.0 ** -6))) - 3)
+    return torch.round(v / step) * step
+
+
+def eight_bit(y, rows):
+    """What a float64 matrix (.., features) stands for in 8 bits, one scale for `rows` rows and 128 features."""
+    out = torch.empty_like(y)
+    for i in range(0, y.shape[0], rows):
+        for j in range(0, y.shape[1], 128):
+            part = y[i:i + rows, j:j + 128]
+            scale = (part.abs().max() / 448).clamp_min(2.0 ** -126)
+            out[i:i + rows, j:j + 128] = e4m3(part / scale) * scale
+    return out
+
+
+def logits_in_64_bits(model, tokens):
+    """Every position's logits of one sequence: the model in float64 with 8-bit products, the S6
+    projections' weights in bf16, nothing else rounded."""
+    weight = {k: v.detach().double().cpu() for k, v in model.named_parameters()}
+    silu, softplus = torch.nn.functional.silu, torch.nn.functional.softplus
+    norm = lambda h, w: h / torch.sqrt(h.square().mean(1, keepdim=True) + 1e-5) * w  # noqa: E731
+    product = lambda x, w: eight_bit(x, 1) @ eight_bit(w, 128).t()  # noqa: E731
+    h = weight["embedding"][tokens.cpu()]
+    for i in range(LAYERS):
+        p = {k[len(f"blocks.{i}."):]: v for k, v in weight.items() if k.startswith(f"blocks.{i}.")}
+        x = norm(h, p["norm.weight"])
+        xin, z = product(x, torch.cat([p["in_proj"], p["z_proj"]])).split(2 * DIM, 1)
+        k = p["conv_weight"].shape[1]
+        wide = torch.cat([xin.new_zeros(k - 1, 2 * DIM), xin])
+        u = silu(p["conv_bias"] + sum(p["conv_weight"][:, j] * wide[j:j + len(xin)] for j in range(k)))
+        r, n = p["s6.dt_proj"].shape[1], p["s6.A_log"].shape[1]
+        dbl = u @ p["s6.x_proj"].bfloat16().double().t()
+        dt = softplus(dbl[:, :r] @ p["s6.dt_proj"].bfloat16().double().t() + p["s6.dt_bias"])
+        A, state, y = -torch.exp(p["s6.A_log"]), u.new_zeros(2 * DIM, n), []
+        for t in range(len(u)):
+            state = torch.exp(dt[t][:, None] * A) * state + (dt[t] * u[t])[:, None] * dbl[t, r:r + n]
+            y.append(state @ dbl[t, r + n:] + p["s6.D"] * u[t])
+        h = h + product(torch.stack(y) * silu(z), p["out_proj"])
+    return product(norm(h, weight["final_norm.weight"]), weight["embedding"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("length", [1, 2, 5, 70, 300])
+def test_path_against_64_bits(length):
+    """Prompt and three steps against the same model in float64 with the same roundings to 8 bits. The
+    path's roundings to bf16 move an 8-bit operand by 2^-8 of itself; that takes it over a border, which
+    lie at least 2^-4 of it apart, with a probability of at most 2^-4, and then by a step, at most 2^-3:
+    2^-5 in root mean square for each of the five products, together sqrt(5) 2^-5 = 0.07 of the logits'
+    size; twice that is allowed."""
+    model = lm(12)
+    with torch.no_grad():
+        for name, p in model.named_parameters():  # norms and D that are not all one
+            if name.endswith(("norm.weight", "s6.D")):
+                p.mul_(1 + 0.3 * torch.randn_like(p))
+    m = Fp8LM(model)
+    tokens = prompt(2, length + 3, seed=length)
+    want = torch.stack([logits_in_64_bits(model, row) for row in tokens])
+    logits, caches = m.prefill(tokens[:, :length])
+    for i in range(4):
+        err = float((logits.double().cpu() - want[:, length - 1 + i]).norm() / want[:, length - 1 + i].norm())
+        print("position", length - 1 + i, "relative error", err, flush=True)
+        assert err < 0.14
+        if i < 3:
+            logits = m.step(tokens[:, length + i], caches)
