@@ -661,3 +661,50 @@ def test_quantise_both_sides_of_the_tiles(f, t, dtype):
     """Token-contiguous activations about the size from which tiles of 64 tokens take them, whole and not."""
     for layout in ("channel", "rows_apart"):
         test_quantise(f, t, layout, dtype)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """More than 2^32 values in every operand of a kind: the last tokens, and rows, against the same by
+    themselves."""
+    g = torch.Generator(device="cuda").manual_seed(71)
+    f, t = 257, (1 << 24) + 5
+    x = torch.randn(f, t, generator=g, device="cuda", dtype=torch.bfloat16)
+    same = lambda a, b: all(torch.equal(i.float(), j.float()) for i, j in zip(a, b))  # noqa: E731
+    end = slice(t - 100, t)
+    q, s = quantize_fp8(x)
+    assert same((q[end], s[:, end]), quantize_fp8(x[:, end].contiguous()))
+    del q, s
+    h = x.float()
+    w = torch.ones(f, device="cuda")
+    hn, q, s = add_rmsnorm_fp8(h, x, w)
+    want = add_rmsnorm_fp8(h[:, end].contiguous(), x[:, end].contiguous(), w)
+    assert torch.equal(hn[:, end], want[0])
+    # (the kernel for few tokens adds the squares in another order: scales to float32 roundings of f + 6)
+    assert torch.equal(q[end].float(), want[1].float())
+    assert torch.allclose(s[:, end], want[2], rtol=(f + 12) * 2.0 ** -24, atol=0)
+    del x, h, hn, q, s
+    m, k, t = 50280, 32, 90001
+    wq, ws = quantize_fp8_weight(torch.randn(m, k, generator=g, device="cuda"))
+    xq, xs = quantize_fp8(torch.randn(k, t, generator=g, device="cuda"))
+    for token_major in (False, True):
+        got = fp8_matmul(wq, ws, xq, xs, token_major=token_major)
+        if token_major:
+            got = got.t()
+        part = slice(m // BLOCK * BLOCK, m)
+        check_mm(got[part, -300:], wq[part], ws[-1:], xq[-300:], xs[:, -300:].contiguous(), False, torch.bfloat16)
+        del got
+
+
+@pytest.mark.gpu
+def test_weight_offsets_past_32_bits():
+    m, k = 4000, 1100000
+    w = torch.randn(m, k, generator=torch.Generator(device="cuda").manual_seed(72), device="cuda", dtype=torch.bfloat16)
+    q, s = quantize_fp8_weight(w)
+    end = m // BLOCK * BLOCK
+    q1, s1 = quantize_fp8_weight(w[end:].contiguous())
+    assert torch.equal(q[end:].float(), q1.float()) and torch.equal(s[-1:], s1)
+    x, xs = quantize_fp8(torch.randn(k, 3, device="cuda"))
+    for out_dtype in (torch.bfloat16, torch.float32):
+        got = fp8_matmul(q, s, x, xs, out_dtype=out_dtype)
+        check_mm(got[end:], q1, s1, x, xs, False, out_dtype)

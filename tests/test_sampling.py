@@ -380,3 +380,16 @@ def test_top_p_of_long_rows_whose_beginning_is_far_below(base, temperature):
     kw = dict(temperature=temperature, top_p=torch.from_numpy(top_p.astype(np.float32)).to("cuda"))
     x = torch.from_numpy(x).to("cuda")
     check(x, u, sample_tokens(x, u, **kw), **kw)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """More than 2^32 logits: the last rows against the same by themselves."""
+    rows, vocab = 4200, 1 << 20
+    g = torch.Generator(device="cuda").manual_seed(81)
+    x = torch.randn(rows, vocab, generator=g, device="cuda", dtype=torch.bfloat16)
+    u = torch.rand(rows, generator=g, device="cuda")
+    for kw in (dict(top_k=50, top_p=0.9), dict(temperature=0.0), dict()):
+        got = sample_tokens(x, u, **kw)
+        assert torch.equal(got[-40:], sample_tokens(x[-40:].clone(), u[-40:], **kw))
+        check(x[-2:], u[-2:], got[-2:], **kw)
