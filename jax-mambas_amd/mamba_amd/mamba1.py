@@ -188,6 +188,18 @@ class ShadowWeights:
         self._table = (table, len(entries), tile0, ptrs)
         return self._table
 
+    def rebind(self, params):
+        """Takes `params`, of the same shapes, for the masters (a model whose parameters were replaced by
+        new ones): the copies stay where they lie and are written at the next refresh. Without
+        transposed groups only."""
+        if self.groups or [p.shape for p in params] != [p.shape for p in self.params]:
+            raise ValueError("only ungrouped weights can be replaced, by weights of their shapes")
+        self.params = list(params)
+        if self.bufs is not None:
+            self.by_id = {id(p): b for p, b in zip(self.params, self.bufs)}
+            self.offsets = {id(p): o for p, o in zip(self.params, self.offsets.values())}
+        self._table = self._current = None
+
     def _token(self):
         return tuple((p.data_ptr(), p._version) for p in self.params)
 

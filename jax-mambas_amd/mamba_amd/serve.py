@@ -87,7 +87,11 @@ class Fp8LM:
             torch._foreach_copy_(self._ends, new)
             for mine, b, A in zip(self._blocks, m.blocks, matrices):
                 torch._foreach_copy_(mine.tensors(), _Block(b, A).tensors())
-        self._small._current = None  # (a master may have been changed behind autograd's version counter)
+        # (the masters may have been replaced, or changed behind autograd's version counter)
+        for mine, b in zip(self._blocks, m.blocks):
+            for k in _SHADOWED:
+                mine.s6._parameters[k] = b.s6._parameters[k]
+        self._small.rebind([getattr(b.s6, w) for b in m.blocks for w in _SHADOWED])
         self._small.refresh(torch.bfloat16)
 
     def _logits(self, h, delta):

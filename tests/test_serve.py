@@ -299,3 +299,31 @@ def test_path_against_64_bits(length):
         assert err < 0.14
         if i < 3:
             logits = m.step(tokens[:, length + i], caches)
+
+
+@pytest.mark.gpu
+def test_refresh_after_the_parameters_were_replaced():
+    """A state dict assigned to the model puts other Parameter objects in place of those Fp8LM has seen:
+    nothing changes until refresh(), and then everything does, a captured step's weights too."""
+    model, other = lm(13), lm(14)
+    m = Fp8LM(model)
+    tokens = prompt(3, 7)
+    held, caches = m.prefill(tokens)
+    token = tokens[:, 0].clone()
+    start = [c["ssm"].clone() for c in caches], [c["conv"].clone() for c in caches]
+    graph = torch.cuda.CUDAGraph()
+    m.step(token, caches)
+    with torch.cuda.graph(graph):
+        logits = m.step(token, caches)
+    model.load_state_dict(other.state_dict(), assign=True)
+    assert torch.equal(m.prefill(tokens)[0], held)
+    m.refresh()
+    fresh = Fp8LM(other)
+    want, new = fresh.prefill(tokens)
+    assert torch.equal(m.prefill(tokens)[0], want)
+    for _ in range(2):
+        for c, n, ssm, conv in zip(caches, new, *start):
+            c["ssm"].copy_(ssm), c["conv"].copy_(conv), n["ssm"].copy_(ssm), n["conv"].copy_(conv)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(logits, fresh.step(token, new))
