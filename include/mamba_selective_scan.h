@@ -48,7 +48,7 @@
 extern "C" {
 #endif
 
-#define MSS_ABI_VERSION 19
+#define MSS_ABI_VERSION 20
 /* dstate limits (MSS_ERR_UNSUPPORTED beyond, MSS_ERR_INVALID_ARGUMENT beyond 256):
  * MSS_MAX_DSTATE_WIDE for the float32 real-A scans — mss_fwd / mss_bwd / mss_bwd_noalloc with
  * io and bc dtype MSS_F32, and the reference-signature mss_scan_* entry points (whose C
@@ -707,6 +707,87 @@ typedef struct mss_sample_args {
 } mss_sample_args;
 
 int mss_sample(const mss_sample_args* args, void* stream);
+
+/* --- Losses towards a target word or a teacher's list (no counterpart symbols in the reference, which
+ * takes a cross-entropy of its head's logits: experiments/mamba_inductionheads.py:129-136). ------
+ * A row (token) wants a distribution q over words of the vocabulary: its target (targets; a target of
+ * ignore_index: none), or, of a list of top words (ids; negative: none) with a teacher's logits (float32
+ * or bf16; -inf: none), softmax(teacher / temperature) over the entries that count; a word that stands
+ * in a list more than once has the sum of its entries. With s = logits / temperature,
+ *   loss = temperature^2 sum_k q_k (log q_k - s[word_k] + log sum_v exp s[v]),
+ *   d loss / d logit[v] = temperature (softmax(s)[v] - q_v).
+ * A row without a word does not count: its loss is 0 and its gradients are zeros, whatever it holds. A row
+ * with a word that is not below vocab, or a teacher logit that is NaN or +inf in an entry that counts, has
+ * a NaN loss and NaN gradients. reduction: MSS_LOSS_NONE (grad then has one value a row), MSS_LOSS_SUM,
+ * MSS_LOSS_MEAN (over the rows that count; 0 without any). loss: [rows], always written; mean: [2] the
+ * reduced loss, and what a mean multiplies by (written unless MSS_LOSS_NONE, read by the backward calls).
+ * saved: what the backward calls read of a forward one, mss_*_saved_bytes bytes, 256-byte aligned.
+ * ids, teacher, targets and all outputs are contiguous; outputs overlap no input. top is 1 to
+ * MSS_LOSS_MAX_TOP, rows * top at most 2^27.
+ *
+ * mss_linear_loss: logits = x^T W^T for x (features, tokens) with element strides stride_f, stride_t (not
+ * negative) and W (vocab, features) with rows of stride ldw, both of io_dtype; the logits are not
+ * kept. With targets (top 0) or lists. Sums are float32; with MSS_BF16 the backward rounds the logits'
+ * gradient to bf16 once, in pieces of the vocabulary of at most 1 GiB in the workspace. dx: [features][tokens]
+ * of io_dtype, dweight: [vocab][features] of dw_dtype; either may be NULL. tokens and vocab at most 2^20, their
+ * product 2^38, features at most 65536 (MSS_ERR_UNSUPPORTED beyond). workspace: for the forward and the
+ * backward call each, mss_linear_loss_workspace_bytes, 256-byte aligned, nothing kept in it.
+ *
+ * mss_distill: logits [rows][vocab] of io_dtype, rows of stride ld (at least vocab), lists only.
+ * mss_distill_fwd_grad is both directions in one reading, dlogits for an upstream gradient of 1 and not
+ * MSS_LOSS_NONE; mss_distill_regrad then writes dlogits anew for *grad, unless that is 1. vocab at most
+ * 2^30. */
+#define MSS_LOSS_NONE 0
+#define MSS_LOSS_SUM 1
+#define MSS_LOSS_MEAN 2
+#define MSS_LOSS_MAX_TOP 1024
+typedef struct mss_linear_loss_args {
+  int32_t tokens, features, vocab, top;
+  int32_t io_dtype, teacher_dtype, dw_dtype, reduction;
+  float temperature; /* above 0; 1 with targets */
+  int64_t ignore_index;
+  int64_t stride_f, stride_t, ldw;
+  const void* x;
+  const void* weight;
+  const int64_t* targets; /* [tokens], top 0 */
+  const int64_t* ids;     /* [tokens][top] */
+  const void* teacher;    /* [tokens][top] */
+  float* loss;
+  float* mean;
+  void* saved;
+  void* workspace;
+  size_t saved_bytes, workspace_bytes;
+  const float* grad; /* backward: [1], or [tokens] */
+  void* dx;
+  void* dweight;
+} mss_linear_loss_args;
+
+size_t mss_linear_loss_saved_bytes(const mss_linear_loss_args* args);
+size_t mss_linear_loss_workspace_bytes(const mss_linear_loss_args* args, int32_t backward);
+int mss_linear_loss_fwd(const mss_linear_loss_args* args, void* stream);
+int mss_linear_loss_bwd(const mss_linear_loss_args* args, void* stream);
+
+typedef struct mss_distill_args {
+  int32_t rows, vocab, top;
+  int32_t io_dtype, teacher_dtype, reduction;
+  float temperature;
+  int64_t ld;
+  const void* logits;
+  const int64_t* ids;  /* [rows][top] */
+  const void* teacher; /* [rows][top] */
+  float* loss;
+  float* mean;
+  void* saved;
+  size_t saved_bytes;
+  const float* grad; /* [1], or [rows] */
+  void* dlogits;     /* [rows][vocab] */
+} mss_distill_args;
+
+size_t mss_distill_saved_bytes(const mss_distill_args* args);
+int mss_distill_fwd(const mss_distill_args* args, void* stream);
+int mss_distill_bwd(const mss_distill_args* args, void* stream);
+int mss_distill_fwd_grad(const mss_distill_args* args, void* stream);
+int mss_distill_regrad(const mss_distill_args* args, void* stream);
 
 /* Human-readable text for a status code. */
 const char* mss_strerror(int status);

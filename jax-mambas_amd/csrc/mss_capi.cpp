@@ -19,6 +19,7 @@
 
 #include "../../include/mamba_selective_scan.h"
 #include "mss_common.h"
+#include "mss_loss.h"
 #include "mss_serve.h"
 
 namespace mss {
@@ -73,6 +74,18 @@ int hip_fail(hipError_t e, const char* what) {
 }
 
 size_t dtype_size(int dt) { return dt == MSS_BF16 ? 2 : 4; }
+
+// A buffer's parts one after the other, each from a multiple of 256 bytes.
+struct Carve {
+  char* base;
+  size_t at;
+  template <typename T>
+  T* take(long long n) {
+    T* p = base ? reinterpret_cast<T*>(base + at) : nullptr;
+    at += (static_cast<size_t>(n) * sizeof(T) + 255) / 256 * 256;
+    return p;
+  }
+};
 
 bool aligned16(const void* p) { return p == nullptr || (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 bool aligned8(const void* p) { return p == nullptr || (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
@@ -1593,6 +1606,277 @@ int mss_scan_bwd(void* stream, int32_t batch, int32_t length, int32_t dim, int32
   e = hipFreeAsync(ws, st);
   if (s != MSS_OK) return s;
   return e == hipSuccess ? MSS_OK : hip_fail(e, "freeing backward workspace");
+}
+
+// ------------------------------------------------------------------ losses
+namespace {
+struct Span {
+  const void* p;
+  long long n;
+};
+
+// Whether an output (those given: not NULL) meets an input or another output.
+bool outputs_meet(const Span* out, int no, const Span* in, int ni) {
+  for (int i = 0; i < no; ++i) {
+    if (out[i].p == nullptr) continue;
+    for (int j = 0; j < ni; ++j)
+      if (bytes_overlap(out[i].p, out[i].n, in[j].p, in[j].n)) return true;
+    for (int j = 0; j < i; ++j)
+      if (bytes_overlap(out[i].p, out[i].n, out[j].p, out[j].n)) return true;
+  }
+  return false;
+}
+
+bool aligned256(const void* p) { return reinterpret_cast<uintptr_t>(p) % 256 == 0; }
+
+int loss_type_bytes(int dtype) { return dtype == MSS_BF16 ? 2 : 4; }
+
+// The checks that both losses share: lists, reduction, temperature.
+int check_loss(int rows, int vocab, int top, int io, int teacher_dtype, int reduction, float temperature) {
+  static_assert(MSS_LOSS_MAX_TOP == mss::kLossMaxTop && MSS_LOSS_NONE == mss::kLossNone &&
+                    MSS_LOSS_SUM == mss::kLossSum && MSS_LOSS_MEAN == mss::kLossMean, "header and kernel disagree");
+  if (rows <= 0 || vocab <= 0 || top <= 0) return MSS_ERR_INVALID_ARGUMENT;
+  if ((io != MSS_F32 && io != MSS_BF16) || (teacher_dtype != MSS_F32 && teacher_dtype != MSS_BF16))
+    return MSS_ERR_INVALID_ARGUMENT;
+  if (reduction < MSS_LOSS_NONE || reduction > MSS_LOSS_MEAN) return MSS_ERR_INVALID_ARGUMENT;
+  if (!(temperature > 0.f) || !(mss::kLog2e / temperature > 0.f) || !(mss::kLog2e / temperature <= 3.4e38f))
+    return MSS_ERR_INVALID_ARGUMENT;
+  if (top > MSS_LOSS_MAX_TOP || static_cast<long long>(rows) * top > (1LL << 27)) return MSS_ERR_UNSUPPORTED;
+  return MSS_OK;
+}
+
+mss::LossRows loss_rows(int rows, int top, int vocab, float temperature, bool lists, Carve* saved) {
+  mss::LossRows r{};
+  r.rows = rows;
+  r.top = top;
+  r.vocab = vocab;
+  r.c = mss::kLog2e / temperature;
+  r.blocks = mss::loss_row_blocks(rows, lists);
+  r.words = saved->take<int>(static_cast<long long>(rows) * top);
+  r.q = saved->take<float>(static_cast<long long>(rows) * top);
+  r.live = saved->take<float>(rows);
+  r.counts = saved->take<int>(r.blocks);
+  return r;
+}
+
+// Everything but the operands' addresses.
+int linear_loss_sizes(const mss_linear_loss_args* a, mss::LinLossParams* p, mss::LinLossPlan* plan, size_t* saved,
+                      size_t* fwd, size_t* bwd) {
+  if (a == nullptr || a->top < 0) return MSS_ERR_INVALID_ARGUMENT;
+  const bool lists = a->top > 0;
+  const int top = lists ? a->top : 1;
+  int s = check_loss(a->tokens, a->vocab, top, a->io_dtype, lists ? a->teacher_dtype : MSS_F32, a->reduction, a->temperature);
+  if (s != MSS_OK) return s;
+  if (a->features <= 0 || (!lists && a->temperature != 1.f)) return MSS_ERR_INVALID_ARGUMENT;
+  if (a->stride_f < 0 || a->stride_t < 0 || a->ldw < a->features) return MSS_ERR_INVALID_ARGUMENT;
+  if (a->tokens > (1 << 20) || a->vocab > (1 << 20) || a->features > 65536 || a->ldw > (1LL << 24) ||
+      static_cast<long long>(a->tokens) * a->vocab > (1LL << 38) || a->stride_f > (1LL << 40) || a->stride_t > (1LL << 40))
+    return MSS_ERR_UNSUPPORTED;
+  p->tokens = a->tokens;
+  p->features = a->features;
+  p->vocab = a->vocab;
+  p->width = (a->features + 63) / 64 * 64;
+  p->planes = a->io_dtype == MSS_BF16 ? 1 : 3;
+  p->reduction = a->reduction;
+  p->temperature = a->temperature;
+  p->sf = a->stride_f;
+  p->st = a->stride_t;
+  p->ldw = a->ldw;
+  p->pack_w = !(a->io_dtype == MSS_BF16 && a->features % 64 == 0 && a->ldw % 8 == 0 && aligned16(a->weight));
+  *plan = mss::linloss_plan(p->tokens, p->features, p->vocab, p->planes);
+  p->parts = plan->parts;
+  p->piece = plan->piece;
+  p->ldg = plan->ldg;
+  p->ldx = plan->ldx;
+  p->x_splits = plan->x_splits;
+  p->w_splits = plan->w_splits;
+  Carve c{static_cast<char*>(a->saved), 0};
+  p->r = loss_rows(a->tokens, top, a->vocab, a->temperature, lists, &c);
+  p->c = p->r.c;
+  p->picked = c.take<float>(static_cast<long long>(a->tokens) * top);
+  p->lse = c.take<float>(a->tokens);
+  p->xp = c.take<mss::bf16_t>(static_cast<long long>(p->planes) * a->tokens * p->width);
+  if (p->pack_w) p->wp = c.take<mss::bf16_t>(static_cast<long long>(p->planes) * a->vocab * p->width);
+  *saved = c.at;
+  Carve f{static_cast<char*>(a->workspace), 0};
+  p->part = f.take<float2>(static_cast<long long>(p->parts) * a->tokens);
+  *fwd = f.at;
+  Carve b{static_cast<char*>(a->workspace), 0};
+  p->scale = b.take<float2>(a->tokens);
+  p->g = b.take<mss::bf16_t>(static_cast<long long>(p->planes) * a->tokens * p->ldg);
+  p->dx_part = b.take<float>(static_cast<long long>(p->x_splits) * p->features * p->ldx);
+  if (p->w_splits > 1) p->dw_part = b.take<float>(static_cast<long long>(p->w_splits) * p->piece * p->features);
+  *bwd = b.at;
+  return MSS_OK;
+}
+
+int linear_loss_params(const mss_linear_loss_args* a, bool bwd, mss::LinLossParams* p, mss::LinLossPlan* plan) {
+  size_t saved, ws_f, ws_b;
+  const int s = linear_loss_sizes(a, p, plan, &saved, &ws_f, &ws_b);
+  if (s != MSS_OK) return s;
+  const int e = loss_type_bytes(a->io_dtype);
+  if (!a->weight || !a->saved || (a->reduction != MSS_LOSS_NONE && !a->mean)) return MSS_ERR_INVALID_ARGUMENT;
+  if (reinterpret_cast<uintptr_t>(a->x) % e != 0 || reinterpret_cast<uintptr_t>(a->weight) % e != 0)
+    return MSS_ERR_INVALID_ARGUMENT;
+  const size_t ws = bwd ? ws_b : ws_f;
+  if (!aligned256(a->saved) || a->saved_bytes < saved || !a->workspace || !aligned256(a->workspace) || a->workspace_bytes < ws)
+    return MSS_ERR_WORKSPACE;
+  const long long x_bytes = ((a->features - 1LL) * a->stride_f + (a->tokens - 1LL) * a->stride_t + 1) * e;
+  const long long w_bytes = ((a->vocab - 1LL) * a->ldw + a->features) * e;
+  Span in[8] = {{a->weight, w_bytes}};
+  Span out[8] = {{a->workspace, static_cast<long long>(ws)}};
+  int ni = 1, no = 1;
+  if (bwd) {
+    if (!a->grad || (!a->dx && !a->dweight) || (a->dw_dtype != MSS_F32 && a->dw_dtype != MSS_BF16))
+      return MSS_ERR_INVALID_ARGUMENT;
+    in[ni++] = {a->saved, static_cast<long long>(saved)};
+    in[ni++] = {a->mean, 8};
+    in[ni++] = {a->grad, a->reduction == MSS_LOSS_NONE ? 4LL * a->tokens : 4};
+    out[no++] = {a->dx, static_cast<long long>(a->features) * a->tokens * e};
+    out[no++] = {a->dweight, static_cast<long long>(a->vocab) * a->features * loss_type_bytes(a->dw_dtype)};
+  } else {
+    if (!a->x || !a->loss) return MSS_ERR_INVALID_ARGUMENT;
+    if (a->top > 0 ? !a->ids || !a->teacher : !a->targets) return MSS_ERR_INVALID_ARGUMENT;
+    in[ni++] = {a->x, x_bytes};
+    const long long n = static_cast<long long>(a->tokens) * (a->top > 0 ? a->top : 1);
+    if (a->top > 0) {
+      in[ni++] = {a->ids, 8 * n};
+      in[ni++] = {a->teacher, n * loss_type_bytes(a->teacher_dtype)};
+    } else {
+      in[ni++] = {a->targets, 8 * n};
+    }
+    out[no++] = {a->loss, 4LL * a->tokens};
+    out[no++] = {a->reduction == MSS_LOSS_NONE ? nullptr : a->mean, 8};
+    out[no++] = {a->saved, static_cast<long long>(saved)};
+  }
+  if (outputs_meet(out, no, in, ni)) return MSS_ERR_INVALID_ARGUMENT;
+  p->x = a->x;
+  p->w = a->weight;
+  p->loss = a->loss;
+  p->mean = a->mean;
+  p->grad = a->grad;
+  p->dx = a->dx;
+  p->dw = a->dweight;
+  p->dw_bf16 = a->dw_dtype == MSS_BF16;
+  if (a->top > 0) {
+    p->r.ids = reinterpret_cast<const long long*>(a->ids);
+    p->r.teacher = a->teacher;
+    p->r.teacher_bf16 = a->teacher_dtype == MSS_BF16;
+  } else {
+    p->r.targets = reinterpret_cast<const long long*>(a->targets);
+    p->r.ignore = a->ignore_index;
+  }
+  return MSS_OK;
+}
+}  // namespace
+
+size_t mss_linear_loss_saved_bytes(const mss_linear_loss_args* a) {
+  mss::LinLossParams p{};
+  mss::LinLossPlan plan;
+  size_t saved = 0, f = 0, b = 0;
+  return linear_loss_sizes(a, &p, &plan, &saved, &f, &b) == MSS_OK ? saved : 0;
+}
+
+size_t mss_linear_loss_workspace_bytes(const mss_linear_loss_args* a, int32_t backward) {
+  mss::LinLossParams p{};
+  mss::LinLossPlan plan;
+  size_t saved = 0, f = 0, b = 0;
+  if (linear_loss_sizes(a, &p, &plan, &saved, &f, &b) != MSS_OK) return 0;
+  return backward ? b : f;
+}
+
+int mss_linear_loss_fwd(const mss_linear_loss_args* a, void* stream) {
+  mss::LinLossParams p{};
+  mss::LinLossPlan plan;
+  const int s = linear_loss_params(a, false, &p, &plan);
+  if (s != MSS_OK) return s;
+  const hipError_t e = mss::launch_linloss_fwd(p, plan, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? MSS_OK : hip_fail(e, "launching linear loss forward");
+}
+
+int mss_linear_loss_bwd(const mss_linear_loss_args* a, void* stream) {
+  mss::LinLossParams p{};
+  mss::LinLossPlan plan;
+  const int s = linear_loss_params(a, true, &p, &plan);
+  if (s != MSS_OK) return s;
+  const hipError_t e = mss::launch_linloss_bwd(p, plan, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? MSS_OK : hip_fail(e, "launching linear loss backward");
+}
+
+namespace {
+int distill_sizes(const mss_distill_args* a, mss::DistillParams* p, size_t* saved) {
+  if (a == nullptr) return MSS_ERR_INVALID_ARGUMENT;
+  const int s = check_loss(a->rows, a->vocab, a->top, a->io_dtype, a->teacher_dtype, a->reduction, a->temperature);
+  if (s != MSS_OK) return s;
+  if (a->ld < a->vocab) return MSS_ERR_INVALID_ARGUMENT;
+  if (a->vocab > (1 << 30) || a->ld > (1LL << 40)) return MSS_ERR_UNSUPPORTED;
+  p->vocab = a->vocab;
+  p->io_bf16 = a->io_dtype == MSS_BF16;
+  p->reduction = a->reduction;
+  p->temperature = a->temperature;
+  p->ld = a->ld;
+  Carve c{static_cast<char*>(a->saved), 0};
+  p->r = loss_rows(a->rows, a->top, a->vocab, a->temperature, true, &c);
+  p->stat = c.take<float2>(a->rows);
+  *saved = c.at;
+  return MSS_OK;
+}
+
+int run_distill(const mss_distill_args* a, int what, void* stream) {
+  mss::DistillParams p{};
+  size_t saved;
+  const int s = distill_sizes(a, &p, &saved);
+  if (s != MSS_OK) return s;
+  const bool fwd = what & mss::kDsFwd, bwd = what & mss::kDsBwd;
+  const int e = loss_type_bytes(a->io_dtype);
+  if (!a->logits || !a->saved || (a->reduction != MSS_LOSS_NONE && !a->mean)) return MSS_ERR_INVALID_ARGUMENT;
+  if (reinterpret_cast<uintptr_t>(a->logits) % e != 0 || reinterpret_cast<uintptr_t>(a->dlogits) % e != 0)
+    return MSS_ERR_INVALID_ARGUMENT;
+  if (fwd && (!a->ids || !a->teacher || !a->loss)) return MSS_ERR_INVALID_ARGUMENT;
+  if (bwd && !a->dlogits) return MSS_ERR_INVALID_ARGUMENT;
+  const bool reads_grad = bwd && !fwd;
+  if (reads_grad && !a->grad) return MSS_ERR_INVALID_ARGUMENT;
+  if (((fwd && bwd) || (what & mss::kDsAgain)) && a->reduction == MSS_LOSS_NONE) return MSS_ERR_INVALID_ARGUMENT;
+  if (!aligned256(a->saved) || a->saved_bytes < saved) return MSS_ERR_WORKSPACE;
+  const long long n = static_cast<long long>(a->rows) * a->top;
+  const long long per_row = a->reduction == MSS_LOSS_NONE ? 4LL * a->rows : 4;
+  const Span logits = {a->logits, ((a->rows - 1LL) * a->ld + a->vocab) * e}, rest = {a->saved, static_cast<long long>(saved)};
+  const Span mean = {a->reduction == MSS_LOSS_NONE ? nullptr : a->mean, 8};
+  const Span d = {bwd ? a->dlogits : nullptr, static_cast<long long>(a->rows) * a->vocab * e};
+  if (fwd) {
+    const Span in[] = {logits, {a->ids, 8 * n}, {a->teacher, n * loss_type_bytes(a->teacher_dtype)}};
+    const Span out[] = {{a->loss, 4LL * a->rows}, mean, rest, d};
+    if (outputs_meet(out, 4, in, 3)) return MSS_ERR_INVALID_ARGUMENT;
+  } else {
+    const Span in[] = {logits, rest, mean, {a->grad, per_row}};
+    if (outputs_meet(&d, 1, in, 4)) return MSS_ERR_INVALID_ARGUMENT;
+  }
+  p.r.ids = reinterpret_cast<const long long*>(a->ids);
+  p.r.teacher = a->teacher;
+  p.r.teacher_bf16 = a->teacher_dtype == MSS_BF16;
+  p.logits = a->logits;
+  p.loss = a->loss;
+  p.mean = a->mean;
+  p.grad = a->grad;
+  p.dlogits = a->dlogits;
+  const hipError_t err = mss::launch_distill(p, what, static_cast<hipStream_t>(stream));
+  return err == hipSuccess ? MSS_OK : hip_fail(err, "launching distillation loss");
+}
+}  // namespace
+
+size_t mss_distill_saved_bytes(const mss_distill_args* a) {
+  mss::DistillParams p{};
+  size_t saved = 0;
+  return distill_sizes(a, &p, &saved) == MSS_OK ? saved : 0;
+}
+
+int mss_distill_fwd(const mss_distill_args* a, void* stream) { return run_distill(a, mss::kDsFwd, stream); }
+int mss_distill_bwd(const mss_distill_args* a, void* stream) { return run_distill(a, mss::kDsBwd, stream); }
+int mss_distill_fwd_grad(const mss_distill_args* a, void* stream) {
+  return run_distill(a, mss::kDsFwd | mss::kDsBwd, stream);
+}
+int mss_distill_regrad(const mss_distill_args* a, void* stream) {
+  return run_distill(a, mss::kDsBwd | mss::kDsAgain, stream);
 }
 
 }  // extern "C"

@@ -1,0 +1,810 @@
+// A language model's loss from its head's operands, the logits not kept, with its gradients:
+// logit[t][v] = sum_d x[d][t] w[v][d] for tokens t and a vocabulary of words v, the losses of
+// mss_loss.h over it, dx[d][t] = sum_v w[v][d] g[t][v], dw[v][d] = sum_t g[t][v] x[d][t] with
+// g[t][v] = d loss / d logit[t][v].
+//
+// Forward: one product whose tiles leave, for each token and tile, only the largest s and the sum of
+// 2^(s - largest); they are merged a token at a time. The wanted words' logits are formed apart, one
+// dot product each. Backward: in pieces of the vocabulary the product is formed again, its tiles
+// turned into g (bf16) in a workspace, from which the two gradients' products read.
+//
+// All products run on v_mfma_f32_32x32x16_bf16 with float32 sums. bf16 operands are taken as they
+// are; g is rounded to bf16 once, as its factors x and w are. A float32 matrix is split into three
+// bf16 planes, each the rounding of what the ones before leave, 24 bits in all, and a product is the sum
+// of the six products of planes that reach 2^-24 of the whole, smallest first: six times the work of
+// a bf16 product, but at 16 times the rate of the float32 matrix instructions.
+//
+// 32x32x16 operand layout (lane l, its 8 bf16): A[i][k] at l = i + 32 (k / 8), element k % 8;
+// B[k][j] at l = j + 32 (k / 8), element k % 8; D[i][j] at l = j + 32 ((i / 4) % 2),
+// register 4 (i / 8) + i % 4.
+#include <hip/hip_runtime.h>
+
+#include "mss_loss.h"
+
+namespace mss {
+
+namespace {
+
+typedef __bf16 lbf16x8 __attribute__((ext_vector_type(8)));
+typedef float lf32x16 __attribute__((ext_vector_type(16)));
+typedef short ls16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) ls16x4* lds_s16x4_t;
+
+constexpr int kBK = 64;  // k of a stage
+
+// Tiles of (32 kMT kWM) x (32 kNT kWN) by kWM x kWN waves of kMT x kNT matrix tiles each, kRing stages in LDS.
+template <int kWM_, int kWN_, int kMT_, int kNT_, int kRing_>
+struct LlShape {
+  static constexpr int kWM = kWM_, kWN = kWN_, kMT = kMT_, kNT = kNT_, kRing = kRing_;
+  static constexpr int kM = 32 * kMT * kWM, kN = 32 * kNT * kWN;
+  static constexpr int kWaves = kWM * kWN, kThreads = 64 * kWaves;
+  static constexpr int kASlots = kM * kBK / 8, kBSlots = kN * kBK / 8, kSlots = kASlots + kBSlots;  // of 16 bytes
+  static constexpr int kACopies = kASlots / kThreads, kBCopies = kBSlots / kThreads;
+  static constexpr int kCopies = kACopies + kBCopies;
+  static_assert(kASlots % kThreads == 0 && kBSlots % kThreads == 0, "whole copies");
+  static_assert(kRing >= 2 && kRing <= 4 && (kRing - 2) * kCopies < 64, "");
+};
+
+template <int kN>
+__device__ __forceinline__ void ll_wait_vm() {
+  static_assert(kN >= 0 && kN < 64, "vmcnt range");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kN) : "memory");
+}
+
+// An operand's part of a stage in LDS. Along: rows of kBK k, 16-byte chunks at chunk ^ ((row >> 1) & 7), so
+// that the 16 lanes of a read phase (16 rows, one chunk) cover all banks; LDS row r holds matrix row
+// perm(r) when kPerm > 1: perm interleaves the kPerm tiles of a wave, lane j's rows then are kPerm
+// neighbours. Across: kBK rows of kTile elements, read with the transposing LDS read (a group of 16
+// lanes takes 4 rows of 16 elements, lane i gets column i); 64-byte units at unit ^ key(row), the
+// four rows of a phase on different banks.
+template <int kTile, bool kAcross, int kPerm>
+struct LlPanel {
+  static constexpr int kUnits = kTile / 32;
+  static __device__ __forceinline__ int key(int k) { return kUnits >= 4 ? k & 3 : kUnits == 2 ? (k >> 1) & 1 : 0; }
+  // Bytes from the stage's first element to what slot `s` holds.
+  static __device__ __forceinline__ uint32_t source(int s, uint32_t ld) {
+    if constexpr (kAcross) {
+      const int k = s / (kTile / 8), c = s % (kTile / 8);
+      return k * ld * 2 + ((((c >> 2) ^ key(k)) << 2) | (c & 3)) * 16;
+    } else {
+      int row = s / 8;
+      const int c = (s % 8) ^ ((row >> 1) & 7);
+      if constexpr (kPerm > 1) row = row / (32 * kPerm) * (32 * kPerm) + kPerm * (row & 31) + (row >> 5) % kPerm;
+      return row * ld * 2 + c * 16;
+    }
+  }
+  // The operand of matrix tile `tile` (32 rows), step ks of 16 k.
+  static __device__ __forceinline__ lbf16x8 fragment(const u32x4* buf, int tile, int ks, int lane) {
+    if constexpr (kAcross) {
+      const int i = lane & 15, sub = (lane >> 4) & 1, g = lane >> 5, kr = i >> 2;
+      const char* at = reinterpret_cast<const char*>(buf) + (ks * 16 + 8 * g + kr) * (kTile * 2) +
+                       ((tile ^ key(kr)) << 6) + 32 * sub + 8 * (i & 3);
+      union {
+        ls16x4 h[2];
+        lbf16x8 v;
+      } u;
+      u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t)(at));
+      u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t)(at + 4 * kTile * 2));
+      return u.v;
+    } else {
+      const int row = 32 * tile + (lane & 31), c = 2 * ks + (lane >> 5);
+      return __builtin_bit_cast(lbf16x8, buf[row * 8 + (c ^ ((row >> 1) & 7))]);
+    }
+  }
+};
+
+// The planes of a product of two split matrices, smallest products first (4 bits each).
+[[maybe_unused]] constexpr unsigned kPairsA = 0x010120, kPairsB = 0x001102;
+
+struct LlArgs {
+  LossMatrix a, b;       // from the piece's first row and k on
+  int k;                 // of the product, a whole number of stages
+  int pairs;             // 1 or 6
+  int tiles_m, tiles_n, splits;
+};
+
+enum { kModeLse, kModeGrad, kModeDx, kModeDw };
+
+// What all tokens' gradients are scaled by.
+struct LlScale {
+  const float* grad;  // NULL: nothing
+  const float* mean;
+  float temperature;
+};
+
+__device__ __forceinline__ float shared_scale(const LlScale& s) {
+  if (s.grad == nullptr) return 1.f;
+  return s.grad[0] * s.temperature * (s.mean ? s.mean[1] : 1.f);
+}
+
+struct LlOut {
+  int rows, cols;        // of the output that exist, from the piece's first on
+  float c;
+  float2* part;          // kModeLse: [part][cols]
+  const float2* scale;   // kModeGrad: [rows]
+  bf16_t* g;
+  long long ld, plane;   // kModeGrad, kModeDx, kModeDw: row stride; planes of g, or from one split to the next
+  int planes;
+  float* f;              // kModeDx, kModeDw with float32 output
+  bf16_t* h;             // kModeDw with bf16 output
+  int add;               // kModeDx: to what is there
+  LlScale by;            // kModeDw
+};
+
+template <class S, int kMode>
+__global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
+#if defined(__HIP_DEVICE_COMPILE__)  // the host's pass knows no buffer resources
+  constexpr bool kAAcross = kMode == kModeDx || kMode == kModeDw, kBAcross = kMode == kModeDw;
+  constexpr int kPerm = kMode == kModeGrad || kMode == kModeDx ? S::kNT : 1;
+  using PA = LlPanel<S::kM, kAAcross, 1>;
+  using PB = LlPanel<S::kN, kBAcross, kPerm>;
+  // Distinct objects, each chosen by a constant: the compiler then tells the copies in flight into one
+  // from the reads of another.
+  __shared__ u32x4 s0[S::kSlots], s1[S::kSlots], s2[S::kRing > 2 ? S::kSlots : 1], s3[S::kRing > 3 ? S::kSlots : 1];
+  const int lane = threadIdx.x & 63, j = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave % S::kWM, wn = wave / S::kWM;
+
+  // Neighbouring tiles on one XCD: 8 of A by all of B share their operands in its L2.
+  int tm, tn, split;
+  {
+    const unsigned n = gridDim.x, per = n / 8, rem = n % 8, x = blockIdx.x % 8;
+    unsigned id = x * per + min(x, rem) + blockIdx.x / 8;
+    const unsigned tiles = p.tiles_m * p.tiles_n;
+    split = id / tiles;
+    id -= split * tiles;
+    const unsigned group = id / (8 * p.tiles_n), first = group * 8, wide = min(8u, p.tiles_m - first);
+    const unsigned in = id - group * 8 * p.tiles_n;
+    tm = first + in % wide;
+    tn = in / wide;
+  }
+  const int m0 = tm * S::kM, n0 = tn * S::kN;
+
+  const int nk = p.k / kBK, all = nk * p.pairs;
+  const int st0 = static_cast<int>(static_cast<long long>(split) * all / p.splits);
+  const int stages = static_cast<int>(static_cast<long long>(split + 1) * all / p.splits) - st0;
+
+  uint32_t off_a[S::kACopies], off_b[S::kBCopies];
+#pragma unroll
+  for (int t = 0; t < S::kACopies; ++t)
+    off_a[t] = PA::source((wave + S::kWaves * t) * 64 + lane, static_cast<uint32_t>(p.a.ld));
+#pragma unroll
+  for (int t = 0; t < S::kBCopies; ++t)
+    off_b[t] = PB::source((wave + S::kWaves * t) * 64 + lane, static_cast<uint32_t>(p.b.ld));
+
+  // The stage that is copied next; what lies past a matrix's end is read as zeros.
+  int next_pair = st0 / nk, next_k = st0 % nk;
+  const auto rsrc = [](const LossMatrix& m, int pl, long long at) {
+    const long long left = (m.end - at) * 2;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t*>(m.base + pl * m.plane + at), 0,
+                                             static_cast<uint32_t>(left < 0 ? 0 : left > 0xfffffff0ll ? 0xfffffff0ll : left),
+                                             0x00027000);
+  };
+  const auto issue = [&](u32x4* d) {
+    const int pa = p.pairs == 1 ? 0 : (kPairsA >> (4 * next_pair)) & 15;
+    const int pb = p.pairs == 1 ? 0 : (kPairsB >> (4 * next_pair)) & 15;
+    const long long k0 = static_cast<long long>(next_k) * kBK;
+    const auto ra = rsrc(p.a, pa, kAAcross ? k0 * p.a.ld + m0 : m0 * p.a.ld + k0);
+    const auto rb = rsrc(p.b, pb, kBAcross ? k0 * p.b.ld + n0 : n0 * p.b.ld + k0);
+#pragma unroll
+    for (int t = 0; t < S::kACopies; ++t)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void_t)(d + 64 * (wave + S::kWaves * t)), 16, off_a[t], 0, 0, 0);
+#pragma unroll
+    for (int t = 0; t < S::kBCopies; ++t)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void_t)(d + S::kASlots + 64 * (wave + S::kWaves * t)), 16,
+                                               off_b[t], 0, 0, 0);
+    if (++next_k == nk) {
+      next_k = 0;
+      ++next_pair;
+    }
+  };
+
+  lf32x16 acc[S::kMT][S::kNT];
+#pragma unroll
+  for (int a = 0; a < S::kMT; ++a)
+#pragma unroll
+    for (int b = 0; b < S::kNT; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[a][b][e] = 0.f;
+
+  const auto compute = [&](const u32x4* buf) {
+    lbf16x8 a[2][S::kMT], b[2][S::kNT];
+    const auto load = [&](int ks) {
+#pragma unroll
+      for (int t = 0; t < S::kMT; ++t) a[ks & 1][t] = PA::fragment(buf, wm * S::kMT + t, ks, lane);
+#pragma unroll
+      for (int t = 0; t < S::kNT; ++t) b[ks & 1][t] = PB::fragment(buf + S::kASlots, wn * S::kNT + t, ks, lane);
+    };
+    load(0);
+#pragma unroll
+    for (int ks = 0; ks < kBK / 16; ++ks) {
+      if (ks + 1 < kBK / 16) load(ks + 1);
+#pragma unroll
+      for (int mt = 0; mt < S::kMT; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < S::kNT; ++nt)
+          acc[mt][nt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[ks & 1][mt], b[ks & 1][nt], acc[mt][nt], 0, 0, 0);
+    }
+  };
+
+  // A ring of kRing stages: while one is multiplied, the next kRing - 1 are in flight. A stage has landed once
+  // at most the copies of those issued after it are outstanding; the barrier makes that hold for all
+  // waves, and says that all are done with the stage whose place the next copies take.
+#define MSS_LL_STEP(O, CUR, NEXT)                                    \
+  {                                                                  \
+    const int st = gg + O;                                           \
+    if (st < stages) {                                               \
+      const int later = min(S::kRing - 2, stages - 1 - st);          \
+      if (S::kRing > 3 && later >= 2) ll_wait_vm<(S::kRing > 3 ? 2 * S::kCopies : 0)>(); \
+      else if (S::kRing > 2 && later == 1) ll_wait_vm<(S::kRing > 2 ? S::kCopies : 0)>(); \
+      else ll_wait_vm<0>();                                          \
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");             \
+      __builtin_amdgcn_s_barrier();                                  \
+      if (st + S::kRing - 1 < stages) issue(NEXT);                   \
+      compute(CUR);                                                  \
+    }                                                                \
+  }
+  if (stages > 0) issue(s0);
+  if (S::kRing > 2 && stages > 1) issue(s1);
+  if (S::kRing > 3 && stages > 2) issue(s2);
+  if constexpr (S::kRing == 2) {
+    for (int gg = 0; gg < stages; gg += 2) {
+      MSS_LL_STEP(0, s0, s1)
+      MSS_LL_STEP(1, s1, s0)
+    }
+  } else if constexpr (S::kRing == 3) {
+    for (int gg = 0; gg < stages; gg += 3) {
+      MSS_LL_STEP(0, s0, s2)
+      MSS_LL_STEP(1, s1, s0)
+      MSS_LL_STEP(2, s2, s1)
+    }
+  } else {
+    for (int gg = 0; gg < stages; gg += 4) {
+      MSS_LL_STEP(0, s0, s3)
+      MSS_LL_STEP(1, s1, s0)
+      MSS_LL_STEP(2, s2, s1)
+      MSS_LL_STEP(3, s3, s2)
+    }
+  }
+#undef MSS_LL_STEP
+
+  const int wm0 = m0 + wm * 32 * S::kMT, wn0 = n0 + wn * 32 * S::kNT;
+  const auto row_of = [&](int mt, int r) { return wm0 + 32 * mt + 8 * (r >> 2) + 4 * g + (r & 3); };
+
+  if constexpr (kMode == kModeLse) {
+    // Rows are words, columns tokens: a lane has the words of one token.
+#pragma unroll
+    for (int nt = 0; nt < S::kNT; ++nt) {
+      if (m0 + S::kM > o.rows) {
+#pragma unroll
+        for (int mt = 0; mt < S::kMT; ++mt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (row_of(mt, r) >= o.rows) acc[mt][nt][r] = -INFINITY;
+      }
+      float m = acc[0][nt][0];
+#pragma unroll
+      for (int mt = 0; mt < S::kMT; ++mt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[mt][nt][r]);
+      m = fmaxf(m, __shfl_xor(m, 32));
+      const float mc = m == -INFINITY ? 0.f : m * o.c;
+      float s = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < S::kMT; ++mt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s += fast_exp2(__builtin_fmaf(acc[mt][nt][r], o.c, -mc));
+      s += __shfl_xor(s, 32);
+      const int t = wn0 + 32 * nt + j;
+      if (g == 0 && t < o.cols)
+        o.part[static_cast<long long>(tm * S::kWM + wm) * o.cols + t] = make_float2(m == -INFINITY ? m : mc, s);
+    }
+  } else if constexpr (kMode == kModeGrad) {
+    // Rows are tokens, columns words, kNT neighbours a lane. The words past the vocabulary are zeros.
+    const int v = wn0 + S::kNT * j;
+#pragma unroll
+    for (int mt = 0; mt < S::kMT; ++mt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int t = row_of(mt, r);
+        if (t >= o.rows) continue;
+        const float2 sc = o.scale[t];
+        float d[S::kNT];
+#pragma unroll
+        for (int nt = 0; nt < S::kNT; ++nt) {
+          d[nt] = fast_exp2(__builtin_fmaf(acc[mt][nt][r], o.c, -sc.x)) * sc.y;
+          if (v + nt >= o.cols) d[nt] = 0.f;
+        }
+        bf16_t* dst = o.g + t * o.ld + v;
+        for (int pl = 0; pl < o.planes; ++pl) {
+          alignas(8) uint16_t w[S::kNT];
+#pragma unroll
+          for (int nt = 0; nt < S::kNT; ++nt) {
+            const bf16_t b = f32_to_bf16(d[nt]);
+            w[nt] = b.bits;
+            d[nt] -= to_f32(b);
+          }
+          __builtin_memcpy(dst + pl * o.plane, w, sizeof(w));
+        }
+      }
+  } else if constexpr (kMode == kModeDx) {
+    // Rows are features, columns tokens, kNT neighbours a lane.
+    float* f = o.f + split * o.plane;
+    const int t = wn0 + S::kNT * j;
+#pragma unroll
+    for (int mt = 0; mt < S::kMT; ++mt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int d = row_of(mt, r);
+        if (d >= o.rows || t >= o.cols) continue;  // (the rows are long enough for the last lane's kNT)
+        float* dst = f + d * o.ld + t;
+        float v[S::kNT];
+        if (o.add) __builtin_memcpy(v, dst, sizeof(v));
+#pragma unroll
+        for (int nt = 0; nt < S::kNT; ++nt) v[nt] = o.add ? v[nt] + acc[mt][nt][r] : acc[mt][nt][r];
+        __builtin_memcpy(dst, v, sizeof(v));
+      }
+  } else {
+    // Rows are words, columns features.
+    const float by = shared_scale(o.by);
+#pragma unroll
+    for (int mt = 0; mt < S::kMT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < S::kNT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int v = row_of(mt, r), d = wn0 + 32 * nt + j;
+          if (v >= o.rows || d >= o.cols) continue;
+          const float x = acc[mt][nt][r] * by;
+          if (o.h != nullptr) store_as(o.h + v * o.ld + d, x);
+          else o.f[split * o.plane + v * o.ld + d] = x;
+        }
+  }
+#endif
+}
+
+// ------------------------------------------------------------------------- operands
+// A value's bf16 planes; the lower ones of what is not finite are zeros.
+template <int kPlanes>
+__device__ __forceinline__ void split_planes(float v, bf16_t (&b)[kPlanes]) {
+  b[0] = f32_to_bf16(v);
+  float left = v - to_f32(b[0]);
+#pragma unroll
+  for (int i = 1; i < kPlanes; ++i) {
+    if (!(fabsf(left) < INFINITY)) left = 0.f;
+    b[i] = f32_to_bf16(left);
+    left -= to_f32(b[i]);
+  }
+}
+
+// x (features, tokens) as token-major rows of `width` features, zeros past the last feature and in rows that
+// do not count (whatever a masked token holds then reaches nothing). Tiles of 64 x 64 through LDS, read
+// along whichever axis is contiguous.
+template <typename in_t, int kPlanes>
+__global__ __launch_bounds__(256) void ll_pack_x_kernel(LinLossParams p) {
+  __shared__ float s[64][65];
+  const int t0 = blockIdx.x * 64, f0 = blockIdx.y * 64;
+  const in_t* x = static_cast<const in_t*>(p.x);
+  const bool along_f = p.sf == 1;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int a = along_f ? lane : w + 4 * i, b = along_f ? w + 4 * i : lane;  // feature, token
+    const int f = f0 + a, t = t0 + b;
+    s[a][b] = f < p.features && t < p.tokens ? to_f32(x[f * p.sf + t * p.st]) : 0.f;
+  }
+  __syncthreads();
+  const long long plane = static_cast<long long>(p.tokens) * p.width;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int slot = threadIdx.x + 256 * i, b = slot / 8, c = 8 * (slot % 8);
+    const int t = t0 + b;
+    if (t >= p.tokens) continue;
+    const bool live = p.r.live[t] != 0.f;
+    alignas(16) bf16_t v[kPlanes][8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      bf16_t q[kPlanes];
+      split_planes<kPlanes>(live ? s[c + e][b] : 0.f, q);
+#pragma unroll
+      for (int pl = 0; pl < kPlanes; ++pl) v[pl][e] = q[pl];
+    }
+#pragma unroll
+    for (int pl = 0; pl < kPlanes; ++pl)
+      *reinterpret_cast<u32x4*>(p.xp + pl * plane + static_cast<long long>(t) * p.width + f0 + c) =
+          *reinterpret_cast<const u32x4*>(v[pl]);
+  }
+}
+
+// The weight's rows, `width` features each.
+template <typename in_t, int kPlanes>
+__global__ __launch_bounds__(256) void ll_pack_w_kernel(LinLossParams p) {
+  const int per = p.width / 8;
+  const long long n = static_cast<long long>(p.vocab) * per, plane = static_cast<long long>(p.vocab) * p.width;
+  const in_t* w = static_cast<const in_t*>(p.w);
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n; i += gridDim.x * 256LL) {
+    const long long row = i / per;
+    const int c = 8 * static_cast<int>(i - row * per);
+    const in_t* src = w + row * p.ldw + c;
+    alignas(16) bf16_t v[kPlanes][8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      bf16_t q[kPlanes];
+      split_planes<kPlanes>(c + e < p.features ? to_f32(src[e]) : 0.f, q);
+#pragma unroll
+      for (int pl = 0; pl < kPlanes; ++pl) v[pl][e] = q[pl];
+    }
+#pragma unroll
+    for (int pl = 0; pl < kPlanes; ++pl)
+      *reinterpret_cast<u32x4*>(p.wp + pl * plane + row * p.width + c) = *reinterpret_cast<const u32x4*>(v[pl]);
+  }
+}
+
+// ------------------------------------------------------------------------- the wanted words' logits
+// A wave takes four words of a token's list at a time.
+__device__ __forceinline__ void add_planes(const bf16_t* at, float (&v)[8]) {
+  const u32x4 u = *reinterpret_cast<const u32x4*>(at);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] += __uint_as_float(u[i] << 16);
+    v[2 * i + 1] += __uint_as_float(u[i] & 0xffff0000u);
+  }
+}
+
+template <int kPlanes>
+__global__ __launch_bounds__(256) void ll_pick_kernel(LinLossParams p, LossMatrix w) {
+  const int lane = threadIdx.x & 63;
+  const int per = (p.r.top + 3) / 4;
+  const long long id = blockIdx.x * 4LL + (threadIdx.x >> 6);
+  const long long t = id / per;
+  if (t >= p.tokens) return;
+  const int k0 = 4 * static_cast<int>(id - t * per);
+  const long long xplane = static_cast<long long>(p.tokens) * p.width;
+  int word[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) word[e] = k0 + e < p.r.top ? p.r.words[t * p.r.top + k0 + e] : -1;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int c = 8 * lane; c < p.width; c += 512) {
+    float x[8] = {};
+#pragma unroll
+    for (int pl = 0; pl < kPlanes; ++pl) add_planes(p.xp + pl * xplane + t * p.width + c, x);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (word[e] < 0) continue;
+      float v[8] = {};
+#pragma unroll
+      for (int pl = 0; pl < kPlanes; ++pl) add_planes(w.base + pl * w.plane + word[e] * w.ld + c, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[e] = __builtin_fmaf(x[i], v[i], sum[e]);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float v = wave_sum(sum[e]);
+    if (lane == 0 && k0 + e < p.r.top) p.picked[t * p.r.top + k0 + e] = v;
+  }
+}
+
+// ------------------------------------------------------------------------- a token's loss
+// 64 tokens a workgroup: the parts' sums merged, 16 waves side by side, then a wave a token over its list.
+constexpr int kFinishTokens = 64;
+
+__global__ __launch_bounds__(1024) void ll_finish_kernel(LinLossParams p) {
+  __shared__ float s_m[16][64], s_s[16][64], s_lse[64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int t0 = blockIdx.x * kFinishTokens;
+  {
+    const int t = t0 + lane;
+    float m = -INFINITY, s = 0.f;
+    if (t < p.tokens)
+      for (int i = w; i < p.parts; i += 16) {
+        const float2 q = p.part[static_cast<long long>(i) * p.tokens + t];
+        const float mx = fmaxf(m, q.x);
+        if (mx == -INFINITY) {
+          s += q.y;  // zero, or NaN
+          continue;
+        }
+        s = s * fast_exp2(m - mx) + q.y * fast_exp2(q.x - mx);
+        m = mx;
+      }
+    s_m[w][lane] = m;
+    s_s[w][lane] = s;
+  }
+  __syncthreads();
+  if (w == 0) {
+    float m = s_m[0][lane], s = s_s[0][lane];
+    for (int i = 1; i < 16; ++i) {
+      const float mx = fmaxf(m, s_m[i][lane]);
+      if (mx == -INFINITY) {
+        s += s_s[i][lane];
+        continue;
+      }
+      s = s * fast_exp2(m - mx) + s_s[i][lane] * fast_exp2(s_m[i][lane] - mx);
+      m = mx;
+    }
+    const int t = t0 + lane;
+    float lse = m + fast_log2(s);
+    if (t < p.tokens) {
+      const float live = p.r.live[t];
+      lse += live - live;  // NaN for a row that has a word outside the vocabulary
+      p.lse[t] = lse;
+    }
+    s_lse[lane] = lse;
+  }
+  __syncthreads();
+  for (int i = w; i < 64; i += 16) {
+    const long long t = t0 + i;
+    float sum = 0.f;
+    if (t < p.tokens) {
+      const float lse = s_lse[i];
+      for (int k = lane; k < p.r.top; k += 64) {
+        const long long at = t * p.r.top + k;
+        if (p.r.words[at] < 0) continue;
+        const float q = p.r.q[at];
+        sum = __builtin_fmaf(q, (lse - p.picked[at] * p.c) + fast_log2(q), sum);
+      }
+      sum = wave_sum(sum) * (kLn2 * p.temperature * p.temperature);
+      const float live = p.r.live[t];
+      if (live == 0.f) sum = 0.f;
+      sum += live - live;
+      if (lane == 0) p.loss[t] = sum;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------- backward, around the products
+// A token's lse, and what its g is scaled by before it is rounded: without a reduction its own upstream
+// gradient; else nothing, since what all tokens share is left to the products' ends (1 / tokens has
+// an error of its own in bf16, the same for every token).
+__global__ __launch_bounds__(256) void ll_scale_kernel(LinLossParams p) {
+  const int t = blockIdx.x * 256 + threadIdx.x;
+  if (t >= p.tokens) return;
+  float f = p.reduction == kLossNone ? p.grad[t] * p.temperature : 1.f;
+  if (p.r.live[t] == 0.f) f = 0.f;
+  p.scale[t] = make_float2(p.lse[t], f);
+}
+
+// g at the wanted words of the piece that begins at word v0, from their own logits.
+template <int kPlanes>
+__global__ __launch_bounds__(256) void ll_wanted_kernel(LinLossParams p, int v0, int words) {
+  const long long i = blockIdx.x * 256LL + threadIdx.x;
+  if (i >= static_cast<long long>(p.tokens) * p.r.top) return;
+  const int v = p.r.words[i] - v0;
+  if (p.r.words[i] < 0 || v < 0 || v >= words) return;
+  const long long t = i / p.r.top;
+  const float2 sc = p.scale[t];
+  bf16_t b[kPlanes];
+  split_planes<kPlanes>((fast_exp2(__builtin_fmaf(p.picked[i], p.c, -sc.x)) - p.r.q[i]) * sc.y, b);
+#pragma unroll
+  for (int pl = 0; pl < kPlanes; ++pl) p.g[pl * (p.tokens * p.ldg) + t * p.ldg + v] = b[pl];
+}
+
+// dx from the splits' sums.
+template <typename out_t>
+__global__ __launch_bounds__(256) void ll_dx_kernel(LinLossParams p, LlScale scale) {
+  const float by = shared_scale(scale);
+  const long long n = static_cast<long long>(p.features) * p.tokens, plane = p.features * p.ldx;
+  out_t* out = static_cast<out_t*>(p.dx);
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n; i += gridDim.x * 256LL) {
+    const long long d = i / p.tokens, t = i - d * p.tokens;
+    const float* src = p.dx_part + d * p.ldx + t;
+    float v = src[0];
+    for (int s = 1; s < p.x_splits; ++s) v += src[s * plane];
+    store_as(out + i, p.r.live[t] == 0.f ? 0.f : v * by);
+  }
+}
+
+// dw of a piece from the splits' sums.
+template <typename out_t>
+__global__ __launch_bounds__(256) void ll_dw_kernel(const float* part, int splits, long long plane, long long n, out_t* out) {
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n; i += gridDim.x * 256LL) {
+    float v = part[i];
+    for (int s = 1; s < splits; ++s) v += part[s * plane + i];
+    store_as(out + i, v);
+  }
+}
+
+unsigned blocks_for(long long n, long long most) {
+  const long long b = (n + 255) / 256;
+  return static_cast<unsigned>(b < most ? b : most);
+}
+
+//                WM WN MT NT ring
+typedef LlShape<2, 4, 4, 2, 2> LlLargeM;   // 256 x 256, waves of 128 x 64
+typedef LlShape<4, 2, 2, 4, 2> LlLargeN;   // 256 x 256, waves of 64 x 128
+typedef LlShape<2, 2, 2, 2, 2> LlSmall;    // 128 x 128, waves of 64 x 64
+typedef LlShape<4, 1, 1, 1, 4> LlThinN;    // 128 x 32, waves of 32 x 32
+typedef LlShape<1, 4, 1, 1, 4> LlThinM;    // 32 x 128
+
+template <class S, int kMode>
+void launch_product(LlArgs a, const LlOut& o, hipStream_t stream) {
+  a.tiles_m = (o.rows + S::kM - 1) / S::kM;
+  a.tiles_n = (o.cols + S::kN - 1) / S::kN;
+  hipLaunchKernelGGL((ll_kernel<S, kMode>), dim3(a.tiles_m * a.tiles_n * a.splits), dim3(S::kThreads), 0, stream, a, o);
+}
+
+template <int kMode>
+void launch_shaped(int shape, const LlArgs& a, const LlOut& o, hipStream_t stream) {
+  // (rows and columns: words x tokens, tokens x words, features x tokens, words x features)
+  if constexpr (kMode == kModeGrad) {
+    if (shape == 0) launch_product<LlSmall, kMode>(a, o, stream);
+    else if (shape == 1) launch_product<LlLargeN, kMode>(a, o, stream);
+    else launch_product<LlThinM, kMode>(a, o, stream);
+  } else if constexpr (kMode == kModeDw) {
+    if (shape == 1) launch_product<LlLargeM, kMode>(a, o, stream);
+    else launch_product<LlSmall, kMode>(a, o, stream);
+  } else {
+    if (shape == 0) launch_product<LlSmall, kMode>(a, o, stream);
+    else if (shape == 1) launch_product<LlLargeM, kMode>(a, o, stream);
+    else launch_product<LlThinN, kMode>(a, o, stream);
+  }
+}
+
+LossMatrix weight_planes(const LinLossParams& p) {
+  LossMatrix w{};
+  w.base = p.pack_w ? p.wp : static_cast<const bf16_t*>(p.w);
+  w.ld = p.pack_w ? p.width : p.ldw;
+  w.plane = static_cast<long long>(p.vocab) * p.width;
+  w.end = (p.vocab - 1LL) * w.ld + p.width;
+  return w;
+}
+
+LossMatrix x_planes(const LinLossParams& p) {
+  const long long n = static_cast<long long>(p.tokens) * p.width;
+  return LossMatrix{p.xp, p.width, n, n};
+}
+
+}  // namespace
+
+static long long tiles_of(long long rows, long long cols, int tm, int tn) {
+  return ((rows + tm - 1) / tm) * ((cols + tn - 1) / tn);
+}
+
+LinLossPlan linloss_plan(int tokens, int features, int vocab, int planes) {
+  LinLossPlan q{};
+  q.shape = tokens <= 32 ? 2 : tiles_of(vocab, tokens, 256, 256) >= 256 ? 1 : 0;
+  const int tv = q.shape == 1 ? 256 : 128;
+  q.parts = static_cast<int>((vocab + tv - 1) / tv) * (q.shape == 2 ? 4 : 2);
+  // Pieces of at most 1 GiB.
+  const long long most = (1LL << 30) / (2LL * planes * tokens) / 256 * 256;
+  const long long whole = (vocab + 255LL) / 256 * 256;
+  const long long pieces = (whole + (most > 256 ? most : 256) - 1) / (most > 256 ? most : 256);
+  q.piece = static_cast<int>(((whole / 256 + pieces - 1) / pieces) * 256);
+  q.ldg = q.piece;
+  q.ldx = (tokens + 3) / 4 * 4;
+  const int tx = q.shape == 1 ? 256 : 128, tt = q.shape == 1 ? 256 : q.shape == 0 ? 128 : 32;
+  const auto splits = [&](long long tiles, long long stages) {
+    long long s = kCUs / tiles;
+    s = s < stages / 4 ? s : stages / 4;
+    return static_cast<int>(s < 1 ? 1 : s);
+  };
+  const int pairs = planes == 1 ? 1 : 6;
+  q.x_splits = splits(tiles_of(features, tokens, tx, tt), static_cast<long long>(q.piece) / kBK * pairs);
+  q.w_splits = splits(tiles_of(q.piece < vocab ? q.piece : vocab, features, tx, tx), (tokens + kBK - 1LL) / kBK * pairs);
+  return q;
+}
+
+hipError_t launch_linloss_fwd(const LinLossParams& p, const LinLossPlan& plan, hipStream_t stream) {
+  const hipError_t e = launch_loss_rows(p.r, stream);
+  if (e != hipSuccess) return e;
+  const bool f32 = p.planes == 3;
+  const dim3 xg((p.tokens + 63) / 64, p.width / 64);
+  if (f32) hipLaunchKernelGGL((ll_pack_x_kernel<float, 3>), xg, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL((ll_pack_x_kernel<bf16_t, 1>), xg, dim3(256), 0, stream, p);
+  if (p.pack_w) {
+    const dim3 wg(blocks_for(static_cast<long long>(p.vocab) * (p.width / 8), 8192));
+    if (f32) hipLaunchKernelGGL((ll_pack_w_kernel<float, 3>), wg, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((ll_pack_w_kernel<bf16_t, 1>), wg, dim3(256), 0, stream, p);
+  }
+  LlArgs a{};
+  a.a = weight_planes(p);
+  a.b = x_planes(p);
+  a.k = p.width;
+  a.pairs = f32 ? 6 : 1;
+  a.splits = 1;
+  LlOut o{};
+  o.rows = p.vocab;
+  o.cols = p.tokens;
+  o.c = p.c;
+  o.part = p.part;
+  launch_shaped<kModeLse>(plan.shape, a, o, stream);
+  const long long picks = static_cast<long long>(p.tokens) * ((p.r.top + 3) / 4);
+  const dim3 pg(static_cast<unsigned>((picks + 3) / 4));
+  if (f32) hipLaunchKernelGGL(ll_pick_kernel<3>, pg, dim3(256), 0, stream, p, a.a);
+  else hipLaunchKernelGGL(ll_pick_kernel<1>, pg, dim3(256), 0, stream, p, a.a);
+  const int blocks = (p.tokens + kFinishTokens - 1) / kFinishTokens;
+  hipLaunchKernelGGL(ll_finish_kernel, dim3(blocks), dim3(1024), 0, stream, p);
+  if (p.reduction != kLossNone) return launch_loss_mean(p.loss, p.r, p.reduction, p.mean, stream);
+  return hipGetLastError();
+}
+
+hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, hipStream_t stream) {
+  const bool f32 = p.planes == 3;
+  hipLaunchKernelGGL(ll_scale_kernel, dim3((p.tokens + 255) / 256), dim3(256), 0, stream, p);
+  const LossMatrix w = weight_planes(p), x = x_planes(p);
+  const LlScale by{p.reduction == kLossNone ? nullptr : p.grad, p.reduction == kLossMean ? p.mean : nullptr, p.temperature};
+  for (long long v0 = 0; v0 < p.vocab; v0 += p.piece) {
+    const int words = static_cast<int>(p.vocab - v0 < p.piece ? p.vocab - v0 : p.piece);
+    LossMatrix wp = w;
+    wp.base += v0 * w.ld;
+    wp.end -= v0 * w.ld;
+    LossMatrix g{};
+    g.base = p.g;
+    g.ld = p.ldg;
+    g.plane = p.tokens * p.ldg;
+    g.end = g.plane;
+    LlArgs a{};
+    a.pairs = f32 ? 6 : 1;
+    // g
+    a.a = x;
+    a.b = wp;
+    a.k = p.width;
+    a.splits = 1;
+    LlOut o{};
+    o.rows = p.tokens;
+    o.cols = words;
+    o.c = p.c;
+    o.scale = p.scale;
+    o.g = p.g;
+    o.ld = p.ldg;
+    o.plane = g.plane;
+    o.planes = p.planes;
+    launch_shaped<kModeGrad>(plan.shape, a, o, stream);
+    const dim3 wg(static_cast<unsigned>((static_cast<long long>(p.tokens) * p.r.top + 255) / 256));
+    if (f32) hipLaunchKernelGGL(ll_wanted_kernel<3>, wg, dim3(256), 0, stream, p, static_cast<int>(v0), words);
+    else hipLaunchKernelGGL(ll_wanted_kernel<1>, wg, dim3(256), 0, stream, p, static_cast<int>(v0), words);
+    if (p.dx != nullptr) {
+      a.a = wp;
+      a.b = g;
+      a.k = (words + kBK - 1) / kBK * kBK;
+      a.splits = p.x_splits;
+      o = LlOut{};
+      o.rows = p.features;
+      o.cols = p.tokens;
+      o.f = p.dx_part;
+      o.ld = p.ldx;
+      o.plane = p.features * p.ldx;
+      o.add = v0 > 0;
+      launch_shaped<kModeDx>(plan.shape, a, o, stream);
+    }
+    if (p.dw != nullptr) {
+      a.a = g;
+      a.b = x;
+      a.k = (p.tokens + kBK - 1) / kBK * kBK;
+      a.splits = p.w_splits;
+      o = LlOut{};
+      o.rows = words;
+      o.cols = p.features;
+      o.ld = p.features;
+      o.by = by;
+      void* dst = static_cast<char*>(p.dw) + v0 * p.features * (p.dw_bf16 ? 2 : 4);
+      const long long n = static_cast<long long>(words) * p.features;
+      if (p.w_splits > 1) {
+        o.f = p.dw_part;
+        o.plane = static_cast<long long>(p.piece) * p.features;
+      } else if (p.dw_bf16) {
+        o.h = static_cast<bf16_t*>(dst);
+      } else {
+        o.f = static_cast<float*>(dst);
+      }
+      launch_shaped<kModeDw>(plan.shape, a, o, stream);
+      if (p.w_splits > 1) {
+        const dim3 dg(blocks_for(n, 4096));
+        if (p.dw_bf16)
+          hipLaunchKernelGGL(ll_dw_kernel<bf16_t>, dg, dim3(256), 0, stream, p.dw_part, p.w_splits, o.plane, n,
+                             static_cast<bf16_t*>(dst));
+        else
+          hipLaunchKernelGGL(ll_dw_kernel<float>, dg, dim3(256), 0, stream, p.dw_part, p.w_splits, o.plane, n,
+                             static_cast<float*>(dst));
+      }
+    }
+  }
+  if (p.dx != nullptr) {
+    const dim3 dg(blocks_for(static_cast<long long>(p.features) * p.tokens, 4096));
+    if (f32) hipLaunchKernelGGL(ll_dx_kernel<float>, dg, dim3(256), 0, stream, p, by);
+    else hipLaunchKernelGGL(ll_dx_kernel<bf16_t>, dg, dim3(256), 0, stream, p, by);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace mss

@@ -13,7 +13,7 @@ from pathlib import Path
 
 LIBRARY_NAME = "libmamba_selective_scan_hip.so"
 
-MSS_ABI_VERSION = 19
+MSS_ABI_VERSION = 20
 MSS_OK = 0
 MSS_ERR_INVALID_ARGUMENT = 1
 MSS_ERR_UNSUPPORTED = 2
@@ -36,6 +36,10 @@ MSS_FP8_MM_MAX_TOKENS = 1 << 19
 MSS_FP8_MAX_TOKENS = 1 << 27
 MSS_FP8_MAX_FEATURES = 1 << 30
 MSS_SAMPLE_MAX_VOCAB = 1 << 20
+MSS_LOSS_NONE = 0
+MSS_LOSS_SUM = 1
+MSS_LOSS_MEAN = 2
+MSS_LOSS_MAX_TOP = 1024
 
 # Every symbol include/mamba_selective_scan.h declares.
 EXPORTED_SYMBOLS = (
@@ -70,6 +74,15 @@ EXPORTED_SYMBOLS = (
     "mss_xent_bwd",
     "mss_xent_fwd_grad",
     "mss_xent_rescale",
+    "mss_linear_loss_saved_bytes",
+    "mss_linear_loss_workspace_bytes",
+    "mss_linear_loss_fwd",
+    "mss_linear_loss_bwd",
+    "mss_distill_saved_bytes",
+    "mss_distill_fwd",
+    "mss_distill_bwd",
+    "mss_distill_fwd_grad",
+    "mss_distill_regrad",
     "mss_scan_step",
     "mss_cscan_step",
     "mss_conv_step",
@@ -239,6 +252,22 @@ class SampleArgs(ctypes.Structure):
                 ("top_ps", _p), ("min_ps", _p), ("tokens", _p)]
 
 
+class LinearLossArgs(ctypes.Structure):
+    _fields_ = [("tokens", _i32), ("features", _i32), ("vocab", _i32), ("top", _i32), ("io_dtype", _i32),
+                ("teacher_dtype", _i32), ("dw_dtype", _i32), ("reduction", _i32), ("temperature", ctypes.c_float),
+                ("ignore_index", ctypes.c_int64), ("stride_f", ctypes.c_int64), ("stride_t", ctypes.c_int64),
+                ("ldw", ctypes.c_int64), ("x", _p), ("weight", _p), ("targets", _p), ("ids", _p), ("teacher", _p),
+                ("loss", _p), ("mean", _p), ("saved", _p), ("workspace", _p), ("saved_bytes", ctypes.c_size_t),
+                ("workspace_bytes", ctypes.c_size_t), ("grad", _p), ("dx", _p), ("dweight", _p)]
+
+
+class DistillArgs(ctypes.Structure):
+    _fields_ = [("rows", _i32), ("vocab", _i32), ("top", _i32), ("io_dtype", _i32), ("teacher_dtype", _i32),
+                ("reduction", _i32), ("temperature", ctypes.c_float), ("ld", ctypes.c_int64), ("logits", _p), ("ids", _p),
+                ("teacher", _p), ("loss", _p), ("mean", _p), ("saved", _p), ("saved_bytes", ctypes.c_size_t),
+                ("grad", _p), ("dlogits", _p)]
+
+
 _LIBRARY = None
 _LIBRARY_PATH = None
 
@@ -351,6 +380,18 @@ def register_hip_kernel(library_path=None):
                        ("mss_sample", SampleArgs)):
         getattr(lib, name).argtypes = [ctypes.POINTER(args), _p]
         getattr(lib, name).restype = ctypes.c_int
+    for name in ("mss_linear_loss_fwd", "mss_linear_loss_bwd"):
+        getattr(lib, name).argtypes = [ctypes.POINTER(LinearLossArgs), _p]
+        getattr(lib, name).restype = ctypes.c_int
+    for name in ("mss_distill_fwd", "mss_distill_bwd", "mss_distill_fwd_grad", "mss_distill_regrad"):
+        getattr(lib, name).argtypes = [ctypes.POINTER(DistillArgs), _p]
+        getattr(lib, name).restype = ctypes.c_int
+    lib.mss_linear_loss_saved_bytes.argtypes = [ctypes.POINTER(LinearLossArgs)]
+    lib.mss_linear_loss_saved_bytes.restype = ctypes.c_size_t
+    lib.mss_linear_loss_workspace_bytes.argtypes = [ctypes.POINTER(LinearLossArgs), _i32]
+    lib.mss_linear_loss_workspace_bytes.restype = ctypes.c_size_t
+    lib.mss_distill_saved_bytes.argtypes = [ctypes.POINTER(DistillArgs)]
+    lib.mss_distill_saved_bytes.restype = ctypes.c_size_t
     lib.mss_strerror.argtypes = [ctypes.c_int]
     lib.mss_strerror.restype = ctypes.c_char_p
     lib.mss_last_hip_error.argtypes = []

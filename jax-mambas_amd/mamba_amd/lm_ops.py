@@ -164,13 +164,13 @@ class GradHolder:
     """Passes the tied output head's float32 gradient of the shared table to the embedding's
     backward, which adds its own part in place and hands the sum to autograd as the table's
     one gradient (instead of two dense gradients and an add). The head's backward runs first:
-    it belongs to the end of the forward."""
+    it belongs to the end of the forward. Losses that share the head add theirs."""
 
     def __init__(self):
         self.grad = None
 
     def put(self, g):
-        self.grad = g
+        self.grad = g if self.grad is None else self.grad.add_(g)
 
     def take(self):
         g, self.grad = self.grad, None

@@ -32,6 +32,7 @@ from . import _lib
 from .decode import (causal_conv1d_update, gemv, gemv_conv_update, gemv_state_update, norm_gemv_conv_update,
                      selective_state_update)
 from .lm_ops import GradHolder, add_rmsnorm, embed_cm
+from .losses import linear_cross_entropy, linear_distill_loss
 from .proj import proj, proj_fits, wgrad, wgrad_fits
 from .selective_scan_hip import _io_tag, _ptr, _stream, launch_fwd, selective_scan_fn
 
@@ -290,6 +291,12 @@ class ShadowWeights:
         if x.dtype == torch.float32 or not self.by_id:
             return x.t() @ e.to(x.dtype).t()
         return _TiedHeadMM.apply(x, e, self.by_id[id(e)], holder)
+
+    def head_copy(self, x, e, holder=None):
+        """What the head's losses (losses.py) take besides x and the tied embedding e: its copy in x's type, and the
+        holder of its gradient."""
+        b = self.by_id.get(id(e))
+        return dict(weight_act=b if b is not None and b.dtype == x.dtype else None, holder=holder)
 
 
 def _uniform_(t, bound):
@@ -625,6 +632,33 @@ class MambaLM(nn.Module):
         """tokens (B, L) int64 -> logits (B*L, vocab) in act_dtype (rows in (b, t) order).
         Low-precision GEMM weights are refreshed from the float32 masters once per call unless
         they already match them (shadow_weights=False casts each weight at its use instead)."""
+        hn, weights, holder = self._hidden(tokens, seq_lens, act_dtype, shadow_weights)
+        return weights.head(hn, self.embedding, holder)
+
+    def loss(self, tokens, targets, seq_lens=None, act_dtype=torch.bfloat16, shadow_weights=True, ignore_index=-100,
+             reduction="mean"):
+        """Cross-entropy of the model's logits for tokens (B, L) against targets (B, L) int64, as
+        losses.linear_cross_entropy takes it: the logits are not kept, targets of ignore_index (padding, a
+        prompt) do not count."""
+        hn, weights, holder = self._hidden(tokens, seq_lens, act_dtype, shadow_weights)
+        return linear_cross_entropy(hn, self.embedding, targets.reshape(-1), ignore_index=ignore_index,
+                                    reduction=reduction, **weights.head_copy(hn, self.embedding, holder))
+
+    def distill_loss(self, tokens, ids, teacher, temperature=1.0, targets=None, seq_lens=None,
+                     act_dtype=torch.bfloat16, shadow_weights=True, ignore_index=-100, reduction="mean"):
+        """Distillation from a teacher's largest logits: ids (B, L, top) int64, the words, negative where there is
+        none, and teacher (B, L, top) their logits, as losses.linear_distill_loss takes them; the model's
+        logits are not kept. With targets, the pair of this loss and loss()'s, of one pass through the model."""
+        hn, weights, holder = self._hidden(tokens, seq_lens, act_dtype, shadow_weights)
+        kw = dict(reduction=reduction, **weights.head_copy(hn, self.embedding, holder))
+        soft = linear_distill_loss(hn, self.embedding, ids.flatten(0, -2), teacher.flatten(0, -2),
+                                   temperature=temperature, **kw)
+        if targets is None:
+            return soft
+        return soft, linear_cross_entropy(hn, self.embedding, targets.reshape(-1), ignore_index=ignore_index, **kw)
+
+    def _hidden(self, tokens, seq_lens, act_dtype, shadow_weights):
+        """The head's operand (d_model, B*L) in act_dtype, the weights' copies and the tied embedding's holder."""
         batch = tokens.shape[0]
         weights = _PLAIN
         if act_dtype != torch.float32 and shadow_weights:
@@ -641,7 +675,7 @@ class MambaLM(nn.Module):
         for blk, A in zip(self.blocks, self.a_matrices()):
             h, delta = blk(h, delta, batch, seq_lens, act_dtype, weights, A)
         _, hn = self.final_norm(h, delta, act_dtype)
-        return weights.head(hn, self.embedding, holder)
+        return hn, weights, holder
 
     def a_matrices(self):
         """Every block's S6 state matrix. Real A = -exp(A_log) of all blocks in one batched op
@@ -691,22 +725,29 @@ class GraphedTrainStep:
     warm-up steps on a side stream, then one captured step with gradients allocated inside
     the graph's memory pool. Callers must hold no autograd graph of earlier steps (e.g. a
     loss tensor): it keeps the parameters' gradient-accumulation nodes bound to the stream
-    they ran on, which breaks the capture."""
+    they ran on, which breaks the capture. With loss_fn None the loss is model.loss(tokens,
+    targets), which keeps no logits."""
 
     def __init__(self, model, optimizer, loss_fn, tokens, targets, warmup=3, act_dtype=torch.bfloat16):
         self.tokens, self.targets = tokens, targets
+
+        def step_loss():
+            if loss_fn is None:
+                return model.loss(tokens, targets, act_dtype=act_dtype)
+            return loss_fn(model(tokens, act_dtype=act_dtype), targets)
+
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
             for _ in range(warmup):
                 optimizer.zero_grad(set_to_none=True)
-                loss_fn(model(tokens, act_dtype=act_dtype), targets).backward()
+                step_loss().backward()
                 optimizer.step()
         torch.cuda.current_stream().wait_stream(side)
         self.graph = torch.cuda.CUDAGraph()
         optimizer.zero_grad(set_to_none=True)
         with torch.cuda.graph(self.graph):
-            self.loss = loss_fn(model(tokens, act_dtype=act_dtype), targets)
+            self.loss = step_loss()
             self.loss.backward()
             optimizer.step()
 

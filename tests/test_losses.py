@@ -1,0 +1,634 @@
+"""Losses of a language model: the head's cross-entropy without logits (the reference takes it of its
+head's logits, experiments/mamba_inductionheads.py:129-136), distillation from a teacher's top logits,
+from the head's operands and from logits.
+
+CPU: refusals. GPU: against the definitions in float64 on the same inputs, gradients against the
+formula's and against differences.
+
+Tolerances, per element, in units of U = 2^-24 (half a float32 step). A product's sum of n terms counts a whole
+step, 2 U, for each addition, relative to the sum S of the magnitudes, and 16 more for the planes that
+a float32 operand is split in and that leave 2^-24 of it: (n + 16) 2 U S. With dz that bound for a
+logit, M the largest logarithm to base 2 that a row meets (its largest |logit| / temperature log2 e, and
+log2 V), K its words and A = min(V, 128 + V / 512) the longest chain of additions in the sum of the V
+exponentials (of a lane, then lanes, waves and tiles): a logarithm, an exponent's argument or their difference is
+off by a few M U, the sum by A steps, so that lse / temperature is off by dz / temperature + (8 M + 4 A + 8) U, a
+loss by temperature^2 (2 dz / temperature + (16 M + 4 A + 16 + 4 K (M + 1)) U); a word's probability relative
+to itself by twice dz / temperature + (16 M + 4 A + 16) U, q by (K + 16) U. g is rounded to bfloat16
+(2^-8) where x is, and the gradients to their types.
+"""
+import numpy as np
+import pytest
+import torch
+
+from mamba_amd import _lib
+from mamba_amd.losses import distill_loss, linear_cross_entropy, linear_distill_loss
+from mamba_amd.lm_ops import GradHolder, cross_entropy
+
+U = 2.0 ** -24
+BF16, F32 = torch.bfloat16, torch.float32
+HALF = {BF16: 2.0 ** -8, F32: U}
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return _lib.register_hip_kernel()
+
+
+# ------------------------------------------------------------------------------- refusals
+P = 1 << 32  # addresses far apart, multiples of 256
+LINEAR = dict(tokens=20, features=64, vocab=100, top=0, io_dtype=1, teacher_dtype=0, dw_dtype=1, reduction=2, temperature=1.0,
+              ignore_index=-100, stride_f=20, stride_t=1, ldw=64, x=P, weight=2 * P, targets=3 * P, ids=4 * P,
+              teacher=5 * P, loss=6 * P, mean=7 * P, saved=8 * P, workspace=9 * P, saved_bytes=1 << 40,
+              workspace_bytes=1 << 31, grad=10 * P, dx=11 * P, dweight=12 * P)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(tokens=0), 1), (dict(features=0), 1), (dict(vocab=0), 1), (dict(top=-1), 1), (dict(io_dtype=2), 1),
+    (dict(reduction=3), 1), (dict(reduction=-1), 1), (dict(temperature=2.0), 1), (dict(stride_f=-1), 1),
+    (dict(stride_t=-1), 1), (dict(ldw=63), 1), (dict(x=None), 1), (dict(weight=None), 1), (dict(targets=None), 1),
+    (dict(loss=None), 1), (dict(mean=None), 1), (dict(saved=None), 1), (dict(x=P + 1), 1), (dict(weight=2 * P + 1), 1),
+    (dict(saved=8 * P + 16), 4), (dict(saved_bytes=100), 4), (dict(workspace=None), 4), (dict(workspace_bytes=10), 4),
+    (dict(workspace=9 * P + 8), 4), (dict(loss=P), 1), (dict(mean=2 * P), 1), (dict(saved=3 * P), 1),
+    (dict(workspace=P), 1), (dict(loss=7 * P), 1), (dict(tokens=1 << 21), 2), (dict(vocab=1 << 21), 2),
+    (dict(features=1 << 17, ldw=1 << 17), 2), (dict(tokens=1 << 19, vocab=1 << 20), 2),
+    (dict(top=5, ids=None), 1), (dict(top=5, teacher=None), 1), (dict(top=5, teacher_dtype=4), 1),
+    (dict(top=5, temperature=0.0), 1), (dict(top=5, temperature=-1.0), 1), (dict(top=5, temperature=float("nan")), 1),
+    (dict(top=5, temperature=float("inf")), 1), (dict(top=5, temperature=1e-39), 1), (dict(top=1025), 2),
+    (dict(top=1000, tokens=1 << 18), 2), (dict(top=5, loss=4 * P), 1), (dict(top=5, saved=5 * P), 1),
+])
+def test_linear_validation(lib, kw, status):
+    assert lib.mss_linear_loss_fwd(_lib.LinearLossArgs(**{**LINEAR, **kw}), None) == status
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(grad=None), 1), (dict(dx=None, dweight=None), 1), (dict(dw_dtype=5), 1), (dict(mean=None), 1),
+    (dict(weight=None), 1), (dict(saved=None), 1), (dict(dx=2 * P), 1), (dict(dweight=8 * P), 1), (dict(dx=12 * P), 1),
+    (dict(dx=10 * P), 1), (dict(workspace=2 * P), 1), (dict(workspace_bytes=10), 4), (dict(saved_bytes=10), 4),
+    (dict(dweight=7 * P), 1),
+])
+def test_linear_backward_validation(lib, kw, status):
+    assert lib.mss_linear_loss_bwd(_lib.LinearLossArgs(**{**LINEAR, **kw}), None) == status
+    assert lib.mss_linear_loss_bwd(None, None) == lib.mss_linear_loss_fwd(None, None) == 1
+    assert lib.mss_linear_loss_saved_bytes(None) == lib.mss_linear_loss_workspace_bytes(None, 1) == 0
+
+
+DISTILL = dict(rows=20, vocab=100, top=5, io_dtype=1, teacher_dtype=0, reduction=2, temperature=1.0, ld=100, logits=P, ids=2 * P,
+               teacher=3 * P, loss=4 * P, mean=5 * P, saved=6 * P, saved_bytes=1 << 31, grad=7 * P, dlogits=8 * P)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(rows=0), 1), (dict(vocab=0), 1), (dict(top=0), 1), (dict(io_dtype=2), 1), (dict(teacher_dtype=-1), 1),
+    (dict(reduction=4), 1), (dict(temperature=0.0), 1), (dict(temperature=float("nan")), 1), (dict(ld=99), 1),
+    (dict(logits=None), 1), (dict(ids=None), 1), (dict(teacher=None), 1), (dict(loss=None), 1), (dict(mean=None), 1),
+    (dict(saved=None), 1), (dict(dlogits=None), 1), (dict(logits=P + 1), 1), (dict(dlogits=8 * P + 1), 1),
+    (dict(reduction=0), 1), (dict(saved=6 * P + 4), 4), (dict(saved_bytes=64), 4), (dict(top=1025), 2),
+    (dict(rows=1 << 18, top=1000), 2), (dict(vocab=(1 << 30) + 1, ld=1 << 31), 2), (dict(dlogits=P + 256), 1),
+    (dict(loss=P), 1), (dict(saved=2 * P), 1), (dict(mean=4 * P), 1), (dict(dlogits=4 * P), 1), (dict(dlogits=6 * P), 1),
+])
+def test_distill_validation(lib, kw, status):
+    assert lib.mss_distill_fwd_grad(_lib.DistillArgs(**{**DISTILL, **kw}), None) == status
+    assert lib.mss_distill_fwd(None, None) == lib.mss_distill_bwd(None, None) == lib.mss_distill_regrad(None, None) == 1
+    assert lib.mss_distill_saved_bytes(None) == 0
+
+
+@pytest.mark.parametrize("kw", [dict(grad=None), dict(dlogits=None), dict(mean=None), dict(dlogits=7 * P), dict(dlogits=P)])
+def test_distill_backward_validation(lib, kw):
+    a = _lib.DistillArgs(**{**DISTILL, **kw})
+    assert lib.mss_distill_bwd(a, None) == lib.mss_distill_regrad(a, None) == 1
+
+
+def test_struct_layouts_match_the_header(tmp_path):
+    import ctypes
+    import subprocess
+    from pathlib import Path
+    structs = {"mss_linear_loss_args": _lib.LinearLossArgs, "mss_distill_args": _lib.DistillArgs}
+    lines = ["#include <stdio.h>", "#include <stddef.h>", '#include "mamba_selective_scan.h"', "int main(void) {"]
+    for c, cls in structs.items():
+        lines.append(f'  printf("%zu\\n", sizeof({c}));')
+        lines += [f'  printf("%zu\\n", offsetof({c}, {f}));' for f, _ in cls._fields_]
+    (tmp_path / "l.c").write_text("\n".join(lines + ["  return 0;", "}"]) + "\n")
+    root = Path(__file__).resolve().parents[1]
+    subprocess.run(["gcc", "-std=c99", "-I", str(root / "include"), str(tmp_path / "l.c"), "-o", str(tmp_path / "l")], check=True)
+    seen = [int(v) for v in subprocess.run([str(tmp_path / "l")], check=True, capture_output=True, text=True).stdout.split()]
+    want = [v for cls in structs.values() for v in (ctypes.sizeof(cls), *(getattr(cls, f).offset for f, _ in cls._fields_))]
+    assert seen == want
+
+
+def test_python_refusals():
+    x, w, tg = torch.randn(8, 5), torch.randn(11, 8), torch.zeros(5, dtype=torch.int64)
+    ids, te = torch.zeros(5, 3, dtype=torch.int64), torch.randn(5, 3)
+    ce, ld, ds = linear_cross_entropy, linear_distill_loss, distill_loss
+    z = torch.randn(5, 11)
+    for call in (lambda: ce(x, w, tg[:4]), lambda: ce(x, w, tg.int()), lambda: ce(x[0], w, tg), lambda: ce(x, w[:, :7], tg),
+                 lambda: ce(x, w, tg, reduction="avg"), lambda: ce(x, w[:0], tg), lambda: ce(x[:0], w[:, :0], tg),
+                 lambda: ce(x, w, tg, weight_act=w.bfloat16()), lambda: ce(x, w, tg, weight_act=w[:5]),
+                 lambda: ce(x.bfloat16(), w.bfloat16(), tg, holder=GradHolder()),
+                 lambda: ld(x, w, ids[:4], te), lambda: ld(x, w, ids.int(), te), lambda: ld(x, w, ids, te[:, :2]),
+                 lambda: ld(x, w, ids, te, temperature=0.0), lambda: ld(x, w, ids, te, temperature=float("nan")),
+                 lambda: ld(x, w, torch.zeros(5, 1025, dtype=torch.int64), torch.zeros(5, 1025)),
+                 lambda: ds(z[0], ids, te), lambda: ds(z, ids, te[:4]), lambda: ds(z, ids, te, temperature=-1),
+                 lambda: ds(z[:, :0], ids, te), lambda: ds(z, ids, te, reduction=None)):
+        with pytest.raises(ValueError):
+            call()
+    for call in (lambda: ce(x.half(), w, tg), lambda: ce(x, w.double(), tg), lambda: ld(x, w, ids, te.half()),
+                 lambda: ds(z.double(), ids, te)):
+        with pytest.raises(TypeError):
+            call()
+    for call in (lambda: ce(x, w, tg), lambda: ld(x, w, ids, te), lambda: ds(z, ids, te)):
+        with pytest.raises(RuntimeError, match="ROCm GPU"):
+            call()
+    with pytest.raises(RuntimeError, match="detach"):
+        ds(z, ids, te.requires_grad_())
+
+
+# ------------------------------------------------------------------------------- the definitions
+def _wanted_targets(targets, vocab, ignore=-100):
+    q = torch.zeros(targets.shape[0], vocab, dtype=torch.float64, device=targets.device)
+    live = targets != ignore
+    rows = live.nonzero()[:, 0]
+    q[rows, targets[rows]] = 1.0
+    return q, live
+
+
+def _wanted_lists(ids, teacher, temperature, vocab):
+    q = torch.zeros(ids.shape[0], vocab, dtype=torch.float64, device=ids.device)
+    t = teacher.double() / temperature
+    for r in range(ids.shape[0]):
+        at = ((ids[r] >= 0) & (teacher[r] != -torch.inf)).nonzero()[:, 0]
+        if len(at):
+            q[r].index_add_(0, ids[r][at], torch.softmax(t[r][at], 0))
+    return q, q.sum(1) > 0
+
+
+class _Bounds:
+    """Losses and gradients in float64, with what the module's docstring allows them to be off by. z: logits, dz
+    their own bound."""
+
+    def __init__(self, z, dz, q, live, temperature, k, dtype):
+        self.live = live
+        v = min(z.shape[1], 128 + z.shape[1] / 512)
+        s = z / temperature
+        lse = torch.logsumexp(s, 1)
+        at = torch.where(live, s.masked_fill(s == -torch.inf, 0).abs().amax(1), 0.0)
+        m = at * np.log2(np.e) + np.log2(max(2, z.shape[1]))
+        dz = dz / temperature
+        self.loss = torch.where(live, temperature ** 2 * (torch.special.xlogy(q, q) - torch.where(
+            q > 0, q * (s - lse[:, None]), 0.0)).sum(1), 0.0)
+        self.loss_tol = temperature ** 2 * (2 * dz + U * (16 * m + 4 * v + 16 + 4 * k * (m + 1))) * live
+        p = torch.exp(s - lse[:, None])
+        self.g = torch.where(live[:, None], temperature * (p - q), 0.0)
+        rel = 2 * dz + U * (16 * m + 4 * v + 16)
+        self.g_tol = temperature * torch.where(live[:, None], p * rel[:, None] + q * U * (k + 16), 0.0)
+        self.g_tol += (HALF[dtype] + 8 * U) * self.g.abs()
+
+    def reduced(self, reduction, upstream=None):
+        """loss and tolerance, and each row's scale of the gradient."""
+        n = max(1, int(self.live.sum()))
+        up = 1.0 if upstream is None else upstream
+        if reduction == "none":
+            return self.loss, self.loss_tol, torch.ones_like(self.loss) * up
+        by = 1.0 / n if reduction == "mean" else 1.0
+        loss = self.loss.sum() * by
+        return loss, self.loss_tol.sum() * by + 2 * U * loss.abs(), torch.full_like(self.loss, by) * up
+
+
+def _check(name, got, want, tol):
+    got = got.detach().double()
+    assert got.shape == want.shape, (name, got.shape, want.shape)
+    err = (got - want).abs()
+    worst = float((err / tol.clamp_min(1e-300)).nan_to_num(posinf=1e300).max()) if err.numel() else 0.0
+    print(f"  {name:8s} max_abs={float(err.max()) if err.numel() else 0:.3e} of tolerance {worst:.3f}", flush=True)
+    assert bool(torch.isfinite(got).all()) and bool((err <= tol).all()), name
+
+
+def _product_tol(a_tol, a, b, terms):
+    """Bound of a @ b for a off by a_tol, b exact."""
+    return torch.mm(a_tol, b.abs()) + (terms + 16) * 2 * U * torch.mm(a.abs() + a_tol, b.abs())
+
+
+def _linear_reference(x, w, q, live, temperature, k):
+    """x (features, tokens), w as they are read."""
+    xd, wd = x.detach().double(), w.detach().double()
+    xd = torch.where(live[None], xd, 0.0)  # (what a row that does not count holds is not looked at)
+    z = torch.mm(xd.t(), wd.t())
+    dz = (x.shape[0] + 16) * 2 * U * torch.mm(xd.abs().t(), wd.abs().t()).amax(1)
+    return _Bounds(z, dz, q, live, temperature, k, x.dtype), xd, wd
+
+
+def _check_linear_grads(ref, xd, wd, scale, x_dtype, w_dtype, dx, dw):
+    g, g_tol = ref.g * scale[:, None], ref.g_tol * scale[:, None].abs()
+    if dx is not None:
+        want = torch.mm(g, wd).t()
+        tol = _product_tol(g_tol, g, wd, g.shape[1]).t() + 8 * U * want.abs()
+        _check("dx", dx, want, tol * (1 + HALF[x_dtype]) + HALF[x_dtype] * want.abs())
+    if dw is not None:
+        want = torch.mm(g.t(), xd.t())
+        tol = _product_tol(g_tol.t(), g.t(), xd.t(), g.shape[0]) + 8 * U * want.abs()
+        _check("dw", dw, want, tol * (1 + HALF[w_dtype]) + HALF[w_dtype] * want.abs())
+
+
+def _inputs(t, d, v, dtype, seed=0, layout="cm"):
+    """x (features, tokens) and a weight, in one of the layouts: channel-major, token-major, rows with gaps and off
+    16 bytes."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(t, d, generator=g, device="cuda").to(dtype)
+    w = (torch.randn(v, d, generator=g, device="cuda") * (2.0 / d ** 0.5)).to(dtype)
+    if layout == "cm":
+        return x.t().contiguous(), w
+    if layout == "tm":
+        return x.t(), w
+    xs = torch.full((d, 2 * t + 1), float("nan"), dtype=dtype, device="cuda")
+    xs[:, 1::2] = x.t()
+    ws = torch.full((v + 1, d + 3), float("nan"), dtype=dtype, device="cuda")
+    ws[1:, 1:1 + d] = w
+    return xs[:, 1::2], ws[1:, 1:1 + d]
+
+
+def _targets(t, v, masked, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    at = torch.randint(0, v, (t,), generator=g)
+    return torch.where(torch.rand(t, generator=g) < masked, -100, at).cuda()
+
+
+def _lists(t, v, top, dtype=F32, seed=0, empty=0.1, again=True):
+    """Lists with absent entries (whose logits are NaN or inf), words that stand twice, empty rows."""
+    g = torch.Generator().manual_seed(seed)
+    ids = torch.stack([torch.randperm(v, generator=g)[:top] if v >= top else torch.randint(0, v, (top,), generator=g)
+                       for _ in range(t)])
+    te = (3 * torch.randn(t, top, generator=g)).to(dtype)
+    if again and top > 2:
+        ids[:, 2] = ids[:, 0]
+    absent = torch.rand(t, top, generator=g) < 0.2
+    absent[torch.rand(t, generator=g) < empty] = True
+    ids = torch.where(absent, -1 - torch.randint(0, 5, (t, top), generator=g), ids)
+    te = torch.where(absent, torch.tensor([float("nan"), float("inf"), 1e30])[torch.randint(0, 3, (t, top), generator=g)].to(dtype), te)
+    gone = (torch.rand(t, top, generator=g) < 0.1) & ~absent
+    te = torch.where(gone, torch.tensor(-float("inf"), dtype=dtype), te)
+    return ids.cuda(), te.cuda()
+
+
+# ------------------------------------------------------------------------------- without logits
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("t,d,v,layout,reduction,masked", [
+    (1, 1, 1, "cm", "mean", 0.0), (1, 64, 2, "tm", "sum", 0.0), (3, 7, 17, "gap", "none", 0.3), (5, 64, 129, "cm", "mean", 0.4),
+    (32, 96, 300, "tm", "none", 0.2), (33, 128, 255, "cm", "sum", 0.2), (64, 65, 1000, "gap", "mean", 0.1),
+    (200, 192, 515, "cm", "none", 0.5), (257, 40, 640, "tm", "mean", 0.1), (130, 320, 16, "cm", "mean", 0.0),
+    (1000, 64, 50, "gap", "sum", 0.9), (40, 64, 70000, "cm", "mean", 0.1)])
+def test_linear_cross_entropy(dtype, t, d, v, layout, reduction, masked):
+    print(f"case linear_cross_entropy {dtype} {t} {d} {v} {layout} {reduction}", flush=True)
+    x, w = _inputs(t, d, v, dtype, t + v, layout)
+    targets = _targets(t, v, masked, t)
+    x = x.clone(memory_format=torch.preserve_format) if layout == "gap" else x
+    q, live = _wanted_targets(targets, v)
+    if masked:  # nothing that a masked token holds is seen
+        x[:, ~live] = float("nan")
+        x[:1, ~live] = float("inf")
+    x.requires_grad_(True)
+    w = w.detach().requires_grad_(True)
+    up = torch.linspace(-1.0, 2.0, t, device="cuda") if reduction == "none" else torch.tensor(0.7, device="cuda")
+    loss = linear_cross_entropy(x, w, targets, reduction=reduction)
+    assert loss.dtype == F32
+    dx, dw = torch.autograd.grad(loss, (x, w), up)
+    assert dx.dtype == x.dtype and dw.dtype == w.dtype
+    ref, xd, wd = _linear_reference(x, w, q, live, 1.0, 1)
+    want, tol, scale = ref.reduced(reduction, up.double())
+    _check("loss", loss, want, tol)
+    _check_linear_grads(ref, xd, wd, scale, dtype, dtype, dx, dw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("t,d,v,top,temperature,reduction,tdtype", [
+    (1, 8, 3, 1, 1.0, "mean", F32), (4, 64, 20, 5, 2.0, "none", BF16), (31, 100, 301, 63, 0.5, "sum", F32),
+    (70, 64, 257, 64, 4.0, "mean", BF16), (129, 72, 400, 65, 1.0, "none", F32), (20, 128, 1024, 200, 3.0, "mean", F32),
+    (10, 64, 1500, 1024, 2.0, "sum", F32), (300, 64, 40, 3, 2.0, "mean", BF16)])
+def test_linear_distill_loss(dtype, t, d, v, top, temperature, reduction, tdtype):
+    print(f"case linear_distill_loss {dtype} {t} {d} {v} {top} {temperature} {reduction}", flush=True)
+    x, w = _inputs(t, d, v, dtype, t + v)
+    ids, te = _lists(t, v, top, tdtype, t)
+    q, live = _wanted_lists(ids, te, temperature, v)
+    x[:, ~live] = float("nan")
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    up = torch.linspace(-1.0, 2.0, t, device="cuda") if reduction == "none" else torch.tensor(-1.5, device="cuda")
+    loss = linear_distill_loss(x, w, ids, te, temperature=temperature, reduction=reduction)
+    dx, dw = torch.autograd.grad(loss, (x, w), up)
+    ref, xd, wd = _linear_reference(x, w, q, live, temperature, top)
+    want, tol, scale = ref.reduced(reduction, up.double())
+    _check("loss", loss, want, tol)
+    _check_linear_grads(ref, xd, wd, scale, dtype, dtype, dx, dw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,t,d,v", [(BF16, 4096, 64, 4100), (BF16, 4000, 200, 5000), (F32, 4096, 64, 4100), (F32, 8192, 40, 24000),
+                                         (BF16, 9000, 64, 61000)])
+def test_linear_cross_entropy_many_tiles(dtype, t, d, v):
+    """Large tiles; a vocabulary in more than one piece (the last two)."""
+    print(f"case many tiles {dtype} {t} {d} {v}", flush=True)
+    x, w = _inputs(t, d, v, dtype, 5)
+    targets = _targets(t, v, 0.1, 6)
+    q, live = _wanted_targets(targets, v)
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    loss = linear_cross_entropy(x, w, targets)
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    n = 2048  # the reference in pieces of the tokens
+    total, dw_want, dw_tol, losses = 0.0, 0.0, 0.0, 0.0
+    by = 1.0 / int(live.sum())
+    for a in range(0, t, n):
+        part = slice(a, min(t, a + n))
+        ref, xd, wd = _linear_reference(x.detach()[:, part], w, q[part], live[part], 1.0, 1)
+        total, losses = total + ref.loss.sum() * by, losses + ref.loss_tol.sum() * by
+        scale = torch.full_like(ref.loss, by)
+        _check_linear_grads(ref, xd, wd, scale, dtype, dtype, dx[:, part], None)
+        g, g_tol = ref.g * by, ref.g_tol * by
+        dw_want = dw_want + torch.mm(g.t(), xd.t())
+        dw_tol = dw_tol + _product_tol(g_tol.t(), g.t(), xd.t(), t)
+    _check("loss", loss, total, losses + 2 * U * total)
+    half = HALF[dtype]
+    _check("dw", dw, dw_want, (dw_tol + 8 * U * dw_want.abs()) * (1 + half) + half * dw_want.abs())
+
+
+@pytest.mark.gpu
+def test_linear_weight_copies_and_holder():
+    """A float32 master with and without its bfloat16 copy; the gradient through a holder; one gradient only."""
+    t, d, v = 100, 64, 300
+    x, w = _inputs(t, d, v, F32, 3)
+    x = x.to(BF16).requires_grad_(True)
+    w.requires_grad_(True)
+    act = w.detach().to(BF16)
+    targets = _targets(t, v, 0.2, 4)
+    q, live = _wanted_targets(targets, v)
+    ref, xd, wd = _linear_reference(x, act, q, live, 1.0, 1)
+    want, tol, scale = ref.reduced("mean")
+    for kw in (dict(), dict(weight_act=act)):
+        loss = linear_cross_entropy(x, w, targets, **kw)
+        _check("loss", loss, want, tol)
+        dx, dw = torch.autograd.grad(loss, (x, w))
+        assert dw.dtype == F32
+        _check_linear_grads(ref, xd, wd, scale, BF16, F32, dx, dw)
+    holder = GradHolder()
+    (dx2,) = torch.autograd.grad(linear_cross_entropy(x, w, targets, holder=holder), (x,), retain_graph=False)
+    loss = linear_cross_entropy(x, w, targets, weight_act=act, holder=holder)
+    loss.backward()
+    assert w.grad is None and torch.equal(holder.take(), dw) and torch.equal(x.grad, dx)
+    (only,) = torch.autograd.grad(linear_cross_entropy(x.detach(), w, targets), (w,))
+    assert torch.equal(only, dw) and torch.equal(dx2, dx)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_nothing_counts_and_no_rows(dtype):
+    x, w = _inputs(6, 64, 50, dtype, 1)
+    z = torch.randn(6, 50, device="cuda").to(dtype)
+    none, no_ids = torch.full((6,), -7, device="cuda"), torch.full((6, 4), -1, device="cuda")
+    te = torch.full((6, 4), float("nan"), device="cuda")
+    x[:, 0], z[0] = float("nan"), -float("inf")
+    for a in (x, w, z):
+        a.requires_grad_(True)
+    calls = [(lambda r: linear_cross_entropy(x, w, none, ignore_index=-7, reduction=r), (x, w)),
+             (lambda r: linear_distill_loss(x, w, no_ids, te, reduction=r), (x, w)),
+             (lambda r: distill_loss(z, no_ids, te, reduction=r), (z,)),
+             (lambda r: linear_cross_entropy(x[:, :0], w, none[:0], reduction=r), (x, w)),
+             (lambda r: linear_distill_loss(x, w, no_ids[:, :0], te[:, :0], reduction=r), (x, w)),
+             (lambda r: distill_loss(z[:0], no_ids[:0], te[:0], reduction=r), (z,)),
+             (lambda r: distill_loss(z, no_ids[:, :0], te[:, :0], reduction=r), (z,))]
+    for f, leaves in calls:
+        for r in ("none", "sum", "mean"):
+            loss = f(r)
+            assert loss.dtype == F32 and bool((loss == 0).all())
+            for g in torch.autograd.grad(loss.sum(), leaves):
+                assert bool((g == 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_words_outside_the_vocabulary_are_nan(dtype):
+    x, w = _inputs(40, 64, 50, dtype, 1)
+    targets = _targets(40, 50, 0.0, 2)
+    targets[3], targets[9], targets[11] = 50, -1, 1 << 40
+    loss = linear_cross_entropy(x.requires_grad_(True), w, targets, reduction="none")
+    bad = torch.zeros(40, dtype=torch.bool, device="cuda")
+    bad[[3, 9, 11]] = True
+    assert torch.equal(loss.isnan(), bad)
+    (dx,) = torch.autograd.grad(loss, (x,), torch.ones_like(loss))
+    assert torch.equal(dx.isnan().all(0), bad) and torch.equal(dx.isnan().any(0), bad)
+    ids, te = _lists(40, 50, 4, seed=3, empty=0.0)
+    ids[:, 0], te[:, 0] = 7, 1.0
+    ids[3, 0], te[9, 0], te[11, 0] = 50, float("nan"), float("inf")
+    z = torch.randn(40, 50, device="cuda").to(dtype).requires_grad_(True)
+    for loss, leaf, rows in ((linear_distill_loss(x, w, ids, te, reduction="none"), x, 0),
+                             (distill_loss(z, ids, te, reduction="none"), z, 1)):
+        assert torch.equal(loss.isnan(), bad)
+        (g,) = torch.autograd.grad(loss, (leaf,), torch.ones_like(loss))
+        assert torch.equal(g.isnan().all(rows), bad) and torch.equal(g.isnan().any(rows), bad)
+
+
+# ------------------------------------------------------------------------------- from logits
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("t,v,top,temperature,reduction,tdtype", [
+    (1, 1, 1, 1.0, "mean", F32), (7, 2, 2, 2.0, "none", F32), (5, 100, 7, 0.7, "sum", BF16), (9, 4096, 64, 2.0, "mean", F32),
+    (6, 4097, 65, 1.0, "none", F32), (4, 16384, 100, 2.0, "sum", F32), (3, 16385, 129, 1.0, "mean", BF16),
+    (3, 50280, 32, 2.0, "mean", F32), (2, 65536, 256, 1.0, "none", F32), (2, 65537, 300, 2.0, "mean", F32),
+    (2, 131071, 20, 1.0, "sum", F32), (37, 999, 1000, 1.0, "mean", F32)])
+def test_distill_loss(dtype, t, v, top, temperature, reduction, tdtype):
+    print(f"case distill_loss {dtype} {t} {v} {top} {temperature} {reduction}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(t + v)
+    big = (2.5 * torch.randn(t, v + 3, generator=g, device="cuda")).to(dtype)
+    z = big[:, 2:2 + v]  # rows off 16 bytes, with gaps
+    ids, te = _lists(t, v, top, tdtype, t + 1)
+    q, live = _wanted_lists(ids, te, temperature, v)
+    # Words of no weight, and rows that do not count, hold anything; a wanted word stays as it is.
+    gone = (torch.rand(t, v, generator=g, device="cuda") < 0.2) & (q == 0)
+    gone[:, 0] = False
+    z[gone] = torch.finfo(dtype).min
+    z[gone & (torch.rand(t, v, generator=g, device="cuda") < 0.5)] = -float("inf")
+    z[~live] = float("nan")
+    z.requires_grad_(True)
+    up = torch.linspace(-1.0, 2.0, t, device="cuda") if reduction == "none" else torch.tensor(0.3, device="cuda")
+    loss = distill_loss(z, ids, te, temperature=temperature, reduction=reduction)
+    zd = torch.where(live[:, None], z.detach().double(), 0.0)
+    zd = torch.where(zd == torch.finfo(dtype).min, -torch.inf, zd)  # (their weight is 0 in float64 too)
+    ref = _Bounds(zd, torch.zeros(t, dtype=torch.float64, device="cuda"), q, live, temperature, top, dtype)
+    want, tol, scale = ref.reduced(reduction, up.double())
+    _check("loss", loss, want, tol)
+    (dz,) = torch.autograd.grad(loss, (z,), up, retain_graph=True)
+    assert dz.dtype == dtype
+    gw = ref.g * scale[:, None]
+    _check("dz", dz, gw, ref.g_tol * scale[:, None].abs() + 8 * U * gw.abs() + 2.0 ** -149)
+    (one,) = torch.autograd.grad(loss, (z,), torch.ones_like(up), retain_graph=True)  # another pass, another upstream
+    want, tol, scale = ref.reduced(reduction)
+    gw = ref.g * scale[:, None]
+    _check("dz at 1", one, gw, ref.g_tol * scale[:, None].abs() + 8 * U * gw.abs() + 2.0 ** -149)
+    first = distill_loss(z, ids, te, temperature=temperature, reduction=reduction)  # and the one-reading pass with an upstream of 1
+    (again,) = torch.autograd.grad(first, (z,), torch.ones_like(up))
+    assert torch.equal(again, one)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_distill_edges_of_the_types(dtype):
+    """All words at the type's lowest value are alike; a wanted word of no weight makes the loss inf, its gradient
+    stays finite; a row without any word, and one with a NaN, are NaN."""
+    lowest = torch.finfo(dtype).min
+    z = torch.zeros(4, 70, device="cuda", dtype=dtype)
+    z[0], z[1, 5], z[2], z[3, 9] = lowest, -float("inf"), -float("inf"), float("nan")
+    ids = torch.tensor([[3], [5], [1], [2]], device="cuda")
+    te = torch.zeros(4, 1, device="cuda")
+    z.requires_grad_(True)
+    loss = distill_loss(z, ids, te, reduction="none")
+    (g,) = torch.autograd.grad(loss, (z,), torch.ones_like(loss))
+    # log2 70, its product with ln 2 and the exponent: a few steps of 8
+    loss = loss.detach()
+    assert abs(float(loss[0]) - np.log(70)) <= 32 * U * np.log(70) + 70 * 2 * U
+    assert float(loss[1]) == float("inf") and bool(loss[2:].isnan().all())
+    want = torch.full((70,), 1 / 70, dtype=torch.float64, device="cuda")
+    want[3] -= 1
+    _check("lowest", g[0], want, (HALF[dtype] + 200 * U) * want.abs())
+    want = torch.full((70,), 1 / 69, dtype=torch.float64, device="cuda")
+    want[5] = -1
+    _check("absent", g[1], want, (HALF[dtype] + 200 * U) * want.abs())
+    assert bool(g[2].isnan().all()) and bool(g[3].isnan().all())
+
+
+# ------------------------------------------------------------------------------- both
+@pytest.mark.gpu
+def test_gradients_against_differences():
+    """Central differences along a direction: the loss's own bound over the step, and the step's square times the third
+    derivative / 6: the sum of the rows' third central moments of the directional logits over temperature, of which
+    each is at most its cubed range / (6 sqrt 3), that of two points' distribution."""
+    t, d, v, h = 24, 64, 90, 0.01
+    x, w = _inputs(t, d, v, F32, 8)
+    ids, te = _lists(t, v, 6, seed=9)
+    targets = _targets(t, v, 0.2, 10)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    along = torch.randn(d, t, generator=g, device="cuda") / d ** 0.5
+    for f, temperature, (q, live) in ((lambda a: linear_cross_entropy(a, w, targets, reduction="sum"), 1.0, _wanted_targets(targets, v)),
+                                      (lambda a: linear_distill_loss(a, w, ids, te, temperature=2.0, reduction="sum"), 2.0,
+                                       _wanted_lists(ids, te, 2.0, v)),
+                                      (lambda a: distill_loss(a.t() @ w.t(), ids, te, temperature=2.0, reduction="sum"), 2.0,
+                                       _wanted_lists(ids, te, 2.0, v))):
+        a = x.clone().requires_grad_(True)
+        (dx,) = torch.autograd.grad(f(a), (a,))
+        slope = float((dx.double() * along.double()).sum())
+        ends = [float(f(x + s * h * along)) for s in (1, -1)]
+        ref, xd, wd = _linear_reference(x, w, q, live, temperature, 6)
+        dz = torch.mm(along.double().t(), wd.t())
+        span = (dz.amax(1) - dz.amin(1))[live] / temperature
+        tol = 2 * float(ref.loss_tol.sum()) / (2 * h) + h * h / 6 * temperature ** 2 * float((span ** 3).sum()) / (6 * 3 ** 0.5)
+        # (x + h along is rounded to float32: its error moves the loss by the gradient's share of it)
+        tol += U * float((dx.abs().double() * (x.abs().double() + h * along.abs().double())).sum()) * 2 / h
+        tol += 2 * U * (abs(ends[0]) + abs(ends[1])) / h + 1e-3 * U
+        print(f"  slope {slope:.6f} differences {(ends[0] - ends[1]) / (2 * h):.6f} tolerance {tol:.2e}", flush=True)
+        assert abs(slope - (ends[0] - ends[1]) / (2 * h)) <= tol
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_runs_are_the_same_and_streams(dtype):
+    x, w = _inputs(300, 128, 700, dtype, 3)
+    ids, te = _lists(300, 700, 20, seed=4)
+    targets = _targets(300, 700, 0.1, 5)
+    z = torch.randn(300, 700, device="cuda").to(dtype)
+    for a in (x, w, z):
+        a.requires_grad_(True)
+
+    def run():
+        out = []
+        for loss, leaves in ((linear_cross_entropy(x, w, targets), (x, w)), (linear_distill_loss(x, w, ids, te), (x, w)),
+                             (distill_loss(z, ids, te), (z,))):
+            out += [loss.detach(), *torch.autograd.grad(loss, leaves)]
+        return out
+
+    first = run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = run()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    for a, b, c in zip(first, second, run()):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_graph_replays(dtype):
+    """Each replay, on new values of the inputs, against the eager calls; two graphs side by side."""
+    t, d, v = 90, 64, 400
+    x, w = _inputs(t, d, v, dtype, 3)
+    z = torch.randn(t, v, device="cuda").to(dtype)
+    ids, te = _lists(t, v, 6, seed=4)
+    targets = _targets(t, v, 0.1, 5)
+    for a in (x, w, z):
+        a.requires_grad_(True)
+
+    def linear():
+        loss = linear_cross_entropy(x, w, targets) + 0.5 * linear_distill_loss(x, w, ids, te, temperature=2.0)
+        return [loss.detach(), *torch.autograd.grad(loss, (x, w))]
+
+    def logits():
+        loss = 2.0 * distill_loss(z, ids, te)
+        return [loss.detach(), *torch.autograd.grad(loss, (z,))]
+
+    graphs = []
+    for f in (linear, logits):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            f()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = f()
+        graphs.append((g, out, f))
+    for i in range(4):
+        with torch.no_grad():
+            x.mul_(0.9)
+            w.add_(0.01)
+            z.mul_(1.1)
+            targets.copy_(torch.roll(targets, 1))
+            te.copy_(te.roll(1, 0))
+            ids.copy_(ids.roll(1, 0))
+        want = [f() for _, _, f in graphs]
+        torch.cuda.synchronize()
+        for (g, out, _), wanted in zip(graphs, want):
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, wanted)), i
+
+
+@pytest.mark.gpu
+def test_against_the_framework_s_cross_entropy():
+    """The two forms of the same loss: from logits rounded to bfloat16 (each off by 2^-8 of itself), and without."""
+    t, d, v = 500, 128, 1000
+    x, w = _inputs(t, d, v, BF16, 3)
+    targets = _targets(t, v, 0.0, 5)
+    z = (x.t().contiguous() @ w.t())
+    apart = 2 * 2.0 ** -8 * float(z.abs().max()) * 1.1
+    assert abs(float(cross_entropy(z, targets)) - float(linear_cross_entropy(x, w, targets))) <= apart
+
+
+@pytest.mark.gpu
+def test_second_backward_and_input_changes():
+    x, w = _inputs(50, 64, 90, BF16, 3)
+    z = torch.randn(50, 90, device="cuda", requires_grad=True)
+    ids, te = _lists(50, 90, 5, seed=1)
+    targets = _targets(50, 90, 0.1, 5)
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    for loss, leaf in ((linear_cross_entropy(x, w, targets), x), (distill_loss(z, ids, te), z)):
+        (a,) = torch.autograd.grad(loss, (leaf,), retain_graph=True)
+        keep = a.clone()
+        a.zero_()
+        (b,) = torch.autograd.grad(loss, (leaf,), retain_graph=True)
+        assert torch.equal(keep, b)
+    # what the backward pass reads again is watched
+    loss = linear_cross_entropy(x, w, targets)
+    with torch.no_grad():
+        w.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(loss, (x,))
