@@ -1688,8 +1688,6 @@ int linear_loss_sizes(const mss_linear_loss_args* a, mss::LinLossParams* p, mss:
   p->piece = plan->piece;
   p->ldg = plan->ldg;
   p->ldx = plan->ldx;
-  p->x_splits = plan->x_splits;
-  p->w_splits = plan->w_splits;
   Carve c{static_cast<char*>(a->saved), 0};
   p->r = loss_rows(a->tokens, top, a->vocab, a->temperature, lists, &c);
   p->c = p->r.c;
@@ -1702,10 +1700,10 @@ int linear_loss_sizes(const mss_linear_loss_args* a, mss::LinLossParams* p, mss:
   p->part = f.take<float2>(static_cast<long long>(p->parts) * a->tokens);
   *fwd = f.at;
   Carve b{static_cast<char*>(a->workspace), 0};
-  p->scale = b.take<float2>(a->tokens);
+  p->scale = b.take<float2>(a->tokens + mss::kLinLossTile);
   p->g = b.take<mss::bf16_t>(static_cast<long long>(p->planes) * a->tokens * p->ldg);
-  p->dx_part = b.take<float>(static_cast<long long>(p->x_splits) * p->features * p->ldx);
-  if (p->w_splits > 1) p->dw_part = b.take<float>(static_cast<long long>(p->w_splits) * p->piece * p->features);
+  p->dx_sum = b.take<float>(p->features * p->ldx);
+  p->partial = b.take<float>(plan->partial);
   *bwd = b.at;
   return MSS_OK;
 }

@@ -30,25 +30,53 @@ typedef float lf32x16 __attribute__((ext_vector_type(16)));
 typedef short ls16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) ls16x4* lds_s16x4_t;
 
-constexpr int kBK = 64;  // k of a stage
+#define LL_INLINE __attribute__((always_inline))  // of lambdas that are called from several places
 
-// Tiles of (32 kMT kWM) x (32 kNT kWN) by kWM x kWN waves of kMT x kNT matrix tiles each, kRing stages in LDS.
-template <int kWM_, int kWN_, int kMT_, int kNT_, int kRing_>
+constexpr int kLlK = 64;  // products' k are whole multiples of it
+
+// Tiles of (32 kMT kWM) x (32 kNT kWN) by kWM x kWN waves of kMT x kNT matrix tiles each, kRing stages of kBK k in
+// LDS.
+template <int kWM_, int kWN_, int kMT_, int kNT_, int kRing_, int kBK_ = 64>
 struct LlShape {
-  static constexpr int kWM = kWM_, kWN = kWN_, kMT = kMT_, kNT = kNT_, kRing = kRing_;
+  static constexpr int kWM = kWM_, kWN = kWN_, kMT = kMT_, kNT = kNT_, kRing = kRing_, kBK = kBK_;
   static constexpr int kM = 32 * kMT * kWM, kN = 32 * kNT * kWN;
   static constexpr int kWaves = kWM * kWN, kThreads = 64 * kWaves;
   static constexpr int kASlots = kM * kBK / 8, kBSlots = kN * kBK / 8, kSlots = kASlots + kBSlots;  // of 16 bytes
   static constexpr int kACopies = kASlots / kThreads, kBCopies = kBSlots / kThreads;
   static constexpr int kCopies = kACopies + kBCopies;
+  static constexpr int kPerCU = kRing * kSlots * 16 > 81920 ? 1 : 2;
+  static constexpr int kSums = 16 * kMT * kNT;  // of a lane
   static_assert(kASlots % kThreads == 0 && kBSlots % kThreads == 0, "whole copies");
-  static_assert(kRing >= 2 && kRing <= 4 && (kRing - 2) * kCopies < 64, "");
+  static_assert(kRing >= 2 && kRing <= 4 && (kRing - 1) * kCopies < 64, "");
 };
 
+typedef uint32_t lu32x4 __attribute__((ext_vector_type(4)));
+
+// 16 bytes a lane from a buffer to LDS, from `lds` (the same in all lanes) on; zeros past the buffer's end. In
+// assembly (there is no register that it writes), since of the builtin's copies the compiler keeps account, and
+// waits for all that are in flight before the next transposing read, whose place it does not know. The
+// account is this file's: ll_meet. (m0 is nobody's across statements: the compiler sets it where it reads it.)
+__device__ __forceinline__ void ll_copy(lu32x4 rsrc, uint32_t offset, const void* lds) {
+  // (the same in all lanes, and in scalar registers already where the compiler knew)
+  uint32_t to = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void_t)lds)));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) rsrc[i] = __builtin_amdgcn_readfirstlane(rsrc[i]);
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %1, %2, 0 offen lds"
+      :
+      : "s"(to), "v"(offset), "s"(rsrc)
+      : "memory");
+}
+
+// All waves' copies but the newest kN have landed, and their reads are done.
 template <int kN>
-__device__ __forceinline__ void ll_wait_vm() {
+__device__ __forceinline__ void ll_meet() {
   static_assert(kN >= 0 && kN < 64, "vmcnt range");
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kN) : "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kN) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
 // An operand's part of a stage in LDS. Along: rows of kBK k, 16-byte chunks at chunk ^ ((row >> 1) & 7), so
@@ -57,9 +85,11 @@ __device__ __forceinline__ void ll_wait_vm() {
 // neighbours. Across: kBK rows of kTile elements, read with the transposing LDS read (a group of 16
 // lanes takes 4 rows of 16 elements, lane i gets column i); 64-byte units at unit ^ key(row), the
 // four rows of a phase on different banks.
-template <int kTile, bool kAcross, int kPerm>
+template <int kTile, int kBK, bool kAcross, int kPerm>
 struct LlPanel {
-  static constexpr int kUnits = kTile / 32;
+  static constexpr int kUnits = kTile / 32, kChunks = kBK / 8;
+  static_assert(kBK == 64 || kBK == 32, "");
+  static __device__ __forceinline__ int chunk(int row, int c) { return kBK == 64 ? c ^ ((row >> 1) & 7) : c ^ ((row >> 2) & 3); }
   static __device__ __forceinline__ int key(int k) { return kUnits >= 4 ? k & 3 : kUnits == 2 ? (k >> 1) & 1 : 0; }
   // Bytes from the stage's first element to what slot `s` holds.
   static __device__ __forceinline__ uint32_t source(int s, uint32_t ld) {
@@ -67,8 +97,8 @@ struct LlPanel {
       const int k = s / (kTile / 8), c = s % (kTile / 8);
       return k * ld * 2 + ((((c >> 2) ^ key(k)) << 2) | (c & 3)) * 16;
     } else {
-      int row = s / 8;
-      const int c = (s % 8) ^ ((row >> 1) & 7);
+      int row = s / kChunks;
+      const int c = chunk(row, s % kChunks);
       if constexpr (kPerm > 1) row = row / (32 * kPerm) * (32 * kPerm) + kPerm * (row & 31) + (row >> 5) % kPerm;
       return row * ld * 2 + c * 16;
     }
@@ -88,7 +118,7 @@ struct LlPanel {
       return u.v;
     } else {
       const int row = 32 * tile + (lane & 31), c = 2 * ks + (lane >> 5);
-      return __builtin_bit_cast(lbf16x8, buf[row * 8 + (c ^ ((row >> 1) & 7))]);
+      return __builtin_bit_cast(lbf16x8, buf[row * kChunks + chunk(row, c)]);
     }
   }
 };
@@ -100,10 +130,13 @@ struct LlArgs {
   LossMatrix a, b;       // from the piece's first row and k on
   int k;                 // of the product, a whole number of stages
   int pairs;             // 1 or 6
-  int tiles_m, tiles_n, splits;
+  int tiles_m, tiles_n;
+  int units;             // of a tile: kRing stages each
+  int teams;             // of the gradients' products
+  float* partial;        // their tiles' parts
 };
 
-enum { kModeLse, kModeGrad, kModeDx, kModeDw };
+enum { kModeLse, kModeGrad, kModeGrad3, kModeDx, kModeDw };  // (kModeGrad3: g in three planes)
 
 // What all tokens' gradients are scaled by.
 struct LlScale {
@@ -121,156 +154,38 @@ struct LlOut {
   int rows, cols;        // of the output that exist, from the piece's first on
   float c;
   float2* part;          // kModeLse: [part][cols]
-  const float2* scale;   // kModeGrad: [rows]
+  const float2* scale;   // kModeGrad: [rows], and a tile's rows more
   bf16_t* g;
-  long long ld, plane;   // kModeGrad, kModeDx, kModeDw: row stride; planes of g, or from one split to the next
-  int planes;
+  long long ld, plane;   // row stride of g, dx, dw; from one plane of g to the next
   float* f;              // kModeDx, kModeDw with float32 output
   bf16_t* h;             // kModeDw with bf16 output
   int add;               // kModeDx: to what is there
   LlScale by;            // kModeDw
 };
 
+// What a tile's sums become.
+template <int kMode>
+constexpr bool kLlTeams = kMode == kModeDx || kMode == kModeDw;
+template <int kMode>
+constexpr bool kLlGrad = kMode == kModeGrad || kMode == kModeGrad3;
 template <class S, int kMode>
-__global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
-#if defined(__HIP_DEVICE_COMPILE__)  // the host's pass knows no buffer resources
-  constexpr bool kAAcross = kMode == kModeDx || kMode == kModeDw, kBAcross = kMode == kModeDw;
-  constexpr int kPerm = kMode == kModeGrad || kMode == kModeDx ? S::kNT : 1;
-  using PA = LlPanel<S::kM, kAAcross, 1>;
-  using PB = LlPanel<S::kN, kBAcross, kPerm>;
-  // Distinct objects, each chosen by a constant: the compiler then tells the copies in flight into one
-  // from the reads of another.
-  __shared__ u32x4 s0[S::kSlots], s1[S::kSlots], s2[S::kRing > 2 ? S::kSlots : 1], s3[S::kRing > 3 ? S::kSlots : 1];
-  const int lane = threadIdx.x & 63, j = lane & 31, g = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave % S::kWM, wn = wave / S::kWM;
+constexpr int ll_perm = kLlGrad<kMode> || kMode == kModeDx ? S::kNT : 1;
+template <bool kValue>
+struct LlBool {
+  static constexpr bool value = kValue;
+};
+template <int kValue>
+struct LlInt {
+  static constexpr int value = kValue;
+};
 
-  // Neighbouring tiles on one XCD: 8 of A by all of B share their operands in its L2.
-  int tm, tn, split;
-  {
-    const unsigned n = gridDim.x, per = n / 8, rem = n % 8, x = blockIdx.x % 8;
-    unsigned id = x * per + min(x, rem) + blockIdx.x / 8;
-    const unsigned tiles = p.tiles_m * p.tiles_n;
-    split = id / tiles;
-    id -= split * tiles;
-    const unsigned group = id / (8 * p.tiles_n), first = group * 8, wide = min(8u, p.tiles_m - first);
-    const unsigned in = id - group * 8 * p.tiles_n;
-    tm = first + in % wide;
-    tn = in / wide;
-  }
-  const int m0 = tm * S::kM, n0 = tn * S::kN;
-
-  const int nk = p.k / kBK, all = nk * p.pairs;
-  const int st0 = static_cast<int>(static_cast<long long>(split) * all / p.splits);
-  const int stages = static_cast<int>(static_cast<long long>(split + 1) * all / p.splits) - st0;
-
-  uint32_t off_a[S::kACopies], off_b[S::kBCopies];
-#pragma unroll
-  for (int t = 0; t < S::kACopies; ++t)
-    off_a[t] = PA::source((wave + S::kWaves * t) * 64 + lane, static_cast<uint32_t>(p.a.ld));
-#pragma unroll
-  for (int t = 0; t < S::kBCopies; ++t)
-    off_b[t] = PB::source((wave + S::kWaves * t) * 64 + lane, static_cast<uint32_t>(p.b.ld));
-
-  // The stage that is copied next; what lies past a matrix's end is read as zeros.
-  int next_pair = st0 / nk, next_k = st0 % nk;
-  const auto rsrc = [](const LossMatrix& m, int pl, long long at) {
-    const long long left = (m.end - at) * 2;
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t*>(m.base + pl * m.plane + at), 0,
-                                             static_cast<uint32_t>(left < 0 ? 0 : left > 0xfffffff0ll ? 0xfffffff0ll : left),
-                                             0x00027000);
-  };
-  const auto issue = [&](u32x4* d) {
-    const int pa = p.pairs == 1 ? 0 : (kPairsA >> (4 * next_pair)) & 15;
-    const int pb = p.pairs == 1 ? 0 : (kPairsB >> (4 * next_pair)) & 15;
-    const long long k0 = static_cast<long long>(next_k) * kBK;
-    const auto ra = rsrc(p.a, pa, kAAcross ? k0 * p.a.ld + m0 : m0 * p.a.ld + k0);
-    const auto rb = rsrc(p.b, pb, kBAcross ? k0 * p.b.ld + n0 : n0 * p.b.ld + k0);
-#pragma unroll
-    for (int t = 0; t < S::kACopies; ++t)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void_t)(d + 64 * (wave + S::kWaves * t)), 16, off_a[t], 0, 0, 0);
-#pragma unroll
-    for (int t = 0; t < S::kBCopies; ++t)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void_t)(d + S::kASlots + 64 * (wave + S::kWaves * t)), 16,
-                                               off_b[t], 0, 0, 0);
-    if (++next_k == nk) {
-      next_k = 0;
-      ++next_pair;
-    }
-  };
-
-  lf32x16 acc[S::kMT][S::kNT];
-#pragma unroll
-  for (int a = 0; a < S::kMT; ++a)
-#pragma unroll
-    for (int b = 0; b < S::kNT; ++b)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[a][b][e] = 0.f;
-
-  const auto compute = [&](const u32x4* buf) {
-    lbf16x8 a[2][S::kMT], b[2][S::kNT];
-    const auto load = [&](int ks) {
-#pragma unroll
-      for (int t = 0; t < S::kMT; ++t) a[ks & 1][t] = PA::fragment(buf, wm * S::kMT + t, ks, lane);
-#pragma unroll
-      for (int t = 0; t < S::kNT; ++t) b[ks & 1][t] = PB::fragment(buf + S::kASlots, wn * S::kNT + t, ks, lane);
-    };
-    load(0);
-#pragma unroll
-    for (int ks = 0; ks < kBK / 16; ++ks) {
-      if (ks + 1 < kBK / 16) load(ks + 1);
-#pragma unroll
-      for (int mt = 0; mt < S::kMT; ++mt)
-#pragma unroll
-        for (int nt = 0; nt < S::kNT; ++nt)
-          acc[mt][nt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[ks & 1][mt], b[ks & 1][nt], acc[mt][nt], 0, 0, 0);
-    }
-  };
-
-  // A ring of kRing stages: while one is multiplied, the next kRing - 1 are in flight. A stage has landed once
-  // at most the copies of those issued after it are outstanding; the barrier makes that hold for all
-  // waves, and says that all are done with the stage whose place the next copies take.
-#define MSS_LL_STEP(O, CUR, NEXT)                                    \
-  {                                                                  \
-    const int st = gg + O;                                           \
-    if (st < stages) {                                               \
-      const int later = min(S::kRing - 2, stages - 1 - st);          \
-      if (S::kRing > 3 && later >= 2) ll_wait_vm<(S::kRing > 3 ? 2 * S::kCopies : 0)>(); \
-      else if (S::kRing > 2 && later == 1) ll_wait_vm<(S::kRing > 2 ? S::kCopies : 0)>(); \
-      else ll_wait_vm<0>();                                          \
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");             \
-      __builtin_amdgcn_s_barrier();                                  \
-      if (st + S::kRing - 1 < stages) issue(NEXT);                   \
-      compute(CUR);                                                  \
-    }                                                                \
-  }
-  if (stages > 0) issue(s0);
-  if (S::kRing > 2 && stages > 1) issue(s1);
-  if (S::kRing > 3 && stages > 2) issue(s2);
-  if constexpr (S::kRing == 2) {
-    for (int gg = 0; gg < stages; gg += 2) {
-      MSS_LL_STEP(0, s0, s1)
-      MSS_LL_STEP(1, s1, s0)
-    }
-  } else if constexpr (S::kRing == 3) {
-    for (int gg = 0; gg < stages; gg += 3) {
-      MSS_LL_STEP(0, s0, s2)
-      MSS_LL_STEP(1, s1, s0)
-      MSS_LL_STEP(2, s2, s1)
-    }
-  } else {
-    for (int gg = 0; gg < stages; gg += 4) {
-      MSS_LL_STEP(0, s0, s3)
-      MSS_LL_STEP(1, s1, s0)
-      MSS_LL_STEP(2, s2, s1)
-      MSS_LL_STEP(3, s3, s2)
-    }
-  }
-#undef MSS_LL_STEP
-
-  const int wm0 = m0 + wm * 32 * S::kMT, wn0 = n0 + wn * 32 * S::kNT;
-  const auto row_of = [&](int mt, int r) { return wm0 + 32 * mt + 8 * (r >> 2) + 4 * g + (r & 3); };
-
+// (table: the scales of the tile's rows, kModeGrad)
+template <class S, int kMode>
+__device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[S::kMT][S::kNT], int tm, int tn, int wm, int wn,
+                                       int lane, const float2* table) {
+  const int j = lane & 31, g = lane >> 5;
+  const int m0 = tm * S::kM, wm0 = m0 + wm * 32 * S::kMT, wn0 = tn * S::kN + wn * 32 * S::kNT;
+  const auto row_of = [&](int mt, int r) LL_INLINE { return wm0 + 32 * mt + 8 * (r >> 2) + 4 * g + (r & 3); };
   if constexpr (kMode == kModeLse) {
     // Rows are words, columns tokens: a lane has the words of one token.
 #pragma unroll
@@ -299,68 +214,373 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
       if (g == 0 && t < o.cols)
         o.part[static_cast<long long>(tm * S::kWM + wm) * o.cols + t] = make_float2(m == -INFINITY ? m : mc, s);
     }
-  } else if constexpr (kMode == kModeGrad) {
+  } else if constexpr (kLlGrad<kMode>) {
     // Rows are tokens, columns words, kNT neighbours a lane. The words past the vocabulary are zeros.
     const int v = wn0 + S::kNT * j;
+    const uint32_t at = static_cast<uint32_t>(4 * g * o.ld + v) * 2;
+    const float2* scale = table + wm * 32 * S::kMT + 4 * g;
+    const auto rows = [&](auto edge) LL_INLINE {
 #pragma unroll
-    for (int mt = 0; mt < S::kMT; ++mt)
+      for (int mt = 0; mt < S::kMT; ++mt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int t = row_of(mt, r);
-        if (t >= o.rows) continue;
-        const float2 sc = o.scale[t];
-        float d[S::kNT];
-#pragma unroll
-        for (int nt = 0; nt < S::kNT; ++nt) {
-          d[nt] = fast_exp2(__builtin_fmaf(acc[mt][nt][r], o.c, -sc.x)) * sc.y;
-          if (v + nt >= o.cols) d[nt] = 0.f;
-        }
-        bf16_t* dst = o.g + t * o.ld + v;
-        for (int pl = 0; pl < o.planes; ++pl) {
-          alignas(8) uint16_t w[S::kNT];
+        for (int r = 0; r < 16; ++r) {
+          const int up = 32 * mt + 8 * (r >> 2) + (r & 3), t = wm0 + up;  // and 4 g more
+          const float2 sc = scale[up];
+          float d[S::kNT];
 #pragma unroll
           for (int nt = 0; nt < S::kNT; ++nt) {
-            const bf16_t b = f32_to_bf16(d[nt]);
-            w[nt] = b.bits;
-            d[nt] -= to_f32(b);
+            d[nt] = fast_exp2(__builtin_fmaf(acc[mt][nt][r], o.c, -sc.x)) * sc.y;
+            if (edge.value && v + nt >= o.cols) d[nt] = 0.f;
           }
-          __builtin_memcpy(dst + pl * o.plane, w, sizeof(w));
+          if (edge.value && t + 4 * g >= o.rows) continue;
+          char* dst = reinterpret_cast<char*>(o.g + t * o.ld) + at;
+#pragma unroll
+          for (int pl = 0; pl < (kMode == kModeGrad3 ? 3 : 1); ++pl) {
+            uint32_t w[(S::kNT + 1) / 2];
+#pragma unroll
+            for (int h = 0; h < (S::kNT + 1) / 2; ++h) w[h] = pack_bf16x2(d[2 * h], d[2 * h + 1 < S::kNT ? 2 * h + 1 : 2 * h]);
+            if constexpr (kMode == kModeGrad3) {
+#pragma unroll
+              for (int nt = 0; nt < S::kNT; ++nt)
+                d[nt] -= __uint_as_float(nt % 2 ? w[nt / 2] & 0xffff0000u : w[nt / 2] << 16);
+            }
+            __builtin_memcpy(dst + pl * o.plane * 2, w, 2 * S::kNT);
+          }
         }
-      }
+    };
+    if (m0 + S::kM <= o.rows && (tn + 1) * S::kN <= o.cols) {
+      rows(LlBool<false>{});
+    } else {
+      rows(LlBool<true>{});
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the next tile counts a whole tile's stores)
+    }
   } else if constexpr (kMode == kModeDx) {
     // Rows are features, columns tokens, kNT neighbours a lane.
-    float* f = o.f + split * o.plane;
     const int t = wn0 + S::kNT * j;
+    const uint32_t at = static_cast<uint32_t>(4 * g * o.ld + t) * 4;
+    if (t >= o.cols) return;  // (the rows are long enough for the last lane's kNT)
 #pragma unroll
     for (int mt = 0; mt < S::kMT; ++mt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int d = row_of(mt, r);
-        if (d >= o.rows || t >= o.cols) continue;  // (the rows are long enough for the last lane's kNT)
-        float* dst = f + d * o.ld + t;
-        float v[S::kNT];
-        if (o.add) __builtin_memcpy(v, dst, sizeof(v));
+      for (int q = 0; q < 4; ++q) {
+        const int d = wm0 + 32 * mt + 8 * q;  // and 4 g more
+        float v[4][S::kNT];
 #pragma unroll
-        for (int nt = 0; nt < S::kNT; ++nt) v[nt] = o.add ? v[nt] + acc[mt][nt][r] : acc[mt][nt][r];
-        __builtin_memcpy(dst, v, sizeof(v));
+        for (int r = 0; r < 4; ++r)
+          if (o.add && d + 4 * g + r < o.rows)
+            __builtin_memcpy(v[r], reinterpret_cast<const char*>(o.f + (d + r) * o.ld) + at, sizeof(v[r]));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+#pragma unroll
+          for (int nt = 0; nt < S::kNT; ++nt) v[r][nt] = o.add ? v[r][nt] + acc[mt][nt][4 * q + r] : acc[mt][nt][4 * q + r];
+          if (d + 4 * g + r < o.rows)
+            __builtin_memcpy(reinterpret_cast<char*>(o.f + (d + r) * o.ld) + at, v[r], sizeof(v[r]));
+        }
+        asm volatile("" ::: "memory");  // (a few rows at a time: all of what is there would not fit the registers)
       }
   } else {
     // Rows are words, columns features.
     const float by = shared_scale(o.by);
 #pragma unroll
+    for (int nt = 0; nt < S::kNT; ++nt) {
+      const int d = wn0 + 32 * nt + j;
+      if (d >= o.cols) continue;
+      const uint32_t at = static_cast<uint32_t>(4 * g * o.ld + d);
+#pragma unroll
+      for (int mt = 0; mt < S::kMT; ++mt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int v = wm0 + 32 * mt + 8 * (r >> 2) + (r & 3);  // and 4 g more
+          if (v + 4 * g >= o.rows) continue;
+          const float x = acc[mt][nt][r] * by;
+          if (o.h != nullptr) store_as(reinterpret_cast<bf16_t*>(reinterpret_cast<char*>(o.h + v * o.ld) + 2 * at), x);
+          else *reinterpret_cast<float*>(reinterpret_cast<char*>(o.f + v * o.ld) + 4 * at) = x;
+        }
+    }
+  }
+}
+
+// A workgroup's work is a row of segments: units of one tile each, whose copies follow one another through the
+// ring without a gap, so that a tile's first stages arrive under the one before's last products and its end.
+//
+// kModeLse, kModeGrad: whole tiles. The tiles are dealt out so that those at hand on one XCD are neighbours (8 of
+// A by all of B share their operands in its L2), and a workgroup's next one is as many further on as the
+// XCD has workgroups.
+//
+// kModeDx, kModeDw: the tiles of one range of tokens (words) are taken by a team of as many workgroups as there
+// are tiles of features, side by side, so that g is read once. The teams share the units of all ranges
+// evenly, in order: a team's first and last range may be a part of one, whose sums go to `partial` and are
+// added in order by ll_join_kernel.
+struct LlSegment {
+  int tm, tn, unit, n;  // the tile, its first unit, units: none at the end
+};
+
+struct LlDeal {
+  int first, step, end;       // whole tiles
+  int team, member;           // teams
+  long long from, to;         // units
+};
+
+__device__ __forceinline__ long long team_start(const LlArgs& p, long long units, int team) { return units * team / p.teams; }
+
+template <int kMode>
+__device__ __forceinline__ LlDeal ll_deal(const LlArgs& p) {
+  const unsigned n = gridDim.x, per = n / 8, rem = n % 8, x = blockIdx.x % 8, on = x < rem ? per + 1 : per;
+  LlDeal d{};
+  if constexpr (kLlTeams<kMode>) {
+    const int size = kMode == kModeDx ? p.tiles_m : p.tiles_n;
+    const unsigned id = x * per + min(x, rem) + blockIdx.x / 8;
+    const int team = id / size;
+    const long long units = static_cast<long long>(kMode == kModeDx ? p.tiles_n : p.tiles_m) * p.units;
+    d.team = team;
+    d.member = id % size;
+    d.from = team_start(p, units, team);
+    d.to = team_start(p, units, team + 1);
+  } else {
+    const long long tiles = static_cast<long long>(p.tiles_m) * p.tiles_n;
+    const long long before = x * per + min(x, rem);  // workgroups of the XCDs before this one
+    d.first = static_cast<int>(tiles * before / n + blockIdx.x / 8);
+    d.end = static_cast<int>(tiles * (before + on) / n);
+    d.step = on;
+  }
+  return d;
+}
+
+template <int kMode>
+__device__ __forceinline__ LlSegment ll_segment(const LlArgs& p, const LlDeal& d, int i) {
+  LlSegment s{};
+  if constexpr (kLlTeams<kMode>) {
+    const int range = static_cast<int>(d.from / p.units) + i;
+    const long long begin = static_cast<long long>(range) * p.units;
+    const long long a = d.from > begin ? d.from : begin, b = d.to < begin + p.units ? d.to : begin + p.units;
+    s.tm = kMode == kModeDx ? d.member : range;
+    s.tn = kMode == kModeDx ? range : d.member;
+    s.unit = static_cast<int>(a - begin);
+    s.n = a < b ? static_cast<int>(b - a) : 0;
+  } else {
+    const int id = d.first + i * d.step;
+    if (id >= d.end) return s;
+    const unsigned group = id / (8u * p.tiles_n), first = group * 8, wide = min(8u, p.tiles_m - first);
+    const unsigned in = id - group * 8 * p.tiles_n;
+    s.tm = first + in % wide;
+    s.tn = in / wide;
+    s.n = p.units;
+  }
+  return s;
+}
+
+// The sums of a part: of a team's first range (which = 0) or its last.
+template <class S, int kMode>
+__device__ __forceinline__ f32x4* ll_part(const LlArgs& p, int team, int which, int member) {
+  const int size = kMode == kModeDx ? p.tiles_m : p.tiles_n;
+  return reinterpret_cast<f32x4*>(p.partial) + ((2LL * team + which) * size + member) * (S::kM * S::kN / 4);
+}
+
+template <class S, int kMode>
+__global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
+#if defined(__HIP_DEVICE_COMPILE__)  // the host's pass knows no buffer resources
+  constexpr bool kAAcross = kLlTeams<kMode>, kBAcross = kMode == kModeDw;
+  constexpr int kBK = S::kBK;
+  using PA = LlPanel<S::kM, kBK, kAAcross, 1>;
+  using PB = LlPanel<S::kN, kBK, kBAcross, ll_perm<S, kMode>>;
+  __shared__ u32x4 s0[S::kSlots], s1[S::kSlots], s2[S::kRing > 2 ? S::kSlots : 1], s3[S::kRing > 3 ? S::kSlots : 1];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave % S::kWM, wn = wave / S::kWM;
+  __shared__ float2 s_scale[kLlGrad<kMode> ? S::kM : 1];
+  const LlDeal deal = ll_deal<kMode>(p);
+  const int nk = p.k / kBK;
+
+  uint32_t off_a[S::kACopies], off_b[S::kBCopies];
+#pragma unroll
+  for (int t = 0; t < S::kACopies; ++t)
+    off_a[t] = PA::source((wave + S::kWaves * t) * 64 + lane, static_cast<uint32_t>(p.a.ld));
+#pragma unroll
+  for (int t = 0; t < S::kBCopies; ++t)
+    off_b[t] = PB::source((wave + S::kWaves * t) * 64 + lane, static_cast<uint32_t>(p.b.ld));
+
+  // The stage that is copied next. What lies past a matrix's end, in a tile's stages past its last k, or past the
+  // last segment is zeros.
+  LlSegment next = ll_segment<kMode>(p, deal, 0);
+  int next_i = 0, next_left = next.n * S::kRing, next_pair = next.unit * S::kRing / nk, next_k = next.unit * S::kRing % nk;
+  const auto rsrc = [&](const LossMatrix& m, int pl, long long at) LL_INLINE {
+    const long long left = next_left > 0 && next_pair < p.pairs ? (m.end - at) * 2 : 0;
+    const uint64_t base = reinterpret_cast<uint64_t>(m.base + pl * m.plane + at);
+    return lu32x4{static_cast<uint32_t>(base), static_cast<uint32_t>(base >> 32) & 0xffff,
+                  static_cast<uint32_t>(left < 0 ? 0 : left > 0xfffffff0ll ? 0xfffffff0ll : left), 0x00027000};
+  };
+  const auto issue = [&](u32x4* d) LL_INLINE {
+    const int pa = p.pairs == 1 ? 0 : (kPairsA >> (4 * next_pair)) & 15;
+    const int pb = p.pairs == 1 ? 0 : (kPairsB >> (4 * next_pair)) & 15;
+    const long long k0 = static_cast<long long>(next_k) * kBK, m0 = static_cast<long long>(next.tm) * S::kM,
+                    n0 = static_cast<long long>(next.tn) * S::kN;
+    const auto ra = rsrc(p.a, pa, kAAcross ? k0 * p.a.ld + m0 : m0 * p.a.ld + k0);
+    const auto rb = rsrc(p.b, pb, kBAcross ? k0 * p.b.ld + n0 : n0 * p.b.ld + k0);
+#pragma unroll
+    for (int t = 0; t < S::kACopies; ++t)
+      ll_copy(ra, off_a[t], d + 64 * (wave + S::kWaves * t));
+#pragma unroll
+    for (int t = 0; t < S::kBCopies; ++t)
+      ll_copy(rb, off_b[t], d + S::kASlots + 64 * (wave + S::kWaves * t));
+    if (++next_k == nk) {
+      next_k = 0;
+      ++next_pair;
+    }
+    if (--next_left == 0) {
+      next = ll_segment<kMode>(p, deal, ++next_i);
+      next_left = next.n * S::kRing;
+      next_pair = next.unit * S::kRing / nk;
+      next_k = next.unit * S::kRing % nk;
+    }
+  };
+
+  // The scales of a tile's rows, by every wave, some of them the same ones.
+  const auto scales = [&](int tm) LL_INLINE {
+    constexpr int kSlices = S::kM / 128 > 0 ? S::kM / 128 : 1;  // of 1 KB
+    const uint64_t base = reinterpret_cast<uint64_t>(o.scale + tm * S::kM);
+    const lu32x4 r{static_cast<uint32_t>(base), static_cast<uint32_t>(base >> 32) & 0xffff, S::kM * 8, 0x00027000};
+    const int slice = wave % kSlices;
+    if (S::kM >= 128 || lane < S::kM / 2) ll_copy(r, 1024 * slice + 16 * lane, reinterpret_cast<const char*>(s_scale) + 1024 * slice);
+  };
+
+  lf32x16 acc[S::kMT][S::kNT];
+  // Operands of the step at hand and of the one after it.
+  lbf16x8 fa[2][S::kMT], fb[2][S::kNT];
+  const auto load = [&](const u32x4* buf, int ks) LL_INLINE {
+#pragma unroll
+    for (int t = 0; t < S::kMT; ++t) fa[ks & 1][t] = PA::fragment(buf, wm * S::kMT + t, ks, lane);
+#pragma unroll
+    for (int t = 0; t < S::kNT; ++t) fb[ks & 1][t] = PB::fragment(buf + S::kASlots, wn * S::kNT + t, ks, lane);
+  };
+  const auto multiply = [&](int ks) LL_INLINE {
+#pragma unroll
     for (int mt = 0; mt < S::kMT; ++mt)
 #pragma unroll
       for (int nt = 0; nt < S::kNT; ++nt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int v = row_of(mt, r), d = wn0 + 32 * nt + j;
-          if (v >= o.rows || d >= o.cols) continue;
-          const float x = acc[mt][nt][r] * by;
-          if (o.h != nullptr) store_as(o.h + v * o.ld + d, x);
-          else o.f[split * o.plane + v * o.ld + d] = x;
-        }
-  }
+        acc[mt][nt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[ks & 1][mt], fb[ks & 1][nt], acc[mt][nt], 0, 0, 0);
+  };
+#ifndef LL_V
+#define LL_V 4
 #endif
+  constexpr int kSteps = kBK / 16;
+  constexpr int kReads = S::kMT * (kAAcross ? 2 : 1) + S::kNT * (kBAcross ? 2 : 1), kProducts = S::kMT * S::kNT;
+  constexpr int kEach = (kReads + kProducts - 1) / kProducts;
+  const auto weave = [&]() LL_INLINE {  // a read behind each product
+    if (LL_V == 4) {
+#pragma unroll
+      for (int i = 0; i < kProducts; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, kEach, 0);
+      }
+    } else if (LL_V == 7) {
+      __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, kProducts, 0);
+    }
+  };
+  // A ring of kRing stages. Before the last step of a stage all waves meet: they have read all of it, so its place
+  // takes the copies of the stage kRing further on, and the stage behind it has landed, so that its first
+  // operands are read under that last step's products.
+  const auto step = [&](u32x4* cur, const u32x4* next, auto newer) LL_INLINE {
+#pragma unroll
+    for (int ks = 0; ks + 1 < kSteps; ++ks) {
+      load(cur, ks + 1);
+      multiply(ks);
+      weave();
+    }
+    ll_meet<(S::kRing - 2) * S::kCopies + newer.value>();
+    issue(cur);
+    load(next, 0);
+    multiply(kSteps - 1);
+    weave();
+  };
+  issue(s0);
+  issue(s1);
+  if constexpr (S::kRing > 2) issue(s2);
+  if constexpr (S::kRing > 3) issue(s3);
+  ll_meet<(S::kRing - 1) * S::kCopies>();
+  load(s0, 0);
+  for (int i = 0;; ++i) {
+    const LlSegment seg = ll_segment<kMode>(p, deal, i);
+    if (seg.n == 0) break;
+#pragma unroll
+    for (int a = 0; a < S::kMT; ++a)
+#pragma unroll
+      for (int b = 0; b < S::kNT; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[a][b][e] = 0.f;
+    const auto unit = [&](auto newer, bool first) LL_INLINE {
+      step(s0, s1, newer);
+      // The scales of the tile's rows, once all waves are through with the ones before.
+      if constexpr (kLlGrad<kMode>) {
+        if (first) scales(seg.tm);
+      }
+      if constexpr (S::kRing == 2) {
+        step(s1, s0, LlInt<0>{});
+      } else {
+        step(s1, s2, LlInt<0>{});
+        step(s2, s3, LlInt<0>{});
+        step(s3, s0, LlInt<0>{});
+      }
+    };
+    // (The first unit of a later tile meets while the stores of the one before, newer than its copies, go on.)
+    constexpr int kStores = S::kRing == 2 && kMode == kModeGrad ? 16 * S::kMT : 0;
+    int u = 0;
+    if constexpr (kLlGrad<kMode>) {
+      if (i > 0) unit(LlInt<kStores>{}, true);
+      else unit(LlInt<0>{}, true);
+      u = 1;
+    }
+    for (; u < seg.n; ++u) unit(LlInt<0>{}, false);
+    if constexpr (kLlTeams<kMode>) {
+      if (seg.n < p.units) {
+        // A part: its sums, in the order in which the lanes hold them.
+        f32x4* dst = ll_part<S, kMode>(p, deal.team, i > 0, deal.member) + wave * (S::kSums / 4 * 64) + lane;
+#pragma unroll
+        for (int e = 0; e < S::kSums / 4; ++e)
+          dst[64 * e] = f32x4{acc[e / 4 / S::kNT][e / 4 % S::kNT][4 * (e % 4)], acc[e / 4 / S::kNT][e / 4 % S::kNT][4 * (e % 4) + 1],
+                              acc[e / 4 / S::kNT][e / 4 % S::kNT][4 * (e % 4) + 2], acc[e / 4 / S::kNT][e / 4 % S::kNT][4 * (e % 4) + 3]};
+        continue;
+      }
+    }
+    ll_end<S, kMode>(o, acc, seg.tm, seg.tn, wm, wn, lane, s_scale);
+    // (Nothing that the compiler knows of is outstanding: else it would wait in the loop, with the copies.)
+    if constexpr (kLlTeams<kMode>) __builtin_amdgcn_s_waitcnt(0x0f70);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy outlives the workgroup's LDS
+#endif
+}
+
+// The tiles of which teams have parts: the parts' sums in order.
+template <class S, int kMode>
+__global__ __launch_bounds__(S::kThreads) void ll_join_kernel(LlArgs p, LlOut o) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int size = kMode == kModeDx ? p.tiles_m : p.tiles_n, ranges = kMode == kModeDx ? p.tiles_n : p.tiles_m;
+  const int range = blockIdx.x / size, member = blockIdx.x % size;
+  const long long units = static_cast<long long>(ranges) * p.units, begin = static_cast<long long>(range) * p.units;
+  int team = static_cast<int>(begin * p.teams / units);  // the one with the range's first unit
+  while (team > 0 && team_start(p, units, team) > begin) --team;
+  while (team_start(p, units, team + 1) <= begin) ++team;
+  if (team_start(p, units, team + 1) >= begin + p.units) return;  // a whole one
+  lf32x16 acc[S::kMT][S::kNT];
+#pragma unroll
+  for (int a = 0; a < S::kMT; ++a)
+#pragma unroll
+    for (int b = 0; b < S::kNT; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[a][b][e] = 0.f;
+  for (; team < p.teams && team_start(p, units, team) < begin + p.units; ++team) {
+    const long long from = team_start(p, units, team);
+    if (from == team_start(p, units, team + 1)) continue;
+    const f32x4* src = ll_part<S, kMode>(p, team, from / p.units != range, member) + wave * (S::kSums / 4 * 64) + lane;
+#pragma unroll
+    for (int e = 0; e < S::kSums / 4; ++e) {
+      const f32x4 v = src[64 * e];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) acc[e / 4 / S::kNT][e / 4 % S::kNT][4 * (e % 4) + q] += v[q];
+    }
+  }
+  ll_end<S, kMode>(o, acc, kMode == kModeDx ? member : range, kMode == kModeDx ? range : member, wave % S::kWM,
+                   wave / S::kWM, lane, nullptr);
 }
 
 // ------------------------------------------------------------------------- operands
@@ -579,28 +799,16 @@ __global__ __launch_bounds__(256) void ll_wanted_kernel(LinLossParams p, int v0,
   for (int pl = 0; pl < kPlanes; ++pl) p.g[pl * (p.tokens * p.ldg) + t * p.ldg + v] = b[pl];
 }
 
-// dx from the splits' sums.
+// dx from its sums over the pieces.
 template <typename out_t>
 __global__ __launch_bounds__(256) void ll_dx_kernel(LinLossParams p, LlScale scale) {
   const float by = shared_scale(scale);
-  const long long n = static_cast<long long>(p.features) * p.tokens, plane = p.features * p.ldx;
+  const long long n = static_cast<long long>(p.features) * p.tokens;
   out_t* out = static_cast<out_t*>(p.dx);
   for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n; i += gridDim.x * 256LL) {
     const long long d = i / p.tokens, t = i - d * p.tokens;
-    const float* src = p.dx_part + d * p.ldx + t;
-    float v = src[0];
-    for (int s = 1; s < p.x_splits; ++s) v += src[s * plane];
+    const float v = p.dx_sum[d * p.ldx + t];
     store_as(out + i, p.r.live[t] == 0.f ? 0.f : v * by);
-  }
-}
-
-// dw of a piece from the splits' sums.
-template <typename out_t>
-__global__ __launch_bounds__(256) void ll_dw_kernel(const float* part, int splits, long long plane, long long n, out_t* out) {
-  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n; i += gridDim.x * 256LL) {
-    float v = part[i];
-    for (int s = 1; s < splits; ++s) v += part[s * plane + i];
-    store_as(out + i, v);
   }
 }
 
@@ -616,17 +824,47 @@ typedef LlShape<2, 2, 2, 2, 2> LlSmall;    // 128 x 128, waves of 64 x 64
 typedef LlShape<4, 1, 1, 1, 4> LlThinN;    // 128 x 32, waves of 32 x 32
 typedef LlShape<1, 4, 1, 1, 4> LlThinM;    // 32 x 128
 
+// Teams of `size` workgroups for `ranges` ranges: as many as there is room for, but at least two units each.
+template <class S>
+int ll_teams(int size, int ranges, int units) {
+  const long long all = static_cast<long long>(ranges) * units;
+  long long n = kCUs * S::kPerCU / size;
+  n = n < all / 2 ? n : all / 2;
+  return static_cast<int>(n < 1 ? 1 : n);
+}
+
 template <class S, int kMode>
 void launch_product(LlArgs a, const LlOut& o, hipStream_t stream) {
   a.tiles_m = (o.rows + S::kM - 1) / S::kM;
   a.tiles_n = (o.cols + S::kN - 1) / S::kN;
-  hipLaunchKernelGGL((ll_kernel<S, kMode>), dim3(a.tiles_m * a.tiles_n * a.splits), dim3(S::kThreads), 0, stream, a, o);
+  const int stages = a.k / S::kBK * a.pairs;
+  a.units = (stages + S::kRing - 1) / S::kRing;
+  const int room = kCUs * S::kPerCU;
+  const long long tiles = static_cast<long long>(a.tiles_m) * a.tiles_n;
+  if constexpr (kLlTeams<kMode>) {
+    const int size = kMode == kModeDx ? a.tiles_m : a.tiles_n;
+    a.teams = ll_teams<S>(size, kMode == kModeDx ? a.tiles_n : a.tiles_m, a.units);
+    hipLaunchKernelGGL((ll_kernel<S, kMode>), dim3(a.teams * size), dim3(S::kThreads), 0, stream, a, o);
+    if (tiles / size * a.units % a.teams != 0 || tiles / size * a.units / a.teams % a.units != 0)
+      hipLaunchKernelGGL((ll_join_kernel<S, kMode>), dim3(static_cast<unsigned>(tiles)), dim3(S::kThreads), 0, stream, a, o);
+  } else {
+    hipLaunchKernelGGL((ll_kernel<S, kMode>), dim3(static_cast<unsigned>(tiles < room ? tiles : room)), dim3(S::kThreads), 0,
+                       stream, a, o);
+  }
+}
+
+// f of the shape of a product: words x tokens, tokens x words, features x tokens, words x features.
+template <typename F>
+auto with_shape(int shape, int mode, F&& f) {
+  if (shape == 0) return f(LlSmall{});
+  if (mode == kModeGrad) return shape == 1 ? f(LlLargeN{}) : f(LlThinM{});
+  if (shape == 1) return f(LlLargeM{});
+  return mode == kModeDw ? f(LlSmall{}) : f(LlThinN{});
 }
 
 template <int kMode>
 void launch_shaped(int shape, const LlArgs& a, const LlOut& o, hipStream_t stream) {
-  // (rows and columns: words x tokens, tokens x words, features x tokens, words x features)
-  if constexpr (kMode == kModeGrad) {
+  if constexpr (kLlGrad<kMode>) {
     if (shape == 0) launch_product<LlSmall, kMode>(a, o, stream);
     else if (shape == 1) launch_product<LlLargeN, kMode>(a, o, stream);
     else launch_product<LlThinM, kMode>(a, o, stream);
@@ -638,6 +876,19 @@ void launch_shaped(int shape, const LlArgs& a, const LlOut& o, hipStream_t strea
     else if (shape == 1) launch_product<LlLargeM, kMode>(a, o, stream);
     else launch_product<LlThinN, kMode>(a, o, stream);
   }
+}
+
+// Floats of the teams' parts in a gradient's product of `features` by `others`.
+template <class S>
+long long part_sums(int features, int others, int stages) {
+  // (features are the tiles' rows in dx, their columns in dw)
+  const int tile_f = S::kM, tile_o = S::kN;
+  const long long size_x = (features + tile_f - 1) / tile_f, ranges_x = (others + tile_o - 1) / tile_o;
+  const long long size_w = (features + tile_o - 1) / tile_o, ranges_w = (others + tile_f - 1) / tile_f;
+  const int units = (stages + S::kRing - 1) / S::kRing;
+  const long long x = 2LL * ll_teams<S>(static_cast<int>(size_x), static_cast<int>(ranges_x), units) * size_x;
+  const long long w = 2LL * ll_teams<S>(static_cast<int>(size_w), static_cast<int>(ranges_w), units) * size_w;
+  return (x > w ? x : w) * S::kM * S::kN;
 }
 
 LossMatrix weight_planes(const LinLossParams& p) {
@@ -672,15 +923,12 @@ LinLossPlan linloss_plan(int tokens, int features, int vocab, int planes) {
   q.piece = static_cast<int>(((whole / 256 + pieces - 1) / pieces) * 256);
   q.ldg = q.piece;
   q.ldx = (tokens + 3) / 4 * 4;
-  const int tx = q.shape == 1 ? 256 : 128, tt = q.shape == 1 ? 256 : q.shape == 0 ? 128 : 32;
-  const auto splits = [&](long long tiles, long long stages) {
-    long long s = kCUs / tiles;
-    s = s < stages / 4 ? s : stages / 4;
-    return static_cast<int>(s < 1 ? 1 : s);
-  };
-  const int pairs = planes == 1 ? 1 : 6;
-  q.x_splits = splits(tiles_of(features, tokens, tx, tt), static_cast<long long>(q.piece) / kBK * pairs);
-  q.w_splits = splits(tiles_of(q.piece < vocab ? q.piece : vocab, features, tx, tx), (tokens + kBK - 1LL) / kBK * pairs);
+  const int x_stages = q.piece / 64 * (planes == 1 ? 1 : 6);
+  const int w_stages = (tokens + kLlK - 1) / kLlK * (kLlK / 64) * (planes == 1 ? 1 : 6);
+  const int words = q.piece < vocab ? q.piece : vocab;
+  const long long x = with_shape(q.shape, kModeDx, [&](auto s) { return part_sums<decltype(s)>(features, tokens, x_stages); });
+  const long long w = with_shape(q.shape, kModeDw, [&](auto s) { return part_sums<decltype(s)>(features, words, w_stages); });
+  q.partial = x > w ? x : w;
   return q;
 }
 
@@ -701,7 +949,6 @@ hipError_t launch_linloss_fwd(const LinLossParams& p, const LinLossPlan& plan, h
   a.b = x_planes(p);
   a.k = p.width;
   a.pairs = f32 ? 6 : 1;
-  a.splits = 1;
   LlOut o{};
   o.rows = p.vocab;
   o.cols = p.tokens;
@@ -739,7 +986,7 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
     a.a = x;
     a.b = wp;
     a.k = p.width;
-    a.splits = 1;
+    a.partial = p.partial;
     LlOut o{};
     o.rows = p.tokens;
     o.cols = words;
@@ -748,55 +995,36 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
     o.g = p.g;
     o.ld = p.ldg;
     o.plane = g.plane;
-    o.planes = p.planes;
-    launch_shaped<kModeGrad>(plan.shape, a, o, stream);
+    if (f32) launch_shaped<kModeGrad3>(plan.shape, a, o, stream);
+    else launch_shaped<kModeGrad>(plan.shape, a, o, stream);
     const dim3 wg(static_cast<unsigned>((static_cast<long long>(p.tokens) * p.r.top + 255) / 256));
     if (f32) hipLaunchKernelGGL(ll_wanted_kernel<3>, wg, dim3(256), 0, stream, p, static_cast<int>(v0), words);
     else hipLaunchKernelGGL(ll_wanted_kernel<1>, wg, dim3(256), 0, stream, p, static_cast<int>(v0), words);
     if (p.dx != nullptr) {
       a.a = wp;
       a.b = g;
-      a.k = (words + kBK - 1) / kBK * kBK;
-      a.splits = p.x_splits;
+      a.k = (words + kLlK - 1) / kLlK * kLlK;
       o = LlOut{};
       o.rows = p.features;
       o.cols = p.tokens;
-      o.f = p.dx_part;
+      o.f = p.dx_sum;
       o.ld = p.ldx;
-      o.plane = p.features * p.ldx;
       o.add = v0 > 0;
       launch_shaped<kModeDx>(plan.shape, a, o, stream);
     }
     if (p.dw != nullptr) {
       a.a = g;
       a.b = x;
-      a.k = (p.tokens + kBK - 1) / kBK * kBK;
-      a.splits = p.w_splits;
+      a.k = (p.tokens + kLlK - 1) / kLlK * kLlK;
       o = LlOut{};
       o.rows = words;
       o.cols = p.features;
       o.ld = p.features;
       o.by = by;
       void* dst = static_cast<char*>(p.dw) + v0 * p.features * (p.dw_bf16 ? 2 : 4);
-      const long long n = static_cast<long long>(words) * p.features;
-      if (p.w_splits > 1) {
-        o.f = p.dw_part;
-        o.plane = static_cast<long long>(p.piece) * p.features;
-      } else if (p.dw_bf16) {
-        o.h = static_cast<bf16_t*>(dst);
-      } else {
-        o.f = static_cast<float*>(dst);
-      }
+      if (p.dw_bf16) o.h = static_cast<bf16_t*>(dst);
+      else o.f = static_cast<float*>(dst);
       launch_shaped<kModeDw>(plan.shape, a, o, stream);
-      if (p.w_splits > 1) {
-        const dim3 dg(blocks_for(n, 4096));
-        if (p.dw_bf16)
-          hipLaunchKernelGGL(ll_dw_kernel<bf16_t>, dg, dim3(256), 0, stream, p.dw_part, p.w_splits, o.plane, n,
-                             static_cast<bf16_t*>(dst));
-        else
-          hipLaunchKernelGGL(ll_dw_kernel<float>, dg, dim3(256), 0, stream, p.dw_part, p.w_splits, o.plane, n,
-                             static_cast<float*>(dst));
-      }
     }
   }
   if (p.dx != nullptr) {

@@ -14,6 +14,7 @@
 namespace mss {
 
 constexpr int kLossMaxTop = 1024;
+constexpr int kLinLossTile = 256;  // largest side of a product's tile
 enum { kLossNone = 0, kLossSum = 1, kLossMean = 2 };
 
 // The rows' wanted words (launch_loss_rows). A row counts if it has one: live is 0 (no), 1 (yes), or NaN
@@ -66,14 +67,12 @@ struct LinLossParams {
   float* mean;     // the reduced loss, then 1 / (rows that count)
   // backward
   const float* grad;  // [1], or [tokens] without a reduction
-  float2* scale;      // [tokens]: lse, and what multiplies the row's gradient
+  float2* scale;      // [tokens + kLinLossTile]: lse, and what multiplies the row's gradient
   bf16_t* g;          // [planes][tokens][ldg] the logits' gradient for a piece of the vocabulary
   long long ldg;
-  float* dx_part;     // [x_splits][features][ldx]
+  float* dx_sum;      // [features][ldx]
   long long ldx;
-  int x_splits;
-  float* dw_part;     // [w_splits][piece][features] where w_splits > 1
-  int w_splits;
+  float* partial;     // sums of tiles that several workgroups share
   int piece;          // words of a piece
   void* dx;           // [features][tokens] as x
   void* dw;           // [vocab][features]
@@ -83,8 +82,8 @@ struct LinLossParams {
 // What the call needs besides its operands; sizes depend on nothing but the arguments.
 struct LinLossPlan {
   int shape;          // of the tiles
-  int parts, piece, x_splits, w_splits;
-  long long ldg, ldx;
+  int parts, piece;
+  long long ldg, ldx, partial;
 };
 LinLossPlan linloss_plan(int tokens, int features, int vocab, int planes);
 

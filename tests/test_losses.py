@@ -369,7 +369,8 @@ def test_linear_weight_copies_and_holder():
         assert dw.dtype == F32
         _check_linear_grads(ref, xd, wd, scale, BF16, F32, dx, dw)
     holder = GradHolder()
-    (dx2,) = torch.autograd.grad(linear_cross_entropy(x, w, targets, holder=holder), (x,), retain_graph=False)
+    (dx2,) = torch.autograd.grad(linear_cross_entropy(x, w, targets, holder=holder), (x,))
+    holder.take()  # (it adds up what it is given)
     loss = linear_cross_entropy(x, w, targets, weight_act=act, holder=holder)
     loss.backward()
     assert w.grad is None and torch.equal(holder.take(), dw) and torch.equal(x.grad, dx)
