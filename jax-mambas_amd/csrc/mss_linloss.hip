@@ -57,10 +57,7 @@ typedef uint32_t lu32x4 __attribute__((ext_vector_type(4)));
 // waits for all that are in flight before the next transposing read, whose place it does not know. The
 // account is this file's: ll_meet. (m0 is nobody's across statements: the compiler sets it where it reads it.)
 __device__ __forceinline__ void ll_copy(lu32x4 rsrc, uint32_t offset, const void* lds) {
-  // (the same in all lanes, and in scalar registers already where the compiler knew)
-  uint32_t to = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void_t)lds)));
-#pragma unroll
-  for (int i = 0; i < 4; ++i) rsrc[i] = __builtin_amdgcn_readfirstlane(rsrc[i]);
+  const uint32_t to = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void_t)lds));
   asm volatile(
       "s_mov_b32 m0, %0\n\t"
       "s_nop 0\n\t"
@@ -179,56 +176,56 @@ struct LlInt {
   static constexpr int value = kValue;
 };
 
-// (table: the scales of the tile's rows, kModeGrad)
-template <class S, int kMode>
-__device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[S::kMT][S::kNT], int tm, int tn, int wm, int wn,
-                                       int lane, const float2* table) {
+// A wave's kMT x kNT matrix tiles: from row wm0 and column wn0 on, in part `part` of the rows. table: the scales of
+// its rows (kModeGrad).
+template <int kMode, int kMT, int kNT>
+__device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT], int wm0, int wn0, int part, int lane,
+                                       const float2* table) {
   const int j = lane & 31, g = lane >> 5;
-  const int m0 = tm * S::kM, wm0 = m0 + wm * 32 * S::kMT, wn0 = tn * S::kN + wn * 32 * S::kNT;
   const auto row_of = [&](int mt, int r) LL_INLINE { return wm0 + 32 * mt + 8 * (r >> 2) + 4 * g + (r & 3); };
   if constexpr (kMode == kModeLse) {
     // Rows are words, columns tokens: a lane has the words of one token.
 #pragma unroll
-    for (int nt = 0; nt < S::kNT; ++nt) {
-      if (m0 + S::kM > o.rows) {
+    for (int nt = 0; nt < kNT; ++nt) {
+      if (wm0 + 32 * kMT > o.rows) {
 #pragma unroll
-        for (int mt = 0; mt < S::kMT; ++mt)
+        for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             if (row_of(mt, r) >= o.rows) acc[mt][nt][r] = -INFINITY;
       }
       float m = acc[0][nt][0];
 #pragma unroll
-      for (int mt = 0; mt < S::kMT; ++mt)
+      for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[mt][nt][r]);
       m = fmaxf(m, __shfl_xor(m, 32));
       const float mc = m == -INFINITY ? 0.f : m * o.c;
       float s = 0.f;
 #pragma unroll
-      for (int mt = 0; mt < S::kMT; ++mt)
+      for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) s += fast_exp2(__builtin_fmaf(acc[mt][nt][r], o.c, -mc));
       s += __shfl_xor(s, 32);
       const int t = wn0 + 32 * nt + j;
       if (g == 0 && t < o.cols)
-        o.part[static_cast<long long>(tm * S::kWM + wm) * o.cols + t] = make_float2(m == -INFINITY ? m : mc, s);
+        o.part[static_cast<long long>(part) * o.cols + t] = make_float2(m == -INFINITY ? m : mc, s);
     }
   } else if constexpr (kLlGrad<kMode>) {
     // Rows are tokens, columns words, kNT neighbours a lane. The words past the vocabulary are zeros.
-    const int v = wn0 + S::kNT * j;
+    const int v = wn0 + kNT * j;
     const uint32_t at = static_cast<uint32_t>(4 * g * o.ld + v) * 2;
-    const float2* scale = table + wm * 32 * S::kMT + 4 * g;
+    const float2* scale = table + 4 * g;
     const auto rows = [&](auto edge) LL_INLINE {
 #pragma unroll
-      for (int mt = 0; mt < S::kMT; ++mt)
+      for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int up = 32 * mt + 8 * (r >> 2) + (r & 3), t = wm0 + up;  // and 4 g more
           const float2 sc = scale[up];
-          float d[S::kNT];
+          float d[kNT];
 #pragma unroll
-          for (int nt = 0; nt < S::kNT; ++nt) {
+          for (int nt = 0; nt < kNT; ++nt) {
             d[nt] = fast_exp2(__builtin_fmaf(acc[mt][nt][r], o.c, -sc.x)) * sc.y;
             if (edge.value && v + nt >= o.cols) d[nt] = 0.f;
           }
@@ -236,19 +233,19 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[S::kMT][S:
           char* dst = reinterpret_cast<char*>(o.g + t * o.ld) + at;
 #pragma unroll
           for (int pl = 0; pl < (kMode == kModeGrad3 ? 3 : 1); ++pl) {
-            uint32_t w[(S::kNT + 1) / 2];
+            uint32_t w[(kNT + 1) / 2];
 #pragma unroll
-            for (int h = 0; h < (S::kNT + 1) / 2; ++h) w[h] = pack_bf16x2(d[2 * h], d[2 * h + 1 < S::kNT ? 2 * h + 1 : 2 * h]);
+            for (int h = 0; h < (kNT + 1) / 2; ++h) w[h] = pack_bf16x2(d[2 * h], d[2 * h + 1 < kNT ? 2 * h + 1 : 2 * h]);
             if constexpr (kMode == kModeGrad3) {
 #pragma unroll
-              for (int nt = 0; nt < S::kNT; ++nt)
+              for (int nt = 0; nt < kNT; ++nt)
                 d[nt] -= __uint_as_float(nt % 2 ? w[nt / 2] & 0xffff0000u : w[nt / 2] << 16);
             }
-            __builtin_memcpy(dst + pl * o.plane * 2, w, 2 * S::kNT);
+            __builtin_memcpy(dst + pl * o.plane * 2, w, 2 * kNT);
           }
         }
     };
-    if (m0 + S::kM <= o.rows && (tn + 1) * S::kN <= o.cols) {
+    if (wm0 + 32 * kMT <= o.rows && wn0 + 32 * kNT <= o.cols) {
       rows(LlBool<false>{});
     } else {
       rows(LlBool<true>{});
@@ -256,15 +253,15 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[S::kMT][S:
     }
   } else if constexpr (kMode == kModeDx) {
     // Rows are features, columns tokens, kNT neighbours a lane.
-    const int t = wn0 + S::kNT * j;
+    const int t = wn0 + kNT * j;
     const uint32_t at = static_cast<uint32_t>(4 * g * o.ld + t) * 4;
     if (t >= o.cols) return;  // (the rows are long enough for the last lane's kNT)
 #pragma unroll
-    for (int mt = 0; mt < S::kMT; ++mt)
+    for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int d = wm0 + 32 * mt + 8 * q;  // and 4 g more
-        float v[4][S::kNT];
+        float v[4][kNT];
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           if (o.add && d + 4 * g + r < o.rows)
@@ -272,7 +269,7 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[S::kMT][S:
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
 #pragma unroll
-          for (int nt = 0; nt < S::kNT; ++nt) v[r][nt] = o.add ? v[r][nt] + acc[mt][nt][4 * q + r] : acc[mt][nt][4 * q + r];
+          for (int nt = 0; nt < kNT; ++nt) v[r][nt] = o.add ? v[r][nt] + acc[mt][nt][4 * q + r] : acc[mt][nt][4 * q + r];
           if (d + 4 * g + r < o.rows)
             __builtin_memcpy(reinterpret_cast<char*>(o.f + (d + r) * o.ld) + at, v[r], sizeof(v[r]));
         }
@@ -282,12 +279,12 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[S::kMT][S:
     // Rows are words, columns features.
     const float by = shared_scale(o.by);
 #pragma unroll
-    for (int nt = 0; nt < S::kNT; ++nt) {
+    for (int nt = 0; nt < kNT; ++nt) {
       const int d = wn0 + 32 * nt + j;
       if (d >= o.cols) continue;
       const uint32_t at = static_cast<uint32_t>(4 * g * o.ld + d);
 #pragma unroll
-      for (int mt = 0; mt < S::kMT; ++mt)
+      for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int v = wm0 + 32 * mt + 8 * (r >> 2) + (r & 3);  // and 4 g more
@@ -438,7 +435,10 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
   const auto scales = [&](int tm) LL_INLINE {
     constexpr int kSlices = S::kM / 128 > 0 ? S::kM / 128 : 1;  // of 1 KB
     const uint64_t base = reinterpret_cast<uint64_t>(o.scale + tm * S::kM);
-    const lu32x4 r{static_cast<uint32_t>(base), static_cast<uint32_t>(base >> 32) & 0xffff, S::kM * 8, 0x00027000};
+    // (readfirstlane: it is the same in all lanes, which the compiler does not see)
+    const lu32x4 r{static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(base))),
+                   static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(base >> 32) & 0xffff)),
+                   S::kM * 8, 0x00027000};
     const int slice = wave % kSlices;
     if (S::kM >= 128 || lane < S::kM / 2) ll_copy(r, 1024 * slice + 16 * lane, reinterpret_cast<const char*>(s_scale) + 1024 * slice);
   };
@@ -475,6 +475,19 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
     } else if (LL_V == 7) {
       __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
       __builtin_amdgcn_sched_group_barrier(0x008, kProducts, 0);
+    } else if (LL_V == 9) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, kProducts - 1, 0);
+    } else if (LL_V == 10) {
+#pragma unroll
+      for (int i = 0; i < (kReads + 1) / 2; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, kProducts - (kReads + 1) / 2, 0);
+    } else if (LL_V == 11 || LL_V == 12) {
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
   // A ring of kRing stages. Before the last step of a stage all waves meet: they have read all of it, so its place
@@ -484,13 +497,19 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
 #pragma unroll
     for (int ks = 0; ks + 1 < kSteps; ++ks) {
       load(cur, ks + 1);
+      if (LL_V == 11 || LL_V == 12) __builtin_amdgcn_sched_barrier(0);
+      if (LL_V == 12) __builtin_amdgcn_s_setprio(1);
       multiply(ks);
+      if (LL_V == 12) __builtin_amdgcn_s_setprio(0);
       weave();
     }
     ll_meet<(S::kRing - 2) * S::kCopies + newer.value>();
     issue(cur);
     load(next, 0);
+    if (LL_V == 11 || LL_V == 12) __builtin_amdgcn_sched_barrier(0);
+    if (LL_V == 12) __builtin_amdgcn_s_setprio(1);
     multiply(kSteps - 1);
+    if (LL_V == 12) __builtin_amdgcn_s_setprio(0);
     weave();
   };
   issue(s0);
@@ -523,7 +542,7 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
       }
     };
     // (The first unit of a later tile meets while the stores of the one before, newer than its copies, go on.)
-    constexpr int kStores = S::kRing == 2 && kMode == kModeGrad ? 16 * S::kMT : 0;
+    constexpr int kStores = S::kRing == 2 && kMode == kModeGrad && S::kMT <= 2 ? 16 * S::kMT : 0;
     int u = 0;
     if constexpr (kLlGrad<kMode>) {
       if (i > 0) unit(LlInt<kStores>{}, true);
@@ -542,7 +561,8 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
         continue;
       }
     }
-    ll_end<S, kMode>(o, acc, seg.tm, seg.tn, wm, wn, lane, s_scale);
+    ll_end<kMode>(o, acc, seg.tm * S::kM + wm * 32 * S::kMT, seg.tn * S::kN + wn * 32 * S::kNT, seg.tm * S::kWM + wm, lane,
+                  s_scale + wm * 32 * S::kMT);
     // (Nothing that the compiler knows of is outstanding: else it would wait in the loop, with the copies.)
     if constexpr (kLlTeams<kMode>) __builtin_amdgcn_s_waitcnt(0x0f70);
   }
@@ -550,37 +570,40 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
 #endif
 }
 
-// The tiles of which teams have parts: the parts' sums in order.
+// The tiles of which teams have parts: the parts' sums in order. A wave of its own for each row of matrix tiles.
 template <class S, int kMode>
-__global__ __launch_bounds__(S::kThreads) void ll_join_kernel(LlArgs p, LlOut o) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+__global__ __launch_bounds__(64) void ll_join_kernel(LlArgs p, LlOut o) {
+  const int lane = threadIdx.x;
   const int size = kMode == kModeDx ? p.tiles_m : p.tiles_n, ranges = kMode == kModeDx ? p.tiles_n : p.tiles_m;
-  const int range = blockIdx.x / size, member = blockIdx.x % size;
+  const int mt = blockIdx.x % S::kMT, wave = blockIdx.x / S::kMT % S::kWaves;
+  const int tile = blockIdx.x / (S::kMT * S::kWaves), range = tile / size, member = tile % size;
   const long long units = static_cast<long long>(ranges) * p.units, begin = static_cast<long long>(range) * p.units;
   int team = static_cast<int>(begin * p.teams / units);  // the one with the range's first unit
   while (team > 0 && team_start(p, units, team) > begin) --team;
   while (team_start(p, units, team + 1) <= begin) ++team;
   if (team_start(p, units, team + 1) >= begin + p.units) return;  // a whole one
-  lf32x16 acc[S::kMT][S::kNT];
+  lf32x16 acc[1][S::kNT];
 #pragma unroll
-  for (int a = 0; a < S::kMT; ++a)
+  for (int b = 0; b < S::kNT; ++b)
 #pragma unroll
-    for (int b = 0; b < S::kNT; ++b)
+    for (int e = 0; e < 16; ++e) acc[0][b][e] = 0.f;
+  int end = static_cast<int>((begin + p.units) * p.teams / units);  // the first team behind the range
+  while (end > 0 && team_start(p, units, end - 1) >= begin + p.units) --end;
+  while (end < p.teams && team_start(p, units, end) < begin + p.units) ++end;
+#pragma unroll 4
+  for (; team < end; ++team) {  // (every team has at least a unit)
+    const f32x4* src = ll_part<S, kMode>(p, team, team_start(p, units, team) / p.units != range, member) +
+                       wave * (S::kSums / 4 * 64) + mt * (S::kNT * 4 * 64) + lane;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[a][b][e] = 0.f;
-  for (; team < p.teams && team_start(p, units, team) < begin + p.units; ++team) {
-    const long long from = team_start(p, units, team);
-    if (from == team_start(p, units, team + 1)) continue;
-    const f32x4* src = ll_part<S, kMode>(p, team, from / p.units != range, member) + wave * (S::kSums / 4 * 64) + lane;
-#pragma unroll
-    for (int e = 0; e < S::kSums / 4; ++e) {
+    for (int e = 0; e < 4 * S::kNT; ++e) {
       const f32x4 v = src[64 * e];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) acc[e / 4 / S::kNT][e / 4 % S::kNT][4 * (e % 4) + q] += v[q];
+      for (int q = 0; q < 4; ++q) acc[0][e / 4][4 * (e % 4) + q] += v[q];
     }
   }
-  ll_end<S, kMode>(o, acc, kMode == kModeDx ? member : range, kMode == kModeDx ? range : member, wave % S::kWM,
-                   wave / S::kWM, lane, nullptr);
+  const int tm = kMode == kModeDx ? member : range, tn = kMode == kModeDx ? range : member;
+  ll_end<kMode>(o, acc, tm * S::kM + (wave % S::kWM * S::kMT + mt) * 32, tn * S::kN + wave / S::kWM * 32 * S::kNT, 0, lane,
+                nullptr);
 }
 
 // ------------------------------------------------------------------------- operands
@@ -706,70 +729,71 @@ __global__ __launch_bounds__(256) void ll_pick_kernel(LinLossParams p, LossMatri
 }
 
 // ------------------------------------------------------------------------- a token's loss
-// 64 tokens a workgroup: the parts' sums merged, 16 waves side by side, then a wave a token over its list.
-constexpr int kFinishTokens = 64;
+// 16 tokens a workgroup: the parts' sums merged, 64 slices of them side by side, then a wave a token over its list.
+constexpr int kFinishTokens = 16, kFinishSlices = 64;
 
-__global__ __launch_bounds__(1024) void ll_finish_kernel(LinLossParams p) {
-  __shared__ float s_m[16][64], s_s[16][64], s_lse[64];
+// (m, s) with (m2, s2): the sums of 2^(. - m), 2^(. - m2).
+__device__ __forceinline__ void sums_merge(float& m, float& s, float m2, float s2) {
+  const float mx = fmaxf(m, m2);
+  if (mx == -INFINITY) {
+    s += s2;  // zero, or NaN
+    return;
+  }
+  s = s * fast_exp2(m - mx) + s2 * fast_exp2(m2 - mx);
+  m = mx;
+}
+
+__global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_finish_kernel(LinLossParams p) {
+  __shared__ float s_m[kFinishSlices][kFinishTokens], s_s[kFinishSlices][kFinishTokens], s_lse[kFinishTokens];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int t0 = blockIdx.x * kFinishTokens;
+  const int mine = threadIdx.x % kFinishTokens, slice = threadIdx.x / kFinishTokens;
   {
-    const int t = t0 + lane;
     float m = -INFINITY, s = 0.f;
-    if (t < p.tokens)
-      for (int i = w; i < p.parts; i += 16) {
-        const float2 q = p.part[static_cast<long long>(i) * p.tokens + t];
-        const float mx = fmaxf(m, q.x);
-        if (mx == -INFINITY) {
-          s += q.y;  // zero, or NaN
-          continue;
-        }
-        s = s * fast_exp2(m - mx) + q.y * fast_exp2(q.x - mx);
-        m = mx;
+    if (t0 + mine < p.tokens) {
+#pragma unroll 4
+      for (int i = slice; i < p.parts; i += kFinishSlices) {
+        const float2 q = p.part[static_cast<long long>(i) * p.tokens + t0 + mine];
+        sums_merge(m, s, q.x, q.y);
       }
-    s_m[w][lane] = m;
-    s_s[w][lane] = s;
+    }
+    s_m[slice][mine] = m;
+    s_s[slice][mine] = s;
+  }
+  for (int h = kFinishSlices / 2; h > 0; h /= 2) {
+    __syncthreads();
+    if (slice < h) {
+      float m = s_m[slice][mine], s = s_s[slice][mine];
+      sums_merge(m, s, s_m[slice + h][mine], s_s[slice + h][mine]);
+      s_m[slice][mine] = m;
+      s_s[slice][mine] = s;
+    }
   }
   __syncthreads();
-  if (w == 0) {
-    float m = s_m[0][lane], s = s_s[0][lane];
-    for (int i = 1; i < 16; ++i) {
-      const float mx = fmaxf(m, s_m[i][lane]);
-      if (mx == -INFINITY) {
-        s += s_s[i][lane];
-        continue;
-      }
-      s = s * fast_exp2(m - mx) + s_s[i][lane] * fast_exp2(s_m[i][lane] - mx);
-      m = mx;
-    }
-    const int t = t0 + lane;
-    float lse = m + fast_log2(s);
-    if (t < p.tokens) {
-      const float live = p.r.live[t];
+  if (threadIdx.x < kFinishTokens) {
+    float lse = s_m[0][mine] + fast_log2(s_s[0][mine]);
+    if (t0 + mine < p.tokens) {
+      const float live = p.r.live[t0 + mine];
       lse += live - live;  // NaN for a row that has a word outside the vocabulary
-      p.lse[t] = lse;
+      p.lse[t0 + mine] = lse;
     }
-    s_lse[lane] = lse;
+    s_lse[mine] = lse;
   }
   __syncthreads();
-  for (int i = w; i < 64; i += 16) {
-    const long long t = t0 + i;
-    float sum = 0.f;
-    if (t < p.tokens) {
-      const float lse = s_lse[i];
-      for (int k = lane; k < p.r.top; k += 64) {
-        const long long at = t * p.r.top + k;
-        if (p.r.words[at] < 0) continue;
-        const float q = p.r.q[at];
-        sum = __builtin_fmaf(q, (lse - p.picked[at] * p.c) + fast_log2(q), sum);
-      }
-      sum = wave_sum(sum) * (kLn2 * p.temperature * p.temperature);
-      const float live = p.r.live[t];
-      if (live == 0.f) sum = 0.f;
-      sum += live - live;
-      if (lane == 0) p.loss[t] = sum;
-    }
+  const long long t = t0 + w;
+  if (t >= p.tokens) return;
+  const float lse = s_lse[w];
+  float sum = 0.f;
+  for (int k = lane; k < p.r.top; k += 64) {
+    const long long at = t * p.r.top + k;
+    if (p.r.words[at] < 0) continue;
+    const float q = p.r.q[at];
+    sum = __builtin_fmaf(q, (lse - p.picked[at] * p.c) + fast_log2(q), sum);
   }
+  sum = wave_sum(sum) * (kLn2 * p.temperature * p.temperature);
+  const float live = p.r.live[t];
+  if (live == 0.f) sum = 0.f;
+  if (lane == 0) p.loss[t] = sum + (live - live);
 }
 
 // ------------------------------------------------------------------------- backward, around the products
@@ -824,12 +848,14 @@ typedef LlShape<2, 2, 2, 2, 2> LlSmall;    // 128 x 128, waves of 64 x 64
 typedef LlShape<4, 1, 1, 1, 4> LlThinN;    // 128 x 32, waves of 32 x 32
 typedef LlShape<1, 4, 1, 1, 4> LlThinM;    // 32 x 128
 
-// Teams of `size` workgroups for `ranges` ranges: as many as there is room for, but at least two units each.
+// Teams of `size` workgroups for `ranges` ranges: as many as there is room for, but of at least kLeast units each,
+// about what a part costs to write and to read again.
 template <class S>
 int ll_teams(int size, int ranges, int units) {
   const long long all = static_cast<long long>(ranges) * units;
   long long n = kCUs * S::kPerCU / size;
-  n = n < all / 2 ? n : all / 2;
+  constexpr int kLeast = 8;
+  n = n < all / kLeast ? n : all / kLeast;
   return static_cast<int>(n < 1 ? 1 : n);
 }
 
@@ -846,7 +872,8 @@ void launch_product(LlArgs a, const LlOut& o, hipStream_t stream) {
     a.teams = ll_teams<S>(size, kMode == kModeDx ? a.tiles_n : a.tiles_m, a.units);
     hipLaunchKernelGGL((ll_kernel<S, kMode>), dim3(a.teams * size), dim3(S::kThreads), 0, stream, a, o);
     if (tiles / size * a.units % a.teams != 0 || tiles / size * a.units / a.teams % a.units != 0)
-      hipLaunchKernelGGL((ll_join_kernel<S, kMode>), dim3(static_cast<unsigned>(tiles)), dim3(S::kThreads), 0, stream, a, o);
+      hipLaunchKernelGGL((ll_join_kernel<S, kMode>), dim3(static_cast<unsigned>(tiles * S::kWaves * S::kMT)), dim3(64), 0,
+                         stream, a, o);
   } else {
     hipLaunchKernelGGL((ll_kernel<S, kMode>), dim3(static_cast<unsigned>(tiles < room ? tiles : room)), dim3(S::kThreads), 0,
                        stream, a, o);
@@ -863,15 +890,16 @@ auto with_shape(int shape, int mode, F&& f) {
 }
 
 template <int kMode>
-void launch_shaped(int shape, const LlArgs& a, const LlOut& o, hipStream_t stream) {
+void launch_shaped(const LinLossPlan& plan, const LlArgs& a, const LlOut& o, hipStream_t stream) {
   if constexpr (kLlGrad<kMode>) {
-    if (shape == 0) launch_product<LlSmall, kMode>(a, o, stream);
-    else if (shape == 1) launch_product<LlLargeN, kMode>(a, o, stream);
+    if (plan.shape == 0) launch_product<LlSmall, kMode>(a, o, stream);
+    else if (plan.shape == 1) launch_product<LlLargeN, kMode>(a, o, stream);
     else launch_product<LlThinM, kMode>(a, o, stream);
   } else if constexpr (kMode == kModeDw) {
-    if (shape == 1) launch_product<LlLargeM, kMode>(a, o, stream);
+    if (plan.shape_w == 1) launch_product<LlLargeM, kMode>(a, o, stream);
     else launch_product<LlSmall, kMode>(a, o, stream);
   } else {
+    const int shape = kMode == kModeDx ? plan.shape_x : plan.shape;
     if (shape == 0) launch_product<LlSmall, kMode>(a, o, stream);
     else if (shape == 1) launch_product<LlLargeM, kMode>(a, o, stream);
     else launch_product<LlThinN, kMode>(a, o, stream);
@@ -911,9 +939,18 @@ static long long tiles_of(long long rows, long long cols, int tm, int tn) {
   return ((rows + tm - 1) / tm) * ((cols + tn - 1) / tn);
 }
 
+// Which tiles: a CU does the work of four small ones (128 x 128) in the time of one large one, of two in 0.7 of it,
+// since it reads each operand half as often and has twice the products for each of its waits.
 LinLossPlan linloss_plan(int tokens, int features, int vocab, int planes) {
   LinLossPlan q{};
-  q.shape = tokens <= 32 ? 2 : tiles_of(vocab, tokens, 256, 256) >= 256 ? 1 : 0;
+  const auto rounds = [](long long n, long long at_once) { return static_cast<double>((n + at_once - 1) / at_once); };
+  if (tokens <= 32) {
+    q.shape = 2;
+  } else {
+    const double large = 4 * rounds(tiles_of(vocab, tokens, 256, 256), kCUs);
+    const double small = 2.8 * rounds(tiles_of(vocab, tokens, 128, 128), 2 * kCUs);
+    q.shape = large <= small ? 1 : 0;
+  }
   const int tv = q.shape == 1 ? 256 : 128;
   q.parts = static_cast<int>((vocab + tv - 1) / tv) * (q.shape == 2 ? 4 : 2);
   // Pieces of at most 1 GiB.
@@ -923,11 +960,15 @@ LinLossPlan linloss_plan(int tokens, int features, int vocab, int planes) {
   q.piece = static_cast<int>(((whole / 256 + pieces - 1) / pieces) * 256);
   q.ldg = q.piece;
   q.ldx = (tokens + 3) / 4 * 4;
+  const int words = q.piece < vocab ? q.piece : vocab;
+  // The gradients' products are shared evenly, so that it is their padding that counts.
+  const auto large = [](int rows, int cols) { return 4. * tiles_of(rows, cols, 256, 256) <= 1.4 * tiles_of(rows, cols, 128, 128); };
+  q.shape_x = tokens <= 32 ? 2 : large(features, tokens) ? 1 : 0;
+  q.shape_w = large(words, features) ? 1 : 0;
   const int x_stages = q.piece / 64 * (planes == 1 ? 1 : 6);
   const int w_stages = (tokens + kLlK - 1) / kLlK * (kLlK / 64) * (planes == 1 ? 1 : 6);
-  const int words = q.piece < vocab ? q.piece : vocab;
-  const long long x = with_shape(q.shape, kModeDx, [&](auto s) { return part_sums<decltype(s)>(features, tokens, x_stages); });
-  const long long w = with_shape(q.shape, kModeDw, [&](auto s) { return part_sums<decltype(s)>(features, words, w_stages); });
+  const long long x = with_shape(q.shape_x, kModeDx, [&](auto s) { return part_sums<decltype(s)>(features, tokens, x_stages); });
+  const long long w = with_shape(q.shape_w, kModeDw, [&](auto s) { return part_sums<decltype(s)>(features, words, w_stages); });
   q.partial = x > w ? x : w;
   return q;
 }
@@ -954,13 +995,13 @@ hipError_t launch_linloss_fwd(const LinLossParams& p, const LinLossPlan& plan, h
   o.cols = p.tokens;
   o.c = p.c;
   o.part = p.part;
-  launch_shaped<kModeLse>(plan.shape, a, o, stream);
+  launch_shaped<kModeLse>(plan, a, o, stream);
   const long long picks = static_cast<long long>(p.tokens) * ((p.r.top + 3) / 4);
   const dim3 pg(static_cast<unsigned>((picks + 3) / 4));
   if (f32) hipLaunchKernelGGL(ll_pick_kernel<3>, pg, dim3(256), 0, stream, p, a.a);
   else hipLaunchKernelGGL(ll_pick_kernel<1>, pg, dim3(256), 0, stream, p, a.a);
   const int blocks = (p.tokens + kFinishTokens - 1) / kFinishTokens;
-  hipLaunchKernelGGL(ll_finish_kernel, dim3(blocks), dim3(1024), 0, stream, p);
+  hipLaunchKernelGGL(ll_finish_kernel, dim3(blocks), dim3(kFinishTokens * kFinishSlices), 0, stream, p);
   if (p.reduction != kLossNone) return launch_loss_mean(p.loss, p.r, p.reduction, p.mean, stream);
   return hipGetLastError();
 }
@@ -995,8 +1036,8 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
     o.g = p.g;
     o.ld = p.ldg;
     o.plane = g.plane;
-    if (f32) launch_shaped<kModeGrad3>(plan.shape, a, o, stream);
-    else launch_shaped<kModeGrad>(plan.shape, a, o, stream);
+    if (f32) launch_shaped<kModeGrad3>(plan, a, o, stream);
+    else launch_shaped<kModeGrad>(plan, a, o, stream);
     const dim3 wg(static_cast<unsigned>((static_cast<long long>(p.tokens) * p.r.top + 255) / 256));
     if (f32) hipLaunchKernelGGL(ll_wanted_kernel<3>, wg, dim3(256), 0, stream, p, static_cast<int>(v0), words);
     else hipLaunchKernelGGL(ll_wanted_kernel<1>, wg, dim3(256), 0, stream, p, static_cast<int>(v0), words);
@@ -1010,7 +1051,7 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
       o.f = p.dx_sum;
       o.ld = p.ldx;
       o.add = v0 > 0;
-      launch_shaped<kModeDx>(plan.shape, a, o, stream);
+      launch_shaped<kModeDx>(plan, a, o, stream);
     }
     if (p.dw != nullptr) {
       a.a = g;
@@ -1024,7 +1065,7 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
       void* dst = static_cast<char*>(p.dw) + v0 * p.features * (p.dw_bf16 ? 2 : 4);
       if (p.dw_bf16) o.h = static_cast<bf16_t*>(dst);
       else o.f = static_cast<float*>(dst);
-      launch_shaped<kModeDw>(plan.shape, a, o, stream);
+      launch_shaped<kModeDw>(plan, a, o, stream);
     }
   }
   if (p.dx != nullptr) {

@@ -81,7 +81,7 @@ struct LinLossParams {
 
 // What the call needs besides its operands; sizes depend on nothing but the arguments.
 struct LinLossPlan {
-  int shape;          // of the tiles
+  int shape, shape_x, shape_w;  // of the tiles: 0 small, 1 large, 2 thin
   int parts, piece;
   long long ldg, ldx, partial;
 };
