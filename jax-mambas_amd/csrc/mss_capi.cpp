@@ -1651,7 +1651,7 @@ mss::LossRows loss_rows(int rows, int top, int vocab, float temperature, bool li
   r.top = top;
   r.vocab = vocab;
   r.c = mss::kLog2e / temperature;
-  r.blocks = mss::loss_row_blocks(rows, lists);
+  r.blocks = lists ? mss::loss_list_blocks(rows) : mss::loss_target_blocks(rows);
   r.words = saved->take<int>(static_cast<long long>(rows) * top);
   r.q = saved->take<float>(static_cast<long long>(rows) * top);
   r.live = saved->take<float>(rows);
@@ -1692,7 +1692,7 @@ int linear_loss_sizes(const mss_linear_loss_args* a, mss::LinLossParams* p, mss:
   p->r = loss_rows(a->tokens, top, a->vocab, a->temperature, lists, &c);
   p->c = p->r.c;
   p->picked = c.take<float>(static_cast<long long>(a->tokens) * top);
-  p->lse = c.take<float>(a->tokens);
+  p->stat = c.take<float2>(a->tokens + mss::kLinLossTile);
   p->xp = c.take<mss::bf16_t>(static_cast<long long>(p->planes) * a->tokens * p->width);
   if (p->pack_w) p->wp = c.take<mss::bf16_t>(static_cast<long long>(p->planes) * a->vocab * p->width);
   *saved = c.at;
@@ -1700,9 +1700,9 @@ int linear_loss_sizes(const mss_linear_loss_args* a, mss::LinLossParams* p, mss:
   p->part = f.take<float2>(static_cast<long long>(p->parts) * a->tokens);
   *fwd = f.at;
   Carve b{static_cast<char*>(a->workspace), 0};
-  p->scale = b.take<float2>(a->tokens + mss::kLinLossTile);
+  if (a->reduction == MSS_LOSS_NONE) p->scale = b.take<float2>(a->tokens + mss::kLinLossTile);
   p->g = b.take<mss::bf16_t>(static_cast<long long>(p->planes) * a->tokens * p->ldg);
-  p->dx_sum = b.take<float>(p->features * p->ldx);
+  if (p->piece < a->vocab) p->dx_sum = b.take<float>(p->features * p->ldx);
   p->partial = b.take<float>(plan->partial);
   *bwd = b.at;
   return MSS_OK;

@@ -26,29 +26,7 @@ __device__ __forceinline__ float wave_sum_f(float v) {
 }
 
 // ------------------------------------------------------------------------- the rows' wanted words
-constexpr int kTargetRows = 256, kListRows = 4;  // rows a workgroup
-
-__global__ __launch_bounds__(kTargetRows) void loss_targets_kernel(LossRows r) {
-  __shared__ int s_n[kTargetRows / 64];
-  const long long t = static_cast<long long>(blockIdx.x) * kTargetRows + threadIdx.x;
-  bool counts = false;
-  if (t < r.rows) {
-    const long long v = r.targets[t];
-    counts = v != r.ignore;
-    const bool inside = v >= 0 && v < r.vocab;
-    r.words[t] = counts && inside ? static_cast<int>(v) : -1;
-    r.q[t] = 1.f;
-    r.live[t] = !counts ? 0.f : inside ? 1.f : __builtin_nanf("");
-  }
-  const int n = __popcll(__ballot(counts));
-  if ((threadIdx.x & 63) == 0) s_n[threadIdx.x >> 6] = n;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    int all = 0;
-    for (int i = 0; i < kTargetRows / 64; ++i) all += s_n[i];
-    r.counts[blockIdx.x] = all;
-  }
-}
+constexpr int kListRows = 4;  // rows a workgroup
 
 // A wave a row, kPer entries a lane (entry 64 i + lane). An entry counts where its id is not negative and its
 // logit not -inf; what an entry that does not count holds is not looked at. A word that stands in a list
@@ -413,12 +391,11 @@ void launch_typed(const DistillParams& p, hipStream_t stream) {
 
 }  // namespace
 
-int loss_row_blocks(int rows, bool lists) { return lists ? (rows + kListRows - 1) / kListRows : (rows + kTargetRows - 1) / kTargetRows; }
+int loss_list_blocks(int rows) { return (rows + kListRows - 1) / kListRows; }
 
 hipError_t launch_loss_rows(const LossRows& r, hipStream_t stream) {
   const dim3 grid(r.blocks);
-  if (r.targets != nullptr) hipLaunchKernelGGL(loss_targets_kernel, grid, dim3(kTargetRows), 0, stream, r);
-  else if (r.top <= 64) hipLaunchKernelGGL(loss_lists_kernel<1>, grid, dim3(64 * kListRows), 0, stream, r);
+  if (r.top <= 64) hipLaunchKernelGGL(loss_lists_kernel<1>, grid, dim3(64 * kListRows), 0, stream, r);
   else if (r.top <= 128) hipLaunchKernelGGL(loss_lists_kernel<2>, grid, dim3(64 * kListRows), 0, stream, r);
   else if (r.top <= 256) hipLaunchKernelGGL(loss_lists_kernel<4>, grid, dim3(64 * kListRows), 0, stream, r);
   else hipLaunchKernelGGL(loss_lists_kernel<16>, grid, dim3(64 * kListRows), 0, stream, r);

@@ -130,6 +130,7 @@ struct LlArgs {
   int tiles_m, tiles_n;
   int units;             // of a tile: kRing stages each
   int teams;             // of the gradients' products
+  int whole;             // ranges of a team; 0: the teams share all units evenly
   float* partial;        // their tiles' parts
 };
 
@@ -157,7 +158,10 @@ struct LlOut {
   float* f;              // kModeDx, kModeDw with float32 output
   bf16_t* h;             // kModeDw with bf16 output
   int add;               // kModeDx: to what is there
-  LlScale by;            // kModeDw
+  LlScale by;            // kModeDx with the last piece, kModeDw
+  void* dx;              // kModeDx with the last piece: [rows][cols]
+  int dx_bf16;
+  const float* live;
 };
 
 // What a tile's sums become.
@@ -175,6 +179,12 @@ template <int kValue>
 struct LlInt {
   static constexpr int value = kValue;
 };
+
+// A value of another lane of the four (kCtrl: 0xb1 of lane ^ 1, 0x4e of lane ^ 2).
+template <int kCtrl>
+__device__ __forceinline__ float quad_mov(float v) {
+  return dpp_mov<kCtrl, 0xF>(0.f, v);
+}
 
 // A wave's kMT x kNT matrix tiles: from row wm0 and column wn0 on, in part `part` of the rows. table: the scales of
 // its rows (kModeGrad).
@@ -252,10 +262,22 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT],
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the next tile counts a whole tile's stores)
     }
   } else if constexpr (kMode == kModeDx) {
-    // Rows are features, columns tokens, kNT neighbours a lane.
+    // Rows are features, columns tokens, kNT neighbours a lane: to the sums over the pieces, or, with the last piece,
+    // to dx.
     const int t = wn0 + kNT * j;
+    if (t >= o.cols) return;  // (a row of sums is long enough for the last lane's kNT)
     const uint32_t at = static_cast<uint32_t>(4 * g * o.ld + t) * 4;
-    if (t >= o.cols) return;  // (the rows are long enough for the last lane's kNT)
+    const bool last = o.dx != nullptr;
+    const long long at_dx = 4LL * g * o.cols + t;
+    static_assert(kNT <= 2, "the last lane has one token or all");
+    const bool all = t + kNT <= o.cols;
+    bool counts[kNT];
+    float f = 1.f;
+    if (last) {
+      f = shared_scale(o.by);
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) counts[nt] = t + nt < o.cols && o.live[t + nt] != 0.f;
+    }
 #pragma unroll
     for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
@@ -270,28 +292,76 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT],
         for (int r = 0; r < 4; ++r) {
 #pragma unroll
           for (int nt = 0; nt < kNT; ++nt) v[r][nt] = o.add ? v[r][nt] + acc[mt][nt][4 * q + r] : acc[mt][nt][4 * q + r];
-          if (d + 4 * g + r < o.rows)
+          if (d + 4 * g + r >= o.rows) continue;
+          if (!last) {
             __builtin_memcpy(reinterpret_cast<char*>(o.f + (d + r) * o.ld) + at, v[r], sizeof(v[r]));
+            continue;
+          }
+#pragma unroll
+          for (int nt = 0; nt < kNT; ++nt) v[r][nt] = counts[nt] ? v[r][nt] * f : 0.f;
+          const long long to = static_cast<long long>(d + r) * o.cols + at_dx;
+          if (o.dx_bf16) {
+            uint32_t u[(kNT + 1) / 2];
+#pragma unroll
+            for (int h = 0; h < (kNT + 1) / 2; ++h) u[h] = pack_bf16x2(v[r][2 * h], v[r][2 * h + 1 < kNT ? 2 * h + 1 : 2 * h]);
+            bf16_t* dst = static_cast<bf16_t*>(o.dx) + to;
+            if (all) __builtin_memcpy(dst, u, 2 * kNT);
+            else dst[0].bits = static_cast<uint16_t>(u[0]);
+          } else {
+            float* dst = static_cast<float*>(o.dx) + to;
+            if (all) __builtin_memcpy(dst, v[r], sizeof(v[r]));
+            else dst[0] = v[r][0];
+          }
         }
         asm volatile("" ::: "memory");  // (a few rows at a time: all of what is there would not fit the registers)
       }
   } else {
-    // Rows are words, columns features.
+    // Rows are words, columns features. Four rows and four lanes change places, so that a lane has four neighbouring
+    // columns of one row: a store instruction then writes 8 rows of 64 bytes (or 128) instead of two, and it is
+    // their number that short sums wait for.
     const float by = shared_scale(o.by);
+    const bool odd = j & 1, high = j & 2;
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
-      const int d = wn0 + 32 * nt + j;
-      if (d >= o.cols) continue;
-      const uint32_t at = static_cast<uint32_t>(4 * g * o.ld + d);
+      const int d = wn0 + 32 * nt + (j & ~3);
+      const uint32_t at = static_cast<uint32_t>((4 * g + (j & 3)) * o.ld + d);
 #pragma unroll
       for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int v = wm0 + 32 * mt + 8 * (r >> 2) + (r & 3);  // and 4 g more
-          if (v + 4 * g >= o.rows) continue;
-          const float x = acc[mt][nt][r] * by;
-          if (o.h != nullptr) store_as(reinterpret_cast<bf16_t*>(reinterpret_cast<char*>(o.h + v * o.ld) + 2 * at), x);
-          else *reinterpret_cast<float*>(reinterpret_cast<char*>(o.f + v * o.ld) + 4 * at) = x;
+        for (int q = 0; q < 4; ++q) {
+          const int v = wm0 + 32 * mt + 8 * q;  // and 4 g + j % 4 more
+          float x[4], y[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[r] = acc[mt][nt][4 * q + r] * by;
+#pragma unroll
+          for (int h = 0; h < 4; h += 2) {  // rows h, h + 1 between neighbours
+            const float z = quad_mov<0xb1>(odd ? x[h] : x[h + 1]);
+            y[h] = odd ? z : x[h];
+            y[h + 1] = odd ? x[h + 1] : z;
+          }
+          const float z0 = quad_mov<0x4e>(high ? y[0] : y[2]), z1 = quad_mov<0x4e>(high ? y[1] : y[3]);
+          const float w[4] = {high ? z0 : y[0], high ? z1 : y[1], high ? y[2] : z0, high ? y[3] : z1};
+          if (v + 4 * g + (j & 3) >= o.rows) continue;
+          if (o.h != nullptr) {
+            char* dst = reinterpret_cast<char*>(o.h + v * o.ld) + 2 * at;
+            const uint32_t u[2] = {pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3])};
+            if (d + 4 <= o.cols) {
+              __builtin_memcpy(dst, u, 8);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 3; ++e)
+                if (d + e < o.cols) reinterpret_cast<uint16_t*>(dst)[e] = static_cast<uint16_t>(u[e / 2] >> (16 * (e & 1)));
+            }
+          } else {
+            char* dst = reinterpret_cast<char*>(o.f + v * o.ld) + 4 * at;
+            if (d + 4 <= o.cols) {
+              __builtin_memcpy(dst, w, 16);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 3; ++e)
+                if (d + e < o.cols) reinterpret_cast<float*>(dst)[e] = w[e];
+            }
+          }
         }
     }
   }
@@ -305,9 +375,9 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT],
 // XCD has workgroups.
 //
 // kModeDx, kModeDw: the tiles of one range of tokens (words) are taken by a team of as many workgroups as there
-// are tiles of features, side by side, so that g is read once. The teams share the units of all ranges
-// evenly, in order: a team's first and last range may be a part of one, whose sums go to `partial` and are
-// added in order by ll_join_kernel.
+// are tiles of features, side by side, so that g is read once. A team has a number of whole ranges, or the teams
+// share the units of all ranges evenly, in order: a team's first and last range may be a part of one then, whose
+// sums go to `partial` and are added in order by ll_join_kernel.
 struct LlSegment {
   int tm, tn, unit, n;  // the tile, its first unit, units: none at the end
 };
@@ -318,7 +388,11 @@ struct LlDeal {
   long long from, to;         // units
 };
 
-__device__ __forceinline__ long long team_start(const LlArgs& p, long long units, int team) { return units * team / p.teams; }
+__device__ __forceinline__ long long team_start(const LlArgs& p, long long units, int team) {
+  if (p.whole == 0) return units * team / p.teams;
+  const long long at = static_cast<long long>(team) * p.whole * p.units;
+  return at < units ? at : units;
+}
 
 template <int kMode>
 __device__ __forceinline__ LlDeal ll_deal(const LlArgs& p) {
@@ -623,13 +697,38 @@ __device__ __forceinline__ void split_planes(float v, bf16_t (&b)[kPlanes]) {
 // x (features, tokens) as token-major rows of `width` features, zeros past the last feature and in rows that
 // do not count (whatever a masked token holds then reaches nothing). Tiles of 64 x 64 through LDS, read
 // along whichever axis is contiguous.
+// With targets the first blocks note the rows' words too.
 template <typename in_t, int kPlanes>
 __global__ __launch_bounds__(256) void ll_pack_x_kernel(LinLossParams p) {
   __shared__ float s[64][65];
+  __shared__ bool s_live[64];
   const int t0 = blockIdx.x * 64, f0 = blockIdx.y * 64;
   const in_t* x = static_cast<const in_t*>(p.x);
   const bool along_f = p.sf == 1;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  if (w == 0) {
+    const int t = t0 + lane;
+    float live = 0.f;
+    if (t < p.tokens) {
+      if (p.r.targets != nullptr) {
+        const long long v = p.r.targets[t];
+        const bool inside = v >= 0 && v < p.r.vocab;
+        live = v == p.r.ignore ? 0.f : inside ? 1.f : __builtin_nanf("");
+        if (blockIdx.y == 0) {
+          p.r.words[t] = live == 1.f ? static_cast<int>(v) : -1;
+          p.r.q[t] = 1.f;
+          p.r.live[t] = live;
+        }
+      } else {
+        live = p.r.live[t];
+      }
+    }
+    s_live[lane] = live != 0.f;
+    if (p.r.targets != nullptr && blockIdx.y == 0) {
+      const int n = __popcll(__ballot(live != 0.f));
+      if (lane == 0) p.r.counts[blockIdx.x] = n;
+    }
+  }
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int a = along_f ? lane : w + 4 * i, b = along_f ? w + 4 * i : lane;  // feature, token
@@ -643,12 +742,11 @@ __global__ __launch_bounds__(256) void ll_pack_x_kernel(LinLossParams p) {
     const int slot = threadIdx.x + 256 * i, b = slot / 8, c = 8 * (slot % 8);
     const int t = t0 + b;
     if (t >= p.tokens) continue;
-    const bool live = p.r.live[t] != 0.f;
     alignas(16) bf16_t v[kPlanes][8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       bf16_t q[kPlanes];
-      split_planes<kPlanes>(live ? s[c + e][b] : 0.f, q);
+      split_planes<kPlanes>(s_live[b] ? s[c + e][b] : 0.f, q);
 #pragma unroll
       for (int pl = 0; pl < kPlanes; ++pl) v[pl][e] = q[pl];
     }
@@ -694,25 +792,19 @@ __device__ __forceinline__ void add_planes(const bf16_t* at, float (&v)[8]) {
   }
 }
 
-template <int kPlanes>
-__global__ __launch_bounds__(256) void ll_pick_kernel(LinLossParams p, LossMatrix w) {
-  const int lane = threadIdx.x & 63;
-  const int per = (p.r.top + 3) / 4;
-  const long long id = blockIdx.x * 4LL + (threadIdx.x >> 6);
-  const long long t = id / per;
-  if (t >= p.tokens) return;
-  const int k0 = 4 * static_cast<int>(id - t * per);
+// The logits of kN words of token t (a negative word: 0), in all lanes.
+template <int kPlanes, int kN>
+__device__ __forceinline__ void ll_dots(const LinLossParams& p, const LossMatrix& w, long long t, const int (&word)[kN],
+                                        int lane, float (&sum)[kN]) {
   const long long xplane = static_cast<long long>(p.tokens) * p.width;
-  int word[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) word[e] = k0 + e < p.r.top ? p.r.words[t * p.r.top + k0 + e] : -1;
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int e = 0; e < kN; ++e) sum[e] = 0.f;
   for (int c = 8 * lane; c < p.width; c += 512) {
     float x[8] = {};
 #pragma unroll
     for (int pl = 0; pl < kPlanes; ++pl) add_planes(p.xp + pl * xplane + t * p.width + c, x);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < kN; ++e) {
       if (word[e] < 0) continue;
       float v[8] = {};
 #pragma unroll
@@ -722,14 +814,30 @@ __global__ __launch_bounds__(256) void ll_pick_kernel(LinLossParams p, LossMatri
     }
   }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float v = wave_sum(sum[e]);
-    if (lane == 0 && k0 + e < p.r.top) p.picked[t * p.r.top + k0 + e] = v;
-  }
+  for (int e = 0; e < kN; ++e) sum[e] = wave_sum(sum[e]);
+}
+
+template <int kPlanes>
+__global__ __launch_bounds__(256) void ll_pick_kernel(LinLossParams p, LossMatrix w) {
+  const int lane = threadIdx.x & 63;
+  const int per = (p.r.top + 3) / 4;
+  const long long id = blockIdx.x * 4LL + (threadIdx.x >> 6);
+  const long long t = id / per;
+  if (t >= p.tokens) return;
+  const int k0 = 4 * static_cast<int>(id - t * per);
+  int word[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) word[e] = k0 + e < p.r.top ? p.r.words[t * p.r.top + k0 + e] : -1;
+  float sum[4];
+  ll_dots<kPlanes>(p, w, t, word, lane, sum);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (lane == 0 && k0 + e < p.r.top) p.picked[t * p.r.top + k0 + e] = sum[e];
 }
 
 // ------------------------------------------------------------------------- a token's loss
 // 16 tokens a workgroup: the parts' sums merged, 64 slices of them side by side, then a wave a token over its list.
+// kPlanes: of the operands, where there is one word a token whose logit is formed here; 0: the logits are there.
 constexpr int kFinishTokens = 16, kFinishSlices = 64;
 
 // (m, s) with (m2, s2): the sums of 2^(. - m), 2^(. - m2).
@@ -743,11 +851,21 @@ __device__ __forceinline__ void sums_merge(float& m, float& s, float m2, float s
   m = mx;
 }
 
-__global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_finish_kernel(LinLossParams p) {
+template <int kPlanes>
+__global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_finish_kernel(LinLossParams p, LossMatrix wm) {
   __shared__ float s_m[kFinishSlices][kFinishTokens], s_s[kFinishSlices][kFinishTokens], s_lse[kFinishTokens];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int t0 = blockIdx.x * kFinishTokens;
   const int mine = threadIdx.x % kFinishTokens, slice = threadIdx.x / kFinishTokens;
+  const long long t = t0 + w;
+  float logit[1] = {0.f};
+  if constexpr (kPlanes > 0) {
+    if (t < p.tokens) {
+      const int word[1] = {p.r.words[t]};
+      ll_dots<kPlanes>(p, wm, t, word, lane, logit);
+      if (lane == 0) p.picked[t] = logit[0];
+    }
+  }
   {
     float m = -INFINITY, s = 0.f;
     if (t0 + mine < p.tokens) {
@@ -775,12 +893,11 @@ __global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_finish_kerne
     if (t0 + mine < p.tokens) {
       const float live = p.r.live[t0 + mine];
       lse += live - live;  // NaN for a row that has a word outside the vocabulary
-      p.lse[t0 + mine] = lse;
+      p.stat[t0 + mine] = make_float2(lse, live == 0.f ? 0.f : 1.f);
     }
     s_lse[mine] = lse;
   }
   __syncthreads();
-  const long long t = t0 + w;
   if (t >= p.tokens) return;
   const float lse = s_lse[w];
   float sum = 0.f;
@@ -788,7 +905,8 @@ __global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_finish_kerne
     const long long at = t * p.r.top + k;
     if (p.r.words[at] < 0) continue;
     const float q = p.r.q[at];
-    sum = __builtin_fmaf(q, (lse - p.picked[at] * p.c) + fast_log2(q), sum);
+    const float z = kPlanes > 0 ? logit[0] : p.picked[at];
+    sum = __builtin_fmaf(q, (lse - z * p.c) + fast_log2(q), sum);
   }
   sum = wave_sum(sum) * (kLn2 * p.temperature * p.temperature);
   const float live = p.r.live[t];
@@ -797,43 +915,29 @@ __global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_finish_kerne
 }
 
 // ------------------------------------------------------------------------- backward, around the products
-// A token's lse, and what its g is scaled by before it is rounded: without a reduction its own upstream
-// gradient; else nothing, since what all tokens share is left to the products' ends (1 / tokens has
-// an error of its own in bf16, the same for every token).
-__global__ __launch_bounds__(256) void ll_scale_kernel(LinLossParams p) {
+// A token's lse, and what its g is scaled by before it is rounded: without a reduction its own upstream gradient. (With
+// one, nothing: what all tokens share is left to the products' ends, since 1 / tokens has an error of its own in
+// bf16, the same for every token.)
+__global__ __launch_bounds__(256) void ll_scale_kernel(LinLossParams p, float2* scale) {
   const int t = blockIdx.x * 256 + threadIdx.x;
   if (t >= p.tokens) return;
-  float f = p.reduction == kLossNone ? p.grad[t] * p.temperature : 1.f;
-  if (p.r.live[t] == 0.f) f = 0.f;
-  p.scale[t] = make_float2(p.lse[t], f);
+  const float2 s = p.stat[t];
+  scale[t] = make_float2(s.x, s.y == 0.f ? 0.f : p.grad[t] * p.temperature);
 }
 
 // g at the wanted words of the piece that begins at word v0, from their own logits.
 template <int kPlanes>
-__global__ __launch_bounds__(256) void ll_wanted_kernel(LinLossParams p, int v0, int words) {
+__global__ __launch_bounds__(256) void ll_wanted_kernel(LinLossParams p, const float2* scale, int v0, int words) {
   const long long i = blockIdx.x * 256LL + threadIdx.x;
   if (i >= static_cast<long long>(p.tokens) * p.r.top) return;
   const int v = p.r.words[i] - v0;
   if (p.r.words[i] < 0 || v < 0 || v >= words) return;
   const long long t = i / p.r.top;
-  const float2 sc = p.scale[t];
+  const float2 sc = scale[t];
   bf16_t b[kPlanes];
   split_planes<kPlanes>((fast_exp2(__builtin_fmaf(p.picked[i], p.c, -sc.x)) - p.r.q[i]) * sc.y, b);
 #pragma unroll
   for (int pl = 0; pl < kPlanes; ++pl) p.g[pl * (p.tokens * p.ldg) + t * p.ldg + v] = b[pl];
-}
-
-// dx from its sums over the pieces.
-template <typename out_t>
-__global__ __launch_bounds__(256) void ll_dx_kernel(LinLossParams p, LlScale scale) {
-  const float by = shared_scale(scale);
-  const long long n = static_cast<long long>(p.features) * p.tokens;
-  out_t* out = static_cast<out_t*>(p.dx);
-  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n; i += gridDim.x * 256LL) {
-    const long long d = i / p.tokens, t = i - d * p.tokens;
-    const float v = p.dx_sum[d * p.ldx + t];
-    store_as(out + i, p.r.live[t] == 0.f ? 0.f : v * by);
-  }
 }
 
 unsigned blocks_for(long long n, long long most) {
@@ -848,15 +952,24 @@ typedef LlShape<2, 2, 2, 2, 2> LlSmall;    // 128 x 128, waves of 64 x 64
 typedef LlShape<4, 1, 1, 1, 4> LlThinN;    // 128 x 32, waves of 32 x 32
 typedef LlShape<1, 4, 1, 1, 4> LlThinM;    // 32 x 128
 
-// Teams of `size` workgroups for `ranges` ranges: as many as there is room for, but of at least kLeast units each,
-// about what a part costs to write and to read again.
+// Teams of `size` workgroups for `ranges` ranges of `units`. Whole ranges where the last team is not waited for
+// longer than a part costs to write and to read again (kPart units); else even shares, of at least that much.
+struct LlTeams {
+  int teams, whole;
+};
+
 template <class S>
-int ll_teams(int size, int ranges, int units) {
+LlTeams ll_teams(int size, int ranges, int units) {
+  constexpr int kPart = 8;
   const long long all = static_cast<long long>(ranges) * units;
   long long n = kCUs * S::kPerCU / size;
-  constexpr int kLeast = 8;
-  n = n < all / kLeast ? n : all / kLeast;
-  return static_cast<int>(n < 1 ? 1 : n);
+  n = n < 1 ? 1 : n;
+  const long long each = (ranges + n - 1) / n;
+  long long shares = all / kPart < n ? all / kPart : n;
+  shares = shares < 1 ? 1 : shares;
+  if (each * units <= all / shares + kPart)
+    return {static_cast<int>((ranges + each - 1) / each), static_cast<int>(each)};
+  return {static_cast<int>(shares), 0};
 }
 
 template <class S, int kMode>
@@ -869,9 +982,11 @@ void launch_product(LlArgs a, const LlOut& o, hipStream_t stream) {
   const long long tiles = static_cast<long long>(a.tiles_m) * a.tiles_n;
   if constexpr (kLlTeams<kMode>) {
     const int size = kMode == kModeDx ? a.tiles_m : a.tiles_n;
-    a.teams = ll_teams<S>(size, kMode == kModeDx ? a.tiles_n : a.tiles_m, a.units);
+    const LlTeams t = ll_teams<S>(size, kMode == kModeDx ? a.tiles_n : a.tiles_m, a.units);
+    a.teams = t.teams;
+    a.whole = t.whole;
     hipLaunchKernelGGL((ll_kernel<S, kMode>), dim3(a.teams * size), dim3(S::kThreads), 0, stream, a, o);
-    if (tiles / size * a.units % a.teams != 0 || tiles / size * a.units / a.teams % a.units != 0)
+    if (a.whole == 0)
       hipLaunchKernelGGL((ll_join_kernel<S, kMode>), dim3(static_cast<unsigned>(tiles * S::kWaves * S::kMT)), dim3(64), 0,
                          stream, a, o);
   } else {
@@ -914,9 +1029,10 @@ long long part_sums(int features, int others, int stages) {
   const long long size_x = (features + tile_f - 1) / tile_f, ranges_x = (others + tile_o - 1) / tile_o;
   const long long size_w = (features + tile_o - 1) / tile_o, ranges_w = (others + tile_f - 1) / tile_f;
   const int units = (stages + S::kRing - 1) / S::kRing;
-  const long long x = 2LL * ll_teams<S>(static_cast<int>(size_x), static_cast<int>(ranges_x), units) * size_x;
-  const long long w = 2LL * ll_teams<S>(static_cast<int>(size_w), static_cast<int>(ranges_w), units) * size_w;
-  return (x > w ? x : w) * S::kM * S::kN;
+  const LlTeams x = ll_teams<S>(static_cast<int>(size_x), static_cast<int>(ranges_x), units);
+  const LlTeams w = ll_teams<S>(static_cast<int>(size_w), static_cast<int>(ranges_w), units);
+  const long long nx = x.whole ? 0 : 2LL * x.teams * size_x, nw = w.whole ? 0 : 2LL * w.teams * size_w;
+  return (nx > nw ? nx : nw) * S::kM * S::kN;
 }
 
 LossMatrix weight_planes(const LinLossParams& p) {
@@ -934,6 +1050,8 @@ LossMatrix x_planes(const LinLossParams& p) {
 }
 
 }  // namespace
+
+int loss_target_blocks(int tokens) { return (tokens + 63) / 64; }
 
 static long long tiles_of(long long rows, long long cols, int tm, int tn) {
   return ((rows + tm - 1) / tm) * ((cols + tn - 1) / tn);
@@ -974,8 +1092,11 @@ LinLossPlan linloss_plan(int tokens, int features, int vocab, int planes) {
 }
 
 hipError_t launch_linloss_fwd(const LinLossParams& p, const LinLossPlan& plan, hipStream_t stream) {
-  const hipError_t e = launch_loss_rows(p.r, stream);
-  if (e != hipSuccess) return e;
+  const bool lists = p.r.targets == nullptr;
+  if (lists) {
+    const hipError_t e = launch_loss_rows(p.r, stream);
+    if (e != hipSuccess) return e;
+  }
   const bool f32 = p.planes == 3;
   const dim3 xg((p.tokens + 63) / 64, p.width / 64);
   if (f32) hipLaunchKernelGGL((ll_pack_x_kernel<float, 3>), xg, dim3(256), 0, stream, p);
@@ -996,19 +1117,29 @@ hipError_t launch_linloss_fwd(const LinLossParams& p, const LinLossPlan& plan, h
   o.c = p.c;
   o.part = p.part;
   launch_shaped<kModeLse>(plan, a, o, stream);
-  const long long picks = static_cast<long long>(p.tokens) * ((p.r.top + 3) / 4);
-  const dim3 pg(static_cast<unsigned>((picks + 3) / 4));
-  if (f32) hipLaunchKernelGGL(ll_pick_kernel<3>, pg, dim3(256), 0, stream, p, a.a);
-  else hipLaunchKernelGGL(ll_pick_kernel<1>, pg, dim3(256), 0, stream, p, a.a);
-  const int blocks = (p.tokens + kFinishTokens - 1) / kFinishTokens;
-  hipLaunchKernelGGL(ll_finish_kernel, dim3(blocks), dim3(kFinishTokens * kFinishSlices), 0, stream, p);
+  const dim3 fg((p.tokens + kFinishTokens - 1) / kFinishTokens), fb(kFinishTokens * kFinishSlices);
+  if (lists) {
+    const long long picks = static_cast<long long>(p.tokens) * ((p.r.top + 3) / 4);
+    const dim3 pg(static_cast<unsigned>((picks + 3) / 4));
+    if (f32) hipLaunchKernelGGL(ll_pick_kernel<3>, pg, dim3(256), 0, stream, p, a.a);
+    else hipLaunchKernelGGL(ll_pick_kernel<1>, pg, dim3(256), 0, stream, p, a.a);
+    hipLaunchKernelGGL(ll_finish_kernel<0>, fg, fb, 0, stream, p, a.a);
+  } else if (f32) {
+    hipLaunchKernelGGL(ll_finish_kernel<3>, fg, fb, 0, stream, p, a.a);
+  } else {
+    hipLaunchKernelGGL(ll_finish_kernel<1>, fg, fb, 0, stream, p, a.a);
+  }
   if (p.reduction != kLossNone) return launch_loss_mean(p.loss, p.r, p.reduction, p.mean, stream);
   return hipGetLastError();
 }
 
 hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, hipStream_t stream) {
   const bool f32 = p.planes == 3;
-  hipLaunchKernelGGL(ll_scale_kernel, dim3((p.tokens + 255) / 256), dim3(256), 0, stream, p);
+  const float2* scale = p.stat;
+  if (p.reduction == kLossNone) {
+    scale = p.scale;
+    hipLaunchKernelGGL(ll_scale_kernel, dim3((p.tokens + 255) / 256), dim3(256), 0, stream, p, p.scale);
+  }
   const LossMatrix w = weight_planes(p), x = x_planes(p);
   const LlScale by{p.reduction == kLossNone ? nullptr : p.grad, p.reduction == kLossMean ? p.mean : nullptr, p.temperature};
   for (long long v0 = 0; v0 < p.vocab; v0 += p.piece) {
@@ -1032,15 +1163,15 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
     o.rows = p.tokens;
     o.cols = words;
     o.c = p.c;
-    o.scale = p.scale;
+    o.scale = scale;
     o.g = p.g;
     o.ld = p.ldg;
     o.plane = g.plane;
     if (f32) launch_shaped<kModeGrad3>(plan, a, o, stream);
     else launch_shaped<kModeGrad>(plan, a, o, stream);
     const dim3 wg(static_cast<unsigned>((static_cast<long long>(p.tokens) * p.r.top + 255) / 256));
-    if (f32) hipLaunchKernelGGL(ll_wanted_kernel<3>, wg, dim3(256), 0, stream, p, static_cast<int>(v0), words);
-    else hipLaunchKernelGGL(ll_wanted_kernel<1>, wg, dim3(256), 0, stream, p, static_cast<int>(v0), words);
+    if (f32) hipLaunchKernelGGL(ll_wanted_kernel<3>, wg, dim3(256), 0, stream, p, scale, static_cast<int>(v0), words);
+    else hipLaunchKernelGGL(ll_wanted_kernel<1>, wg, dim3(256), 0, stream, p, scale, static_cast<int>(v0), words);
     if (p.dx != nullptr) {
       a.a = wp;
       a.b = g;
@@ -1051,6 +1182,12 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
       o.f = p.dx_sum;
       o.ld = p.ldx;
       o.add = v0 > 0;
+      if (v0 + words == p.vocab) {
+        o.dx = p.dx;
+        o.dx_bf16 = !f32;
+        o.by = by;
+        o.live = p.r.live;
+      }
       launch_shaped<kModeDx>(plan, a, o, stream);
     }
     if (p.dw != nullptr) {
@@ -1067,11 +1204,6 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
       else o.f = static_cast<float*>(dst);
       launch_shaped<kModeDw>(plan, a, o, stream);
     }
-  }
-  if (p.dx != nullptr) {
-    const dim3 dg(blocks_for(static_cast<long long>(p.features) * p.tokens, 4096));
-    if (f32) hipLaunchKernelGGL(ll_dx_kernel<float>, dg, dim3(256), 0, stream, p, by);
-    else hipLaunchKernelGGL(ll_dx_kernel<bf16_t>, dg, dim3(256), 0, stream, p, by);
   }
   return hipGetLastError();
 }

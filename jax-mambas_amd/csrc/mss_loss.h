@@ -17,7 +17,7 @@ constexpr int kLossMaxTop = 1024;
 constexpr int kLinLossTile = 256;  // largest side of a product's tile
 enum { kLossNone = 0, kLossSum = 1, kLossMean = 2 };
 
-// The rows' wanted words (launch_loss_rows). A row counts if it has one: live is 0 (no), 1 (yes), or NaN
+// The rows' wanted words (of lists: launch_loss_rows). A row counts if it has one: live is 0 (no), 1 (yes), or NaN
 // for one with a word outside the vocabulary, whose loss and gradients are NaN.
 struct LossRows {
   int rows, top, vocab;
@@ -34,7 +34,8 @@ struct LossRows {
   int blocks;
 };
 
-int loss_row_blocks(int rows, bool lists);
+int loss_list_blocks(int rows);
+int loss_target_blocks(int tokens);
 hipError_t launch_loss_rows(const LossRows& r, hipStream_t stream);
 
 // A matrix of bf16 in one plane, or of float32 as the sum of three (each the rounding of what the
@@ -62,15 +63,15 @@ struct LinLossParams {
   float2* part;    // [parts][tokens]: a part's largest s and sum of 2^(s - largest), base 2
   int parts;
   float* picked;   // [rows][top] logits of the wanted words
-  float* lse;      // [tokens] base 2
+  float2* stat;    // [tokens + kLinLossTile]: log of the sum of exp s, base 2, and whether the row counts (0, 1)
   float* loss;     // [tokens]
   float* mean;     // the reduced loss, then 1 / (rows that count)
   // backward
   const float* grad;  // [1], or [tokens] without a reduction
-  float2* scale;      // [tokens + kLinLossTile]: lse, and what multiplies the row's gradient
+  float2* scale;      // without a reduction: stat with the row's upstream gradient in place of 1
   bf16_t* g;          // [planes][tokens][ldg] the logits' gradient for a piece of the vocabulary
   long long ldg;
-  float* dx_sum;      // [features][ldx]
+  float* dx_sum;      // [features][ldx] where there are pieces
   long long ldx;
   float* partial;     // sums of tiles that several workgroups share
   int piece;          // words of a piece

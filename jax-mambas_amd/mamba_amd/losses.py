@@ -31,6 +31,7 @@ keeps one, else a cast; float32 operands keep float32 precision throughout. ``ho
 """
 from __future__ import annotations
 
+import contextlib
 import math
 
 import torch
@@ -70,9 +71,12 @@ def _check_lists(ids, teacher, rows, temperature):
     return _io_tag(teacher.dtype, "teacher")
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _guard(t):
     """Launches go to the device of `t`, whichever is current."""
-    return torch.cuda.device(t.device)
+    return _HERE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def _bytes(n, device):
