@@ -1675,8 +1675,8 @@ int linear_loss_sizes(const mss_linear_loss_args* a, mss::LinLossParams* p, mss:
   p->tokens = a->tokens;
   p->features = a->features;
   p->vocab = a->vocab;
-  p->width = (a->features + 63) / 64 * 64;
-  p->planes = a->io_dtype == MSS_BF16 ? 1 : 3;
+  p->planes = a->io_dtype == MSS_BF16 ? 1 : 2;
+  p->width = p->planes == 1 ? (a->features + 63) / 64 * 64 : (a->features + 127) / 128 * 128;
   p->reduction = a->reduction;
   p->temperature = a->temperature;
   p->sf = a->stride_f;
@@ -1693,14 +1693,17 @@ int linear_loss_sizes(const mss_linear_loss_args* a, mss::LinLossParams* p, mss:
   p->c = p->r.c;
   p->picked = c.take<float>(static_cast<long long>(a->tokens) * top);
   p->stat = c.take<float2>(a->tokens + mss::kLinLossTile);
+  p->powers = c.take<int>(2);
   p->xp = c.take<mss::bf16_t>(static_cast<long long>(p->planes) * a->tokens * p->width);
   if (p->pack_w) p->wp = c.take<mss::bf16_t>(static_cast<long long>(p->planes) * a->vocab * p->width);
   *saved = c.at;
   Carve f{static_cast<char*>(a->workspace), 0};
   p->part = f.take<float2>(static_cast<long long>(p->parts) * a->tokens);
+  if (p->planes > 1) p->maxima = f.take<uint32_t>(mss::kLinLossMaxima);
   *fwd = f.at;
   Carve b{static_cast<char*>(a->workspace), 0};
   if (a->reduction == MSS_LOSS_NONE) p->scale = b.take<float2>(a->tokens + mss::kLinLossTile);
+  p->power_g = b.take<int>(1);
   p->g = b.take<mss::bf16_t>(static_cast<long long>(p->planes) * a->tokens * p->ldg);
   if (p->piece < a->vocab) p->dx_sum = b.take<float>(p->features * p->ldx);
   p->partial = b.take<float>(plan->partial);

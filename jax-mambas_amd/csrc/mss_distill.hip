@@ -31,9 +31,12 @@ constexpr int kListRows = 4;  // rows a workgroup
 // A wave a row, kPer entries a lane (entry 64 i + lane). An entry counts where its id is not negative and its
 // logit not -inf; what an entry that does not count holds is not looked at. A word that stands in a list
 // more than once has the sum of its entries, in the first one's place.
+// (Whether one does, a table in LDS tells: four places an entry, each word put in the first free one from its own on.)
 template <int kPer>
 __global__ __launch_bounds__(64 * kListRows) void loss_lists_kernel(LossRows r) {
+  constexpr int kPlaces = 256 * kPer;
   __shared__ int s_n[kListRows];
+  __shared__ int s_table[kListRows][kPlaces];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const long long t = static_cast<long long>(blockIdx.x) * kListRows + w;
   bool any = false;
@@ -70,12 +73,33 @@ __global__ __launch_bounds__(64 * kListRows) void loss_lists_kernel(LossRows r) 
     }
     sum = wave_sum_f(sum);
     const float by = 1.f / sum;
-    float q[kPer] = {};
-    bool first[kPer];
+    float q[kPer];
+    bool first[kPer], again = false;
+    int* table = s_table[w];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) first[i] = true;
+    for (int i = 0; i < kPlaces / 64; ++i) table[64 * i + lane] = -1;
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      q[i] = z[i];
+      first[i] = true;
+      if (word[i] < 0) continue;
+      uint32_t at = static_cast<uint32_t>(word[i]) * 2654435761u >> 16;
+      for (int tries = 0; tries < kPlaces; ++tries, ++at) {
+        const int was = atomicCAS(table + at % kPlaces, -1, word[i]);
+        again |= was == word[i];
+        if (was == -1 || was == word[i]) break;
+      }
+    }
+    again = __any(again);
+    if (again) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) q[i] = 0.f;
+    }
 #pragma unroll
     for (int a = 0; a < kPer; ++a) {
+      if (!again) break;
       const int n = min(64, r.top - 64 * a);
       for (int l = 0; l < n; ++l) {
         const int other = __builtin_amdgcn_readlane(word[a], l);

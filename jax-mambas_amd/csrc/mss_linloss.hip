@@ -8,11 +8,13 @@
 // dot product each. Backward: in pieces of the vocabulary the product is formed again, its tiles
 // turned into g (bf16) in a workspace, from which the two gradients' products read.
 //
-// All products run on v_mfma_f32_32x32x16_bf16 with float32 sums. bf16 operands are taken as they
-// are; g is rounded to bf16 once, as its factors x and w are. A float32 matrix is split into three
-// bf16 planes, each the rounding of what the ones before leave, 24 bits in all, and a product is the sum
-// of the six products of planes that reach 2^-24 of the whole, smallest first: six times the work of
-// a bf16 product, but at 16 times the rate of the float32 matrix instructions.
+// All products run on the matrix cores with float32 sums. bf16 operands are taken as they are
+// (v_mfma_f32_32x32x16_bf16); g is rounded to bf16 once, as its factors x and w are. A float32 matrix is taken to
+// a power of two's multiple whose largest element lies below 2^15, and split into two planes of half precision: the
+// rounding to 11 bits, and that of what it leaves times 2^11. Together they hold 24 bits of what is at least 2^-28
+// of the largest, and 2^-51 of the largest below. A product is the sum of three products of planes
+// (v_mfma_f32_32x32x16_f16), the two with a lower plane first: what is dropped is 2^-24 of each term. Three times
+// the work of a bf16 product, at 16 times the rate of the float32 matrix instructions.
 //
 // 32x32x16 operand layout (lane l, its 8 bf16): A[i][k] at l = i + 32 (k / 8), element k % 8;
 // B[k][j] at l = j + 32 (k / 8), element k % 8; D[i][j] at l = j + 32 ((i / 4) % 2),
@@ -27,12 +29,13 @@ namespace {
 
 typedef __bf16 lbf16x8 __attribute__((ext_vector_type(8)));
 typedef float lf32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 lf16x8 __attribute__((ext_vector_type(8)));
 typedef short ls16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) ls16x4* lds_s16x4_t;
 
 #define LL_INLINE __attribute__((always_inline))  // of lambdas that are called from several places
 
-constexpr int kLlK = 64;  // products' k are whole multiples of it
+constexpr int kLlK = 128;  // the gradients' products' k, and those of split matrices, are whole multiples of it
 
 // Tiles of (32 kMT kWM) x (32 kNT kWN) by kWM x kWN waves of kMT x kNT matrix tiles each, kRing stages of kBK k in
 // LDS.
@@ -120,13 +123,19 @@ struct LlPanel {
   }
 };
 
-// The planes of a product of two split matrices, smallest products first (4 bits each).
-[[maybe_unused]] constexpr unsigned kPairsA = 0x010120, kPairsB = 0x001102;
+// The planes of a product of two split matrices (a bit each): of A and of B in pair 0, 1, 2. The sums of the first
+// two are taken times 2^-11 before the third's.
+constexpr int kPairs = 3;
+[[maybe_unused]] constexpr int kLowPairs = 2;
+[[maybe_unused]] constexpr unsigned kPairsA = 0b010, kPairsB = 0b001;
+constexpr float kLowScale = 0x1p-11f;
+constexpr int kGradExponent = 15;  // of the power of two that g is taken times into its planes
+constexpr float kGradScale = 1 << kGradExponent;
 
 struct LlArgs {
   LossMatrix a, b;       // from the piece's first row and k on
   int k;                 // of the product, a whole number of stages
-  int pairs;             // 1 or 6
+  int pairs;             // 1 or kPairs
   int tiles_m, tiles_n;
   int units;             // of a tile: kRing stages each
   int teams;             // of the gradients' products
@@ -134,23 +143,38 @@ struct LlArgs {
   float* partial;        // their tiles' parts
 };
 
-enum { kModeLse, kModeGrad, kModeGrad3, kModeDx, kModeDw };  // (kModeGrad3: g in three planes)
+enum { kModeLse, kModeGrad, kModeDx, kModeDw };
 
 // What all tokens' gradients are scaled by.
 struct LlScale {
   const float* grad;  // NULL: nothing
   const float* mean;
   float temperature;
+  const int* power;    // of the split matrix that g is multiplied with; NULL: of bf16 operands
+  const int* power_g;  // of the rows' upstream gradients, or NULL
 };
 
-__device__ __forceinline__ float shared_scale(const LlScale& s) {
-  if (s.grad == nullptr) return 1.f;
-  return s.grad[0] * s.temperature * (s.mean ? s.mean[1] : 1.f);
-}
+// As a factor and a power of two, which go on one after the other: their product may lie outside float32 where what
+// they make of a sum does not.
+template <bool kF32>
+struct LlFactor {
+  float f = 1.f;
+  int k = 0;
+  __device__ __forceinline__ explicit LlFactor(const LlScale& s) {
+    if (s.grad != nullptr) f = s.grad[0] * s.temperature * (s.mean ? s.mean[1] : 1.f);
+    if constexpr (kF32) {
+      k = __builtin_amdgcn_frexp_expf(f) - *s.power - kGradExponent;
+      f = __builtin_amdgcn_frexp_mantf(f);
+      if (s.power_g != nullptr) k -= *s.power_g;
+    }
+  }
+  __device__ __forceinline__ float operator()(float v) const { return kF32 ? ldexpf(v * f, k) : v * f; }
+};
 
 struct LlOut {
   int rows, cols;        // of the output that exist, from the piece's first on
   float c;
+  const int* powers;     // of two, of x and of w where they are split
   float2* part;          // kModeLse: [part][cols]
   const float2* scale;   // kModeGrad: [rows], and a tile's rows more
   bf16_t* g;
@@ -167,10 +191,8 @@ struct LlOut {
 // What a tile's sums become.
 template <int kMode>
 constexpr bool kLlTeams = kMode == kModeDx || kMode == kModeDw;
-template <int kMode>
-constexpr bool kLlGrad = kMode == kModeGrad || kMode == kModeGrad3;
 template <class S, int kMode>
-constexpr int ll_perm = kLlGrad<kMode> || kMode == kModeDx ? S::kNT : 1;
+constexpr int ll_perm = kMode == kModeGrad || kMode == kModeDx ? S::kNT : 1;
 template <bool kValue>
 struct LlBool {
   static constexpr bool value = kValue;
@@ -180,6 +202,14 @@ struct LlInt {
   static constexpr int value = kValue;
 };
 
+// A value's planes of half precision. (An upper one that is not finite has a lower one of zero.)
+__device__ __forceinline__ void split_half(float v, uint16_t& hi, uint16_t& lo) {
+  const _Float16 h = static_cast<_Float16>(v);
+  const float left = (v - static_cast<float>(h)) * (1.f / kLowScale);
+  hi = __builtin_bit_cast(uint16_t, h);
+  lo = fabsf(left) < INFINITY ? __builtin_bit_cast(uint16_t, static_cast<_Float16>(left)) : 0;
+}
+
 // A value of another lane of the four (kCtrl: 0xb1 of lane ^ 1, 0x4e of lane ^ 2).
 template <int kCtrl>
 __device__ __forceinline__ float quad_mov(float v) {
@@ -188,10 +218,12 @@ __device__ __forceinline__ float quad_mov(float v) {
 
 // A wave's kMT x kNT matrix tiles: from row wm0 and column wn0 on, in part `part` of the rows. table: the scales of
 // its rows (kModeGrad).
-template <int kMode, int kMT, int kNT>
+template <int kMode, bool kF32, int kMT, int kNT>
 __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT], int wm0, int wn0, int part, int lane,
                                        const float2* table) {
   const int j = lane & 31, g = lane >> 5;
+  // (from a split product's sums to a logit to base 2)
+  [[maybe_unused]] const float c = kF32 && !kLlTeams<kMode> ? ldexpf(o.c, -(o.powers[0] + o.powers[1])) : o.c;
   const auto row_of = [&](int mt, int r) LL_INLINE { return wm0 + 32 * mt + 8 * (r >> 2) + 4 * g + (r & 3); };
   if constexpr (kMode == kModeLse) {
     // Rows are words, columns tokens: a lane has the words of one token.
@@ -210,18 +242,18 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT],
 #pragma unroll
         for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[mt][nt][r]);
       m = fmaxf(m, __shfl_xor(m, 32));
-      const float mc = m == -INFINITY ? 0.f : m * o.c;
+      const float mc = m == -INFINITY ? 0.f : m * c;
       float s = 0.f;
 #pragma unroll
       for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s += fast_exp2(__builtin_fmaf(acc[mt][nt][r], o.c, -mc));
+        for (int r = 0; r < 16; ++r) s += fast_exp2(__builtin_fmaf(acc[mt][nt][r], c, -mc));
       s += __shfl_xor(s, 32);
       const int t = wn0 + 32 * nt + j;
       if (g == 0 && t < o.cols)
         o.part[static_cast<long long>(part) * o.cols + t] = make_float2(m == -INFINITY ? m : mc, s);
     }
-  } else if constexpr (kLlGrad<kMode>) {
+  } else if constexpr (kMode == kModeGrad) {
     // Rows are tokens, columns words, kNT neighbours a lane. The words past the vocabulary are zeros.
     const int v = wn0 + kNT * j;
     const uint32_t at = static_cast<uint32_t>(4 * g * o.ld + v) * 2;
@@ -233,25 +265,26 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT],
         for (int r = 0; r < 16; ++r) {
           const int up = 32 * mt + 8 * (r >> 2) + (r & 3), t = wm0 + up;  // and 4 g more
           const float2 sc = scale[up];
+          const float by = kF32 ? sc.y * kGradScale : sc.y;
           float d[kNT];
 #pragma unroll
           for (int nt = 0; nt < kNT; ++nt) {
-            d[nt] = fast_exp2(__builtin_fmaf(acc[mt][nt][r], o.c, -sc.x)) * sc.y;
+            d[nt] = fast_exp2(__builtin_fmaf(acc[mt][nt][r], c, -sc.x)) * by;
             if (edge.value && v + nt >= o.cols) d[nt] = 0.f;
           }
           if (edge.value && t + 4 * g >= o.rows) continue;
           char* dst = reinterpret_cast<char*>(o.g + t * o.ld) + at;
+          if constexpr (kF32) {
+            uint16_t hi[kNT], lo[kNT];
 #pragma unroll
-          for (int pl = 0; pl < (kMode == kModeGrad3 ? 3 : 1); ++pl) {
+            for (int nt = 0; nt < kNT; ++nt) split_half(d[nt], hi[nt], lo[nt]);
+            __builtin_memcpy(dst, hi, sizeof(hi));
+            __builtin_memcpy(dst + o.plane * 2, lo, sizeof(lo));
+          } else {
             uint32_t w[(kNT + 1) / 2];
 #pragma unroll
             for (int h = 0; h < (kNT + 1) / 2; ++h) w[h] = pack_bf16x2(d[2 * h], d[2 * h + 1 < kNT ? 2 * h + 1 : 2 * h]);
-            if constexpr (kMode == kModeGrad3) {
-#pragma unroll
-              for (int nt = 0; nt < kNT; ++nt)
-                d[nt] -= __uint_as_float(nt % 2 ? w[nt / 2] & 0xffff0000u : w[nt / 2] << 16);
-            }
-            __builtin_memcpy(dst + pl * o.plane * 2, w, 2 * kNT);
+            __builtin_memcpy(dst, w, 2 * kNT);
           }
         }
     };
@@ -272,9 +305,8 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT],
     static_assert(kNT <= 2, "the last lane has one token or all");
     const bool all = t + kNT <= o.cols;
     bool counts[kNT];
-    float f = 1.f;
+    const LlFactor<kF32> by(last ? o.by : LlScale{nullptr, nullptr, 1.f, o.powers, nullptr});
     if (last) {
-      f = shared_scale(o.by);
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) counts[nt] = t + nt < o.cols && o.live[t + nt] != 0.f;
     }
@@ -298,7 +330,7 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT],
             continue;
           }
 #pragma unroll
-          for (int nt = 0; nt < kNT; ++nt) v[r][nt] = counts[nt] ? v[r][nt] * f : 0.f;
+          for (int nt = 0; nt < kNT; ++nt) v[r][nt] = counts[nt] ? by(v[r][nt]) : 0.f;
           const long long to = static_cast<long long>(d + r) * o.cols + at_dx;
           if (o.dx_bf16) {
             uint32_t u[(kNT + 1) / 2];
@@ -319,7 +351,7 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT],
     // Rows are words, columns features. Four rows and four lanes change places, so that a lane has four neighbouring
     // columns of one row: a store instruction then writes 8 rows of 64 bytes (or 128) instead of two, and it is
     // their number that short sums wait for.
-    const float by = shared_scale(o.by);
+    const LlFactor<kF32> by(o.by);
     const bool odd = j & 1, high = j & 2;
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
@@ -332,7 +364,7 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT],
           const int v = wm0 + 32 * mt + 8 * q;  // and 4 g + j % 4 more
           float x[4], y[4];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) x[r] = acc[mt][nt][4 * q + r] * by;
+          for (int r = 0; r < 4; ++r) x[r] = by(acc[mt][nt][4 * q + r]);
 #pragma unroll
           for (int h = 0; h < 4; h += 2) {  // rows h, h + 1 between neighbours
             const float z = quad_mov<0xb1>(odd ? x[h] : x[h + 1]);
@@ -447,7 +479,7 @@ __device__ __forceinline__ f32x4* ll_part(const LlArgs& p, int team, int which, 
   return reinterpret_cast<f32x4*>(p.partial) + ((2LL * team + which) * size + member) * (S::kM * S::kN / 4);
 }
 
-template <class S, int kMode>
+template <class S, int kMode, bool kF32>
 __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host's pass knows no buffer resources
   constexpr bool kAAcross = kLlTeams<kMode>, kBAcross = kMode == kModeDw;
@@ -458,7 +490,7 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % S::kWM, wn = wave / S::kWM;
-  __shared__ float2 s_scale[kLlGrad<kMode> ? S::kM : 1];
+  __shared__ float2 s_scale[kMode == kModeGrad ? S::kM : 1];
   const LlDeal deal = ll_deal<kMode>(p);
   const int nk = p.k / kBK;
 
@@ -481,8 +513,7 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
                   static_cast<uint32_t>(left < 0 ? 0 : left > 0xfffffff0ll ? 0xfffffff0ll : left), 0x00027000};
   };
   const auto issue = [&](u32x4* d) LL_INLINE {
-    const int pa = p.pairs == 1 ? 0 : (kPairsA >> (4 * next_pair)) & 15;
-    const int pb = p.pairs == 1 ? 0 : (kPairsB >> (4 * next_pair)) & 15;
+    const int pa = kF32 ? (kPairsA >> next_pair) & 1 : 0, pb = kF32 ? (kPairsB >> next_pair) & 1 : 0;
     const long long k0 = static_cast<long long>(next_k) * kBK, m0 = static_cast<long long>(next.tm) * S::kM,
                     n0 = static_cast<long long>(next.tn) * S::kN;
     const auto ra = rsrc(p.a, pa, kAAcross ? k0 * p.a.ld + m0 : m0 * p.a.ld + k0);
@@ -531,7 +562,17 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
     for (int mt = 0; mt < S::kMT; ++mt)
 #pragma unroll
       for (int nt = 0; nt < S::kNT; ++nt)
-        acc[mt][nt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[ks & 1][mt], fb[ks & 1][nt], acc[mt][nt], 0, 0, 0);
+        if constexpr (kF32)
+          acc[mt][nt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(lf16x8, fa[ks & 1][mt]),
+                                                               __builtin_bit_cast(lf16x8, fb[ks & 1][nt]), acc[mt][nt], 0, 0, 0);
+        else
+          acc[mt][nt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[ks & 1][mt], fb[ks & 1][nt], acc[mt][nt], 0, 0, 0);
+  };
+  const auto lower = [&]() LL_INLINE {  // the sums with a lower plane
+#pragma unroll
+    for (int mt = 0; mt < S::kMT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < S::kNT; ++nt) acc[mt][nt] *= kLowScale;
   };
 #ifndef LL_V
 #define LL_V 4
@@ -604,7 +645,7 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
     const auto unit = [&](auto newer, bool first) LL_INLINE {
       step(s0, s1, newer);
       // The scales of the tile's rows, once all waves are through with the ones before.
-      if constexpr (kLlGrad<kMode>) {
+      if constexpr (kMode == kModeGrad) {
         if (first) scales(seg.tm);
       }
       if constexpr (S::kRing == 2) {
@@ -616,14 +657,23 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
       }
     };
     // (The first unit of a later tile meets while the stores of the one before, newer than its copies, go on.)
-    constexpr int kStores = S::kRing == 2 && kMode == kModeGrad && S::kMT <= 2 ? 16 * S::kMT : 0;
+    constexpr int kStores = S::kRing == 2 && kMode == kModeGrad && (kF32 ? 2 : 1) * 16 * S::kMT <= 55 ? (kF32 ? 2 : 1) * 16 * S::kMT : 0;
+    const int low = kLowPairs * nk / S::kRing - seg.unit;  // units with a lower plane (a product's k is whole units)
     int u = 0;
-    if constexpr (kLlGrad<kMode>) {
+    if constexpr (kMode == kModeGrad) {
       if (i > 0) unit(LlInt<kStores>{}, true);
       else unit(LlInt<0>{}, true);
       u = 1;
     }
-    for (; u < seg.n; ++u) unit(LlInt<0>{}, false);
+    for (; u < seg.n; ++u) {
+      if constexpr (kF32) {
+        if (u == low) lower();
+      }
+      unit(LlInt<0>{}, false);
+    }
+    if constexpr (kF32) {
+      if (seg.n <= low) lower();
+    }
     if constexpr (kLlTeams<kMode>) {
       if (seg.n < p.units) {
         // A part: its sums, in the order in which the lanes hold them.
@@ -635,7 +685,7 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
         continue;
       }
     }
-    ll_end<kMode>(o, acc, seg.tm * S::kM + wm * 32 * S::kMT, seg.tn * S::kN + wn * 32 * S::kNT, seg.tm * S::kWM + wm, lane,
+    ll_end<kMode, kF32>(o, acc, seg.tm * S::kM + wm * 32 * S::kMT, seg.tn * S::kN + wn * 32 * S::kNT, seg.tm * S::kWM + wm, lane,
                   s_scale + wm * 32 * S::kMT);
     // (Nothing that the compiler knows of is outstanding: else it would wait in the loop, with the copies.)
     if constexpr (kLlTeams<kMode>) __builtin_amdgcn_s_waitcnt(0x0f70);
@@ -645,7 +695,7 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
 }
 
 // The tiles of which teams have parts: the parts' sums in order. A wave of its own for each row of matrix tiles.
-template <class S, int kMode>
+template <class S, int kMode, bool kF32>
 __global__ __launch_bounds__(64) void ll_join_kernel(LlArgs p, LlOut o) {
   const int lane = threadIdx.x;
   const int size = kMode == kModeDx ? p.tiles_m : p.tiles_n, ranges = kMode == kModeDx ? p.tiles_n : p.tiles_m;
@@ -676,30 +726,105 @@ __global__ __launch_bounds__(64) void ll_join_kernel(LlArgs p, LlOut o) {
     }
   }
   const int tm = kMode == kModeDx ? member : range, tn = kMode == kModeDx ? range : member;
-  ll_end<kMode>(o, acc, tm * S::kM + (wave % S::kWM * S::kMT + mt) * 32, tn * S::kN + wave / S::kWM * 32 * S::kNT, 0, lane,
+  ll_end<kMode, kF32>(o, acc, tm * S::kM + (wave % S::kWM * S::kMT + mt) * 32, tn * S::kN + wave / S::kWM * 32 * S::kNT, 0, lane,
                 nullptr);
 }
 
 // ------------------------------------------------------------------------- operands
-// A value's bf16 planes; the lower ones of what is not finite are zeros.
-template <int kPlanes>
-__device__ __forceinline__ void split_planes(float v, bf16_t (&b)[kPlanes]) {
-  b[0] = f32_to_bf16(v);
-  float left = v - to_f32(b[0]);
+// The largest finite magnitudes of float32 matrices, a block's each (as bits, in the order of the values): x's of the
+// tokens that count in the first kMaxX, w's behind them.
+constexpr int kMaxX = 128, kMaxW = 512;
+static_assert(kMaxX + kMaxW == kLinLossMaxima, "");
+
+__device__ __forceinline__ uint32_t finite_bits(float v) {
+  const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0u;
+}
+
+__device__ __forceinline__ bool row_counts(const LinLossParams& p, int t) {
+  return p.r.targets != nullptr ? p.r.targets[t] != p.r.ignore : p.r.live[t] != 0.f;
+}
+
+template <int kWaves>
+__device__ __forceinline__ uint32_t block_max(uint32_t m, uint32_t* s) {
 #pragma unroll
-  for (int i = 1; i < kPlanes; ++i) {
-    if (!(fabsf(left) < INFINITY)) left = 0.f;
-    b[i] = f32_to_bf16(left);
-    left -= to_f32(b[i]);
+  for (int off = 32; off > 0; off >>= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), off)));
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) m = max(m, s[i]);
+  return m;
+}
+
+// 16 waves, so that enough of the matrix is on its way.
+__global__ __launch_bounds__(1024) void ll_max_kernel(LinLossParams p) {
+  __shared__ uint32_t s[16];
+  uint32_t m = 0;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  if (blockIdx.x < kMaxX) {
+    const float* x = static_cast<const float*>(p.x);
+    const bool along_f = p.sf == 1;
+    const int rows = along_f ? p.tokens : p.features, cols = along_f ? p.features : p.tokens;
+    for (int r = blockIdx.x * 16 + w; r < rows; r += 16 * kMaxX)
+#pragma unroll 4
+      for (int c = lane; c < cols; c += 64) {
+        const int f = along_f ? c : r, t = along_f ? r : c;
+        const float v = x[f * p.sf + t * p.st];
+        if (row_counts(p, t)) m = max(m, finite_bits(v));
+      }
+  } else {
+    const float* v = static_cast<const float*>(p.w);
+    for (int r = (blockIdx.x - kMaxX) * 16 + w; r < p.vocab; r += 16 * kMaxW) {
+      const float* row = v + r * p.ldw;
+#pragma unroll 2
+      for (int c = 4 * lane; c + 4 <= p.features; c += 256) {
+        const u32x4 u = *reinterpret_cast<const u32x4_any*>(row + c);
+        m = max(max(m, max(finite_bits(__uint_as_float(u[0])), finite_bits(__uint_as_float(u[1])))),
+                max(finite_bits(__uint_as_float(u[2])), finite_bits(__uint_as_float(u[3]))));
+      }
+      if (lane < p.features % 4) m = max(m, finite_bits(row[p.features - 1 - lane]));
+    }
   }
+  m = block_max<16>(m, s);
+  if (threadIdx.x == 0) p.maxima[blockIdx.x] = m;
+}
+
+// The power of two that takes the largest of kN maxima to 2^14 and more, below 2^15, to all of a block.
+template <int kN>
+__device__ __forceinline__ int plane_power(const uint32_t* maxima, int* power) {
+  __shared__ uint32_t s[4];
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < kN; i += 256)
+    if (i + static_cast<int>(threadIdx.x) < kN) m = max(m, maxima[i + threadIdx.x]);
+  m = block_max<4>(m, s);
+  const int e = m == 0 ? 0 : 15 - __builtin_amdgcn_frexp_expf(__uint_as_float(m));
+  if (power != nullptr && threadIdx.x == 0) *power = e;
+  return e;
+}
+
+// 8 neighbours of a row in their planes: as they are, or split after scaling.
+template <bool kF32>
+__device__ __forceinline__ void store_planes(const float (&v)[8], int power, bf16_t* dst, long long plane) {
+  alignas(16) uint16_t hi[8], lo[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if constexpr (kF32) split_half(ldexpf(v[e], power), hi[e], lo[e]);
+    else hi[e] = f32_to_bf16(v[e]).bits;
+  }
+  *reinterpret_cast<u32x4*>(dst) = *reinterpret_cast<const u32x4*>(hi);
+  if constexpr (kF32) *reinterpret_cast<u32x4*>(dst + plane) = *reinterpret_cast<const u32x4*>(lo);
 }
 
 // x (features, tokens) as token-major rows of `width` features, zeros past the last feature and in rows that
 // do not count (whatever a masked token holds then reaches nothing). Tiles of 64 x 64 through LDS, read
 // along whichever axis is contiguous.
 // With targets the first blocks note the rows' words too.
-template <typename in_t, int kPlanes>
+template <typename in_t>
 __global__ __launch_bounds__(256) void ll_pack_x_kernel(LinLossParams p) {
+  constexpr bool kF32 = sizeof(in_t) == 4;
+  int power = 0;
+  if constexpr (kF32) power = plane_power<kMaxX>(p.maxima, blockIdx.x + blockIdx.y == 0 ? p.powers : nullptr);
   __shared__ float s[64][65];
   __shared__ bool s_live[64];
   const int t0 = blockIdx.x * 64, f0 = blockIdx.y * 64;
@@ -742,24 +867,19 @@ __global__ __launch_bounds__(256) void ll_pack_x_kernel(LinLossParams p) {
     const int slot = threadIdx.x + 256 * i, b = slot / 8, c = 8 * (slot % 8);
     const int t = t0 + b;
     if (t >= p.tokens) continue;
-    alignas(16) bf16_t v[kPlanes][8];
+    float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      bf16_t q[kPlanes];
-      split_planes<kPlanes>(s_live[b] ? s[c + e][b] : 0.f, q);
-#pragma unroll
-      for (int pl = 0; pl < kPlanes; ++pl) v[pl][e] = q[pl];
-    }
-#pragma unroll
-    for (int pl = 0; pl < kPlanes; ++pl)
-      *reinterpret_cast<u32x4*>(p.xp + pl * plane + static_cast<long long>(t) * p.width + f0 + c) =
-          *reinterpret_cast<const u32x4*>(v[pl]);
+    for (int e = 0; e < 8; ++e) v[e] = s_live[b] ? s[c + e][b] : 0.f;
+    store_planes<kF32>(v, power, p.xp + static_cast<long long>(t) * p.width + f0 + c, plane);
   }
 }
 
 // The weight's rows, `width` features each.
-template <typename in_t, int kPlanes>
+template <typename in_t>
 __global__ __launch_bounds__(256) void ll_pack_w_kernel(LinLossParams p) {
+  constexpr bool kF32 = sizeof(in_t) == 4;
+  int power = 0;
+  if constexpr (kF32) power = plane_power<kMaxW>(p.maxima + kMaxX, blockIdx.x == 0 ? p.powers + 1 : nullptr);
   const int per = p.width / 8;
   const long long n = static_cast<long long>(p.vocab) * per, plane = static_cast<long long>(p.vocab) * p.width;
   const in_t* w = static_cast<const in_t*>(p.w);
@@ -767,57 +887,68 @@ __global__ __launch_bounds__(256) void ll_pack_w_kernel(LinLossParams p) {
     const long long row = i / per;
     const int c = 8 * static_cast<int>(i - row * per);
     const in_t* src = w + row * p.ldw + c;
-    alignas(16) bf16_t v[kPlanes][8];
+    alignas(16) in_t raw[8];
+    float v[8];
+    if (c + 8 <= p.features) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      bf16_t q[kPlanes];
-      split_planes<kPlanes>(c + e < p.features ? to_f32(src[e]) : 0.f, q);
+      for (int e = 0; e < static_cast<int>(sizeof(raw) / 16); ++e)
+        reinterpret_cast<u32x4*>(raw)[e] = reinterpret_cast<const u32x4_any*>(src)[e];
 #pragma unroll
-      for (int pl = 0; pl < kPlanes; ++pl) v[pl][e] = q[pl];
+      for (int e = 0; e < 8; ++e) v[e] = to_f32(raw[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = c + e < p.features ? to_f32(src[e]) : 0.f;
     }
-#pragma unroll
-    for (int pl = 0; pl < kPlanes; ++pl)
-      *reinterpret_cast<u32x4*>(p.wp + pl * plane + row * p.width + c) = *reinterpret_cast<const u32x4*>(v[pl]);
+    store_planes<kF32>(v, power, p.wp + row * p.width + c, plane);
   }
 }
 
 // ------------------------------------------------------------------------- the wanted words' logits
 // A wave takes four words of a token's list at a time.
-__device__ __forceinline__ void add_planes(const bf16_t* at, float (&v)[8]) {
+template <bool kF32>
+__device__ __forceinline__ void load_planes(const bf16_t* at, long long plane, float (&v)[8]) {
   const u32x4 u = *reinterpret_cast<const u32x4*>(at);
+  if constexpr (kF32) {
+    const u32x4 l = *reinterpret_cast<const u32x4*>(at + plane);
+    const lf16x8 hi = __builtin_bit_cast(lf16x8, u), lo = __builtin_bit_cast(lf16x8, l);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] += __uint_as_float(u[i] << 16);
-    v[2 * i + 1] += __uint_as_float(u[i] & 0xffff0000u);
+    for (int i = 0; i < 8; ++i) v[i] = __builtin_fmaf(static_cast<float>(lo[i]), kLowScale, static_cast<float>(hi[i]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(u[i] << 16);
+      v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    }
   }
 }
 
 // The logits of kN words of token t (a negative word: 0), in all lanes.
-template <int kPlanes, int kN>
+template <bool kF32, int kN>
 __device__ __forceinline__ void ll_dots(const LinLossParams& p, const LossMatrix& w, long long t, const int (&word)[kN],
                                         int lane, float (&sum)[kN]) {
   const long long xplane = static_cast<long long>(p.tokens) * p.width;
 #pragma unroll
   for (int e = 0; e < kN; ++e) sum[e] = 0.f;
   for (int c = 8 * lane; c < p.width; c += 512) {
-    float x[8] = {};
-#pragma unroll
-    for (int pl = 0; pl < kPlanes; ++pl) add_planes(p.xp + pl * xplane + t * p.width + c, x);
+    float x[8];
+    load_planes<kF32>(p.xp + t * p.width + c, xplane, x);
 #pragma unroll
     for (int e = 0; e < kN; ++e) {
       if (word[e] < 0) continue;
-      float v[8] = {};
-#pragma unroll
-      for (int pl = 0; pl < kPlanes; ++pl) add_planes(w.base + pl * w.plane + word[e] * w.ld + c, v);
+      float v[8];
+      load_planes<kF32>(w.base + word[e] * w.ld + c, w.plane, v);
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum[e] = __builtin_fmaf(x[i], v[i], sum[e]);
     }
   }
 #pragma unroll
-  for (int e = 0; e < kN; ++e) sum[e] = wave_sum(sum[e]);
+  for (int e = 0; e < kN; ++e) {
+    sum[e] = wave_sum(sum[e]);
+    if constexpr (kF32) sum[e] = ldexpf(sum[e], -(p.powers[0] + p.powers[1]));
+  }
 }
 
-template <int kPlanes>
+template <bool kF32>
 __global__ __launch_bounds__(256) void ll_pick_kernel(LinLossParams p, LossMatrix w) {
   const int lane = threadIdx.x & 63;
   const int per = (p.r.top + 3) / 4;
@@ -829,7 +960,7 @@ __global__ __launch_bounds__(256) void ll_pick_kernel(LinLossParams p, LossMatri
 #pragma unroll
   for (int e = 0; e < 4; ++e) word[e] = k0 + e < p.r.top ? p.r.words[t * p.r.top + k0 + e] : -1;
   float sum[4];
-  ll_dots<kPlanes>(p, w, t, word, lane, sum);
+  ll_dots<kF32>(p, w, t, word, lane, sum);
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (lane == 0 && k0 + e < p.r.top) p.picked[t * p.r.top + k0 + e] = sum[e];
@@ -837,7 +968,7 @@ __global__ __launch_bounds__(256) void ll_pick_kernel(LinLossParams p, LossMatri
 
 // ------------------------------------------------------------------------- a token's loss
 // 16 tokens a workgroup: the parts' sums merged, 64 slices of them side by side, then a wave a token over its list.
-// kPlanes: of the operands, where there is one word a token whose logit is formed here; 0: the logits are there.
+// kPick: there is one word a token, whose logit is formed here.
 constexpr int kFinishTokens = 16, kFinishSlices = 64;
 
 // (m, s) with (m2, s2): the sums of 2^(. - m), 2^(. - m2).
@@ -851,7 +982,7 @@ __device__ __forceinline__ void sums_merge(float& m, float& s, float m2, float s
   m = mx;
 }
 
-template <int kPlanes>
+template <bool kPick, bool kF32>
 __global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_finish_kernel(LinLossParams p, LossMatrix wm) {
   __shared__ float s_m[kFinishSlices][kFinishTokens], s_s[kFinishSlices][kFinishTokens], s_lse[kFinishTokens];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -859,10 +990,10 @@ __global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_finish_kerne
   const int mine = threadIdx.x % kFinishTokens, slice = threadIdx.x / kFinishTokens;
   const long long t = t0 + w;
   float logit[1] = {0.f};
-  if constexpr (kPlanes > 0) {
+  if constexpr (kPick) {
     if (t < p.tokens) {
       const int word[1] = {p.r.words[t]};
-      ll_dots<kPlanes>(p, wm, t, word, lane, logit);
+      ll_dots<kF32>(p, wm, t, word, lane, logit);
       if (lane == 0) p.picked[t] = logit[0];
     }
   }
@@ -905,7 +1036,7 @@ __global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_finish_kerne
     const long long at = t * p.r.top + k;
     if (p.r.words[at] < 0) continue;
     const float q = p.r.q[at];
-    const float z = kPlanes > 0 ? logit[0] : p.picked[at];
+    const float z = kPick ? logit[0] : p.picked[at];
     sum = __builtin_fmaf(q, (lse - z * p.c) + fast_log2(q), sum);
   }
   sum = wave_sum(sum) * (kLn2 * p.temperature * p.temperature);
@@ -918,15 +1049,31 @@ __global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_finish_kerne
 // A token's lse, and what its g is scaled by before it is rounded: without a reduction its own upstream gradient. (With
 // one, nothing: what all tokens share is left to the products' ends, since 1 / tokens has an error of its own in
 // bf16, the same for every token.)
-__global__ __launch_bounds__(256) void ll_scale_kernel(LinLossParams p, float2* scale) {
-  const int t = blockIdx.x * 256 + threadIdx.x;
-  if (t >= p.tokens) return;
-  const float2 s = p.stat[t];
-  scale[t] = make_float2(s.x, s.y == 0.f ? 0.f : p.grad[t] * p.temperature);
+// (Split, they are taken to a power of two's multiple below 1 first: one workgroup.)
+template <bool kF32>
+__global__ __launch_bounds__(1024) void ll_scale_kernel(LinLossParams p, float2* scale) {
+  int power = 0;
+  if constexpr (kF32) {
+    __shared__ uint32_t s[16];
+    uint32_t m = 0;
+#pragma unroll 4
+    for (int t = threadIdx.x; t < p.tokens; t += 1024) m = max(m, finite_bits(p.grad[t] * p.temperature));
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), off)));
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
+    __syncthreads();
+    for (int i = 0; i < 16; ++i) m = max(m, s[i]);
+    power = m == 0 ? 0 : -__builtin_amdgcn_frexp_expf(__uint_as_float(m));
+    if (threadIdx.x == 0) p.power_g[0] = power;
+  }
+  for (int t = blockIdx.x * 1024 + threadIdx.x; t < p.tokens; t += gridDim.x * 1024) {
+    const float2 st = p.stat[t];
+    scale[t] = make_float2(st.x, st.y == 0.f ? 0.f : ldexpf(p.grad[t] * p.temperature, power));
+  }
 }
 
 // g at the wanted words of the piece that begins at word v0, from their own logits.
-template <int kPlanes>
+template <bool kF32>
 __global__ __launch_bounds__(256) void ll_wanted_kernel(LinLossParams p, const float2* scale, int v0, int words) {
   const long long i = blockIdx.x * 256LL + threadIdx.x;
   if (i >= static_cast<long long>(p.tokens) * p.r.top) return;
@@ -934,10 +1081,10 @@ __global__ __launch_bounds__(256) void ll_wanted_kernel(LinLossParams p, const f
   if (p.r.words[i] < 0 || v < 0 || v >= words) return;
   const long long t = i / p.r.top;
   const float2 sc = scale[t];
-  bf16_t b[kPlanes];
-  split_planes<kPlanes>((fast_exp2(__builtin_fmaf(p.picked[i], p.c, -sc.x)) - p.r.q[i]) * sc.y, b);
-#pragma unroll
-  for (int pl = 0; pl < kPlanes; ++pl) p.g[pl * (p.tokens * p.ldg) + t * p.ldg + v] = b[pl];
+  const float d = (fast_exp2(__builtin_fmaf(p.picked[i], p.c, -sc.x)) - p.r.q[i]) * sc.y;
+  bf16_t* dst = p.g + t * p.ldg + v;
+  if constexpr (kF32) split_half(d * kGradScale, dst->bits, dst[p.tokens * p.ldg].bits);
+  else store_as(dst, d);
 }
 
 unsigned blocks_for(long long n, long long most) {
@@ -972,7 +1119,7 @@ LlTeams ll_teams(int size, int ranges, int units) {
   return {static_cast<int>(shares), 0};
 }
 
-template <class S, int kMode>
+template <class S, int kMode, bool kF32 = false>
 void launch_product(LlArgs a, const LlOut& o, hipStream_t stream) {
   a.tiles_m = (o.rows + S::kM - 1) / S::kM;
   a.tiles_n = (o.cols + S::kN - 1) / S::kN;
@@ -985,12 +1132,12 @@ void launch_product(LlArgs a, const LlOut& o, hipStream_t stream) {
     const LlTeams t = ll_teams<S>(size, kMode == kModeDx ? a.tiles_n : a.tiles_m, a.units);
     a.teams = t.teams;
     a.whole = t.whole;
-    hipLaunchKernelGGL((ll_kernel<S, kMode>), dim3(a.teams * size), dim3(S::kThreads), 0, stream, a, o);
+    hipLaunchKernelGGL((ll_kernel<S, kMode, kF32>), dim3(a.teams * size), dim3(S::kThreads), 0, stream, a, o);
     if (a.whole == 0)
-      hipLaunchKernelGGL((ll_join_kernel<S, kMode>), dim3(static_cast<unsigned>(tiles * S::kWaves * S::kMT)), dim3(64), 0,
+      hipLaunchKernelGGL((ll_join_kernel<S, kMode, kF32>), dim3(static_cast<unsigned>(tiles * S::kWaves * S::kMT)), dim3(64), 0,
                          stream, a, o);
   } else {
-    hipLaunchKernelGGL((ll_kernel<S, kMode>), dim3(static_cast<unsigned>(tiles < room ? tiles : room)), dim3(S::kThreads), 0,
+    hipLaunchKernelGGL((ll_kernel<S, kMode, kF32>), dim3(static_cast<unsigned>(tiles < room ? tiles : room)), dim3(S::kThreads), 0,
                        stream, a, o);
   }
 }
@@ -1004,20 +1151,20 @@ auto with_shape(int shape, int mode, F&& f) {
   return mode == kModeDw ? f(LlSmall{}) : f(LlThinN{});
 }
 
-template <int kMode>
+template <int kMode, bool kF32>
 void launch_shaped(const LinLossPlan& plan, const LlArgs& a, const LlOut& o, hipStream_t stream) {
-  if constexpr (kLlGrad<kMode>) {
-    if (plan.shape == 0) launch_product<LlSmall, kMode>(a, o, stream);
-    else if (plan.shape == 1) launch_product<LlLargeN, kMode>(a, o, stream);
-    else launch_product<LlThinM, kMode>(a, o, stream);
+  if constexpr (kMode == kModeGrad) {
+    if (plan.shape == 0) launch_product<LlSmall, kMode, kF32>(a, o, stream);
+    else if (plan.shape == 1) launch_product<LlLargeN, kMode, kF32>(a, o, stream);
+    else launch_product<LlThinM, kMode, kF32>(a, o, stream);
   } else if constexpr (kMode == kModeDw) {
-    if (plan.shape_w == 1) launch_product<LlLargeM, kMode>(a, o, stream);
-    else launch_product<LlSmall, kMode>(a, o, stream);
+    if (plan.shape_w == 1) launch_product<LlLargeM, kMode, kF32>(a, o, stream);
+    else launch_product<LlSmall, kMode, kF32>(a, o, stream);
   } else {
     const int shape = kMode == kModeDx ? plan.shape_x : plan.shape;
-    if (shape == 0) launch_product<LlSmall, kMode>(a, o, stream);
-    else if (shape == 1) launch_product<LlLargeM, kMode>(a, o, stream);
-    else launch_product<LlThinN, kMode>(a, o, stream);
+    if (shape == 0) launch_product<LlSmall, kMode, kF32>(a, o, stream);
+    else if (shape == 1) launch_product<LlLargeM, kMode, kF32>(a, o, stream);
+    else launch_product<LlThinN, kMode, kF32>(a, o, stream);
   }
 }
 
@@ -1083,8 +1230,8 @@ LinLossPlan linloss_plan(int tokens, int features, int vocab, int planes) {
   const auto large = [](int rows, int cols) { return 4. * tiles_of(rows, cols, 256, 256) <= 1.4 * tiles_of(rows, cols, 128, 128); };
   q.shape_x = tokens <= 32 ? 2 : large(features, tokens) ? 1 : 0;
   q.shape_w = large(words, features) ? 1 : 0;
-  const int x_stages = q.piece / 64 * (planes == 1 ? 1 : 6);
-  const int w_stages = (tokens + kLlK - 1) / kLlK * (kLlK / 64) * (planes == 1 ? 1 : 6);
+  const int x_stages = q.piece / 64 * (planes == 1 ? 1 : kPairs);
+  const int w_stages = (tokens + kLlK - 1) / kLlK * (kLlK / 64) * (planes == 1 ? 1 : kPairs);
   const long long x = with_shape(q.shape_x, kModeDx, [&](auto s) { return part_sums<decltype(s)>(features, tokens, x_stages); });
   const long long w = with_shape(q.shape_w, kModeDw, [&](auto s) { return part_sums<decltype(s)>(features, words, w_stages); });
   q.partial = x > w ? x : w;
@@ -1097,51 +1244,56 @@ hipError_t launch_linloss_fwd(const LinLossParams& p, const LinLossPlan& plan, h
     const hipError_t e = launch_loss_rows(p.r, stream);
     if (e != hipSuccess) return e;
   }
-  const bool f32 = p.planes == 3;
+  const bool f32 = p.planes == 2;
   const dim3 xg((p.tokens + 63) / 64, p.width / 64);
-  if (f32) hipLaunchKernelGGL((ll_pack_x_kernel<float, 3>), xg, dim3(256), 0, stream, p);
-  else hipLaunchKernelGGL((ll_pack_x_kernel<bf16_t, 1>), xg, dim3(256), 0, stream, p);
+  if (f32) hipLaunchKernelGGL(ll_max_kernel, dim3(kMaxX + kMaxW), dim3(1024), 0, stream, p);
+  if (f32) hipLaunchKernelGGL(ll_pack_x_kernel<float>, xg, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL(ll_pack_x_kernel<bf16_t>, xg, dim3(256), 0, stream, p);
   if (p.pack_w) {
     const dim3 wg(blocks_for(static_cast<long long>(p.vocab) * (p.width / 8), 8192));
-    if (f32) hipLaunchKernelGGL((ll_pack_w_kernel<float, 3>), wg, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((ll_pack_w_kernel<bf16_t, 1>), wg, dim3(256), 0, stream, p);
+    if (f32) hipLaunchKernelGGL(ll_pack_w_kernel<float>, wg, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL(ll_pack_w_kernel<bf16_t>, wg, dim3(256), 0, stream, p);
   }
   LlArgs a{};
   a.a = weight_planes(p);
   a.b = x_planes(p);
   a.k = p.width;
-  a.pairs = f32 ? 6 : 1;
+  a.pairs = f32 ? kPairs : 1;
   LlOut o{};
   o.rows = p.vocab;
   o.cols = p.tokens;
   o.c = p.c;
   o.part = p.part;
-  launch_shaped<kModeLse>(plan, a, o, stream);
+  o.powers = p.powers;
+  if (f32) launch_shaped<kModeLse, true>(plan, a, o, stream);
+  else launch_shaped<kModeLse, false>(plan, a, o, stream);
   const dim3 fg((p.tokens + kFinishTokens - 1) / kFinishTokens), fb(kFinishTokens * kFinishSlices);
   if (lists) {
     const long long picks = static_cast<long long>(p.tokens) * ((p.r.top + 3) / 4);
     const dim3 pg(static_cast<unsigned>((picks + 3) / 4));
-    if (f32) hipLaunchKernelGGL(ll_pick_kernel<3>, pg, dim3(256), 0, stream, p, a.a);
-    else hipLaunchKernelGGL(ll_pick_kernel<1>, pg, dim3(256), 0, stream, p, a.a);
-    hipLaunchKernelGGL(ll_finish_kernel<0>, fg, fb, 0, stream, p, a.a);
+    if (f32) hipLaunchKernelGGL(ll_pick_kernel<true>, pg, dim3(256), 0, stream, p, a.a);
+    else hipLaunchKernelGGL(ll_pick_kernel<false>, pg, dim3(256), 0, stream, p, a.a);
+    hipLaunchKernelGGL((ll_finish_kernel<false, false>), fg, fb, 0, stream, p, a.a);
   } else if (f32) {
-    hipLaunchKernelGGL(ll_finish_kernel<3>, fg, fb, 0, stream, p, a.a);
+    hipLaunchKernelGGL((ll_finish_kernel<true, true>), fg, fb, 0, stream, p, a.a);
   } else {
-    hipLaunchKernelGGL(ll_finish_kernel<1>, fg, fb, 0, stream, p, a.a);
+    hipLaunchKernelGGL((ll_finish_kernel<true, false>), fg, fb, 0, stream, p, a.a);
   }
   if (p.reduction != kLossNone) return launch_loss_mean(p.loss, p.r, p.reduction, p.mean, stream);
   return hipGetLastError();
 }
 
 hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, hipStream_t stream) {
-  const bool f32 = p.planes == 3;
+  const bool f32 = p.planes == 2;
   const float2* scale = p.stat;
   if (p.reduction == kLossNone) {
     scale = p.scale;
-    hipLaunchKernelGGL(ll_scale_kernel, dim3((p.tokens + 255) / 256), dim3(256), 0, stream, p, p.scale);
+    if (f32) hipLaunchKernelGGL(ll_scale_kernel<true>, dim3(1), dim3(1024), 0, stream, p, p.scale);
+    else hipLaunchKernelGGL(ll_scale_kernel<false>, dim3((p.tokens + 1023) / 1024), dim3(1024), 0, stream, p, p.scale);
   }
   const LossMatrix w = weight_planes(p), x = x_planes(p);
-  const LlScale by{p.reduction == kLossNone ? nullptr : p.grad, p.reduction == kLossMean ? p.mean : nullptr, p.temperature};
+  LlScale by{p.reduction == kLossNone ? nullptr : p.grad, p.reduction == kLossMean ? p.mean : nullptr, p.temperature,
+             nullptr, f32 && p.reduction == kLossNone ? p.power_g : nullptr};
   for (long long v0 = 0; v0 < p.vocab; v0 += p.piece) {
     const int words = static_cast<int>(p.vocab - v0 < p.piece ? p.vocab - v0 : p.piece);
     LossMatrix wp = w;
@@ -1153,7 +1305,7 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
     g.plane = p.tokens * p.ldg;
     g.end = g.plane;
     LlArgs a{};
-    a.pairs = f32 ? 6 : 1;
+    a.pairs = f32 ? kPairs : 1;
     // g
     a.a = x;
     a.b = wp;
@@ -1167,11 +1319,12 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
     o.g = p.g;
     o.ld = p.ldg;
     o.plane = g.plane;
-    if (f32) launch_shaped<kModeGrad3>(plan, a, o, stream);
-    else launch_shaped<kModeGrad>(plan, a, o, stream);
+    o.powers = p.powers;
+    if (f32) launch_shaped<kModeGrad, true>(plan, a, o, stream);
+    else launch_shaped<kModeGrad, false>(plan, a, o, stream);
     const dim3 wg(static_cast<unsigned>((static_cast<long long>(p.tokens) * p.r.top + 255) / 256));
-    if (f32) hipLaunchKernelGGL(ll_wanted_kernel<3>, wg, dim3(256), 0, stream, p, scale, static_cast<int>(v0), words);
-    else hipLaunchKernelGGL(ll_wanted_kernel<1>, wg, dim3(256), 0, stream, p, scale, static_cast<int>(v0), words);
+    if (f32) hipLaunchKernelGGL(ll_wanted_kernel<true>, wg, dim3(256), 0, stream, p, scale, static_cast<int>(v0), words);
+    else hipLaunchKernelGGL(ll_wanted_kernel<false>, wg, dim3(256), 0, stream, p, scale, static_cast<int>(v0), words);
     if (p.dx != nullptr) {
       a.a = wp;
       a.b = g;
@@ -1182,13 +1335,16 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
       o.f = p.dx_sum;
       o.ld = p.ldx;
       o.add = v0 > 0;
+      o.powers = p.powers;
       if (v0 + words == p.vocab) {
         o.dx = p.dx;
         o.dx_bf16 = !f32;
         o.by = by;
+        o.by.power = f32 ? p.powers + 1 : nullptr;
         o.live = p.r.live;
       }
-      launch_shaped<kModeDx>(plan, a, o, stream);
+      if (f32) launch_shaped<kModeDx, true>(plan, a, o, stream);
+      else launch_shaped<kModeDx, false>(plan, a, o, stream);
     }
     if (p.dw != nullptr) {
       a.a = g;
@@ -1199,10 +1355,12 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
       o.cols = p.features;
       o.ld = p.features;
       o.by = by;
+      o.by.power = f32 ? p.powers : nullptr;
       void* dst = static_cast<char*>(p.dw) + v0 * p.features * (p.dw_bf16 ? 2 : 4);
       if (p.dw_bf16) o.h = static_cast<bf16_t*>(dst);
       else o.f = static_cast<float*>(dst);
-      launch_shaped<kModeDw>(plan, a, o, stream);
+      if (f32) launch_shaped<kModeDw, true>(plan, a, o, stream);
+      else launch_shaped<kModeDw, false>(plan, a, o, stream);
     }
   }
   return hipGetLastError();

@@ -14,6 +14,7 @@
 namespace mss {
 
 constexpr int kLossMaxTop = 1024;
+constexpr int kLinLossMaxima = 640;
 constexpr int kLinLossTile = 256;  // largest side of a product's tile
 enum { kLossNone = 0, kLossSum = 1, kLossMean = 2 };
 
@@ -47,8 +48,8 @@ struct LossMatrix {
 };
 
 struct LinLossParams {
-  int tokens, features, vocab, width;  // width: features up to a whole number of stages
-  int planes;                          // 1: bf16, 3: float32
+  int tokens, features, vocab, width;  // width: features up to a multiple of 64, of 128 split
+  int planes;                          // 1: bf16, 2: float32, split
   int reduction;
   float temperature, c;
   LossRows r;
@@ -60,6 +61,9 @@ struct LinLossParams {
   int pack_w;
   bf16_t* xp;      // [planes][tokens][width]
   bf16_t* wp;      // [planes][vocab][width] where pack_w
+  uint32_t* maxima;  // of float32 operands, kLinLossMaxima of them
+  int* powers;       // [2]: of two, that x's planes and w's are taken times
+  int* power_g;      // and the rows' upstream gradients
   float2* part;    // [parts][tokens]: a part's largest s and sum of 2^(s - largest), base 2
   int parts;
   float* picked;   // [rows][top] logits of the wanted words

@@ -351,6 +351,42 @@ def test_linear_cross_entropy_many_tiles(dtype, t, d, v):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("x_exp,w_exp,g_exp", [(0, 0, 0), (60, -60, 0), (-70, 66, 5), (100, -104, -20), (-126, 100, 40), (8, 3, -60)])
+def test_float32_of_any_size(x_exp, w_exp, g_exp, reduction):
+    """Operands far from 1, elements that differ by 2^24 among themselves, upstream gradients of any size."""
+    t, d, v = 70, 72, 300
+    x, w = _inputs(t, d, v, F32, 3)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x *= torch.exp2(-24.0 * torch.rand(d, 1, generator=g, device="cuda"))
+    w *= torch.exp2(-24.0 * torch.rand(v, 1, generator=g, device="cuda"))
+    x = torch.ldexp(x, torch.tensor(x_exp, device="cuda")).requires_grad_(True)
+    w = torch.ldexp(w, torch.tensor(w_exp, device="cuda")).requires_grad_(True)
+    targets = _targets(t, v, 0.2, 5)
+    q, live = _wanted_targets(targets, v)
+    up = torch.full((t,) if reduction == "none" else (), 2.0 ** g_exp, device="cuda")
+    loss = linear_cross_entropy(x, w, targets, reduction=reduction)
+    dx, dw = torch.autograd.grad(loss, (x, w), up)
+    ref, xd, wd = _linear_reference(x, w, q, live, 1.0, 1)
+    # (what is 2^-28 of the largest and less keeps 2^-51 of it, g 2^-52)
+    floor = 2.0 ** -50 * d * float(xd.abs().max()) * float(wd.abs().max())
+    ref.loss_tol += 2 * floor * live
+    ref.g_tol += (2 * floor * (ref.g.abs() + q) + 2.0 ** -50) * live[:, None]
+    want, tol, scale = ref.reduced(reduction, up.double())
+    _check("loss", loss, want, tol)
+    gs, gt = ref.g * scale[:, None], ref.g_tol * scale[:, None]
+    small = 2.0 ** -149  # (float32's own end)
+    wantx = torch.mm(gs, wd).t()
+    tol = _product_tol(gt, gs, wd, v).t() + 2.0 ** -50 * float(wd.abs().max()) * gs.abs().sum(1)
+    big = wantx.abs() >= torch.finfo(F32).max * (1 + U)  # what float32 does not hold is rounded to inf
+    assert torch.equal(dx[big], torch.sign(wantx[big]).float() * torch.inf)
+    _check("dx", dx.masked_fill(big, 0), wantx.masked_fill(big, 0), tol + 16 * U * wantx.abs() + small)
+    wantw = torch.mm(gs.t(), xd.t())
+    tol = _product_tol(gt.t(), gs.t(), xd.t(), t) + 2.0 ** -50 * float(xd.abs().max()) * gs.abs().sum(0)[:, None]
+    _check("dw", dw, wantw, tol + 16 * U * wantw.abs() + small)
+
+
+@pytest.mark.gpu
 def test_linear_weight_copies_and_holder():
     """A float32 master with and without its bfloat16 copy; the gradient through a holder; one gradient only."""
     t, d, v = 100, 64, 300
