@@ -719,8 +719,8 @@ int mss_sample(const mss_sample_args* args, void* stream);
  * A row without a word does not count: its loss is 0 and its gradients are zeros, whatever it holds. A row
  * with a word that is not below vocab, or a teacher logit that is NaN or +inf in an entry that counts, has
  * a NaN loss and NaN gradients. reduction: MSS_LOSS_NONE (grad then has one value a row), MSS_LOSS_SUM,
- * MSS_LOSS_MEAN (over the rows that count; 0 without any). loss: [rows], always written; mean: [2] the
- * reduced loss, and what a mean multiplies by (written unless MSS_LOSS_NONE, read by the backward calls).
+ * MSS_LOSS_MEAN (over the rows that count; 0 without any). loss: [rows], always written; mean: the
+ * reduced loss (one value, unless MSS_LOSS_NONE).
  * saved: what the backward calls read of a forward one, mss_*_saved_bytes bytes, 256-byte aligned.
  * ids, teacher, targets and all outputs are contiguous; outputs overlap no input. top is 1 to
  * MSS_LOSS_MAX_TOP, rows * top at most 2^27.

@@ -1645,7 +1645,7 @@ int check_loss(int rows, int vocab, int top, int io, int teacher_dtype, int redu
   return MSS_OK;
 }
 
-mss::LossRows loss_rows(int rows, int top, int vocab, float temperature, bool lists, Carve* saved) {
+mss::LossRows loss_rows(int rows, int top, int vocab, float temperature, bool lists, Carve* saved, float** by) {
   mss::LossRows r{};
   r.rows = rows;
   r.top = top;
@@ -1656,6 +1656,7 @@ mss::LossRows loss_rows(int rows, int top, int vocab, float temperature, bool li
   r.q = saved->take<float>(static_cast<long long>(rows) * top);
   r.live = saved->take<float>(rows);
   r.counts = saved->take<int>(r.blocks);
+  *by = saved->take<float>(1);
   return r;
 }
 
@@ -1689,7 +1690,7 @@ int linear_loss_sizes(const mss_linear_loss_args* a, mss::LinLossParams* p, mss:
   p->ldg = plan->ldg;
   p->ldx = plan->ldx;
   Carve c{static_cast<char*>(a->saved), 0};
-  p->r = loss_rows(a->tokens, top, a->vocab, a->temperature, lists, &c);
+  p->r = loss_rows(a->tokens, top, a->vocab, a->temperature, lists, &c, &p->by);
   p->c = p->r.c;
   p->picked = c.take<float>(static_cast<long long>(a->tokens) * top);
   p->stat = c.take<float2>(a->tokens + mss::kLinLossTile);
@@ -1716,7 +1717,7 @@ int linear_loss_params(const mss_linear_loss_args* a, bool bwd, mss::LinLossPara
   const int s = linear_loss_sizes(a, p, plan, &saved, &ws_f, &ws_b);
   if (s != MSS_OK) return s;
   const int e = loss_type_bytes(a->io_dtype);
-  if (!a->weight || !a->saved || (a->reduction != MSS_LOSS_NONE && !a->mean)) return MSS_ERR_INVALID_ARGUMENT;
+  if (!a->weight || !a->saved || (!bwd && a->reduction != MSS_LOSS_NONE && !a->mean)) return MSS_ERR_INVALID_ARGUMENT;
   if (reinterpret_cast<uintptr_t>(a->x) % e != 0 || reinterpret_cast<uintptr_t>(a->weight) % e != 0)
     return MSS_ERR_INVALID_ARGUMENT;
   const size_t ws = bwd ? ws_b : ws_f;
@@ -1731,7 +1732,6 @@ int linear_loss_params(const mss_linear_loss_args* a, bool bwd, mss::LinLossPara
     if (!a->grad || (!a->dx && !a->dweight) || (a->dw_dtype != MSS_F32 && a->dw_dtype != MSS_BF16))
       return MSS_ERR_INVALID_ARGUMENT;
     in[ni++] = {a->saved, static_cast<long long>(saved)};
-    in[ni++] = {a->mean, 8};
     in[ni++] = {a->grad, a->reduction == MSS_LOSS_NONE ? 4LL * a->tokens : 4};
     out[no++] = {a->dx, static_cast<long long>(a->features) * a->tokens * e};
     out[no++] = {a->dweight, static_cast<long long>(a->vocab) * a->features * loss_type_bytes(a->dw_dtype)};
@@ -1747,7 +1747,7 @@ int linear_loss_params(const mss_linear_loss_args* a, bool bwd, mss::LinLossPara
       in[ni++] = {a->targets, 8 * n};
     }
     out[no++] = {a->loss, 4LL * a->tokens};
-    out[no++] = {a->reduction == MSS_LOSS_NONE ? nullptr : a->mean, 8};
+    out[no++] = {a->reduction == MSS_LOSS_NONE ? nullptr : a->mean, 4};
     out[no++] = {a->saved, static_cast<long long>(saved)};
   }
   if (outputs_meet(out, no, in, ni)) return MSS_ERR_INVALID_ARGUMENT;
@@ -1817,7 +1817,7 @@ int distill_sizes(const mss_distill_args* a, mss::DistillParams* p, size_t* save
   p->temperature = a->temperature;
   p->ld = a->ld;
   Carve c{static_cast<char*>(a->saved), 0};
-  p->r = loss_rows(a->rows, a->top, a->vocab, a->temperature, true, &c);
+  p->r = loss_rows(a->rows, a->top, a->vocab, a->temperature, true, &c, &p->by);
   p->stat = c.take<float2>(a->rows);
   *saved = c.at;
   return MSS_OK;
@@ -1830,7 +1830,7 @@ int run_distill(const mss_distill_args* a, int what, void* stream) {
   if (s != MSS_OK) return s;
   const bool fwd = what & mss::kDsFwd, bwd = what & mss::kDsBwd;
   const int e = loss_type_bytes(a->io_dtype);
-  if (!a->logits || !a->saved || (a->reduction != MSS_LOSS_NONE && !a->mean)) return MSS_ERR_INVALID_ARGUMENT;
+  if (!a->logits || !a->saved || (fwd && a->reduction != MSS_LOSS_NONE && !a->mean)) return MSS_ERR_INVALID_ARGUMENT;
   if (reinterpret_cast<uintptr_t>(a->logits) % e != 0 || reinterpret_cast<uintptr_t>(a->dlogits) % e != 0)
     return MSS_ERR_INVALID_ARGUMENT;
   if (fwd && (!a->ids || !a->teacher || !a->loss)) return MSS_ERR_INVALID_ARGUMENT;
@@ -1842,15 +1842,15 @@ int run_distill(const mss_distill_args* a, int what, void* stream) {
   const long long n = static_cast<long long>(a->rows) * a->top;
   const long long per_row = a->reduction == MSS_LOSS_NONE ? 4LL * a->rows : 4;
   const Span logits = {a->logits, ((a->rows - 1LL) * a->ld + a->vocab) * e}, rest = {a->saved, static_cast<long long>(saved)};
-  const Span mean = {a->reduction == MSS_LOSS_NONE ? nullptr : a->mean, 8};
+  const Span mean = {a->reduction == MSS_LOSS_NONE ? nullptr : a->mean, 4};
   const Span d = {bwd ? a->dlogits : nullptr, static_cast<long long>(a->rows) * a->vocab * e};
   if (fwd) {
     const Span in[] = {logits, {a->ids, 8 * n}, {a->teacher, n * loss_type_bytes(a->teacher_dtype)}};
     const Span out[] = {{a->loss, 4LL * a->rows}, mean, rest, d};
     if (outputs_meet(out, 4, in, 3)) return MSS_ERR_INVALID_ARGUMENT;
   } else {
-    const Span in[] = {logits, rest, mean, {a->grad, per_row}};
-    if (outputs_meet(&d, 1, in, 4)) return MSS_ERR_INVALID_ARGUMENT;
+    const Span in[] = {logits, rest, {a->grad, per_row}};
+    if (outputs_meet(&d, 1, in, 3)) return MSS_ERR_INVALID_ARGUMENT;
   }
   p.r.ids = reinterpret_cast<const long long*>(a->ids);
   p.r.teacher = a->teacher;

@@ -137,7 +137,7 @@ __global__ __launch_bounds__(64 * kListRows) void loss_lists_kernel(LossRows r) 
 
 // The reduced loss, and what a mean divides by (that alone without losses).
 __global__ __launch_bounds__(1024) void loss_mean_kernel(const float* loss, int rows, const int* counts, int blocks,
-                                                         int mean, float* out) {
+                                                         int mean, float* out, float* out_by) {
   __shared__ double s_v[16];
   __shared__ long long s_n[16];
   double v = 0.;
@@ -164,8 +164,8 @@ __global__ __launch_bounds__(1024) void loss_mean_kernel(const float* loss, int 
     n += s_n[i];
   }
   const double by = mean && n > 1 ? 1. / n : 1.;
-  if (loss != nullptr) out[0] = static_cast<float>(v * by);
-  out[1] = static_cast<float>(by);
+  if (loss != nullptr) *out = static_cast<float>(v * by);
+  *out_by = static_cast<float>(by);
 }
 
 // ------------------------------------------------------------------------- the loss from logits
@@ -375,7 +375,7 @@ __global__ __launch_bounds__(kWaves < 4 ? 256 : 64 * kWaves) void distill_kernel
     float f = p.temperature;
     if constexpr ((kDo & kDsAgain) != 0) f *= factor;
     else if constexpr ((kDo & kDsFwd) == 0) f *= p.grad[p.reduction == kLossNone ? t : 0];
-    if (p.reduction == kLossMean) f *= p.mean[1];
+    if (p.reduction == kLossMean) f *= *p.by;
     each([&](int i, const u32x4& u) {
       float v[V::kN];
       V::get(u, v);
@@ -426,9 +426,9 @@ hipError_t launch_loss_rows(const LossRows& r, hipStream_t stream) {
   return hipGetLastError();
 }
 
-hipError_t launch_loss_mean(const float* loss, const LossRows& r, int reduction, float* mean, hipStream_t stream) {
+hipError_t launch_loss_mean(const float* loss, const LossRows& r, int reduction, float* mean, float* by, hipStream_t stream) {
   hipLaunchKernelGGL(loss_mean_kernel, dim3(1), dim3(1024), 0, stream, loss, r.rows, r.counts, r.blocks,
-                     reduction == kLossMean ? 1 : 0, mean);
+                     reduction == kLossMean ? 1 : 0, mean, by);
   return hipGetLastError();
 }
 
@@ -437,7 +437,7 @@ hipError_t launch_distill(const DistillParams& p, int what, hipStream_t stream) 
     hipError_t e = launch_loss_rows(p.r, stream);
     if (e != hipSuccess) return e;
     if (what == (kDsFwd | kDsBwd) && p.reduction == kLossMean) {
-      e = launch_loss_mean(nullptr, p.r, p.reduction, p.mean, stream);
+      e = launch_loss_mean(nullptr, p.r, p.reduction, nullptr, p.by, stream);
       if (e != hipSuccess) return e;
     }
   }
@@ -447,7 +447,7 @@ hipError_t launch_distill(const DistillParams& p, int what, hipStream_t stream) 
   else launch_typed<kDsBwd | kDsAgain>(p, stream);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  if ((what & kDsFwd) && p.reduction != kLossNone) return launch_loss_mean(p.loss, p.r, p.reduction, p.mean, stream);
+  if ((what & kDsFwd) && p.reduction != kLossNone) return launch_loss_mean(p.loss, p.r, p.reduction, p.mean, p.by, stream);
   return hipSuccess;
 }
 

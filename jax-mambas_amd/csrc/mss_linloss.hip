@@ -148,7 +148,7 @@ enum { kModeLse, kModeGrad, kModeDx, kModeDw };
 // What all tokens' gradients are scaled by.
 struct LlScale {
   const float* grad;  // NULL: nothing
-  const float* mean;
+  const float* by;    // NULL: 1
   float temperature;
   const int* power;    // of the split matrix that g is multiplied with; NULL: of bf16 operands
   const int* power_g;  // of the rows' upstream gradients, or NULL
@@ -161,7 +161,7 @@ struct LlFactor {
   float f = 1.f;
   int k = 0;
   __device__ __forceinline__ explicit LlFactor(const LlScale& s) {
-    if (s.grad != nullptr) f = s.grad[0] * s.temperature * (s.mean ? s.mean[1] : 1.f);
+    if (s.grad != nullptr) f = s.grad[0] * s.temperature * (s.by != nullptr ? *s.by : 1.f);
     if constexpr (kF32) {
       k = __builtin_amdgcn_frexp_expf(f) - *s.power - kGradExponent;
       f = __builtin_amdgcn_frexp_mantf(f);
@@ -353,48 +353,57 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT],
     // their number that short sums wait for.
     const LlFactor<kF32> by(o.by);
     const bool odd = j & 1, high = j & 2;
+    const auto rows = [&](auto edge) LL_INLINE {
 #pragma unroll
-    for (int nt = 0; nt < kNT; ++nt) {
-      const int d = wn0 + 32 * nt + (j & ~3);
-      const uint32_t at = static_cast<uint32_t>((4 * g + (j & 3)) * o.ld + d);
+      for (int nt = 0; nt < kNT; ++nt) {
+        const int d = wn0 + 32 * nt + (j & ~3);
+        const uint32_t at = static_cast<uint32_t>((4 * g + (j & 3)) * o.ld + d);
 #pragma unroll
-      for (int mt = 0; mt < kMT; ++mt)
+        for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int v = wm0 + 32 * mt + 8 * q;  // and 4 g + j % 4 more
-          float x[4], y[4];
+          for (int q = 0; q < 4; ++q) {
+            const int v = wm0 + 32 * mt + 8 * q;  // and 4 g + j % 4 more
+            float x[4], y[4];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) x[r] = by(acc[mt][nt][4 * q + r]);
+            for (int r = 0; r < 4; ++r) x[r] = by(acc[mt][nt][4 * q + r]);
 #pragma unroll
-          for (int h = 0; h < 4; h += 2) {  // rows h, h + 1 between neighbours
-            const float z = quad_mov<0xb1>(odd ? x[h] : x[h + 1]);
-            y[h] = odd ? z : x[h];
-            y[h + 1] = odd ? x[h + 1] : z;
-          }
-          const float z0 = quad_mov<0x4e>(high ? y[0] : y[2]), z1 = quad_mov<0x4e>(high ? y[1] : y[3]);
-          const float w[4] = {high ? z0 : y[0], high ? z1 : y[1], high ? y[2] : z0, high ? y[3] : z1};
-          if (v + 4 * g + (j & 3) >= o.rows) continue;
-          if (o.h != nullptr) {
-            char* dst = reinterpret_cast<char*>(o.h + v * o.ld) + 2 * at;
-            const uint32_t u[2] = {pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3])};
-            if (d + 4 <= o.cols) {
-              __builtin_memcpy(dst, u, 8);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 3; ++e)
-                if (d + e < o.cols) reinterpret_cast<uint16_t*>(dst)[e] = static_cast<uint16_t>(u[e / 2] >> (16 * (e & 1)));
+            for (int h = 0; h < 4; h += 2) {  // rows h, h + 1 between neighbours
+              const float z = quad_mov<0xb1>(odd ? x[h] : x[h + 1]);
+              y[h] = odd ? z : x[h];
+              y[h + 1] = odd ? x[h + 1] : z;
             }
-          } else {
-            char* dst = reinterpret_cast<char*>(o.f + v * o.ld) + 4 * at;
-            if (d + 4 <= o.cols) {
-              __builtin_memcpy(dst, w, 16);
-            } else {
+            const float z0 = quad_mov<0x4e>(high ? y[0] : y[2]), z1 = quad_mov<0x4e>(high ? y[1] : y[3]);
+            const float w[4] = {high ? z0 : y[0], high ? z1 : y[1], high ? y[2] : z0, high ? y[3] : z1};
+            if (edge.value && v + 4 * g + (j & 3) >= o.rows) continue;
+            const bool all = !edge.value || d + 4 <= o.cols;
+            if (o.h != nullptr) {
+              char* dst = reinterpret_cast<char*>(o.h + v * o.ld) + 2 * at;
+              const uint32_t u[2] = {pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3])};
+              if (all) {
+                __builtin_memcpy(dst, u, 8);
+              } else {
 #pragma unroll
-              for (int e = 0; e < 3; ++e)
-                if (d + e < o.cols) reinterpret_cast<float*>(dst)[e] = w[e];
+                for (int e = 0; e < 3; ++e)
+                  if (d + e < o.cols) reinterpret_cast<uint16_t*>(dst)[e] = static_cast<uint16_t>(u[e / 2] >> (16 * (e & 1)));
+              }
+            } else {
+              char* dst = reinterpret_cast<char*>(o.f + v * o.ld) + 4 * at;
+              if (all) {
+                __builtin_memcpy(dst, w, 16);
+              } else {
+#pragma unroll
+                for (int e = 0; e < 3; ++e)
+                  if (d + e < o.cols) reinterpret_cast<float*>(dst)[e] = w[e];
+              }
             }
           }
-        }
+      }
+    };
+    if (wm0 + 32 * kMT <= o.rows && wn0 + 32 * kNT <= o.cols) {
+      rows(LlBool<false>{});
+    } else {
+      rows(LlBool<true>{});
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the next tile counts a whole tile's stores)
     }
   }
 }
@@ -538,14 +547,14 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
 
   // The scales of a tile's rows, by every wave, some of them the same ones.
   const auto scales = [&](int tm) LL_INLINE {
-    constexpr int kSlices = S::kM / 128 > 0 ? S::kM / 128 : 1;  // of 1 KB
+    constexpr int kSlices = (S::kM + 127) / 128;  // of 1 KB
     const uint64_t base = reinterpret_cast<uint64_t>(o.scale + tm * S::kM);
     // (readfirstlane: it is the same in all lanes, which the compiler does not see)
     const lu32x4 r{static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(base))),
                    static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(base >> 32) & 0xffff)),
                    S::kM * 8, 0x00027000};
     const int slice = wave % kSlices;
-    if (S::kM >= 128 || lane < S::kM / 2) ll_copy(r, 1024 * slice + 16 * lane, reinterpret_cast<const char*>(s_scale) + 1024 * slice);
+    if (S::kM % 128 == 0 || 1024 * slice + 16 * lane < S::kM * 8) ll_copy(r, 1024 * slice + 16 * lane, reinterpret_cast<const char*>(s_scale) + 1024 * slice);
   };
 
   lf32x16 acc[S::kMT][S::kNT];
@@ -657,10 +666,12 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
       }
     };
     // (The first unit of a later tile meets while the stores of the one before, newer than its copies, go on.)
-    constexpr int kStores = S::kRing == 2 && kMode == kModeGrad && (kF32 ? 2 : 1) * 16 * S::kMT <= 55 ? (kF32 ? 2 : 1) * 16 * S::kMT : 0;
+    // (dw: a part's stores are as many.)
+    constexpr int kOut = kMode == kModeGrad ? (kF32 ? 2 : 1) * 16 * S::kMT : kMode == kModeDw ? S::kSums / 4 : 0;
+    constexpr int kStores = S::kRing == 2 && kOut <= 55 ? kOut : 0;
     const int low = kLowPairs * nk / S::kRing - seg.unit;  // units with a lower plane (a product's k is whole units)
     int u = 0;
-    if constexpr (kMode == kModeGrad) {
+    if constexpr (kMode == kModeGrad || kStores > 0) {
       if (i > 0) unit(LlInt<kStores>{}, true);
       else unit(LlInt<0>{}, true);
       u = 1;
@@ -687,17 +698,21 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
     }
     ll_end<kMode, kF32>(o, acc, seg.tm * S::kM + wm * 32 * S::kMT, seg.tn * S::kN + wn * 32 * S::kNT, seg.tm * S::kWM + wm, lane,
                   s_scale + wm * 32 * S::kMT);
-    // (Nothing that the compiler knows of is outstanding: else it would wait in the loop, with the copies.)
-    if constexpr (kLlTeams<kMode>) __builtin_amdgcn_s_waitcnt(0x0f70);
+    // (None of the loads that the compiler knows of is outstanding: else it would wait in the loop, with the copies.)
+    if constexpr (kMode == kModeDx) __builtin_amdgcn_s_waitcnt(0x0f70);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy outlives the workgroup's LDS
 #endif
 }
 
-// The tiles of which teams have parts: the parts' sums in order. A wave of its own for each row of matrix tiles.
+// The tiles of which teams have parts: the parts' sums, in a fixed order. A workgroup for each row of matrix tiles of a
+// wave, whose four waves take every fourth part.
+constexpr int kJoinWaves = 4;
+
 template <class S, int kMode, bool kF32>
-__global__ __launch_bounds__(64) void ll_join_kernel(LlArgs p, LlOut o) {
-  const int lane = threadIdx.x;
+__global__ __launch_bounds__(64 * kJoinWaves) void ll_join_kernel(LlArgs p, LlOut o) {
+  __shared__ f32x4 s_sum[kJoinWaves - 1][4 * S::kNT][64];
+  const int lane = threadIdx.x & 63, mine = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int size = kMode == kModeDx ? p.tiles_m : p.tiles_n, ranges = kMode == kModeDx ? p.tiles_n : p.tiles_m;
   const int mt = blockIdx.x % S::kMT, wave = blockIdx.x / S::kMT % S::kWaves;
   const int tile = blockIdx.x / (S::kMT * S::kWaves), range = tile / size, member = tile % size;
@@ -714,8 +729,8 @@ __global__ __launch_bounds__(64) void ll_join_kernel(LlArgs p, LlOut o) {
   int end = static_cast<int>((begin + p.units) * p.teams / units);  // the first team behind the range
   while (end > 0 && team_start(p, units, end - 1) >= begin + p.units) --end;
   while (end < p.teams && team_start(p, units, end) < begin + p.units) ++end;
-#pragma unroll 4
-  for (; team < end; ++team) {  // (every team has at least a unit)
+#pragma unroll 2
+  for (team += mine; team < end; team += kJoinWaves) {  // (every team has at least a unit)
     const f32x4* src = ll_part<S, kMode>(p, team, team_start(p, units, team) / p.units != range, member) +
                        wave * (S::kSums / 4 * 64) + mt * (S::kNT * 4 * 64) + lane;
 #pragma unroll
@@ -725,6 +740,22 @@ __global__ __launch_bounds__(64) void ll_join_kernel(LlArgs p, LlOut o) {
       for (int q = 0; q < 4; ++q) acc[0][e / 4][4 * (e % 4) + q] += v[q];
     }
   }
+  if (mine > 0) {
+#pragma unroll
+    for (int e = 0; e < 4 * S::kNT; ++e)
+      s_sum[mine - 1][e][lane] = f32x4{acc[0][e / 4][4 * (e % 4)], acc[0][e / 4][4 * (e % 4) + 1], acc[0][e / 4][4 * (e % 4) + 2],
+                                       acc[0][e / 4][4 * (e % 4) + 3]};
+  }
+  __syncthreads();
+  if (mine > 0) return;
+#pragma unroll
+  for (int i = 0; i < kJoinWaves - 1; ++i)
+#pragma unroll
+    for (int e = 0; e < 4 * S::kNT; ++e) {
+      const f32x4 v = s_sum[i][e][lane];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) acc[0][e / 4][4 * (e % 4) + q] += v[q];
+    }
   const int tm = kMode == kModeDx ? member : range, tn = kMode == kModeDx ? range : member;
   ll_end<kMode, kF32>(o, acc, tm * S::kM + (wave % S::kWM * S::kMT + mt) * 32, tn * S::kN + wave / S::kWM * 32 * S::kNT, 0, lane,
                 nullptr);
@@ -1095,6 +1126,8 @@ unsigned blocks_for(long long n, long long most) {
 //                WM WN MT NT ring
 typedef LlShape<2, 4, 4, 2, 2> LlLargeM;   // 256 x 256, waves of 128 x 64
 typedef LlShape<4, 2, 2, 4, 2> LlLargeN;   // 256 x 256, waves of 64 x 128
+typedef LlShape<4, 2, 2, 3, 2> LlMidM;     // 256 x 192, waves of 64 x 96
+typedef LlShape<2, 4, 3, 2, 2> LlMidN;     // 192 x 256, waves of 96 x 64
 typedef LlShape<2, 2, 2, 2, 2> LlSmall;    // 128 x 128, waves of 64 x 64
 typedef LlShape<4, 1, 1, 1, 4> LlThinN;    // 128 x 32, waves of 32 x 32
 typedef LlShape<1, 4, 1, 1, 4> LlThinM;    // 32 x 128
@@ -1134,7 +1167,7 @@ void launch_product(LlArgs a, const LlOut& o, hipStream_t stream) {
     a.whole = t.whole;
     hipLaunchKernelGGL((ll_kernel<S, kMode, kF32>), dim3(a.teams * size), dim3(S::kThreads), 0, stream, a, o);
     if (a.whole == 0)
-      hipLaunchKernelGGL((ll_join_kernel<S, kMode, kF32>), dim3(static_cast<unsigned>(tiles * S::kWaves * S::kMT)), dim3(64), 0,
+      hipLaunchKernelGGL((ll_join_kernel<S, kMode, kF32>), dim3(static_cast<unsigned>(tiles * S::kWaves * S::kMT)), dim3(64 * kJoinWaves), 0,
                          stream, a, o);
   } else {
     hipLaunchKernelGGL((ll_kernel<S, kMode, kF32>), dim3(static_cast<unsigned>(tiles < room ? tiles : room)), dim3(S::kThreads), 0,
@@ -1156,12 +1189,16 @@ void launch_shaped(const LinLossPlan& plan, const LlArgs& a, const LlOut& o, hip
   if constexpr (kMode == kModeGrad) {
     if (plan.shape == 0) launch_product<LlSmall, kMode, kF32>(a, o, stream);
     else if (plan.shape == 1) launch_product<LlLargeN, kMode, kF32>(a, o, stream);
+    else if (plan.shape == 3) launch_product<LlMidN, kMode, kF32>(a, o, stream);
     else launch_product<LlThinM, kMode, kF32>(a, o, stream);
   } else if constexpr (kMode == kModeDw) {
     if (plan.shape_w == 1) launch_product<LlLargeM, kMode, kF32>(a, o, stream);
     else launch_product<LlSmall, kMode, kF32>(a, o, stream);
   } else {
     const int shape = kMode == kModeDx ? plan.shape_x : plan.shape;
+    if constexpr (kMode == kModeLse) {
+      if (shape == 3) return launch_product<LlMidM, kMode, kF32>(a, o, stream);
+    }
     if (shape == 0) launch_product<LlSmall, kMode, kF32>(a, o, stream);
     else if (shape == 1) launch_product<LlLargeM, kMode, kF32>(a, o, stream);
     else launch_product<LlThinN, kMode, kF32>(a, o, stream);
@@ -1204,8 +1241,10 @@ static long long tiles_of(long long rows, long long cols, int tm, int tn) {
   return ((rows + tm - 1) / tm) * ((cols + tn - 1) / tn);
 }
 
-// Which tiles: a CU does the work of four small ones (128 x 128) in the time of one large one, of two in 0.7 of it,
-// since it reads each operand half as often and has twice the products for each of its waits.
+// Which tiles: the ones whose rounds take the least time, in quarters of a large one's (256 x 256): 3.2 for 256 words
+// by 192 tokens, 2.8 for two small ones (128 x 128) on a CU, which reads each operand twice as often and has half
+// the products for each of its waits. Up to 32 tokens in thin ones. (us, 333 tokens x 768 x 50280, large, 192, small:
+// MEASURE)
 LinLossPlan linloss_plan(int tokens, int features, int vocab, int planes) {
   LinLossPlan q{};
   const auto rounds = [](long long n, long long at_once) { return static_cast<double>((n + at_once - 1) / at_once); };
@@ -1213,11 +1252,12 @@ LinLossPlan linloss_plan(int tokens, int features, int vocab, int planes) {
     q.shape = 2;
   } else {
     const double large = 4 * rounds(tiles_of(vocab, tokens, 256, 256), kCUs);
+    const double mid = 3.2 * rounds(tiles_of(vocab, tokens, 256, 192), kCUs);
     const double small = 2.8 * rounds(tiles_of(vocab, tokens, 128, 128), 2 * kCUs);
-    q.shape = large <= small ? 1 : 0;
+    q.shape = large <= small && large <= mid ? 1 : mid <= small ? 3 : 0;
   }
-  const int tv = q.shape == 1 ? 256 : 128;
-  q.parts = static_cast<int>((vocab + tv - 1) / tv) * (q.shape == 2 ? 4 : 2);
+  const int tv = q.shape == 1 || q.shape == 3 ? 256 : 128;
+  q.parts = static_cast<int>((vocab + tv - 1) / tv) * (q.shape == 2 || q.shape == 3 ? 4 : 2);
   // Pieces of at most 1 GiB.
   const long long most = (1LL << 30) / (2LL * planes * tokens) / 256 * 256;
   const long long whole = (vocab + 255LL) / 256 * 256;
@@ -1279,7 +1319,7 @@ hipError_t launch_linloss_fwd(const LinLossParams& p, const LinLossPlan& plan, h
   } else {
     hipLaunchKernelGGL((ll_finish_kernel<true, false>), fg, fb, 0, stream, p, a.a);
   }
-  if (p.reduction != kLossNone) return launch_loss_mean(p.loss, p.r, p.reduction, p.mean, stream);
+  if (p.reduction != kLossNone) return launch_loss_mean(p.loss, p.r, p.reduction, p.mean, p.by, stream);
   return hipGetLastError();
 }
 
@@ -1292,7 +1332,7 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
     else hipLaunchKernelGGL(ll_scale_kernel<false>, dim3((p.tokens + 1023) / 1024), dim3(1024), 0, stream, p, p.scale);
   }
   const LossMatrix w = weight_planes(p), x = x_planes(p);
-  LlScale by{p.reduction == kLossNone ? nullptr : p.grad, p.reduction == kLossMean ? p.mean : nullptr, p.temperature,
+  LlScale by{p.reduction == kLossNone ? nullptr : p.grad, p.reduction == kLossMean ? p.by : nullptr, p.temperature,
              nullptr, f32 && p.reduction == kLossNone ? p.power_g : nullptr};
   for (long long v0 = 0; v0 < p.vocab; v0 += p.piece) {
     const int words = static_cast<int>(p.vocab - v0 < p.piece ? p.vocab - v0 : p.piece);

@@ -69,7 +69,8 @@ struct LinLossParams {
   float* picked;   // [rows][top] logits of the wanted words
   float2* stat;    // [tokens + kLinLossTile]: log of the sum of exp s, base 2, and whether the row counts (0, 1)
   float* loss;     // [tokens]
-  float* mean;     // the reduced loss, then 1 / (rows that count)
+  float* mean;     // the reduced loss
+  float* by;       // 1 / (rows that count), for a mean
   // backward
   const float* grad;  // [1], or [tokens] without a reduction
   float2* scale;      // without a reduction: stat with the row's upstream gradient in place of 1
@@ -104,7 +105,8 @@ struct DistillParams {
   float* loss;      // [rows]
   float2* stat;     // [rows]: largest logit, log2 of the sum of 2^((logit - largest) c)
   float* picked;    // [rows][top]
-  float* mean;      // the reduced loss, then 1 / (rows that count)
+  float* mean;      // the reduced loss
+  float* by;        // 1 / (rows that count), for a mean
   const float* grad;  // [1], or [rows] without a reduction
   void* dlogits;      // [rows][vocab]
 };
@@ -113,6 +115,6 @@ struct DistillParams {
 // or the gradient once more unless the upstream one is 1 (kDsAgain).
 enum { kDsFwd = 1, kDsBwd = 2, kDsAgain = 4 };
 hipError_t launch_distill(const DistillParams& p, int what, hipStream_t stream);
-hipError_t launch_loss_mean(const float* loss, const LossRows& r, int reduction, float* mean, hipStream_t stream);
+hipError_t launch_loss_mean(const float* loss, const LossRows& r, int reduction, float* mean, float* by, hipStream_t stream);
 
 }  // namespace mss

@@ -108,16 +108,16 @@ class _LinearLoss(torch.autograd.Function):
             saved = _bytes(lib.mss_linear_loss_saved_bytes(a), dev)
             ws = _bytes(lib.mss_linear_loss_workspace_bytes(a, 0), dev)
             loss = torch.empty(t, dtype=_F32, device=dev)
-            mean = torch.empty(2, dtype=_F32, device=dev)
+            mean = torch.empty((), dtype=_F32, device=dev)
             a.loss, a.mean, a.saved, a.saved_bytes = loss.data_ptr(), mean.data_ptr(), saved.data_ptr(), saved.numel()
             a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
             _lib.check(lib.mss_linear_loss_fwd(a, _stream(x)), "mss_linear_loss_fwd")
-        ctx.save_for_backward(w, saved, mean)
+        ctx.save_for_backward(w, saved)
         ctx.args = a
         ctx.x_like = (x.dtype, (f, t))
         ctx.dw_dtype, ctx.holder = weight.dtype, holder
         ctx.set_materialize_grads(False)
-        return loss if reduction == _lib.MSS_LOSS_NONE else mean[0]
+        return loss if reduction == _lib.MSS_LOSS_NONE else mean
 
     @staticmethod
     @once_differentiable
@@ -126,7 +126,7 @@ class _LinearLoss(torch.autograd.Function):
         if grad is None or not (need_x or need_w):
             return (None,) * 11
         lib = _lib.register_hip_kernel()
-        w, saved, mean = ctx.saved_tensors
+        w, saved = ctx.saved_tensors
         src = ctx.args
         dtype, shape = ctx.x_like
         dev = w.device
@@ -135,7 +135,7 @@ class _LinearLoss(torch.autograd.Function):
             dx = torch.empty(shape, dtype=dtype, device=dev) if need_x else None
             dw = torch.empty(w.shape, dtype=ctx.dw_dtype, device=dev) if need_w else None
             a = _lib.LinearLossArgs.from_buffer_copy(src)
-            a.x = a.loss = a.targets = a.ids = a.teacher = None
+            a.x = a.loss = a.mean = a.targets = a.ids = a.teacher = None
             a.weight = w.data_ptr()
             ws = _bytes(lib.mss_linear_loss_workspace_bytes(a, 1), dev)
             a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
@@ -209,16 +209,16 @@ class _Distill(torch.autograd.Function):
         with _guard(logits):
             saved = _bytes(lib.mss_distill_saved_bytes(a), dev)
             loss = torch.empty(rows, dtype=_F32, device=dev)
-            mean = torch.empty(2, dtype=_F32, device=dev)
+            mean = torch.empty((), dtype=_F32, device=dev)
             d = torch.empty(rows, vocab, dtype=logits.dtype, device=dev) if both else None
             a.loss, a.mean, a.saved, a.saved_bytes = loss.data_ptr(), mean.data_ptr(), saved.data_ptr(), saved.numel()
             a.dlogits = _ptr(d)
             name = "mss_distill_fwd_grad" if both else "mss_distill_fwd"
             _lib.check(getattr(lib, name)(a, _stream(logits)), name)
-        ctx.save_for_backward(logits, saved, mean)
+        ctx.save_for_backward(logits, saved)
         ctx.args, ctx.d = a, d
         ctx.set_materialize_grads(False)
-        return loss if reduction == _lib.MSS_LOSS_NONE else mean[0]
+        return loss if reduction == _lib.MSS_LOSS_NONE else mean
 
     @staticmethod
     @once_differentiable
@@ -226,7 +226,7 @@ class _Distill(torch.autograd.Function):
         if grad is None:
             return (None,) * 7
         lib = _lib.register_hip_kernel()
-        logits, saved, mean = ctx.saved_tensors
+        logits, saved = ctx.saved_tensors
         src = ctx.args
         with _guard(logits):
             grad = _upstream(grad, src.reduction, src.rows)
@@ -235,7 +235,7 @@ class _Distill(torch.autograd.Function):
             if d is None:
                 d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
             a = _lib.DistillArgs.from_buffer_copy(src)
-            a.ids = a.teacher = a.loss = None
+            a.ids = a.teacher = a.loss = a.mean = None
             a.grad, a.dlogits = grad.data_ptr(), d.data_ptr()
             _lib.check(getattr(lib, name)(a, _stream(logits)), name)
         return (d,) + (None,) * 6
