@@ -730,13 +730,18 @@ int mss_sample(const mss_sample_args* args, void* stream);
  * kept. With targets (top 0) or lists. Sums are float32; with MSS_BF16 the backward rounds the logits'
  * gradient to bf16 once, in pieces of the vocabulary of at most 1 GiB in the workspace. dx: [features][tokens]
  * of io_dtype, dweight: [vocab][features] of dw_dtype; either may be NULL. tokens and vocab at most 2^20, their
- * product 2^38, features at most 65536 (MSS_ERR_UNSUPPORTED beyond). workspace: for the forward and the
- * backward call each, mss_linear_loss_workspace_bytes, 256-byte aligned, nothing kept in it.
+ * product 2^38, features at most 65536 (MSS_ERR_UNSUPPORTED beyond). workspace:
+ * mss_linear_loss_workspace_bytes for the forward call (which 0), the backward call (1) and
+ * mss_linear_loss_fwd_grad (2), 256-byte aligned, nothing kept in it.
+ * mss_linear_loss_fwd_grad is both directions at once, dx and dweight for an upstream gradient of 1: the logits are
+ * formed once, and the rows of x rounded to bf16 once more, divided by their sum over the vocabulary. Where it is not
+ * offered (MSS_F32, MSS_LOSS_NONE, small heads) its workspace takes 0 bytes and the call returns MSS_ERR_UNSUPPORTED.
+ * mss_linear_loss_rescale then multiplies dx and dweight by *grad, rounding them once more, unless that is 1.
  *
  * mss_distill: logits [rows][vocab] of io_dtype, rows of stride ld (at least vocab), lists only.
  * mss_distill_fwd_grad is both directions in one reading, dlogits for an upstream gradient of 1 and not
- * MSS_LOSS_NONE; mss_distill_regrad then writes dlogits anew for *grad, unless that is 1. vocab at most
- * 2^30. */
+ * MSS_LOSS_NONE; mss_distill_regrad then writes dlogits anew for *grad, unless that is 1. rows at most
+ * 2^21, vocab 2^30. */
 #define MSS_LOSS_NONE 0
 #define MSS_LOSS_SUM 1
 #define MSS_LOSS_MEAN 2
@@ -763,9 +768,11 @@ typedef struct mss_linear_loss_args {
 } mss_linear_loss_args;
 
 size_t mss_linear_loss_saved_bytes(const mss_linear_loss_args* args);
-size_t mss_linear_loss_workspace_bytes(const mss_linear_loss_args* args, int32_t backward);
+size_t mss_linear_loss_workspace_bytes(const mss_linear_loss_args* args, int32_t which);
 int mss_linear_loss_fwd(const mss_linear_loss_args* args, void* stream);
 int mss_linear_loss_bwd(const mss_linear_loss_args* args, void* stream);
+int mss_linear_loss_fwd_grad(const mss_linear_loss_args* args, void* stream);
+int mss_linear_loss_rescale(const mss_linear_loss_args* args, void* stream);
 
 typedef struct mss_distill_args {
   int32_t rows, vocab, top;

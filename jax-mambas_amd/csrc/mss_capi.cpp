@@ -1661,8 +1661,10 @@ mss::LossRows loss_rows(int rows, int top, int vocab, float temperature, bool li
 }
 
 // Everything but the operands' addresses.
-int linear_loss_sizes(const mss_linear_loss_args* a, mss::LinLossParams* p, mss::LinLossPlan* plan, size_t* saved,
-                      size_t* fwd, size_t* bwd) {
+// ws: of the forward, the backward call, and of both at once (0: not offered). What they carve of a->workspace is set for
+// call `which`.
+int linear_loss_sizes(const mss_linear_loss_args* a, int which, mss::LinLossParams* p, mss::LinLossPlan* plan, size_t* saved,
+                      size_t (&ws)[3]) {
   if (a == nullptr || a->top < 0) return MSS_ERR_INVALID_ARGUMENT;
   const bool lists = a->top > 0;
   const int top = lists ? a->top : 1;
@@ -1683,7 +1685,8 @@ int linear_loss_sizes(const mss_linear_loss_args* a, mss::LinLossParams* p, mss:
   p->sf = a->stride_f;
   p->st = a->stride_t;
   p->ldw = a->ldw;
-  p->pack_w = !(a->io_dtype == MSS_BF16 && a->features % 64 == 0 && a->ldw % 8 == 0 && aligned16(a->weight));
+  // (a tile's rows are addressed in 32 bits)
+  p->pack_w = !(a->io_dtype == MSS_BF16 && a->features % 64 == 0 && a->ldw % 8 == 0 && a->ldw <= (1 << 22) && aligned16(a->weight));
   *plan = mss::linloss_plan(p->tokens, p->features, p->vocab, p->planes);
   p->parts = plan->parts;
   p->piece = plan->piece;
@@ -1698,29 +1701,50 @@ int linear_loss_sizes(const mss_linear_loss_args* a, mss::LinLossParams* p, mss:
   p->xp = c.take<mss::bf16_t>(static_cast<long long>(p->planes) * a->tokens * p->width);
   if (p->pack_w) p->wp = c.take<mss::bf16_t>(static_cast<long long>(p->planes) * a->vocab * p->width);
   *saved = c.at;
-  Carve f{static_cast<char*>(a->workspace), 0};
-  p->part = f.take<float2>(static_cast<long long>(p->parts) * a->tokens);
-  if (p->planes > 1) p->maxima = f.take<uint32_t>(mss::kLinLossMaxima);
-  *fwd = f.at;
-  Carve b{static_cast<char*>(a->workspace), 0};
-  if (a->reduction == MSS_LOSS_NONE) p->scale = b.take<float2>(a->tokens + mss::kLinLossTile);
-  p->power_g = b.take<int>(1);
-  p->g = b.take<mss::bf16_t>(static_cast<long long>(p->planes) * a->tokens * p->ldg);
-  if (p->piece < a->vocab) p->dx_sum = b.take<float>(p->features * p->ldx);
-  p->partial = b.take<float>(plan->partial);
-  *bwd = b.at;
+  for (int i = 0; i < 3; ++i) {
+    ws[i] = 0;
+    const bool both = i == 2, fwd = i != 1, bwd = i != 0;
+    if (both && !(plan->both && a->reduction != MSS_LOSS_NONE)) continue;
+    mss::LinLossParams q = *p;
+    Carve f{static_cast<char*>(a->workspace), 0};
+    if (fwd) q.part = f.take<float2>(static_cast<long long>(p->parts) * a->tokens);
+    if (fwd && p->planes > 1) q.maxima = f.take<uint32_t>(mss::kLinLossMaxima);
+    if (bwd) {
+      if (a->reduction == MSS_LOSS_NONE || both) q.scale = f.take<float2>(a->tokens + mss::kLinLossTile);
+      q.power_g = f.take<int>(1);
+      const long long g = static_cast<long long>(p->planes) * a->tokens * p->ldg, e = both ? plan->block * plan->lde : 0;
+      q.g = f.take<mss::bf16_t>(g > e ? g : e);
+      if (p->piece < a->vocab) q.dx_sum = f.take<float>(p->features * p->ldx);
+      q.partial = f.take<float>(both && plan->partial_both > plan->partial ? plan->partial_both : plan->partial);
+    }
+    if (both) {
+      q.factor = f.take<float>(plan->block);
+      q.row_sums = f.take<float>(static_cast<long long>(plan->parts_both) * plan->block);
+      q.xs = f.take<mss::bf16_t>(static_cast<long long>(plan->block) * p->width);
+      if (plan->block < a->tokens) q.dw_sum = f.take<float>(static_cast<long long>(a->vocab) * a->features);
+      q.bad = f.take<int>(1);
+    }
+    ws[i] = f.at;
+    if (i == which) {
+      *p = q;
+      p->parts = plan->parts;
+    }
+  }
   return MSS_OK;
 }
 
-int linear_loss_params(const mss_linear_loss_args* a, bool bwd, mss::LinLossParams* p, mss::LinLossPlan* plan) {
-  size_t saved, ws_f, ws_b;
-  const int s = linear_loss_sizes(a, p, plan, &saved, &ws_f, &ws_b);
+// which: 0 the forward, 1 the backward call, 2 both at once.
+int linear_loss_params(const mss_linear_loss_args* a, int which, mss::LinLossParams* p, mss::LinLossPlan* plan) {
+  size_t saved, sizes[3];
+  const int s = linear_loss_sizes(a, which, p, plan, &saved, sizes);
   if (s != MSS_OK) return s;
+  const bool fwd = which != 1, bwd = which != 0;
+  if (which == 2 && sizes[2] == 0) return MSS_ERR_UNSUPPORTED;
   const int e = loss_type_bytes(a->io_dtype);
-  if (!a->weight || !a->saved || (!bwd && a->reduction != MSS_LOSS_NONE && !a->mean)) return MSS_ERR_INVALID_ARGUMENT;
+  if (!a->weight || !a->saved || (fwd && a->reduction != MSS_LOSS_NONE && !a->mean)) return MSS_ERR_INVALID_ARGUMENT;
   if (reinterpret_cast<uintptr_t>(a->x) % e != 0 || reinterpret_cast<uintptr_t>(a->weight) % e != 0)
     return MSS_ERR_INVALID_ARGUMENT;
-  const size_t ws = bwd ? ws_b : ws_f;
+  const size_t ws = sizes[which];
   if (!aligned256(a->saved) || a->saved_bytes < saved || !a->workspace || !aligned256(a->workspace) || a->workspace_bytes < ws)
     return MSS_ERR_WORKSPACE;
   const long long x_bytes = ((a->features - 1LL) * a->stride_f + (a->tokens - 1LL) * a->stride_t + 1) * e;
@@ -1729,13 +1753,14 @@ int linear_loss_params(const mss_linear_loss_args* a, bool bwd, mss::LinLossPara
   Span out[8] = {{a->workspace, static_cast<long long>(ws)}};
   int ni = 1, no = 1;
   if (bwd) {
-    if (!a->grad || (!a->dx && !a->dweight) || (a->dw_dtype != MSS_F32 && a->dw_dtype != MSS_BF16))
-      return MSS_ERR_INVALID_ARGUMENT;
-    in[ni++] = {a->saved, static_cast<long long>(saved)};
-    in[ni++] = {a->grad, a->reduction == MSS_LOSS_NONE ? 4LL * a->tokens : 4};
+    if (fwd ? !a->dx || !a->dweight : !a->grad || (!a->dx && !a->dweight)) return MSS_ERR_INVALID_ARGUMENT;
+    if (a->dw_dtype != MSS_F32 && a->dw_dtype != MSS_BF16) return MSS_ERR_INVALID_ARGUMENT;
+    if (!fwd) in[ni++] = {a->saved, static_cast<long long>(saved)};
+    if (!fwd) in[ni++] = {a->grad, a->reduction == MSS_LOSS_NONE ? 4LL * a->tokens : 4};
     out[no++] = {a->dx, static_cast<long long>(a->features) * a->tokens * e};
     out[no++] = {a->dweight, static_cast<long long>(a->vocab) * a->features * loss_type_bytes(a->dw_dtype)};
-  } else {
+  }
+  if (fwd) {
     if (!a->x || !a->loss) return MSS_ERR_INVALID_ARGUMENT;
     if (a->top > 0 ? !a->ids || !a->teacher : !a->targets) return MSS_ERR_INVALID_ARGUMENT;
     in[ni++] = {a->x, x_bytes};
@@ -1774,34 +1799,53 @@ int linear_loss_params(const mss_linear_loss_args* a, bool bwd, mss::LinLossPara
 size_t mss_linear_loss_saved_bytes(const mss_linear_loss_args* a) {
   mss::LinLossParams p{};
   mss::LinLossPlan plan;
-  size_t saved = 0, f = 0, b = 0;
-  return linear_loss_sizes(a, &p, &plan, &saved, &f, &b) == MSS_OK ? saved : 0;
+  size_t saved = 0, ws[3];
+  return linear_loss_sizes(a, 0, &p, &plan, &saved, ws) == MSS_OK ? saved : 0;
 }
 
-size_t mss_linear_loss_workspace_bytes(const mss_linear_loss_args* a, int32_t backward) {
+size_t mss_linear_loss_workspace_bytes(const mss_linear_loss_args* a, int32_t which) {
   mss::LinLossParams p{};
   mss::LinLossPlan plan;
-  size_t saved = 0, f = 0, b = 0;
-  if (linear_loss_sizes(a, &p, &plan, &saved, &f, &b) != MSS_OK) return 0;
-  return backward ? b : f;
+  size_t saved = 0, ws[3];
+  return which >= 0 && which <= 2 && linear_loss_sizes(a, 0, &p, &plan, &saved, ws) == MSS_OK ? ws[which] : 0;
 }
 
-int mss_linear_loss_fwd(const mss_linear_loss_args* a, void* stream) {
+namespace {
+int run_linear_loss(const mss_linear_loss_args* a, int which, void* stream) {
   mss::LinLossParams p{};
   mss::LinLossPlan plan;
-  const int s = linear_loss_params(a, false, &p, &plan);
+  const int s = linear_loss_params(a, which, &p, &plan);
   if (s != MSS_OK) return s;
-  const hipError_t e = mss::launch_linloss_fwd(p, plan, static_cast<hipStream_t>(stream));
-  return e == hipSuccess ? MSS_OK : hip_fail(e, "launching linear loss forward");
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const hipError_t e = which == 0   ? mss::launch_linloss_fwd(p, plan, st)
+                       : which == 1 ? mss::launch_linloss_bwd(p, plan, st)
+                                    : mss::launch_linloss_both(p, plan, st);
+  return e == hipSuccess ? MSS_OK : hip_fail(e, "launching linear loss");
 }
+}  // namespace
 
-int mss_linear_loss_bwd(const mss_linear_loss_args* a, void* stream) {
+int mss_linear_loss_fwd(const mss_linear_loss_args* a, void* stream) { return run_linear_loss(a, 0, stream); }
+int mss_linear_loss_bwd(const mss_linear_loss_args* a, void* stream) { return run_linear_loss(a, 1, stream); }
+int mss_linear_loss_fwd_grad(const mss_linear_loss_args* a, void* stream) { return run_linear_loss(a, 2, stream); }
+
+int mss_linear_loss_rescale(const mss_linear_loss_args* a, void* stream) {
   mss::LinLossParams p{};
   mss::LinLossPlan plan;
-  const int s = linear_loss_params(a, true, &p, &plan);
+  size_t saved, ws[3];
+  const int s = linear_loss_sizes(a, 0, &p, &plan, &saved, ws);
   if (s != MSS_OK) return s;
-  const hipError_t e = mss::launch_linloss_bwd(p, plan, static_cast<hipStream_t>(stream));
-  return e == hipSuccess ? MSS_OK : hip_fail(e, "launching linear loss backward");
+  if (ws[2] == 0) return MSS_ERR_UNSUPPORTED;
+  if (!a->dx || !a->dweight || !a->grad || (a->dw_dtype != MSS_F32 && a->dw_dtype != MSS_BF16)) return MSS_ERR_INVALID_ARGUMENT;
+  const Span in = {a->grad, 4};
+  const Span out[] = {{a->dx, static_cast<long long>(a->features) * a->tokens * 2},
+                      {a->dweight, static_cast<long long>(a->vocab) * a->features * loss_type_bytes(a->dw_dtype)}};
+  if (outputs_meet(out, 2, &in, 1)) return MSS_ERR_INVALID_ARGUMENT;
+  p.grad = a->grad;
+  p.dx = a->dx;
+  p.dw = a->dweight;
+  p.dw_bf16 = a->dw_dtype == MSS_BF16;
+  const hipError_t e = mss::launch_linloss_rescale(p, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? MSS_OK : hip_fail(e, "launching gradient rescale");
 }
 
 namespace {
@@ -1810,7 +1854,8 @@ int distill_sizes(const mss_distill_args* a, mss::DistillParams* p, size_t* save
   const int s = check_loss(a->rows, a->vocab, a->top, a->io_dtype, a->teacher_dtype, a->reduction, a->temperature);
   if (s != MSS_OK) return s;
   if (a->ld < a->vocab) return MSS_ERR_INVALID_ARGUMENT;
-  if (a->vocab > (1 << 30) || a->ld > (1LL << 40)) return MSS_ERR_UNSUPPORTED;
+  // (launches of a workgroup a row stay below 2^32 threads)
+  if (a->rows > (1 << 21) || a->vocab > (1 << 30) || a->ld > (1LL << 40)) return MSS_ERR_UNSUPPORTED;
   p->vocab = a->vocab;
   p->io_bf16 = a->io_dtype == MSS_BF16;
   p->reduction = a->reduction;

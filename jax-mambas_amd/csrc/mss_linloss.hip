@@ -21,6 +21,8 @@
 // register 4 (i / 8) + i % 4.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "mss_loss.h"
 
 namespace mss {
@@ -143,17 +145,16 @@ struct LlArgs {
   float* partial;        // their tiles' parts
 };
 
-enum { kModeLse, kModeGrad, kModeDx, kModeDw };
+enum { kModeLse, kModeGrad, kModeExp, kModeDx, kModeDw };
 
 // What all tokens' gradients are scaled by.
 struct LlScale {
-  const float* grad;  // NULL: nothing
-  const float* by;    // NULL: 1
+  const float* grad;  // NULL: 1, and so the next
+  const float* by;
   float temperature;
   const int* power;    // of the split matrix that g is multiplied with; NULL: of bf16 operands
   const int* power_g;  // of the rows' upstream gradients, or NULL
 };
-
 // As a factor and a power of two, which go on one after the other: their product may lie outside float32 where what
 // they make of a sum does not.
 template <bool kF32>
@@ -161,7 +162,9 @@ struct LlFactor {
   float f = 1.f;
   int k = 0;
   __device__ __forceinline__ explicit LlFactor(const LlScale& s) {
-    if (s.grad != nullptr) f = s.grad[0] * s.temperature * (s.by != nullptr ? *s.by : 1.f);
+    f = s.temperature;
+    if (s.grad != nullptr) f *= *s.grad;
+    if (s.by != nullptr) f *= *s.by;
     if constexpr (kF32) {
       k = __builtin_amdgcn_frexp_expf(f) - *s.power - kGradExponent;
       f = __builtin_amdgcn_frexp_mantf(f);
@@ -181,18 +184,25 @@ struct LlOut {
   long long ld, plane;   // row stride of g, dx, dw; from one plane of g to the next
   float* f;              // kModeDx, kModeDw with float32 output
   bf16_t* h;             // kModeDw with bf16 output
-  int add;               // kModeDx: to what is there
+  int add;               // kModeDx, kModeDw: to what is there
   LlScale by;            // kModeDx with the last piece, kModeDw
-  void* dx;              // kModeDx with the last piece: [rows][cols]
+  void* dx;              // kModeDx with the last piece: [rows][ld_dx]
+  long long ld_dx;
   int dx_bf16;
-  const float* live;
+  const float* live;     // and what each column is taken times where that is not 0 (with kModeExp's g)
+  float* row_sums;       // kModeExp: [part][rows]
+  float* sum;            // kModeDw in blocks of the tokens: [rows][ld], added to where `add`; the last one writes dw
+  int last;
+  const int* only_if;    // NULL, or nothing is done where this is 0
 };
 
 // What a tile's sums become.
 template <int kMode>
 constexpr bool kLlTeams = kMode == kModeDx || kMode == kModeDw;
+template <int kMode>
+constexpr bool kLlGrad = kMode == kModeGrad || kMode == kModeExp;
 template <class S, int kMode>
-constexpr int ll_perm = kMode == kModeGrad || kMode == kModeDx ? S::kNT : 1;
+constexpr int ll_perm = kLlGrad<kMode> || kMode == kModeDx ? S::kNT : 1;
 template <bool kValue>
 struct LlBool {
   static constexpr bool value = kValue;
@@ -210,13 +220,14 @@ __device__ __forceinline__ void split_half(float v, uint16_t& hi, uint16_t& lo) 
   lo = fabsf(left) < INFINITY ? __builtin_bit_cast(uint16_t, static_cast<_Float16>(left)) : 0;
 }
 
-// A value of another lane of the four (kCtrl: 0xb1 of lane ^ 1, 0x4e of lane ^ 2).
+// A value of another lane (kCtrl: 0xb1 of lane ^ 1, 0x4e of lane ^ 2, 0x141 of the mirror place in eight lanes, 0x140 in
+// sixteen).
 template <int kCtrl>
 __device__ __forceinline__ float quad_mov(float v) {
   return dpp_mov<kCtrl, 0xF>(0.f, v);
 }
 
-// A wave's kMT x kNT matrix tiles: from row wm0 and column wn0 on, in part `part` of the rows. table: the scales of
+// A wave's kMT x kNT matrix tiles: from row wm0 and column wn0 on, in part `part` of the words. table: the scales of
 // its rows (kModeGrad).
 template <int kMode, bool kF32, int kMT, int kNT>
 __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT], int wm0, int wn0, int part, int lane,
@@ -253,11 +264,12 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT],
       if (g == 0 && t < o.cols)
         o.part[static_cast<long long>(part) * o.cols + t] = make_float2(m == -INFINITY ? m : mc, s);
     }
-  } else if constexpr (kMode == kModeGrad) {
+  } else if constexpr (kLlGrad<kMode>) {
     // Rows are tokens, columns words, kNT neighbours a lane. The words past the vocabulary are zeros.
     const int v = wn0 + kNT * j;
     const uint32_t at = static_cast<uint32_t>(4 * g * o.ld + v) * 2;
     const float2* scale = table + 4 * g;
+    float mine[kMT];  // kModeExp: of the rows' sums over the wave's words, lane 16 + r has that of register r
     const auto rows = [&](auto edge) LL_INLINE {
 #pragma unroll
       for (int mt = 0; mt < kMT; ++mt)
@@ -271,6 +283,17 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT],
           for (int nt = 0; nt < kNT; ++nt) {
             d[nt] = fast_exp2(__builtin_fmaf(acc[mt][nt][r], c, -sc.x)) * by;
             if (edge.value && v + nt >= o.cols) d[nt] = 0.f;
+          }
+          if constexpr (kMode == kModeExp) {
+            float s = d[0];
+#pragma unroll
+            for (int nt = 1; nt < kNT; ++nt) s += d[nt];
+            s += quad_mov<0xb1>(s);
+            s += quad_mov<0x4e>(s);
+            s += quad_mov<0x141>(s);               // of the other four of eight
+            s += quad_mov<0x140>(s);               // of the other eight of sixteen
+            s += dpp_mov<kRowBcast15, 0xa>(0.f, s);  // lanes 16 to 31: of both sixteens
+            mine[mt] = r == 0 || (lane & 15) == r ? s : mine[mt];
           }
           if (edge.value && t + 4 * g >= o.rows) continue;
           char* dst = reinterpret_cast<char*>(o.g + t * o.ld) + at;
@@ -288,12 +311,18 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT],
           }
         }
     };
-    if (wm0 + 32 * kMT <= o.rows && wn0 + 32 * kNT <= o.cols) {
-      rows(LlBool<false>{});
-    } else {
-      rows(LlBool<true>{});
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the next tile counts a whole tile's stores)
+    const bool whole = wm0 + 32 * kMT <= o.rows && wn0 + 32 * kNT <= o.cols;
+    if (whole) rows(LlBool<false>{});
+    else rows(LlBool<true>{});
+    if constexpr (kMode == kModeExp) {
+      const int i = j & 15;
+#pragma unroll
+      for (int mt = 0; mt < kMT; ++mt) {
+        const int t = wm0 + 32 * mt + 8 * (i >> 2) + 4 * g + (i & 3);
+        if (j >= 16 && t < o.rows) o.row_sums[static_cast<long long>(part) * o.rows + t] = mine[mt];
+      }
     }
+    if (!whole) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the next tile counts a whole tile's stores)
   } else if constexpr (kMode == kModeDx) {
     // Rows are features, columns tokens, kNT neighbours a lane: to the sums over the pieces, or, with the last piece,
     // to dx.
@@ -301,14 +330,14 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT],
     if (t >= o.cols) return;  // (a row of sums is long enough for the last lane's kNT)
     const uint32_t at = static_cast<uint32_t>(4 * g * o.ld + t) * 4;
     const bool last = o.dx != nullptr;
-    const long long at_dx = 4LL * g * o.cols + t;
+    const long long at_dx = 4LL * g * o.ld_dx + t;
     static_assert(kNT <= 2, "the last lane has one token or all");
     const bool all = t + kNT <= o.cols;
-    bool counts[kNT];
+    float counts[kNT];
     const LlFactor<kF32> by(last ? o.by : LlScale{nullptr, nullptr, 1.f, o.powers, nullptr});
     if (last) {
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt) counts[nt] = t + nt < o.cols && o.live[t + nt] != 0.f;
+      for (int nt = 0; nt < kNT; ++nt) counts[nt] = t + nt < o.cols ? o.live[t + nt] : 0.f;
     }
 #pragma unroll
     for (int mt = 0; mt < kMT; ++mt)
@@ -330,8 +359,8 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT],
             continue;
           }
 #pragma unroll
-          for (int nt = 0; nt < kNT; ++nt) v[r][nt] = counts[nt] ? by(v[r][nt]) : 0.f;
-          const long long to = static_cast<long long>(d + r) * o.cols + at_dx;
+          for (int nt = 0; nt < kNT; ++nt) v[r][nt] = counts[nt] != 0.f ? by(v[r][nt]) * counts[nt] : 0.f;
+          const long long to = (d + r) * o.ld_dx + at_dx;
           if (o.dx_bf16) {
             uint32_t u[(kNT + 1) / 2];
 #pragma unroll
@@ -365,7 +394,7 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT],
             const int v = wm0 + 32 * mt + 8 * q;  // and 4 g + j % 4 more
             float x[4], y[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[r] = by(acc[mt][nt][4 * q + r]);
+            for (int r = 0; r < 4; ++r) x[r] = acc[mt][nt][4 * q + r];
 #pragma unroll
             for (int h = 0; h < 4; h += 2) {  // rows h, h + 1 between neighbours
               const float z = quad_mov<0xb1>(odd ? x[h] : x[h + 1]);
@@ -373,9 +402,29 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT],
               y[h + 1] = odd ? x[h + 1] : z;
             }
             const float z0 = quad_mov<0x4e>(high ? y[0] : y[2]), z1 = quad_mov<0x4e>(high ? y[1] : y[3]);
-            const float w[4] = {high ? z0 : y[0], high ? z1 : y[1], high ? y[2] : z0, high ? y[3] : z1};
+            float w[4] = {high ? z0 : y[0], high ? z1 : y[1], high ? y[2] : z0, high ? y[3] : z1};
             if (edge.value && v + 4 * g + (j & 3) >= o.rows) continue;
             const bool all = !edge.value || d + 4 <= o.cols;
+            if (o.sum != nullptr) {
+              float* sum = o.sum + v * o.ld + at;
+              if (o.add) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (all || d + e < o.cols) w[e] += sum[e];
+              }
+              if (!o.last) {
+                if (all) {
+                  __builtin_memcpy(sum, w, 16);
+                } else {
+#pragma unroll
+                  for (int e = 0; e < 3; ++e)
+                    if (d + e < o.cols) sum[e] = w[e];
+                }
+                continue;
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = by(w[e]);
             if (o.h != nullptr) {
               char* dst = reinterpret_cast<char*>(o.h + v * o.ld) + 2 * at;
               const uint32_t u[2] = {pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3])};
@@ -499,7 +548,8 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % S::kWM, wn = wave / S::kWM;
-  __shared__ float2 s_scale[kMode == kModeGrad ? S::kM : 1];
+  __shared__ float2 s_scale[kLlGrad<kMode> ? S::kM : 1];
+  if (o.only_if != nullptr && *o.only_if == 0) return;
   const LlDeal deal = ll_deal<kMode>(p);
   const int nk = p.k / kBK;
 
@@ -583,35 +633,14 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
 #pragma unroll
       for (int nt = 0; nt < S::kNT; ++nt) acc[mt][nt] *= kLowScale;
   };
-#ifndef LL_V
-#define LL_V 4
-#endif
   constexpr int kSteps = kBK / 16;
   constexpr int kReads = S::kMT * (kAAcross ? 2 : 1) + S::kNT * (kBAcross ? 2 : 1), kProducts = S::kMT * S::kNT;
   constexpr int kEach = (kReads + kProducts - 1) / kProducts;
   const auto weave = [&]() LL_INLINE {  // a read behind each product
-    if (LL_V == 4) {
 #pragma unroll
-      for (int i = 0; i < kProducts; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, kEach, 0);
-      }
-    } else if (LL_V == 7) {
-      __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, kProducts, 0);
-    } else if (LL_V == 9) {
+    for (int i = 0; i < kProducts; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, kProducts - 1, 0);
-    } else if (LL_V == 10) {
-#pragma unroll
-      for (int i = 0; i < (kReads + 1) / 2; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-      }
-      __builtin_amdgcn_sched_group_barrier(0x008, kProducts - (kReads + 1) / 2, 0);
-    } else if (LL_V == 11 || LL_V == 12) {
-      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_sched_group_barrier(0x100, kEach, 0);
     }
   };
   // A ring of kRing stages. Before the last step of a stage all waves meet: they have read all of it, so its place
@@ -621,19 +650,13 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
 #pragma unroll
     for (int ks = 0; ks + 1 < kSteps; ++ks) {
       load(cur, ks + 1);
-      if (LL_V == 11 || LL_V == 12) __builtin_amdgcn_sched_barrier(0);
-      if (LL_V == 12) __builtin_amdgcn_s_setprio(1);
       multiply(ks);
-      if (LL_V == 12) __builtin_amdgcn_s_setprio(0);
       weave();
     }
     ll_meet<(S::kRing - 2) * S::kCopies + newer.value>();
     issue(cur);
     load(next, 0);
-    if (LL_V == 11 || LL_V == 12) __builtin_amdgcn_sched_barrier(0);
-    if (LL_V == 12) __builtin_amdgcn_s_setprio(1);
     multiply(kSteps - 1);
-    if (LL_V == 12) __builtin_amdgcn_s_setprio(0);
     weave();
   };
   issue(s0);
@@ -654,7 +677,7 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
     const auto unit = [&](auto newer, bool first) LL_INLINE {
       step(s0, s1, newer);
       // The scales of the tile's rows, once all waves are through with the ones before.
-      if constexpr (kMode == kModeGrad) {
+      if constexpr (kLlGrad<kMode>) {
         if (first) scales(seg.tm);
       }
       if constexpr (S::kRing == 2) {
@@ -667,11 +690,11 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
     };
     // (The first unit of a later tile meets while the stores of the one before, newer than its copies, go on.)
     // (dw: a part's stores are as many.)
-    constexpr int kOut = kMode == kModeGrad ? (kF32 ? 2 : 1) * 16 * S::kMT : kMode == kModeDw ? S::kSums / 4 : 0;
+    constexpr int kOut = kLlGrad<kMode> ? (kF32 ? 2 : 1) * 16 * S::kMT : kMode == kModeDw ? S::kSums / 4 : 0;
     constexpr int kStores = S::kRing == 2 && kOut <= 55 ? kOut : 0;
     const int low = kLowPairs * nk / S::kRing - seg.unit;  // units with a lower plane (a product's k is whole units)
     int u = 0;
-    if constexpr (kMode == kModeGrad || kStores > 0) {
+    if constexpr (kLlGrad<kMode> || kStores > 0) {
       if (i > 0) unit(LlInt<kStores>{}, true);
       else unit(LlInt<0>{}, true);
       u = 1;
@@ -696,10 +719,14 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
         continue;
       }
     }
-    ll_end<kMode, kF32>(o, acc, seg.tm * S::kM + wm * 32 * S::kMT, seg.tn * S::kN + wn * 32 * S::kNT, seg.tm * S::kWM + wm, lane,
+    ll_end<kMode, kF32>(o, acc, seg.tm * S::kM + wm * 32 * S::kMT, seg.tn * S::kN + wn * 32 * S::kNT,
+                      kMode == kModeExp ? seg.tn * S::kWN + wn : seg.tm * S::kWM + wm, lane,
                   s_scale + wm * 32 * S::kMT);
     // (None of the loads that the compiler knows of is outstanding: else it would wait in the loop, with the copies.)
     if constexpr (kMode == kModeDx) __builtin_amdgcn_s_waitcnt(0x0f70);
+    if constexpr (kMode == kModeDw) {
+      if (o.add) __builtin_amdgcn_s_waitcnt(0x0f70);
+    }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy outlives the workgroup's LDS
 #endif
@@ -712,6 +739,7 @@ constexpr int kJoinWaves = 4;
 template <class S, int kMode, bool kF32>
 __global__ __launch_bounds__(64 * kJoinWaves) void ll_join_kernel(LlArgs p, LlOut o) {
   __shared__ f32x4 s_sum[kJoinWaves - 1][4 * S::kNT][64];
+  if (o.only_if != nullptr && *o.only_if == 0) return;
   const int lane = threadIdx.x & 63, mine = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int size = kMode == kModeDx ? p.tiles_m : p.tiles_n, ranges = kMode == kModeDx ? p.tiles_n : p.tiles_m;
   const int mt = blockIdx.x % S::kMT, wave = blockIdx.x / S::kMT % S::kWaves;
@@ -979,9 +1007,12 @@ __device__ __forceinline__ void ll_dots(const LinLossParams& p, const LossMatrix
   }
 }
 
+// table (or NULL): what a token's exponentials are taken relative to, to base 2 (kModeExp), the largest logit of its
+// list's first four words; and whether it counts.
 template <bool kF32>
-__global__ __launch_bounds__(256) void ll_pick_kernel(LinLossParams p, LossMatrix w) {
+__global__ __launch_bounds__(256) void ll_pick_kernel(LinLossParams p, LossMatrix w, float2* table) {
   const int lane = threadIdx.x & 63;
+  if (table != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *p.bad = 0;
   const int per = (p.r.top + 3) / 4;
   const long long id = blockIdx.x * 4LL + (threadIdx.x >> 6);
   const long long t = id / per;
@@ -995,6 +1026,13 @@ __global__ __launch_bounds__(256) void ll_pick_kernel(LinLossParams p, LossMatri
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (lane == 0 && k0 + e < p.r.top) p.picked[t * p.r.top + k0 + e] = sum[e];
+  if (table != nullptr && k0 == 0 && lane == 0) {
+    float ref = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (word[e] >= 0) ref = fmaxf(ref, sum[e]);
+    table[t] = make_float2(fabsf(ref) < INFINITY ? ref * p.c : 0.f, p.r.live[t] == 0.f ? 0.f : 1.f);
+  }
 }
 
 // ------------------------------------------------------------------------- a token's loss
@@ -1016,6 +1054,7 @@ __device__ __forceinline__ void sums_merge(float& m, float& s, float m2, float s
 template <bool kPick, bool kF32>
 __global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_finish_kernel(LinLossParams p, LossMatrix wm) {
   __shared__ float s_m[kFinishSlices][kFinishTokens], s_s[kFinishSlices][kFinishTokens], s_lse[kFinishTokens];
+  if (p.only_if != nullptr && *p.only_if == 0) return;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int t0 = blockIdx.x * kFinishTokens;
   const int mine = threadIdx.x % kFinishTokens, slice = threadIdx.x / kFinishTokens;
@@ -1076,6 +1115,87 @@ __global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_finish_kerne
   if (lane == 0) p.loss[t] = sum + (live - live);
 }
 
+// ------------------------------------------------------------------------- both directions at once
+// For a block of tokens and the whole vocabulary at a time, kModeExp leaves e = 2^(s - ref) in bf16, with ref a logit of
+// the token's own list, and its sums S: then lse = ref + log S, softmax = e / S, and g = (e - S q) / S. The division goes
+// to the rows of x for dw, and to dx's columns, so that the logits are formed once, not twice. It fails where S is
+// outside 2^-100 .. 2^100 (a list's words 69 below the largest logit, or above it): such a row is noted in `bad`, and the
+// two-pass kernels, launched behind, do everything anew; else they return at once.
+struct LlBlock {
+  int t0, n, parts;
+  const float* row_sums;  // [part][n]
+  const float2* table;    // from the block's first token on
+  bf16_t* e;
+  long long lde;
+  float* factor;          // [n] 1 / S; 0 where a token does not count
+  bf16_t* xs;             // [n][width] x / S
+};
+
+__global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_block_kernel(LinLossParams p, LlBlock b) {
+  __shared__ float s_s[kFinishSlices][kFinishTokens];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int first = blockIdx.x * kFinishTokens;
+  const int mine = threadIdx.x % kFinishTokens, slice = threadIdx.x / kFinishTokens;
+  {
+    float s = 0.f;
+    if (first + mine < b.n) {
+#pragma unroll 4
+      for (int i = slice; i < b.parts; i += kFinishSlices) s += b.row_sums[static_cast<long long>(i) * b.n + first + mine];
+    }
+    s_s[slice][mine] = s;
+  }
+  for (int h = kFinishSlices / 2; h > 0; h /= 2) {
+    __syncthreads();
+    if (slice < h) s_s[slice][mine] += s_s[slice + h][mine];
+  }
+  __syncthreads();
+  const int at = first + w;
+  if (at >= b.n) return;
+  const long long t = b.t0 + at;
+  const float live = p.r.live[t], S = s_s[0][w], ref = b.table[at].x;
+  const bool counts = live != 0.f;
+  const float lse = (counts ? ref + fast_log2(S) : 0.f) + (live - live);  // NaN for a row with a word outside the vocabulary
+  const float a = counts ? 1.f / S + (live - live) : 0.f;
+  if (lane == 0) {
+    p.stat[t] = make_float2(lse, counts ? 1.f : 0.f);
+    b.factor[at] = a;
+    if (counts && !(S > 0x1p-100f && S < 0x1p100f)) *p.bad = 1;
+  }
+  float sum = 0.f;
+  for (int k = lane; k < p.r.top; k += 64) {
+    const long long i = t * p.r.top + k;
+    const int word = p.r.words[i];
+    if (word < 0) continue;
+    const float q = p.r.q[i], z = p.picked[i] * p.c;
+    sum = __builtin_fmaf(q, (lse - z) + fast_log2(q), sum);
+    store_as(b.e + at * b.lde + word, __builtin_fmaf(-q, S, fast_exp2(z - ref)));
+  }
+  sum = wave_sum(sum) * (kLn2 * p.temperature * p.temperature);
+  if (lane == 0) p.loss[t] = (counts ? sum : 0.f) + (live - live);
+  for (int c = 8 * lane; c < p.width; c += 512) {
+    float x[8];
+    load_planes<false>(p.xp + t * p.width + c, 0, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= a;
+    store_planes<false>(x, 0, b.xs + at * static_cast<long long>(p.width) + c, 0);
+  }
+}
+
+// Gradients of an upstream gradient of 1 to those of another one (nothing for 1).
+template <typename T>
+__device__ __forceinline__ void rescale(T* v, long long n, float f) {
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n; i += gridDim.x * 256LL) store_as(v + i, to_f32(v[i]) * f);
+}
+
+__global__ __launch_bounds__(256) void ll_rescale_kernel(bf16_t* dx, long long nx, void* dw, int dw_bf16, long long nw,
+                                                         const float* grad) {
+  const float f = *grad;
+  if (f == 1.f) return;
+  rescale(dx, nx, f);
+  if (dw_bf16) rescale(static_cast<bf16_t*>(dw), nw, f);
+  else rescale(static_cast<float*>(dw), nw, f);
+}
+
 // ------------------------------------------------------------------------- backward, around the products
 // A token's lse, and what its g is scaled by before it is rounded: without a reduction its own upstream gradient. (With
 // one, nothing: what all tokens share is left to the products' ends, since 1 / tokens has an error of its own in
@@ -1107,7 +1227,7 @@ __global__ __launch_bounds__(1024) void ll_scale_kernel(LinLossParams p, float2*
 template <bool kF32>
 __global__ __launch_bounds__(256) void ll_wanted_kernel(LinLossParams p, const float2* scale, int v0, int words) {
   const long long i = blockIdx.x * 256LL + threadIdx.x;
-  if (i >= static_cast<long long>(p.tokens) * p.r.top) return;
+  if (i >= static_cast<long long>(p.tokens) * p.r.top || (p.only_if != nullptr && *p.only_if == 0)) return;
   const int v = p.r.words[i] - v0;
   if (p.r.words[i] < 0 || v < 0 || v >= words) return;
   const long long t = i / p.r.top;
@@ -1244,7 +1364,7 @@ static long long tiles_of(long long rows, long long cols, int tm, int tn) {
 // Which tiles: the ones whose rounds take the least time, in quarters of a large one's (256 x 256): 3.2 for 256 words
 // by 192 tokens, 2.8 for two small ones (128 x 128) on a CU, which reads each operand twice as often and has half
 // the products for each of its waits. Up to 32 tokens in thin ones. (us, 333 tokens x 768 x 50280, large, 192, small:
-// MEASURE)
+// 46.6, 37.6, 37.0; 256 tokens 26.6, 36.7, 28.8; 128 tokens 25.4, 20.9, 18.7.)
 LinLossPlan linloss_plan(int tokens, int features, int vocab, int planes) {
   LinLossPlan q{};
   const auto rounds = [](long long n, long long at_once) { return static_cast<double>((n + at_once - 1) / at_once); };
@@ -1275,12 +1395,31 @@ LinLossPlan linloss_plan(int tokens, int features, int vocab, int planes) {
   const long long x = with_shape(q.shape_x, kModeDx, [&](auto s) { return part_sums<decltype(s)>(features, tokens, x_stages); });
   const long long w = with_shape(q.shape_w, kModeDw, [&](auto s) { return part_sums<decltype(s)>(features, words, w_stages); });
   q.partial = x > w ? x : w;
+  // Both directions at once, where the logits' product is worth more than the launches that may not be needed.
+  q.both = planes == 1 && tokens >= 512 && static_cast<double>(tokens) * features * vocab >= 0x1p35;
+  if (q.both) {
+    q.lde = whole;
+    const long long rows = (1LL << 30) / (2 * q.lde) / 256 * 256, blocks = (tokens + rows - 1) / rows;
+    q.block = static_cast<int>(((tokens + blocks - 1) / blocks + 255) / 256 * 256);
+    const int n = q.block < tokens ? q.block : tokens;
+    const long long bx = part_sums<LlLargeM>(features, n, static_cast<int>((vocab + kLlK - 1) / kLlK * (kLlK / 64)));
+    const long long bw = part_sums<LlLargeM>(features, vocab, (n + kLlK - 1) / kLlK * (kLlK / 64));
+    q.partial_both = bx > bw ? bx : bw;
+    // (the last block may be shorter, and be shared out in another way)
+    const int rest = tokens % q.block;
+    if (rest > 0) {
+      const long long rx = part_sums<LlLargeM>(features, rest, static_cast<int>((vocab + kLlK - 1) / kLlK * (kLlK / 64)));
+      const long long rw = part_sums<LlLargeM>(features, vocab, (rest + kLlK - 1) / kLlK * (kLlK / 64));
+      q.partial_both = std::max(q.partial_both, std::max(rx, rw));
+    }
+    q.parts_both = static_cast<int>(whole / 256) * LlLargeN::kWN;
+  }
   return q;
 }
 
-hipError_t launch_linloss_fwd(const LinLossParams& p, const LinLossPlan& plan, hipStream_t stream) {
-  const bool lists = p.r.targets == nullptr;
-  if (lists) {
+// The rows' words, x token-major, the weight's copy where it needs one.
+static hipError_t launch_operands(const LinLossParams& p, hipStream_t stream) {
+  if (p.r.targets == nullptr) {
     const hipError_t e = launch_loss_rows(p.r, stream);
     if (e != hipSuccess) return e;
   }
@@ -1294,6 +1433,12 @@ hipError_t launch_linloss_fwd(const LinLossParams& p, const LinLossPlan& plan, h
     if (f32) hipLaunchKernelGGL(ll_pack_w_kernel<float>, wg, dim3(256), 0, stream, p);
     else hipLaunchKernelGGL(ll_pack_w_kernel<bf16_t>, wg, dim3(256), 0, stream, p);
   }
+  return hipGetLastError();
+}
+
+// The words' logits (unless they are there), the sums over the vocabulary, the tokens' losses.
+static void launch_losses(const LinLossParams& p, const LinLossPlan& plan, bool picked, hipStream_t stream) {
+  const bool f32 = p.planes == 2, lists = p.r.targets == nullptr;
   LlArgs a{};
   a.a = weight_planes(p);
   a.b = x_planes(p);
@@ -1305,20 +1450,29 @@ hipError_t launch_linloss_fwd(const LinLossParams& p, const LinLossPlan& plan, h
   o.c = p.c;
   o.part = p.part;
   o.powers = p.powers;
+  o.only_if = p.only_if;
   if (f32) launch_shaped<kModeLse, true>(plan, a, o, stream);
   else launch_shaped<kModeLse, false>(plan, a, o, stream);
   const dim3 fg((p.tokens + kFinishTokens - 1) / kFinishTokens), fb(kFinishTokens * kFinishSlices);
-  if (lists) {
+  if (picked) {
+    hipLaunchKernelGGL((ll_finish_kernel<false, false>), fg, fb, 0, stream, p, a.a);
+  } else if (lists) {
     const long long picks = static_cast<long long>(p.tokens) * ((p.r.top + 3) / 4);
     const dim3 pg(static_cast<unsigned>((picks + 3) / 4));
-    if (f32) hipLaunchKernelGGL(ll_pick_kernel<true>, pg, dim3(256), 0, stream, p, a.a);
-    else hipLaunchKernelGGL(ll_pick_kernel<false>, pg, dim3(256), 0, stream, p, a.a);
+    if (f32) hipLaunchKernelGGL(ll_pick_kernel<true>, pg, dim3(256), 0, stream, p, a.a, static_cast<float2*>(nullptr));
+    else hipLaunchKernelGGL(ll_pick_kernel<false>, pg, dim3(256), 0, stream, p, a.a, static_cast<float2*>(nullptr));
     hipLaunchKernelGGL((ll_finish_kernel<false, false>), fg, fb, 0, stream, p, a.a);
   } else if (f32) {
     hipLaunchKernelGGL((ll_finish_kernel<true, true>), fg, fb, 0, stream, p, a.a);
   } else {
     hipLaunchKernelGGL((ll_finish_kernel<true, false>), fg, fb, 0, stream, p, a.a);
   }
+}
+
+hipError_t launch_linloss_fwd(const LinLossParams& p, const LinLossPlan& plan, hipStream_t stream) {
+  const hipError_t e = launch_operands(p, stream);
+  if (e != hipSuccess) return e;
+  launch_losses(p, plan, false, stream);
   if (p.reduction != kLossNone) return launch_loss_mean(p.loss, p.r, p.reduction, p.mean, p.by, stream);
   return hipGetLastError();
 }
@@ -1332,7 +1486,8 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
     else hipLaunchKernelGGL(ll_scale_kernel<false>, dim3((p.tokens + 1023) / 1024), dim3(1024), 0, stream, p, p.scale);
   }
   const LossMatrix w = weight_planes(p), x = x_planes(p);
-  LlScale by{p.reduction == kLossNone ? nullptr : p.grad, p.reduction == kLossMean ? p.by : nullptr, p.temperature,
+  LlScale by{p.reduction == kLossNone ? nullptr : p.grad, p.reduction == kLossMean ? p.by : nullptr,
+             p.reduction == kLossNone ? 1.f : p.temperature,
              nullptr, f32 && p.reduction == kLossNone ? p.power_g : nullptr};
   for (long long v0 = 0; v0 < p.vocab; v0 += p.piece) {
     const int words = static_cast<int>(p.vocab - v0 < p.piece ? p.vocab - v0 : p.piece);
@@ -1360,6 +1515,7 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
     o.ld = p.ldg;
     o.plane = g.plane;
     o.powers = p.powers;
+    o.only_if = p.only_if;
     if (f32) launch_shaped<kModeGrad, true>(plan, a, o, stream);
     else launch_shaped<kModeGrad, false>(plan, a, o, stream);
     const dim3 wg(static_cast<unsigned>((static_cast<long long>(p.tokens) * p.r.top + 255) / 256));
@@ -1376,8 +1532,10 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
       o.ld = p.ldx;
       o.add = v0 > 0;
       o.powers = p.powers;
+      o.only_if = p.only_if;
       if (v0 + words == p.vocab) {
         o.dx = p.dx;
+        o.ld_dx = p.tokens;
         o.dx_bf16 = !f32;
         o.by = by;
         o.by.power = f32 ? p.powers + 1 : nullptr;
@@ -1394,6 +1552,7 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
       o.rows = words;
       o.cols = p.features;
       o.ld = p.features;
+      o.only_if = p.only_if;
       o.by = by;
       o.by.power = f32 ? p.powers : nullptr;
       void* dst = static_cast<char*>(p.dw) + v0 * p.features * (p.dw_bf16 ? 2 : 4);
@@ -1403,6 +1562,82 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
       else launch_shaped<kModeDw, false>(plan, a, o, stream);
     }
   }
+  return hipGetLastError();
+}
+
+hipError_t launch_linloss_both(const LinLossParams& given, const LinLossPlan& plan, hipStream_t stream) {
+  LinLossParams p = given;
+  hipError_t e = launch_operands(p, stream);
+  if (e != hipSuccess) return e;
+  e = launch_loss_mean(nullptr, p.r, p.reduction, nullptr, p.by, stream);
+  if (e != hipSuccess) return e;
+  const LossMatrix w = weight_planes(p);
+  const long long picks = static_cast<long long>(p.tokens) * ((p.r.top + 3) / 4);
+  hipLaunchKernelGGL(ll_pick_kernel<false>, dim3(static_cast<unsigned>((picks + 3) / 4)), dim3(256), 0, stream, p, w, p.scale);
+  const LlScale by{nullptr, p.reduction == kLossMean ? p.by : nullptr, p.temperature, nullptr, nullptr};
+  for (int t0 = 0; t0 < p.tokens; t0 += plan.block) {
+    const int n = p.tokens - t0 < plan.block ? p.tokens - t0 : plan.block;
+    LossMatrix x = x_planes(p);
+    x.base += static_cast<long long>(t0) * p.width;
+    x.end = static_cast<long long>(n) * p.width;
+    LossMatrix g{p.g, plan.lde, 0, n * plan.lde};
+    LlArgs a{};
+    a.pairs = 1;
+    a.partial = p.partial;
+    a.a = x;
+    a.b = w;
+    a.k = p.width;
+    LlOut o{};
+    o.rows = n;
+    o.cols = p.vocab;
+    o.c = p.c;
+    o.scale = p.scale + t0;
+    o.g = p.g;
+    o.ld = plan.lde;
+    o.row_sums = p.row_sums;
+    launch_product<LlLargeN, kModeExp>(a, o, stream);
+    LlBlock b{t0, n, (p.vocab + 255) / 256 * LlLargeN::kWN, p.row_sums, p.scale + t0, p.g, plan.lde, p.factor, p.xs};
+    hipLaunchKernelGGL(ll_block_kernel, dim3((n + kFinishTokens - 1) / kFinishTokens), dim3(kFinishTokens * kFinishSlices), 0,
+                       stream, p, b);
+    a.a = w;
+    a.b = g;
+    a.k = (p.vocab + kLlK - 1) / kLlK * kLlK;
+    o = LlOut{};
+    o.rows = p.features;
+    o.cols = n;
+    o.dx = static_cast<bf16_t*>(p.dx) + t0;
+    o.ld_dx = p.tokens;
+    o.dx_bf16 = 1;
+    o.by = by;
+    o.live = p.factor;
+    launch_product<LlLargeM, kModeDx>(a, o, stream);
+    a.a = g;
+    a.b = LossMatrix{p.xs, p.width, 0, static_cast<long long>(n) * p.width};
+    a.k = (n + kLlK - 1) / kLlK * kLlK;
+    o = LlOut{};
+    o.rows = p.vocab;
+    o.cols = p.features;
+    o.ld = p.features;
+    o.by = by;
+    o.sum = p.tokens > plan.block ? p.dw_sum : nullptr;
+    o.add = t0 > 0;
+    o.last = t0 + n == p.tokens;
+    if (p.dw_bf16) o.h = static_cast<bf16_t*>(p.dw);
+    else o.f = static_cast<float*>(p.dw);
+    launch_product<LlLargeM, kModeDw>(a, o, stream);
+  }
+  p.only_if = p.bad;
+  p.grad = nullptr;
+  launch_losses(p, plan, true, stream);
+  e = launch_loss_mean(p.loss, p.r, p.reduction, p.mean, p.by, stream);
+  if (e != hipSuccess) return e;
+  return launch_linloss_bwd(p, plan, stream);
+}
+
+hipError_t launch_linloss_rescale(const LinLossParams& p, hipStream_t stream) {
+  const long long nx = static_cast<long long>(p.features) * p.tokens, nw = static_cast<long long>(p.vocab) * p.features;
+  hipLaunchKernelGGL(ll_rescale_kernel, dim3(blocks_for(nx > nw ? nx : nw, 4096)), dim3(256), 0, stream,
+                     static_cast<bf16_t*>(p.dx), nx, p.dw, p.dw_bf16, nw, p.grad);
   return hipGetLastError();
 }
 

@@ -83,6 +83,13 @@ struct LinLossParams {
   void* dx;           // [features][tokens] as x
   void* dw;           // [vocab][features]
   int dw_bf16;
+  // both directions at once
+  float* factor;      // [block]
+  float* row_sums;    // [parts_both][block]
+  bf16_t* xs;         // [block][width]
+  float* dw_sum;      // [vocab][features] where there are blocks
+  int* bad;
+  const int* only_if; // NULL, or nothing is done where this is 0
 };
 
 // What the call needs besides its operands; sizes depend on nothing but the arguments.
@@ -90,10 +97,14 @@ struct LinLossPlan {
   int shape, shape_x, shape_w;  // of the tiles: 0 small, 1 large, 2 thin
   int parts, piece;
   long long ldg, ldx, partial;
+  int both, block, parts_both;  // both directions at once: whether, tokens of a block
+  long long lde, partial_both;
 };
 LinLossPlan linloss_plan(int tokens, int features, int vocab, int planes);
 
 hipError_t launch_linloss_fwd(const LinLossParams& p, const LinLossPlan& plan, hipStream_t stream);
+hipError_t launch_linloss_both(const LinLossParams& p, const LinLossPlan& plan, hipStream_t stream);
+hipError_t launch_linloss_rescale(const LinLossParams& p, hipStream_t stream);
 hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, hipStream_t stream);
 
 struct DistillParams {

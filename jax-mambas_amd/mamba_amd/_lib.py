@@ -78,6 +78,8 @@ EXPORTED_SYMBOLS = (
     "mss_linear_loss_workspace_bytes",
     "mss_linear_loss_fwd",
     "mss_linear_loss_bwd",
+    "mss_linear_loss_fwd_grad",
+    "mss_linear_loss_rescale",
     "mss_distill_saved_bytes",
     "mss_distill_fwd",
     "mss_distill_bwd",
@@ -380,7 +382,7 @@ def register_hip_kernel(library_path=None):
                        ("mss_sample", SampleArgs)):
         getattr(lib, name).argtypes = [ctypes.POINTER(args), _p]
         getattr(lib, name).restype = ctypes.c_int
-    for name in ("mss_linear_loss_fwd", "mss_linear_loss_bwd"):
+    for name in ("mss_linear_loss_fwd", "mss_linear_loss_bwd", "mss_linear_loss_fwd_grad", "mss_linear_loss_rescale"):
         getattr(lib, name).argtypes = [ctypes.POINTER(LinearLossArgs), _p]
         getattr(lib, name).restype = ctypes.c_int
     for name in ("mss_distill_fwd", "mss_distill_bwd", "mss_distill_fwd_grad", "mss_distill_regrad"):

@@ -45,6 +45,7 @@ __all__ = ["linear_cross_entropy", "linear_distill_loss", "distill_loss"]
 _F32, _I64 = torch.float32, torch.int64
 _REDUCTIONS = {"none": _lib.MSS_LOSS_NONE, "sum": _lib.MSS_LOSS_SUM, "mean": _lib.MSS_LOSS_MEAN}
 _MAX_ENTRIES = 1 << 27
+_MAX_ROWS = 1 << 21
 
 
 def _reduction(name):
@@ -90,9 +91,12 @@ def _upstream(grad, reduction, rows):
 
 
 class _LinearLoss(torch.autograd.Function):
+    """Where the loss is reduced and both gradients are wanted, large heads' come with it, for an upstream gradient of
+    1: the logits are formed once. The backward pass multiplies them by another one; a second one makes its own."""
+
     @staticmethod
     def forward(ctx, x, weight, weight_act, targets, ids, teacher, ignore_index, temperature, reduction, teacher_tag,
-                holder):
+                holder, both):
         lib = _lib.register_hip_kernel()
         f, t = x.shape
         w = weight_act
@@ -106,12 +110,19 @@ class _LinearLoss(torch.autograd.Function):
         dev = x.device
         with _guard(x):
             saved = _bytes(lib.mss_linear_loss_saved_bytes(a), dev)
-            ws = _bytes(lib.mss_linear_loss_workspace_bytes(a, 0), dev)
+            need = lib.mss_linear_loss_workspace_bytes(a, 2) if both else 0
+            name = "mss_linear_loss_fwd_grad" if need else "mss_linear_loss_fwd"
+            ws = _bytes(need or lib.mss_linear_loss_workspace_bytes(a, 0), dev)
+            ctx.d = None
+            if need:
+                dx, dw = torch.empty(f, t, dtype=x.dtype, device=dev), torch.empty(w.shape, dtype=weight.dtype, device=dev)
+                a.dx, a.dweight, a.dw_dtype = dx.data_ptr(), dw.data_ptr(), _io_tag(weight.dtype, "weight")
+                ctx.d = dx, dw
             loss = torch.empty(t, dtype=_F32, device=dev)
             mean = torch.empty((), dtype=_F32, device=dev)
             a.loss, a.mean, a.saved, a.saved_bytes = loss.data_ptr(), mean.data_ptr(), saved.data_ptr(), saved.numel()
             a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-            _lib.check(lib.mss_linear_loss_fwd(a, _stream(x)), "mss_linear_loss_fwd")
+            _lib.check(getattr(lib, name)(a, _stream(x)), name)
         ctx.save_for_backward(w, saved)
         ctx.args = a
         ctx.x_like = (x.dtype, (f, t))
@@ -124,7 +135,7 @@ class _LinearLoss(torch.autograd.Function):
     def backward(ctx, grad):
         need_x, need_w = ctx.needs_input_grad[:2]
         if grad is None or not (need_x or need_w):
-            return (None,) * 11
+            return (None,) * 12
         lib = _lib.register_hip_kernel()
         w, saved = ctx.saved_tensors
         src = ctx.args
@@ -132,20 +143,27 @@ class _LinearLoss(torch.autograd.Function):
         dev = w.device
         with _guard(w):
             grad = _upstream(grad, src.reduction, src.tokens)
-            dx = torch.empty(shape, dtype=dtype, device=dev) if need_x else None
-            dw = torch.empty(w.shape, dtype=ctx.dw_dtype, device=dev) if need_w else None
             a = _lib.LinearLossArgs.from_buffer_copy(src)
             a.x = a.loss = a.mean = a.targets = a.ids = a.teacher = None
             a.weight = w.data_ptr()
-            ws = _bytes(lib.mss_linear_loss_workspace_bytes(a, 1), dev)
-            a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
             a.dw_dtype = _io_tag(ctx.dw_dtype, "weight")
+            d, ctx.d = ctx.d, None  # the caller may write over them
+            if d is not None:
+                dx, dw = d
+                name = "mss_linear_loss_rescale"
+            else:
+                dx = torch.empty(shape, dtype=dtype, device=dev) if need_x else None
+                dw = torch.empty(w.shape, dtype=ctx.dw_dtype, device=dev) if need_w else None
+                ws = _bytes(lib.mss_linear_loss_workspace_bytes(a, 1), dev)
+                a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+                name = "mss_linear_loss_bwd"
             a.grad, a.dx, a.dweight = grad.data_ptr(), _ptr(dx), _ptr(dw)
-            _lib.check(lib.mss_linear_loss_bwd(a, _stream(w)), "mss_linear_loss_bwd")
+            _lib.check(getattr(lib, name)(a, _stream(w)), name)
+            dx, dw = dx if need_x else None, dw if need_w else None
         if dw is not None and ctx.holder is not None:
             ctx.holder.put(dw)
             dw = None
-        return (dx, dw) + (None,) * 9
+        return (dx, dw) + (None,) * 10
 
 
 def _linear_loss(x, weight, weight_act, holder, targets, ids, teacher, ignore_index, temperature, reduction, teacher_tag):
@@ -176,8 +194,9 @@ def _linear_loss(x, weight, weight_act, holder, targets, ids, teacher, ignore_in
     if f > 1 and weight_act.stride(1) != 1 or vocab > 1 and weight_act.stride(0) < f:
         weight_act = weight_act.contiguous()
     conform = [None if v is None else _resolved(v).contiguous() for v in (targets, ids, teacher)]
+    both = reduction != _lib.MSS_LOSS_NONE and torch.is_grad_enabled() and x.requires_grad and weight.requires_grad
     return _LinearLoss.apply(_resolved(x), weight, weight_act, *conform, ignore_index, temperature, reduction, teacher_tag,
-                             holder)
+                             holder, both)
 
 
 def linear_cross_entropy(x, weight, targets, ignore_index=-100, reduction="mean", weight_act=None, holder=None):
@@ -249,6 +268,8 @@ def distill_loss(logits, ids, teacher, temperature=1.0, reduction="mean"):
     rows, vocab = logits.shape
     if vocab == 0:
         raise ValueError("logits have no words")
+    if rows > _MAX_ROWS:
+        raise ValueError(f"logits have at most {_MAX_ROWS} rows, got {rows}")
     tag = _check_lists(ids, teacher, rows, temperature)
     _require_gpu(logits, ids, teacher)
     if rows == 0 or ids.shape[1] == 0:

@@ -71,6 +71,40 @@ def test_linear_backward_validation(lib, kw, status):
     assert lib.mss_linear_loss_saved_bytes(None) == lib.mss_linear_loss_workspace_bytes(None, 1) == 0
 
 
+BIG = dict(LINEAR, tokens=4096, features=256, vocab=1 << 17, stride_f=4096, ldw=256, workspace_bytes=1 << 40)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(tokens=4), 2), (dict(io_dtype=0), 2), (dict(reduction=0), 2), (dict(x=None), 1), (dict(weight=None), 1),
+    (dict(targets=None), 1), (dict(loss=None), 1), (dict(mean=None), 1), (dict(dx=None), 1), (dict(dweight=None), 1),
+    (dict(dw_dtype=3), 1), (dict(workspace_bytes=1 << 20), 4), (dict(saved_bytes=100), 4), (dict(dx=P), 1), (dict(dx=12 * P), 1),
+    (dict(dweight=2 * P), 1), (dict(dweight=8 * P), 1), (dict(dx=9 * P), 1), (dict(loss=11 * P), 1),
+])
+def test_linear_both_validation(lib, kw, status):
+    assert lib.mss_linear_loss_fwd_grad(_lib.LinearLossArgs(**{**BIG, **kw}), None) == status
+    assert lib.mss_linear_loss_fwd_grad(None, None) == 1
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(tokens=4), 2), (dict(io_dtype=0), 2), (dict(reduction=0), 2), (dict(dx=None), 1), (dict(dweight=None), 1), (dict(grad=None), 1),
+    (dict(dw_dtype=3), 1), (dict(dx=10 * P), 1), (dict(dweight=11 * P), 1),
+])
+def test_linear_rescale_validation(lib, kw, status):
+    assert lib.mss_linear_loss_rescale(_lib.LinearLossArgs(**{**BIG, **kw}), None) == status
+    assert lib.mss_linear_loss_rescale(None, None) == 1
+
+
+def test_linear_workspaces(lib):
+    def sizes(**kw):
+        return [lib.mss_linear_loss_workspace_bytes(_lib.LinearLossArgs(**{**BIG, **kw}), i) for i in (-1, 0, 1, 2, 3)]
+    none, fwd, bwd, both, none2 = sizes()
+    assert none == none2 == 0 and 0 < fwd < bwd < both
+    assert sizes(io_dtype=0)[3] == sizes(reduction=0)[3] == sizes(tokens=4)[3] == 0
+    # A weight whose rows lie further apart than 32 bits address in a tile is copied.
+    saved = [lib.mss_linear_loss_saved_bytes(_lib.LinearLossArgs(**{**LINEAR, "ldw": ldw})) for ldw in (64, 1 << 22, (1 << 22) + 8)]
+    assert saved[0] == saved[1] and saved[2] >= saved[1] + 100 * 64 * 2
+
+
 DISTILL = dict(rows=20, vocab=100, top=5, io_dtype=1, teacher_dtype=0, reduction=2, temperature=1.0, ld=100, logits=P, ids=2 * P,
                teacher=3 * P, loss=4 * P, mean=5 * P, saved=6 * P, saved_bytes=1 << 31, grad=7 * P, dlogits=8 * P)
 
@@ -81,7 +115,7 @@ DISTILL = dict(rows=20, vocab=100, top=5, io_dtype=1, teacher_dtype=0, reduction
     (dict(logits=None), 1), (dict(ids=None), 1), (dict(teacher=None), 1), (dict(loss=None), 1), (dict(mean=None), 1),
     (dict(saved=None), 1), (dict(dlogits=None), 1), (dict(logits=P + 1), 1), (dict(dlogits=8 * P + 1), 1),
     (dict(reduction=0), 1), (dict(saved=6 * P + 4), 4), (dict(saved_bytes=64), 4), (dict(top=1025), 2),
-    (dict(rows=1 << 18, top=1000), 2), (dict(vocab=(1 << 30) + 1, ld=1 << 31), 2), (dict(dlogits=P + 256), 1),
+    (dict(rows=1 << 18, top=1000), 2), (dict(rows=(1 << 21) + 1, top=1), 2), (dict(vocab=(1 << 30) + 1, ld=1 << 31), 2), (dict(dlogits=P + 256), 1),
     (dict(loss=P), 1), (dict(saved=2 * P), 1), (dict(mean=4 * P), 1), (dict(dlogits=4 * P), 1), (dict(dlogits=6 * P), 1),
 ])
 def test_distill_validation(lib, kw, status):
@@ -138,6 +172,9 @@ def test_python_refusals():
             call()
     with pytest.raises(RuntimeError, match="detach"):
         ds(z, ids, te.requires_grad_())
+    rows = (1 << 21) + 1
+    with pytest.raises(ValueError, match="rows"):
+        ds(torch.zeros(1, 1).expand(rows, 1), torch.zeros(1, 1, dtype=torch.int64).expand(rows, 1), torch.zeros(1, 1).expand(rows, 1))
 
 
 # ------------------------------------------------------------------------------- the definitions
@@ -344,9 +381,150 @@ def test_linear_cross_entropy_many_tiles(dtype, t, d, v):
         g, g_tol = ref.g * by, ref.g_tol * by
         dw_want = dw_want + torch.mm(g.t(), xd.t())
         dw_tol = dw_tol + _product_tol(g_tol.t(), g.t(), xd.t(), t)
+        if dtype == BF16 and t * d * v >= 2 ** 35:
+            # (Both directions at once, as below: a term is bf16(e) bf16(x / S) for e x / S, so that each has another
+            # (1 + 2^-8) from the second rounding.)
+            dw_tol = dw_tol + HALF[BF16] * torch.mm((g.abs() + g_tol).t(), xd.abs().t())
     _check("loss", loss, total, losses + 2 * U * total)
     half = HALF[dtype]
     _check("dw", dw, dw_want, (dw_tol + 8 * U * dw_want.abs()) * (1 + half) + half * dw_want.abs())
+
+
+def _check_both(x, w, q, live, temperature, k, reduction, up, loss, dx, dw):
+    """In pieces of the tokens. The division of x's rows by their sums rounds them to bfloat16 once more, which dw has
+    2^-8 of its terms' magnitudes from; an upstream gradient that is not a power of two rounds dx and dw once more."""
+    t, n = x.shape[1], 1024
+    by = (1.0 / int(live.sum()) if reduction == "mean" else 1.0)
+    total, tol, dw_want, dw_tol = 0.0, 0.0, 0.0, 0.0
+    more = 0.0 if abs(np.log2(abs(up))) % 1 == 0 else 1.0
+    for a in range(0, t, n):
+        part = slice(a, min(t, a + n))
+        ref, xd, wd = _linear_reference(x.detach()[:, part], w, q(part), live[part], temperature, k)
+        total, tol = total + ref.loss.sum() * by, tol + ref.loss_tol.sum() * by
+        g, g_tol = ref.g * by * up, ref.g_tol * by * abs(up)
+        if dx is not None:
+            want = torch.mm(g, wd).t()
+            bound = _product_tol(g_tol, g, wd, g.shape[1]).t() + 8 * U * want.abs()
+            half = HALF[x.dtype] * (1 + more)
+            _check("dx", dx[:, part], want, bound * (1 + 2 * half) + half * want.abs())
+        if dw is not None:
+            dw_want = dw_want + torch.mm(g.t(), xd.t())
+            dw_tol = dw_tol + _product_tol(g_tol.t(), g.t(), xd.t(), t) + HALF[BF16] * torch.mm((g.abs() + g_tol).t(), xd.abs().t())
+    _check("loss", loss, total, tol + 2 * U * total.abs())
+    if dw is not None:
+        half = HALF[dw.dtype] * (1 + more)
+        _check("dw", dw, dw_want, (dw_tol + 8 * U * dw_want.abs()) * (1 + 2 * half) + half * dw_want.abs())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,d,v,layout,top,temperature,reduction,up,w_dtype", [
+    (2048, 320, 53000, "cm", 0, 1.0, "mean", 1.0, BF16), (10500, 64, 53000, "tm", 0, 1.0, "sum", 0.25, F32),
+    (1100, 640, 50001, "cm", 5, 2.0, "mean", -0.7, F32), (513, 1300, 52001, "gap", 0, 1.0, "mean", 1.0, BF16),
+    (4100, 40, 212345, "tm", 1, 0.5, "sum", 1.0, BF16)])
+def test_linear_both_directions_at_once(t, d, v, layout, top, temperature, reduction, up, w_dtype):
+    """Large heads, whose gradients come with the loss; tokens in more than one block (the second and the last), and the
+    gradients of a second pass, which come without it."""
+    print(f"case both {t} {d} {v} {layout} {top} {temperature} {reduction} {up} {w_dtype}", flush=True)
+    x, w = _inputs(t, d, v, BF16, t + v, layout)
+    x = x.clone(memory_format=torch.preserve_format) if layout == "gap" else x
+    if top:
+        ids, te = _lists(t, v, top, F32, t) if v < 100000 else (_targets(t, v, 0.1, t)[:, None], torch.randn(t, 1, device="cuda"))
+        live = ((ids >= 0) & (te != -torch.inf)).any(1)
+        q = lambda part: _wanted_lists(ids[part], te[part], temperature, v)[0]
+    else:
+        targets = _targets(t, v, 0.1, t)
+        live = targets != -100
+        q = lambda part: _wanted_targets(targets[part], v)[0]
+    x[:, ~live] = float("nan")
+    x.requires_grad_(True)
+    leaf = w.detach().to(w_dtype).requires_grad_(True)
+    run = lambda: (linear_distill_loss(x, leaf, ids, te, temperature, reduction) if top else
+                   linear_cross_entropy(x, leaf, targets, reduction=reduction))
+    loss = run()
+    upstream = torch.tensor(up, device="cuda")
+    dx, dw = torch.autograd.grad(loss, (x, leaf), upstream, retain_graph=True)
+    assert dw.dtype == w_dtype and dx.shape == x.shape
+    _check_both(x, w, q, live, temperature, max(1, top), reduction, up, loss, dx, dw)
+    dx2, dw2 = torch.autograd.grad(loss, (x, leaf), upstream)
+    assert dx2.data_ptr() != dx.data_ptr() and dw2.data_ptr() != dw.data_ptr()
+    _check_both(x, w, q, live, temperature, max(1, top), reduction, up, loss, dx2, dw2)
+    (dx3,) = torch.autograd.grad(run(), (x,), upstream)
+    assert torch.equal(dx3, dx)
+
+
+@pytest.mark.gpu
+def test_linear_both_directions_far_from_the_target():
+    """Tokens whose word is too far below the largest logit: as the two directions apart, to the bit, also where a
+    captured run is replayed with such tokens and without."""
+    t, d, v = 1024, 640, 53000
+    print(f"case far {t} {d} {v}", flush=True)
+    near, w = _inputs(t, d, v, BF16, 7)
+    w.requires_grad_(True)
+    targets = _targets(t, v, 0.1, 8)
+    far, broken = near.clone(), near.clone()
+    far[:, [5, 700]] *= 32
+    broken[3, 9] = float("inf")
+    targets[[5, 700, 9]] = 11
+
+    def run(x):
+        x = x.detach().requires_grad_(True)
+        loss = linear_cross_entropy(x, w, targets)
+        return (loss.detach(), *torch.autograd.grad(loss, (x, w)))
+
+    def apart(x):
+        x = x.detach().requires_grad_(True)
+        loss = linear_cross_entropy(x, w, targets)
+        torch.autograd.grad(loss, (x, w), retain_graph=True)
+        with torch.no_grad():
+            forward = linear_cross_entropy(x, w, targets)
+        return (forward, *torch.autograd.grad(loss, (x, w)))
+
+    want = {}
+    for name, x in (("far", far), ("near", near), ("broken", broken)):
+        got, two = run(x), apart(x)
+        if name != "near":
+            for a, b in zip(got, two):
+                assert torch.equal(a.nan_to_num(12345.0), b.nan_to_num(12345.0)), name
+        want[name] = got
+    q, live = _wanted_targets(targets, v)
+    _check_both(far, w.detach(), lambda part: q[part], live, 1.0, 1, "mean", 1.0, *want["far"])
+    assert not torch.isfinite(want["broken"][0])
+
+    x = near.clone().requires_grad_(True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        loss = linear_cross_entropy(x, w, targets)
+        torch.autograd.grad(loss, (x, w))
+        del loss
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = linear_cross_entropy(x, w, targets)
+        dx, dw = torch.autograd.grad(loss, (x, w))
+    for name, given in (("near", near), ("far", far), ("near", near), ("broken", broken), ("far", far), ("near", near)):
+        with torch.no_grad():
+            x.copy_(given)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip((loss.detach(), dx, dw), want[name]):
+            assert torch.equal(a.nan_to_num(12345.0), b.nan_to_num(12345.0)), name
+
+
+@pytest.mark.gpu
+def test_weight_rows_far_apart():
+    t, d, v = 300, 64, 300
+    x, w = _inputs(t, d, v, BF16, 1)
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    targets = _targets(t, v, 0.1, 1)
+    a = linear_cross_entropy(x, w, targets)
+    wide = torch.empty_strided((v, d), ((1 << 22) + 8, 1), dtype=BF16, device="cuda")
+    wide.copy_(w.detach())
+    b = linear_cross_entropy(x, w, targets, weight_act=wide)
+    assert torch.equal(a, b)
+    for one, two in zip(torch.autograd.grad(a, (x, w)), torch.autograd.grad(b, (x, w))):
+        assert torch.equal(one, two)
 
 
 @pytest.mark.gpu
