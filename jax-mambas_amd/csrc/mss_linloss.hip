@@ -232,6 +232,9 @@ __device__ __forceinline__ float quad_mov(float v) {
 template <int kMode, bool kF32, int kMT, int kNT>
 __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT], int wm0, int wn0, int part, int lane,
                                        const float2* table) {
+  // (What is made of the lane's number is made anew for each tile; kept from one to the next it costs the
+  // registers of a copy's offset, whose reload waits for the stores.)
+  asm volatile("" : "+v"(lane));
   const int j = lane & 31, g = lane >> 5;
   // (from a split product's sums to a logit to base 2)
   [[maybe_unused]] const float c = kF32 && !kLlTeams<kMode> ? ldexpf(o.c, -(o.powers[0] + o.powers[1])) : o.c;
