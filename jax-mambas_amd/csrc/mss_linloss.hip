@@ -141,7 +141,7 @@ struct LlArgs {
   int tiles_m, tiles_n;
   int units;             // of a tile: kRing stages each
   int teams;             // of the gradients' products
-  int whole;             // ranges of a team; 0: the teams share all units evenly
+  int whole, rest;       // whole ranges of a team; the first range of those whose units the teams share evenly
   float* partial;        // their tiles' parts
 };
 
@@ -468,9 +468,9 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT],
 // XCD has workgroups.
 //
 // kModeDx, kModeDw: the tiles of one range of tokens (words) are taken by a team of as many workgroups as there
-// are tiles of features, side by side, so that g is read once. A team has a number of whole ranges, or the teams
-// share the units of all ranges evenly, in order: a team's first and last range may be a part of one then, whose
-// sums go to `partial` and are added in order by ll_join_kernel.
+// are tiles of features, side by side, so that g is read once. A team has a number of whole ranges, and the teams
+// share evenly the units of the fewer than a range for each that are left, in order: a part of one range, or the end of
+// one and the beginning of the next, whose sums go to `partial` and are added in order by ll_join_kernel.
 struct LlSegment {
   int tm, tn, unit, n;  // the tile, its first unit, units: none at the end
 };
@@ -478,14 +478,11 @@ struct LlSegment {
 struct LlDeal {
   int first, step, end;       // whole tiles
   int team, member;           // teams
-  long long from, to;         // units
+  long long from, to;         // units of the shared ranges
 };
 
-__device__ __forceinline__ long long team_start(const LlArgs& p, long long units, int team) {
-  if (p.whole == 0) return units * team / p.teams;
-  const long long at = static_cast<long long>(team) * p.whole * p.units;
-  return at < units ? at : units;
-}
+// Where a team's share of the `units` of the shared ranges begins.
+__device__ __forceinline__ long long share_start(const LlArgs& p, long long units, int team) { return units * team / p.teams; }
 
 template <int kMode>
 __device__ __forceinline__ LlDeal ll_deal(const LlArgs& p) {
@@ -495,11 +492,11 @@ __device__ __forceinline__ LlDeal ll_deal(const LlArgs& p) {
     const int size = kMode == kModeDx ? p.tiles_m : p.tiles_n;
     const unsigned id = x * per + min(x, rem) + blockIdx.x / 8;
     const int team = id / size;
-    const long long units = static_cast<long long>(kMode == kModeDx ? p.tiles_n : p.tiles_m) * p.units;
+    const long long units = static_cast<long long>((kMode == kModeDx ? p.tiles_n : p.tiles_m) - p.rest) * p.units;
     d.team = team;
     d.member = id % size;
-    d.from = team_start(p, units, team);
-    d.to = team_start(p, units, team + 1);
+    d.from = share_start(p, units, team);
+    d.to = share_start(p, units, team + 1);
   } else {
     const long long tiles = static_cast<long long>(p.tiles_m) * p.tiles_n;
     const long long before = x * per + min(x, rem);  // workgroups of the XCDs before this one
@@ -514,13 +511,19 @@ template <int kMode>
 __device__ __forceinline__ LlSegment ll_segment(const LlArgs& p, const LlDeal& d, int i) {
   LlSegment s{};
   if constexpr (kLlTeams<kMode>) {
-    const int range = static_cast<int>(d.from / p.units) + i;
-    const long long begin = static_cast<long long>(range) * p.units;
-    const long long a = d.from > begin ? d.from : begin, b = d.to < begin + p.units ? d.to : begin + p.units;
+    int range = d.team * p.whole + i;
+    if (i < p.whole) {
+      s.n = range < p.rest ? p.units : 0;
+    } else {
+      const int shared = static_cast<int>(d.from / p.units) + i - p.whole;
+      const long long begin = static_cast<long long>(shared) * p.units;
+      const long long a = d.from > begin ? d.from : begin, b = d.to < begin + p.units ? d.to : begin + p.units;
+      range = p.rest + shared;
+      s.unit = static_cast<int>(a - begin);
+      s.n = a < b ? static_cast<int>(b - a) : 0;
+    }
     s.tm = kMode == kModeDx ? d.member : range;
     s.tn = kMode == kModeDx ? range : d.member;
-    s.unit = static_cast<int>(a - begin);
-    s.n = a < b ? static_cast<int>(b - a) : 0;
   } else {
     const int id = d.first + i * d.step;
     if (id >= d.end) return s;
@@ -533,7 +536,7 @@ __device__ __forceinline__ LlSegment ll_segment(const LlArgs& p, const LlDeal& d
   return s;
 }
 
-// The sums of a part: of a team's first range (which = 0) or its last.
+// The sums of a part: of a team's first shared range (which = 0) or its second.
 template <class S, int kMode>
 __device__ __forceinline__ f32x4* ll_part(const LlArgs& p, int team, int which, int member) {
   const int size = kMode == kModeDx ? p.tiles_m : p.tiles_n;
@@ -714,7 +717,7 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
     if constexpr (kLlTeams<kMode>) {
       if (seg.n < p.units) {
         // A part: its sums, in the order in which the lanes hold them.
-        f32x4* dst = ll_part<S, kMode>(p, deal.team, i > 0, deal.member) + wave * (S::kSums / 4 * 64) + lane;
+        f32x4* dst = ll_part<S, kMode>(p, deal.team, i > p.whole, deal.member) + wave * (S::kSums / 4 * 64) + lane;
 #pragma unroll
         for (int e = 0; e < S::kSums / 4; ++e)
           dst[64 * e] = f32x4{acc[e / 4 / S::kNT][e / 4 % S::kNT][4 * (e % 4)], acc[e / 4 / S::kNT][e / 4 % S::kNT][4 * (e % 4) + 1],
@@ -735,7 +738,7 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
 #endif
 }
 
-// The tiles of which teams have parts: the parts' sums, in a fixed order. A workgroup for each row of matrix tiles of a
+// The tiles of the shared ranges: the parts' sums, in a fixed order. A workgroup for each row of matrix tiles of a
 // wave, whose four waves take every fourth part.
 constexpr int kJoinWaves = 4;
 
@@ -746,23 +749,23 @@ __global__ __launch_bounds__(64 * kJoinWaves) void ll_join_kernel(LlArgs p, LlOu
   const int lane = threadIdx.x & 63, mine = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int size = kMode == kModeDx ? p.tiles_m : p.tiles_n, ranges = kMode == kModeDx ? p.tiles_n : p.tiles_m;
   const int mt = blockIdx.x % S::kMT, wave = blockIdx.x / S::kMT % S::kWaves;
-  const int tile = blockIdx.x / (S::kMT * S::kWaves), range = tile / size, member = tile % size;
-  const long long units = static_cast<long long>(ranges) * p.units, begin = static_cast<long long>(range) * p.units;
+  const int tile = blockIdx.x / (S::kMT * S::kWaves), shared = tile / size, member = tile % size, range = p.rest + shared;
+  const long long units = static_cast<long long>(ranges - p.rest) * p.units, begin = static_cast<long long>(shared) * p.units;
   int team = static_cast<int>(begin * p.teams / units);  // the one with the range's first unit
-  while (team > 0 && team_start(p, units, team) > begin) --team;
-  while (team_start(p, units, team + 1) <= begin) ++team;
-  if (team_start(p, units, team + 1) >= begin + p.units) return;  // a whole one
+  while (team > 0 && share_start(p, units, team) > begin) --team;
+  while (share_start(p, units, team + 1) <= begin) ++team;
   lf32x16 acc[1][S::kNT];
 #pragma unroll
   for (int b = 0; b < S::kNT; ++b)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[0][b][e] = 0.f;
   int end = static_cast<int>((begin + p.units) * p.teams / units);  // the first team behind the range
-  while (end > 0 && team_start(p, units, end - 1) >= begin + p.units) --end;
-  while (end < p.teams && team_start(p, units, end) < begin + p.units) ++end;
+  while (end > 0 && share_start(p, units, end - 1) >= begin + p.units) --end;
+  while (end < p.teams && share_start(p, units, end) < begin + p.units) ++end;
 #pragma unroll 2
-  for (team += mine; team < end; team += kJoinWaves) {  // (every team has at least a unit)
-    const f32x4* src = ll_part<S, kMode>(p, team, team_start(p, units, team) / p.units != range, member) +
+  for (team += mine; team < end; team += kJoinWaves) {
+    if (share_start(p, units, team) == share_start(p, units, team + 1)) continue;  // (fewer units than teams)
+    const f32x4* src = ll_part<S, kMode>(p, team, share_start(p, units, team) / p.units != shared, member) +
                        wave * (S::kSums / 4 * 64) + mt * (S::kNT * 4 * 64) + lane;
 #pragma unroll
     for (int e = 0; e < 4 * S::kNT; ++e) {
@@ -1255,10 +1258,12 @@ typedef LlShape<2, 2, 2, 2, 2> LlSmall;    // 128 x 128, waves of 64 x 64
 typedef LlShape<4, 1, 1, 1, 4> LlThinN;    // 128 x 32, waves of 32 x 32
 typedef LlShape<1, 4, 1, 1, 4> LlThinM;    // 32 x 128
 
-// Teams of `size` workgroups for `ranges` ranges of `units`. Whole ranges where the last team is not waited for
-// longer than a part costs to write and to read again (kPart units); else even shares, of at least that much.
+// Teams of `size` workgroups for `ranges` ranges of `units`. Only whole ranges where the last team is not waited for
+// longer than a part costs to write and to read again (kPart units); else what is left of them in even shares, a team
+// having at least that much in all. (With all ranges shared, two parts a team instead of one, the weight's gradient of
+// 8192 x 768 x 50280 took 573 us and 69 us to join, so 557 and 22.)
 struct LlTeams {
-  int teams, whole;
+  int teams, whole, rest;
 };
 
 template <class S>
@@ -1271,8 +1276,9 @@ LlTeams ll_teams(int size, int ranges, int units) {
   long long shares = all / kPart < n ? all / kPart : n;
   shares = shares < 1 ? 1 : shares;
   if (each * units <= all / shares + kPart)
-    return {static_cast<int>((ranges + each - 1) / each), static_cast<int>(each)};
-  return {static_cast<int>(shares), 0};
+    return {static_cast<int>((ranges + each - 1) / each), static_cast<int>(each), ranges};
+  const int teams = static_cast<int>(shares), whole = ranges / teams;
+  return {teams, whole, whole * teams};
 }
 
 template <class S, int kMode, bool kF32 = false>
@@ -1288,10 +1294,12 @@ void launch_product(LlArgs a, const LlOut& o, hipStream_t stream) {
     const LlTeams t = ll_teams<S>(size, kMode == kModeDx ? a.tiles_n : a.tiles_m, a.units);
     a.teams = t.teams;
     a.whole = t.whole;
+    a.rest = t.rest;
     hipLaunchKernelGGL((ll_kernel<S, kMode, kF32>), dim3(a.teams * size), dim3(S::kThreads), 0, stream, a, o);
-    if (a.whole == 0)
-      hipLaunchKernelGGL((ll_join_kernel<S, kMode, kF32>), dim3(static_cast<unsigned>(tiles * S::kWaves * S::kMT)), dim3(64 * kJoinWaves), 0,
-                         stream, a, o);
+    const int shared = (kMode == kModeDx ? a.tiles_n : a.tiles_m) - a.rest;
+    if (shared > 0)
+      hipLaunchKernelGGL((ll_join_kernel<S, kMode, kF32>), dim3(static_cast<unsigned>(shared) * size * S::kWaves * S::kMT),
+                         dim3(64 * kJoinWaves), 0, stream, a, o);
   } else {
     hipLaunchKernelGGL((ll_kernel<S, kMode, kF32>), dim3(static_cast<unsigned>(tiles < room ? tiles : room)), dim3(S::kThreads), 0,
                        stream, a, o);
@@ -1338,7 +1346,7 @@ long long part_sums(int features, int others, int stages) {
   const int units = (stages + S::kRing - 1) / S::kRing;
   const LlTeams x = ll_teams<S>(static_cast<int>(size_x), static_cast<int>(ranges_x), units);
   const LlTeams w = ll_teams<S>(static_cast<int>(size_w), static_cast<int>(ranges_w), units);
-  const long long nx = x.whole ? 0 : 2LL * x.teams * size_x, nw = w.whole ? 0 : 2LL * w.teams * size_w;
+  const long long nx = x.rest == ranges_x ? 0 : 2LL * x.teams * size_x, nw = w.rest == ranges_w ? 0 : 2LL * w.teams * size_w;
   return (nx > nw ? nx : nw) * S::kM * S::kN;
 }
 
