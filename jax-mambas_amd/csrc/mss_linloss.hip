@@ -1397,17 +1397,21 @@ LinLossPlan linloss_plan(int tokens, int features, int vocab, int planes) {
   q.ldg = q.piece;
   q.ldx = (tokens + 3) / 4 * 4;
   const int words = q.piece < vocab ? q.piece : vocab;
-  // The gradients' products are shared evenly, so that it is their padding that counts.
+  // The gradients' products are shared evenly, so that it is their padding that counts, and for dx of few tokens the
+  // parts, of which larger tiles have more (us with the join, large and small, x 768 x 50280: 128 tokens 48 and 37, 256
+  // tokens 50 and 45, 384 tokens 67 and 45, 512 tokens 56 and 57, 700 tokens 67 and 92).
   const auto large = [](int rows, int cols) { return 4. * tiles_of(rows, cols, 256, 256) <= 1.4 * tiles_of(rows, cols, 128, 128); };
-  q.shape_x = tokens <= 32 ? 2 : large(features, tokens) ? 1 : 0;
+  q.shape_x = tokens <= 32 ? 2 : tokens > 384 && large(features, tokens) ? 1 : 0;
   q.shape_w = large(words, features) ? 1 : 0;
   const int x_stages = q.piece / 64 * (planes == 1 ? 1 : kPairs);
   const int w_stages = (tokens + kLlK - 1) / kLlK * (kLlK / 64) * (planes == 1 ? 1 : kPairs);
   const long long x = with_shape(q.shape_x, kModeDx, [&](auto s) { return part_sums<decltype(s)>(features, tokens, x_stages); });
   const long long w = with_shape(q.shape_w, kModeDw, [&](auto s) { return part_sums<decltype(s)>(features, words, w_stages); });
   q.partial = x > w ? x : w;
-  // Both directions at once, where the logits' product is worth more than the launches that may not be needed.
-  q.both = planes == 1 && tokens >= 512 && static_cast<double>(tokens) * features * vocab >= 0x1p35;
+  // Both directions at once, where the logits' product is worth more than the launches that may not be needed (us of
+  // both, apart and at once: 2048 x 64 x 50280 234 and 274; 1024 x 256 x 50280 238 and 206; 512 x 768 x 50280 286 and
+  // 266; 2048 x 768 x 50280 748 and 645).
+  q.both = planes == 1 && tokens >= 512 && static_cast<double>(tokens) * features * vocab >= 0x1p33;
   if (q.both) {
     q.lde = whole;
     const long long rows = (1LL << 30) / (2 * q.lde) / 256 * 256, blocks = (tokens + rows - 1) / rows;
