@@ -220,8 +220,8 @@ __device__ __forceinline__ void split_half(float v, uint16_t& hi, uint16_t& lo) 
   lo = fabsf(left) < INFINITY ? __builtin_bit_cast(uint16_t, static_cast<_Float16>(left)) : 0;
 }
 
-// A value of another lane (kCtrl: 0xb1 of lane ^ 1, 0x4e of lane ^ 2, 0x141 of the mirror place in eight lanes, 0x140 in
-// sixteen).
+// A value of another lane (kCtrl: 0xb1 of lane ^ 1, 0x4e of lane ^ 2, 0x124 and 0x128 of 4 and 8 places back, around
+// sixteen lanes).
 template <int kCtrl>
 __device__ __forceinline__ float quad_mov(float v) {
   return dpp_mov<kCtrl, 0xF>(0.f, v);
@@ -272,7 +272,10 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT],
     const int v = wn0 + kNT * j;
     const uint32_t at = static_cast<uint32_t>(4 * g * o.ld + v) * 2;
     const float2* scale = table + 4 * g;
-    float mine[kMT];  // kModeExp: of the rows' sums over the wave's words, lane 16 + r has that of register r
+    // kModeExp: of the rows' sums over the wave's words, lane r of sixteen has that of register r. Four rows at a time:
+    // lanes exchange the sums of two rows for one's, then of two for one, lane % 4 of four; the other quads' are added.
+    float mine[kMT], four[4];
+    const bool odd = j & 1, high = j & 2;
     const auto rows = [&](auto edge) LL_INLINE {
 #pragma unroll
       for (int mt = 0; mt < kMT; ++mt)
@@ -284,19 +287,23 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT],
           float d[kNT];
 #pragma unroll
           for (int nt = 0; nt < kNT; ++nt) {
-            d[nt] = fast_exp2(__builtin_fmaf(acc[mt][nt][r], c, -sc.x)) * by;
+            d[nt] = fast_exp2(__builtin_fmaf(acc[mt][nt][r], c, -sc.x));
+            if constexpr (kMode == kModeGrad) d[nt] *= by;  // (kModeExp: sc.x is inf in a row that does not count)
             if (edge.value && v + nt >= o.cols) d[nt] = 0.f;
           }
           if constexpr (kMode == kModeExp) {
             float s = d[0];
 #pragma unroll
             for (int nt = 1; nt < kNT; ++nt) s += d[nt];
-            s += quad_mov<0xb1>(s);
-            s += quad_mov<0x4e>(s);
-            s += quad_mov<0x141>(s);               // of the other four of eight
-            s += quad_mov<0x140>(s);               // of the other eight of sixteen
-            s += dpp_mov<kRowBcast15, 0xa>(0.f, s);  // lanes 16 to 31: of both sixteens
-            mine[mt] = r == 0 || (lane & 15) == r ? s : mine[mt];
+            four[r & 3] = s;
+            if (r % 4 == 3) {
+              const float a = (odd ? four[1] : four[0]) + quad_mov<0xb1>(odd ? four[0] : four[1]);
+              const float b = (odd ? four[3] : four[2]) + quad_mov<0xb1>(odd ? four[2] : four[3]);
+              s = (high ? b : a) + quad_mov<0x4e>(high ? a : b);
+              s += quad_mov<0x124>(s);
+              s += quad_mov<0x128>(s);
+              mine[mt] = r == 3 || (lane & 12) == r - 3 ? s : mine[mt];
+            }
           }
           if (edge.value && t + 4 * g >= o.rows) continue;
           char* dst = reinterpret_cast<char*>(o.g + t * o.ld) + at;
@@ -322,7 +329,8 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT],
 #pragma unroll
       for (int mt = 0; mt < kMT; ++mt) {
         const int t = wm0 + 32 * mt + 8 * (i >> 2) + 4 * g + (i & 3);
-        if (j >= 16 && t < o.rows) o.row_sums[static_cast<long long>(part) * o.rows + t] = mine[mt];
+        mine[mt] += __shfl_xor(mine[mt], 16);
+        if (j < 16 && t < o.rows) o.row_sums[static_cast<long long>(part) * o.rows + t] = mine[mt];
       }
     }
     if (!whole) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the next tile counts a whole tile's stores)
@@ -1014,7 +1022,7 @@ __device__ __forceinline__ void ll_dots(const LinLossParams& p, const LossMatrix
 }
 
 // table (or NULL): what a token's exponentials are taken relative to, to base 2 (kModeExp), the largest logit of its
-// list's first four words; and whether it counts.
+// list's first four words; inf for one that does not count.
 template <bool kF32>
 __global__ __launch_bounds__(256) void ll_pick_kernel(LinLossParams p, LossMatrix w, float2* table) {
   const int lane = threadIdx.x & 63;
@@ -1037,7 +1045,7 @@ __global__ __launch_bounds__(256) void ll_pick_kernel(LinLossParams p, LossMatri
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (word[e] >= 0) ref = fmaxf(ref, sum[e]);
-    table[t] = make_float2(fabsf(ref) < INFINITY ? ref * p.c : 0.f, p.r.live[t] == 0.f ? 0.f : 1.f);
+    table[t].x = p.r.live[t] == 0.f ? INFINITY : fabsf(ref) < INFINITY ? ref * p.c : 0.f;
   }
 }
 
