@@ -1416,10 +1416,10 @@ LinLossPlan linloss_plan(int tokens, int features, int vocab, int planes) {
   const long long x = with_shape(q.shape_x, kModeDx, [&](auto s) { return part_sums<decltype(s)>(features, tokens, x_stages); });
   const long long w = with_shape(q.shape_w, kModeDw, [&](auto s) { return part_sums<decltype(s)>(features, words, w_stages); });
   q.partial = x > w ? x : w;
-  // Both directions at once, where the logits' product is worth more than the launches that may not be needed (us of
-  // both, apart and at once: 2048 x 64 x 50280 234 and 274; 1024 x 256 x 50280 238 and 206; 512 x 768 x 50280 286 and
-  // 266; 2048 x 768 x 50280 748 and 645).
-  q.both = planes == 1 && tokens >= 512 && static_cast<double>(tokens) * features * vocab >= 0x1p33;
+  // Both directions at once, where the logits' product is worth more than x's rows divided and the launches that may not
+  // be needed (us of both, apart and at once: 2048 x 64 x 50280 234 and 274; 32768 x 128 x 4200 365 and 388; 65536 x 64 x
+  // 8200 1093 and 1148; 512 x 768 x 50280 286 and 266; 16384 x 64 x 16500 574 and 562; 2048 x 768 x 50280 748 and 645).
+  q.both = planes == 1 && tokens >= 512 && vocab >= 16384 && static_cast<double>(tokens) * features * vocab >= 0x1p34;
   if (q.both) {
     q.lde = whole;
     const long long rows = (1LL << 30) / (2 * q.lde) / 256 * 256, blocks = (tokens + rows - 1) / rows;
