@@ -734,7 +734,7 @@ int mss_sample(const mss_sample_args* args, void* stream);
  * mss_linear_loss_workspace_bytes for the forward call (which 0), the backward call (1) and
  * mss_linear_loss_fwd_grad (2), 256-byte aligned, nothing kept in it.
  * mss_linear_loss_fwd_grad is both directions at once, dx and dweight for an upstream gradient of 1: the logits are
- * formed once, and the rows of x rounded to bf16 once more, divided by their sum over the vocabulary. Where it is not
+ * formed once, and kept in 16 bits, to 2^-10 of a probability, until its gradient takes their place. Where it is not
  * offered (MSS_F32, MSS_LOSS_NONE, small heads) its workspace takes 0 bytes and the call returns MSS_ERR_UNSUPPORTED.
  * mss_linear_loss_rescale then multiplies dx and dweight by *grad, rounding them once more, unless that is 1.
  *

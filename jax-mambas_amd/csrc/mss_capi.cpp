@@ -1718,9 +1718,7 @@ int linear_loss_sizes(const mss_linear_loss_args* a, int which, mss::LinLossPara
       q.partial = f.take<float>(both && plan->partial_both > plan->partial ? plan->partial_both : plan->partial);
     }
     if (both) {
-      q.factor = f.take<float>(plan->block);
       q.row_sums = f.take<float>(static_cast<long long>(plan->parts_both) * plan->block);
-      q.xs = f.take<mss::bf16_t>(static_cast<long long>(plan->block) * p->width);
       if (plan->block < a->tokens) q.dw_sum = f.take<float>(static_cast<long long>(a->vocab) * a->features);
       q.bad = f.take<int>(1);
     }

@@ -145,6 +145,10 @@ struct LlArgs {
   float* partial;        // their tiles' parts
 };
 
+// kModeExp leaves s - ref, both to base 2, in steps of 2^-9 from -48 on: 0 to 65535 as a part of 65535, and 0 also below.
+constexpr float kFixedStep = 0x1p-9f, kFixedLow = -48.f, kFixedUnit = 1.f / (65535.f * kFixedStep);
+typedef unsigned short ll_u16x2 __attribute__((ext_vector_type(2)));
+
 enum { kModeLse, kModeGrad, kModeExp, kModeDx, kModeDw };
 
 // What all tokens' gradients are scaled by.
@@ -189,7 +193,7 @@ struct LlOut {
   void* dx;              // kModeDx with the last piece: [rows][ld_dx]
   long long ld_dx;
   int dx_bf16;
-  const float* live;     // and what each column is taken times where that is not 0 (with kModeExp's g)
+  const float* live;
   float* row_sums;       // kModeExp: [part][rows]
   float* sum;            // kModeDw in blocks of the tokens: [rows][ld], added to where `add`; the last one writes dw
   int last;
@@ -285,11 +289,16 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT],
           const float2 sc = scale[up];
           const float by = kF32 ? sc.y * kGradScale : sc.y;
           float d[kNT];
+          [[maybe_unused]] float fixed[kNT];
 #pragma unroll
           for (int nt = 0; nt < kNT; ++nt) {
             d[nt] = fast_exp2(__builtin_fmaf(acc[mt][nt][r], c, -sc.x));
             if constexpr (kMode == kModeGrad) d[nt] *= by;  // (kModeExp: sc.x is inf in a row that does not count)
             if (edge.value && v + nt >= o.cols) d[nt] = 0.f;
+            if constexpr (kMode == kModeExp) {
+              fixed[nt] = __builtin_fmaf(acc[mt][nt][r], c * kFixedUnit, sc.y);
+              if (edge.value && v + nt >= o.cols) fixed[nt] = 0.f;
+            }
           }
           if constexpr (kMode == kModeExp) {
             float s = d[0];
@@ -307,7 +316,12 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT],
           }
           if (edge.value && t + 4 * g >= o.rows) continue;
           char* dst = reinterpret_cast<char*>(o.g + t * o.ld) + at;
-          if constexpr (kF32) {
+          if constexpr (kMode == kModeExp) {
+            ll_u16x2 w[kNT / 2];
+#pragma unroll
+            for (int h = 0; h < kNT / 2; ++h) w[h] = __builtin_amdgcn_cvt_pknorm_u16(fixed[2 * h], fixed[2 * h + 1]);
+            __builtin_memcpy(dst, w, 2 * kNT);
+          } else if constexpr (kF32) {
             uint16_t hi[kNT], lo[kNT];
 #pragma unroll
             for (int nt = 0; nt < kNT; ++nt) split_half(d[nt], hi[nt], lo[nt]);
@@ -344,11 +358,11 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT],
     const long long at_dx = 4LL * g * o.ld_dx + t;
     static_assert(kNT <= 2, "the last lane has one token or all");
     const bool all = t + kNT <= o.cols;
-    float counts[kNT];
+    bool counts[kNT];
     const LlFactor<kF32> by(last ? o.by : LlScale{nullptr, nullptr, 1.f, o.powers, nullptr});
     if (last) {
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt) counts[nt] = t + nt < o.cols ? o.live[t + nt] : 0.f;
+      for (int nt = 0; nt < kNT; ++nt) counts[nt] = t + nt < o.cols && o.live[t + nt] != 0.f;
     }
 #pragma unroll
     for (int mt = 0; mt < kMT; ++mt)
@@ -370,7 +384,7 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT],
             continue;
           }
 #pragma unroll
-          for (int nt = 0; nt < kNT; ++nt) v[r][nt] = counts[nt] != 0.f ? by(v[r][nt]) * counts[nt] : 0.f;
+          for (int nt = 0; nt < kNT; ++nt) v[r][nt] = counts[nt] ? by(v[r][nt]) : 0.f;
           const long long to = (d + r) * o.ld_dx + at_dx;
           if (o.dx_bf16) {
             uint32_t u[(kNT + 1) / 2];
@@ -1045,7 +1059,8 @@ __global__ __launch_bounds__(256) void ll_pick_kernel(LinLossParams p, LossMatri
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (word[e] >= 0) ref = fmaxf(ref, sum[e]);
-    table[t].x = p.r.live[t] == 0.f ? INFINITY : fabsf(ref) < INFINITY ? ref * p.c : 0.f;
+    ref = p.r.live[t] == 0.f ? INFINITY : fabsf(ref) < INFINITY ? ref * p.c : 0.f;
+    table[t] = make_float2(ref, (-kFixedLow - ref) * kFixedUnit);
   }
 }
 
@@ -1130,19 +1145,18 @@ __global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_finish_kerne
 }
 
 // ------------------------------------------------------------------------- both directions at once
-// For a block of tokens and the whole vocabulary at a time, kModeExp leaves e = 2^(s - ref) in bf16, with ref a logit of
-// the token's own list, and its sums S: then lse = ref + log S, softmax = e / S, and g = (e - S q) / S. The division goes
-// to the rows of x for dw, and to dx's columns, so that the logits are formed once, not twice. It fails where S is
-// outside 2^-100 .. 2^100 (a list's words 69 below the largest logit, or above it): such a row is noted in `bad`, and the
-// two-pass kernels, launched behind, do everything anew; else they return at once.
+// For a block of tokens and the whole vocabulary at a time, kModeExp leaves the words' s - ref in 16 bits, with ref a logit of
+// the token's own list, and the sums S of 2^(s - ref); then lse = ref + log S, and g = 2^(s - lse) - q, rounded to bf16,
+// takes their place: the logits are formed once, not twice. The 16 bits hold s to half of 2^-9, so that g is off by
+// 2^-10.5 of itself before it is rounded (by 2^-8 at most); a bf16 2^(s - ref) would cost it another whole rounding.
+// It fails where S passes 2^79, a token whose words lie that far below the largest logit: such a row is noted in
+// `bad`, and the two-pass kernels, launched behind, do everything anew; else they return at once.
 struct LlBlock {
   int t0, n, parts;
   const float* row_sums;  // [part][n]
-  const float2* table;    // from the block's first token on
-  bf16_t* e;
-  long long lde;
-  float* factor;          // [n] 1 / S; 0 where a token does not count
-  bf16_t* xs;             // [n][width] x / S
+  const float2* table;    // from token t0 on
+  bf16_t* g;
+  long long ldg;
 };
 
 __global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_block_kernel(LinLossParams p, LlBlock b) {
@@ -1166,32 +1180,50 @@ __global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_block_kernel
   const int at = first + w;
   if (at >= b.n) return;
   const long long t = b.t0 + at;
-  const float live = p.r.live[t], S = s_s[0][w], ref = b.table[at].x;
+  const float live = p.r.live[t], S = s_s[0][w];
   const bool counts = live != 0.f;
-  const float lse = (counts ? ref + fast_log2(S) : 0.f) + (live - live);  // NaN for a row with a word outside the vocabulary
-  const float a = counts ? 1.f / S + (live - live) : 0.f;
+  const float lse = (counts ? b.table[at].x + fast_log2(S) : 0.f) + (live - live);  // NaN: a word outside the vocabulary
   if (lane == 0) {
     p.stat[t] = make_float2(lse, counts ? 1.f : 0.f);
-    b.factor[at] = a;
-    if (counts && !(S > 0x1p-100f && S < 0x1p100f)) *p.bad = 1;
+    if (counts && !(S > 0x1p-10f && S < 0x1p79f)) *p.bad = 1;
   }
   float sum = 0.f;
   for (int k = lane; k < p.r.top; k += 64) {
     const long long i = t * p.r.top + k;
-    const int word = p.r.words[i];
-    if (word < 0) continue;
-    const float q = p.r.q[i], z = p.picked[i] * p.c;
-    sum = __builtin_fmaf(q, (lse - z) + fast_log2(q), sum);
-    store_as(b.e + at * b.lde + word, __builtin_fmaf(-q, S, fast_exp2(z - ref)));
+    if (p.r.words[i] < 0) continue;
+    const float q = p.r.q[i];
+    sum = __builtin_fmaf(q, (lse - p.picked[i] * p.c) + fast_log2(q), sum);
   }
   sum = wave_sum(sum) * (kLn2 * p.temperature * p.temperature);
   if (lane == 0) p.loss[t] = (counts ? sum : 0.f) + (live - live);
-  for (int c = 8 * lane; c < p.width; c += 512) {
-    float x[8];
-    load_planes<false>(p.xp + t * p.width + c, 0, x);
+}
+
+// A workgroup a token: its 16 bits to g, then its list's words anew. (8192 x 50280: 322 us, 5.1 TB/s. In parts of 1280
+// tokens, which stay in the cache of 256 MB, 45 us each, but the product then has fewer tiles a launch: 1115 us for both
+// instead of 1010.)
+__global__ __launch_bounds__(256) void ll_convert_kernel(LinLossParams p, LlBlock b) {
+  const int at = gridDim.x - 1 - blockIdx.x;  // (the last ones are in the caches)
+  const long long t = b.t0 + at;
+  bf16_t* row = b.g + at * b.ldg;
+  const float lse = p.stat[t].x, ref = b.table[at].x;
+  const float by = ref < INFINITY ? (kFixedLow + ref) - lse : 0.f;  // (a row that does not count has zeros)
+#pragma unroll 4
+  for (int c = 8 * threadIdx.x; c < b.ldg; c += 8 * 256) {
+    u32x4 v = *reinterpret_cast<const u32x4*>(row + c);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] *= a;
-    store_planes<false>(x, 0, b.xs + at * static_cast<long long>(p.width) + c, 0);
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t lo = v[i] & 0xffffu, hi = v[i] >> 16;
+      const float a = fast_exp2(__builtin_fmaf(static_cast<float>(lo), kFixedStep, by));
+      const float d = fast_exp2(__builtin_fmaf(static_cast<float>(hi), kFixedStep, by));
+      v[i] = pack_bf16x2(lo == 0 ? by - by : a, hi == 0 ? by - by : d);
+    }
+    *reinterpret_cast<u32x4*>(row + c) = v;
+  }
+  __syncthreads();
+  for (int k = threadIdx.x; k < p.r.top; k += 256) {
+    const long long i = t * p.r.top + k;
+    const int word = p.r.words[i];
+    if (word >= 0) store_as(row + word, fast_exp2(__builtin_fmaf(p.picked[i], p.c, -lse)) - p.r.q[i]);
   }
 }
 
@@ -1416,10 +1448,11 @@ LinLossPlan linloss_plan(int tokens, int features, int vocab, int planes) {
   const long long x = with_shape(q.shape_x, kModeDx, [&](auto s) { return part_sums<decltype(s)>(features, tokens, x_stages); });
   const long long w = with_shape(q.shape_w, kModeDw, [&](auto s) { return part_sums<decltype(s)>(features, words, w_stages); });
   q.partial = x > w ? x : w;
-  // Both directions at once, where the logits' product is worth more than x's rows divided and the launches that may not
-  // be needed (us of both, apart and at once: 2048 x 64 x 50280 234 and 274; 32768 x 128 x 4200 365 and 388; 65536 x 64 x
-  // 8200 1093 and 1148; 512 x 768 x 50280 286 and 266; 16384 x 64 x 16500 574 and 562; 2048 x 768 x 50280 748 and 645).
-  q.both = planes == 1 && tokens >= 512 && vocab >= 16384 && static_cast<double>(tokens) * features * vocab >= 0x1p34;
+  // Both directions at once, where the logits' product costs more than their 16 bits read and g written, which its
+  // features decide, and launches that may not be needed (us of both, apart and at once, x 50280: 4096 x 256 612 and 690;
+  // 512 x 768 276 and 276; 1024 x 768 433 and 408; 16384 x 768 4875 and 4536; 2048 x 2560 2071 and 1723; 131072 x
+  // 1280 x 260 1200 and 1208).
+  q.both = planes == 1 && tokens >= 512 && features >= 640 && vocab >= 1024 && static_cast<long long>(tokens) * vocab >= 1LL << 25;
   if (q.both) {
     q.lde = whole;
     const long long rows = (1LL << 30) / (2 * q.lde) / 256 * 256, blocks = (tokens + rows - 1) / rows;
@@ -1603,14 +1636,14 @@ hipError_t launch_linloss_both(const LinLossParams& given, const LinLossPlan& pl
     LossMatrix x = x_planes(p);
     x.base += static_cast<long long>(t0) * p.width;
     x.end = static_cast<long long>(n) * p.width;
-    LossMatrix g{p.g, plan.lde, 0, n * plan.lde};
+    const LossMatrix g{p.g, plan.lde, 0, n * plan.lde};
     LlArgs a{};
     a.pairs = 1;
     a.partial = p.partial;
+    LlOut o{};
     a.a = x;
     a.b = w;
     a.k = p.width;
-    LlOut o{};
     o.rows = n;
     o.cols = p.vocab;
     o.c = p.c;
@@ -1619,9 +1652,10 @@ hipError_t launch_linloss_both(const LinLossParams& given, const LinLossPlan& pl
     o.ld = plan.lde;
     o.row_sums = p.row_sums;
     launch_product<LlLargeN, kModeExp>(a, o, stream);
-    LlBlock b{t0, n, (p.vocab + 255) / 256 * LlLargeN::kWN, p.row_sums, p.scale + t0, p.g, plan.lde, p.factor, p.xs};
+    const LlBlock b{t0, n, (p.vocab + 255) / 256 * LlLargeN::kWN, p.row_sums, p.scale + t0, p.g, plan.lde};
     hipLaunchKernelGGL(ll_block_kernel, dim3((n + kFinishTokens - 1) / kFinishTokens), dim3(kFinishTokens * kFinishSlices), 0,
                        stream, p, b);
+    hipLaunchKernelGGL(ll_convert_kernel, dim3(n), dim3(256), 0, stream, p, b);
     a.a = w;
     a.b = g;
     a.k = (p.vocab + kLlK - 1) / kLlK * kLlK;
@@ -1632,10 +1666,10 @@ hipError_t launch_linloss_both(const LinLossParams& given, const LinLossPlan& pl
     o.ld_dx = p.tokens;
     o.dx_bf16 = 1;
     o.by = by;
-    o.live = p.factor;
+    o.live = p.r.live + t0;
     launch_product<LlLargeM, kModeDx>(a, o, stream);
     a.a = g;
-    a.b = LossMatrix{p.xs, p.width, 0, static_cast<long long>(n) * p.width};
+    a.b = x;
     a.k = (n + kLlK - 1) / kLlK * kLlK;
     o = LlOut{};
     o.rows = p.vocab;

@@ -84,9 +84,7 @@ struct LinLossParams {
   void* dw;           // [vocab][features]
   int dw_bf16;
   // both directions at once
-  float* factor;      // [block]
   float* row_sums;    // [parts_both][block]
-  bf16_t* xs;         // [block][width]
   float* dw_sum;      // [vocab][features] where there are blocks
   int* bad;
   const int* only_if; // NULL, or nothing is done where this is 0

@@ -25,7 +25,8 @@ outside the vocabulary, or a teacher's logit that is NaN or inf, makes its row's
 ``reduction``: "mean" over the rows that count (0 if none does), "sum", or "none" for (rows,)
 losses. The loss is float32. Differentiable, once, in x, weight and logits; gradients have their input's
 type. Products are summed in float32. For a bfloat16 x the logits' gradient is rounded to bfloat16 once, as
-the operands are, and a float32 weight is read in a bfloat16 copy: ``weight_act``, where the caller
+the operands are (of a large head whose two gradients come with its loss, from probabilities held to less than
+2^-10 of themselves), and a float32 weight is read in a bfloat16 copy: ``weight_act``, where the caller
 keeps one, else a cast; float32 operands keep float32 precision throughout. ``holder``
 (``lm_ops.GradHolder``) takes the weight's float32 gradient instead of autograd. There is no CPU path.
 """
