@@ -217,7 +217,10 @@ struct LlInt {
 };
 
 // A value's planes of half precision. (An upper one that is not finite has a lower one of zero.)
+// v is the rounded float32 number for both: the compiler would round the operation that it comes from straight to the
+// upper plane, but take the lower one from v, so that they disagreed where the two roundings do.
 __device__ __forceinline__ void split_half(float v, uint16_t& hi, uint16_t& lo) {
+  asm volatile("" : "+v"(v));
   const _Float16 h = static_cast<_Float16>(v);
   const float left = (v - static_cast<float>(h)) * (1.f / kLowScale);
   hi = __builtin_bit_cast(uint16_t, h);
@@ -1123,7 +1126,7 @@ __global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_finish_kerne
     if (t0 + mine < p.tokens) {
       const float live = p.r.live[t0 + mine];
       lse += live - live;  // NaN for a row that has a word outside the vocabulary
-      p.stat[t0 + mine] = make_float2(lse, live == 0.f ? 0.f : 1.f);
+      p.stat[t0 + mine] = make_float2(s_m[0][mine], live == 0.f ? 0.f : 1.f / s_s[0][mine] + (live - live));
     }
     s_lse[mine] = lse;
   }
@@ -1184,7 +1187,7 @@ __global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_block_kernel
   const bool counts = live != 0.f;
   const float lse = (counts ? b.table[at].x + fast_log2(S) : 0.f) + (live - live);  // NaN: a word outside the vocabulary
   if (lane == 0) {
-    p.stat[t] = make_float2(lse, counts ? 1.f : 0.f);
+    p.stat[t] = make_float2(b.table[at].x, counts ? 1.f / S + (live - live) : 0.f);
     if (counts && !(S > 0x1p-10f && S < 0x1p79f)) *p.bad = 1;
   }
   float sum = 0.f;
@@ -1205,8 +1208,9 @@ __global__ __launch_bounds__(256) void ll_convert_kernel(LinLossParams p, LlBloc
   const int at = gridDim.x - 1 - blockIdx.x;  // (the last ones are in the caches)
   const long long t = b.t0 + at;
   bf16_t* row = b.g + at * b.ldg;
-  const float lse = p.stat[t].x, ref = b.table[at].x;
-  const float by = ref < INFINITY ? (kFixedLow + ref) - lse : 0.f;  // (a row that does not count has zeros)
+  const float2 st = p.stat[t];
+  const float by = kFixedLow + fast_log2(st.y);  // (a row that does not count has zeros: -inf)
+  const float zero = st.y - st.y;  // or NaN
 #pragma unroll 4
   for (int c = 8 * threadIdx.x; c < b.ldg; c += 8 * 256) {
     u32x4 v = *reinterpret_cast<const u32x4*>(row + c);
@@ -1215,7 +1219,7 @@ __global__ __launch_bounds__(256) void ll_convert_kernel(LinLossParams p, LlBloc
       const uint32_t lo = v[i] & 0xffffu, hi = v[i] >> 16;
       const float a = fast_exp2(__builtin_fmaf(static_cast<float>(lo), kFixedStep, by));
       const float d = fast_exp2(__builtin_fmaf(static_cast<float>(hi), kFixedStep, by));
-      v[i] = pack_bf16x2(lo == 0 ? by - by : a, hi == 0 ? by - by : d);
+      v[i] = pack_bf16x2(lo == 0 ? zero : a, hi == 0 ? zero : d);
     }
     *reinterpret_cast<u32x4*>(row + c) = v;
   }
@@ -1223,7 +1227,7 @@ __global__ __launch_bounds__(256) void ll_convert_kernel(LinLossParams p, LlBloc
   for (int k = threadIdx.x; k < p.r.top; k += 256) {
     const long long i = t * p.r.top + k;
     const int word = p.r.words[i];
-    if (word >= 0) store_as(row + word, fast_exp2(__builtin_fmaf(p.picked[i], p.c, -lse)) - p.r.q[i]);
+    if (word >= 0) store_as(row + word, __builtin_fmaf(fast_exp2(__builtin_fmaf(p.picked[i], p.c, -st.x)), st.y, -p.r.q[i]));
   }
 }
 
@@ -1243,8 +1247,8 @@ __global__ __launch_bounds__(256) void ll_rescale_kernel(bf16_t* dx, long long n
 }
 
 // ------------------------------------------------------------------------- backward, around the products
-// A token's lse, and what its g is scaled by before it is rounded: without a reduction its own upstream gradient. (With
-// one, nothing: what all tokens share is left to the products' ends, since 1 / tokens has an error of its own in
+// A token's largest s, and what its 2^(s - largest) are scaled by: one over their sum, and without a reduction its own
+// upstream gradient, before g is rounded. (With one, no gradient: what all tokens share is left to the products' ends, since 1 / tokens has an error of its own in
 // bf16, the same for every token.)
 // (Split, they are taken to a power of two's multiple below 1 first: one workgroup.)
 template <bool kF32>
@@ -1265,11 +1269,13 @@ __global__ __launch_bounds__(1024) void ll_scale_kernel(LinLossParams p, float2*
   }
   for (int t = blockIdx.x * 1024 + threadIdx.x; t < p.tokens; t += gridDim.x * 1024) {
     const float2 st = p.stat[t];
-    scale[t] = make_float2(st.x, st.y == 0.f ? 0.f : ldexpf(p.grad[t] * p.temperature, power));
+    scale[t] = make_float2(st.x, st.y == 0.f ? 0.f : st.y * ldexpf(p.grad[t] * p.temperature, power));
   }
 }
 
-// g at the wanted words of the piece that begins at word v0, from their own logits.
+// g at the wanted words of the piece that begins at word v0. In bf16 from their own logits, since their probabilities
+// are rounded there. The planes of a float32 one hold it to 24 bits: it is the product's own then, whose exponential is
+// part of the row's sum, so that what they are both off by cancels where the probability is nearly 1.
 template <bool kF32>
 __global__ __launch_bounds__(256) void ll_wanted_kernel(LinLossParams p, const float2* scale, int v0, int words) {
   const long long i = blockIdx.x * 256LL + threadIdx.x;
@@ -1277,11 +1283,18 @@ __global__ __launch_bounds__(256) void ll_wanted_kernel(LinLossParams p, const f
   const int v = p.r.words[i] - v0;
   if (p.r.words[i] < 0 || v < 0 || v >= words) return;
   const long long t = i / p.r.top;
-  const float2 sc = scale[t];
-  const float d = (fast_exp2(__builtin_fmaf(p.picked[i], p.c, -sc.x)) - p.r.q[i]) * sc.y;
+  float up = 1.f;
+  if (p.reduction == kLossNone) up = ldexpf(p.grad[t] * p.temperature, kF32 ? p.power_g[0] : 0);
   bf16_t* dst = p.g + t * p.ldg + v;
-  if constexpr (kF32) split_half(d * kGradScale, dst->bits, dst[p.tokens * p.ldg].bits);
-  else store_as(dst, d);
+  if constexpr (kF32) {
+    bf16_t* low = dst + p.tokens * p.ldg;
+    const float d = __builtin_fmaf(static_cast<float>(__builtin_bit_cast(_Float16, low->bits)), kLowScale,
+                                   static_cast<float>(__builtin_bit_cast(_Float16, dst->bits)));
+    split_half(__builtin_fmaf(-p.r.q[i] * up, kGradScale, d), dst->bits, low->bits);
+  } else {
+    const float2 sc = scale[t];
+    store_as(dst, __builtin_fmaf(fast_exp2(__builtin_fmaf(p.picked[i], p.c, -sc.x)), sc.y, -p.r.q[i] * up));
+  }
 }
 
 unsigned blocks_for(long long n, long long most) {

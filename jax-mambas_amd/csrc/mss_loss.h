@@ -67,13 +67,14 @@ struct LinLossParams {
   float2* part;    // [parts][tokens]: a part's largest s and sum of 2^(s - largest), base 2
   int parts;
   float* picked;   // [rows][top] logits of the wanted words
-  float2* stat;    // [tokens + kLinLossTile]: log of the sum of exp s, base 2, and whether the row counts (0, 1)
+  float2* stat;    // [tokens + kLinLossTile]: m, the largest s to base 2 or near it, and 1 / sum 2^(s - m), 0 where the row
+                   // does not count: (their logarithm, in 32 bits, would cost a probability log2 |lse| of its bits)
   float* loss;     // [tokens]
   float* mean;     // the reduced loss
   float* by;       // 1 / (rows that count), for a mean
   // backward
   const float* grad;  // [1], or [tokens] without a reduction
-  float2* scale;      // without a reduction: stat with the row's upstream gradient in place of 1
+  float2* scale;      // without a reduction: stat with the row's upstream gradient in its factor
   bf16_t* g;          // [planes][tokens][ldg] the logits' gradient for a piece of the vocabulary
   long long ldg;
   float* dx_sum;      // [features][ldx] where there are pieces

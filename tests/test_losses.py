@@ -530,6 +530,27 @@ def test_weight_rows_far_apart():
 
 
 @pytest.mark.gpu
+def test_float32_gradients_of_single_words():
+    """A weight of 8 on the diagonal: dx is 8 times the logits' gradient, a word each, whose two planes have to agree in
+    every one of two million. A logit has one product, held to 2^-24 and 2^-23 of it (its planes, and their products that
+    are dropped), a probability the rounding of the logarithm's argument, 2 M U, of the exponential and the sum of 128
+    words, and g its planes and the last rounding: (2 (3 |z| + 2 M) + 160) U p, and 4 U |g|. The planes hold 2^15 g,
+    the lower one times 2^-11 in steps of 2^-24 at least: half of 2^-50 of g's own unit, however small it is."""
+    t, d = 16384, 128
+    g = torch.Generator(device="cuda").manual_seed(12)
+    x = (0.4 * torch.randn(d, t, generator=g, device="cuda")).requires_grad_(True)
+    w = 8.0 * torch.eye(d, device="cuda")
+    targets = _targets(t, d, 0.0, 13)
+    (dx,) = torch.autograd.grad(linear_cross_entropy(x, w, targets, reduction="sum"), (x,))
+    z = 8.0 * x.detach().double().t()
+    p = torch.softmax(z, 1)
+    want = p - torch.nn.functional.one_hot(targets, d)
+    m = z.abs().amax(1, keepdim=True) * np.log2(np.e) + 7
+    tol = (2 * (3 * z.abs().amax(1, keepdim=True) + 2 * m) + 160) * U * p + 4 * U * want.abs() + 2.0 ** -51
+    _check("dx / 8", dx.t() / 8, want, tol)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("reduction", ["mean", "none"])
 @pytest.mark.parametrize("x_exp,w_exp,g_exp", [(0, 0, 0), (60, -60, 0), (-70, 66, 5), (100, -104, -20), (-126, 100, 40), (8, 3, -60)])
 def test_float32_of_any_size(x_exp, w_exp, g_exp, reduction):
