@@ -6,7 +6,8 @@
 // Forward: one product whose tiles leave, for each token and tile, only the largest s and the sum of
 // 2^(s - largest); they are merged a token at a time. The wanted words' logits are formed apart, one
 // dot product each. Backward: in pieces of the vocabulary the product is formed again, its tiles
-// turned into g (bf16) in a workspace, from which the two gradients' products read.
+// turned into g (bf16) in a workspace, from which the two gradients' products read. Both at once (bf16 operands,
+// wide heads): one product leaves s in 16 bits in the workspace, beside the sums, and g takes its place.
 //
 // All products run on the matrix cores with float32 sums. bf16 operands are taken as they are
 // (v_mfma_f32_32x32x16_bf16); g is rounded to bf16 once, as its factors x and w are. A float32 matrix is taken to
