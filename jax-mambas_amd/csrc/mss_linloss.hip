@@ -945,11 +945,16 @@ __global__ __launch_bounds__(256) void ll_pack_x_kernel(LinLossParams p) {
       if (lane == 0) p.r.counts[blockIdx.x] = n;
     }
   }
+  in_t v[16];  // (all of them on their way at once: loads under a condition would follow one another)
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int f = min(f0 + (along_f ? lane : w + 4 * i), p.features - 1), t = min(t0 + (along_f ? w + 4 * i : lane), p.tokens - 1);
+    v[i] = x[f * p.sf + t * p.st];
+  }
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int a = along_f ? lane : w + 4 * i, b = along_f ? w + 4 * i : lane;  // feature, token
-    const int f = f0 + a, t = t0 + b;
-    s[a][b] = f < p.features && t < p.tokens ? to_f32(x[f * p.sf + t * p.st]) : 0.f;
+    s[a][b] = f0 + a < p.features && t0 + b < p.tokens ? to_f32(v[i]) : 0.f;
   }
   __syncthreads();
   const long long plane = static_cast<long long>(p.tokens) * p.width;
@@ -1086,7 +1091,7 @@ __device__ __forceinline__ void sums_merge(float& m, float& s, float m2, float s
 
 template <bool kPick, bool kF32>
 __global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_finish_kernel(LinLossParams p, LossMatrix wm) {
-  __shared__ float s_m[kFinishSlices][kFinishTokens], s_s[kFinishSlices][kFinishTokens], s_lse[kFinishTokens];
+  __shared__ float s_m[kFinishSlices][kFinishTokens], s_s[kFinishSlices][kFinishTokens], s_log[kFinishTokens];
   if (p.only_if != nullptr && *p.only_if == 0) return;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int t0 = blockIdx.x * kFinishTokens;
@@ -1103,10 +1108,14 @@ __global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_finish_kerne
   {
     float m = -INFINITY, s = 0.f;
     if (t0 + mine < p.tokens) {
-#pragma unroll 4
-      for (int i = slice; i < p.parts; i += kFinishSlices) {
-        const float2 q = p.part[static_cast<long long>(i) * p.tokens + t0 + mine];
-        sums_merge(m, s, q.x, q.y);
+      for (int i0 = slice; i0 < p.parts; i0 += 4 * kFinishSlices) {
+        float2 q[4];  // (on their way at once)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          q[e] = p.part[static_cast<long long>(min(i0 + e * kFinishSlices, p.parts - 1)) * p.tokens + t0 + mine];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (i0 + e * kFinishSlices < p.parts) sums_merge(m, s, q[e].x, q[e].y);
       }
     }
     s_m[slice][mine] = m;
@@ -1123,24 +1132,22 @@ __global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_finish_kerne
   }
   __syncthreads();
   if (threadIdx.x < kFinishTokens) {
-    float lse = s_m[0][mine] + fast_log2(s_s[0][mine]);
     if (t0 + mine < p.tokens) {
-      const float live = p.r.live[t0 + mine];
-      lse += live - live;  // NaN for a row that has a word outside the vocabulary
+      const float live = p.r.live[t0 + mine];  // (NaN for a row that has a word outside the vocabulary)
       p.stat[t0 + mine] = make_float2(s_m[0][mine], live == 0.f ? 0.f : 1.f / s_s[0][mine] + (live - live));
     }
-    s_lse[mine] = lse;
+    s_log[mine] = fast_log2(s_s[0][mine]);
   }
   __syncthreads();
   if (t >= p.tokens) return;
-  const float lse = s_lse[w];
+  const float m = s_m[0][w], log_s = s_log[w];
   float sum = 0.f;
   for (int k = lane; k < p.r.top; k += 64) {
     const long long at = t * p.r.top + k;
     if (p.r.words[at] < 0) continue;
     const float q = p.r.q[at];
     const float z = kPick ? logit[0] : p.picked[at];
-    sum = __builtin_fmaf(q, (lse - z * p.c) + fast_log2(q), sum);
+    sum = __builtin_fmaf(q, (m - z * p.c) + log_s + fast_log2(q), sum);
   }
   sum = wave_sum(sum) * (kLn2 * p.temperature * p.temperature);
   const float live = p.r.live[t];
@@ -1186,9 +1193,9 @@ __global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_block_kernel
   const long long t = b.t0 + at;
   const float live = p.r.live[t], S = s_s[0][w];
   const bool counts = live != 0.f;
-  const float lse = (counts ? b.table[at].x + fast_log2(S) : 0.f) + (live - live);  // NaN: a word outside the vocabulary
-  if (lane == 0) {
-    p.stat[t] = make_float2(b.table[at].x, counts ? 1.f / S + (live - live) : 0.f);
+  const float ref = b.table[at].x, log_s = fast_log2(S);
+  if (lane == 0) {  // (a live of NaN: a word outside the vocabulary)
+    p.stat[t] = make_float2(ref, counts ? 1.f / S + (live - live) : 0.f);
     if (counts && !(S > 0x1p-10f && S < 0x1p79f)) *p.bad = 1;
   }
   float sum = 0.f;
@@ -1196,7 +1203,7 @@ __global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_block_kernel
     const long long i = t * p.r.top + k;
     if (p.r.words[i] < 0) continue;
     const float q = p.r.q[i];
-    sum = __builtin_fmaf(q, (lse - p.picked[i] * p.c) + fast_log2(q), sum);
+    sum = __builtin_fmaf(q, (ref - p.picked[i] * p.c) + log_s + fast_log2(q), sum);
   }
   sum = wave_sum(sum) * (kLn2 * p.temperature * p.temperature);
   if (lane == 0) p.loss[t] = (counts ? sum : 0.f) + (live - live);
