@@ -53,7 +53,7 @@ struct LlShape {
   static constexpr int kPerCU = kRing * kSlots * 16 > 81920 ? 1 : 2;
   static constexpr int kSums = 16 * kMT * kNT;  // of a lane
   static_assert(kASlots % kThreads == 0 && kBSlots % kThreads == 0, "whole copies");
-  static_assert(kRing >= 2 && kRing <= 4 && (kRing - 1) * kCopies < 64, "");
+  static_assert((kRing == 2 || kRing == 4) && (kRing - 1) * kCopies < 64, "");
 };
 
 typedef uint32_t lu32x4 __attribute__((ext_vector_type(4)));
@@ -91,8 +91,8 @@ __device__ __forceinline__ void ll_meet() {
 template <int kTile, int kBK, bool kAcross, int kPerm>
 struct LlPanel {
   static constexpr int kUnits = kTile / 32, kChunks = kBK / 8;
-  static_assert(kBK == 64 || kBK == 32, "");
-  static __device__ __forceinline__ int chunk(int row, int c) { return kBK == 64 ? c ^ ((row >> 1) & 7) : c ^ ((row >> 2) & 3); }
+  static_assert(kBK == 64, "the chunks of a row are eight");
+  static __device__ __forceinline__ int chunk(int row, int c) { return c ^ ((row >> 1) & 7); }
   static __device__ __forceinline__ int key(int k) { return kUnits >= 4 ? k & 3 : kUnits == 2 ? (k >> 1) & 1 : 0; }
   // Bytes from the stage's first element to what slot `s` holds.
   static __device__ __forceinline__ uint32_t source(int s, uint32_t ld) {
@@ -184,7 +184,7 @@ struct LlOut {
   float c;
   const int* powers;     // of two, of x and of w where they are split
   float2* part;          // kModeLse: [part][cols]
-  const float2* scale;   // kModeGrad: [rows], and a tile's rows more
+  const float2* scale;   // kModeGrad, kModeExp: [rows], and a tile's rows more
   bf16_t* g;
   long long ld, plane;   // row stride of g, dx, dw; from one plane of g to the next
   float* f;              // kModeDx, kModeDw with float32 output
@@ -236,7 +236,7 @@ __device__ __forceinline__ float quad_mov(float v) {
 }
 
 // A wave's kMT x kNT matrix tiles: from row wm0 and column wn0 on, in part `part` of the words. table: the scales of
-// its rows (kModeGrad).
+// its rows (kModeGrad: a subtrahend and a factor; kModeExp: a subtrahend, and what the 16 bits' fraction adds).
 template <int kMode, bool kF32, int kMT, int kNT>
 __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT], int wm0, int wn0, int part, int lane,
                                        const float2* table) {
@@ -489,7 +489,7 @@ __device__ __forceinline__ void ll_end(const LlOut& o, lf32x16 (&acc)[kMT][kNT],
 // A workgroup's work is a row of segments: units of one tile each, whose copies follow one another through the
 // ring without a gap, so that a tile's first stages arrive under the one before's last products and its end.
 //
-// kModeLse, kModeGrad: whole tiles. The tiles are dealt out so that those at hand on one XCD are neighbours (8 of
+// kModeLse, kModeGrad, kModeExp: whole tiles. The tiles are dealt out so that those at hand on one XCD are neighbours (8 of
 // A by all of B share their operands in its L2), and a workgroup's next one is as many further on as the
 // XCD has workgroups.
 //
@@ -576,7 +576,7 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
   constexpr int kBK = S::kBK;
   using PA = LlPanel<S::kM, kBK, kAAcross, 1>;
   using PB = LlPanel<S::kN, kBK, kBAcross, ll_perm<S, kMode>>;
-  __shared__ u32x4 s0[S::kSlots], s1[S::kSlots], s2[S::kRing > 2 ? S::kSlots : 1], s3[S::kRing > 3 ? S::kSlots : 1];
+  __shared__ u32x4 s0[S::kSlots], s1[S::kSlots], s2[S::kRing == 4 ? S::kSlots : 1], s3[S::kRing == 4 ? S::kSlots : 1];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % S::kWM, wn = wave / S::kWM;
@@ -636,7 +636,8 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
                    static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(base >> 32) & 0xffff)),
                    S::kM * 8, 0x00027000};
     const int slice = wave % kSlices;
-    if (S::kM % 128 == 0 || 1024 * slice + 16 * lane < S::kM * 8) ll_copy(r, 1024 * slice + 16 * lane, reinterpret_cast<const char*>(s_scale) + 1024 * slice);
+    if (S::kM % 128 == 0 || 1024 * slice + 16 * lane < S::kM * 8)
+      ll_copy(r, 1024 * slice + 16 * lane, reinterpret_cast<const char*>(s_scale) + 1024 * slice);
   };
 
   lf32x16 acc[S::kMT][S::kNT];
@@ -693,8 +694,10 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
   };
   issue(s0);
   issue(s1);
-  if constexpr (S::kRing > 2) issue(s2);
-  if constexpr (S::kRing > 3) issue(s3);
+  if constexpr (S::kRing == 4) {
+    issue(s2);
+    issue(s3);
+  }
   ll_meet<(S::kRing - 1) * S::kCopies>();
   load(s0, 0);
   for (int i = 0;; ++i) {
@@ -857,21 +860,30 @@ __global__ __launch_bounds__(1024) void ll_max_kernel(LinLossParams p) {
     const bool along_f = p.sf == 1;
     const int rows = along_f ? p.tokens : p.features, cols = along_f ? p.features : p.tokens;
     for (int r = blockIdx.x * 16 + w; r < rows; r += 16 * kMaxX)
-#pragma unroll 4
-      for (int c = lane; c < cols; c += 64) {
-        const int f = along_f ? c : r, t = along_f ? r : c;
-        const float v = x[f * p.sf + t * p.st];
-        if (row_counts(p, t)) m = max(m, finite_bits(v));
+      for (int c0 = lane; c0 < cols; c0 += 8 * 64) {
+        float v[8];  // (on their way at once; a place past the row's end takes its last one)
+        bool counts[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int c = min(c0 + 64 * e, cols - 1), f = along_f ? c : r, t = along_f ? r : c;
+          v[e] = x[f * p.sf + t * p.st];
+          counts[e] = row_counts(p, t);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = counts[e] ? max(m, finite_bits(v[e])) : m;
       }
   } else {
     const float* v = static_cast<const float*>(p.w);
     for (int r = (blockIdx.x - kMaxX) * 16 + w; r < p.vocab; r += 16 * kMaxW) {
       const float* row = v + r * p.ldw;
-#pragma unroll 2
-      for (int c = 4 * lane; c + 4 <= p.features; c += 256) {
-        const u32x4 u = *reinterpret_cast<const u32x4_any*>(row + c);
-        m = max(max(m, max(finite_bits(__uint_as_float(u[0])), finite_bits(__uint_as_float(u[1])))),
-                max(finite_bits(__uint_as_float(u[2])), finite_bits(__uint_as_float(u[3]))));
+      for (int c0 = 4 * lane; c0 + 4 <= p.features; c0 += 4 * 256) {
+        u32x4 u[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) u[e] = *reinterpret_cast<const u32x4_any*>(row + min(c0 + 256 * e, p.features - 4));
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          m = max(max(m, max(finite_bits(__uint_as_float(u[e][0])), finite_bits(__uint_as_float(u[e][1])))),
+                  max(finite_bits(__uint_as_float(u[e][2])), finite_bits(__uint_as_float(u[e][3]))));
       }
       if (lane < p.features % 4) m = max(m, finite_bits(row[p.features - 1 - lane]));
     }
@@ -948,7 +960,8 @@ __global__ __launch_bounds__(256) void ll_pack_x_kernel(LinLossParams p) {
   in_t v[16];  // (all of them on their way at once: loads under a condition would follow one another)
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const int f = min(f0 + (along_f ? lane : w + 4 * i), p.features - 1), t = min(t0 + (along_f ? w + 4 * i : lane), p.tokens - 1);
+    const int f = min(f0 + (along_f ? lane : w + 4 * i), p.features - 1);
+    const int t = min(t0 + (along_f ? w + 4 * i : lane), p.tokens - 1);
     v[i] = x[f * p.sf + t * p.st];
   }
 #pragma unroll
@@ -1156,12 +1169,13 @@ __global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_finish_kerne
 }
 
 // ------------------------------------------------------------------------- both directions at once
-// For a block of tokens and the whole vocabulary at a time, kModeExp leaves the words' s - ref in 16 bits, with ref a logit of
-// the token's own list, and the sums S of 2^(s - ref); then lse = ref + log S, and g = 2^(s - lse) - q, rounded to bf16,
-// takes their place: the logits are formed once, not twice. The 16 bits hold s to half of 2^-9, so that g is off by
-// 2^-10.5 of itself before it is rounded (by 2^-8 at most); a bf16 2^(s - ref) would cost it another whole rounding.
-// It fails where S passes 2^79, a token whose words lie that far below the largest logit: such a row is noted in
-// `bad`, and the two-pass kernels, launched behind, do everything anew; else they return at once.
+// For a block of tokens and the whole vocabulary at a time, kModeExp leaves the words' s - ref in 16 bits, with ref a
+// logit of the token's own list, and the sums S of 2^(s - ref); then g = 2^(s - ref) / S - q, rounded to bf16, takes
+// their place: the logits are formed once, not twice. The 16 bits hold s to half of 2^-9, so that g is off by 2^-10.5
+// of itself before it is rounded (by 2^-8 at most); a bf16 2^(s - ref), the division left to x's rows and dx's
+// columns, would need no conversion, but cost dw another whole rounding. It fails where S passes 2^79, a token whose
+// words lie that far below its largest logit: such a row is noted in `bad`, and the kernels of the two apart,
+// launched behind, do everything anew; else they return at once.
 struct LlBlock {
   int t0, n, parts;
   const float* row_sums;  // [part][n]
@@ -1256,8 +1270,8 @@ __global__ __launch_bounds__(256) void ll_rescale_kernel(bf16_t* dx, long long n
 
 // ------------------------------------------------------------------------- backward, around the products
 // A token's largest s, and what its 2^(s - largest) are scaled by: one over their sum, and without a reduction its own
-// upstream gradient, before g is rounded. (With one, no gradient: what all tokens share is left to the products' ends, since 1 / tokens has an error of its own in
-// bf16, the same for every token.)
+// upstream gradient, before g is rounded. (With one, no gradient: what all tokens share is left to the products' ends,
+// since 1 / tokens has an error of its own in bf16, the same for every token.)
 // (Split, they are taken to a power of two's multiple below 1 first: one workgroup.)
 template <bool kF32>
 __global__ __launch_bounds__(1024) void ll_scale_kernel(LinLossParams p, float2* scale) {
@@ -1367,13 +1381,10 @@ void launch_product(LlArgs a, const LlOut& o, hipStream_t stream) {
   }
 }
 
-// f of the shape of a product: words x tokens, tokens x words, features x tokens, words x features.
+// f of the shape of a gradient's product.
 template <typename F>
-auto with_shape(int shape, int mode, F&& f) {
-  if (shape == 0) return f(LlSmall{});
-  if (mode == kModeGrad) return shape == 1 ? f(LlLargeN{}) : f(LlThinM{});
-  if (shape == 1) return f(LlLargeM{});
-  return mode == kModeDw ? f(LlSmall{}) : f(LlThinN{});
+auto with_shape(int shape, F&& f) {
+  return shape == 0 ? f(LlSmall{}) : shape == 1 ? f(LlLargeM{}) : f(LlThinN{});
 }
 
 template <int kMode, bool kF32>
@@ -1466,8 +1477,8 @@ LinLossPlan linloss_plan(int tokens, int features, int vocab, int planes) {
   q.shape_w = large(words, features) ? 1 : 0;
   const int x_stages = q.piece / 64 * (planes == 1 ? 1 : kPairs);
   const int w_stages = (tokens + kLlK - 1) / kLlK * (kLlK / 64) * (planes == 1 ? 1 : kPairs);
-  const long long x = with_shape(q.shape_x, kModeDx, [&](auto s) { return part_sums<decltype(s)>(features, tokens, x_stages); });
-  const long long w = with_shape(q.shape_w, kModeDw, [&](auto s) { return part_sums<decltype(s)>(features, words, w_stages); });
+  const long long x = with_shape(q.shape_x, [&](auto s) { return part_sums<decltype(s)>(features, tokens, x_stages); });
+  const long long w = with_shape(q.shape_w, [&](auto s) { return part_sums<decltype(s)>(features, words, w_stages); });
   q.partial = x > w ? x : w;
   // Both directions at once, where the logits' product costs more than their 16 bits read and g written, which its
   // features decide, and launches that may not be needed (us of both, apart and at once, x 50280: 4096 x 256 612 and 690;
