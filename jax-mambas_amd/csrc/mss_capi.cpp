@@ -1709,18 +1709,20 @@ int linear_loss_sizes(const mss_linear_loss_args* a, int which, mss::LinLossPara
     Carve f{static_cast<char*>(a->workspace), 0};
     if (fwd) q.part = f.take<float2>(static_cast<long long>(p->parts) * a->tokens);
     if (fwd && p->planes > 1) q.maxima = f.take<uint32_t>(mss::kLinLossMaxima);
-    if (bwd) {
-      if (a->reduction == MSS_LOSS_NONE || both) q.scale = f.take<float2>(a->tokens + mss::kLinLossTile);
-      q.power_g = f.take<int>(1);
-      const long long g = static_cast<long long>(p->planes) * a->tokens * p->ldg, e = both ? plan->block * plan->lde : 0;
-      q.g = f.take<mss::bf16_t>(g > e ? g : e);
-      if (p->piece < a->vocab) q.dx_sum = f.take<float>(p->features * p->ldx);
-      q.partial = f.take<float>(both && plan->partial_both > plan->partial ? plan->partial_both : plan->partial);
-    }
     if (both) {
+      q.scale = f.take<float2>(a->tokens + mss::kLinLossTile);
+      q.ldg = plan->lde;
+      q.g = f.take<mss::bf16_t>(plan->block * plan->lde);
       q.row_sums = f.take<float>(static_cast<long long>(plan->parts_both) * plan->block);
+      q.partial = f.take<float>(plan->partial_both);
       if (plan->block < a->tokens) q.dw_sum = f.take<float>(static_cast<long long>(a->vocab) * a->features);
-      q.bad = f.take<int>(1);
+      q.bad = f.take<int>((a->tokens + plan->block - 1) / plan->block);
+    } else if (bwd) {
+      if (a->reduction == MSS_LOSS_NONE) q.scale = f.take<float2>(a->tokens + mss::kLinLossTile);
+      q.power_g = f.take<int>(1);
+      q.g = f.take<mss::bf16_t>(static_cast<long long>(p->planes) * a->tokens * p->ldg);
+      if (p->piece < a->vocab) q.dx_sum = f.take<float>(p->features * p->ldx);
+      q.partial = f.take<float>(plan->partial);
     }
     ws[i] = f.at;
     if (i == which) {

@@ -581,7 +581,9 @@ __global__ __launch_bounds__(S::kThreads) void ll_kernel(LlArgs p, LlOut o) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % S::kWM, wn = wave / S::kWM;
   __shared__ float2 s_scale[kLlGrad<kMode> ? S::kM : 1];
-  if (o.only_if != nullptr && *o.only_if == 0) return;
+  if constexpr (!kLlTeams<kMode>) {
+    if (o.only_if != nullptr && *o.only_if == 0) return;
+  }
   const LlDeal deal = ll_deal<kMode>(p);
   const int nk = p.k / kBK;
 
@@ -774,7 +776,6 @@ constexpr int kJoinWaves = 4;
 template <class S, int kMode, bool kF32>
 __global__ __launch_bounds__(64 * kJoinWaves) void ll_join_kernel(LlArgs p, LlOut o) {
   __shared__ f32x4 s_sum[kJoinWaves - 1][4 * S::kNT][64];
-  if (o.only_if != nullptr && *o.only_if == 0) return;
   const int lane = threadIdx.x & 63, mine = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int size = kMode == kModeDx ? p.tiles_m : p.tiles_n, ranges = kMode == kModeDx ? p.tiles_n : p.tiles_m;
   const int mt = blockIdx.x % S::kMT, wave = blockIdx.x / S::kMT % S::kWaves;
@@ -1058,11 +1059,12 @@ __device__ __forceinline__ void ll_dots(const LinLossParams& p, const LossMatrix
 }
 
 // table (or NULL): what a token's exponentials are taken relative to, to base 2 (kModeExp), the largest logit of its
-// list's first four words; inf for one that does not count.
+// list's first four words; inf for one that does not count. blocks: of tokens, whose notes are cleared.
 template <bool kF32>
-__global__ __launch_bounds__(256) void ll_pick_kernel(LinLossParams p, LossMatrix w, float2* table) {
+__global__ __launch_bounds__(256) void ll_pick_kernel(LinLossParams p, LossMatrix w, float2* table, int blocks) {
   const int lane = threadIdx.x & 63;
-  if (table != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *p.bad = 0;
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < blocks; i += 256) p.bad[i] = 0;
   const int per = (p.r.top + 3) / 4;
   const long long id = blockIdx.x * 4LL + (threadIdx.x >> 6);
   const long long t = id / per;
@@ -1175,25 +1177,18 @@ __global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_finish_kerne
 // of itself before it is rounded (by 2^-8 at most); a bf16 2^(s - ref), the division left to x's rows and dx's
 // columns, would need no conversion, but cost dw another whole rounding. It fails where S passes 2^79, a token whose
 // words lie that far below its largest logit: such a row is noted in `bad`, and the kernels of the two apart,
-// launched behind, do everything anew; else they return at once.
-struct LlBlock {
-  int t0, n, parts;
-  const float* row_sums;  // [part][n]
-  const float2* table;    // from token t0 on
-  bf16_t* g;
-  long long ldg;
-};
-
-__global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_block_kernel(LinLossParams p, LlBlock b) {
+// launched behind, make the block's losses and g anew; else they return at once.
+// (These kernels' tokens are a block's.)
+__global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_block_kernel(LinLossParams p, int parts) {
   __shared__ float s_s[kFinishSlices][kFinishTokens];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int first = blockIdx.x * kFinishTokens;
   const int mine = threadIdx.x % kFinishTokens, slice = threadIdx.x / kFinishTokens;
   {
     float s = 0.f;
-    if (first + mine < b.n) {
+    if (first + mine < p.tokens) {
 #pragma unroll 4
-      for (int i = slice; i < b.parts; i += kFinishSlices) s += b.row_sums[static_cast<long long>(i) * b.n + first + mine];
+      for (int i = slice; i < parts; i += kFinishSlices) s += p.row_sums[static_cast<long long>(i) * p.tokens + first + mine];
     }
     s_s[slice][mine] = s;
   }
@@ -1202,12 +1197,11 @@ __global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_block_kernel
     if (slice < h) s_s[slice][mine] += s_s[slice + h][mine];
   }
   __syncthreads();
-  const int at = first + w;
-  if (at >= b.n) return;
-  const long long t = b.t0 + at;
+  const long long t = first + w;
+  if (t >= p.tokens) return;
   const float live = p.r.live[t], S = s_s[0][w];
   const bool counts = live != 0.f;
-  const float ref = b.table[at].x, log_s = fast_log2(S);
+  const float ref = p.scale[t].x, log_s = fast_log2(S);
   if (lane == 0) {  // (a live of NaN: a word outside the vocabulary)
     p.stat[t] = make_float2(ref, counts ? 1.f / S + (live - live) : 0.f);
     if (counts && !(S > 0x1p-10f && S < 0x1p79f)) *p.bad = 1;
@@ -1226,15 +1220,15 @@ __global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_block_kernel
 // A workgroup a token: its 16 bits to g, then its list's words anew. (8192 x 50280: 322 us, 5.1 TB/s. In parts of 1280
 // tokens, which stay in the cache of 256 MB, 45 us each, but the product then has fewer tiles a launch: 1115 us for both
 // instead of 1010.)
-__global__ __launch_bounds__(256) void ll_convert_kernel(LinLossParams p, LlBlock b) {
-  const int at = gridDim.x - 1 - blockIdx.x;  // (the last ones are in the caches)
-  const long long t = b.t0 + at;
-  bf16_t* row = b.g + at * b.ldg;
+__global__ __launch_bounds__(256) void ll_convert_kernel(LinLossParams p) {
+  if (*p.bad != 0) return;
+  const long long t = gridDim.x - 1 - blockIdx.x;  // (the last ones are in the caches)
+  bf16_t* row = p.g + t * p.ldg;
   const float2 st = p.stat[t];
   const float by = kFixedLow + fast_log2(st.y);  // (a row that does not count has zeros: -inf)
   const float zero = st.y - st.y;  // or NaN
 #pragma unroll 4
-  for (int c = 8 * threadIdx.x; c < b.ldg; c += 8 * 256) {
+  for (int c = 8 * threadIdx.x; c < p.ldg; c += 8 * 256) {
     u32x4 v = *reinterpret_cast<const u32x4*>(row + c);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -1547,8 +1541,8 @@ static void launch_losses(const LinLossParams& p, const LinLossPlan& plan, bool 
   } else if (lists) {
     const long long picks = static_cast<long long>(p.tokens) * ((p.r.top + 3) / 4);
     const dim3 pg(static_cast<unsigned>((picks + 3) / 4));
-    if (f32) hipLaunchKernelGGL(ll_pick_kernel<true>, pg, dim3(256), 0, stream, p, a.a, static_cast<float2*>(nullptr));
-    else hipLaunchKernelGGL(ll_pick_kernel<false>, pg, dim3(256), 0, stream, p, a.a, static_cast<float2*>(nullptr));
+    if (f32) hipLaunchKernelGGL(ll_pick_kernel<true>, pg, dim3(256), 0, stream, p, a.a, static_cast<float2*>(nullptr), 0);
+    else hipLaunchKernelGGL(ll_pick_kernel<false>, pg, dim3(256), 0, stream, p, a.a, static_cast<float2*>(nullptr), 0);
     hipLaunchKernelGGL((ll_finish_kernel<false, false>), fg, fb, 0, stream, p, a.a);
   } else if (f32) {
     hipLaunchKernelGGL((ll_finish_kernel<true, true>), fg, fb, 0, stream, p, a.a);
@@ -1603,7 +1597,6 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
     o.ld = p.ldg;
     o.plane = g.plane;
     o.powers = p.powers;
-    o.only_if = p.only_if;
     if (f32) launch_shaped<kModeGrad, true>(plan, a, o, stream);
     else launch_shaped<kModeGrad, false>(plan, a, o, stream);
     const dim3 wg(static_cast<unsigned>((static_cast<long long>(p.tokens) * p.r.top + 255) / 256));
@@ -1620,7 +1613,6 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
       o.ld = p.ldx;
       o.add = v0 > 0;
       o.powers = p.powers;
-      o.only_if = p.only_if;
       if (v0 + words == p.vocab) {
         o.dx = p.dx;
         o.ld_dx = p.tokens;
@@ -1640,7 +1632,6 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
       o.rows = words;
       o.cols = p.features;
       o.ld = p.features;
-      o.only_if = p.only_if;
       o.by = by;
       o.by.power = f32 ? p.powers : nullptr;
       void* dst = static_cast<char*>(p.dw) + v0 * p.features * (p.dw_bf16 ? 2 : 4);
@@ -1653,56 +1644,68 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
   return hipGetLastError();
 }
 
-hipError_t launch_linloss_both(const LinLossParams& given, const LinLossPlan& plan, hipStream_t stream) {
-  LinLossParams p = given;
+hipError_t launch_linloss_both(const LinLossParams& p, const LinLossPlan& plan, hipStream_t stream) {
   hipError_t e = launch_operands(p, stream);
   if (e != hipSuccess) return e;
   e = launch_loss_mean(nullptr, p.r, p.reduction, nullptr, p.by, stream);
   if (e != hipSuccess) return e;
   const LossMatrix w = weight_planes(p);
   const long long picks = static_cast<long long>(p.tokens) * ((p.r.top + 3) / 4);
-  hipLaunchKernelGGL(ll_pick_kernel<false>, dim3(static_cast<unsigned>((picks + 3) / 4)), dim3(256), 0, stream, p, w, p.scale);
+  hipLaunchKernelGGL(ll_pick_kernel<false>, dim3(static_cast<unsigned>((picks + 3) / 4)), dim3(256), 0, stream, p, w, p.scale,
+                     (p.tokens + plan.block - 1) / plan.block);
   const LlScale by{nullptr, p.reduction == kLossMean ? p.by : nullptr, p.temperature, nullptr, nullptr};
   for (int t0 = 0; t0 < p.tokens; t0 += plan.block) {
-    const int n = p.tokens - t0 < plan.block ? p.tokens - t0 : plan.block;
-    LossMatrix x = x_planes(p);
-    x.base += static_cast<long long>(t0) * p.width;
-    x.end = static_cast<long long>(n) * p.width;
-    const LossMatrix g{p.g, plan.lde, 0, n * plan.lde};
+    LinLossParams b = p;  // of the block's tokens
+    b.tokens = b.r.rows = p.tokens - t0 < plan.block ? p.tokens - t0 : plan.block;
+    b.r.words += static_cast<long long>(t0) * p.r.top;
+    b.r.q += static_cast<long long>(t0) * p.r.top;
+    b.picked += static_cast<long long>(t0) * p.r.top;
+    b.r.live += t0;
+    b.scale += t0;
+    b.stat += t0;
+    b.loss += t0;
+    b.xp += static_cast<long long>(t0) * p.width;
+    b.bad += t0 / plan.block;
+    const LossMatrix x = x_planes(b), g{b.g, b.ldg, 0, b.tokens * b.ldg};
     LlArgs a{};
     a.pairs = 1;
     a.partial = p.partial;
-    LlOut o{};
     a.a = x;
     a.b = w;
     a.k = p.width;
-    o.rows = n;
+    LlOut o{};
+    o.rows = b.tokens;
     o.cols = p.vocab;
     o.c = p.c;
-    o.scale = p.scale + t0;
-    o.g = p.g;
-    o.ld = plan.lde;
+    o.scale = b.scale;
+    o.g = b.g;
+    o.ld = b.ldg;
     o.row_sums = p.row_sums;
     launch_product<LlLargeN, kModeExp>(a, o, stream);
-    const LlBlock b{t0, n, (p.vocab + 255) / 256 * LlLargeN::kWN, p.row_sums, p.scale + t0, p.g, plan.lde};
-    hipLaunchKernelGGL(ll_block_kernel, dim3((n + kFinishTokens - 1) / kFinishTokens), dim3(kFinishTokens * kFinishSlices), 0,
-                       stream, p, b);
-    hipLaunchKernelGGL(ll_convert_kernel, dim3(n), dim3(256), 0, stream, p, b);
+    hipLaunchKernelGGL(ll_block_kernel, dim3((b.tokens + kFinishTokens - 1) / kFinishTokens),
+                       dim3(kFinishTokens * kFinishSlices), 0, stream, b, (p.vocab + 255) / 256 * LlLargeN::kWN);
+    hipLaunchKernelGGL(ll_convert_kernel, dim3(b.tokens), dim3(256), 0, stream, b);
+    b.only_if = o.only_if = b.bad;
+    launch_losses(b, plan, true, stream);
+    o.scale = b.stat;
+    launch_product<LlLargeN, kModeGrad>(a, o, stream);
+    hipLaunchKernelGGL(ll_wanted_kernel<false>, dim3(static_cast<unsigned>((static_cast<long long>(b.tokens) * p.r.top + 255) / 256)),
+                       dim3(256), 0, stream, b, b.stat, 0, p.vocab);
     a.a = w;
     a.b = g;
     a.k = (p.vocab + kLlK - 1) / kLlK * kLlK;
     o = LlOut{};
     o.rows = p.features;
-    o.cols = n;
+    o.cols = b.tokens;
     o.dx = static_cast<bf16_t*>(p.dx) + t0;
     o.ld_dx = p.tokens;
     o.dx_bf16 = 1;
     o.by = by;
-    o.live = p.r.live + t0;
+    o.live = b.r.live;
     launch_product<LlLargeM, kModeDx>(a, o, stream);
     a.a = g;
     a.b = x;
-    a.k = (n + kLlK - 1) / kLlK * kLlK;
+    a.k = (b.tokens + kLlK - 1) / kLlK * kLlK;
     o = LlOut{};
     o.rows = p.vocab;
     o.cols = p.features;
@@ -1710,17 +1713,12 @@ hipError_t launch_linloss_both(const LinLossParams& given, const LinLossPlan& pl
     o.by = by;
     o.sum = p.tokens > plan.block ? p.dw_sum : nullptr;
     o.add = t0 > 0;
-    o.last = t0 + n == p.tokens;
+    o.last = t0 + b.tokens == p.tokens;
     if (p.dw_bf16) o.h = static_cast<bf16_t*>(p.dw);
     else o.f = static_cast<float*>(p.dw);
     launch_product<LlLargeM, kModeDw>(a, o, stream);
   }
-  p.only_if = p.bad;
-  p.grad = nullptr;
-  launch_losses(p, plan, true, stream);
-  e = launch_loss_mean(p.loss, p.r, p.reduction, p.mean, p.by, stream);
-  if (e != hipSuccess) return e;
-  return launch_linloss_bwd(p, plan, stream);
+  return launch_loss_mean(p.loss, p.r, p.reduction, p.mean, p.by, stream);
 }
 
 hipError_t launch_linloss_rescale(const LinLossParams& p, hipStream_t stream) {

@@ -87,7 +87,7 @@ struct LinLossParams {
   // both directions at once
   float* row_sums;    // [parts_both][block]
   float* dw_sum;      // [vocab][features] where there are blocks
-  int* bad;
+  int* bad;           // [blocks]
   const int* only_if; // NULL, or nothing is done where this is 0
 };
 

@@ -514,6 +514,22 @@ def test_linear_both_directions_far_from_the_target():
 
 
 @pytest.mark.gpu
+def test_linear_both_directions_one_block_far():
+    """Such a token in the second of two blocks, none in the first."""
+    t, d, v = 3000, 640, 212345
+    print(f"case one block far {t} {d} {v}", flush=True)
+    x, w = _inputs(t, d, v, BF16, 17)
+    x[:, 2900] *= 32
+    targets = _targets(t, v, 0.1, 18)
+    targets[2900] = 7
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    loss = linear_cross_entropy(x, w, targets)
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    _check_both(x, w.detach(), lambda part: _wanted_targets(targets[part], v)[0], targets != -100, 1.0, 1, "mean", 1.0, loss, dx, dw)
+
+
+@pytest.mark.gpu
 def test_weight_rows_far_apart():
     t, d, v = 300, 64, 300
     x, w = _inputs(t, d, v, BF16, 1)
