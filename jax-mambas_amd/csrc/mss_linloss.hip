@@ -144,6 +144,7 @@ struct LlArgs {
   int teams;             // of the gradients' products
   int whole, rest;       // whole ranges of a team; the first range of those whose units the teams share evenly
   float* partial;        // their tiles' parts
+  long long room;        // floats that these have
 };
 
 // kModeExp leaves s - ref, both to base 2, in steps of 2^-9 from -48 on: 0 to 65535 as a part of 65535, and 0 also below.
@@ -1350,70 +1351,93 @@ LlTeams ll_teams(int size, int ranges, int units) {
   return {teams, whole, whole * teams};
 }
 
+// How a gradient's product of `rows` by `cols`, its k `stages` long over all pairs of planes, is shared out.
+struct LlShare {
+  int tiles_m, tiles_n, units, size, ranges;
+  LlTeams t;
+  long long sums;  // floats of the teams' parts
+};
+
+template <class S, int kMode>
+LlShare ll_share(int rows, int cols, int stages) {
+  LlShare h{};
+  h.tiles_m = (rows + S::kM - 1) / S::kM;
+  h.tiles_n = (cols + S::kN - 1) / S::kN;
+  h.units = (stages + S::kRing - 1) / S::kRing;
+  h.size = kMode == kModeDx ? h.tiles_m : h.tiles_n;
+  h.ranges = kMode == kModeDx ? h.tiles_n : h.tiles_m;
+  h.t = ll_teams<S>(h.size, h.ranges, h.units);
+  h.sums = h.t.rest == h.ranges ? 0 : 2LL * h.t.teams * h.size * S::kM * S::kN;
+  return h;
+}
+
+// The gradients' k is taken up to whole steps of kLlK.
+int grad_k(int n) { return (n + kLlK - 1) / kLlK * kLlK; }
+
+// Floats of the parts of one piece's gradients: dx of `features` by `tokens` over `words`, dw of `words` by `features` over
+// `tokens`, in tiles of SX and SW.
+template <class SX, class SW>
+long long part_sums(int features, int tokens, int words, int pairs) {
+  return std::max(ll_share<SX, kModeDx>(features, tokens, grad_k(words) / SX::kBK * pairs).sums,
+                  ll_share<SW, kModeDw>(words, features, grad_k(tokens) / SW::kBK * pairs).sums);
+}
+
+// (A gradient's parts have to fit the workspace that the plan asked for: refused, if they ever should not.)
 template <class S, int kMode, bool kF32 = false>
-void launch_product(LlArgs a, const LlOut& o, hipStream_t stream) {
-  a.tiles_m = (o.rows + S::kM - 1) / S::kM;
-  a.tiles_n = (o.cols + S::kN - 1) / S::kN;
+hipError_t launch_product(LlArgs a, const LlOut& o, hipStream_t stream) {
   const int stages = a.k / S::kBK * a.pairs;
-  a.units = (stages + S::kRing - 1) / S::kRing;
-  const int room = kCUs * S::kPerCU;
-  const long long tiles = static_cast<long long>(a.tiles_m) * a.tiles_n;
   if constexpr (kLlTeams<kMode>) {
-    const int size = kMode == kModeDx ? a.tiles_m : a.tiles_n;
-    const LlTeams t = ll_teams<S>(size, kMode == kModeDx ? a.tiles_n : a.tiles_m, a.units);
-    a.teams = t.teams;
-    a.whole = t.whole;
-    a.rest = t.rest;
-    hipLaunchKernelGGL((ll_kernel<S, kMode, kF32>), dim3(a.teams * size), dim3(S::kThreads), 0, stream, a, o);
-    const int shared = (kMode == kModeDx ? a.tiles_n : a.tiles_m) - a.rest;
+    const LlShare h = ll_share<S, kMode>(o.rows, o.cols, stages);
+    if (h.sums > a.room) return hipErrorInvalidValue;
+    a.tiles_m = h.tiles_m;
+    a.tiles_n = h.tiles_n;
+    a.units = h.units;
+    a.teams = h.t.teams;
+    a.whole = h.t.whole;
+    a.rest = h.t.rest;
+    hipLaunchKernelGGL((ll_kernel<S, kMode, kF32>), dim3(a.teams * h.size), dim3(S::kThreads), 0, stream, a, o);
+    const int shared = h.ranges - a.rest;
     if (shared > 0)
-      hipLaunchKernelGGL((ll_join_kernel<S, kMode, kF32>), dim3(static_cast<unsigned>(shared) * size * S::kWaves * S::kMT),
+      hipLaunchKernelGGL((ll_join_kernel<S, kMode, kF32>), dim3(static_cast<unsigned>(shared) * h.size * S::kWaves * S::kMT),
                          dim3(64 * kJoinWaves), 0, stream, a, o);
   } else {
+    a.tiles_m = (o.rows + S::kM - 1) / S::kM;
+    a.tiles_n = (o.cols + S::kN - 1) / S::kN;
+    a.units = (stages + S::kRing - 1) / S::kRing;
+    const int room = kCUs * S::kPerCU;
+    const long long tiles = static_cast<long long>(a.tiles_m) * a.tiles_n;
     hipLaunchKernelGGL((ll_kernel<S, kMode, kF32>), dim3(static_cast<unsigned>(tiles < room ? tiles : room)), dim3(S::kThreads), 0,
                        stream, a, o);
   }
+  return hipSuccess;
 }
 
-// f of the shape of a gradient's product.
+// f of the tiles of dx and of dw, as launch_shaped takes them.
 template <typename F>
-auto with_shape(int shape, F&& f) {
-  return shape == 0 ? f(LlSmall{}) : shape == 1 ? f(LlLargeM{}) : f(LlThinN{});
+auto with_grad_shapes(int shape_x, int shape_w, F&& f) {
+  const auto both = [&](auto x) { return shape_w == 1 ? f(x, LlLargeM{}) : f(x, LlSmall{}); };
+  return shape_x == 0 ? both(LlSmall{}) : shape_x == 1 ? both(LlLargeM{}) : both(LlThinN{});
 }
 
 template <int kMode, bool kF32>
-void launch_shaped(const LinLossPlan& plan, const LlArgs& a, const LlOut& o, hipStream_t stream) {
+hipError_t launch_shaped(const LinLossPlan& plan, const LlArgs& a, const LlOut& o, hipStream_t stream) {
   if constexpr (kMode == kModeGrad) {
-    if (plan.shape == 0) launch_product<LlSmall, kMode, kF32>(a, o, stream);
-    else if (plan.shape == 1) launch_product<LlLargeN, kMode, kF32>(a, o, stream);
-    else if (plan.shape == 3) launch_product<LlMidN, kMode, kF32>(a, o, stream);
-    else launch_product<LlThinM, kMode, kF32>(a, o, stream);
+    if (plan.shape == 0) return launch_product<LlSmall, kMode, kF32>(a, o, stream);
+    if (plan.shape == 1) return launch_product<LlLargeN, kMode, kF32>(a, o, stream);
+    if (plan.shape == 3) return launch_product<LlMidN, kMode, kF32>(a, o, stream);
+    return launch_product<LlThinM, kMode, kF32>(a, o, stream);
   } else if constexpr (kMode == kModeDw) {
-    if (plan.shape_w == 1) launch_product<LlLargeM, kMode, kF32>(a, o, stream);
-    else launch_product<LlSmall, kMode, kF32>(a, o, stream);
+    if (plan.shape_w == 1) return launch_product<LlLargeM, kMode, kF32>(a, o, stream);
+    return launch_product<LlSmall, kMode, kF32>(a, o, stream);
   } else {
     const int shape = kMode == kModeDx ? plan.shape_x : plan.shape;
     if constexpr (kMode == kModeLse) {
       if (shape == 3) return launch_product<LlMidM, kMode, kF32>(a, o, stream);
     }
-    if (shape == 0) launch_product<LlSmall, kMode, kF32>(a, o, stream);
-    else if (shape == 1) launch_product<LlLargeM, kMode, kF32>(a, o, stream);
-    else launch_product<LlThinN, kMode, kF32>(a, o, stream);
+    if (shape == 0) return launch_product<LlSmall, kMode, kF32>(a, o, stream);
+    if (shape == 1) return launch_product<LlLargeM, kMode, kF32>(a, o, stream);
+    return launch_product<LlThinN, kMode, kF32>(a, o, stream);
   }
-}
-
-// Floats of the teams' parts in a gradient's product of `features` by `others`.
-template <class S>
-long long part_sums(int features, int others, int stages) {
-  // (features are the tiles' rows in dx, their columns in dw)
-  const int tile_f = S::kM, tile_o = S::kN;
-  const long long size_x = (features + tile_f - 1) / tile_f, ranges_x = (others + tile_o - 1) / tile_o;
-  const long long size_w = (features + tile_o - 1) / tile_o, ranges_w = (others + tile_f - 1) / tile_f;
-  const int units = (stages + S::kRing - 1) / S::kRing;
-  const LlTeams x = ll_teams<S>(static_cast<int>(size_x), static_cast<int>(ranges_x), units);
-  const LlTeams w = ll_teams<S>(static_cast<int>(size_w), static_cast<int>(ranges_w), units);
-  const long long nx = x.rest == ranges_x ? 0 : 2LL * x.teams * size_x, nw = w.rest == ranges_w ? 0 : 2LL * w.teams * size_w;
-  return (nx > nw ? nx : nw) * S::kM * S::kN;
 }
 
 LossMatrix weight_planes(const LinLossParams& p) {
@@ -1469,11 +1493,12 @@ LinLossPlan linloss_plan(int tokens, int features, int vocab, int planes) {
   const auto large = [](int rows, int cols) { return 4. * tiles_of(rows, cols, 256, 256) <= 1.4 * tiles_of(rows, cols, 128, 128); };
   q.shape_x = tokens <= 32 ? 2 : tokens > 384 && large(features, tokens) ? 1 : 0;
   q.shape_w = large(words, features) ? 1 : 0;
-  const int x_stages = q.piece / 64 * (planes == 1 ? 1 : kPairs);
-  const int w_stages = (tokens + kLlK - 1) / kLlK * (kLlK / 64) * (planes == 1 ? 1 : kPairs);
-  const long long x = with_shape(q.shape_x, [&](auto s) { return part_sums<decltype(s)>(features, tokens, x_stages); });
-  const long long w = with_shape(q.shape_w, [&](auto s) { return part_sums<decltype(s)>(features, words, w_stages); });
-  q.partial = x > w ? x : w;
+  // (The last piece may be shorter, and be shared out in another way.)
+  const int last = vocab - (vocab - 1) / q.piece * q.piece;
+  q.partial = with_grad_shapes(q.shape_x, q.shape_w, [&](auto x, auto w) {
+    const auto of = [&](int n) { return part_sums<decltype(x), decltype(w)>(features, tokens, n, planes == 1 ? 1 : kPairs); };
+    return std::max(of(words), of(last));
+  });
   // Both directions at once, where the logits' product costs more than their 16 bits read and g written, which its
   // features decide, and launches that may not be needed (us of both, apart and at once, x 50280: 4096 x 256 612 and 690;
   // 512 x 768 276 and 276; 1024 x 768 433 and 408; 16384 x 768 4875 and 4536; 2048 x 2560 2071 and 1723; 131072 x
@@ -1483,17 +1508,9 @@ LinLossPlan linloss_plan(int tokens, int features, int vocab, int planes) {
     q.lde = whole;
     const long long rows = (1LL << 30) / (2 * q.lde) / 256 * 256, blocks = (tokens + rows - 1) / rows;
     q.block = static_cast<int>(((tokens + blocks - 1) / blocks + 255) / 256 * 256);
-    const int n = q.block < tokens ? q.block : tokens;
-    const long long bx = part_sums<LlLargeM>(features, n, static_cast<int>((vocab + kLlK - 1) / kLlK * (kLlK / 64)));
-    const long long bw = part_sums<LlLargeM>(features, vocab, (n + kLlK - 1) / kLlK * (kLlK / 64));
-    q.partial_both = bx > bw ? bx : bw;
-    // (the last block may be shorter, and be shared out in another way)
-    const int rest = tokens % q.block;
-    if (rest > 0) {
-      const long long rx = part_sums<LlLargeM>(features, rest, static_cast<int>((vocab + kLlK - 1) / kLlK * (kLlK / 64)));
-      const long long rw = part_sums<LlLargeM>(features, vocab, (rest + kLlK - 1) / kLlK * (kLlK / 64));
-      q.partial_both = std::max(q.partial_both, std::max(rx, rw));
-    }
+    const int n = q.block < tokens ? q.block : tokens, last_n = tokens - (tokens - 1) / q.block * q.block;
+    const auto of = [&](int t) { return part_sums<LlLargeM, LlLargeM>(features, t, vocab, 1); };
+    q.partial_both = std::max(of(n), of(last_n));  // (so may the last block)
     q.parts_both = static_cast<int>(whole / 256) * LlLargeN::kWN;
   }
   return q;
@@ -1519,7 +1536,7 @@ static hipError_t launch_operands(const LinLossParams& p, hipStream_t stream) {
 }
 
 // The words' logits (unless they are there), the sums over the vocabulary, the tokens' losses.
-static void launch_losses(const LinLossParams& p, const LinLossPlan& plan, bool picked, hipStream_t stream) {
+static hipError_t launch_losses(const LinLossParams& p, const LinLossPlan& plan, bool picked, hipStream_t stream) {
   const bool f32 = p.planes == 2, lists = p.r.targets == nullptr;
   LlArgs a{};
   a.a = weight_planes(p);
@@ -1533,8 +1550,8 @@ static void launch_losses(const LinLossParams& p, const LinLossPlan& plan, bool 
   o.part = p.part;
   o.powers = p.powers;
   o.only_if = p.only_if;
-  if (f32) launch_shaped<kModeLse, true>(plan, a, o, stream);
-  else launch_shaped<kModeLse, false>(plan, a, o, stream);
+  const hipError_t e = f32 ? launch_shaped<kModeLse, true>(plan, a, o, stream) : launch_shaped<kModeLse, false>(plan, a, o, stream);
+  if (e != hipSuccess) return e;
   const dim3 fg((p.tokens + kFinishTokens - 1) / kFinishTokens), fb(kFinishTokens * kFinishSlices);
   if (picked) {
     hipLaunchKernelGGL((ll_finish_kernel<false, false>), fg, fb, 0, stream, p, a.a);
@@ -1549,14 +1566,14 @@ static void launch_losses(const LinLossParams& p, const LinLossPlan& plan, bool 
   } else {
     hipLaunchKernelGGL((ll_finish_kernel<true, false>), fg, fb, 0, stream, p, a.a);
   }
+  return hipGetLastError();
 }
 
 hipError_t launch_linloss_fwd(const LinLossParams& p, const LinLossPlan& plan, hipStream_t stream) {
-  const hipError_t e = launch_operands(p, stream);
-  if (e != hipSuccess) return e;
-  launch_losses(p, plan, false, stream);
-  if (p.reduction != kLossNone) return launch_loss_mean(p.loss, p.r, p.reduction, p.mean, p.by, stream);
-  return hipGetLastError();
+  hipError_t e = launch_operands(p, stream);
+  if (e == hipSuccess) e = launch_losses(p, plan, false, stream);
+  if (e != hipSuccess || p.reduction == kLossNone) return e;
+  return launch_loss_mean(p.loss, p.r, p.reduction, p.mean, p.by, stream);
 }
 
 hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, hipStream_t stream) {
@@ -1571,6 +1588,7 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
   LlScale by{p.reduction == kLossNone ? nullptr : p.grad, p.reduction == kLossMean ? p.by : nullptr,
              p.reduction == kLossNone ? 1.f : p.temperature,
              nullptr, f32 && p.reduction == kLossNone ? p.power_g : nullptr};
+  hipError_t e = hipSuccess;
   for (long long v0 = 0; v0 < p.vocab; v0 += p.piece) {
     const int words = static_cast<int>(p.vocab - v0 < p.piece ? p.vocab - v0 : p.piece);
     LossMatrix wp = w;
@@ -1588,6 +1606,7 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
     a.b = wp;
     a.k = p.width;
     a.partial = p.partial;
+    a.room = plan.partial;
     LlOut o{};
     o.rows = p.tokens;
     o.cols = words;
@@ -1597,15 +1616,15 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
     o.ld = p.ldg;
     o.plane = g.plane;
     o.powers = p.powers;
-    if (f32) launch_shaped<kModeGrad, true>(plan, a, o, stream);
-    else launch_shaped<kModeGrad, false>(plan, a, o, stream);
+    e = f32 ? launch_shaped<kModeGrad, true>(plan, a, o, stream) : launch_shaped<kModeGrad, false>(plan, a, o, stream);
+    if (e != hipSuccess) return e;
     const dim3 wg(static_cast<unsigned>((static_cast<long long>(p.tokens) * p.r.top + 255) / 256));
     if (f32) hipLaunchKernelGGL(ll_wanted_kernel<true>, wg, dim3(256), 0, stream, p, scale, static_cast<int>(v0), words);
     else hipLaunchKernelGGL(ll_wanted_kernel<false>, wg, dim3(256), 0, stream, p, scale, static_cast<int>(v0), words);
     if (p.dx != nullptr) {
       a.a = wp;
       a.b = g;
-      a.k = (words + kLlK - 1) / kLlK * kLlK;
+      a.k = grad_k(words);
       o = LlOut{};
       o.rows = p.features;
       o.cols = p.tokens;
@@ -1621,13 +1640,13 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
         o.by.power = f32 ? p.powers + 1 : nullptr;
         o.live = p.r.live;
       }
-      if (f32) launch_shaped<kModeDx, true>(plan, a, o, stream);
-      else launch_shaped<kModeDx, false>(plan, a, o, stream);
+      e = f32 ? launch_shaped<kModeDx, true>(plan, a, o, stream) : launch_shaped<kModeDx, false>(plan, a, o, stream);
+      if (e != hipSuccess) return e;
     }
     if (p.dw != nullptr) {
       a.a = g;
       a.b = x;
-      a.k = (p.tokens + kLlK - 1) / kLlK * kLlK;
+      a.k = grad_k(p.tokens);
       o = LlOut{};
       o.rows = words;
       o.cols = p.features;
@@ -1637,8 +1656,8 @@ hipError_t launch_linloss_bwd(const LinLossParams& p, const LinLossPlan& plan, h
       void* dst = static_cast<char*>(p.dw) + v0 * p.features * (p.dw_bf16 ? 2 : 4);
       if (p.dw_bf16) o.h = static_cast<bf16_t*>(dst);
       else o.f = static_cast<float*>(dst);
-      if (f32) launch_shaped<kModeDw, true>(plan, a, o, stream);
-      else launch_shaped<kModeDw, false>(plan, a, o, stream);
+      e = f32 ? launch_shaped<kModeDw, true>(plan, a, o, stream) : launch_shaped<kModeDw, false>(plan, a, o, stream);
+      if (e != hipSuccess) return e;
     }
   }
   return hipGetLastError();
@@ -1670,6 +1689,7 @@ hipError_t launch_linloss_both(const LinLossParams& p, const LinLossPlan& plan, 
     LlArgs a{};
     a.pairs = 1;
     a.partial = p.partial;
+    a.room = plan.partial_both;
     a.a = x;
     a.b = w;
     a.k = p.width;
@@ -1681,19 +1701,22 @@ hipError_t launch_linloss_both(const LinLossParams& p, const LinLossPlan& plan, 
     o.g = b.g;
     o.ld = b.ldg;
     o.row_sums = p.row_sums;
-    launch_product<LlLargeN, kModeExp>(a, o, stream);
+    e = launch_product<LlLargeN, kModeExp>(a, o, stream);
+    if (e != hipSuccess) return e;
     hipLaunchKernelGGL(ll_block_kernel, dim3((b.tokens + kFinishTokens - 1) / kFinishTokens),
                        dim3(kFinishTokens * kFinishSlices), 0, stream, b, (p.vocab + 255) / 256 * LlLargeN::kWN);
     hipLaunchKernelGGL(ll_convert_kernel, dim3(b.tokens), dim3(256), 0, stream, b);
     b.only_if = o.only_if = b.bad;
-    launch_losses(b, plan, true, stream);
+    e = launch_losses(b, plan, true, stream);
+    if (e != hipSuccess) return e;
     o.scale = b.stat;
-    launch_product<LlLargeN, kModeGrad>(a, o, stream);
+    e = launch_product<LlLargeN, kModeGrad>(a, o, stream);
+    if (e != hipSuccess) return e;
     hipLaunchKernelGGL(ll_wanted_kernel<false>, dim3(static_cast<unsigned>((static_cast<long long>(b.tokens) * p.r.top + 255) / 256)),
                        dim3(256), 0, stream, b, b.stat, 0, p.vocab);
     a.a = w;
     a.b = g;
-    a.k = (p.vocab + kLlK - 1) / kLlK * kLlK;
+    a.k = grad_k(p.vocab);
     o = LlOut{};
     o.rows = p.features;
     o.cols = b.tokens;
@@ -1702,10 +1725,11 @@ hipError_t launch_linloss_both(const LinLossParams& p, const LinLossPlan& plan, 
     o.dx_bf16 = 1;
     o.by = by;
     o.live = b.r.live;
-    launch_product<LlLargeM, kModeDx>(a, o, stream);
+    e = launch_product<LlLargeM, kModeDx>(a, o, stream);
+    if (e != hipSuccess) return e;
     a.a = g;
     a.b = x;
-    a.k = (b.tokens + kLlK - 1) / kLlK * kLlK;
+    a.k = grad_k(b.tokens);
     o = LlOut{};
     o.rows = p.vocab;
     o.cols = p.features;
@@ -1716,7 +1740,8 @@ hipError_t launch_linloss_both(const LinLossParams& p, const LinLossPlan& plan, 
     o.last = t0 + b.tokens == p.tokens;
     if (p.dw_bf16) o.h = static_cast<bf16_t*>(p.dw);
     else o.f = static_cast<float*>(p.dw);
-    launch_product<LlLargeM, kModeDw>(a, o, stream);
+    e = launch_product<LlLargeM, kModeDw>(a, o, stream);
+    if (e != hipSuccess) return e;
   }
   return launch_loss_mean(p.loss, p.r, p.reduction, p.mean, p.by, stream);
 }

@@ -105,6 +105,88 @@ def test_linear_workspaces(lib):
     assert saved[0] == saved[1] and saved[2] >= saved[1] + 100 * 64 * 2
 
 
+# Tiles of the gradients' products: rows, columns, stages of the ring, workgroups a CU.
+SMALL, LARGE, THIN = (128, 128, 2, 2), (256, 256, 2, 1), (128, 32, 4, 2)
+
+
+def _parts(tile, rows, cols, k, pairs, dx):
+    """Floats of the parts that the product's teams leave: 256 CUs' workgroups in teams of one for each tile of features;
+    ranges that are dealt out whole unless some team would then be 8 units longer than an even share, two parts
+    a team else."""
+    up = lambda a, b: -(-a // b)
+    m, n, ring, per_cu = tile
+    units = up(up(k, 128) * 2 * pairs, ring)
+    size, ranges = (up(rows, m), up(cols, n))[::1 if dx else -1]
+    units_all, at_once = ranges * units, max(1, 256 * per_cu // size)
+    shares = max(1, min(units_all // 8, at_once))
+    whole = up(ranges, at_once) * units <= units_all // shares + 8
+    return 0 if whole else 2 * shares * size * m * n
+
+
+def _backward_plan(t, d, v, planes):
+    """The pieces of the vocabulary and, for each, the floats of its gradients' parts."""
+    up = lambda a, b: -(-a // b)
+    most = max(256, (1 << 30) // (2 * planes * t) // 256 * 256)
+    piece = up(up(v, 256), up(up(v, 256) * 256, most)) * 256
+    large = lambda r, c: 4 * up(r, 256) * up(c, 256) <= 1.4 * up(r, 128) * up(c, 128)
+    tile_x = THIN if t <= 32 else LARGE if t > 384 and large(d, t) else SMALL
+    tile_w = LARGE if large(min(piece, v), d) else SMALL
+    pairs = 1 if planes == 1 else 3
+    words = {min(piece, v - a) for a in range(0, v, piece)}
+    return piece, max(max(_parts(tile_x, d, t, n, pairs, True), _parts(tile_w, n, d, t, pairs, False)) for n in words)
+
+
+def _sweep():
+    shapes = [(16384, 1024, 32000), (24576, 2048, 32000), (19037, 2560, 152390), (16384, 896, 128256), (16384, 1024, 128256),
+              (32768, 2048, 32000), (1602, 320, 352845), (543, 384, 554631), (1, 64, 1 << 20), (33, 40, 1 << 20)]
+    for v in (4096, 10007, 32000, 32768, 50280, 65024, 100352, 128256, 152064, 202048, 256000):
+        for d in (64, 320, 512, 640, 768, 896, 1024, 1536, 2048, 2560, 4096):
+            shapes += [(t, d, v) for t in range(1024, 32769, 1024)]
+    return shapes
+
+
+def test_linear_workspace_holds_the_parts_of_every_piece(lib):
+    """The parts are the workspace's last buffer. Its size has to be what the largest of the vocabulary's pieces leaves:
+    the last one has fewer words, and may be shared out where the others are dealt out whole."""
+    step = lambda n: -(-n // 256) * 256
+    several = 0
+    for t, d, v in _sweep():
+        for planes in (1, 2):
+            for reduction in (0, 2):
+                a = _lib.LinearLossArgs(**{**LINEAR, "tokens": t, "features": d, "vocab": v, "ldw": d, "reduction": reduction,
+                                           "io_dtype": 2 - planes})
+                piece, parts = _backward_plan(t, d, v, planes)
+                before = (step(8 * (t + 256)) if reduction == 0 else 0) + 256 + step(2 * planes * t * piece)
+                before += step(4 * d * (-(-t // 4) * 4)) if piece < v else 0
+                room = lib.mss_linear_loss_workspace_bytes(a, 1) - before
+                assert room == step(4 * parts), (t, d, v, planes, room, 4 * parts)
+                several += piece < v
+    assert several > 1000
+
+
+def test_linear_workspace_holds_the_parts_of_every_block(lib):
+    """The same for both directions at once, in blocks of tokens."""
+    step = lambda n: -(-n // 256) * 256
+    several = 0
+    for t, d, v in _sweep():
+        a = _lib.LinearLossArgs(**{**LINEAR, "tokens": t, "features": d, "vocab": v, "ldw": d})
+        total = lib.mss_linear_loss_workspace_bytes(a, 2)
+        if total == 0:
+            continue
+        lde = -(-v // 256) * 256
+        rows = (1 << 30) // (2 * lde) // 256 * 256
+        block = -(--(-t // -(-t // rows)) // 256) * 256
+        parts = max(max(_parts(LARGE, d, n, v, 1, True), _parts(LARGE, v, d, n, 1, False))
+                    for n in {min(block, t - b) for b in range(0, t, block)})
+        rest = total - step(4 * parts)
+        # (what else is there: sums of the forward call's tiles, scales, the block's logits, sums of rows and of dw, notes)
+        least = step(8 * (t + 256)) + step(2 * block * lde) + step(lde // 256 * 2 * block * 4) + (step(4 * v * d) if block < t else 0)
+        sums = rest - least - step(4 * -(-t // block))
+        assert sums in [step(8 * t * n) for n in (-(-v // 128) * 2, -(-v // 256) * 2, -(-v // 256) * 4)], (t, d, v)
+        several += block < t
+    assert several > 1000
+
+
 DISTILL = dict(rows=20, vocab=100, top=5, io_dtype=1, teacher_dtype=0, reduction=2, temperature=1.0, ld=100, logits=P, ids=2 * P,
                teacher=3 * P, loss=4 * P, mean=5 * P, saved=6 * P, saved_bytes=1 << 31, grad=7 * P, dlogits=8 * P)
 
@@ -382,6 +464,40 @@ def test_linear_cross_entropy_many_tiles(dtype, t, d, v):
         dw_want = dw_want + torch.mm(g.t(), xd.t())
         dw_tol = dw_tol + _product_tol(g_tol.t(), g.t(), xd.t(), t)
     _check("loss", loss, total, losses + 2 * U * total)
+    half = HALF[dtype]
+    _check("dw", dw, dw_want, (dw_tol + 8 * U * dw_want.abs()) * (1 + half) + half * dw_want.abs())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,t,d,v,reduction", [(BF16, 1602, 320, 352845, "none"), (F32, 543, 384, 554631, "mean")])
+def test_linear_last_piece_shared_otherwise(dtype, t, d, v, reduction):
+    """A last piece of the vocabulary whose ranges the teams share where they take the other pieces' whole."""
+    print(f"case last piece {dtype} {t} {d} {v} {reduction}", flush=True)
+    piece, parts = _backward_plan(t, d, v, 1 if dtype == BF16 else 2)
+    first = _backward_plan(t, d, piece, 1 if dtype == BF16 else 2)
+    assert piece < v and first[0] == piece and first[1] < parts
+    x, w = _inputs(t, d, v, dtype, 21)
+    targets = _targets(t, v, 0.1, 22)
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    loss = linear_cross_entropy(x, w, targets, reduction=reduction)
+    up = torch.linspace(-1.0, 2.0, t, device="cuda") if reduction == "none" else torch.tensor(1.0, device="cuda")
+    dx, dw = torch.autograd.grad(loss, (x, w), up)
+    by = 1.0 / int((targets != -100).sum()) if reduction == "mean" else 1.0
+    total, tol, dw_want, dw_tol = 0.0, 0.0, 0.0, 0.0
+    for a in range(0, t, 256):
+        part = slice(a, min(t, a + 256))
+        ref, xd, wd = _linear_reference(x.detach()[:, part], w, *_wanted_targets(targets[part], v), 1.0, 1)
+        scale = up.double()[part] if reduction == "none" else torch.full_like(ref.loss, by)
+        if reduction == "none":
+            _check("loss", loss[part], ref.loss, ref.loss_tol)
+        total, tol = total + ref.loss.sum() * by, tol + ref.loss_tol.sum() * by
+        _check_linear_grads(ref, xd, wd, scale, dtype, dtype, dx[:, part], None)
+        g, g_tol = ref.g * scale[:, None], ref.g_tol * scale[:, None].abs()
+        dw_want = dw_want + torch.mm(g.t(), xd.t())
+        dw_tol = dw_tol + _product_tol(g_tol.t(), g.t(), xd.t(), t)
+    if reduction == "mean":
+        _check("loss", loss, total, tol + 2 * U * total)
     half = HALF[dtype]
     _check("dw", dw, dw_want, (dw_tol + 8 * U * dw_want.abs()) * (1 + half) + half * dw_want.abs())
 
