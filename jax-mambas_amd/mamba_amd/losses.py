@@ -85,6 +85,16 @@ def _bytes(n, device):
     return torch.empty(n, dtype=torch.uint8, device=device)
 
 
+def _row_stride(m):
+    return m.stride(0) if m.shape[0] > 1 else m.shape[1]
+
+
+def _weight_rows(w):
+    """`w` with contiguous rows that do not overlap."""
+    v, f = w.shape
+    return w.contiguous() if f > 1 and w.stride(1) != 1 or v > 1 and w.stride(0) < f else w
+
+
 def _upstream(grad, reduction, rows):
     """The upstream gradient as the kernels read it."""
     g = _resolved(grad).to(_F32)
@@ -106,7 +116,7 @@ class _LinearLoss(torch.autograd.Function):
                                 io_dtype=_io_tag(x.dtype, "x"), teacher_dtype=teacher_tag, reduction=reduction,
                                 temperature=temperature, ignore_index=ignore_index,
                                 stride_f=x.stride(0) if f > 1 else 0, stride_t=x.stride(1) if t > 1 else 0,
-                                ldw=w.stride(0) if w.shape[0] > 1 else f, x=x.data_ptr(), weight=w.data_ptr(),
+                                ldw=_row_stride(w), x=x.data_ptr(), weight=w.data_ptr(),
                                 targets=_ptr(targets), ids=_ptr(ids), teacher=_ptr(teacher))
         dev = x.device
         with _guard(x):
@@ -146,7 +156,13 @@ class _LinearLoss(torch.autograd.Function):
             grad = _upstream(grad, src.reduction, src.tokens)
             a = _lib.LinearLossArgs.from_buffer_copy(src)
             a.x = a.loss = a.mean = a.targets = a.ids = a.teacher = None
-            a.weight = w.data_ptr()
+            # (Saved-tensor hooks may have put both elsewhere, and the weight's rows at another distance.)
+            a.saved, a.saved_bytes = saved.data_ptr(), saved.numel()
+            w = _weight_rows(w)
+            a.weight, a.ldw = w.data_ptr(), _row_stride(w)
+            if saved.numel() < lib.mss_linear_loss_saved_bytes(a):  # it was read in place, and cannot be here
+                w = w.clone(memory_format=torch.contiguous_format)
+                a.weight, a.ldw = w.data_ptr(), _row_stride(w)
             a.dw_dtype = _io_tag(ctx.dw_dtype, "weight")
             d, ctx.d = ctx.d, None  # the caller may write over them
             if d is not None:
@@ -191,9 +207,7 @@ def _linear_loss(x, weight, weight_act, holder, targets, ids, teacher, ignore_in
         weight_act = weight.detach() if weight.dtype == x.dtype else weight.detach().to(x.dtype)
     else:
         weight_act = weight_act.detach()
-    weight_act = _resolved(weight_act)
-    if f > 1 and weight_act.stride(1) != 1 or vocab > 1 and weight_act.stride(0) < f:
-        weight_act = weight_act.contiguous()
+    weight_act = _weight_rows(_resolved(weight_act))
     conform = [None if v is None else _resolved(v).contiguous() for v in (targets, ids, teacher)]
     both = reduction != _lib.MSS_LOSS_NONE and torch.is_grad_enabled() and x.requires_grad and weight.requires_grad
     return _LinearLoss.apply(_resolved(x), weight, weight_act, *conform, ignore_index, temperature, reduction, teacher_tag,

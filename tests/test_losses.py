@@ -259,6 +259,85 @@ def test_python_refusals():
         ds(torch.zeros(1, 1).expand(rows, 1), torch.zeros(1, 1, dtype=torch.int64).expand(rows, 1), torch.zeros(1, 1).expand(rows, 1))
 
 
+class _Hooks:
+    """Saved-tensor hooks that keep a copy, as offloading and checkpoints do; `layout` gives the copy its layout."""
+
+    def __init__(self, layout=torch.Tensor.clone):
+        self.layout, self.unpacked = layout, []
+
+    def pack(self, t):
+        return self.layout(t.detach())
+
+    def unpack(self, t):
+        self.unpacked.append(t)
+        return t
+
+    def __enter__(self):
+        self.context = torch.autograd.graph.saved_tensors_hooks(self.pack, self.unpack)
+        return self.context.__enter__()
+
+    def __exit__(self, *e):
+        return self.context.__exit__(*e)
+
+
+class _Calls:
+    """The library, its sizes its own, with calls that are noted instead of made."""
+
+    def __init__(self, lib):
+        self.lib, self.seen = lib, []
+
+    def __getattr__(self, name):
+        if name.endswith("_bytes"):
+            return getattr(self.lib, name)
+
+        def call(a, stream):
+            self.seen.append((name, type(a).from_buffer_copy(a)))
+            return 0
+        return call
+
+
+@pytest.fixture
+def calls(lib, monkeypatch):
+    import contextlib
+
+    from mamba_amd import losses
+    noted = _Calls(lib)
+    monkeypatch.setattr(losses._lib, "register_hip_kernel", lambda: noted)
+    monkeypatch.setattr(losses, "_stream", lambda t: None)
+    monkeypatch.setattr(losses, "_require_gpu", lambda *a: None)
+    monkeypatch.setattr(losses, "_guard", lambda t: contextlib.nullcontext())
+    return noted
+
+
+def _off_16(t):
+    """A copy whose rows lie off 16 bytes and further apart."""
+    if t.dim() != 2:
+        return t.clone()
+    wide = torch.zeros(t.shape[0], t.shape[1] + 3, dtype=t.dtype)
+    wide[:, 1:1 + t.shape[1]] = t
+    return wide[:, 1:1 + t.shape[1]]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("d,layout,given", [(64, "clone", "plain"), (64, "off", "plain"), (64, "clone", "off"), (64, "t", "plain"),
+                                            (40, "clone", "plain"), (40, "off", "plain")])
+def test_linear_backward_reads_what_the_hooks_return(calls, lib, dtype, d, layout, given):
+    x, w = torch.randn(d, 20).to(dtype).requires_grad_(True), torch.randn(100, d).to(dtype)
+    w = (_off_16(w) if given == "off" else w).requires_grad_(True)
+    hooks = _Hooks({"clone": lambda t: t.clone(memory_format=torch.contiguous_format), "off": _off_16,
+                    "t": lambda t: t.t().contiguous().t() if t.dim() == 2 else t.clone()}[layout])
+    with hooks:
+        loss = linear_cross_entropy(x, w, torch.zeros(20, dtype=torch.int64))
+    torch.autograd.grad(loss, (x, w))
+    (_, fwd), (name, a) = calls.seen
+    w2, saved = hooks.unpacked
+    assert name == "mss_linear_loss_bwd" and a.saved == saved.data_ptr() != fwd.saved and a.saved_bytes == saved.numel()
+    assert a.weight != fwd.weight and a.ldw >= d
+    assert lib.mss_linear_loss_saved_bytes(a) <= a.saved_bytes  # what the call takes from it is there
+    if layout == "clone":
+        assert a.weight == w2.data_ptr() and a.ldw == d
+
+
 # ------------------------------------------------------------------------------- the definitions
 def _wanted_targets(targets, vocab, ignore=-100):
     q = torch.zeros(targets.shape[0], vocab, dtype=torch.float64, device=targets.device)
@@ -1006,3 +1085,47 @@ def test_second_backward_and_input_changes():
         w.mul_(2.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         torch.autograd.grad(loss, (x,))
+
+
+def _saved_elsewhere(run, way):
+    """run() with what it saves put elsewhere until the backward pass, and what it had before written over."""
+    if way == "checkpoint":
+        from torch.utils.checkpoint import checkpoint
+        return checkpoint(run, use_reentrant=False)
+    with (torch.autograd.graph.save_on_cpu() if way == "cpu" else _Hooks()):
+        loss = run()
+    torch.cuda.synchronize()
+    full = [torch.full((n,), 0x7f, dtype=torch.uint8, device="cuda") for n in (1 << 12, 1 << 16, 1 << 19, 1 << 20, 1 << 22, 1 << 24) for _ in range(8)]
+    del full
+    return loss
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("way", ["clone", "cpu", "checkpoint"])
+@pytest.mark.parametrize("dtype,d,layout,reduction", [(BF16, 64, "cm", "none"), (BF16, 64, "gap", "mean"), (F32, 40, "cm", "sum")])
+def test_linear_saved_elsewhere(dtype, d, layout, reduction, way):
+    x, w = _inputs(90, d, 400, dtype, 3, layout)
+    targets, (ids, te) = _targets(90, 400, 0.1, 5), _lists(90, 400, 6, seed=4)
+    x, w = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    up = torch.linspace(-1.0, 2.0, 90, device="cuda") if reduction == "none" else torch.tensor(0.7, device="cuda")
+    for run in (lambda: linear_cross_entropy(x, w, targets, reduction=reduction),
+                lambda: linear_distill_loss(x, w, ids, te, temperature=2.0, reduction=reduction)):
+        want = torch.autograd.grad(run(), (x, w), up)
+        got = torch.autograd.grad(_saved_elsewhere(run, way), (x, w), up)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("way", ["clone", "cpu"])
+def test_linear_both_directions_saved_elsewhere(way):
+    """A head whose gradients come with its loss: the first pass has them, the second one makes its own."""
+    x, w = _inputs(1024, 640, 33000, BF16, 3)
+    targets = _targets(1024, 33000, 0.1, 5)
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    run = lambda: linear_cross_entropy(x, w, targets)
+
+    def passes(loss):
+        return [torch.autograd.grad(loss, (x, w), retain_graph=keep) for keep in (True, False)]
+    for got, want in zip(passes(_saved_elsewhere(run, way)), passes(run())):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
