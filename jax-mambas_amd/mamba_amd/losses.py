@@ -89,10 +89,10 @@ def _row_stride(m):
     return m.stride(0) if m.shape[0] > 1 else m.shape[1]
 
 
-def _weight_rows(w):
-    """`w` with contiguous rows that do not overlap."""
-    v, f = w.shape
-    return w.contiguous() if f > 1 and w.stride(1) != 1 or v > 1 and w.stride(0) < f else w
+def _rows(m):
+    """`m` with contiguous rows that do not overlap."""
+    rows, cols = m.shape
+    return m.contiguous() if cols > 1 and m.stride(1) != 1 or rows > 1 and m.stride(0) < cols else m
 
 
 def _upstream(grad, reduction, rows):
@@ -158,7 +158,7 @@ class _LinearLoss(torch.autograd.Function):
             a.x = a.loss = a.mean = a.targets = a.ids = a.teacher = None
             # (Saved-tensor hooks may have put both elsewhere, and the weight's rows at another distance.)
             a.saved, a.saved_bytes = saved.data_ptr(), saved.numel()
-            w = _weight_rows(w)
+            w = _rows(w)
             a.weight, a.ldw = w.data_ptr(), _row_stride(w)
             if saved.numel() < lib.mss_linear_loss_saved_bytes(a):  # it was read in place, and cannot be here
                 w = w.clone(memory_format=torch.contiguous_format)
@@ -207,7 +207,7 @@ def _linear_loss(x, weight, weight_act, holder, targets, ids, teacher, ignore_in
         weight_act = weight.detach() if weight.dtype == x.dtype else weight.detach().to(x.dtype)
     else:
         weight_act = weight_act.detach()
-    weight_act = _weight_rows(_resolved(weight_act))
+    weight_act = _rows(_resolved(weight_act))
     conform = [None if v is None else _resolved(v).contiguous() for v in (targets, ids, teacher)]
     both = reduction != _lib.MSS_LOSS_NONE and torch.is_grad_enabled() and x.requires_grad and weight.requires_grad
     return _LinearLoss.apply(_resolved(x), weight, weight_act, *conform, ignore_index, temperature, reduction, teacher_tag,
@@ -237,7 +237,7 @@ class _Distill(torch.autograd.Function):
         rows, vocab = logits.shape
         a = _lib.DistillArgs(rows=rows, vocab=vocab, top=ids.shape[1], io_dtype=_io_tag(logits.dtype, "logits"),
                              teacher_dtype=teacher_tag, reduction=reduction, temperature=temperature,
-                             ld=logits.stride(0) if rows > 1 else vocab, logits=logits.data_ptr(), ids=ids.data_ptr(),
+                             ld=_row_stride(logits), logits=logits.data_ptr(), ids=ids.data_ptr(),
                              teacher=teacher.data_ptr())
         dev = logits.device
         with _guard(logits):
@@ -270,6 +270,10 @@ class _Distill(torch.autograd.Function):
                 d = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
             a = _lib.DistillArgs.from_buffer_copy(src)
             a.ids = a.teacher = a.loss = a.mean = None
+            # (Saved-tensor hooks may have put both elsewhere, and the rows at another distance.)
+            logits = _rows(logits)
+            a.logits, a.ld = logits.data_ptr(), _row_stride(logits)
+            a.saved, a.saved_bytes = saved.data_ptr(), saved.numel()
             a.grad, a.dlogits = grad.data_ptr(), d.data_ptr()
             _lib.check(getattr(lib, name)(a, _stream(logits)), name)
         return (d,) + (None,) * 6
@@ -290,9 +294,7 @@ def distill_loss(logits, ids, teacher, temperature=1.0, reduction="mean"):
     if rows == 0 or ids.shape[1] == 0:
         none = logits.new_zeros(rows, dtype=_F32) + 0.0 * logits[:0].sum().float()
         return none if reduction == _lib.MSS_LOSS_NONE else none.sum()
-    logits = _resolved(logits)
-    if vocab > 1 and logits.stride(1) != 1 or rows > 1 and logits.stride(0) < vocab:
-        logits = logits.contiguous()
+    logits = _rows(_resolved(logits))
     both = reduction != _lib.MSS_LOSS_NONE and torch.is_grad_enabled() and logits.requires_grad
     return _Distill.apply(logits, _resolved(ids).contiguous(), _resolved(teacher).detach().contiguous(), temperature,
                           reduction, tag, both)

@@ -338,6 +338,27 @@ def test_linear_backward_reads_what_the_hooks_return(calls, lib, dtype, d, layou
         assert a.weight == w2.data_ptr() and a.ldw == d
 
 
+@pytest.mark.parametrize("layout", ["clone", "off", "t"])
+@pytest.mark.parametrize("reduction,second", [("mean", False), ("none", False), ("sum", True)])
+def test_distill_backward_reads_what_the_hooks_return(calls, layout, reduction, second):
+    z, ids = torch.randn(20, 100, requires_grad=True), torch.zeros(20, 3, dtype=torch.int64)
+    hooks = _Hooks({"clone": torch.Tensor.clone, "off": _off_16, "t": lambda t: t.t().contiguous().t() if t.dim() == 2 else t.clone()}[layout])
+    with hooks:
+        loss = distill_loss(_off_16(z), ids, torch.zeros(20, 3), reduction=reduction)
+    up = torch.ones_like(loss)
+    torch.autograd.grad(loss, (z,), up, retain_graph=second)
+    if second:
+        torch.autograd.grad(loss, (z,), up)
+    (_, fwd), (name, a) = calls.seen[0], calls.seen[-1]
+    logits, saved = hooks.unpacked[-2:]
+    assert name == ("mss_distill_regrad" if reduction == "mean" else "mss_distill_bwd")
+    assert a.saved == saved.data_ptr() != fwd.saved and a.saved_bytes == saved.numel() and a.logits != fwd.logits
+    if layout == "t":
+        assert a.ld == 100
+    else:
+        assert a.logits == logits.data_ptr() and a.ld == logits.stride(0)
+
+
 # ------------------------------------------------------------------------------- the definitions
 def _wanted_targets(targets, vocab, ignore=-100):
     q = torch.zeros(targets.shape[0], vocab, dtype=torch.float64, device=targets.device)
@@ -1129,3 +1150,19 @@ def test_linear_both_directions_saved_elsewhere(way):
         return [torch.autograd.grad(loss, (x, w), retain_graph=keep) for keep in (True, False)]
     for got, want in zip(passes(_saved_elsewhere(run, way)), passes(run())):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("way", ["clone", "cpu", "checkpoint"])
+@pytest.mark.parametrize("dtype,reduction", [(BF16, "none"), (BF16, "mean"), (F32, "sum")])
+def test_distill_saved_elsewhere(dtype, reduction, way):
+    big = torch.randn(90, 405, device="cuda").to(dtype)
+    z = big[:, 2:402].detach().requires_grad_(True)  # rows off 16 bytes, with gaps
+    ids, te = _lists(90, 400, 6, seed=4)
+    up = torch.linspace(-1.0, 2.0, 90, device="cuda") if reduction == "none" else torch.tensor(0.7, device="cuda")
+    run = lambda: distill_loss(z, ids, te, temperature=2.0, reduction=reduction)
+
+    def passes(loss):
+        return [torch.autograd.grad(loss, (z,), up, retain_graph=keep)[0] for keep in ((True, False) if way != "checkpoint" else (False,))]
+    for got, want in zip(passes(_saved_elsewhere(run, way)), passes(run())):
+        assert torch.equal(got, want)
