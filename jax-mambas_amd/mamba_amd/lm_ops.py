@@ -164,17 +164,26 @@ class GradHolder:
     """Passes the tied output head's float32 gradient of the shared table to the embedding's
     backward, which adds its own part in place and hands the sum to autograd as the table's
     one gradient (instead of two dense gradients and an add). The head's backward runs first:
-    it belongs to the end of the forward. Losses that share the head add theirs."""
+    it belongs to the end of the forward. Losses that share the head add theirs. A gradient is of
+    one backward pass: what is left by a pass that did not come to the embedding (one that was
+    asked for other parameters' gradients) is not the next one's."""
 
     def __init__(self):
         self.grad = None
+        self._pass = -1  # the backward pass that put it, -1: outside of any
+
+    def _left(self, now):
+        return self._pass != now and self._pass != -1 and now != -1
 
     def put(self, g):
-        self.grad = g if self.grad is None else self.grad.add_(g)
+        now = torch._C._current_graph_task_id()
+        self.grad = g if self.grad is None or self._left(now) else self.grad.add_(g)
+        self._pass = now
 
     def take(self):
-        g, self.grad = self.grad, None
-        return g
+        left = self._left(torch._C._current_graph_task_id())
+        g, self.grad, self._pass = self.grad, None, -1
+        return None if left else g
 
 
 class _EmbedCM(torch.autograd.Function):

@@ -9,7 +9,8 @@ import pytest
 import torch
 import torch.nn.functional as F
 
-from mamba_amd.mamba1 import GraphedTrainStep, MambaLM
+from mamba_amd.lm_ops import GradHolder, cross_entropy
+from mamba_amd.mamba1 import GraphedTrainStep, MambaLM, _TiedHeadMM
 from mamba_amd.optim import AdamW
 from oracle import mamba1_torch as ref
 
@@ -46,6 +47,51 @@ def _oracle_distill(logits, ids, teacher, temperature):
         q = torch.softmax(teacher[r][at] / temperature, 0)
         total = total + temperature ** 2 * (q * (q.log() - log_p[r][ids[r][at]])).sum()
     return total / int(live.sum())
+
+
+class _Gather(torch.autograd.Function):
+    """The embedding of embed_cm, with its holder, on the CPU."""
+
+    @staticmethod
+    def forward(ctx, table, tokens, holder):
+        ctx.save_for_backward(tokens)
+        ctx.holder, ctx.shape = holder, table.shape
+        return table[tokens].t().contiguous()
+
+    @staticmethod
+    def backward(ctx, dh):
+        de = ctx.holder.take()
+        de = torch.zeros(ctx.shape) if de is None else de
+        return de.index_add_(0, ctx.saved_tensors[0], dh.t()), None, None
+
+
+def test_a_holder_s_gradient_is_of_one_pass():
+    """A pass for another parameter's gradient runs the heads and not the embedding: the next one starts anew. Whole numbers,
+    whose sums are exact."""
+    g = torch.Generator().manual_seed(1)
+    table = torch.randint(-4, 5, (11, 6), generator=g).float().requires_grad_(True)
+    middle = torch.randint(-2, 3, (6, 6), generator=g).float().requires_grad_(True)
+    tokens = torch.randint(0, 11, (9,), generator=g)
+    heads = [torch.randint(-2, 3, (9, 11), generator=g).float() for _ in range(2)]
+
+    def losses(held):
+        holder = GradHolder()
+        h = _Gather.apply(table, tokens, holder) if held else table[tokens].t()
+        x = middle @ h
+        return [((_TiedHeadMM.apply(x, table, table.detach(), holder) if held else x.t() @ table.t()) * w).sum() for w in heads]
+
+    leaves = (table, middle)
+    soft, hard = losses(False)
+    want = {"both": torch.autograd.grad(soft + hard, leaves, retain_graph=True),
+            "soft": torch.autograd.grad(soft, leaves, retain_graph=True), "hard": torch.autograd.grad(hard, leaves)}
+    soft, hard = losses(True)
+    loss = {"both": soft + hard, "soft": soft, "hard": hard}
+    for name in ("both", "soft", "hard", "both"):
+        for other in ("soft", "both"):  # what these leave in the holder is nobody's
+            (got,) = torch.autograd.grad(loss[other], (middle,), retain_graph=True)
+            assert torch.equal(got, want[other][1])
+        for got, exact in zip(torch.autograd.grad(loss[name], leaves, retain_graph=True), want[name]):
+            assert torch.equal(got, exact), name
 
 
 @pytest.mark.gpu
@@ -141,3 +187,27 @@ def test_training_steps_graph_matches_eager():
     print("  eager", eager, "graph", graph, flush=True)
     for a, b in zip(eager[2:], graph):
         assert abs(a - b) <= 2e-3 * abs(a), (a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["loss", "pair", "logits"])
+def test_gradients_after_a_pass_for_one_parameter(which):
+    """Another parameter's gradient alone, then all of them: as without the first pass, to the bit."""
+    tokens, targets, ids, teacher = (t.cuda() for t in _batch())
+    grads = []
+    for first in (False, True):
+        m = _model()
+        if which == "loss":
+            loss = m.loss(tokens, targets)
+        elif which == "pair":
+            loss = sum(m.distill_loss(tokens, ids, teacher, temperature=2.0, targets=targets))
+        else:
+            loss = cross_entropy(m(tokens), targets.reshape(-1).clamp_min(0))
+        if first:
+            name, some = next((k, v) for k, v in m.named_parameters() if "blocks.1" in k)
+            (alone,) = torch.autograd.grad(loss, (some,), retain_graph=True)
+        loss.backward()
+        grads.append({k: v.grad for k, v in m.named_parameters()})
+    assert torch.equal(alone, grads[1][name])
+    for k in grads[0]:
+        assert torch.equal(grads[0][k], grads[1][k]), k
