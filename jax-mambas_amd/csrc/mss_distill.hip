@@ -314,9 +314,9 @@ __global__ __launch_bounds__(kWaves < 4 ? 256 : 64 * kWaves) void distill_kernel
           s *= fast_exp2((m - mx) * p.r.c);
           m = mx;
         }
-        if (m == -INFINITY) return;
+        const float from = m == -INFINITY ? 0.f : m;  // (then there are words of no weight, and NaNs, which count)
 #pragma unroll
-        for (int e = 0; e < V::kN; ++e) s += fast_exp2((v[e] - m) * p.r.c);
+        for (int e = 0; e < V::kN; ++e) s += fast_exp2((v[e] - from) * p.r.c);
       });
     }
     const float mine = m;

@@ -962,6 +962,37 @@ def test_distill_edges_of_the_types(dtype):
     assert bool(g[2].isnan().all()) and bool(g[3].isnan().all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("v", [3000, 70001, 131072])
+@pytest.mark.parametrize("reduction", ["none", "sum"])
+def test_distill_a_nan_anywhere_makes_its_row_nan(dtype, v, reduction):
+    """Also where what a lane has read before it is words of no weight, and where it reads nothing else."""
+    inf = float("inf")
+    g = torch.Generator(device="cuda").manual_seed(v)
+    z = torch.randn(9, v, generator=g, device="cuda").to(dtype)
+    z[0, :16] = float("nan")         # a whole vector, the first of its lane
+    z[1, :16], z[1, 3] = -inf, float("nan")
+    z[2], z[2, 5], z[2, 100] = -inf, 1.0, float("nan")
+    z[3] = float("nan")
+    z[4], z[4, v - 1] = -inf, float("nan")
+    z[5, v - 1] = float("nan")
+    z[6, :2000] = -inf               # and none in these
+    z[7] = -inf
+    z[7, 5] = 2.0
+    z.requires_grad_(True)
+    ids = torch.full((9, 1), 5, device="cuda")
+    z.data[6, 5] = 1.0
+    loss = distill_loss(z, ids, torch.zeros(9, 1, device="cuda"), reduction="none")
+    bad = torch.tensor([True] * 6 + [False] * 3, device="cuda")
+    assert torch.equal(loss.isnan(), bad) and bool(loss[6:].isfinite().all()) and float(loss[7].detach()) == 0.0
+    if reduction == "sum":
+        loss = distill_loss(z, ids, torch.zeros(9, 1, device="cuda"), reduction="sum")
+        assert bool(loss.isnan())
+    (d,) = torch.autograd.grad(loss, (z,), torch.ones_like(loss))
+    assert torch.equal(d.isnan().all(1), bad) and torch.equal(d.isnan().any(1), bad)
+
+
 # ------------------------------------------------------------------------------- both
 @pytest.mark.gpu
 def test_gradients_against_differences():
