@@ -1275,7 +1275,10 @@ __global__ __launch_bounds__(1024) void ll_scale_kernel(LinLossParams p, float2*
     __shared__ uint32_t s[16];
     uint32_t m = 0;
 #pragma unroll 4
-    for (int t = threadIdx.x; t < p.tokens; t += 1024) m = max(m, finite_bits(p.grad[t] * p.temperature));
+    for (int t = threadIdx.x; t < p.tokens; t += 1024) {
+      const uint32_t up = finite_bits(p.grad[t] * p.temperature);
+      m = p.stat[t].y == 0.f ? m : max(m, up);  // (whatever comes to a row that does not count)
+    }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), off)));
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;

@@ -819,6 +819,27 @@ def test_float32_of_any_size(x_exp, w_exp, g_exp, reduction):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("held", [1e30, 3e38, float("inf"), float("nan")])
+def test_upstream_gradients_of_rows_that_do_not_count(dtype, held):
+    """They reach nothing: the gradients are those of upstream zeros there, to the bit."""
+    x, w = _inputs(70, 72, 300, dtype, 3)
+    targets, (ids, te) = _targets(70, 300, 0.3, 5), _lists(70, 300, 6, seed=4, empty=0.3)
+    z = torch.randn(70, 300, device="cuda").to(dtype).requires_grad_(True)
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    empty = ~((ids >= 0) & (te != -torch.inf)).any(1)
+    for run, leaves, off in ((lambda: linear_cross_entropy(x, w, targets, reduction="none"), (x, w), targets == -100),
+                             (lambda: linear_distill_loss(x, w, ids, te, temperature=2.0, reduction="none"), (x, w), empty),
+                             (lambda: distill_loss(z, ids, te, temperature=2.0, reduction="none"), (z,), empty)):
+        assert bool(off.any()) and not bool(off.all())
+        up = torch.linspace(-1.0, 2.0, 70, device="cuda")
+        want = torch.autograd.grad(run(), leaves, up.masked_fill(off, 0.0))
+        got = torch.autograd.grad(run(), leaves, up.masked_fill(off, held))
+        assert all(bool(a.isfinite().all()) and torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
 def test_linear_weight_copies_and_holder():
     """A float32 master with and without its bfloat16 copy; the gradient through a holder; one gradient only."""
     t, d, v = 100, 64, 300
