@@ -81,6 +81,13 @@ def _guard(t):
     return _HERE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
+def _require_one_gpu(*tensors):
+    _require_gpu(*tensors)
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) > 1:
+        raise ValueError(f"the operands lie on several devices: {', '.join(sorted(map(str, devices)))}")
+
+
 def _bytes(n, device):
     return torch.empty(n, dtype=torch.uint8, device=device)
 
@@ -198,7 +205,7 @@ def _linear_loss(x, weight, weight_act, holder, targets, ids, teacher, ignore_in
         raise ValueError("weight_act must be the weight in x's type")
     if holder is not None and weight.dtype != _F32:
         raise ValueError("a holder takes a float32 weight's gradient")
-    _require_gpu(x, weight, weight_act, targets, ids, teacher)
+    _require_one_gpu(x, weight, weight_act, targets, ids, teacher)
     if t == 0 or (ids is not None and ids.shape[1] == 0):
         # No row counts: zeros that depend on the operands.
         none = x.new_zeros(t, dtype=_F32) + 0.0 * (x[:0].sum() + weight[:0].sum()).float()
@@ -290,7 +297,7 @@ def distill_loss(logits, ids, teacher, temperature=1.0, reduction="mean"):
     if rows > _MAX_ROWS:
         raise ValueError(f"logits have at most {_MAX_ROWS} rows, got {rows}")
     tag = _check_lists(ids, teacher, rows, temperature)
-    _require_gpu(logits, ids, teacher)
+    _require_one_gpu(logits, ids, teacher)
     if rows == 0 or ids.shape[1] == 0:
         none = logits.new_zeros(rows, dtype=_F32) + 0.0 * logits[:0].sum().float()
         return none if reduction == _lib.MSS_LOSS_NONE else none.sum()

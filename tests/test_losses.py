@@ -359,6 +359,19 @@ def test_distill_backward_reads_what_the_hooks_return(calls, layout, reduction, 
         assert a.logits == logits.data_ptr() and a.ld == logits.stride(0)
 
 
+def test_operands_on_several_devices_are_refused(calls):
+    x, w, tg = torch.randn(8, 5), torch.randn(11, 8), torch.zeros(5, dtype=torch.int64)
+    ids, te, z = torch.zeros(5, 3, dtype=torch.int64), torch.randn(5, 3), torch.randn(5, 11)
+    for f, operands in ((linear_cross_entropy, (x, w, tg)), (linear_distill_loss, (x, w, ids, te)), (distill_loss, (z, ids, te))):
+        f(*operands)
+        for i in range(len(operands)):
+            with pytest.raises(ValueError, match="devices"):
+                f(*(t.to("meta") if j == i else t for j, t in enumerate(operands)))
+    with pytest.raises(ValueError, match="devices"):
+        linear_cross_entropy(x, w, tg, weight_act=w.to("meta"))
+    assert len(calls.seen) == 3
+
+
 # ------------------------------------------------------------------------------- the definitions
 def _wanted_targets(targets, vocab, ignore=-100):
     q = torch.zeros(targets.shape[0], vocab, dtype=torch.float64, device=targets.device)
