@@ -722,7 +722,8 @@ int mss_sample(const mss_sample_args* args, void* stream);
  * MSS_LOSS_MEAN (over the rows that count; 0 without any). loss: [rows], always written; mean: the
  * reduced loss (one value, unless MSS_LOSS_NONE).
  * saved: what the backward calls read of a forward one, mss_*_saved_bytes bytes, 256-byte aligned.
- * ids, teacher, targets and all outputs are contiguous; outputs overlap no input. top is 1 to
+ * ids, teacher, targets and all outputs are contiguous, every address a multiple of its type's size (and mss_linear_loss's
+ * ldw at most 2^24, its other strides 2^40); outputs overlap no input. top is 1 to
  * MSS_LOSS_MAX_TOP, rows * top at most 2^27.
  *
  * mss_linear_loss: logits = x^T W^T for x (features, tokens) with element strides stride_f, stride_t (not

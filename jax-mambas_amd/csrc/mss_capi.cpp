@@ -1628,6 +1628,7 @@ bool outputs_meet(const Span* out, int no, const Span* in, int ni) {
 }
 
 bool aligned256(const void* p) { return reinterpret_cast<uintptr_t>(p) % 256 == 0; }
+bool aligned_to(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }  // (NULL too)
 
 int loss_type_bytes(int dtype) { return dtype == MSS_BF16 ? 2 : 4; }
 
@@ -1733,6 +1734,11 @@ int linear_loss_sizes(const mss_linear_loss_args* a, int which, mss::LinLossPara
   return MSS_OK;
 }
 
+bool grads_aligned(const mss_linear_loss_args* a, bool reads_grad) {
+  return aligned_to(a->dx, loss_type_bytes(a->io_dtype)) && aligned_to(a->dweight, loss_type_bytes(a->dw_dtype)) &&
+         (!reads_grad || aligned_to(a->grad, 4));
+}
+
 // which: 0 the forward, 1 the backward call, 2 both at once.
 int linear_loss_params(const mss_linear_loss_args* a, int which, mss::LinLossParams* p, mss::LinLossPlan* plan) {
   size_t saved, sizes[3];
@@ -1742,8 +1748,13 @@ int linear_loss_params(const mss_linear_loss_args* a, int which, mss::LinLossPar
   if (which == 2 && sizes[2] == 0) return MSS_ERR_UNSUPPORTED;
   const int e = loss_type_bytes(a->io_dtype);
   if (!a->weight || !a->saved || (fwd && a->reduction != MSS_LOSS_NONE && !a->mean)) return MSS_ERR_INVALID_ARGUMENT;
-  if (reinterpret_cast<uintptr_t>(a->x) % e != 0 || reinterpret_cast<uintptr_t>(a->weight) % e != 0)
-    return MSS_ERR_INVALID_ARGUMENT;
+  if (fwd) {
+    if (!aligned_to(a->x, e) || !aligned_to(a->loss, 4) || (a->reduction != MSS_LOSS_NONE && !aligned_to(a->mean, 4)))
+      return MSS_ERR_INVALID_ARGUMENT;
+    if (a->top > 0 ? !aligned_to(a->ids, 8) || !aligned_to(a->teacher, loss_type_bytes(a->teacher_dtype)) : !aligned_to(a->targets, 8))
+      return MSS_ERR_INVALID_ARGUMENT;
+  }
+  if (!aligned_to(a->weight, e) || (bwd && !grads_aligned(a, !fwd))) return MSS_ERR_INVALID_ARGUMENT;
   const size_t ws = sizes[which];
   if (!aligned256(a->saved) || a->saved_bytes < saved || !a->workspace || !aligned256(a->workspace) || a->workspace_bytes < ws)
     return MSS_ERR_WORKSPACE;
@@ -1836,6 +1847,7 @@ int mss_linear_loss_rescale(const mss_linear_loss_args* a, void* stream) {
   if (s != MSS_OK) return s;
   if (ws[2] == 0) return MSS_ERR_UNSUPPORTED;
   if (!a->dx || !a->dweight || !a->grad || (a->dw_dtype != MSS_F32 && a->dw_dtype != MSS_BF16)) return MSS_ERR_INVALID_ARGUMENT;
+  if (!grads_aligned(a, true)) return MSS_ERR_INVALID_ARGUMENT;
   const Span in = {a->grad, 4};
   const Span out[] = {{a->dx, static_cast<long long>(a->features) * a->tokens * 2},
                       {a->dweight, static_cast<long long>(a->vocab) * a->features * loss_type_bytes(a->dw_dtype)}};
@@ -1876,12 +1888,14 @@ int run_distill(const mss_distill_args* a, int what, void* stream) {
   const bool fwd = what & mss::kDsFwd, bwd = what & mss::kDsBwd;
   const int e = loss_type_bytes(a->io_dtype);
   if (!a->logits || !a->saved || (fwd && a->reduction != MSS_LOSS_NONE && !a->mean)) return MSS_ERR_INVALID_ARGUMENT;
-  if (reinterpret_cast<uintptr_t>(a->logits) % e != 0 || reinterpret_cast<uintptr_t>(a->dlogits) % e != 0)
-    return MSS_ERR_INVALID_ARGUMENT;
+  if (!aligned_to(a->logits, e) || !aligned_to(a->dlogits, e)) return MSS_ERR_INVALID_ARGUMENT;
   if (fwd && (!a->ids || !a->teacher || !a->loss)) return MSS_ERR_INVALID_ARGUMENT;
+  if (fwd && (!aligned_to(a->ids, 8) || !aligned_to(a->teacher, loss_type_bytes(a->teacher_dtype)) || !aligned_to(a->loss, 4) ||
+              (a->reduction != MSS_LOSS_NONE && !aligned_to(a->mean, 4))))
+    return MSS_ERR_INVALID_ARGUMENT;
   if (bwd && !a->dlogits) return MSS_ERR_INVALID_ARGUMENT;
   const bool reads_grad = bwd && !fwd;
-  if (reads_grad && !a->grad) return MSS_ERR_INVALID_ARGUMENT;
+  if (reads_grad && (!a->grad || !aligned_to(a->grad, 4))) return MSS_ERR_INVALID_ARGUMENT;
   if (((fwd && bwd) || (what & mss::kDsAgain)) && a->reduction == MSS_LOSS_NONE) return MSS_ERR_INVALID_ARGUMENT;
   if (!aligned256(a->saved) || a->saved_bytes < saved) return MSS_ERR_WORKSPACE;
   const long long n = static_cast<long long>(a->rows) * a->top;

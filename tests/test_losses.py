@@ -212,6 +212,31 @@ def test_distill_backward_validation(lib, kw):
     assert lib.mss_distill_bwd(a, None) == lib.mss_distill_regrad(a, None) == 1
 
 
+def test_addresses_off_their_type_are_refused(lib):
+    """Each address, in the calls that take it."""
+    big = {**BIG, "saved_bytes": 1 << 40}
+    lists, tgts = dict(big, top=5), dict(big)
+
+    def refused(call, base, kw):
+        return call(_lib.LinearLossArgs(**{**base, **kw}) if base is not DISTILL else _lib.DistillArgs(**{**base, **kw}), None) == 1
+    for call in (lib.mss_linear_loss_fwd, lib.mss_linear_loss_fwd_grad):
+        for kw in (dict(x=P + 1), dict(weight=2 * P + 1), dict(loss=6 * P + 2), dict(mean=7 * P + 1), dict(targets=3 * P + 4)):
+            assert refused(call, tgts, kw), kw
+        for kw in (dict(ids=4 * P + 4), dict(teacher=5 * P + 2), dict(teacher=5 * P + 1, teacher_dtype=1)):
+            assert refused(call, lists, kw), kw
+    for call in (lib.mss_linear_loss_bwd, lib.mss_linear_loss_fwd_grad, lib.mss_linear_loss_rescale):
+        for kw in (dict(dx=11 * P + 1), dict(dweight=12 * P + 1), dict(dweight=12 * P + 2, dw_dtype=0)):
+            assert refused(call, tgts, kw), kw
+    for call in (lib.mss_linear_loss_bwd, lib.mss_linear_loss_rescale):
+        assert refused(call, tgts, dict(grad=10 * P + 2))
+    for call in (lib.mss_distill_fwd, lib.mss_distill_fwd_grad):
+        for kw in (dict(ids=2 * P + 4), dict(teacher=3 * P + 2), dict(loss=4 * P + 1), dict(mean=5 * P + 2), dict(logits=P + 1)):
+            assert refused(call, DISTILL, kw), kw
+    for call in (lib.mss_distill_bwd, lib.mss_distill_regrad):
+        for kw in (dict(grad=7 * P + 2), dict(dlogits=8 * P + 1)):
+            assert refused(call, DISTILL, kw), kw
+
+
 def test_struct_layouts_match_the_header(tmp_path):
     import ctypes
     import subprocess
