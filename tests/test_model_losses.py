@@ -211,3 +211,29 @@ def test_gradients_after_a_pass_for_one_parameter(which):
     assert torch.equal(alone, grads[1][name])
     for k in grads[0]:
         assert torch.equal(grads[0][k], grads[1][k]), k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("way", ["cpu", "checkpoint"])
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+def test_model_losses_with_what_they_save_elsewhere(way, act):
+    """Offloaded, or made again by a checkpoint: the gradients of a plain pass, to the bit."""
+    from torch.utils.checkpoint import checkpoint
+    tokens, targets, ids, teacher = (t.cuda() for t in _batch())
+    adt = torch.float32 if act == "f32" else torch.bfloat16
+    grads = []
+    for elsewhere in (False, True):
+        m = _model()
+        run = lambda: 0.7 * sum(m.distill_loss(tokens, ids, teacher, temperature=2.0, targets=targets, act_dtype=adt))
+        if not elsewhere:
+            loss = run()
+        elif way == "checkpoint":
+            loss = checkpoint(run, use_reentrant=False)
+        else:
+            with torch.autograd.graph.save_on_cpu():
+                loss = run()
+        loss.backward()
+        grads.append((loss.detach(), {k: v.grad for k, v in m.named_parameters()}))
+    assert torch.equal(grads[0][0], grads[1][0])
+    for k in grads[0][1]:
+        assert torch.equal(grads[0][1][k], grads[1][1][k]), k
