@@ -12,10 +12,12 @@
 // All products run on the matrix cores with float32 sums. bf16 operands are taken as they are
 // (v_mfma_f32_32x32x16_bf16); g is rounded to bf16 once, as its factors x and w are. A float32 matrix is taken to
 // a power of two's multiple whose largest element lies below 2^15, and split into two planes of half precision: the
-// rounding to 11 bits, and that of what it leaves times 2^11. Together they hold 24 bits of what is at least 2^-28
-// of the largest, and 2^-51 of the largest below. A product is the sum of three products of planes
-// (v_mfma_f32_32x32x16_f16), the two with a lower plane first: what is dropped is 2^-24 of each term. Three times
-// the work of a bf16 product, at 16 times the rate of the float32 matrix instructions.
+// rounding to 11 bits, and that of what it leaves times 2^11. Together they hold an element to 2^-23 of itself down to
+// 2^-27 of the largest, and to 2^-50 of the largest below. A product is the sum of three products of planes
+// (v_mfma_f32_32x32x16_f16), the two with a lower plane first: what is dropped, the lower ones' own, is at most 2^-22
+// of a term, 2^-24.6 in the mean square. g, taken times 2^15, is held to 2^-23 of itself down to 2^-28, and to 2^-51
+// below (2^-27 and 2^-50 of the largest upstream gradient where each row has its own). Three times the work of a bf16 product, at 16
+// times the rate of the float32 matrix instructions.
 //
 // 32x32x16 operand layout (lane l, its 8 bf16): A[i][k] at l = i + 32 (k / 8), element k % 8;
 // B[k][j] at l = j + 32 (k / 8), element k % 8; D[i][j] at l = j + 32 ((i / 4) % 2),
@@ -1175,7 +1177,8 @@ __global__ __launch_bounds__(kFinishTokens * kFinishSlices) void ll_finish_kerne
 // For a block of tokens and the whole vocabulary at a time, kModeExp leaves the words' s - ref in 16 bits, with ref a
 // logit of the token's own list, and the sums S of 2^(s - ref); then g = 2^(s - ref) / S - q, rounded to bf16, takes
 // their place: the logits are formed once, not twice. The 16 bits hold s to half of 2^-9, so that g is off by 2^-10.5
-// of itself before it is rounded (by 2^-8 at most); a bf16 2^(s - ref), the division left to x's rows and dx's
+// of itself before it is rounded (by 2^-8 at most), and zero where s - ref is below -48, a probability below 2^-38 (S
+// being more than 2^-10); a bf16 2^(s - ref), the division left to x's rows and dx's
 // columns, would need no conversion, but cost dw another whole rounding. It fails where S passes 2^79, a token whose
 // words lie that far below its largest logit: such a row is noted in `bad`, and the kernels of the two apart,
 // launched behind, make the block's losses and g anew; else they return at once.
@@ -1294,7 +1297,7 @@ __global__ __launch_bounds__(1024) void ll_scale_kernel(LinLossParams p, float2*
 }
 
 // g at the wanted words of the piece that begins at word v0. In bf16 from their own logits, since their probabilities
-// are rounded there. The planes of a float32 one hold it to 24 bits: it is the product's own then, whose exponential is
+// are rounded there. The planes of a float32 one hold it to 2^-23: it is the product's own then, whose exponential is
 // part of the row's sum, so that what they are both off by cancels where the probability is nearly 1.
 template <bool kF32>
 __global__ __launch_bounds__(256) void ll_wanted_kernel(LinLossParams p, const float2* scale, int v0, int words) {

@@ -39,8 +39,8 @@ int loss_list_blocks(int rows);
 int loss_target_blocks(int tokens);
 hipError_t launch_loss_rows(const LossRows& r, hipStream_t stream);
 
-// A matrix of bf16 in one plane, or of float32 as the sum of three (each the rounding of what the
-// ones before leave).
+// A matrix of bf16 in one plane, or of float32, a power of two's multiple of it, in two of half precision: the
+// rounding to 11 bits, and that of what it leaves times 2^11.
 struct LossMatrix {
   const bf16_t* base;
   long long ld, plane;  // elements from one row, one plane to the next
@@ -93,7 +93,7 @@ struct LinLossParams {
 
 // What the call needs besides its operands; sizes depend on nothing but the arguments.
 struct LinLossPlan {
-  int shape, shape_x, shape_w;  // of the tiles: 0 small, 1 large, 2 thin
+  int shape, shape_x, shape_w;  // of the tiles: 0 small, 1 large, 2 thin, and of the logits' 3: of 192 tokens
   int parts, piece;
   long long ldg, ldx, partial;
   int both, block, parts_both;  // both directions at once: whether, tokens of a block
@@ -114,7 +114,6 @@ struct DistillParams {
   long long ld;
   float* loss;      // [rows]
   float2* stat;     // [rows]: largest logit, log2 of the sum of 2^((logit - largest) c)
-  float* picked;    // [rows][top]
   float* mean;      // the reduced loss
   float* by;        // 1 / (rows that count), for a mean
   const float* grad;  // [1], or [rows] without a reduction

@@ -24,11 +24,22 @@ outside the vocabulary, or a teacher's logit that is NaN or inf, makes its row's
 
 ``reduction``: "mean" over the rows that count (0 if none does), "sum", or "none" for (rows,)
 losses. The loss is float32. Differentiable, once, in x, weight and logits; gradients have their input's
-type. Products are summed in float32. For a bfloat16 x the logits' gradient is rounded to bfloat16 once, as
-the operands are (of a large head whose two gradients come with its loss, from probabilities held to less than
-2^-10 of themselves), and a float32 weight is read in a bfloat16 copy: ``weight_act``, where the caller
-keeps one, else a cast; float32 operands keep float32 precision throughout. ``holder``
-(``lm_ops.GradHolder``) takes the weight's float32 gradient instead of autograd. There is no CPU path.
+type. ``holder`` (``lm_ops.GradHolder``) takes the weight's float32 gradient instead of autograd. There is no
+CPU path. A loss from logits keeps them, and a reduced one their gradient beside them, until its backward pass.
+
+What is held in how many bits, of a head's losses (sums are float32):
+
+* a bfloat16 x: the logits' gradient is rounded to bfloat16 once, as the operands are. A float32 weight is
+  read in a bfloat16 copy: ``weight_act``, where the caller keeps one, else a cast.
+* The same, a reduced loss, x and weight both requiring gradients, from 512 tokens, 640 features, 1024 words and
+  2^25 logits on: the gradients come with the loss, from logits held in 16 bits, that is probabilities to
+  less than 2^-10 of themselves, and zeros for those below 2^-38; an upstream gradient that is not a power
+  of two rounds them a second time. A second backward pass, ``"none"``, one gradient alone and smaller heads
+  form the logits again and have neither.
+* a float32 x: an element of x and weight counts to 2^-23 of itself down to 2^-27 of its matrix's largest, and
+  to 2^-50 of that below; their products to 2^-22; the logits' gradient to 2^-23 of itself down to 2^-28 and
+  to 2^-51 below, with ``"none"`` down to 2^-27 and to 2^-50 of the largest upstream gradient of the rows that
+  count. (Float32 operations keep what is smaller still to 2^-24 of itself.)
 """
 from __future__ import annotations
 
