@@ -178,7 +178,8 @@ class _LinearLoss(torch.autograd.Function):
             a.saved, a.saved_bytes = saved.data_ptr(), saved.numel()
             w = _rows(w)
             a.weight, a.ldw = w.data_ptr(), _row_stride(w)
-            if saved.numel() < lib.mss_linear_loss_saved_bytes(a):  # it was read in place, and cannot be here
+            if (a.weight, a.ldw) != (src.weight, src.ldw) and saved.numel() < lib.mss_linear_loss_saved_bytes(a):
+                # (It was read in place, and cannot be here.)
                 w = w.clone(memory_format=torch.contiguous_format)
                 a.weight, a.ldw = w.data_ptr(), _row_stride(w)
             a.dw_dtype = _io_tag(ctx.dw_dtype, "weight")
