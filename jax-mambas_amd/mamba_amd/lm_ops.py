@@ -160,30 +160,57 @@ def cross_entropy(logits, targets):
     return _CrossEntropy.apply(logits, targets)
 
 
+class _HeldGrad:
+    """What the heads of one backward pass have put."""
+
+    def __init__(self, number, head, grad):
+        self.number, self.heads, self.grad, self.over = number, {head}, grad, False
+
+    def end(self):
+        self.over = True
+
+
 class GradHolder:
     """Passes the tied output head's float32 gradient of the shared table to the embedding's
     backward, which adds its own part in place and hands the sum to autograd as the table's
     one gradient (instead of two dense gradients and an add). The head's backward runs first:
-    it belongs to the end of the forward. Losses that share the head add theirs. A gradient is of
-    one backward pass: what is left by a pass that did not come to the embedding (one that was
-    asked for other parameters' gradients) is not the next one's."""
+    it belongs to the end of the forward. Losses that share the head add theirs.
+
+    A gradient is of one backward pass, with the passes within it (of checkpoints with re-entry
+    around the heads, or around the gather; not of one around each): what was left by one that did
+    not come to the embedding, since it was asked for other parameters' gradients, is dropped.
+    Passes are numbered as they begin, so one that has ended and has a lower number is an
+    earlier one, and one with a higher number lies within the one at hand. `head`: whatever tells
+    one head from the others; what it left in an earlier pass makes room for what it puts."""
 
     def __init__(self):
-        self.grad = None
-        self._pass = -1  # the backward pass that put it, -1: outside of any
+        self._parts = []
 
-    def _left(self, now):
-        return self._pass != now and self._pass != -1 and now != -1
+    @property
+    def grad(self):
+        return self._parts[-1].grad if self._parts else None
 
-    def put(self, g):
-        now = torch._C._current_graph_task_id()
-        self.grad = g if self.grad is None or self._left(now) else self.grad.add_(g)
-        self._pass = now
+    def put(self, g, head=None):
+        now = torch._C._current_graph_task_id()  # (-1: outside of any pass)
+        if head is not None:
+            self._parts = [p for p in self._parts if head not in p.heads]
+        for p in self._parts:
+            if p.number == now:
+                p.grad.add_(g)
+                p.heads.add(head)
+                return
+        self._parts.append(_HeldGrad(now, head, g))
+        if now != -1:
+            torch.autograd.Variable._execution_engine.queue_callback(self._parts[-1].end)
 
     def take(self):
-        left = self._left(torch._C._current_graph_task_id())
-        g, self.grad, self._pass = self.grad, None, -1
-        return None if left else g
+        now = torch._C._current_graph_task_id()
+        parts, self._parts = self._parts, []
+        total = None
+        for p in parts:
+            if not (p.over and p.number < now):
+                total = p.grad if total is None else total.add_(p.grad)
+        return total
 
 
 class _EmbedCM(torch.autograd.Function):

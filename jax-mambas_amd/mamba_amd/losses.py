@@ -155,7 +155,7 @@ class _LinearLoss(torch.autograd.Function):
         ctx.save_for_backward(w, saved)
         ctx.args = a
         ctx.x_like = (x.dtype, (f, t))
-        ctx.dw_dtype, ctx.holder = weight.dtype, holder
+        ctx.dw_dtype, ctx.holder, ctx.head = weight.dtype, holder, object()
         ctx.set_materialize_grads(False)
         return loss if reduction == _lib.MSS_LOSS_NONE else mean
 
@@ -197,7 +197,7 @@ class _LinearLoss(torch.autograd.Function):
             _lib.check(getattr(lib, name)(a, _stream(w)), name)
             dx, dw = dx if need_x else None, dw if need_w else None
         if dw is not None and ctx.holder is not None:
-            ctx.holder.put(dw)
+            ctx.holder.put(dw, ctx.head)
             dw = None
         return (dx, dw) + (None,) * 10
 

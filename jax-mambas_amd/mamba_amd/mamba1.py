@@ -105,7 +105,7 @@ class _TiedHeadMM(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, e, e_act, holder=None):
         ctx.save_for_backward(x, e_act)
-        ctx.holder = holder
+        ctx.holder, ctx.head = holder, object()
         # From a token-major copy of x: hipBLASLt's product with both operands K-contiguous
         # took 1.128 ms against 1.420 from the features-major view at the 130M shape (16384
         # tokens, 768 features, 50280 words; MI355X), and the copy 0.054 ms.
@@ -117,7 +117,7 @@ class _TiedHeadMM(torch.autograd.Function):
         dx = e_act.t() @ dy.t() if ctx.needs_input_grad[0] else None
         de = _mm_fp32(dy.t(), x.t()) if ctx.needs_input_grad[1] else None
         if de is not None and ctx.holder is not None:
-            ctx.holder.put(de)  # the embedding's backward adds its part and returns the sum
+            ctx.holder.put(de, ctx.head)  # the embedding's backward adds its part and returns the sum
             de = None
         return dx, de, None, None
 

@@ -94,6 +94,56 @@ def test_a_holder_s_gradient_is_of_one_pass():
             assert torch.equal(got, exact), name
 
 
+def test_a_holder_keeps_one_gradient_of_passes_that_leave_it():
+    """Passes for another parameter's gradient, over and over: what they leave does not pile up."""
+    g = torch.Generator().manual_seed(5)
+    table, middle = torch.randn(11, 6, generator=g).requires_grad_(True), torch.randn(6, 6, generator=g).requires_grad_(True)
+    holder = GradHolder()
+    x = middle @ _Gather.apply(table, torch.arange(9), holder)
+    loss = sum(_TiedHeadMM.apply(x, table, table.detach(), holder).square().sum() for _ in range(2))
+    for _ in range(5):
+        torch.autograd.grad(loss, (middle,), retain_graph=True)
+        assert len(holder._parts) == 1
+    torch.autograd.grad(loss, (table, middle), retain_graph=True)
+    assert holder.grad is None
+
+
+@pytest.mark.parametrize("inside", ["heads", "one head", "gather", "both"])
+def test_a_holder_across_the_passes_of_checkpoints(inside):
+    """A checkpoint with re-entry runs a pass of its own within the backward pass."""
+    from torch.utils.checkpoint import checkpoint
+    g = torch.Generator().manual_seed(2)
+    table = torch.randint(-4, 5, (11, 6), generator=g).float().requires_grad_(True)
+    middle = torch.randint(-2, 3, (6, 6), generator=g).float().requires_grad_(True)
+    tokens = torch.randint(0, 11, (9,), generator=g)
+    weights = [torch.randint(-2, 3, (9, 11), generator=g).float() for _ in range(2)]
+    again = lambda f, *a: checkpoint(f, *a, use_reentrant=True)
+
+    def loss(held):
+        holder = GradHolder()
+        gather = lambda t: _Gather.apply(t, tokens, holder)
+        heads = [lambda x, w=w: (_TiedHeadMM.apply(x, table, table.detach(), holder) * w).sum() for w in weights]
+        if not held:
+            x = middle @ table[tokens].t()
+            return sum(((x.t() @ table.t()) * w).sum() for w in weights)
+        if inside == "both":
+            return again(lambda m: sum(f(m @ gather(table)) for f in heads), middle)
+        x = middle @ (again(gather, table) if inside == "gather" else gather(table))
+        if inside == "heads":
+            return sum(again(f, x) for f in heads)
+        return (again(heads[0], x) if inside == "one head" else heads[0](x)) + heads[1](x)
+
+    def grads(held):
+        table.grad = middle.grad = None
+        loss(held).backward()
+        return table.grad, middle.grad
+
+    want = grads(False)
+    for _ in range(2):
+        for a, b in zip(grads(True), want):
+            assert torch.equal(a, b)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("act", ["f32", "bf16"])
 def test_model_losses_match_the_oracle(act):
