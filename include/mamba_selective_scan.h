@@ -722,22 +722,24 @@ int mss_sample(const mss_sample_args* args, void* stream);
  * MSS_LOSS_MEAN (over the rows that count; 0 without any). loss: [rows], always written; mean: the
  * reduced loss (one value, unless MSS_LOSS_NONE).
  * saved: what the backward calls read of a forward one, mss_*_saved_bytes bytes, 256-byte aligned.
- * ids, teacher, targets and all outputs are contiguous, every address a multiple of its type's size (and mss_linear_loss's
- * ldw at most 2^24, its other strides 2^40); outputs overlap no input. top is 1 to
+ * ids, teacher, targets and all outputs are contiguous, every address is a multiple of its type's size;
+ * outputs overlap no input. top is 1 to
  * MSS_LOSS_MAX_TOP, rows * top at most 2^27.
  *
  * mss_linear_loss: logits = x^T W^T for x (features, tokens) with element strides stride_f, stride_t (not
  * negative) and W (vocab, features) with rows of stride ldw, both of io_dtype; the logits are not
  * kept. With targets (top 0) or lists. Sums are float32; with MSS_F32 the operands, and the logits' gradient, are
  * split in two planes of 11 bits under one power of two each: 2^-23 of an element down to 2^-27 of the largest.
- * With MSS_BF16 the backward rounds the logits' gradient to bf16 once. It goes in pieces of the vocabulary of at most 1 GiB in the workspace. dx: [features][tokens]
- * of io_dtype, dweight: [vocab][features] of dw_dtype; either may be NULL. tokens and vocab at most 2^20, their
- * product 2^38, features at most 65536 (MSS_ERR_UNSUPPORTED beyond). workspace:
+ * With MSS_BF16 the backward rounds the logits' gradient to bf16 once. It goes in pieces of the vocabulary of at
+ * most 1 GiB in the workspace. dx: [features][tokens] of io_dtype, dweight: [vocab][features] of dw_dtype; either
+ * may be NULL. tokens and vocab at most 2^20, their product 2^38, features at most 65536, ldw 2^24, stride_f and
+ * stride_t 2^40 (MSS_ERR_UNSUPPORTED beyond). workspace:
  * mss_linear_loss_workspace_bytes for the forward call (which 0), the backward call (1) and
  * mss_linear_loss_fwd_grad (2), 256-byte aligned, nothing kept in it.
  * mss_linear_loss_fwd_grad is both directions at once, dx and dweight for an upstream gradient of 1: the logits are
  * formed once, and kept in 16 bits, to 2^-10 of a probability (zero below 2^-38), until its gradient takes their
- * place. Where it is not offered (MSS_F32, MSS_LOSS_NONE, small heads) its workspace takes 0 bytes and the call returns MSS_ERR_UNSUPPORTED.
+ * place. Where it is not offered (MSS_F32, MSS_LOSS_NONE, small heads) its workspace takes 0 bytes and the call
+ * returns MSS_ERR_UNSUPPORTED.
  * mss_linear_loss_rescale then multiplies dx and dweight by *grad, rounding them once more, unless that is 1.
  *
  * mss_distill: logits [rows][vocab] of io_dtype, rows of stride ld (at least vocab), lists only.

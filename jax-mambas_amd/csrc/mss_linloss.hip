@@ -16,8 +16,8 @@
 // 2^-27 of the largest, and to 2^-50 of the largest below. A product is the sum of three products of planes
 // (v_mfma_f32_32x32x16_f16), the two with a lower plane first: what is dropped, the lower ones' own, is at most 2^-22
 // of a term, 2^-24.6 in the mean square. g, taken times 2^15, is held to 2^-23 of itself down to 2^-28, and to 2^-51
-// below (2^-27 and 2^-50 of the largest upstream gradient where each row has its own). Three times the work of a bf16 product, at 16
-// times the rate of the float32 matrix instructions.
+// below (2^-27 and 2^-50 of the largest upstream gradient where each row has its own). Three times the work of a bf16
+// product, at 16 times the rate of the float32 matrix instructions.
 //
 // 32x32x16 operand layout (lane l, its 8 bf16): A[i][k] at l = i + 32 (k / 8), element k % 8;
 // B[k][j] at l = j + 32 (k / 8), element k % 8; D[i][j] at l = j + 32 ((i / 4) % 2),
@@ -52,6 +52,8 @@ struct LlShape {
   static constexpr int kASlots = kM * kBK / 8, kBSlots = kN * kBK / 8, kSlots = kASlots + kBSlots;  // of 16 bytes
   static constexpr int kACopies = kASlots / kThreads, kBCopies = kBSlots / kThreads;
   static constexpr int kCopies = kACopies + kBCopies;
+  // (By the ring alone: with the rows' scales beside it one workgroup of LlThinM fits, which only means that its second
+  // half of the tiles is begun when the first is done.)
   static constexpr int kPerCU = kRing * kSlots * 16 > 81920 ? 1 : 2;
   static constexpr int kSums = 16 * kMT * kNT;  // of a lane
   static_assert(kASlots % kThreads == 0 && kBSlots % kThreads == 0, "whole copies");
