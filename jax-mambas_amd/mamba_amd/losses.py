@@ -94,9 +94,10 @@ def _guard(t):
 
 def _require_one_gpu(*tensors):
     _require_gpu(*tensors)
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) > 1:
-        raise ValueError(f"the operands lie on several devices: {', '.join(sorted(map(str, devices)))}")
+    device = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"the operands lie on several devices: {device}, {t.device}")
 
 
 def _bytes(n, device):
@@ -176,12 +177,12 @@ class _LinearLoss(torch.autograd.Function):
             a.x = a.loss = a.mean = a.targets = a.ids = a.teacher = None
             # (Saved-tensor hooks may have put both elsewhere, and the weight's rows at another distance.)
             a.saved, a.saved_bytes = saved.data_ptr(), saved.numel()
-            w = _rows(w)
-            a.weight, a.ldw = w.data_ptr(), _row_stride(w)
-            if (a.weight, a.ldw) != (src.weight, src.ldw) and saved.numel() < lib.mss_linear_loss_saved_bytes(a):
-                # (It was read in place, and cannot be here.)
-                w = w.clone(memory_format=torch.contiguous_format)
+            if w.data_ptr() != src.weight or w.stride() != (src.ldw, 1):
+                w = _rows(w)
                 a.weight, a.ldw = w.data_ptr(), _row_stride(w)
+                if saved.numel() < lib.mss_linear_loss_saved_bytes(a):  # it was read in place, and cannot be here
+                    w = w.clone(memory_format=torch.contiguous_format)
+                    a.weight, a.ldw = w.data_ptr(), _row_stride(w)
             a.dw_dtype = _io_tag(ctx.dw_dtype, "weight")
             d, ctx.d = ctx.d, None  # the caller may write over them
             if d is not None:
@@ -290,8 +291,9 @@ class _Distill(torch.autograd.Function):
             a = _lib.DistillArgs.from_buffer_copy(src)
             a.ids = a.teacher = a.loss = a.mean = None
             # (Saved-tensor hooks may have put both elsewhere, and the rows at another distance.)
-            logits = _rows(logits)
-            a.logits, a.ld = logits.data_ptr(), _row_stride(logits)
+            if logits.data_ptr() != src.logits or logits.stride() != (src.ld, 1):
+                logits = _rows(logits)
+                a.logits, a.ld = logits.data_ptr(), _row_stride(logits)
             a.saved, a.saved_bytes = saved.data_ptr(), saved.numel()
             a.grad, a.dlogits = grad.data_ptr(), d.data_ptr()
             _lib.check(getattr(lib, name)(a, _stream(logits)), name)

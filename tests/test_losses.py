@@ -384,6 +384,24 @@ def test_distill_backward_reads_what_the_hooks_return(calls, layout, reduction, 
         assert a.logits == logits.data_ptr() and a.ld == logits.stride(0)
 
 
+def test_backward_reads_another_layout_at_the_same_address(calls):
+    """Memory that was freed and given out again: the address is the forward call's, the rows lie closer."""
+    def closer(t):
+        return t.as_strided(t.shape, (t.shape[1], 1)) if t.dim() == 2 else t.clone()
+    x, targets = torch.randn(64, 20, requires_grad=True), torch.zeros(20, dtype=torch.int64)
+    wide = torch.zeros(100, 72)[:, :64].requires_grad_(True)
+    with _Hooks(closer):
+        loss = linear_cross_entropy(x, wide, targets)
+    torch.autograd.grad(loss, (x,))
+    fwd, bwd = (a for _, a in calls.seen)
+    assert bwd.weight == fwd.weight and (fwd.ldw, bwd.ldw) == (72, 64)
+    with _Hooks(closer):
+        loss = distill_loss(wide, torch.zeros(100, 3, dtype=torch.int64), torch.zeros(100, 3))
+    torch.autograd.grad(loss, (wide,))
+    fwd, bwd = (a for _, a in calls.seen[2:])
+    assert bwd.logits == fwd.logits and (fwd.ld, bwd.ld) == (72, 64)
+
+
 def test_operands_on_several_devices_are_refused(calls):
     x, w, tg = torch.randn(8, 5), torch.randn(11, 8), torch.zeros(5, dtype=torch.int64)
     ids, te, z = torch.zeros(5, 3, dtype=torch.int64), torch.randn(5, 3), torch.randn(5, 11)
